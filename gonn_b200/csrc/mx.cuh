@@ -1,0 +1,174 @@
+// Microscaled formats (OCP Microscaling 1.0): blocks of 32 values that share a power of two.
+//
+// A block's scale is 2^e with e = clamp(floor(log2(largest magnitude)) - E, -127, 127), held as e + 127 in a byte (E8M0); its
+// values are v / 2^e rounded to nearest even, saturating: MXFP8 has E4M3 codes (E = 8, largest 448), MXFP4 E2M1 codes
+// (E = 2, largest 6), two to a byte, the first in the lower half.  A block of zeros has e = -127.  A block that holds an
+// infinity or a NaN has scale code 255, which makes every value of it NaN, here and in the tensor core.
+//
+// Codes: row-major, each row padded with zeros to whole blocks (32 or 16 bytes).  Scales: as the tensor core's copies into TMEM
+// take them, in pieces of 512 bytes for 128 rows and four blocks (of 128 columns of the matrix), the pieces of a row
+// of pieces behind one another; row r of a piece lies at byte 16 (r % 32) + 4 (r / 32).  A row of pieces covers whole 128-byte
+// steps of the codes, so MXFP4 has an even number of pieces; the scales behind the last block are zeros.
+#pragma once
+#include "common.cuh"
+
+namespace gbmx {
+
+enum Format : int { FP8 = 0, FP4 = 1 };
+
+__host__ __device__ constexpr int pieces(int K, int fmt) { return fmt == FP8 ? (K + 127) / 128 : 2 * ((K + 255) / 256); }
+__host__ __device__ constexpr int row_bytes(int K, int fmt) { return (K + 31) / 32 * (fmt == FP8 ? 32 : 16); }
+
+// Where the four scales of columns 128 g .. 128 g + 127 of a row lie; P: pieces of a row of pieces.
+__device__ __forceinline__ long long scale_word(long long row, int g, int P) {
+  return ((row >> 7) * P + g) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4;
+}
+
+// Products with powers of two must keep subnormal operands and results, which -ftz=true (part of --use_fast_math) would not.
+__device__ __forceinline__ float mul_exact(float a, float b) {
+  float d;
+  asm("mul.rn.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// The scale code of a block whose largest magnitude has these bits (as fp32), and 1 / scale.  (Magnitudes compare as whole numbers:
+// an infinity or a NaN is above all others, subnormal numbers are not lost.)
+__device__ __forceinline__ uint32_t scale_code(uint32_t amax, int fmt) {
+  const int c = (int)(amax >> 23) - (fmt == FP8 ? 8 : 2);
+  return amax >= 0x7f800000u ? 255u : (uint32_t)max(c, 0);
+}
+__device__ __forceinline__ float scale_inverse(uint32_t code) { return code == 255u ? 0.f : __uint_as_float((254u - code) << 23); }
+__device__ __forceinline__ float scale_value(uint32_t code) {
+  return __uint_as_float(code == 255u ? 0x7fffffffu : code == 0u ? 0x00400000u : code << 23);      // (2^-127 is subnormal)
+}
+
+// Eight scaled values as codes: E4M3 in 8 bytes, E2M1 in 4.
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  uint32_t r;
+  asm("{\n.reg .b16 lo, hi;\ncvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\ncvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\nmov.b32 %0, {lo, hi};\n}"
+      : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d));
+  return r;
+}
+__device__ __forceinline__ uint32_t e2m1x8(const float* v) {
+  uint32_t r;
+  asm("{\n.reg .b8 b0, b1, b2, b3;\n"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\ncvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\ncvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n"
+      "mov.b32 %0, {b0, b1, b2, b3};\n}"
+      : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+
+// n / d for n below 2^31 by a multiplication (Granlund and Montgomery's division by invariant integers).
+struct FastDiv {
+  uint32_t d, m, s;
+  __host__ explicit FastDiv(uint32_t div) : d(div), m(0), s(0) {
+    while ((1ull << s) < d) s++;
+    m = (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, m) + n) >> s; }
+};
+
+template <typename T> struct Elem;
+template <> struct Elem<__nv_bfloat16> {     // (not by way of fp32 arithmetic, which would lose subnormal numbers)
+  static constexpr int SZ = 2;
+  static __device__ __forceinline__ void unpack(const uint32_t* w, float* f) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) { const float2 p = pair(w[i]); f[2 * i] = p.x; f[2 * i + 1] = p.y; }
+  }
+  static __device__ __forceinline__ float2 pair(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return gb::pack_bf16(a, b); }
+};
+template <> struct Elem<__half> {
+  static constexpr int SZ = 2;
+  static __device__ __forceinline__ void unpack(const uint32_t* w, float* f) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) { const float2 p = pair(w[i]); f[2 * i] = p.x; f[2 * i + 1] = p.y; }
+  }
+  static __device__ __forceinline__ float2 pair(uint32_t w) { return gb::unpack_f16(w); }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return gb::pack_f16(a, b); }
+};
+template <> struct Elem<float> {
+  static constexpr int SZ = 4;
+  static __device__ __forceinline__ void unpack(const uint32_t* w, float* f) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) f[i] = __uint_as_float(w[i]);
+  }
+};
+
+// Extent of a matrix in memory: vectors are read as long as they lie within it.
+struct Extent {
+  uintptr_t begin, end;
+};
+
+// Elements k .. k + 7 of a row of K (zeros behind its end) as raw words: W = 4 for 16-bit types, 8 for fp32.
+// A row that does not start on a 16-byte boundary is read as the vectors around it, shifted.
+template <typename T>
+__device__ __forceinline__ void load8(const T* row, int k, int K, const Extent& ext, uint32_t (&w)[2 * Elem<T>::SZ]) {
+  constexpr int W = 2 * Elem<T>::SZ;                     // words of eight elements
+  const uintptr_t at = reinterpret_cast<uintptr_t>(row + k);
+  const uint32_t o = at & 15;
+  if (k + 8 <= K && o == 0) {
+    const uint4* p = reinterpret_cast<const uint4*>(at);
+#pragma unroll
+    for (int i = 0; i < W / 4; i++) { const uint4 u = __ldg(p + i); w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w; }
+    return;
+  }
+  const uintptr_t first = at & ~(uintptr_t)15;
+  if (k + 8 <= K && first >= ext.begin && first + 4 * W + 16 <= ext.end) {
+    uint32_t v[W + 5];
+    const uint4* p = reinterpret_cast<const uint4*>(first);
+#pragma unroll
+    for (int i = 0; i < W / 4 + 1; i++) { const uint4 u = __ldg(p + i); v[4 * i] = u.x; v[4 * i + 1] = u.y; v[4 * i + 2] = u.z; v[4 * i + 3] = u.w; }
+    v[W + 4] = 0;
+    if (o & 8) {
+#pragma unroll
+      for (int i = 0; i < W + 2; i++) v[i] = v[i + 2];
+    }
+    if (o & 4) {
+#pragma unroll
+      for (int i = 0; i < W + 1; i++) v[i] = v[i + 1];
+    }
+#pragma unroll
+    for (int i = 0; i < W; i++) w[i] = Elem<T>::SZ == 4 ? v[i] : __funnelshift_r(v[i], v[i + 1], (o & 2) * 8);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < W; i++) w[i] = 0;
+  if (Elem<T>::SZ == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (k + i < K) w[i % W] = __ldg(reinterpret_cast<const uint32_t*>(row) + k + i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (k + i < K) w[i / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(row) + k + i) << (16 * (i & 1));
+  }
+}
+
+// Eight values of a lane, of which four lanes in a row hold a block and sixteen (all of them here) 128 columns: codes of the
+// lane in `out` (the first word alone for FP4), the scales of the four blocks as a word in every lane.
+__device__ __forceinline__ uint32_t quantize8(const float* v, int fmt, unsigned mask, int lane, uint32_t (&out)[2]) {
+  uint32_t amax = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) amax = max(amax, __float_as_uint(v[i]) & 0x7fffffffu);
+  amax = max(amax, __shfl_xor_sync(mask, amax, 1));
+  amax = max(amax, __shfl_xor_sync(mask, amax, 2));
+  const uint32_t code = scale_code(amax, fmt);
+  const float inv = scale_inverse(code);
+  float q[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) q[i] = mul_exact(v[i], inv);
+  if (fmt == FP8) {
+    out[0] = e4m3x4(q[0], q[1], q[2], q[3]);
+    out[1] = e4m3x4(q[4], q[5], q[6], q[7]);
+  } else {
+    out[0] = e2m1x8(q);
+  }
+  uint32_t word = code << (8 * ((lane >> 2) & 3));
+  word |= __shfl_xor_sync(mask, word, 4);
+  word |= __shfl_xor_sync(mask, word, 8);
+  return word;
+}
+
+}  // namespace gbmx

@@ -16,6 +16,8 @@ import torch
 from .. import lib as _l
 from ..nn.linear import Linear
 from ..nn.module import Module
+from .microscale import (MXBlock, MXLinear, MXRMSNorm, MXTrainLinear, QTensorMX, QuantizeMX, QuantizeMXPair, DequantizeMX,  # noqa: F401
+                         AddRMSNormMX, MatMulMX, LinearMX, TrainLinearMX, NewMXLinearFrom, NewMXTrainLinearFrom)
 
 QMin, QMax = -128, 127
 DefaultAveragingConstant = 0.01

@@ -1,0 +1,231 @@
+"""Microscaled formats on CPU tensors: the oracle against a plain restatement of the definition, layouts, refusals, layers."""
+import math
+
+import pytest
+import torch
+
+from gonn_b200 import quant as Q
+from gonn_b200.nn import Linear, RMSNorm
+
+FORMATS = ["mxfp8", "mxfp4"]
+
+
+def numbers(format):
+    """The magnitudes of a format, from its bits: exponent and fraction fields, no infinities."""
+    if format == "mxfp8":
+        return [(f / 8) * 2.0 ** -6 for f in range(8)] + [(1 + f / 8) * 2.0 ** (e - 7) for e in range(1, 16) for f in range(8)][:-1]
+    return [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0]
+
+
+def restated(row, format):
+    """(values, scale codes) of a row: block by block, value by value."""
+    top, grid = (8, numbers(format)) if format == "mxfp8" else (2, numbers(format))
+    values, codes = [], []
+    for b in range(0, len(row), 32):
+        block = row[b:b + 32]
+        if not all(math.isfinite(v) for v in block):
+            values += [math.nan] * len(block)
+            codes.append(255)
+            continue
+        big = max(abs(v) for v in block)
+        e = -127 if big == 0 else min(127, max(-127, math.frexp(big)[1] - 1 - top))
+        codes.append(e + 127)
+        for v in block:
+            m = abs(v) / 2.0 ** e
+            near = min(range(len(grid)), key=lambda i: (abs(grid[i] - m), i % 2))
+            values.append(math.copysign(grid[near] * 2.0 ** e, v))
+    return values, codes
+
+
+def same(a, b):
+    return bool(((a == b) | (torch.isnan(a) & torch.isnan(b))).all())
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("shape", [(1, 1), (3, 31), (2, 32), (5, 33), (130, 97), (2, 3, 300)])
+def test_quantize_is_the_definition(format, shape):
+    t = torch.randn(*shape, dtype=torch.float64) * torch.exp2(torch.randint(-30, 30, (*shape[:-1], 1)).double())
+    t.view(-1)[::7] = 0
+    q = Q.QuantizeMX(t, format)
+    v = Q.DequantizeMX(q, torch.float64)
+    assert v.shape == t.shape and q.Numel() == t.numel()
+    rows = t.reshape(-1, shape[-1])
+    for r in range(rows.shape[0]):
+        values, codes = restated(rows[r].tolist(), format)
+        assert v.reshape(rows.shape)[r].tolist() == values
+        assert q.ScaleCodes()[r].tolist() == codes
+
+
+@pytest.mark.parametrize("format", FORMATS)
+def test_ties_saturation_extremes(format):
+    grid = numbers(format)
+    mids = [(a + b) / 2 for a, b in zip(grid, grid[1:])]
+    # the largest number of the block fixes the scale at 1
+    rows = [grid[-1:] + mids[i:i + 31] for i in range(0, len(mids), 31)]
+    rows += [[2.0 ** (9 if format == "mxfp8" else 3) * 0.99, 1.0, -grid[-1], 0.0], [0.0] * 4, [1e-40, -3e-45], [3e38, -1e-30], [math.inf, 1.0], [math.nan, -2.0] + [1.0] * 40]
+    for row in rows:
+        t = torch.tensor([row], dtype=torch.float64)
+        values, codes = restated(row, format)
+        q = Q.QuantizeMX(t, format)
+        assert same(Q.DequantizeMX(q, torch.float64)[0], torch.tensor(values, dtype=torch.float64)), row
+        assert q.ScaleCodes()[0].tolist() == codes
+
+
+@pytest.mark.parametrize("format", FORMATS)
+def test_layout(format):
+    """Where the documented bytes lie."""
+    R, K = 150, 300
+    q = Q.QuantizeMX(torch.randn(R, K), format)
+    per = 1 if format == "mxfp8" else 2
+    assert q.Data.shape == (R, 320 // per) and q.Scales.numel() == 2 * (3 if format == "mxfp8" else 4) * 512
+    codes, P = q.ScaleCodes(), 3 if format == "mxfp8" else 4
+    for r in (0, 31, 32, 127, 128, 149):
+        for b in range(10):
+            assert int(q.Scales[((r // 128) * P + b // 4) * 512 + 16 * (r % 32) + 4 * (r % 128 // 32) + b % 4]) == int(codes[r, b])
+    assert int(q.Data[3, 300 // per:].sum()) == 0                # the padding of a row
+    if format == "mxfp4":
+        one = Q.QuantizeMX(torch.tensor([[1.0, -4.0]]), format)   # scale 1: codes 2 and 8 + 6
+        assert int(one.Data[0, 0]) == 2 | 14 << 4
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("act", [None, "relu", "gelu", "geluexact"])
+def test_matmul(format, act):
+    a, b = torch.randn(2, 3, 70), torch.randn(9, 70)
+    qa, qb, bias = Q.QuantizeMX(a, format), Q.QuantizeMX(b, format), torch.randn(9)
+    want = Q.DequantizeMX(qa, torch.float64) @ Q.DequantizeMX(qb, torch.float64).T + bias.double()
+    if act:
+        want = {"relu": torch.relu, "gelu": lambda v: torch.nn.functional.gelu(v, approximate="tanh"), "geluexact": torch.nn.functional.gelu}[act](want)
+    assert torch.equal(Q.MatMulMX(qa, qb, bias, torch.float64, act), want)
+    assert torch.equal(Q.LinearMX(a, qb, bias, act), want.float())
+    assert Q.LinearMX(qa, qb, bias, act).dtype == torch.bfloat16
+
+
+def test_norm_hands_on_the_sum():
+    x, r, w = torch.randn(4, 5, 40), torch.randn(4, 5, 40), torch.rand(40) + 0.5
+    q, h = Q.AddRMSNormMX(x, r, w, 1e-6, "mxfp8")
+    assert torch.equal(h, x + r)
+    y = h.float() * torch.rsqrt(h.square().mean(-1, keepdim=True) + 1e-6) * w
+    assert torch.equal(Q.DequantizeMX(q), Q.DequantizeMX(Q.QuantizeMX(y)))
+    q, h = Q.AddRMSNormMX(x, None, w)
+    assert h is x
+    zero, _ = Q.AddRMSNormMX(torch.zeros(2, 40), None, w)
+    assert int(Q.DequantizeMX(zero).abs().sum()) == 0
+
+
+def test_train_linear_gradients():
+    x, w, b = (torch.randn(*s, dtype=torch.float64, requires_grad=True) for s in ((2, 11, 37), (13, 37), (13,)))
+    dy = torch.randn(2, 11, 13, dtype=torch.float64)
+    y = Q.TrainLinearMX(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+
+    def rounded(t):
+        return Q.DequantizeMX(Q.QuantizeMX(t), torch.float64)
+
+    x2, g = x.detach().reshape(22, 37), dy.reshape(22, 13)
+    assert torch.equal(y.detach().reshape(22, 13), rounded(x2) @ rounded(w).T + b.detach())
+    assert torch.equal(dx.reshape(22, 37), rounded(g) @ rounded(w.detach().T).T)
+    assert torch.equal(dw, rounded(g.T) @ rounded(x2.T).T)
+    assert torch.allclose(db, g.sum(0), rtol=1e-12)
+    # differences: on values that the format holds exactly, the layer is linear and its gradients are the layer's
+    x = torch.randint(-4, 5, (32, 32)).double().requires_grad_()
+    w = torch.randint(-4, 5, (32, 32)).double().requires_grad_()
+    dy = torch.randint(-4, 5, (32, 32)).double()
+    dx, dw = torch.autograd.grad(Q.TrainLinearMX(x, w), (x, w), dy)
+    for t, d in ((x, dx), (w, dw)):
+        i, j, base = 3, 5, t.detach()[3, 5].item()
+        loss = []
+        for v in ((base + 1, base - 1) if abs(base) < 4 else (base, base - 2 * math.copysign(1, base))):
+            with torch.no_grad():
+                t[i, j] = v
+                loss.append((v, (Q.TrainLinearMX(x, w) * dy).sum().item()))
+        with torch.no_grad():
+            t[i, j] = base
+        assert (loss[0][1] - loss[1][1]) / (loss[0][0] - loss[1][0]) == pytest.approx(d[i, j].item(), rel=1e-12)
+
+
+def test_train_linear_asks_for_what_is_needed():
+    x, w = torch.randn(3, 8), torch.randn(5, 8, requires_grad=True)
+    (dw,) = torch.autograd.grad(Q.TrainLinearMX(x, w).sum(), w)
+    assert dw.shape == w.shape
+    x.requires_grad_()
+    (dx,) = torch.autograd.grad(Q.TrainLinearMX(x, w.detach()).sum(), x)
+    assert dx.shape == x.shape
+    empty = torch.randn(0, 8, requires_grad=True)
+    b = torch.randn(5, requires_grad=True)
+    grads = torch.autograd.grad(Q.TrainLinearMX(empty, w, b).sum(), (empty, w, b))
+    assert [tuple(g.shape) for g in grads] == [(0, 8), (5, 8), (5,)] and all(not g.any() for g in grads)
+    with torch.no_grad():
+        assert not Q.TrainLinearMX(x, w).requires_grad
+
+
+def test_layers():
+    lin, norm = Linear(40, 24, activation="gelu"), RMSNorm(40)
+    x, r = torch.randn(6, 40), torch.randn(6, 40)
+    for format in FORMATS:
+        q, h = Q.MXRMSNorm(norm, format)(x, r)
+        m = Q.NewMXLinearFrom(lin, format)
+        y = m(q, torch.float32)
+        n = norm(x + r)
+        assert torch.equal(y, m(n)) and torch.equal(h, x + r)
+        assert (y - lin(n)).norm() / lin(n).norm() < (0.06 if format == "mxfp8" else 0.3)       # twice a rounding of 2^-4 and 2^-2 of each operand
+        again = Q.NewMXLinearFrom(Linear(40, 24, activation="gelu"), format)
+        again.load_state_dict(m.state_dict())
+        assert torch.equal(again(n), m(n))
+    t = Q.NewMXTrainLinearFrom(Linear(40, 24))
+    t(x).sum().backward()
+    assert t.linear.weight.grad is not None and t.linear.bias.grad is not None
+    assert torch.equal(t.Convert()(x), t(x).detach())
+
+
+def test_empty():
+    q = Q.QuantizeMX(torch.zeros(0, 40))
+    assert Q.DequantizeMX(q).shape == (0, 40) and q.ScaleCodes().shape == (0, 2)
+    w = Q.QuantizeMX(torch.randn(5, 40))
+    assert Q.MatMulMX(q, w).shape == (0, 5)
+    assert Q.LinearMX(torch.zeros(2, 0, 40), w).shape == (2, 0, 5)
+
+
+def test_refusals():
+    x, w = torch.randn(4, 64), torch.randn(8, 64)
+    qx, qw = Q.QuantizeMX(x), Q.QuantizeMX(w)
+    with pytest.raises(ValueError, match="formats"):
+        Q.QuantizeMX(x, "mxfp6")
+    with pytest.raises(ValueError, match="last dimension"):
+        Q.QuantizeMX(torch.zeros(4, 0))
+    with pytest.raises(ValueError, match="last dimension"):
+        Q.QuantizeMX(torch.tensor(1.0))
+    with pytest.raises(TypeError, match="floating"):
+        Q.QuantizeMX(torch.zeros(4, 4, dtype=torch.int32))
+    with pytest.raises(ValueError, match="one row"):
+        Q.QuantizeMXPair(torch.zeros(0, 4))
+    with pytest.raises(ValueError, match="one format"):
+        Q.MatMulMX(qx, Q.QuantizeMX(w, "mxfp4"))
+    with pytest.raises(ValueError, match="do not match"):
+        Q.MatMulMX(qx, Q.QuantizeMX(torch.randn(8, 65)))
+    with pytest.raises(ValueError, match="do not match"):
+        Q.MatMulMX(qx, Q.QuantizeMX(torch.randn(2, 8, 64)))
+    with pytest.raises(ValueError, match="activation"):
+        Q.MatMulMX(qx, qw, act="swish")
+    with pytest.raises(ValueError, match="bias"):
+        Q.MatMulMX(qx, qw, torch.zeros(7))
+    with pytest.raises(ValueError, match="do not belong"):
+        Q.DequantizeMX(Q.QTensorMX(qx.Data, qx.Scales, "mxfp8", (4, 128)))
+    with pytest.raises(ValueError, match="do not belong"):
+        Q.DequantizeMX(Q.QTensorMX(qx.Data, qx.Scales[:-1], "mxfp8", (4, 64)))
+    with pytest.raises(ValueError, match="contiguous"):
+        Q.DequantizeMX(Q.QTensorMX(qx.Data.t().contiguous().t(), qx.Scales, "mxfp8", (4, 64)))
+    with pytest.raises(TypeError, match="uint8"):
+        Q.DequantizeMX(Q.QTensorMX(qx.Data.int(), qx.Scales, "mxfp8", (4, 64)))
+    with pytest.raises(ValueError, match="residual"):
+        Q.AddRMSNormMX(x, torch.zeros(4, 63), torch.ones(64))
+    with pytest.raises(ValueError, match="residual"):
+        Q.AddRMSNormMX(x, torch.zeros(4, 64, dtype=torch.bfloat16), torch.ones(64))
+    with pytest.raises(ValueError, match="weight"):
+        Q.AddRMSNormMX(x, None, torch.ones(63))
+    with pytest.raises(TypeError, match="weight"):
+        Q.AddRMSNormMX(x, None, torch.ones(64, dtype=torch.float16))
+    with pytest.raises(ValueError, match="do not match"):
+        Q.TrainLinearMX(x, torch.zeros(8, 63))
+    with pytest.raises(ValueError, match="activation"):
+        Q.MXTrainLinear(Linear(4, 4, activation="relu"))

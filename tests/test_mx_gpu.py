@@ -1,0 +1,413 @@
+"""Microscaled kernels against the CPU oracle and against 64 bits.
+
+Quantised codes have to be equal: rounding is part of the format.  Products are first taken of values whose sums the fp32
+accumulator holds exactly (whole numbers times powers of two, every partial sum below 2^24 units), so that results have to be
+equal as well; random operands follow with tolerances that count roundings."""
+import math
+
+import pytest
+import torch
+
+from gonn_b200 import lib as _l
+from gonn_b200 import quant as Q
+from gonn_b200.nn import Linear, RMSNorm
+
+pytestmark = pytest.mark.gpu
+
+FORMATS = ["mxfp8", "mxfp4"]
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+DEV = "cuda"
+
+
+def wild(*shape, dtype):
+    """Values over many magnitudes, zeros and ties among them."""
+    t = torch.randn(*shape) * torch.exp2(torch.randint(-12, 12, shape[:-1] + (1,)).float())
+    t = torch.where(torch.rand(shape) < 0.1, torch.zeros(()), t)
+    t = torch.where(torch.rand(shape) < 0.3, torch.round(t * 8) / 8, t)
+    return t.to(dtype)
+
+
+def equal(q, want):
+    assert torch.equal(q.Data.cpu(), want.Data)
+    assert torch.equal(q.ScaleCodes().cpu(), want.ScaleCodes())
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1, 1), (1, 31), (2, 32), (3, 33), (5, 127), (129, 130), (7, 256), (130, 257), (33, 1000), (300, 2048), (1, 8192), (2, 3, 77)])
+def test_quantize_is_the_oracle(format, dtype, shape, status_ok):
+    t = wild(*shape, dtype=dtype)
+    q = Q.QuantizeMX(t.to(DEV), format)
+    want = Q.QuantizeMX(t, format)
+    equal(q, want)
+    # scales behind the last block are zeros
+    blocks, rows = -(-shape[-1] // 32), want.Data.shape[0]
+    s = q.Scales.cpu().view(-(-rows // 128), -1, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(-(-rows // 128) * 128, -1)
+    assert not s[:rows, blocks:].any()
+    for out in DTYPES:
+        assert torch.equal(Q.DequantizeMX(q, out).cpu(), Q.DequantizeMX(want, torch.float64).to(out))
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_extremes(format, dtype, status_ok):
+    top = torch.finfo(dtype).max
+    tiny = torch.finfo(dtype).smallest_normal
+    sub = tiny * torch.finfo(dtype).eps
+    rows = [[0.0], [top, -top, 1.0], [tiny, -tiny / 2, sub], [sub, -sub, 3 * sub, 0.0], [math.inf, 1.0, 2.0], [-math.inf], [math.nan, 1.0], [1.0] * 32 + [math.nan] + [2.0] * 40,
+            [-0.0, 0.0, -1e-7], [tiny * 2 ** i for i in range(12)]]
+    t = torch.zeros(len(rows), 80, dtype=dtype)
+    for i, r in enumerate(rows):
+        t[i, :len(r)] = torch.tensor(r, dtype=torch.float64).to(dtype)
+    q, want = Q.QuantizeMX(t.to(DEV), format), Q.QuantizeMX(t, format)
+    assert torch.equal(q.ScaleCodes().cpu(), want.ScaleCodes())
+    for out in DTYPES:
+        a, b = Q.DequantizeMX(q, out).cpu(), Q.DequantizeMX(want, torch.float64).to(out)
+        assert torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(a.nan_to_num(0, 1, 1), b.nan_to_num(0, 1, 1))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("offset", [1, 2, 3, 5, 8])
+@pytest.mark.parametrize("K,pitch", [(100, 100), (100, 101), (97, 131), (1003, 1003)])
+def test_quantize_views(dtype, offset, K, pitch, status_ok):
+    """Rows at any address and distance; what lies before, between and behind them is not taken."""
+    R = 9
+    flat = torch.full((offset + R * pitch + 16,), float("nan"), dtype=dtype)
+    view = flat[offset:offset + R * pitch].as_strided((R, K), (pitch, 1), offset)
+    view.copy_(wild(R, K, dtype=dtype))
+    d = flat.to(DEV)
+    dv = d.as_strided((R, K), (pitch, 1), offset)
+    for format in FORMATS:
+        equal(Q.QuantizeMX(dv, format), Q.QuantizeMX(view, format))
+    q, qt = Q.QuantizeMXPair(dv)
+    equal(q, Q.QuantizeMX(view))
+    equal(qt, Q.QuantizeMX(view.t()))
+    equal(Q.QuantizeMX(dv.t()), Q.QuantizeMX(view.t()))
+    w = torch.rand(K) + 0.5
+    a, _ = Q.AddRMSNormMX(dv, dv, w.to(DEV))
+    b, _ = Q.AddRMSNormMX(dv.contiguous(), dv.contiguous(), w.to(DEV))
+    assert torch.equal(a.Data, b.Data) and torch.equal(a.ScaleCodes(), b.ScaleCodes())
+
+
+def test_quantize_broadcast_rows(status_ok):
+    row = torch.randn(64, device=DEV)
+    equal(Q.QuantizeMX(row.expand(5, 64)), Q.QuantizeMX(row.cpu().expand(5, 64)))
+    column = torch.randn(5, 1, device=DEV)
+    equal(Q.QuantizeMX(column.expand(5, 64)), Q.QuantizeMX(column.cpu().expand(5, 64)))
+    equal(Q.QuantizeMX(column), Q.QuantizeMX(column.cpu()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1, 1), (31, 33), (32, 128), (128, 128), (129, 127), (300, 1000), (1001, 200), (4, 2048)])
+def test_quantize_pair(dtype, shape, status_ok):
+    t = wild(*shape, dtype=dtype)
+    q, qt = Q.QuantizeMXPair(t.to(DEV))
+    equal(q, Q.QuantizeMX(t))
+    equal(qt, Q.QuantizeMX(t.t()))
+
+
+def nearly(q, y, ulps):
+    """Whether codes are those of a y that was off by `ulps` roundings of fp32 at most: each value is the nearest number, up to that error
+    and half a step of its block."""
+    K = y.shape[-1]
+    fp8 = q.Format == "mxfp8"
+    s = torch.exp2(q.ScaleCodes().double() - 127).repeat_interleave(32, 1)[:, :K]
+    v = Q.DequantizeMX(q, torch.float32).double().cpu().reshape(y.shape)
+    m = (y / s).abs()
+    # the largest magnitude lies where the scale puts it, up to the error of y
+    big = torch.nn.functional.pad(m, (0, -K % 32)).view(m.shape[0], -1, 32).amax(2)
+    lo, hi = (256, 512) if fp8 else (4, 8)
+    rel = ulps * 2.0 ** -24
+    assert bool(((big >= lo * (1 - rel)) & (big <= hi * (1 + rel)) | (big == 0)).all())
+    # half a step: 2^-4 or 2^-2 of the power of two below the value; what is above the largest number saturates
+    mant, least, top = (3, -6, 448.0) if fp8 else (1, 0, 6.0)
+    e = (torch.frexp(m).exponent - 1).clamp(min=least)
+    half = torch.exp2((e - mant - 1).double())
+    allowed = torch.where(m > top, (m - top).abs() + m * rel, half + m * rel)
+    assert bool(((v / s - y / s).abs() <= allowed * (1 + 1e-9)).all())
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1, 1), (3, 40), (1, 255), (9, 256), (301, 257), (700, 768), (5, 1000), (301, 1024), (2, 2048), (400, 2050), (3, 4100), (2, 8192), (2, 10000), (3, 40000)])
+@pytest.mark.parametrize("residual", [True, False])
+def test_norm(format, dtype, shape, residual, status_ok):
+    x, r = torch.randn(shape).to(dtype), torch.randn(shape).to(dtype)
+    w = (torch.rand(shape[-1]) + 0.5).to(dtype)
+    q, h = Q.AddRMSNormMX(x.to(DEV), r.to(DEV) if residual else None, w.to(DEV), 1e-6, format)
+    total = x.double() + (r.double() if residual else 0)
+    if residual:
+        assert torch.equal(h.cpu(), (x.float() + r.float()).to(dtype))
+    y = total / torch.sqrt(total.square().mean(-1, keepdim=True) + 1e-6) * w.double()
+    # roundings of y: the sum, its product with 1 / rms and with w (half a unit each), 1 / rms (half), and the sum of squares, whose error
+    # enters by half: at most 2 ceil(K / 32) + 12 roundings of a thread's chain and the tree, K no larger than 32 values a thread
+    # but for the widest rows
+    chain = 32 if shape[-1] <= 32768 else shape[-1] / 1024 + 8
+    nearly(cpu(q), y, 4 + chain / 2 + 12)
+
+
+def cpu(q):
+    return Q.QTensorMX(q.Data.cpu(), q.Scales.cpu(), q.Format, q.Shape)
+
+
+def test_norm_special_rows(status_ok):
+    x = torch.randn(6, 96, device=DEV)
+    x[1] = 0
+    x[2, 5] = math.nan
+    x[3, 40] = math.inf
+    w = torch.ones(96, device=DEV)
+    q, _ = Q.AddRMSNormMX(x, None, w)
+    v = Q.DequantizeMX(q)
+    assert not v[1].any() and torch.isnan(v[2]).all()
+    # an infinite sum of squares: the finite values become 0, the infinite one NaN, and with it its block
+    assert torch.isnan(v[3, 32:64]).all() and not v[3, :32].any() and not v[3, 64:].any()
+    alone, _ = Q.AddRMSNormMX(x[4:5], None, w)
+    assert torch.equal(Q.DequantizeMX(alone)[0], v[4])
+    mixed, _ = Q.AddRMSNormMX(x.bfloat16(), None, w)             # fp32 weights of 16-bit rows
+    same, _ = Q.AddRMSNormMX(x.bfloat16(), None, w.bfloat16())
+    assert torch.equal(mixed.Data, same.Data)
+
+
+def whole(rows, K, format):
+    """Quantised whole numbers up to 4 (6) times 1, 2, 4 or 8 for each block: exact in the format."""
+    t = torch.randint(-4, 5, (rows, K)).float()
+    if format == "mxfp4":
+        t = torch.where((t == 4) & (torch.rand(rows, K) < 0.5), torch.tensor(6.0), t)
+    s = torch.exp2(torch.randint(0, 4, (rows, -(-K // 32))).float()).repeat_interleave(32, 1)[:, :K]
+    return t * s
+
+
+SHAPES = [(1, 1, 1), (1, 8, 32), (3, 5, 7), (2, 128, 128), (16, 130, 257), (17, 129, 300), (33, 64, 1000), (64, 384, 256), (65, 300, 1000), (128, 256, 512), (129, 257, 640),
+          (300, 520, 1000), (1, 2048, 4096), (4, 300, 4096), (40, 100, 4096), (100, 1000, 4000)]
+#: 37 tiles of 256 x 256 and more run as pairs of CTAs; 74 pairs at a time
+PAIR_SHAPES = [(1700, 1700, 96), (1601, 1543, 333), (2560, 2560, 520), (2600, 2330, 1024), (9473, 256, 64), (256, 9999, 300)]
+
+
+def product(M, N, K, format, dtype, bias, act):
+    a, b = whole(M, K, format), whole(N, K, format)
+    qa, qb = Q.QuantizeMX(a.to(DEV), format), Q.QuantizeMX(b.to(DEV), format)
+    v = torch.randint(-100, 100, (N,)).to(dtype) if bias else None
+    y = Q.MatMulMX(qa, qb, None if v is None else v.to(DEV), dtype, act)
+    _l.assert_status_ok()
+    want = a.to(DEV, torch.float64) @ b.to(DEV, torch.float64).T
+    if bias:
+        want = want + v.to(DEV, torch.float64)
+    if act == "relu":
+        want = want.relu()
+    return y, want.to(dtype)
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_matmul_exact(format, M, N, K, status_ok):
+    for dtype, bias, act in ((torch.float32, False, None), (torch.bfloat16, True, None), (torch.float16, True, "relu")):
+        y, want = product(M, N, K, format, dtype, bias, act)
+        assert torch.equal(y, want), (dtype, (y.double() - want.double()).abs().max())
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("M,N,K", PAIR_SHAPES)
+def test_matmul_exact_pairs(format, M, N, K, status_ok):
+    for dtype, bias, act in ((torch.float32, True, None), (torch.bfloat16, True, "relu"), (torch.float16, False, None)):
+        y, want = product(M, N, K, format, dtype, bias, act)
+        assert torch.equal(y, want), (dtype, (y.double() - want.double()).abs().max())
+
+
+def off(y, want):
+    return ((y.double() - want).norm() / want.norm()).item()
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("act", [None, "gelu", "geluexact"])
+@pytest.mark.parametrize("M,N,K", [(5, 700, 1000), (1000, 2500, 700), (3000, 1111, 4096)])
+def test_matmul_random(format, act, M, N, K, status_ok):
+    """fp32 results: the tensor core truncates a sum at the accumulator's last bit once an instruction (32 or 64 of K), at most
+    K / 32 times 2^-23 of the largest partial sum, for random signs of its root; 16-bit results are roundings of those."""
+    a, b = torch.randn(M, K, device=DEV), torch.randn(N, K, device=DEV) / math.sqrt(K)
+    qa, qb, bias = Q.QuantizeMX(a, format), Q.QuantizeMX(b, format), torch.randn(N, device=DEV)
+    want = Q.DequantizeMX(qa).double() @ Q.DequantizeMX(qb).double().T + bias.double()
+    if act:
+        want = torch.nn.functional.gelu(want, approximate="tanh" if act == "gelu" else "none")
+    # the hardware's tanh has an error of 2^-11, and erff of a unit
+    most = (K / 32 + 2) * 2.0 ** -23 + (2.0 ** -10.5 if act == "gelu" else 0)
+    assert off(Q.MatMulMX(qa, qb, bias, torch.float32, act), want) <= most
+    assert off(Q.MatMulMX(qa, qb, bias, torch.float16, act), want) <= most + 2.0 ** -11
+    assert off(Q.MatMulMX(qa, qb, bias, torch.bfloat16, act), want) <= most + 2.0 ** -8
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("M,N", [(3, 200), (2000, 2100)])
+def test_matmul_nan_stays_in_its_rows(format, M, N, status_ok):
+    K = 333
+    a, b = torch.randn(M, K), torch.randn(N, K)
+    a[1, 70] = math.nan
+    b[130, 5] = math.inf
+    y = Q.MatMulMX(Q.QuantizeMX(a.to(DEV), format), Q.QuantizeMX(b.to(DEV), format))
+    nan = torch.zeros(M, N, dtype=torch.bool)
+    nan[1] = nan[:, 130] = True
+    assert torch.equal(torch.isnan(y).cpu(), nan)
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("M,N", [(5, 140), (2000, 2100)])
+def test_scales_of_rows_that_are_not_there(format, M, N, status_ok):
+    """Scales behind the last row hold anything, NaN's code too."""
+    K = 200
+    a, b = Q.QuantizeMX(whole(M, K, format).to(DEV), format), Q.QuantizeMX(whole(N, K, format).to(DEV), format)
+    y = Q.MatMulMX(a, b)
+    for q in (a, b):
+        rows = q.Data.shape[0]
+        s = q.Scales.view(-(-rows // 128), -1, 32, 4, 4).permute(0, 3, 2, 1, 4)
+        at = torch.arange(s.shape[0] * 128, device=DEV).view(s.shape[0], 4, 32)[:, :, :, None, None].expand(s.shape)
+        s[at >= rows] = 255
+    assert torch.equal(Q.MatMulMX(a, b), y)
+
+
+def test_products_of_extreme_scales(status_ok):
+    """Scales at both ends: 2^-127 and above, sums that overflow."""
+    a = torch.full((3, 32), 2.0 ** -120)
+    b = torch.full((4, 32), 2.0 ** 100)
+    y = Q.MatMulMX(Q.QuantizeMX(a.to(DEV)), Q.QuantizeMX(b.to(DEV)), dtype=torch.float32)
+    assert torch.equal(y.cpu(), torch.full((3, 4), 32 * 2.0 ** -20))
+    y = Q.MatMulMX(Q.QuantizeMX(b.to(DEV)), Q.QuantizeMX(b.to(DEV)), dtype=torch.float32)
+    assert torch.isinf(y).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("shape,N", [((1, 33), 17), ((7, 64), 128), ((2, 50, 300), 200), ((1001, 1000), 520), ((2100, 768), 2304)])
+def test_train_linear(dtype, shape, N, status_ok):
+    K = shape[-1]
+    x = torch.randn(shape, device=DEV).to(dtype).requires_grad_()
+    w = (torch.randn(N, K, device=DEV) / math.sqrt(K)).to(dtype).requires_grad_()
+    b = torch.randn(N, device=DEV).to(dtype).requires_grad_()
+    dy = torch.randn(*shape[:-1], N, device=DEV).to(dtype)
+    y = Q.TrainLinearMX(x, w, b)
+    got = (y, *torch.autograd.grad(y, (x, w, b), dy))
+
+    def rounded(t):
+        return Q.DequantizeMX(Q.QuantizeMX(t)).double()
+
+    x2, g = x.detach().reshape(-1, K), dy.reshape(-1, N)
+    want = (rounded(x2) @ rounded(w).T + b.detach().double(), rounded(g) @ rounded(w.detach().T).T, rounded(g.T) @ rounded(x2.T).T, g.double().sum(0))
+    for a, e, length in zip(got, want, (K, N, x2.shape[0], x2.shape[0])):
+        assert a.dtype == dtype
+        assert off(a.detach().reshape(e.shape), e) <= (length / 32 + 4) * 2.0 ** -23 + torch.finfo(dtype).eps / 2
+
+
+def test_train_linear_broadcast_gradient(status_ok):
+    """A gradient that is one value everywhere (y.sum()), a gradient of strided rows, and an input that appears twice."""
+    x = torch.randint(-4, 5, (70, 64), device=DEV).float().requires_grad_()
+    w = torch.randint(-4, 5, (40, 64), device=DEV).float().requires_grad_()
+    dx, dw = torch.autograd.grad(Q.TrainLinearMX(x, w).sum(), (x, w))
+    assert torch.equal(dx, w.detach().sum(0).expand(70, 64)) and torch.equal(dw, x.detach().sum(0).expand(40, 64))
+    dy = torch.randint(-4, 5, (70, 80), device=DEV).float()
+    dx, dw = torch.autograd.grad(Q.TrainLinearMX(x, w), (x, w), dy[:, ::2])
+    assert torch.equal(dx, dy[:, ::2] @ w) and torch.equal(dw, dy[:, ::2].T @ x)
+    (both,) = torch.autograd.grad((Q.TrainLinearMX(x, w) + Q.TrainLinearMX(x, w)).sum(), x)
+    assert torch.equal(both, 2 * w.detach().sum(0).expand(70, 64))
+
+
+@pytest.mark.parametrize("format", FORMATS)
+def test_block_of_layers(format, status_ok):
+    """Norm, projection with activation, second projection, norm with the residual: as an evaluation runs them."""
+    E, Fd, T = 256, 512, 37
+    norm, up, down = RMSNorm(E), Linear(E, Fd, activation="gelu"), Linear(Fd, E)
+    parts = [Q.MXRMSNorm(norm, format), Q.MXLinear(up, format), Q.MXLinear(down, format)]
+    x, r = torch.randn(2, T, E), torch.randn(2, T, E)
+
+    def go(device):
+        n, u, d = (p.to(device) for p in parts)
+        q, h = n(x.to(device), r.to(device))
+        q2, h2 = n(d(u(q, torch.float32)), h)
+        return u(q2, torch.float32), h, h2
+
+    want = [t.clone() for t in go("cpu")]
+    got = go(DEV)
+    assert torch.equal(got[1].cpu(), want[1])
+    # a value that moves to the next code is off by a step of it at most; few do
+    assert off(got[2].cpu(), want[2].double()) < 1e-2 and off(got[0].cpu(), want[0].double()) < 3e-2
+
+
+def test_streams_and_graphs(status_ok):
+    w = Q.QuantizeMX(torch.randn(700, 512, device=DEV))
+    big = Q.QuantizeMX(torch.randn(2048, 512, device=DEV))
+    x = torch.randn(2000, 512, device=DEV, dtype=torch.bfloat16)
+    few = torch.randn(3, 512, device=DEV, dtype=torch.bfloat16)
+    weight = torch.ones(512, device=DEV, dtype=torch.bfloat16)
+
+    def run(x, few):
+        q, h = Q.AddRMSNormMX(x, x, weight)
+        return Q.LinearMX(q, big), h, Q.LinearMX(few, w, act="relu"), Q.DequantizeMX(Q.QuantizeMX(few, "mxfp4"))
+
+    want = run(x, few)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            got.append(run(x, few))
+    torch.cuda.synchronize()
+    for g in got:
+        assert all(torch.equal(a, b) for a, b in zip(g, want))
+    graph = torch.cuda.CUDAGraph()
+    sx, sf = x.clone(), few.clone()
+    with torch.cuda.graph(graph):
+        out = run(sx, sf)
+    for seed in (1, 2):
+        torch.manual_seed(seed)
+        sx.copy_(torch.randn_like(sx))
+        sf.copy_(torch.randn_like(sf))
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(out, run(sx, sf)))
+
+
+def test_training_step_in_a_graph(status_ok):
+    torch.manual_seed(0)
+    x, dy = torch.randn(300, 256, device=DEV, dtype=torch.bfloat16), torch.randn(300, 128, device=DEV, dtype=torch.bfloat16)
+    w = torch.randn(128, 256, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    b = torch.randn(128, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+
+    def step():
+        y = Q.TrainLinearMX(x, w, b)
+        return (y.detach(), *torch.autograd.grad(y, (w, b), dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    x.copy_(torch.randn_like(x))
+    graph.replay()
+    assert all(torch.equal(a, c) for a, c in zip(out, step()))
+
+
+def test_the_same_twice(status_ok):
+    x = torch.randn(1500, 700, device=DEV, dtype=torch.bfloat16)
+    w = Q.QuantizeMX(torch.randn(2100, 700, device=DEV), "mxfp4")
+    assert torch.equal(Q.LinearMX(x, w), Q.LinearMX(x, w))
+    assert torch.equal(Q.LinearMX(x[:9], w), Q.LinearMX(x[:9], w))
+    # a row's result does not depend on the rows beside it, within one kernel
+    assert torch.equal(Q.LinearMX(x[:9], w)[4], Q.LinearMX(x[4:9], w)[0])
+
+
+def test_refusals_on_the_device(status_ok):
+    x = torch.randn(4, 64, device=DEV)
+    q = Q.QuantizeMX(x)
+    with pytest.raises(TypeError, match="no CUDA kernel"):
+        Q.QuantizeMX(x.double())
+    with pytest.raises(TypeError, match="no CUDA kernel"):
+        Q.DequantizeMX(q, torch.float64)
+    with pytest.raises(TypeError, match="no CUDA kernel"):
+        Q.MatMulMX(q, q, dtype=torch.float64)
+    with pytest.raises(ValueError, match="operands on"):
+        Q.MatMulMX(q, Q.QuantizeMX(x.cpu()))
+    with pytest.raises(ValueError, match="bias"):
+        Q.MatMulMX(q, q, torch.zeros(4))
+    with pytest.raises(ValueError, match="weight"):
+        Q.AddRMSNormMX(x, None, torch.ones(64))
+    off_by_one = torch.empty(q.Scales.numel() + 1, dtype=torch.uint8, device=DEV)[1:]
+    with pytest.raises(ValueError, match="aligned"):
+        Q.DequantizeMX(Q.QTensorMX(q.Data, off_by_one, "mxfp8", (4, 64)))
