@@ -78,6 +78,7 @@ template <> struct Elem<__nv_bfloat16> {     // (not by way of fp32 arithmetic, 
   }
   static __device__ __forceinline__ float2 pair(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return gb::pack_bf16(a, b); }
+  static __device__ __forceinline__ uint32_t bits(uint32_t h) { return h << 16; }
 };
 template <> struct Elem<__half> {
   static constexpr int SZ = 2;
@@ -87,6 +88,7 @@ template <> struct Elem<__half> {
   }
   static __device__ __forceinline__ float2 pair(uint32_t w) { return gb::unpack_f16(w); }
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return gb::pack_f16(a, b); }
+  static __device__ __forceinline__ uint32_t bits(uint32_t h) { return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h))); }
 };
 template <> struct Elem<float> {
   static constexpr int SZ = 4;
@@ -146,29 +148,132 @@ __device__ __forceinline__ void load8(const T* row, int k, int K, const Extent& 
   }
 }
 
-// Eight values of a lane, of which four lanes in a row hold a block and sixteen (all of them here) 128 columns: codes of the
-// lane in `out` (the first word alone for FP4), the scales of the four blocks as a word in every lane.
-__device__ __forceinline__ uint32_t quantize8(const float* v, int fmt, unsigned mask, int lane, uint32_t (&out)[2]) {
-  uint32_t amax = 0;
+// Sixteen elements from k on as raw words.  Rows on 16-byte boundaries with K a multiple of eight (ALIGNED) are read in vectors, of
+// 32 bytes where every row starts on such a boundary and K is a multiple of sixteen (wide).
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void load16(const T* row, int k, int K, bool wide, const Extent& ext, uint32_t (&w)[4 * Elem<T>::SZ]) {
+  constexpr int W = 4 * Elem<T>::SZ;
+  if constexpr (!ALIGNED) {
 #pragma unroll
-  for (int i = 0; i < 8; i++) amax = max(amax, __float_as_uint(v[i]) & 0x7fffffffu);
+    for (int h = 0; h < 2; h++) {
+      uint32_t u[W / 2];
+      load8(row, k + 8 * h, K, ext, u);
+#pragma unroll
+      for (int i = 0; i < W / 2; i++) w[h * (W / 2) + i] = u[i];
+    }
+  } else if (wide) {
+#pragma unroll
+    for (int i = 0; i < W; i++) w[i] = 0;
+    if (k < K) {
+#pragma unroll
+      for (int i = 0; i < W; i += 8)
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]), "=r"(w[i + 5]), "=r"(w[i + 6]), "=r"(w[i + 7])
+                     : "l"(reinterpret_cast<const uint32_t*>(row + k) + i));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; i += 4) {
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (k + (i < W / 2 ? 0 : 8) < K) u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(row + k) + i);
+      w[i] = u.x; w[i + 1] = u.y; w[i + 2] = u.z; w[i + 3] = u.w;
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void unpack16(const uint32_t (&w)[4 * Elem<T>::SZ], float (&v)[16]) {
+  Elem<T>::unpack(w, v);
+  Elem<T>::unpack(w + 2 * Elem<T>::SZ, v + 8);
+}
+
+// Sixteen values to consecutive elements on a 16-byte boundary, of which those from K on are left out (whole vectors of eight).
+template <typename T>
+__device__ __forceinline__ void store16(T* row, int k, int K, const float* v) {
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    if (k + 8 * h >= K) break;
+    uint4* to = reinterpret_cast<uint4*>(row + k + 8 * h);
+    const float* f = v + 8 * h;
+    if constexpr (sizeof(T) == 4) {
+      to[0] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+      to[1] = make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7]));
+    } else {
+      to[0] = make_uint4(Elem<T>::pack(f[0], f[1]), Elem<T>::pack(f[2], f[3]), Elem<T>::pack(f[4], f[5]), Elem<T>::pack(f[6], f[7]));
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ T to_type(float v);
+template <> __device__ __forceinline__ float to_type<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half to_type<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 to_type<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// The same for rows at any address: L lanes side by side hold 16 L consecutive values, from column `first` on, and write them one column
+// a lane, so that a store covers whole sectors.  buf: 16 L floats of shared memory.
+template <typename T, int L>
+__device__ __forceinline__ void store16_any(T* row, int first, int K, const float (&v)[16], float* buf, int lane, unsigned mask) {
+  __syncwarp(mask);
+#pragma unroll
+  for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(buf + lane * 16 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+  __syncwarp(mask);
+#pragma unroll
+  for (int i = 0; i < 16; i++)
+    if (first + i * L + lane < K) row[first + i * L + lane] = to_type<T>(buf[i * L + lane]);
+}
+
+// Bits of the largest magnitude of sixteen elements.  16-bit magnitudes compare in pairs, as whole numbers.
+template <typename T>
+__device__ __forceinline__ uint32_t largest16(const uint32_t (&w)[4 * Elem<T>::SZ]) {
+  if constexpr (Elem<T>::SZ == 2) {
+    uint32_t m = w[0] & 0x7fff7fffu;
+#pragma unroll
+    for (int i = 1; i < 8; i++) asm("max.u16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i] & 0x7fff7fffu));
+    return Elem<T>::bits(max(m >> 16, m & 0xffffu));
+  } else {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 16; i++) m = max(m, w[i] & 0x7fffffffu);
+    return m;
+  }
+}
+// The same of sixteen numbers (NaN if there is one; keeps subnormal numbers).
+__device__ __forceinline__ uint32_t largest16(const float (&v)[16]) {
+  float m = fabsf(v[0]);
+#pragma unroll
+  for (int i = 1; i < 15; i += 2) asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(fabsf(v[i])), "f"(fabsf(v[i + 1])));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v[15])));
+  return __float_as_uint(m);
+}
+
+// Sixteen values of a lane, two lanes to a block, eight (all of them here) to 128 columns; amax: bits of the largest magnitude of the
+// lane's.  Codes of the lane in `out` (two words for FP4), the scales of the four blocks as a word in every lane.
+template <int FMT>
+__device__ __forceinline__ uint32_t quantize16(const float (&v)[16], uint32_t amax, unsigned mask, int lane, uint32_t (&out)[4]) {
   amax = max(amax, __shfl_xor_sync(mask, amax, 1));
-  amax = max(amax, __shfl_xor_sync(mask, amax, 2));
-  const uint32_t code = scale_code(amax, fmt);
+  const uint32_t code = scale_code(amax, FMT);
   const float inv = scale_inverse(code);
-  float q[8];
+  float q[16];
 #pragma unroll
-  for (int i = 0; i < 8; i++) q[i] = mul_exact(v[i], inv);
-  if (fmt == FP8) {
-    out[0] = e4m3x4(q[0], q[1], q[2], q[3]);
-    out[1] = e4m3x4(q[4], q[5], q[6], q[7]);
+  for (int i = 0; i < 16; i++) q[i] = mul_exact(v[i], inv);
+  if (FMT == FP8) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) out[i] = e4m3x4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]);
   } else {
     out[0] = e2m1x8(q);
+    out[1] = e2m1x8(q + 8);
   }
-  uint32_t word = code << (8 * ((lane >> 2) & 3));
+  uint32_t word = code << (8 * ((lane >> 1) & 3));
+  word |= __shfl_xor_sync(mask, word, 2);
   word |= __shfl_xor_sync(mask, word, 4);
-  word |= __shfl_xor_sync(mask, word, 8);
   return word;
+}
+// Codes of columns k .. k + 15 of a row.
+template <int FMT>
+__device__ __forceinline__ void store_codes(uint8_t* row, int k, int row_bytes, const uint32_t (&c)[4]) {
+  const int b = FMT == FP8 ? k : k / 2;
+  if (b >= row_bytes) return;
+  if (FMT == FP8) *reinterpret_cast<uint4*>(row + b) = make_uint4(c[0], c[1], c[2], c[3]);
+  else *reinterpret_cast<uint2*>(row + b) = make_uint2(c[0], c[1]);
 }
 
 }  // namespace gbmx

@@ -3,8 +3,8 @@
 // tcgen05.mma with block scales: kind::mxf8f6f4 for MXFP8 (32 of K an instruction), kind::mxf4 for MXFP4 (64), fp32 accumulators in
 // TMEM.  A step of the main loop is 128 bytes of every row in either format (128 or 256 of K, four instructions); its
 // codes arrive by TMA with a 128-byte swizzle, its scales as the 512-byte pieces in which they are kept, and the issuing thread copies
-// those from shared memory into TMEM (tcgen05.cp) before the instructions that read them.  Two sets of scale columns take
-// turns; a set is written again once the step that read it has ended.
+// those from shared memory into TMEM (tcgen05.cp) before the instructions that read them.  A set of scale columns
+// is written again once the step that read it has ended.
 //
 // Two kernels.  Pairs: a cluster of two CTAs per 256 x 256 tile (cta_group::2), persistent, for products with tiles enough to fill
 // the SMs.  Clusters: one tile of 128 columns of C (rows of B: the 128 rows of an instruction) by 16 to 128 rows of C per cluster of up to
@@ -30,7 +30,8 @@ struct MxArgs {
   void* C;                 // rows ldc elements apart
   long long ldc;
   const void* bias;        // N values in C's type, or fp32; null: none
-  int bias_f32, act, out, tma_out;
+  int bias_f32, act, out;
+  int vectors;             // rows of C on boundaries and of whole pieces of 32 or of 16 bytes: that; else 0
   int* status;
 };
 
@@ -96,80 +97,119 @@ __device__ __forceinline__ void tile_at(int t, int num_m, int num_n, int& m, int
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------
-// Pairs.  Each CTA stages its 128 rows of A with their scales and 128 of the tile's 256 rows of B, and the scales of all 256 (its
-// half of the accumulator has all columns); CTA 0 issues.  Two accumulators of 256 columns and the scales do not fit into TMEM's
-// 512, so the two overlap in columns 192 to 255: the epilogue drains those first, and then the next tile starts.
+// Pairs: tiles of 256 x 256.  Each CTA stages its 128 rows of A with their scales and half of the tile's rows of B, and the scales of all of
+// these (its half of the accumulator has all columns); CTA 0 issues.  Two accumulators of 256 columns and the scales do not fit into TMEM's
+// 512, so the two overlap in columns 128 to 255: the epilogue drains those first, and then the next tile starts.  (Tiles of 192 columns,
+// whose accumulators do not overlap, were no faster for a K of 768, 24 against 25 us at 16384 x 2304 in MXFP4, and slower for longer ones:
+// 8192^3 437 against 358 us in MXFP8.)  Four sets of scale columns take turns.
 // ---------------------------------------------------------------------------------------------------------------------------
 template <int FMT>
 struct PairCfg {
-  static constexpr int STAGES = 5, EW = 8, THREADS = 64 + 32 * EW;
+  static constexpr int STAGES = 6, EW = 8, THREADS = 64 + 32 * EW;
   static constexpr int A_BYTES = 128 * 128, B_BYTES = 128 * 128, TILE_BYTES = A_BYTES + B_BYTES;
   static constexpr int PIECE = 512, S_BYTES = 3 * Fmt<FMT>::PIECES * PIECE;      // A's row of pieces, B's two
   static constexpr int OFF_SCALES = STAGES * TILE_BYTES;
   static constexpr int OFF_OUT = OFF_SCALES + STAGES * S_BYTES;
-  static constexpr int OUT_BUF = 4096;                       // of an epilogue warp: 32 x 32 values, two buffers of 16-bit ones
-  static constexpr int OFF_BIAS = OFF_OUT + EW * OUT_BUF;
-  static constexpr int OFF_BARS = OFF_BIAS + EW * 128;
+  static constexpr int OUT_BUF = 2048;                       // of an epilogue warp
+  static constexpr int OFF_BARS = OFF_OUT + EW * OUT_BUF;
   static constexpr int BYTES = OFF_BARS + 256;
-  static constexpr int ACC1 = 192, SCALES = 448;             // TMEM columns
-  static_assert(BYTES <= 232448 && OFF_OUT % 512 == 0, "shared memory");
-  static_assert(SCALES + 32 + 12 * Fmt<FMT>::PIECES <= 512, "TMEM");
+  static constexpr int ACC1 = 128, SCALES = 384, SETS = 4, SET = 12 * Fmt<FMT>::PIECES;      // TMEM columns
+  static_assert(BYTES <= 232448 && OFF_OUT % 16 == 0, "shared memory");
+  static_assert(SCALES + SETS * SET <= 512, "TMEM");
 };
 
-__device__ __forceinline__ void put_shared(uint32_t at, const uint4& v) {
-  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+// 32 bytes: one store on a 32-byte boundary (wide), else two of which the second may be left out.
+__device__ __forceinline__ void store32(uint32_t* to, bool wide, bool both, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e, uint32_t f, uint32_t g, uint32_t h) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(a), "r"(b), "r"(c), "r"(d), "r"(e), "r"(f), "r"(g), "r"(h) : "memory");
+  } else {
+    *reinterpret_cast<uint4*>(to) = make_uint4(a, b, c, d);
+    if (both) *reinterpret_cast<uint4*>(to + 4) = make_uint4(e, f, g, h);
+  }
 }
 
-// 32 x 32 results of a warp (a lane has a row) into C: by way of `buf` and TMA, or, where C has no tensor map, row by row.
-__device__ __forceinline__ void store_chunk(const MxArgs& a, const CUtensorMap* tmC, uint8_t* buf, int flip, int slice, int row0, int col0, const float (&v)[32]) {
+// 32 x 32 results of a warp (a lane has a row) into C.  Rows on 32-byte boundaries: 32 bytes a lane and store, whole sectors straight from the
+// registers (an SM stores 32 bytes a clock in any case; by way of shared memory and whole lines a tile took longer: FIGURES).  Other rows,
+// a sector at a time, would write each sector many times: they go through `buf`, a column a lane.
+__device__ __forceinline__ void store_chunk(const MxArgs& a, uint8_t* buf, int slice, int row0, int col0, const float (&v)[32]) {
   const int lane = threadIdx.x & 31;
-  if (a.tma_out) {
-    // 64-byte rows, swizzled in 16-byte pieces
-    const uint32_t swz = (lane >> 1) & 3, row = smem_u32(buf) + lane * 64;
+  const long long first = (long long)slice * a.M + row0;
+  if (a.vectors) {
+    if (row0 + lane >= a.M) return;
+    const bool wide = a.vectors == 32;
     if (a.out == OUT_F32) {
-      if (lane == 0) tma_store_wait_read<0>();
-      __syncwarp();
+      float* to = (float*)a.C + (first + lane) * a.ldc + col0;
 #pragma unroll
-      for (int h = 0; h < 2; h++)
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-          put_shared(row + h * 2048 + ((j ^ swz) << 4), make_uint4(__float_as_uint(v[h * 16 + j * 4]), __float_as_uint(v[h * 16 + j * 4 + 1]),
-                                                                   __float_as_uint(v[h * 16 + j * 4 + 2]), __float_as_uint(v[h * 16 + j * 4 + 3])));
+      for (int j = 0; j < 32; j += 8)
+        if (col0 + j < a.N) store32(reinterpret_cast<uint32_t*>(to + j), wide, col0 + j + 4 < a.N, __float_as_uint(v[j]), __float_as_uint(v[j + 1]), __float_as_uint(v[j + 2]),
+                                    __float_as_uint(v[j + 3]), __float_as_uint(v[j + 4]), __float_as_uint(v[j + 5]), __float_as_uint(v[j + 6]), __float_as_uint(v[j + 7]));
     } else {
-      if (lane == 0) tma_store_wait_read<1>();               // the store before last has left this buffer
-      __syncwarp();
+      uint16_t* to = (uint16_t*)a.C + (first + lane) * a.ldc + col0;
 #pragma unroll
-      for (int j = 0; j < 4; j++)
-        put_shared(row + flip * 2048 + ((j ^ swz) << 4), make_uint4(pack_out(a, v[j * 8], v[j * 8 + 1]), pack_out(a, v[j * 8 + 2], v[j * 8 + 3]),
-                                                                    pack_out(a, v[j * 8 + 4], v[j * 8 + 5]), pack_out(a, v[j * 8 + 6], v[j * 8 + 7])));
-    }
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      if (a.out == OUT_F32) {
-        tma_store_3d(tmC, buf, col0, row0, slice);
-        if (col0 + 16 < a.N) tma_store_3d(tmC, buf + 2048, col0 + 16, row0, slice);
-      } else {
-        tma_store_3d(tmC, buf + flip * 2048, col0, row0, slice);
-      }
-      tma_store_commit();
+      for (int j = 0; j < 32; j += 16)
+        if (col0 + j < a.N) store32(reinterpret_cast<uint32_t*>(to + j), wide, col0 + j + 8 < a.N, pack_out(a, v[j], v[j + 1]), pack_out(a, v[j + 2], v[j + 3]),
+                                    pack_out(a, v[j + 4], v[j + 5]), pack_out(a, v[j + 6], v[j + 7]), pack_out(a, v[j + 8], v[j + 9]), pack_out(a, v[j + 10], v[j + 11]),
+                                    pack_out(a, v[j + 12], v[j + 13]), pack_out(a, v[j + 14], v[j + 15]));
     }
     return;
   }
-  float* f = reinterpret_cast<float*>(buf);
+  const int rows = min(32, a.M - row0);
+  if (a.out == OUT_F32) {                                    // sixteen rows at a time
+    float* f = reinterpret_cast<float*>(buf);
+#pragma unroll 1
+    for (int h = 0; h < 2; h++) {
+      __syncwarp();
+      if (lane >> 4 == h) {
+#pragma unroll
+        for (int j = 0; j < 32; j++) f[(lane & 15) * 32 + (j ^ lane)] = v[j];
+      }
+      __syncwarp();
+      if (col0 + lane < a.N)
+        for (int r = 16 * h; r < min(rows, 16 * h + 16); r++) ((float*)a.C)[(first + r) * a.ldc + col0 + lane] = f[(r & 15) * 32 + (lane ^ r)];
+    }
+    return;
+  }
+  uint32_t* w = reinterpret_cast<uint32_t*>(buf);
   __syncwarp();
 #pragma unroll
-  for (int j = 0; j < 32; j++) f[lane * 32 + (j ^ lane)] = v[j];
+  for (int j = 0; j < 16; j++) w[lane * 16 + (j ^ (lane & 15))] = pack_out(a, v[2 * j], v[2 * j + 1]);
   __syncwarp();
-  const int rows = min(32, a.M - row0);
   if (col0 + lane < a.N)
-    for (int r = 0; r < rows; r++) store_out(a, (row0 + r) * a.ldc + col0 + lane, f[r * 32 + (lane ^ r)]);
+    for (int r = 0; r < rows; r++) ((uint16_t*)a.C)[(first + r) * a.ldc + col0 + lane] = (uint16_t)(w[r * 16 + (lane >> 1 ^ (r & 15))] >> (16 * (lane & 1)));
+}
+
+// The bias of 32 columns, the same in every lane.
+__device__ __forceinline__ void add_bias(const MxArgs& a, int col0, float (&v)[32]) {
+  if (a.bias == nullptr) return;
+  if (col0 + 32 <= a.N && ((uintptr_t)a.bias & 15) == 0) {
+    if (a.bias_f32) {
+#pragma unroll
+      for (int j = 0; j < 32; j += 4) {
+        const float4 b = __ldg(reinterpret_cast<const float4*>((const float*)a.bias + col0 + j));
+        v[j] += b.x; v[j + 1] += b.y; v[j + 2] += b.z; v[j + 3] += b.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; j += 8) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>((const uint16_t*)a.bias + col0 + j));
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float2 b = a.out == OUT_BF16 ? unpack_bf16(w[i]) : unpack_f16(w[i]);
+          v[j + 2 * i] += b.x; v[j + 2 * i + 1] += b.y;
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; j++) v[j] += bias_at(a, col0 + j);
+  }
 }
 
 template <int FMT>
 __global__ void __launch_bounds__(PairCfg<FMT>::THREADS, 1)
 mx_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmSA,
-               const __grid_constant__ CUtensorMap tmSB, const __grid_constant__ CUtensorMap tmC, const MxArgs args) {
+               const __grid_constant__ CUtensorMap tmSB, const MxArgs args) {
   using C = PairCfg<FMT>;
   using F = Fmt<FMT>;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -202,7 +242,6 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     tma_prefetch_desc(&tmB);
     tma_prefetch_desc(&tmSA);
     tma_prefetch_desc(&tmSB);
-    if (args.tma_out) tma_prefetch_desc(&tmC);
   }
   if (warp == 1) {
     tmem_alloc_2sm(slot, 512);
@@ -262,12 +301,12 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
           const int stage = n % C::STAGES;
           ok = mbar_wait(&full[stage], (n / C::STAGES) & 1, abort_flag, args.status, ST_GEMM_TIMEOUT, 33);
           // the step that read this set of scale columns has ended
-          if (ok && n >= 2) ok = mbar_wait(&empty[(n - 2) % C::STAGES], ((n - 2) / C::STAGES) & 1, abort_flag, args.status, ST_GEMM_TIMEOUT, 34);
+          if (ok && n >= C::SETS) ok = mbar_wait(&empty[(n - C::SETS) % C::STAGES], ((n - C::SETS) / C::STAGES) & 1, abort_flag, args.status, ST_GEMM_TIMEOUT, 34);
           if (!ok) break;
           tc_fence_after();
           const uint32_t sa = smem_u32(smem + stage * C::TILE_BYTES), sb = sa + C::A_BYTES;
           const uint32_t ss = smem_u32(smem + C::OFF_SCALES + stage * C::S_BYTES);
-          const uint32_t ta = tmem + C::SCALES + (n & 1) * 32, tb = ta + 4 * F::PIECES;
+          const uint32_t ta = tmem + C::SCALES + n % C::SETS * C::SET, tb = ta + 4 * F::PIECES;
 #pragma unroll
           for (int p = 0; p < F::PIECES; p++) {
             copy_scales<2>(ta + 4 * p, ss + p * C::PIECE);
@@ -293,59 +332,42 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
   } else {
     const int q = warp & 3, half = (warp - 2) >> 2;
     uint8_t* buf = smem + C::OFF_OUT + (warp - 2) * C::OUT_BUF;
-    float* sbias = reinterpret_cast<float*>(smem + C::OFF_BIAS) + (warp - 2) * 32;
-    int local = 0, flip = 0;
+    int local = 0;
     for (int u = pair; u < units; u += pairs, local++) {
       const int slice = u / tiles, which = local & 1;
       int mb, nb;
       tile_at(u - slice * tiles, args.num_m, args.num_n, mb, nb);
       const int row0 = mb * 256 + (int)cta * 128 + q * 32;
-      // four chunks of 32 columns for a warp, the one that lies in the other accumulator's columns first
-      int cols[4];
-      float bl[4];
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int c = i == 0 ? (which ? 0 : 6) + half : (which ? 2 : 0) + half * 3 + i - 1;
-        cols[i] = c * 32;
-        bl[i] = bias_at(args, nb * 256 + cols[i] + lane);
-      }
       if (!mbar_wait(&ready[which], (local >> 1) & 1, abort_flag, args.status, ST_GEMM_TIMEOUT, 35)) break;
       tc_fence_after();
       const uint32_t acc = tmem + which * C::ACC1 + ((uint32_t)(q * 32) << 16);
-#pragma unroll 1
+      // four chunks of 32 columns, two of them in flight; first the two that lie in the other accumulator's columns
+      auto column = [&](int i) { return ((i < 2) == (which != 0) ? 0 : 128) + half * 64 + (i & 1) * 32; };
+      uint32_t r[2][32];
+      tmem_ld32(acc + column(0), r[0]);
+#pragma unroll
       for (int i = 0; i < 4; i++) {
-        uint32_t r[32];
-        tmem_ld32(acc + cols[i], r);
         tmem_ld_wait();
-        if (i == 0) {
+        if (i + 1 < 4) tmem_ld32(acc + column(i + 1), r[(i + 1) & 1]);
+        if (i == 0) {                      // the next tile may start
+          tmem_ld_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(smem_u32(drained) & ~kPeerBit);
+          if (lane == 0) mbar_arrive_cluster_relaxed(smem_u32(drained) & ~kPeerBit);
         }
-        const int col0 = nb * 256 + cols[i];
+        const int col0 = nb * 256 + column(i);
         if (row0 >= args.M || col0 >= args.N) continue;
         float v[32];
 #pragma unroll
-        for (int j = 0; j < 32; j++) v[j] = __uint_as_float(r[j]);
-        if (args.bias != nullptr) {
-          __syncwarp();
-          sbias[lane] = i == 0 ? bl[0] : i == 1 ? bl[1] : i == 2 ? bl[2] : bl[3];
-          __syncwarp();
-#pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 b = *reinterpret_cast<const float4*>(sbias + j);
-            v[j] += b.x; v[j + 1] += b.y; v[j + 2] += b.z; v[j + 3] += b.w;
-          }
-        }
+        for (int j = 0; j < 32; j++) v[j] = __uint_as_float(r[i & 1][j]);
+        add_bias(args, col0, v);
         if (args.act != ACT_NONE) {
 #pragma unroll
           for (int j = 0; j < 32; j++) v[j] = activate(v[j], args.act);
         }
-        store_chunk(args, &tmC, buf, flip, slice, row0, col0, v);
-        flip ^= 1;
+        store_chunk(args, buf, slice, row0, col0, v);
       }
     }
-    if (args.tma_out && lane == 0) tma_store_wait<0>();
   }
 
   tc_fence_before();
@@ -363,22 +385,29 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
 // ---------------------------------------------------------------------------------------------------------------------------
 template <int FMT, int BN>
 struct ClusterCfg {
-  static constexpr int STAGES = BN <= 32 ? 8 : 6, THREADS = 192;
+  // at most half of an SM's shared memory, so that the next kernel's CTAs set up beside this one's
+  static constexpr int STAGES = BN <= 32 ? 5 : BN == 64 ? 4 : 3, THREADS = BN >= 64 ? 320 : 192;     // (more hands for the results)
   static constexpr int A_BYTES = 128 * 128, B_BYTES = BN * 128, TILE_BYTES = A_BYTES + B_BYTES;
   static constexpr int PIECE = 512, S_BYTES = 2 * Fmt<FMT>::PIECES * PIECE;
   static constexpr int OFF_SCALES = STAGES * TILE_BYTES;
   static constexpr int OFF_BARS = OFF_SCALES + STAGES * S_BYTES;
   static constexpr int BYTES = OFF_BARS + 256;
-  static constexpr int TMEM = BN <= 32 ? 64 : 2 * BN;        // the accumulator, then two sets of 8 x PIECES scale columns
-  static_assert(BYTES <= 232448 && BN * 512 <= OFF_SCALES, "shared memory (the partial tile reuses the ring)");
-  static_assert(BN + 16 + 8 * Fmt<FMT>::PIECES <= TMEM, "TMEM");
+  static constexpr int SET = 8 * Fmt<FMT>::PIECES, TMEM = BN <= 64 ? 128 : 256;      // columns: the accumulator, a set of scales for each stage
+  static_assert(BYTES <= 115712 && BN * 512 <= OFF_SCALES, "shared memory (the partial tile reuses the ring)");
+  static_assert(BN + STAGES * SET <= TMEM, "TMEM");
 };
 
+// Bytes that lie side by side (16-byte boundaries and sizes) into shared memory.
+__device__ __forceinline__ void load_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
 template <int FMT, int BN>
-__global__ void __launch_bounds__(ClusterCfg<FMT, BN>::THREADS, 1)
-mx_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmSA,
-                  const __grid_constant__ CUtensorMap tmSB, const MxArgs args) {
-  // "A" of the instruction: args' B (columns of C); its "B": args' A (rows of C)
+__global__ void __launch_bounds__(ClusterCfg<FMT, BN>::THREADS, 2)
+mx_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const uint8_t* __restrict__ sA, const uint8_t* __restrict__ sB,
+                  const MxArgs args) {
+  // "A" of the instruction: the product's B (columns of C); its "B": the product's A (rows of C)
   using C = ClusterCfg<FMT, BN>;
   using F = Fmt<FMT>;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -402,8 +431,6 @@ mx_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
     mbar_fence_init();
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
-    tma_prefetch_desc(&tmSA);
-    tma_prefetch_desc(&tmSB);
   }
   if (warp == 1) {
     tmem_alloc(slot, C::TMEM);
@@ -426,9 +453,9 @@ mx_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         uint8_t* ss = smem + C::OFF_SCALES + stage * C::S_BYTES;
         mbar_expect_tx(&full[stage], C::TILE_BYTES + C::S_BYTES);
         tma_load_3d(sa, &tmA, &full[stage], k * 128, c0, 0);
-        tma_load_3d(ss, &tmSA, &full[stage], 0, k * F::PIECES, c0 >> 7);
         tma_load_3d(sa + C::A_BYTES, &tmB, &full[stage], k * 128, r0, 0);
-        tma_load_3d(ss + F::PIECES * C::PIECE, &tmSB, &full[stage], 0, k * F::PIECES, r0 >> 7);
+        load_bulk(ss, sA + ((long long)(c0 >> 7) * args.steps + k) * (F::PIECES * C::PIECE), F::PIECES * C::PIECE, &full[stage]);
+        load_bulk(ss + F::PIECES * C::PIECE, sB + ((long long)(r0 >> 7) * args.steps + k) * (F::PIECES * C::PIECE), F::PIECES * C::PIECE, &full[stage]);
       }
       if (!ok) {   // a bounded time for the copies in flight
         const uint64_t t0 = globaltimer_ns();
@@ -441,12 +468,10 @@ mx_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
       for (int k = k0, n = 0; k < k1; k++, n++) {
         const int stage = n % C::STAGES;
         if (!mbar_wait(&full[stage], (n / C::STAGES) & 1, abort_flag, args.status, ST_GEMM_TIMEOUT, 42)) break;
-        // the step that read this set of scale columns has ended
-        if (n >= 2 && !mbar_wait(&empty[(n - 2) % C::STAGES], ((n - 2) / C::STAGES) & 1, abort_flag, args.status, ST_GEMM_TIMEOUT, 43)) break;
         tc_fence_after();
         const uint32_t sa = smem_u32(smem + stage * C::TILE_BYTES), sb = sa + C::A_BYTES;
         const uint32_t ss = smem_u32(smem + C::OFF_SCALES + stage * C::S_BYTES);
-        const uint32_t ta = tmem + BN + (n & 1) * (C::TMEM - BN) / 2, tb = ta + 4 * F::PIECES;
+        const uint32_t ta = tmem + BN + stage * C::SET, tb = ta + 4 * F::PIECES;
 #pragma unroll
         for (int p = 0; p < 2 * F::PIECES; p++) copy_scales<1>(ta + 4 * p, ss + p * C::PIECE);
 #pragma unroll
@@ -461,12 +486,13 @@ mx_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
   } else {
     // the accumulator into the ring, transposed (every load has been consumed by then): rows of C of 128 fp32 columns
     const bool ok = mbar_wait(done, 0, abort_flag, args.status, ST_GEMM_TIMEOUT, 44);
-    const int q = warp & 3;
+    const int q = warp & 3, half = (warp - 2) >> 2;          // (of 320 threads: two warps for 32 lanes, 16 columns in turn)
     float* col = reinterpret_cast<float*>(smem) + q * 32 + lane;
     if (__all_sync(0xffffffffu, ok)) {
       tc_fence_after();
 #pragma unroll
-      for (int c = 0; c < BN; c += 16) {
+      for (int c = 16 * half; c < BN; c += 16 * ((C::THREADS - 64) / 128)) {
+        if (c >= args.M - r0) break;                         // (rows of C that are not there)
         uint32_t r[16];
         if (k1 > k0) {
           tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + c, r);
@@ -487,35 +513,49 @@ mx_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
     tmem_dealloc(tmem, C::TMEM);
   }
   if (S > 1) cluster_sync_all();
-  // groups of four columns of a row, dealt to the CTAs of the cluster in turn: sum over the CTAs in order, epilogue, store
-  const int groups = min(BN, args.M - r0) * 32;
-  for (int i = threadIdx.x * S + rank; i < groups; i += C::THREADS * S) {
-    const int r = i >> 5, c = c0 + (i & 31) * 4;
-    const uint32_t at = smem_u32(smem) + i * 16;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (S == 1) {
-      const float4 u = *reinterpret_cast<const float4*>(smem + i * 16);
-      v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
-    } else {
+  // groups of four columns of a row, dealt to the CTAs of the cluster in turn: sum over the CTAs in order, epilogue, store.  A thread stays
+  // in its columns; U groups are in flight.
+  constexpr int U = BN >= 64 ? 4 : 2;
+  const int groups = min(BN, args.M - r0) * 32, first = threadIdx.x * S + rank, stride = C::THREADS * S;
+  const int c = c0 + (first & 31) * 4, size = args.out == OUT_F32 ? 4 : 2;
+  static_assert(C::THREADS % 32 == 0, "a thread stays in its columns");
+  const bool vector = c + 4 <= args.N && (((uintptr_t)args.C | (uintptr_t)(args.ldc * size)) & (4 * size - 1)) == 0;
+  float bias[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) bias[j] = bias_at(args, c + j);
+  for (int i0 = first; i0 < groups; i0 += U * stride) {
+    float4 v[U];
+#pragma unroll
+    for (int k = 0; k < U; k++) {
+      const int i = i0 + k * stride;
+      v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i >= groups) continue;
+      if (S == 1) {
+        v[k] = *reinterpret_cast<const float4*>(smem + i * 16);
+      } else {
+        const uint32_t at = smem_u32(smem) + i * 16;
 #pragma unroll 4
-      for (int p = 0; p < S; p++) {
-        uint32_t remote;
-        float4 u;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(p));
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(u.x), "=f"(u.y), "=f"(u.z), "=f"(u.w) : "r"(remote) : "memory");
-        v[0] += u.x; v[1] += u.y; v[2] += u.z; v[3] += u.w;
+        for (int p = 0; p < S; p++) {
+          uint32_t remote;
+          float4 u;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(p));
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(u.x), "=f"(u.y), "=f"(u.z), "=f"(u.w) : "r"(remote) : "memory");
+          v[k].x += u.x; v[k].y += u.y; v[k].z += u.z; v[k].w += u.w;
+        }
       }
     }
-    if (c >= args.N) continue;
 #pragma unroll
-    for (int j = 0; j < 4; j++) v[j] = activate(v[j] + bias_at(args, c + j), args.act);
-    const long long to = (r0 + r) * args.ldc + c;
-    const int size = args.out == OUT_F32 ? 4 : 2;
-    if (c + 4 <= args.N && (((uintptr_t)args.C + to * size) & (4 * size - 1)) == 0) {
-      if (args.out == OUT_F32) *reinterpret_cast<float4*>((float*)args.C + to) = make_float4(v[0], v[1], v[2], v[3]);
-      else *reinterpret_cast<uint2*>((uint16_t*)args.C + to) = make_uint2(pack_out(args, v[0], v[1]), pack_out(args, v[2], v[3]));
-    } else {
-      for (int j = 0; j < 4 && c + j < args.N; j++) store_out(args, to + j, v[j]);
+    for (int k = 0; k < U; k++) {
+      const int i = i0 + k * stride;
+      if (i >= groups || c >= args.N) break;
+      const float y[4] = {activate(v[k].x + bias[0], args.act), activate(v[k].y + bias[1], args.act), activate(v[k].z + bias[2], args.act), activate(v[k].w + bias[3], args.act)};
+      const long long to = (long long)(r0 + (i >> 5)) * args.ldc + c;
+      if (vector) {
+        if (args.out == OUT_F32) *reinterpret_cast<float4*>((float*)args.C + to) = make_float4(y[0], y[1], y[2], y[3]);
+        else *reinterpret_cast<uint2*>((uint16_t*)args.C + to) = make_uint2(pack_out(args, y[0], y[1]), pack_out(args, y[2], y[3]));
+      } else {
+        for (int j = 0; j < 4 && c + j < args.N; j++) store_out(args, to + j, y[j]);
+      }
     }
   }
   if (S > 1) cluster_sync_all();   // nobody leaves while another may still read its shared memory
@@ -547,20 +587,56 @@ struct Plan {
   long long workspace;     // bytes: fp32 slices of a cut product of the pair kernel
 };
 
+thread_local int g_kind = 0, g_splits = 0;       // gb_mx_tune
+
+// Microseconds that a product takes in either kernel, by what was measured of them.  A step takes 0.3 of either (an SM's 32 KB; or the 1.6 us
+// of a load over the 100 KB that a cluster's CTA has in flight).  Pairs: 4 for the launch, the first loads and the last results, 1.5 for a
+// tile's own, and for slices a second launch and their values' way through L2.  Clusters: 2.5 and what a tile's rows cost; from two CTAs
+// on the exchange, whose values the more CTAs share the way of, the longer they take.  us, measured | so, of 64 steps (MXFP8, N = 2048, K = 8192):
+//   clusters of 1, 2, 4, 8: 1 row 20.6, 12.4, 7.9, 6.2 | 20.4, 12.5, 8.1, 6.1; 64 rows 22.2, 14.5, 10.8, 13.3 | 21.6, 14.6, 11.2, 13.7;
+//   128 rows 23.0, 15.9, 13.9, 20.4 | 22.7, 16.7, 14.2, 23.7; 200 rows in clusters of 4 17.8 | 18.1;  pairs: 128 rows 23.6 | 24.7, 384 in 4 slices 16.5 | 15.9
+// and 2304 x 768 x 16384 as pairs in 1, 2, 5 slices 43.7, 32.7, 34.8 | 43.9, 30.7, 34.5; 1 x 2304 x 768 as clusters of 1, 2, 4 4.2, 4.4, 4.0 | 4.2, 4.4, 4.2.
+double pair_us(long long M, long long N, long long tiles, int steps, int splits) {
+  const long long units = tiles * splits, waves = (units + 73) / 74;
+  const int per = (steps + splits - 1) / splits;
+  return 4.0 + waves * (per * 0.3 + 1.5) + (splits > 1 ? 2.5 + splits * 1e-6 * M * N : 0.0);
+}
+double cluster_us(long long M, int bn, long long tiles, int steps, int splits) {
+  const double ctas = (double)tiles * splits, rows = M < bn ? M : bn, waves = ctas > 296 ? ctas / 296 : 1.0;      // (two CTAs on an SM)
+  return 1.0 + waves * (1.5 + rows * 0.018) + (steps + splits - 1) / splits * 0.28 * (ctas > 148 ? ctas / 148 : 1.0) +
+         (splits > 1 ? 0.9 + 0.05 * splits + 0.0075 * splits * rows * (ctas > 64 ? ctas / 64 : 1.0) : 0.0);
+}
+
 Plan plan_of(long long M, long long N, long long K, int fmt) {
   Plan p{};
   p.steps = (int)((K + (fmt == FP8 ? 127 : 255)) / (fmt == FP8 ? 128 : 256));
-  const long long tiles2 = ((M + 255) / 256) * ((N + 255) / 256);
-  p.splits = 1;
-  if (M > 128 && tiles2 >= 37) {
-    p.pair = 1;
-    p.steps_per = p.steps;
-    return p;
+  const int bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  const long long pair_tiles = ((M + 255) / 256) * ((N + 255) / 256), tiles = ((M + bn - 1) / bn) * ((N + 127) / 128);
+  double best = 1e30;
+  if (g_kind != 2) {
+    const int least = g_splits ? g_splits : 1, most = g_splits ? g_splits : pair_tiles < 74 ? 8 : 1;
+    for (int s = least; s <= most && (s == 1 || (s <= p.steps && N % 4 == 0)); s++) {
+      const double us = pair_us(M, N, pair_tiles, p.steps, s);
+      if (us < best) { best = us; p.pair = 1; p.splits = s; }
+    }
   }
-  p.bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-  const long long tiles = ((M + p.bn - 1) / p.bn) * ((N + 127) / 128);
-  while (p.splits < 8 && tiles * p.splits * 2 <= 148 + 18 && p.splits * 2 <= p.steps) p.splits *= 2;
+  if (g_kind != 1) {
+    for (int s = 1; s <= 8; s *= 2) {
+      if (g_splits ? s != (g_splits < 8 ? g_splits : 8) : (s > 1 && (s > p.steps || tiles * s > 296))) continue;
+      const double us = cluster_us(M, bn, tiles, p.steps, s);
+      if (us < best) { best = us; p.pair = 0; p.splits = s; }
+    }
+  }
+  if (p.splits == 0) {         // (asked for slices that this product cannot have)
+    p.pair = g_kind != 2;
+    p.splits = 1;
+  }
+  p.bn = p.pair ? 256 : bn;
   p.steps_per = (p.steps + p.splits - 1) / p.splits;
+  if (p.pair) {
+    p.splits = (p.steps + p.steps_per - 1) / p.steps_per;      // no empty slice
+    p.workspace = p.splits > 1 ? M * N * 4 * p.splits : 0;
+  }
   return p;
 }
 
@@ -576,7 +652,7 @@ int allow_shared(K kern, int bytes, std::atomic<uint32_t>& done) {
 }
 
 struct Maps {
-  CUtensorMap a, b, sa, sb, c;
+  CUtensorMap a, b, sa, sb;
 };
 
 int map_codes(CUtensorMap* m, const void* p, long long rows, long long rb, int box_rows) {
@@ -598,21 +674,33 @@ int launch_pair(const Maps& tm, const MxArgs& args, cudaStream_t st) {
   if (int rc = allow_shared(mx_pair_kernel<FMT>, C::BYTES, done)) return rc;
   const long long units = (long long)args.num_m * args.num_n * args.splits;
   const int pairs = units < 74 ? (int)units : 74;
-  GB_CUDA_OK(gbh::launch(mx_pair_kernel<FMT>, dim3(2 * pairs), dim3(C::THREADS), C::BYTES, st, 2, tm.a, tm.b, tm.sa, tm.sb, tm.c, args));
+  GB_CUDA_OK(gbh::launch(mx_pair_kernel<FMT>, dim3(2 * pairs), dim3(C::THREADS), C::BYTES, st, 2, tm.a, tm.b, tm.sa, tm.sb, args));
   return gbh::E_OK;
 }
 template <int FMT, int BN>
-int launch_cluster(const Maps& tm, const MxArgs& args, cudaStream_t st) {
+int launch_cluster(const Maps& tm, const void* sa, const void* sb, const MxArgs& args, cudaStream_t st) {
   using C = ClusterCfg<FMT, BN>;
   static std::atomic<uint32_t> done{0};
   if (int rc = allow_shared(mx_cluster_kernel<FMT, BN>, C::BYTES, done)) return rc;
-  GB_CUDA_OK(gbh::launch(mx_cluster_kernel<FMT, BN>, dim3(args.num_m * args.num_n * args.splits), dim3(C::THREADS), C::BYTES, st, args.splits, tm.a, tm.b, tm.sa, tm.sb, args));
+  GB_CUDA_OK(gbh::launch(mx_cluster_kernel<FMT, BN>, dim3(args.num_m * args.num_n * args.splits), dim3(C::THREADS), C::BYTES, st, args.splits, tm.a, tm.b,
+                         (const uint8_t*)sa, (const uint8_t*)sb, args));
   return gbh::E_OK;
 }
 
 }  // namespace
 
-// How a product runs (for tests): 1 pairs, 2 clusters; rows of a cluster's tile; slices of K; workspace bytes.
+// The kernel of products from this thread: kind 0 by size, 1 pairs, 2 clusters; splits 0 by size, else that many slices of K.
+GB_EXPORT int gb_mx_tune(int kind, int splits) {
+  if (kind < 0 || kind > 2 || splits < 0 || splits > 64) {
+    gbh::set_error("gb_mx_tune: kind %d, splits %d", kind, splits);
+    return gbh::E_BAD_ARG;
+  }
+  g_kind = kind;
+  g_splits = splits;
+  return gbh::E_OK;
+}
+
+// How a product runs (for tests): 1 pairs, 2 clusters; rows of a tile; slices of K; workspace bytes.
 GB_EXPORT int gb_mx_plan(long long M, long long N, long long K, int fmt, long long* out4) {
   if (M <= 0 || N <= 0 || K <= 0 || M > 0x7fffffffLL || N > 0x7fffffffLL || K > (1LL << 30) || (fmt != FP8 && fmt != FP4)) {
     gbh::set_error("gb_mx_plan: bad extents %lld x %lld x %lld, format %d", M, N, K, fmt);
@@ -620,7 +708,7 @@ GB_EXPORT int gb_mx_plan(long long M, long long N, long long K, int fmt, long lo
   }
   const Plan p = plan_of(M, N, K, fmt);
   out4[0] = p.pair ? 1 : 2;
-  out4[1] = p.pair ? 256 : p.bn;
+  out4[1] = p.bn;
   out4[2] = p.splits;
   out4[3] = p.workspace;
   return gbh::E_OK;
@@ -659,12 +747,8 @@ GB_EXPORT int gb_mx_matmul(int fmt, const void* a, const void* sa, const void* b
       run.C = workspace; run.ldc = N; run.out = OUT_F32; run.bias = nullptr; run.act = ACT_NONE;
     }
     const int size = run.out == OUT_F32 ? 4 : 2;
-    run.tma_out = ((uintptr_t)run.C & 15) == 0 && run.ldc * size % 16 == 0;
-    if (run.tma_out) {
-      const uint64_t dims[3] = {(uint64_t)N, (uint64_t)M, (uint64_t)p.splits}, strides[2] = {(uint64_t)(run.ldc * size), (uint64_t)(run.ldc * size * M)};
-      const uint32_t box[3] = {(uint32_t)(64 / size), 32, 1};
-      rc = gbh::encode_tmap(&tm.c, size == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, run.C, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
-    }
+    const auto whole = [&](int bytes) { return (uintptr_t)run.C % bytes == 0 && run.ldc * size % bytes == 0 && N * size % bytes == 0; };
+    run.vectors = whole(32) ? 32 : whole(16) ? 16 : 0;
     if (!rc) rc = map_codes(&tm.a, a, M, RB, 128);
     if (!rc) rc = map_codes(&tm.b, b, N, RB, 128);
     if (!rc) rc = map_scales(&tm.sa, sa, M, P, per, 1);
@@ -683,13 +767,11 @@ GB_EXPORT int gb_mx_matmul(int fmt, const void* a, const void* sa, const void* b
   }
   rc = map_codes(&tm.a, b, N, RB, 128);
   if (!rc) rc = map_codes(&tm.b, a, M, RB, p.bn);
-  if (!rc) rc = map_scales(&tm.sa, sb, N, P, per, 1);
-  if (!rc) rc = map_scales(&tm.sb, sa, M, P, per, 1);
   if (rc) return rc;
   switch (p.bn) {
-    case 16: return fmt == FP8 ? launch_cluster<FP8, 16>(tm, args, st) : launch_cluster<FP4, 16>(tm, args, st);
-    case 32: return fmt == FP8 ? launch_cluster<FP8, 32>(tm, args, st) : launch_cluster<FP4, 32>(tm, args, st);
-    case 64: return fmt == FP8 ? launch_cluster<FP8, 64>(tm, args, st) : launch_cluster<FP4, 64>(tm, args, st);
-    default: return fmt == FP8 ? launch_cluster<FP8, 128>(tm, args, st) : launch_cluster<FP4, 128>(tm, args, st);
+    case 16: return fmt == FP8 ? launch_cluster<FP8, 16>(tm, sb, sa, args, st) : launch_cluster<FP4, 16>(tm, sb, sa, args, st);
+    case 32: return fmt == FP8 ? launch_cluster<FP8, 32>(tm, sb, sa, args, st) : launch_cluster<FP4, 32>(tm, sb, sa, args, st);
+    case 64: return fmt == FP8 ? launch_cluster<FP8, 64>(tm, sb, sa, args, st) : launch_cluster<FP4, 64>(tm, sb, sa, args, st);
+    default: return fmt == FP8 ? launch_cluster<FP8, 128>(tm, sb, sa, args, st) : launch_cluster<FP4, 128>(tm, sb, sa, args, st);
   }
 }

@@ -1,8 +1,9 @@
 // Microscaled quantisation (formats: mx.cuh): rows of a tensor into codes and scales, back into values, and the residual's
 // addition with the root-mean-square norm whose output is quantised where it is made.
 //
-// All three are bound by memory.  Sixteen lanes hold 128 columns, eight each: 16-byte loads of 16-bit types, a block's largest
-// magnitude by two shuffles over its four lanes, its scales as one word by two more, codes of 8 or 4 bytes a lane in whole lines.
+// All are bound by memory, and by instructions if those are not few: a lane takes sixteen columns (32 bytes of a 16-bit type), two
+// lanes a block, eight lanes the 128 columns whose scales are one word.  Magnitudes of 16-bit types compare in pairs, before anything is
+// converted.
 #include "mx.cuh"
 
 #include <atomic>
@@ -22,45 +23,40 @@ struct QuantArgs {
   uint8_t* data;
   uint8_t* scales;
   long long ld;            // elements from row to row of x
-  int rows, K, pieces, row_bytes;
+  int rows, K, pieces, row_bytes, wide;
   FastDiv by_pieces;
   Extent ext;
 };
 
-// A unit is 128 columns of a row, taken by sixteen lanes; NU units of a lane are in flight.
-template <typename T, int FMT>
+// A unit is 128 columns of a row; NU units of a lane are in flight.
+template <typename T, int FMT, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const QuantArgs a) {
-  constexpr int NU = 2;
+  constexpr int NU = Elem<T>::SZ == 2 ? 2 : 1;
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31, l16 = threadIdx.x & 15;
-  const unsigned mask = 0xffffu << (lane & 16);
-  const uint32_t units = (uint32_t)a.rows * (uint32_t)a.pieces, stride = gridDim.x * (kThreads / 16);
-  for (uint32_t u0 = blockIdx.x * (kThreads / 16) + (threadIdx.x >> 4); u0 < units; u0 += NU * stride) {
-    uint32_t w[NU][2 * Elem<T>::SZ];
+  const int lane = threadIdx.x & 31, l8 = threadIdx.x & 7;
+  const unsigned mask = 0xffu << (lane & 24);
+  const uint32_t units = (uint32_t)a.rows * (uint32_t)a.pieces, stride = gridDim.x * (kThreads / 8);
+  for (uint32_t u0 = blockIdx.x * (kThreads / 8) + (threadIdx.x >> 3); u0 < units; u0 += NU * stride) {
+    uint32_t w[NU][4 * Elem<T>::SZ];
     uint32_t row[NU];
     int g[NU];
 #pragma unroll
     for (int i = 0; i < NU; i++) {
-      const uint32_t u = u0 + i * stride;
-      row[i] = a.by_pieces.div(u < units ? u : u0);
-      g[i] = (int)((u < units ? u : u0) - row[i] * a.by_pieces.d);
-      load8(reinterpret_cast<const T*>(a.x) + row[i] * a.ld, g[i] * 128 + l16 * 8, a.K, a.ext, w[i]);
+      const uint32_t u = min(u0 + i * stride, units - 1);
+      row[i] = a.by_pieces.div(u);
+      g[i] = (int)(u - row[i] * a.by_pieces.d);
+      load16<T, ALIGNED>(reinterpret_cast<const T*>(a.x) + row[i] * a.ld, g[i] * 128 + l8 * 16, a.K, a.wide, a.ext, w[i]);
     }
 #pragma unroll
     for (int i = 0; i < NU; i++) {
       if (u0 + i * stride >= units) break;
-      float v[8];
-      Elem<T>::unpack(w[i], v);
-      uint32_t out[2];
-      const uint32_t word = quantize8(v, FMT, mask, lane, out);
-      const int b = (g[i] * 128 + l16 * 8) / (FMT == FP8 ? 1 : 2);
-      if (b < a.row_bytes) {
-        uint8_t* to = a.data + (long long)row[i] * a.row_bytes + b;
-        if (FMT == FP8) *reinterpret_cast<uint2*>(to) = make_uint2(out[0], out[1]);
-        else *reinterpret_cast<uint32_t*>(to) = out[0];
-      }
-      if (l16 == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_word(row[i], g[i], a.pieces)) = word;
+      float v[16];
+      unpack16<T>(w[i], v);
+      uint32_t out[4];
+      const uint32_t word = quantize16<FMT>(v, largest16<T>(w[i]), mask, lane, out);
+      store_codes<FMT>(a.data + (long long)row[i] * a.row_bytes, g[i] * 128 + l8 * 16, a.row_bytes, out);
+      if (l8 == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_word(row[i], g[i], a.pieces)) = word;
     }
   }
 }
@@ -76,7 +72,8 @@ struct BothArgs {
   uint8_t* data_t;         // codes of the transpose along the rows, K x row_bytes_t
   uint8_t* scales_t;
   long long ld;
-  int rows, K, pieces, row_bytes, pieces_t, row_bytes_t;
+  int rows, K, pieces, row_bytes, pieces_t, row_bytes_t, wide;
+  float* sums;             // column sums of each 128 rows (row pieces x K), or null
   Extent ext;
 };
 
@@ -89,54 +86,76 @@ struct BothCfg {
   static constexpr int BYTES = TILE + 128 * PITCH + 1024;
 };
 
-template <typename T>
+template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads) mx_quantize_both_kernel(const BothArgs a) {
   using C = BothCfg<T>;
-  constexpr int W = 2 * Elem<T>::SZ;                     // words of eight elements
+  constexpr int W = 4 * Elem<T>::SZ;                     // words of sixteen elements
   extern __shared__ __align__(16) uint8_t smem[];
   uint8_t* codes = smem + C::TILE;
   uint32_t* piece = reinterpret_cast<uint32_t*>(codes + 128 * C::PITCH);
   uint8_t* piece_t = reinterpret_cast<uint8_t*>(piece + 128);
+  __shared__ float part[4][128];
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31, l16 = threadIdx.x & 15, h = threadIdx.x >> 4;
+  const int lane = threadIdx.x & 31, l8 = threadIdx.x & 7, h = threadIdx.x >> 3;
+  const unsigned mask = 0xffu << (lane & 24);
   const int g = blockIdx.x % a.pieces, gt = blockIdx.x / a.pieces;       // pieces along the columns and the rows
-  const int k = g * 128 + l16 * 8;
-#pragma unroll 4
-  for (int i = 0; i < 8; i++) {
-    const int r = h + 16 * i;
+  const int k = g * 128 + l8 * 16;
+  uint32_t w[4][W];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const long long row = gt * 128LL + h + 32 * i;
+#pragma unroll
+    for (int j = 0; j < W; j++) w[i][j] = 0;
+    if (row < a.rows) load16<T, ALIGNED>(reinterpret_cast<const T*>(a.x) + row * a.ld, k, a.K, a.wide, a.ext, w[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int r = h + 32 * i;
     const long long row = gt * 128LL + r;
-    uint32_t w[W];
 #pragma unroll
-    for (int j = 0; j < W; j++) w[j] = 0;
-    if (row < a.rows) load8(reinterpret_cast<const T*>(a.x) + row * a.ld, k, a.K, a.ext, w);
-#pragma unroll
-    for (int j = 0; j < W; j += 4) *reinterpret_cast<uint4*>(smem + (r * 128 + l16 * 8) * Elem<T>::SZ + j * 4) = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
-    float v[8];
-    Elem<T>::unpack(w, v);
-    uint32_t out[2];
-    const uint32_t word = quantize8(v, FP8, 0xffffu << (lane & 16), lane, out);
-    if (row < a.rows && k < a.row_bytes) *reinterpret_cast<uint2*>(a.data + row * a.row_bytes + k) = make_uint2(out[0], out[1]);
-    if (l16 == 0) piece[(r & 31) * 4 + (r >> 5)] = word;
+    for (int j = 0; j < W; j += 4) *reinterpret_cast<uint4*>(smem + (r * 128 + l8 * 16) * Elem<T>::SZ + j * 4) = make_uint4(w[i][j], w[i][j + 1], w[i][j + 2], w[i][j + 3]);
+    float v[16];
+    unpack16<T>(w[i], v);
+    uint32_t out[4];
+    const uint32_t word = quantize16<FP8>(v, largest16<T>(w[i]), mask, lane, out);
+    if (row < a.rows) store_codes<FP8>(a.data + row * a.row_bytes, k, a.row_bytes, out);
+    if (l8 == 0) piece[h * 4 + i] = word;
   }
   __syncthreads();
   // columns 2 p and 2 p + 1, rows 32 b .. 32 b + 31
   const int p = threadIdx.x & 63, b = threadIdx.x >> 6;
-  float x0[32], x1[32];
   uint32_t m0 = 0, m1 = 0;
+  float x0[32], x1[32];
+  if constexpr (Elem<T>::SZ == 2) {
+    uint32_t u[32], m = 0;
 #pragma unroll
-  for (int i = 0; i < 32; i++) {
-    const uint8_t* at = smem + ((b * 32 + i) * 128 + p * 2) * Elem<T>::SZ;
-    if constexpr (Elem<T>::SZ == 4) {
-      const float2 f = *reinterpret_cast<const float2*>(at);
-      x0[i] = f.x; x1[i] = f.y;
-    } else if constexpr (sizeof(T) == 2) {
-      const uint32_t u = *reinterpret_cast<const uint32_t*>(at);
-      const float2 f = Elem<T>::pair(u);
+    for (int i = 0; i < 32; i++) {
+      u[i] = *reinterpret_cast<const uint32_t*>(smem + ((b * 32 + i) * 128 + p * 2) * 2);
+      asm("max.u16x2 %0, %0, %1;" : "+r"(m) : "r"(u[i] & 0x7fff7fffu));
+    }
+    m0 = Elem<T>::bits(m & 0xffffu);
+    m1 = Elem<T>::bits(m >> 16);
+#pragma unroll
+    for (int i = 0; i < 32; i++) {
+      const float2 f = Elem<T>::pair(u[i]);
       x0[i] = f.x; x1[i] = f.y;
     }
-    m0 = max(m0, __float_as_uint(x0[i]) & 0x7fffffffu);
-    m1 = max(m1, __float_as_uint(x1[i]) & 0x7fffffffu);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; i++) {
+      const float2 f = *reinterpret_cast<const float2*>(smem + ((b * 32 + i) * 128 + p * 2) * 4);
+      x0[i] = f.x; x1[i] = f.y;
+      m0 = max(m0, __float_as_uint(f.x) & 0x7fffffffu);
+      m1 = max(m1, __float_as_uint(f.y) & 0x7fffffffu);
+    }
+  }
+  if (a.sums != nullptr) {
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; i++) { s0 += x0[i]; s1 += x1[i]; }
+    part[b][2 * p] = s0;
+    part[b][2 * p + 1] = s1;
   }
   const uint32_t c0 = scale_code(m0, FP8), c1 = scale_code(m1, FP8);
   const float i0 = scale_inverse(c0), i1 = scale_inverse(c1);
@@ -154,6 +173,8 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_both_kernel(const BothAr
     piece_t[(col & 31) * 16 + (col >> 5) * 4 + b] = (uint8_t)(c == 0 ? c0 : c1);
   }
   __syncthreads();
+  if (a.sums != nullptr && threadIdx.x < 128 && g * 128 + threadIdx.x < a.K)
+    a.sums[(long long)gt * a.K + g * 128 + threadIdx.x] = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
   if (threadIdx.x < 128) reinterpret_cast<uint32_t*>(a.scales + ((long long)gt * a.pieces + g) * 512)[threadIdx.x] = piece[threadIdx.x];
   else reinterpret_cast<uint32_t*>(a.scales_t + ((long long)g * a.pieces_t + gt) * 512)[threadIdx.x - 128] = reinterpret_cast<const uint32_t*>(piece_t)[threadIdx.x - 128];
   const int at = gt * 128 + (threadIdx.x & 7) * 16;
@@ -162,6 +183,25 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_both_kernel(const BothAr
     const int col = (threadIdx.x >> 3) + 32 * i;
     if (g * 128 + col < a.K && at < a.row_bytes_t)
       *reinterpret_cast<uint4*>(a.data_t + (g * 128LL + col) * a.row_bytes_t + at) = *reinterpret_cast<const uint4*>(codes + col * C::PITCH + (threadIdx.x & 7) * 16);
+  }
+}
+
+// Sums over the pieces of rows that mx_quantize_both_kernel left, in fp32 and in one order: 32 columns a block, eight strips of pieces.
+template <typename T>
+__global__ void __launch_bounds__(256) mx_column_sum_kernel(const float* __restrict__ sums, T* __restrict__ out, int pieces, int K) {
+  __shared__ float part[8][32];
+  pdl_trigger();
+  pdl_wait();
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), strip = threadIdx.x >> 5;
+  float s = 0.f;
+  if (c < K)
+    for (int i = strip; i < pieces; i += 8) s += __ldg(sums + (long long)i * K + c);
+  part[strip][threadIdx.x & 31] = s;
+  __syncthreads();
+  if (strip == 0 && c < K) {
+#pragma unroll
+    for (int i = 1; i < 8; i++) s += part[i][threadIdx.x];
+    out[c] = to_type<T>(s);
   }
 }
 
@@ -176,61 +216,61 @@ struct DequantArgs {
   FastDiv by_pieces;
 };
 
-template <typename T>
-__device__ __forceinline__ T to_type(float v);
-template <> __device__ __forceinline__ float to_type<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half to_type<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 to_type<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <int FMT>
+__device__ __forceinline__ void numbers16(const uint32_t (&c)[4], float (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    uint32_t h;
+    if (FMT == FP8) asm("{\n.reg .b16 t;\ncvt.u16.u32 t, %1;\ncvt.rn.f16x2.e4m3x2 %0, t;\n}" : "=r"(h) : "r"(c[i / 2] >> (16 * (i & 1))));
+    else asm("{\n.reg .b8 t, u0, u1, u2;\nmov.b32 {t, u0, u1, u2}, %1;\ncvt.rn.f16x2.e2m1x2 %0, t;\n}" : "=r"(h) : "r"(c[i / 4] >> (8 * (i & 3))));
+    const float2 f = unpack_f16(h);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
 
-template <typename T, int FMT>
+template <typename T, int FMT, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads) mx_dequantize_kernel(const DequantArgs a) {
+  constexpr int NU = 2;
+  __shared__ __align__(16) float bufs[ALIGNED ? 4 : kThreads * 16];
   pdl_trigger();
   pdl_wait();
-  const int l16 = threadIdx.x & 15;
-  const uint32_t units = (uint32_t)a.rows * (uint32_t)a.pieces, stride = gridDim.x * (kThreads / 16);
-  for (uint32_t u = blockIdx.x * (kThreads / 16) + (threadIdx.x >> 4); u < units; u += stride) {
-    const uint32_t row = a.by_pieces.div(u);
-    const int g = (int)(u - row * a.by_pieces.d), k = g * 128 + l16 * 8;
-    if (k >= a.K) continue;
-    const uint8_t* from = a.data + (long long)row * a.row_bytes + k / (FMT == FP8 ? 1 : 2);
-    const float s = scale_value(__ldg(a.scales + scale_word(row, g, a.pieces) + (l16 >> 2)));
-    float v[8];
-    if (FMT == FP8) {
-      const uint2 c = __ldg(reinterpret_cast<const uint2*>(from));
+  const int lane = threadIdx.x & 31, l8 = threadIdx.x & 7;
+  const uint32_t units = (uint32_t)a.rows * (uint32_t)a.pieces, stride = gridDim.x * (kThreads / 8);
+  for (uint32_t u0 = blockIdx.x * (kThreads / 8) + (threadIdx.x >> 3); u0 < units; u0 += NU * stride) {
+    uint32_t c[NU][4], row[NU];
+    int g[NU];
+    uint8_t s[NU];
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const uint32_t two = ((i < 2 ? c.x : c.y) >> (16 * (i & 1))) & 0xffffu;
-        uint32_t h;
-        asm("{\n.reg .b16 t;\ncvt.u16.u32 t, %1;\ncvt.rn.f16x2.e4m3x2 %0, t;\n}" : "=r"(h) : "r"(two));
-        const float2 f = unpack_f16(h);
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
+    for (int i = 0; i < NU; i++) {
+      const uint32_t u = min(u0 + i * stride, units - 1);
+      row[i] = a.by_pieces.div(u);
+      g[i] = (int)(u - row[i] * a.by_pieces.d);
+      const int k = g[i] * 128 + l8 * 16, b = FMT == FP8 ? k : k / 2;
+      const uint8_t* from = a.data + (long long)row[i] * a.row_bytes + b;
+      c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0;
+      if (b < a.row_bytes) {
+        if (FMT == FP8) {
+          const uint4 q = __ldg(reinterpret_cast<const uint4*>(from));
+          c[i][0] = q.x; c[i][1] = q.y; c[i][2] = q.z; c[i][3] = q.w;
+        } else {
+          const uint2 q = __ldg(reinterpret_cast<const uint2*>(from));
+          c[i][0] = q.x; c[i][1] = q.y;
+        }
       }
-    } else {
-      const uint32_t c = __ldg(reinterpret_cast<const uint32_t*>(from));
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        uint32_t h;
-        asm("{\n.reg .b8 t, u0, u1, u2;\nmov.b32 {t, u0, u1, u2}, %1;\ncvt.rn.f16x2.e2m1x2 %0, t;\n}" : "=r"(h) : "r"(c >> (8 * i)));
-        const float2 f = unpack_f16(h);
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-      }
+      s[i] = __ldg(a.scales + scale_word(row[i], g[i], a.pieces) + (l8 >> 1));
     }
 #pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = mul_exact(v[i], s);
-    T* to = reinterpret_cast<T*>(a.y) + (long long)row * a.K + k;
-    if (k + 8 <= a.K && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
-      if constexpr (sizeof(T) == 4) {
-        reinterpret_cast<float4*>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
-      } else {
-        *reinterpret_cast<uint4*>(to) = make_uint4(Elem<T>::pack(v[0], v[1]), Elem<T>::pack(v[2], v[3]), Elem<T>::pack(v[4], v[5]), Elem<T>::pack(v[6], v[7]));
-      }
-    } else {
+    for (int i = 0; i < NU; i++) {
+      if (u0 + i * stride >= units) break;
+      float v[16];
+      numbers16<FMT>(c[i], v);
+      const float scale = scale_value(s[i]);
 #pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (k + i < a.K) to[i] = to_type<T>(v[i]);
+      for (int j = 0; j < 16; j++) v[j] = mul_exact(v[j], scale);
+      T* to = reinterpret_cast<T*>(a.y) + (long long)row[i] * a.K;
+      if constexpr (ALIGNED) store16(to, g[i] * 128 + l8 * 16, a.K, v);
+      else store16_any<T, 8>(to, g[i] * 128, a.K, v, bufs + (threadIdx.x >> 3) * 128, l8, 0xffu << (lane & 24));
     }
   }
 }
@@ -246,78 +286,69 @@ struct NormArgs {
   uint8_t* data;
   uint8_t* scales;
   long long ldx, ldr;
-  int rows, K, pieces, row_bytes, w_f32, fmt;
+  int rows, K, pieces, row_bytes, w_f32, wide;
   float eps;
   Extent ex, er, ew;
 };
 
-// The sum of a row in fp32; its inverse root in fp64 and rounded once (approximations of a last bit would move a row's values
-// over the borders between codes more often than the roundings of the two products do).
-__device__ __forceinline__ float inverse_root(float sum, int K, float eps) { return (float)(1.0 / sqrt((double)sum / K + (double)eps)); }
+__device__ __forceinline__ float add_exact(float a, float b) {
+  float d;
+  asm("add.rn.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 
-template <typename T>
-__device__ __forceinline__ void weights8(const NormArgs& a, int k, float* f) {
-  if (a.w_f32) {
-    uint32_t u[8];
-    load8(reinterpret_cast<const float*>(a.w), k, a.K, a.ew, u);
-    Elem<float>::unpack(u, f);
+// 1 / sqrt(sum / K + eps) to its last bit or nearly so (the approximation, corrected by its residual: a row's values would otherwise move
+// over the borders between codes more often than the roundings of their two products move them).
+__device__ __forceinline__ float inverse_root(float sum, int K, float eps) {
+  const float v = add_exact(__fdiv_rn(sum, (float)K), eps);
+  float r;
+  asm("rsqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  if (v > 1e-30f && v < 1e30f) {
+    const float t = v * r, e = fmaf(-t, r, 1.f) - fmaf(v, r, -t) * r;      // 1 - v r^2
+    r = fmaf(0.5f * r, e, r);
+  }
+  return r;
+}
+
+// A row's weights stand still while rows come and go: vectors from L1.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void weights16(const NormArgs& a, int k, float (&f)[16]) {
+  if (sizeof(T) == 2 && a.w_f32) {
+    uint32_t u[16];
+    load16<float, false>(reinterpret_cast<const float*>(a.w), k, a.K, false, a.ew, u);
+    unpack16<float>(u, f);
   } else {
-    uint32_t u[2 * Elem<T>::SZ];
-    load8(reinterpret_cast<const T*>(a.w), k, a.K, a.ew, u);
-    Elem<T>::unpack(u, f);
+    uint32_t u[4 * Elem<T>::SZ];
+    load16<T, ALIGNED>(reinterpret_cast<const T*>(a.w), k, a.K, false, a.ew, u);
+    unpack16<T>(u, f);
   }
 }
 
-// x + r of eight columns, in fp32 and unrounded for the norm, rounded into h.
-template <typename T>
-__device__ __forceinline__ void sum8(const NormArgs& a, long long row, int k, bool write, float* v) {
-  uint32_t u[2 * Elem<T>::SZ];
-  load8(reinterpret_cast<const T*>(a.x) + row * a.ldx, k, a.K, a.ex, u);
-  Elem<T>::unpack(u, v);
-  if (a.r == nullptr) return;
-  float f[8];
-  load8(reinterpret_cast<const T*>(a.r) + row * a.ldr, k, a.K, a.er, u);
-  Elem<T>::unpack(u, f);
-#pragma unroll
-  for (int i = 0; i < 8; i++) asm("add.rn.f32 %0, %1, %2;" : "=f"(v[i]) : "f"(v[i]), "f"(f[i]));     // (keeps subnormal sums)
-  if (!write || k >= a.K) return;
-  T* to = reinterpret_cast<T*>(a.h) + row * a.K + k;
-  if (k + 8 <= a.K && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
-    if constexpr (sizeof(T) == 4) {
-      reinterpret_cast<float4*>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      *reinterpret_cast<uint4*>(to) = make_uint4(Elem<T>::pack(v[0], v[1]), Elem<T>::pack(v[2], v[3]), Elem<T>::pack(v[4], v[5]), Elem<T>::pack(v[6], v[7]));
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-      if (k + i < a.K) to[i] = to_type<T>(v[i]);
-  }
+template <typename T, bool ALIGNED, int L>
+__device__ __forceinline__ void write_sum(const NormArgs& a, long long row, int k, const float (&v)[16], float* buf, int lane, unsigned mask) {
+  T* to = reinterpret_cast<T*>(a.h) + row * a.K;
+  if constexpr (ALIGNED) store16(to, k, a.K, v);
+  else store16_any<T, L>(to, k - lane * 16, a.K, v, buf, lane, mask);
 }
 
-template <typename T>
-__device__ __forceinline__ void norm8(const NormArgs& a, long long row, int k, float* v, float rstd) {
-  float w[8];
-  weights8<T>(a, k, w);
+template <typename T, int FMT, bool ALIGNED>
+__device__ __forceinline__ void write_norm(const NormArgs& a, long long row, int k, float (&v)[16], float rstd) {
+  float w[16];
+  weights16<T, ALIGNED>(a, k, w);
 #pragma unroll
-  for (int i = 0; i < 8; i++) v[i] = mul_exact(mul_exact(v[i], rstd), w[i]);
-  uint32_t out[2];
+  for (int i = 0; i < 16; i++) v[i] = mul_exact(mul_exact(v[i], rstd), w[i]);
+  uint32_t out[4];
   const int lane = threadIdx.x & 31;
-  const uint32_t word = quantize8(v, a.fmt, 0xffffu << (lane & 16), lane, out);
-  const int b = k / (a.fmt == FP8 ? 1 : 2);
-  if (b < a.row_bytes) {
-    uint8_t* to = a.data + row * a.row_bytes + b;
-    if (a.fmt == FP8) *reinterpret_cast<uint2*>(to) = make_uint2(out[0], out[1]);
-    else *reinterpret_cast<uint32_t*>(to) = out[0];
-  }
-  if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_word(row, k >> 7, a.pieces)) = word;
+  const uint32_t word = quantize16<FMT>(v, largest16(v), 0xffu << (lane & 24), lane, out);
+  store_codes<FMT>(a.data + row * a.row_bytes, k, a.row_bytes, out);
+  if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_word(row, k >> 7, a.pieces)) = word;
 }
 
 template <int G>
 __device__ __forceinline__ float row_sum(float s, float* red) {
-  s = warp_sum(s);
-  if (G == 32) return s;
+#pragma unroll
+  for (int o = (G < 32 ? G : 32) / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (G <= 32) return s;
   // the row's warps: their sums in one order, the same for every thread
   const int warp = threadIdx.x >> 5, first = (threadIdx.x / G) * (G / 32);
   if ((threadIdx.x & 31) == 0) red[warp] = s;
@@ -329,53 +360,89 @@ __device__ __forceinline__ float row_sum(float s, float* red) {
   return s;
 }
 
-// G threads of a block take a row, VPT vectors of eight columns each, which stay in registers between the two passes.  VPT = 0: rows
+// G threads of a block take a row, VPT vectors of sixteen columns each, which stay in registers between the two passes.  VPT = 0: rows
 // of any length, read a second time for their codes.
-template <typename T, int G, int VPT>
+template <typename T, int FMT, int G, int VPT, bool ALIGNED>
 __global__ void __launch_bounds__(G > kThreads ? G : kThreads) mx_norm_kernel(const NormArgs a) {
+  constexpr int THREADS = G > kThreads ? G : kThreads, L = G < 32 ? G : 32, W = 4 * Elem<T>::SZ;
   __shared__ float red[32];
+  __shared__ __align__(16) float bufs[ALIGNED ? 4 : THREADS * 16];
   pdl_trigger();
   pdl_wait();
-  const int t = threadIdx.x % G;
-  const int vecs = a.pieces * 16;                        // whole pieces: sixteen lanes work together
-  const int per = blockDim.x / G;
+  const int t = threadIdx.x % G, lane = threadIdx.x % L;
+  float* buf = bufs + (ALIGNED ? 0 : threadIdx.x / L * L * 16);
+  const unsigned mask = L == 32 ? 0xffffffffu : ((1u << L) - 1u) << (threadIdx.x & 31 & ~(L - 1));
+  const int vecs = a.pieces * 8;                         // whole pieces: eight lanes work together
+  const bool sum = a.r != nullptr;
+  constexpr int per = THREADS / G;
   for (long long first = (long long)blockIdx.x * per; first < a.rows; first += (long long)gridDim.x * per) {
     const long long row = first + threadIdx.x / G;
     const bool live = row < a.rows;
+    const T* x = reinterpret_cast<const T*>(a.x) + row * a.ldx;
+    const T* r = reinterpret_cast<const T*>(a.r) + row * a.ldr;
     float s = 0.f;
     if constexpr (VPT > 0) {
-      float v[VPT][8];
+      float v[VPT][16];
+      {
+        uint32_t wx[VPT][W], wr[VPT][W];
 #pragma unroll
-      for (int i = 0; i < VPT; i++)
-        if (live && t + i * G < vecs) {
-          sum8<T>(a, row, (t + i * G) * 8, true, v[i]);
-        } else {
+        for (int i = 0; i < VPT; i++) {
+          const int k = (t + i * G) * 16;
 #pragma unroll
-          for (int j = 0; j < 8; j++) v[i][j] = 0.f;
+          for (int j = 0; j < W; j++) wx[i][j] = wr[i][j] = 0;
+          if (live) {
+            load16<T, ALIGNED>(x, k, a.K, a.wide, a.ex, wx[i]);
+            if (sum) load16<T, ALIGNED>(r, k, a.K, a.wide, a.er, wr[i]);
+          }
         }
 #pragma unroll
-      for (int i = 0; i < VPT; i++)
+        for (int i = 0; i < VPT; i++) {
+          unpack16<T>(wx[i], v[i]);
+          if (sum) {
+            float f[16];
+            unpack16<T>(wr[i], f);
 #pragma unroll
-        for (int j = 0; j < 8; j++) s = fmaf(v[i][j], v[i][j], s);
+            for (int j = 0; j < 16; j++) v[i][j] = add_exact(v[i][j], f[j]);
+          }
+#pragma unroll
+          for (int j = 0; j < 16; j++) asm("fma.rn.f32 %0, %1, %1, %0;" : "+f"(s) : "f"(v[i][j]));
+        }
+      }
+      if (sum) {
+#pragma unroll
+        for (int i = 0; i < VPT; i++)
+          if (live) write_sum<T, ALIGNED, L>(a, row, (t + i * G) * 16, v[i], buf, lane, mask);
+      }
       const float rstd = inverse_root(row_sum<G>(s, red), a.K, a.eps);
 #pragma unroll
       for (int i = 0; i < VPT; i++)
-        if (live && t + i * G < vecs) norm8<T>(a, row, (t + i * G) * 8, v[i], rstd);
+        if (live && t + i * G < vecs) write_norm<T, FMT, ALIGNED>(a, row, (t + i * G) * 16, v[i], rstd);
     } else {
-      if (live)
-        for (int i = t; i < vecs; i += G) {
-          float v[8];
-          sum8<T>(a, row, i * 8, true, v);
+      // (the row's threads take each step together: their stores do)
+      auto take = [&](int k, float (&v)[16]) {
+        uint32_t u[W];
+        load16<T, ALIGNED>(x, k, a.K, a.wide, a.ex, u);
+        unpack16<T>(u, v);
+        if (!sum) return;
+        float f[16];
+        load16<T, ALIGNED>(r, k, a.K, a.wide, a.er, u);
+        unpack16<T>(u, f);
 #pragma unroll
-          for (int j = 0; j < 8; j++) s = fmaf(v[j], v[j], s);
-        }
+        for (int j = 0; j < 16; j++) v[j] = add_exact(v[j], f[j]);
+      };
+      for (int i = t; i - t < vecs; i += G) {
+        float v[16];
+        take(i * 16, v);
+        if (sum) write_sum<T, ALIGNED, L>(a, row, i * 16, v, buf, lane, mask);
+#pragma unroll
+        for (int j = 0; j < 16; j++) asm("fma.rn.f32 %0, %1, %1, %0;" : "+f"(s) : "f"(v[j]));
+      }
       const float rstd = inverse_root(row_sum<G>(s, red), a.K, a.eps);
-      if (live)
-        for (int i = t; i < vecs; i += G) {
-          float v[8];
-          sum8<T>(a, row, i * 8, false, v);
-          norm8<T>(a, row, i * 8, v, rstd);
-        }
+      for (int i = t; i < vecs; i += G) {
+        float v[16];
+        take(i * 16, v);
+        write_norm<T, FMT, ALIGNED>(a, row, i * 16, v, rstd);
+      }
     }
   }
 }
@@ -410,25 +477,33 @@ unsigned grid_of(long long units, int per_block, int blocks_per_sm) {
   return (unsigned)(g < 1 ? 1 : g < most ? g : most);
 }
 
-template <typename T>
+// Rows on 16-byte boundaries, whole vectors of eight; and of sixteen, on 32-byte boundaries.
+bool aligned_rows(const void* p, long long ld, long long K, int size) { return ((uintptr_t)p & 15) == 0 && ld * size % 16 == 0 && K % 8 == 0; }
+bool wide_rows(const void* p, long long ld, long long K, int size) { return ((uintptr_t)p & 31) == 0 && ld * size % 32 == 0 && K % 16 == 0; }
+
+template <typename T, int FMT, bool ALIGNED>
 int norm_launch(const NormArgs& a, cudaStream_t st) {
-  const int vecs = a.pieces * 16;
-  auto go = [&](auto kern, int G, int threads) {
-    const int per = threads / G;
-    const long long blocks = ((long long)a.rows + per - 1) / per, most = 148LL * (2048 / threads);
-    return gbh::launch(kern, dim3((unsigned)(blocks < most ? blocks : most)), dim3(threads), 0, st, 1, a);
+  const int vecs = a.pieces * 8;
+  cudaError_t e = cudaSuccess;
+  auto go = [&](auto kern, int G) {
+    const int threads = G > kThreads ? G : kThreads, per = threads / G;
+    const long long blocks = ((long long)a.rows + per - 1) / per, most = 148LL * 8;
+    e = gbh::launch(kern, dim3((unsigned)(blocks < most ? blocks : most)), dim3(threads), 0, st, 1, a);
   };
-  // few rows: a row's loads over as many threads as it has vectors
-  const bool few = a.rows <= 2 * 148;
-  cudaError_t e;
-  if (vecs <= 32) e = go(mx_norm_kernel<T, 32, 1>, 32, kThreads);
-  else if (vecs <= 64 && !few) e = go(mx_norm_kernel<T, 32, 2>, 32, kThreads);
-  else if (vecs <= 128 && !few) e = go(mx_norm_kernel<T, 32, 4>, 32, kThreads);
-  else if (vecs <= 256) e = go(mx_norm_kernel<T, 256, 1>, 256, 256);
-  else if (vecs <= 512) e = go(mx_norm_kernel<T, 256, 2>, 256, 256);
-  else if (vecs <= 1024) e = go(mx_norm_kernel<T, 256, 4>, 256, 256);
-  else if (vecs <= 4096) e = go(mx_norm_kernel<T, 1024, 4>, 1024, 1024);
-  else e = go(mx_norm_kernel<T, 1024, 0>, 1024, 1024);
+  if (a.rows <= 4 * 148 && vecs <= 512) {    // few rows: each over as many threads as it has vectors
+    if (vecs <= 32) go(mx_norm_kernel<T, FMT, 32, 1, ALIGNED>, 32);
+    else if (vecs <= 128) go(mx_norm_kernel<T, FMT, 128, 1, ALIGNED>, 128);
+    else go(mx_norm_kernel<T, FMT, 512, 1, ALIGNED>, 512);
+  } else if (vecs <= 16) go(mx_norm_kernel<T, FMT, 16, 1, ALIGNED>, 16);
+  else if (vecs <= 32) go(mx_norm_kernel<T, FMT, 16, 2, ALIGNED>, 16);
+  else if (vecs <= 48) go(mx_norm_kernel<T, FMT, 16, 3, ALIGNED>, 16);
+  else if (vecs <= 64) go(mx_norm_kernel<T, FMT, 32, 2, ALIGNED>, 32);
+  else if (vecs <= 96) go(mx_norm_kernel<T, FMT, 32, 3, ALIGNED>, 32);
+  else if (vecs <= 128) go(mx_norm_kernel<T, FMT, 64, 2, ALIGNED>, 64);
+  else if (vecs <= 256) go(mx_norm_kernel<T, FMT, 128, 2, ALIGNED>, 128);
+  else if (vecs <= 512) go(mx_norm_kernel<T, FMT, 256, 2, ALIGNED>, 256);
+  else if (vecs <= 1024) go(mx_norm_kernel<T, FMT, 512, 2, ALIGNED>, 512);
+  else go(mx_norm_kernel<T, FMT, 512, 0, ALIGNED>, 512);
   GB_CUDA_OK(e);
   return gbh::E_OK;
 }
@@ -436,6 +511,21 @@ int norm_launch(const NormArgs& a, cudaStream_t st) {
 }  // namespace
 
 enum { DT_BF16 = 0, DT_F16 = 1, DT_F32 = 2 };
+
+// CALL with the type T, the format FMT and ALIGNED.
+#define GB_MX_PICK(TYPE, fmt, aligned, CALL)                                          \
+  {                                                                                   \
+    using T = TYPE;                                                                   \
+    if (fmt == FP8) { constexpr int FMT = FP8; GB_MX_PICK_ALIGNED(aligned, CALL) }    \
+    else { constexpr int FMT = FP4; GB_MX_PICK_ALIGNED(aligned, CALL) }               \
+  }
+#define GB_MX_PICK_ALIGNED(aligned, CALL)                        \
+  if (aligned) { constexpr bool ALIGNED = true; CALL; }          \
+  else { constexpr bool ALIGNED = false; CALL; }
+#define GB_MX_DISPATCH(dtype, fmt, aligned, CALL)                        \
+  if (dtype == DT_BF16) GB_MX_PICK(__nv_bfloat16, fmt, aligned, CALL)    \
+  else if (dtype == DT_F16) GB_MX_PICK(__half, fmt, aligned, CALL)       \
+  else GB_MX_PICK(float, fmt, aligned, CALL)
 
 // Bytes of a row of codes and of the scales of a matrix (fmt 0: MXFP8, 1: MXFP4).
 GB_EXPORT long long gb_mx_row_bytes(long long K, int fmt) { return K <= 0 || K > (1LL << 30) ? 0 : row_bytes((int)K, fmt); }
@@ -453,18 +543,20 @@ GB_EXPORT int gb_mx_quantize(int dtype, int fmt, const void* x, long long ld, vo
   const int P = pieces((int)K, fmt), RB = row_bytes((int)K, fmt), size = dtype == DT_F32 ? 4 : 2;
   for (long long r0 = 0, n; r0 < rows; r0 += n) {
     n = rows_at_once(rows - r0, P);
-    QuantArgs a{(const uint8_t*)x + r0 * ld * size, (uint8_t*)data + r0 * RB, (uint8_t*)scales + r0 / 128 * P * 512, ld, (int)n, (int)K, P, RB, FastDiv((uint32_t)P),
-                extent_of(x, rows, ld, K, size)};
-    auto go = [&](auto kern) { return gbh::launch(kern, dim3(grid_of(n * P, kThreads / 16, 8)), dim3(kThreads), 0, (cudaStream_t)stream, 1, a); };
-    if (dtype == DT_BF16) GB_CUDA_OK(fmt == FP8 ? go(mx_quantize_kernel<__nv_bfloat16, FP8>) : go(mx_quantize_kernel<__nv_bfloat16, FP4>));
-    else if (dtype == DT_F16) GB_CUDA_OK(fmt == FP8 ? go(mx_quantize_kernel<__half, FP8>) : go(mx_quantize_kernel<__half, FP4>));
-    else GB_CUDA_OK(fmt == FP8 ? go(mx_quantize_kernel<float, FP8>) : go(mx_quantize_kernel<float, FP4>));
+    QuantArgs a{(const uint8_t*)x + r0 * ld * size, (uint8_t*)data + r0 * RB, (uint8_t*)scales + r0 / 128 * P * 512, ld, (int)n, (int)K, P, RB,
+                wide_rows(x, ld, K, size), FastDiv((uint32_t)P), extent_of(x, rows, ld, K, size)};
+    cudaError_t e = cudaSuccess;
+    auto go = [&](auto kern) { e = gbh::launch(kern, dim3(grid_of(n * P, kThreads / 8, 8)), dim3(kThreads), 0, (cudaStream_t)stream, 1, a); };
+    GB_MX_DISPATCH(dtype, fmt, aligned_rows(x, ld, K, size), go(mx_quantize_kernel<T, FMT, ALIGNED>))
+    GB_CUDA_OK(e);
   }
   return gbh::E_OK;
 }
 
-// Codes and scales (MXFP8) of x (rows x K, rows `ld` elements apart) along its columns, and of its transpose along the rows.
-GB_EXPORT int gb_mx_quantize_both(int dtype, const void* x, long long ld, void* data, void* scales, void* data_t, void* scales_t, long long rows, long long K, void* stream) {
+// Codes and scales (MXFP8) of x (rows x K, rows `ld` elements apart) along its columns, and of its transpose along the rows.  sums: null, or
+// fp32 scratch of (rows / 128, rounded up) x K, for the column sums of x in column_sums (of type sum_dtype).
+GB_EXPORT int gb_mx_quantize_both(int dtype, const void* x, long long ld, void* data, void* scales, void* data_t, void* scales_t, float* sums, void* column_sums,
+                                  int sum_dtype, long long rows, long long K, void* stream) {
   if (bad_shape("gb_mx_quantize_both", rows, K, ld, FP8, data, scales) || bad_shape("gb_mx_quantize_both", K, rows, ld, FP8, data_t, scales_t)) return gbh::E_BAD_ARG;
   const int P = pieces((int)K, FP8), PT = pieces((int)rows, FP8);
   const long long blocks = (long long)P * PT;
@@ -472,25 +564,42 @@ GB_EXPORT int gb_mx_quantize_both(int dtype, const void* x, long long ld, void* 
     gbh::set_error("gb_mx_quantize_both: %lld x %lld is too large", rows, K);
     return gbh::E_TOO_LARGE;
   }
-  auto go = [&](auto kern, int bytes, int size, std::atomic<uint32_t>& done) -> int {
+  const int size = dtype == DT_F32 ? 4 : 2;
+  const BothArgs a{x, (uint8_t*)data, (uint8_t*)scales, (uint8_t*)data_t, (uint8_t*)scales_t, ld, (int)rows, (int)K, P, row_bytes((int)K, FP8), PT,
+                   row_bytes((int)rows, FP8), wide_rows(x, ld, K, size), sums, extent_of(x, rows, ld, K, size)};
+  cudaStream_t st = (cudaStream_t)stream;
+  auto go = [&](auto kern, int bytes, std::atomic<uint32_t>& done) -> int {
     int dev = 0;
     GB_CUDA_OK(cudaGetDevice(&dev));
     if (dev >= 32 || !(done.load() >> dev & 1u)) {       // more shared memory than 48 KB: once per device
       GB_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
       if (dev < 32) done.fetch_or(1u << dev);
     }
-    BothArgs a{x, (uint8_t*)data, (uint8_t*)scales, (uint8_t*)data_t, (uint8_t*)scales_t, ld, (int)rows, (int)K, P, row_bytes((int)K, FP8), PT, row_bytes((int)rows, FP8),
-               extent_of(x, rows, ld, K, size)};
-    GB_CUDA_OK(gbh::launch(kern, dim3((unsigned)blocks), dim3(kThreads), bytes, (cudaStream_t)stream, 1, a));
+    GB_CUDA_OK(gbh::launch(kern, dim3((unsigned)blocks), dim3(kThreads), bytes, st, 1, a));
     return gbh::E_OK;
   };
-  static std::atomic<uint32_t> done[3];
+  static std::atomic<uint32_t> done[6];
+  const bool aligned = aligned_rows(x, ld, K, size);
+  int rc;
   switch (dtype) {
-    case DT_BF16: return go(mx_quantize_both_kernel<__nv_bfloat16>, BothCfg<__nv_bfloat16>::BYTES, 2, done[0]);
-    case DT_F16: return go(mx_quantize_both_kernel<__half>, BothCfg<__half>::BYTES, 2, done[1]);
-    case DT_F32: return go(mx_quantize_both_kernel<float>, BothCfg<float>::BYTES, 4, done[2]);
+    case DT_BF16: rc = aligned ? go(mx_quantize_both_kernel<__nv_bfloat16, true>, BothCfg<__nv_bfloat16>::BYTES, done[0])
+                               : go(mx_quantize_both_kernel<__nv_bfloat16, false>, BothCfg<__nv_bfloat16>::BYTES, done[1]); break;
+    case DT_F16: rc = aligned ? go(mx_quantize_both_kernel<__half, true>, BothCfg<__half>::BYTES, done[2])
+                              : go(mx_quantize_both_kernel<__half, false>, BothCfg<__half>::BYTES, done[3]); break;
+    case DT_F32: rc = aligned ? go(mx_quantize_both_kernel<float, true>, BothCfg<float>::BYTES, done[4])
+                              : go(mx_quantize_both_kernel<float, false>, BothCfg<float>::BYTES, done[5]); break;
     default: gbh::set_error("gb_mx_quantize_both: unsupported dtype %d", dtype); return gbh::E_BAD_ARG;
   }
+  if (rc || sums == nullptr) return rc;
+  const dim3 grid((unsigned)((K + 31) / 32));
+  if (sum_dtype == DT_BF16) GB_CUDA_OK(gbh::launch(mx_column_sum_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, 1, (const float*)sums, (__nv_bfloat16*)column_sums, PT, (int)K));
+  else if (sum_dtype == DT_F16) GB_CUDA_OK(gbh::launch(mx_column_sum_kernel<__half>, grid, dim3(256), 0, st, 1, (const float*)sums, (__half*)column_sums, PT, (int)K));
+  else if (sum_dtype == DT_F32) GB_CUDA_OK(gbh::launch(mx_column_sum_kernel<float>, grid, dim3(256), 0, st, 1, (const float*)sums, (float*)column_sums, PT, (int)K));
+  else {
+    gbh::set_error("gb_mx_quantize_both: unsupported dtype %d of the sums", sum_dtype);
+    return gbh::E_BAD_ARG;
+  }
+  return gbh::E_OK;
 }
 
 // The values (rows x K, contiguous) that codes and scales stand for.
@@ -504,10 +613,10 @@ GB_EXPORT int gb_mx_dequantize(int dtype, int fmt, const void* data, const void*
   for (long long r0 = 0, n; r0 < rows; r0 += n) {
     n = rows_at_once(rows - r0, P);
     DequantArgs a{(const uint8_t*)data + r0 * RB, (const uint8_t*)scales + r0 / 128 * P * 512, (uint8_t*)y + r0 * K * size, (int)n, (int)K, P, RB, FastDiv((uint32_t)P)};
-    auto go = [&](auto kern) { return gbh::launch(kern, dim3(grid_of(n * P, kThreads / 16, 8)), dim3(kThreads), 0, (cudaStream_t)stream, 1, a); };
-    if (dtype == DT_BF16) GB_CUDA_OK(fmt == FP8 ? go(mx_dequantize_kernel<__nv_bfloat16, FP8>) : go(mx_dequantize_kernel<__nv_bfloat16, FP4>));
-    else if (dtype == DT_F16) GB_CUDA_OK(fmt == FP8 ? go(mx_dequantize_kernel<__half, FP8>) : go(mx_dequantize_kernel<__half, FP4>));
-    else GB_CUDA_OK(fmt == FP8 ? go(mx_dequantize_kernel<float, FP8>) : go(mx_dequantize_kernel<float, FP4>));
+    cudaError_t e = cudaSuccess;
+    auto go = [&](auto kern) { e = gbh::launch(kern, dim3(grid_of(n * P, kThreads / 8, 8)), dim3(kThreads), 0, (cudaStream_t)stream, 1, a); };
+    GB_MX_DISPATCH(dtype, fmt, aligned_rows(y, K, K, size), go(mx_dequantize_kernel<T, FMT, ALIGNED>))
+    GB_CUDA_OK(e);
   }
   return gbh::E_OK;
 }
@@ -522,9 +631,11 @@ GB_EXPORT int gb_mx_add_rms_norm(int dtype, int fmt, const void* x, long long ld
     return gbh::E_BAD_ARG;
   }
   const int size = dtype == DT_F32 ? 4 : 2;
-  NormArgs a{x, r, w, h, (uint8_t*)data, (uint8_t*)scales, ldx, ldr, (int)rows, (int)K, pieces((int)K, fmt), row_bytes((int)K, fmt), w_f32 || dtype == DT_F32, fmt, eps,
-             extent_of(x, rows, ldx, K, size), extent_of(r, rows, ldr, K, size), extent_of(w, 1, K, K, w_f32 ? 4 : size)};
-  if (dtype == DT_BF16) return norm_launch<__nv_bfloat16>(a, (cudaStream_t)stream);
-  if (dtype == DT_F16) return norm_launch<__half>(a, (cudaStream_t)stream);
-  return norm_launch<float>(a, (cudaStream_t)stream);
+  const bool aligned = aligned_rows(x, ldx, K, size) && aligned_rows(w, K, K, 2) && (r == nullptr || (aligned_rows(r, ldr, K, size) && aligned_rows(h, K, K, size)));
+  const bool wide = wide_rows(x, ldx, K, size) && (r == nullptr || wide_rows(r, ldr, K, size));
+  const NormArgs a{x, r, w, h, (uint8_t*)data, (uint8_t*)scales, ldx, ldr, (int)rows, (int)K, pieces((int)K, fmt), row_bytes((int)K, fmt), w_f32, wide, eps,
+                   extent_of(x, rows, ldx, K, size), extent_of(r, rows, ldr, K, size), extent_of(w, 1, K, K, w_f32 ? 4 : size)};
+  int rc = gbh::E_OK;
+  GB_MX_DISPATCH(dtype, fmt, aligned, (rc = norm_launch<T, FMT, ALIGNED>(a, (cudaStream_t)stream)))
+  return rc;
 }

@@ -42,4 +42,10 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_addr) : "memory");
 }
 
+// The same where nothing in memory is handed over (TMEM columns that have been read, behind tcgen05.wait and a fence): a release to the
+// cluster waits until the thread's earlier stores to global memory have been performed, 2 000 clocks behind a tile's results.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_addr) : "memory");
+}
+
 }  // namespace gb

@@ -29,6 +29,15 @@ DT_BF16, DT_F16, DT_F32, DT_F64, DT_I8 = 0, 1, 2, 3, 4
 _DT = {torch.bfloat16: DT_BF16, torch.float16: DT_F16, torch.float32: DT_F32,
        torch.float64: DT_F64, torch.int8: DT_I8}
 
+# Argument types of entry points that are called with plain numbers and addresses (i int, L long long, f float, p pointer): a call of
+# seventeen arguments takes the host 1 us so, 3 us with an object for each of them.
+_ARGUMENTS = {
+    "gb_mx_quantize": "iipLppLLp", "gb_mx_quantize_both": "ipLppppppiLLp", "gb_mx_dequantize": "iipppLLp",
+    "gb_mx_add_rms_norm": "iipLpLpipppLLfp", "gb_mx_matmul": "ipppppLpiLLLiipLp", "gb_mx_linear": "iipLppppiLLLiipLp",
+    "gb_mx_train_forward": "iipLpLppiLLLiipLpLp", "gb_mx_train_backward": "ipLppipipiLLLpLp",
+    "gb_mx_plan": "LLLip", "gb_mx_linear_bytes": "LLLi", "gb_mx_train_bytes": "LLLiii",
+}
+
 _lib = None
 _lock = threading.Lock()
 launch_count = 0  # native entry points called through this binding
@@ -39,6 +48,7 @@ KERNELS_PER_CALL = {
     "gb_norm_bwd": 2, "gb_channel_sum": 2, "gb_ce_fwd": 2, "gb_ce_fused": 2, "gb_flash_bwd": 2, "gb_flash_bwd_ws": 2, "gb_embedding_bwd": 5,
     "gb_status_read": 0, "gb_comm_alloc": 0, "gb_comm_open": 0, "gb_comm_emulate": 0,
     "gb_comm_free": 0, "gb_reduce": 1, "gb_gemm_f32x3": 3, "gb_conv_wgrad": 2, "gb_conv_cl_fwd": 2, "gb_conv_cl_bwd": 4, "gb_stack_fwd": 0, "gb_set_words": 1, "gb_norm_bwd_res": 2, "gb_q_dynamic": 2,
+    "gb_mx_linear": 2, "gb_mx_train_forward": 3, "gb_mx_train_backward": 4,
 }
 
 
@@ -76,10 +86,13 @@ def lib() -> ctypes.CDLL:
             l.gb_last_error.restype = ctypes.c_char_p
             l.gb_gemm_f32x3_workspace.restype = c_longlong
             l.gb_gemm_f32x3_workspace.argtypes = [c_int, c_int, c_int, c_int]
-            for name in ("gb_conv_cl_fwd_ws", "gb_conv_cl_bwd_ws", "gb_conv_cl_part", "gb_block_ws", "gb_lstm_seq_bwd_words"):
+            for name in ("gb_conv_cl_fwd_ws", "gb_conv_cl_bwd_ws", "gb_conv_cl_part", "gb_block_ws", "gb_lstm_seq_bwd_words",
+                         "gb_mx_linear_bytes", "gb_mx_train_bytes"):
                 getattr(l, name).restype = c_longlong
             for name in ("gb_bench_matmul", "gb_bench_add", "gb_bench_flash_attn"):
                 getattr(l, name).restype = c_double
+            for name, kinds in _ARGUMENTS.items():
+                getattr(l, name).argtypes = [{"i": c_int, "L": c_longlong, "f": c_float, "p": c_void_p}[k] for k in kinds]
             _lib = l
     return _lib
 

@@ -15,6 +15,7 @@ this package; ``TrainLinearMX`` is differentiable.
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from typing import Optional, Tuple, Union
 
@@ -25,10 +26,11 @@ from ..nn.linear import Linear
 from ..nn.module import Module
 from ..nn.norm import RMSNorm
 from ..ops.gemm import ACT, _act_ref
+from ..ops.linear import emit_grad, emit_vector_grad
 
 MXBlock = 32
 _FMT = {"mxfp8": 0, "mxfp4": 1}
-_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+_TYPES = {torch.bfloat16: _l.DT_BF16, torch.float16: _l.DT_F16, torch.float32: _l.DT_F32}
 
 
 @dataclass
@@ -45,10 +47,7 @@ class QTensorMX:
     Shape: tuple
 
     def Numel(self) -> int:
-        n = 1
-        for s in self.Shape:
-            n *= s
-        return n
+        return math.prod(self.Shape)
 
     def ScaleCodes(self) -> torch.Tensor:
         """The scale codes as (rows, blocks)."""
@@ -74,34 +73,42 @@ def _pieces(K: int, fmt: int) -> int:
     return -(-K // 128) if fmt == 0 else 2 * -(-K // 256)
 
 
-def _empty(rows: int, shape: tuple, fmt: int, device) -> QTensorMX:
+def _empty(rows: int, shape: tuple, fmt: int, like: torch.Tensor) -> QTensorMX:
     K = shape[-1]
-    data = torch.empty((rows, _row_bytes(K, fmt)), dtype=torch.uint8, device=device)
-    scales = torch.empty(-(-rows // 128) * _pieces(K, fmt) * 512, dtype=torch.uint8, device=device)
+    data = like.new_empty((rows, _row_bytes(K, fmt)), dtype=torch.uint8)
+    scales = like.new_empty(-(-rows // 128) * _pieces(K, fmt) * 512, dtype=torch.uint8)
     return QTensorMX(data, scales, "mxfp4" if fmt else "mxfp8", shape)
 
 
 def _rows(t: torch.Tensor, what: str) -> torch.Tensor:
     """``t`` as a matrix of its last dimension: a view where its rows lie evenly spaced and its elements side by side."""
-    if t.dim() == 0 or t.shape[-1] == 0:
-        raise ValueError(f"{what}: a last dimension of at least one value is needed, got shape {tuple(t.shape)}")
-    if not t.is_floating_point():
+    shape = t.shape
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"{what}: a last dimension of at least one value is needed, got shape {tuple(shape)}")
+    if t.is_cuda:
+        if t.dtype not in _TYPES:
+            raise TypeError(f"{what}: no CUDA kernel for dtype {t.dtype}")
+    elif not t.is_floating_point():
         raise TypeError(f"{what}: a floating point tensor is needed, got {t.dtype}")
-    if t.is_cuda and t.dtype not in _TYPES:
-        raise TypeError(f"{what}: no CUDA kernel for dtype {t.dtype}")
-    t = t.detach()
-    if t.dim() != 2:
-        t = t.reshape(-1, t.shape[-1])
-    return t if t.stride(1) == 1 and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1) or t.shape[1] == 1 and t.stride(0) >= 1 else t.contiguous()
+    if len(shape) != 2:
+        t = t.reshape(-1, shape[-1])
+    s0, s1 = t.stride()
+    if (s1 != 1 and shape[-1] > 1) or (s0 < shape[-1] and t.shape[0] > 1):
+        t = t.contiguous()
+    return t if t.is_cuda else t.detach()
 
 
-def _call(device, name: str, *args) -> None:
-    """A native call on ``device``'s current stream, whichever device is the current one."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        _l.call(name, *args, _l.stream_ptr())
+def _call(device: int, name: str, *args) -> None:
+    """A native call on the current stream of a device, whichever is the current one."""
+    if device == _device():
+        _l.call(name, *args, _l.current_stream_handle())
     else:
         with torch.cuda.device(device):
-            _l.call(name, *args, _l.stream_ptr())
+            _l.call(name, *args, _l.current_stream_handle())
+
+
+def _device() -> int:
+    return _l._raw_device() if _l._raw_device is not None else torch.cuda.current_device()
 
 
 # ---------------------------------------------------------------------------------------
@@ -168,10 +175,9 @@ def QuantizeMX(t: torch.Tensor, format: str = "mxfp8") -> QTensorMX:
     if not x.is_cuda:
         return _quantize_ref(x, fmt, shape)
     rows, K = x.shape
-    q = _empty(rows, shape, fmt, x.device)
+    q = _empty(rows, shape, fmt, x)
     if rows:
-        _call(x.device, "gb_mx_quantize", _l.I(_l.dtype_code(x.dtype)), _l.I(fmt), _l.ptr(x), _l.L(x.stride(0)), _l.ptr(q.Data), _l.ptr(q.Scales),
-              _l.L(rows), _l.L(K))
+        _call(x.get_device(), "gb_mx_quantize", _TYPES[x.dtype], fmt, x.data_ptr(), x.stride(0), q.Data.data_ptr(), q.Scales.data_ptr(), rows, K)
     return q
 
 
@@ -185,25 +191,22 @@ def QuantizeMXPair(t: torch.Tensor) -> Tuple[QTensorMX, QTensorMX]:
         raise ValueError("QuantizeMXPair: at least one row is needed")
     if not x.is_cuda:
         return _quantize_ref(x, 0, shape), _quantize_ref(x.t(), 0, (K, rows))
-    q, qt = _empty(rows, shape, 0, x.device), _empty(K, (K, rows), 0, x.device)
-    _call(x.device, "gb_mx_quantize_both", _l.I(_l.dtype_code(x.dtype)), _l.ptr(x), _l.L(x.stride(0)), _l.ptr(q.Data), _l.ptr(q.Scales), _l.ptr(qt.Data),
-          _l.ptr(qt.Scales), _l.L(rows), _l.L(K))
+    q, qt = _empty(rows, shape, 0, x), _empty(K, (K, rows), 0, x)
+    _call(x.get_device(), "gb_mx_quantize_both", _TYPES[x.dtype], x.data_ptr(), x.stride(0), q.Data.data_ptr(), q.Scales.data_ptr(), qt.Data.data_ptr(),
+          qt.Scales.data_ptr(), None, None, 0, rows, K)
     return q, qt
 
 
 def _checked(q: QTensorMX, what: str) -> int:
     """The format's code, once codes and scales fit the shape."""
-    fmt = _format(q.Format)
-    if len(q.Shape) == 0 or q.Shape[-1] < 1:
-        raise ValueError(f"{what}: a quantised tensor of shape {tuple(q.Shape)}")
-    rows, K = 1, q.Shape[-1]
-    for s in q.Shape[:-1]:
-        rows *= s
-    d, s = q.Data, q.Scales
+    fmt, shape, d, s = _format(q.Format), q.Shape, q.Data, q.Scales
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"{what}: a quantised tensor of shape {tuple(shape)}")
+    rows, K = math.prod(shape[:-1]), shape[-1]
     if d.dtype != torch.uint8 or s.dtype != torch.uint8 or d.device != s.device:
         raise TypeError(f"{what}: codes and scales are uint8 tensors of one device")
-    if tuple(d.shape) != (rows, _row_bytes(K, fmt)) or s.numel() != -(-rows // 128) * _pieces(K, fmt) * 512:
-        raise ValueError(f"{what}: codes {tuple(d.shape)} and {s.numel()} scales do not belong to shape {tuple(q.Shape)} in {q.Format}")
+    if d.shape != (rows, _row_bytes(K, fmt)) or s.numel() != -(-rows // 128) * _pieces(K, fmt) * 512:
+        raise ValueError(f"{what}: codes {tuple(d.shape)} and {s.numel()} scales do not belong to shape {tuple(shape)} in {q.Format}")
     if not (d.is_contiguous() and s.is_contiguous()):
         raise ValueError(f"{what}: codes and scales must be contiguous")
     if d.is_cuda and (d.data_ptr() | s.data_ptr()) & 15:
@@ -212,16 +215,15 @@ def _checked(q: QTensorMX, what: str) -> int:
 
 
 def DequantizeMX(q: QTensorMX, dtype=torch.float32) -> torch.Tensor:
-    """The values that ``q`` stands for, rounded to ``dtype`` (exact in fp32, but for MXFP8 values below 2^-149)."""
+    """The values that ``q`` stands for, rounded to ``dtype`` (exact in fp32)."""
     fmt = _checked(q, "DequantizeMX")
     if not q.Data.is_cuda:
         return _values_ref(q).to(dtype).reshape(q.Shape)
     if dtype not in _TYPES:
         raise TypeError(f"DequantizeMX: no CUDA kernel for dtype {dtype}")
-    y = torch.empty(q.Shape, dtype=dtype, device=q.Data.device)
+    y = q.Data.new_empty(q.Shape, dtype=dtype)
     if y.numel():
-        _call(y.device, "gb_mx_dequantize", _l.I(_l.dtype_code(dtype)), _l.I(fmt), _l.ptr(q.Data), _l.ptr(q.Scales), _l.ptr(y), _l.L(q.Data.shape[0]),
-              _l.L(q.Shape[-1]))
+        _call(y.get_device(), "gb_mx_dequantize", _TYPES[dtype], fmt, q.Data.data_ptr(), q.Scales.data_ptr(), y.data_ptr(), q.Data.shape[0], q.Shape[-1])
     return y
 
 
@@ -235,10 +237,10 @@ def AddRMSNormMX(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
     rows, K = a.shape
     r = None
     if residual is not None:
-        if tuple(residual.shape) != shape or residual.dtype != x.dtype or residual.device != x.device:
+        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
             raise ValueError(f"AddRMSNormMX: the residual must be like x ({shape}, {x.dtype}, {x.device})")
         r = _rows(residual, "AddRMSNormMX")
-    if tuple(weight.shape) != (K,) or weight.device != x.device:
+    if weight.shape != (K,) or weight.device != x.device:
         raise ValueError(f"AddRMSNormMX: weight must have shape ({K},) on {x.device}")
     if weight.dtype not in (x.dtype, torch.float32):
         raise TypeError("AddRMSNormMX: weight dtype must equal the input dtype or be float32")
@@ -247,112 +249,161 @@ def AddRMSNormMX(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
         h = a.to(ct) if r is None else a.to(ct) + r.to(ct)
         y = h * torch.rsqrt(h.square().mean(-1, keepdim=True) + eps) * weight.detach().to(ct)
         return _quantize_ref(y, fmt, shape), (x if r is None else h.to(x.dtype).reshape(shape))
-    w = weight.detach().contiguous()
-    q = _empty(rows, shape, fmt, x.device)
-    h = None if r is None else torch.empty(shape, dtype=x.dtype, device=x.device)
+    w = weight if weight.is_contiguous() else weight.contiguous()
+    q = _empty(rows, shape, fmt, a)
+    h = None if r is None else a.new_empty(shape)
     if rows:
-        _call(x.device, "gb_mx_add_rms_norm", _l.I(_l.dtype_code(x.dtype)), _l.I(fmt), _l.ptr(a), _l.L(a.stride(0)), _l.ptr(r),
-              _l.L(K if r is None else r.stride(0)), _l.ptr(w), _l.I(int(w.dtype == torch.float32)), _l.ptr(h), _l.ptr(q.Data), _l.ptr(q.Scales),
-              _l.L(rows), _l.L(K), _l.F(eps))
+        _call(a.get_device(), "gb_mx_add_rms_norm", _TYPES[x.dtype], fmt, a.data_ptr(), a.stride(0), None if r is None else r.data_ptr(),
+              K if r is None else r.stride(0), w.data_ptr(), w.dtype == torch.float32, None if h is None else h.data_ptr(), q.Data.data_ptr(),
+              q.Scales.data_ptr(), rows, K, eps)
     return q, (x if h is None else h)
+
+
+def _epilogue(bias, N: int, device, dtype, act, what: str):
+    """(bias, its address, whether it is fp32, the activation's code) of a product in ``dtype``."""
+    code = ACT.get(act)
+    if code is None:
+        raise ValueError(f"{what}: unknown activation {act!r}")
+    if bias is None:
+        return None, None, False, code
+    if bias.shape != (N,) or bias.device != device:
+        raise ValueError(f"{what}: bias must have shape ({N},) on {device}")
+    if bias.is_cuda:
+        if bias.dtype != dtype and bias.dtype != torch.float32:
+            bias = bias.float()
+        bias = bias.contiguous()
+    return bias, bias.data_ptr(), bias.dtype == torch.float32, code
 
 
 def MatMulMX(a: QTensorMX, b: QTensorMX, bias: Optional[torch.Tensor] = None, dtype=torch.bfloat16, act: Optional[str] = None) -> torch.Tensor:
     """``act(A B^T + bias)`` in ``dtype`` (bf16, fp16 or fp32) for A (..., K) and B (N, K), both quantised along K in one format.
-    ``act``: relu, gelu or geluexact, as ``nn.Linear`` takes it."""
+    ``act``: relu, gelu or geluexact, as ``nn.Linear`` takes it.  No gradients."""
     fmt = _checked(a, "MatMulMX")
     if _checked(b, "MatMulMX") != fmt:
         raise ValueError(f"MatMulMX: both operands have one format, got {a.Format} and {b.Format}")
+    ad, bd = a.Data, b.Data
     if len(b.Shape) != 2 or a.Shape[-1] != b.Shape[-1]:
         raise ValueError(f"MatMulMX: shapes {tuple(a.Shape)} and {tuple(b.Shape)} do not match (..., K) and (N, K)")
-    if a.Data.device != b.Data.device:
-        raise ValueError(f"MatMulMX: operands on {a.Data.device} and {b.Data.device}")
-    if act not in ACT:
-        raise ValueError(f"MatMulMX: unknown activation {act!r}")
+    if ad.device != bd.device:
+        raise ValueError(f"MatMulMX: operands on {ad.device} and {bd.device}")
     N, K = b.Shape
-    M, dev = a.Data.shape[0], a.Data.device
-    if bias is not None:
-        if tuple(bias.shape) != (N,) or bias.device != dev:
-            raise ValueError(f"MatMulMX: bias must have shape ({N},) on {dev}")
-        bias = bias.detach()
+    M = ad.shape[0]
+    bias, bias_at, bias_f32, code = _epilogue(bias, N, ad.device, dtype, act, "MatMulMX")
     shape = (*a.Shape[:-1], N)
-    if not a.Data.is_cuda:
+    if not ad.is_cuda:
         y = _values_ref(a) @ _values_ref(b).t()
         if bias is not None:
-            y = y + bias.double()
+            y = y + bias.detach().double()
         return _act_ref(y, act).to(dtype).reshape(shape)
     if dtype not in _TYPES:
         raise TypeError(f"MatMulMX: no CUDA kernel for dtype {dtype}")
-    if bias is not None:
-        bias = (bias if bias.dtype in (dtype, torch.float32) else bias.float()).contiguous()
-    y = torch.empty(shape, dtype=dtype, device=dev)
-    if y.numel() == 0:
+    y = ad.new_empty(shape, dtype=dtype)
+    if M == 0 or N == 0:
         return y
-    need = _workspace(M, N, K, fmt)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call(dev, "gb_mx_matmul", _l.I(fmt), _l.ptr(a.Data), _l.ptr(a.Scales), _l.ptr(b.Data), _l.ptr(b.Scales), _l.ptr(y), _l.L(N), _l.ptr(bias),
-          _l.I(int(bias is not None and bias.dtype == torch.float32)), _l.L(M), _l.L(N), _l.L(K), _l.I(_l.dtype_code(dtype)), _l.I(ACT[act]), _l.ptr(ws),
-          _l.L(need))
-    return y
-
-
-def _workspace(M: int, N: int, K: int, fmt: int) -> int:
     out = (_l.L * 4)()
-    _l.check(_l.lib().gb_mx_plan(_l.L(M), _l.L(N), _l.L(K), _l.I(fmt), out), "gb_mx_plan")
-    return out[3]
+    _l.check(_l.lib().gb_mx_plan(M, N, K, fmt, out), "gb_mx_plan")
+    ws = ad.new_empty(out[3]) if out[3] else None
+    _call(ad.get_device(), "gb_mx_matmul", fmt, ad.data_ptr(), a.Scales.data_ptr(), bd.data_ptr(), b.Scales.data_ptr(), y.data_ptr(), N, bias_at, bias_f32,
+          M, N, K, _TYPES[dtype], code, None if ws is None else ws.data_ptr(), out[3])
+    return y
 
 
 def LinearMX(x: Union[torch.Tensor, QTensorMX], weight: QTensorMX, bias: Optional[torch.Tensor] = None, act: Optional[str] = None,
              dtype=None) -> torch.Tensor:
     """``act(Q(x) W^T + bias)`` with quantised weights (out, in).  ``x``: a tensor, quantised here in the weights' format, or what
-    ``AddRMSNormMX`` returned.  ``dtype``: of the result; x's own, or bf16 for a quantised x.  Evaluation only, no gradients."""
+    ``AddRMSNormMX`` returned.  ``dtype``: of the result; x's own, or bf16 for a quantised x.  No gradients."""
     if isinstance(x, QTensorMX):
         return MatMulMX(x, weight, bias, dtype or torch.bfloat16, act)
-    return MatMulMX(QuantizeMX(x, weight.Format), weight, bias, dtype or x.dtype, act)
+    if not x.is_cuda:
+        return MatMulMX(QuantizeMX(x, weight.Format), weight, bias, dtype or x.dtype, act)
+    fmt = _checked(weight, "LinearMX")
+    a = _rows(x, "LinearMX")
+    if len(weight.Shape) != 2 or a.shape[1] != weight.Shape[1]:
+        raise ValueError(f"LinearMX: shapes {tuple(x.shape)} and {tuple(weight.Shape)} do not match (..., K) and (N, K)")
+    wd = weight.Data
+    if a.device != wd.device:
+        raise ValueError(f"LinearMX: x on {a.device}, weights on {wd.device}")
+    dtype = dtype or x.dtype
+    if dtype not in _TYPES:
+        raise TypeError(f"LinearMX: no CUDA kernel for dtype {dtype}")
+    (M, K), N = a.shape, weight.Shape[0]
+    bias, bias_at, bias_f32, code = _epilogue(bias, N, a.device, dtype, act, "LinearMX")
+    y = wd.new_empty((*x.shape[:-1], N), dtype=dtype)
+    if M == 0 or N == 0:
+        return y
+    need = _l.lib().gb_mx_linear_bytes(M, N, K, fmt)
+    scratch = wd.new_empty(need)
+    _call(wd.get_device(), "gb_mx_linear", _TYPES[x.dtype], fmt, a.data_ptr(), a.stride(0), wd.data_ptr(), weight.Scales.data_ptr(), y.data_ptr(), bias_at,
+          bias_f32, M, N, K, _TYPES[dtype], code, scratch.data_ptr(), need)
+    return y
 
 
 class _TrainLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
-        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         N, K = weight.shape
-        ctx.xshape, ctx.params, ctx.xdtype = x.shape, (weight, bias), x.dtype
-        ctx.saved = ()
-        if x.numel() == 0:
-            ctx.empty = True
-            return x.new_empty((*x.shape[:-1], N))
-        ctx.empty = False
-        xq, xt = QuantizeMXPair(x) if need_w else (QuantizeMX(x), None)
-        wq, wt = QuantizeMXPair(weight) if need_x else (QuantizeMX(weight), None)
-        ctx.save_for_backward(*(t for q in (xt, wt) if q is not None for t in (q.Data, q.Scales)))
-        ctx.kept = (xt is not None, wt is not None)
-        return MatMulMX(xq, wq, bias, x.dtype)
+        need_x, need_w, _ = ctx.needs_input_grad
+        a, w = _rows(x, "TrainLinearMX"), _rows(weight, "TrainLinearMX")
+        M = a.shape[0]
+        ctx.meta = (x.shape, x.dtype, M, N, K, need_x, need_w)
+        ctx.params = (weight, bias)
+        y = x.new_empty((*x.shape[:-1], N))
+        if M == 0:
+            return y
+        if not x.is_cuda:
+            xq, xt = QuantizeMXPair(a)
+            wq, wt = QuantizeMXPair(w)
+            ctx.save_for_backward(xt.Data, xt.Scales, wt.Data, wt.Scales)
+            return MatMulMX(xq, wq, bias, x.dtype).view(y.shape)
+        sizes = _l.lib().gb_mx_train_bytes
+        kept = scratch = None
+        n_kept, n_scratch = sizes(M, N, K, need_x, need_w, 0), sizes(M, N, K, need_x, need_w, 1)
+        if n_kept:
+            kept = x.new_empty(n_kept, dtype=torch.uint8)
+        scratch = x.new_empty(n_scratch, dtype=torch.uint8)
+        _, bias_at, bias_f32, _ = keep = _epilogue(bias, N, x.device, x.dtype, None, "TrainLinearMX")
+        _call(x.get_device(), "gb_mx_train_forward", _TYPES[x.dtype], _TYPES[weight.dtype], a.data_ptr(), a.stride(0), w.data_ptr(), w.stride(0), y.data_ptr(),
+              bias_at, bias_f32, M, N, K, need_x, need_w, None if kept is None else kept.data_ptr(), n_kept, scratch.data_ptr(), n_scratch)
+        del keep
+        ctx.save_for_backward(kept)
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        from ..ops.linear import emit_grad, emit_vector_grad
+        xshape, xdtype, M, N, K, need_x, need_w = ctx.meta
         weight, bias = ctx.params
-        N, K = weight.shape
+        need_b = bias is not None and ctx.needs_input_grad[2]
         dx = dw = db = None
-        if ctx.empty:
-            z = torch.zeros
-            dx = z(ctx.xshape, dtype=ctx.xdtype, device=dy.device) if ctx.needs_input_grad[0] else None
-            dw = emit_grad(weight, torch.zeros_like(weight)) if ctx.needs_input_grad[1] else None
-            db = emit_grad(bias, torch.zeros_like(bias)) if bias is not None and ctx.needs_input_grad[2] else None
-            return dx, dw, db
-        saved = list(ctx.saved_tensors)
-        rows = dy.numel() // N
-        xt = QTensorMX(saved.pop(0), saved.pop(0), "mxfp8", (K, rows)) if ctx.kept[0] else None
-        wt = QTensorMX(saved.pop(0), saved.pop(0), "mxfp8", (K, N)) if ctx.kept[1] else None
+        if M == 0:
+            return (dy.new_zeros(xshape, dtype=xdtype) if need_x else None, emit_grad(weight, torch.zeros_like(weight)) if need_w else None,
+                    emit_grad(bias, torch.zeros_like(bias)) if need_b else None)
         g = _rows(dy, "TrainLinearMX")
-        gq, gt = QuantizeMXPair(g) if xt is not None else (QuantizeMX(g) if wt is not None else None, None)
-        if wt is not None:
-            dx = MatMulMX(gq, wt, None, ctx.xdtype).reshape(ctx.xshape)
-        if xt is not None:
-            dw = emit_grad(weight, MatMulMX(gt, xt, None, weight.dtype))
-        if bias is not None and ctx.needs_input_grad[2]:
-            db = emit_vector_grad(bias, g)
+        if not dy.is_cuda:
+            xt, xs, wt, ws = ctx.saved_tensors
+            gq, gt = QuantizeMXPair(g)
+            if need_x:
+                dx = MatMulMX(gq, QTensorMX(wt, ws, "mxfp8", (K, N)), None, xdtype).reshape(xshape)
+            if need_w:
+                dw = MatMulMX(gt, QTensorMX(xt, xs, "mxfp8", (K, M)), None, weight.dtype)
+        elif need_x or need_w:
+            (kept,) = ctx.saved_tensors
+            n_scratch = _l.lib().gb_mx_train_bytes(M, N, K, need_x, need_w, 2)
+            scratch = dy.new_empty(n_scratch, dtype=torch.uint8)
+            if need_x:
+                dx = dy.new_empty(xshape, dtype=xdtype)
+            if need_w:
+                dw = torch.empty_like(weight, memory_format=torch.contiguous_format)
+                if need_b and bias.dtype in _TYPES:
+                    db = torch.empty_like(bias)
+            _call(dy.get_device(), "gb_mx_train_backward", _TYPES[dy.dtype], g.data_ptr(), g.stride(0), kept.data_ptr(), None if dx is None else dx.data_ptr(),
+                  _TYPES[xdtype], None if dw is None else dw.data_ptr(), _TYPES[weight.dtype], None if db is None else db.data_ptr(),
+                  0 if db is None else _TYPES[db.dtype], M, N, K, scratch.data_ptr(), n_scratch)
+        # gradients go to their sinks last: a sink may start a step that rewrites the parameters
+        if need_b:
+            db = emit_vector_grad(bias, g) if db is None else emit_grad(bias, db)
+        if dw is not None:
+            dw = emit_grad(weight, dw)
         return dx, dw, db
 
 
@@ -364,6 +415,10 @@ def TrainLinearMX(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
         raise ValueError(f"TrainLinearMX: shapes {tuple(x.shape)} and {tuple(weight.shape)} do not match (..., K) and (N, K)")
     if weight.device != x.device:
         raise ValueError(f"TrainLinearMX: x on {x.device}, weight on {weight.device}")
+    if weight.shape[0] == 0:
+        raise ValueError("TrainLinearMX: a layer needs outputs")
+    if bias is not None and (bias.shape != weight.shape[:1] or bias.device != x.device):
+        raise ValueError(f"TrainLinearMX: bias must have shape ({weight.shape[0]},) on {x.device}")
     return _TrainLinear.apply(x, weight, bias)
 
 
