@@ -186,20 +186,34 @@ __device__ __forceinline__ void unpack16(const uint32_t (&w)[4 * Elem<T>::SZ], f
   Elem<T>::unpack(w + 2 * Elem<T>::SZ, v + 8);
 }
 
-// Sixteen values to consecutive elements on a 16-byte boundary, of which those from K on are left out (whole vectors of eight).
+// Sixteen values to consecutive elements on a 16-byte boundary (wide: 32), of which those from K on are left out (whole vectors of eight).  A
+// store of 32 bytes fills a sector; two of 16 write it twice: bf16 values of 50304 x 2048 in MXFP4 57 us so, FIGURES.
+__device__ __forceinline__ void store8(void* to, bool wide, const uint32_t* w) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(to)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(to)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
 template <typename T>
-__device__ __forceinline__ void store16(T* row, int k, int K, const float* v) {
+__device__ __forceinline__ void store16(T* row, int k, int K, bool wide, const float (&v)[16]) {
+  if (k >= K) return;
+  uint32_t w[4 * Elem<T>::SZ];
 #pragma unroll
-  for (int h = 0; h < 2; h++) {
-    if (k + 8 * h >= K) break;
-    uint4* to = reinterpret_cast<uint4*>(row + k + 8 * h);
-    const float* f = v + 8 * h;
-    if constexpr (sizeof(T) == 4) {
-      to[0] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-      to[1] = make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7]));
-    } else {
-      to[0] = make_uint4(Elem<T>::pack(f[0], f[1]), Elem<T>::pack(f[2], f[3]), Elem<T>::pack(f[4], f[5]), Elem<T>::pack(f[6], f[7]));
-    }
+  for (int i = 0; i < 4 * Elem<T>::SZ; i++) {
+    if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(v[i]);
+    else w[i] = Elem<T>::pack(v[2 * i], v[2 * i + 1]);
+  }
+  uint32_t* to = reinterpret_cast<uint32_t*>(row + k);
+  if constexpr (sizeof(T) == 4) {
+    store8(to, wide, w);
+    if (k + 8 < K) store8(to + 8, wide, w + 8);
+  } else if (k + 8 < K) {
+    store8(to, wide, w);
+  } else {
+    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 template <typename T>

@@ -14,6 +14,7 @@
 
 #include <atomic>
 #include <string.h>
+#include <type_traits>
 
 using namespace gb;
 using namespace gbmx;
@@ -403,11 +404,46 @@ __device__ __forceinline__ void load_bulk(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-template <int FMT, int BN>
+// Rows of x that the kernel quantises itself.
+struct RowsArgs {
+  const void* x;
+  long long ld;
+  int K;
+  Extent ext;
+};
+
+// Codes and scales of one step's columns of the rows of x, from a warp into a stage's shared memory, in the order of the swizzle.
+template <int FMT, typename X>
+__device__ __forceinline__ void stage_rows(const RowsArgs& x, int rows, int step, uint8_t* codes, uint8_t* scales) {
+  constexpr int L = FMT == FP8 ? 8 : 16;                     // lanes of a row
+  const int lane = threadIdx.x & 31, l = lane % L, k = (step * L + l) * 16;
+  for (int r0 = 0; r0 < rows; r0 += 32 / L) {
+    const int r = r0 + lane / L;
+    uint32_t w[4 * Elem<X>::SZ];
+#pragma unroll
+    for (int j = 0; j < 4 * Elem<X>::SZ; j++) w[j] = 0;
+    if (r < rows) load16<X, false>(reinterpret_cast<const X*>(x.x) + r * x.ld, k, x.K, false, x.ext, w);
+    float v[16];
+    unpack16<X>(w, v);
+    uint32_t c[4];
+    const uint32_t word = quantize16<FMT>(v, largest16<X>(w), 0xffu << (lane & 24), lane, c);
+    if (r >= rows) continue;
+    uint8_t* row = codes + r * 128;
+    if (FMT == FP8) *reinterpret_cast<uint4*>(row + ((l ^ (r & 7)) << 4)) = make_uint4(c[0], c[1], c[2], c[3]);
+    else *reinterpret_cast<uint2*>(row + ((l >> 1 ^ (r & 7)) << 4) + (l & 1) * 8) = make_uint2(c[0], c[1]);
+    if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(scales + (l >> 3) * 512 + r * 16) = word;
+  }
+}
+
+// X: void, or the type of rows that come as they are (16 at most): the warps that wait for the results quantise them, each its steps, into the
+// ring.  Every CTA does so for its part of K, which costs less than a launch of their own: one token through 8192 -> 2048 in MXFP4, us, FIGURES.
+template <int FMT, int BN, typename X>
 __global__ void __launch_bounds__(ClusterCfg<FMT, BN>::THREADS, 2)
 mx_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const uint8_t* __restrict__ sA, const uint8_t* __restrict__ sB,
-                  const MxArgs args) {
+                  const RowsArgs x, const MxArgs args) {
   // "A" of the instruction: the product's B (columns of C); its "B": the product's A (rows of C)
+  constexpr bool ROWS = !std::is_same<X, void>::value;
+  static_assert(!ROWS || BN == 16, "rows as they are: sixteen at most");
   using C = ClusterCfg<FMT, BN>;
   using F = Fmt<FMT>;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -425,12 +461,12 @@ mx_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
   const int c0 = (tile % args.num_n) * 128, r0 = (tile / args.num_n) * BN;       // columns and rows of C
   const int k0 = rank * args.steps_per, k1 = min(args.steps, k0 + args.steps_per);
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::STAGES; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < C::STAGES; s++) { mbar_init(&full[s], ROWS ? 2 : 1); mbar_init(&empty[s], 1); }
     mbar_init(done, 1);
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tmA);
-    tma_prefetch_desc(&tmB);
+    if (!ROWS) tma_prefetch_desc(&tmB);
   }
   if (warp == 1) {
     tmem_alloc(slot, C::TMEM);
@@ -451,11 +487,13 @@ mx_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         if (!ok) break;
         uint8_t* sa = smem + stage * C::TILE_BYTES;
         uint8_t* ss = smem + C::OFF_SCALES + stage * C::S_BYTES;
-        mbar_expect_tx(&full[stage], C::TILE_BYTES + C::S_BYTES);
+        mbar_expect_tx(&full[stage], ROWS ? C::A_BYTES + C::S_BYTES / 2 : C::TILE_BYTES + C::S_BYTES);
         tma_load_3d(sa, &tmA, &full[stage], k * 128, c0, 0);
-        tma_load_3d(sa + C::A_BYTES, &tmB, &full[stage], k * 128, r0, 0);
         load_bulk(ss, sA + ((long long)(c0 >> 7) * args.steps + k) * (F::PIECES * C::PIECE), F::PIECES * C::PIECE, &full[stage]);
-        load_bulk(ss + F::PIECES * C::PIECE, sB + ((long long)(r0 >> 7) * args.steps + k) * (F::PIECES * C::PIECE), F::PIECES * C::PIECE, &full[stage]);
+        if (!ROWS) {
+          tma_load_3d(sa + C::A_BYTES, &tmB, &full[stage], k * 128, r0, 0);
+          load_bulk(ss + F::PIECES * C::PIECE, sB + ((long long)(r0 >> 7) * args.steps + k) * (F::PIECES * C::PIECE), F::PIECES * C::PIECE, &full[stage]);
+        }
       }
       if (!ok) {   // a bounded time for the copies in flight
         const uint64_t t0 = globaltimer_ns();
@@ -484,6 +522,16 @@ mx_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
     }
     __syncwarp();
   } else {
+    if constexpr (ROWS) {
+      for (int k = k0 + warp - 2, i = warp - 2; k < k1; k += 4, i += 4) {
+        const int stage = i % C::STAGES;
+        if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], ((i / C::STAGES) & 1) ^ 1, abort_flag, args.status, ST_GEMM_TIMEOUT, 45))) break;
+        stage_rows<FMT, X>(x, args.M, k, smem + stage * C::TILE_BYTES + C::A_BYTES, smem + C::OFF_SCALES + stage * C::S_BYTES + F::PIECES * C::PIECE);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[stage]);
+      }
+    }
     // the accumulator into the ring, transposed (every load has been consumed by then): rows of C of 128 fp32 columns
     const bool ok = mbar_wait(done, 0, abort_flag, args.status, ST_GEMM_TIMEOUT, 44);
     const int q = warp & 3, half = (warp - 2) >> 2;          // (of 320 threads: two warps for 32 lanes, 16 columns in turn)
@@ -607,33 +655,39 @@ double cluster_us(long long M, int bn, long long tiles, int steps, int splits) {
          (splits > 1 ? 0.9 + 0.05 * splits + 0.0075 * splits * rows * (ctas > 64 ? ctas / 64 : 1.0) : 0.0);
 }
 
+struct Choice {
+  int splits;
+  double us;
+};
+Choice best_clusters(long long M, int bn, long long tiles, int steps) {
+  Choice c{0, 1e30};
+  for (int s = 1; s <= 8; s *= 2) {
+    if (g_splits ? s != (g_splits < 8 ? g_splits : 8) : (s > 1 && (s > steps || tiles * s > 296))) continue;
+    const double us = cluster_us(M, bn, tiles, steps, s);
+    if (us < c.us) c = {s, us};
+  }
+  if (c.splits == 0) c.splits = 1;       // (slices were asked for that there are not)
+  return c;
+}
+Choice best_pairs(long long M, long long N, long long tiles, int steps) {
+  Choice c{1, pair_us(M, N, tiles, steps, 1)};
+  for (int s = 2; s <= 8 && s <= steps && N % 4 == 0 && tiles < 74; s++)
+    if (g_splits ? s == g_splits : pair_us(M, N, tiles, steps, s) < c.us) c = {s, pair_us(M, N, tiles, steps, s)};
+  return c;
+}
+
+// Up to 64 rows run as clusters, without a workspace (pairs were the faster ones at none of the sizes above).
 Plan plan_of(long long M, long long N, long long K, int fmt) {
   Plan p{};
   p.steps = (int)((K + (fmt == FP8 ? 127 : 255)) / (fmt == FP8 ? 128 : 256));
-  const int bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-  const long long pair_tiles = ((M + 255) / 256) * ((N + 255) / 256), tiles = ((M + bn - 1) / bn) * ((N + 127) / 128);
-  double best = 1e30;
-  if (g_kind != 2) {
-    const int least = g_splits ? g_splits : 1, most = g_splits ? g_splits : pair_tiles < 74 ? 8 : 1;
-    for (int s = least; s <= most && (s == 1 || (s <= p.steps && N % 4 == 0)); s++) {
-      const double us = pair_us(M, N, pair_tiles, p.steps, s);
-      if (us < best) { best = us; p.pair = 1; p.splits = s; }
-    }
-  }
-  if (g_kind != 1) {
-    for (int s = 1; s <= 8; s *= 2) {
-      if (g_splits ? s != (g_splits < 8 ? g_splits : 8) : (s > 1 && (s > p.steps || tiles * s > 296))) continue;
-      const double us = cluster_us(M, bn, tiles, p.steps, s);
-      if (us < best) { best = us; p.pair = 0; p.splits = s; }
-    }
-  }
-  if (p.splits == 0) {         // (asked for slices that this product cannot have)
-    p.pair = g_kind != 2;
-    p.splits = 1;
-  }
-  p.bn = p.pair ? 256 : bn;
+  p.bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  const Choice pairs = best_pairs(M, N, ((M + 255) / 256) * ((N + 255) / 256), p.steps);
+  const Choice clusters = best_clusters(M, p.bn, ((M + p.bn - 1) / p.bn) * ((N + 127) / 128), p.steps);
+  p.pair = g_kind ? g_kind == 1 : M > 64 && pairs.us < clusters.us;
+  p.splits = p.pair ? pairs.splits : clusters.splits;
   p.steps_per = (p.steps + p.splits - 1) / p.splits;
   if (p.pair) {
+    p.bn = 256;
     p.splits = (p.steps + p.steps_per - 1) / p.steps_per;      // no empty slice
     p.workspace = p.splits > 1 ? M * N * 4 * p.splits : 0;
   }
@@ -677,13 +731,13 @@ int launch_pair(const Maps& tm, const MxArgs& args, cudaStream_t st) {
   GB_CUDA_OK(gbh::launch(mx_pair_kernel<FMT>, dim3(2 * pairs), dim3(C::THREADS), C::BYTES, st, 2, tm.a, tm.b, tm.sa, tm.sb, args));
   return gbh::E_OK;
 }
-template <int FMT, int BN>
-int launch_cluster(const Maps& tm, const void* sa, const void* sb, const MxArgs& args, cudaStream_t st) {
+template <int FMT, int BN, typename X = void>
+int launch_cluster(const Maps& tm, const void* sa, const void* sb, const MxArgs& args, cudaStream_t st, const RowsArgs& x = RowsArgs{}) {
   using C = ClusterCfg<FMT, BN>;
   static std::atomic<uint32_t> done{0};
-  if (int rc = allow_shared(mx_cluster_kernel<FMT, BN>, C::BYTES, done)) return rc;
-  GB_CUDA_OK(gbh::launch(mx_cluster_kernel<FMT, BN>, dim3(args.num_m * args.num_n * args.splits), dim3(C::THREADS), C::BYTES, st, args.splits, tm.a, tm.b,
-                         (const uint8_t*)sa, (const uint8_t*)sb, args));
+  if (int rc = allow_shared(mx_cluster_kernel<FMT, BN, X>, C::BYTES, done)) return rc;
+  GB_CUDA_OK(gbh::launch(mx_cluster_kernel<FMT, BN, X>, dim3(args.num_m * args.num_n * args.splits), dim3(C::THREADS), C::BYTES, st, args.splits, tm.a, tm.b,
+                         (const uint8_t*)sa, (const uint8_t*)sb, x, args));
   return gbh::E_OK;
 }
 
@@ -774,4 +828,33 @@ GB_EXPORT int gb_mx_matmul(int fmt, const void* a, const void* sa, const void* b
     case 64: return fmt == FP8 ? launch_cluster<FP8, 64>(tm, sb, sa, args, st) : launch_cluster<FP4, 64>(tm, sb, sa, args, st);
     default: return fmt == FP8 ? launch_cluster<FP8, 128>(tm, sb, sa, args, st) : launch_cluster<FP4, 128>(tm, sb, sa, args, st);
   }
+}
+
+// The same for up to 16 rows of x as they are (bf16, fp16 or fp32, K elements, ld apart), quantised within the product's kernel.
+GB_EXPORT int gb_mx_matmul_rows(int dtype, int fmt, const void* x, long long ld, const void* b, const void* sb, void* c, long long ldc, const void* bias, int bias_f32,
+                                long long M, long long N, long long K, int out, int act, void* stream) {
+  long long p4[4];
+  if (int rc = gb_mx_plan(M, N, K, fmt, p4)) return rc;
+  if (M > 16 || dtype < 0 || dtype > 2 || out < 0 || out > 2 || act < 0 || act > 3 || ldc < N || ld < 0) {
+    gbh::set_error("gb_mx_matmul_rows: %lld rows (16 at most), types %d and %d, activation %d, row pitches %lld and %lld", M, dtype, out, act, ld, ldc);
+    return gbh::E_BAD_ARG;
+  }
+  MxArgs args{};
+  args.M = (int)M; args.N = (int)N;
+  args.steps = (int)((K + (fmt == FP8 ? 127 : 255)) / (fmt == FP8 ? 128 : 256));
+  args.num_m = 1;
+  args.num_n = (int)((N + 127) / 128);
+  args.splits = best_clusters(M, 16, args.num_n, args.steps).splits;
+  args.steps_per = (args.steps + args.splits - 1) / args.splits;
+  args.C = c; args.ldc = ldc; args.bias = bias; args.bias_f32 = bias_f32 || out == OUT_F32; args.act = act; args.out = out;
+  args.status = gbh::status_ptr();
+  const int size = dtype == 2 ? 4 : 2;
+  RowsArgs rows{x, ld, (int)K, {reinterpret_cast<uintptr_t>(x), reinterpret_cast<uintptr_t>(x) + (uintptr_t)(((M - 1) * ld + K) * size)}};
+  Maps tm;
+  memset(&tm, 0, sizeof(tm));
+  if (int rc = map_codes(&tm.a, b, N, row_bytes((int)K, fmt), 128)) return rc;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == 0) return fmt == FP8 ? launch_cluster<FP8, 16, __nv_bfloat16>(tm, sb, nullptr, args, st, rows) : launch_cluster<FP4, 16, __nv_bfloat16>(tm, sb, nullptr, args, st, rows);
+  if (dtype == 1) return fmt == FP8 ? launch_cluster<FP8, 16, __half>(tm, sb, nullptr, args, st, rows) : launch_cluster<FP4, 16, __half>(tm, sb, nullptr, args, st, rows);
+  return fmt == FP8 ? launch_cluster<FP8, 16, float>(tm, sb, nullptr, args, st, rows) : launch_cluster<FP4, 16, float>(tm, sb, nullptr, args, st, rows);
 }

@@ -10,8 +10,12 @@ GB_EXPORT int gb_mx_quantize_both(int dtype, const void* x, long long ld, void* 
 GB_EXPORT int gb_mx_plan(long long M, long long N, long long K, int fmt, long long* out4);
 GB_EXPORT int gb_mx_matmul(int fmt, const void* a, const void* sa, const void* b, const void* sb, void* c, long long ldc, const void* bias, int bias_f32, long long M,
                            long long N, long long K, int out, int act, void* workspace, long long workspace_bytes, void* stream);
+GB_EXPORT int gb_mx_matmul_rows(int dtype, int fmt, const void* x, long long ld, const void* b, const void* sb, void* c, long long ldc, const void* bias, int bias_f32,
+                                long long M, long long N, long long K, int out, int act, void* stream);
 
 namespace {
+
+constexpr int kFew = 16;         // rows that the product's kernel quantises itself
 
 long long up256(long long n) { return (n + 255) & ~255LL; }
 bool fits(long long rows, long long K) { return rows > 0 && K > 0 && rows <= 0x7fffffffLL && K <= (1LL << 30); }
@@ -49,8 +53,9 @@ long long backward_bytes(long long M, long long N, long long K) {
   return packed_bytes(M, N, FP8) + packed_bytes(N, M, FP8) + up256((M + 127) / 128 * N * 4) + max2(workspace_of(M, K, N, FP8), workspace_of(N, K, M, FP8));
 }
 
+// need: bytes of scratch, 0 where the extents are bad.
 bool bad(const char* what, long long M, long long N, long long K, const void* scratch, long long have, long long need) {
-  if (!fits(M, K) || !fits(N, K) || !fits(M, N) || !fits(N, M) || !fits(K, M)) {
+  if (need <= 0) {
     gbh::set_error("%s: bad extents %lld x %lld x %lld", what, M, N, K);
     return true;
   }
@@ -63,14 +68,15 @@ bool bad(const char* what, long long M, long long N, long long K, const void* sc
 
 }  // namespace
 
-// Scratch bytes of gb_mx_linear, 0 for bad extents.
+// Scratch bytes of gb_mx_linear, 0 for none (16 rows at most) and for bad extents.
 GB_EXPORT long long gb_mx_linear_bytes(long long M, long long N, long long K, int fmt) {
-  return fits(M, K) && fits(N, K) ? packed_bytes(M, K, fmt) + workspace_of(M, N, K, fmt) : 0;
+  return M > kFew && fits(M, K) && fits(N, K) ? packed_bytes(M, K, fmt) + workspace_of(M, N, K, fmt) : 0;
 }
 
 // y (M x N, of x's type or `out`) = act(Q(x) W^T + bias): x M x K, rows `ld` apart; W quantised (N, K).
 GB_EXPORT int gb_mx_linear(int dtype, int fmt, const void* x, long long ld, const void* w, const void* sw, void* y, const void* bias, int bias_f32, long long M, long long N,
                            long long K, int out, int act, void* scratch, long long scratch_bytes, void* stream) {
+  if (M <= kFew) return gb_mx_matmul_rows(dtype, fmt, x, ld, w, sw, y, N, bias, bias_f32, M, N, K, out, act, stream);
   if (bad("gb_mx_linear", M, N, K, scratch, scratch_bytes, gb_mx_linear_bytes(M, N, K, fmt))) return gbh::E_BAD_ARG;
   Carver c{(uint8_t*)scratch};
   const Packed q = c.packed(M, K, fmt);

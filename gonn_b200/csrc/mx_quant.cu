@@ -212,7 +212,7 @@ struct DequantArgs {
   const uint8_t* data;
   const uint8_t* scales;
   void* y;                 // rows x K, contiguous
-  int rows, K, pieces, row_bytes;
+  int rows, K, pieces, row_bytes, wide;
   FastDiv by_pieces;
 };
 
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(kThreads) mx_dequantize_kernel(const DequantAr
 #pragma unroll
       for (int j = 0; j < 16; j++) v[j] = mul_exact(v[j], scale);
       T* to = reinterpret_cast<T*>(a.y) + (long long)row[i] * a.K;
-      if constexpr (ALIGNED) store16(to, g[i] * 128 + l8 * 16, a.K, v);
+      if constexpr (ALIGNED) store16(to, g[i] * 128 + l8 * 16, a.K, a.wide, v);
       else store16_any<T, 8>(to, g[i] * 128, a.K, v, bufs + (threadIdx.x >> 3) * 128, l8, 0xffu << (lane & 24));
     }
   }
@@ -287,27 +287,49 @@ struct NormArgs {
   uint8_t* scales;
   long long ldx, ldr;
   int rows, K, pieces, row_bytes, w_f32, wide;
-  float eps;
+  double eps, inv_K;
   Extent ex, er, ew;
 };
 
+// fp32 arithmetic that keeps subnormal numbers.
 __device__ __forceinline__ float add_exact(float a, float b) {
   float d;
   asm("add.rn.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
+__device__ __forceinline__ float fma_exact(float a, float b, float c) {
+  float d;
+  asm("fma.rn.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
-// 1 / sqrt(sum / K + eps) to its last bit or nearly so (the approximation, corrected by its residual: a row's values would otherwise move
-// over the borders between codes more often than the roundings of their two products move them).
-__device__ __forceinline__ float inverse_root(float sum, int K, float eps) {
-  const float v = add_exact(__fdiv_rn(sum, (float)K), eps);
-  float r;
-  asm("rsqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
-  if (v > 1e-30f && v < 1e30f) {
-    const float t = v * r, e = fmaf(-t, r, 1.f) - fmaf(v, r, -t) * r;      // 1 - v r^2
-    r = fmaf(0.5f * r, e, r);
-  }
-  return r;
+// 1 / sqrt(sum / K + eps) in two parts: the approximation and a step of Newton's iteration in fp64.
+struct Root {
+  float hi, lo;
+};
+__device__ __forceinline__ Root inverse_root(double sum, double inv_K, double eps) {
+  const double v = fma(sum, inv_K, eps);
+  float r0;
+  asm("rsqrt.approx.f32 %0, %1;" : "=f"(r0) : "f"((float)v));
+  if (!(v > 1e-36 && v < 1e36)) return {r0, 0.f};
+  const double r = fma(0.5 * (double)r0, fma(-v * (double)r0, (double)r0, 1.0), (double)r0);
+  const float hi = (float)r;
+  return {hi, (float)(r - (double)hi)};
+}
+
+// h (hi + lo) * root * w, rounded to odd: the last bit stands for all that lies behind it, so that the rounding to a code afterwards is that of
+// the product itself.  (A value next to the border between two codes falls on the side where it belongs: with three roundings of fp32 one in
+// a million fell on the other, a step of the code away.)
+template <bool LO>
+__device__ __forceinline__ float normalized(float h, float lo, const Root& root, float w) {
+  const float p = mul_exact(h, root.hi);
+  float e = fma_exact(h, root.lo, fma_exact(h, root.hi, -p));
+  if (LO) e = fma_exact(lo, root.hi, e);
+  const float ew = mul_exact(e, w);
+  float z;
+  asm("fma.rz.f32 %0, %1, %2, %3;" : "=f"(z) : "f"(p), "f"(w), "f"(ew));
+  const float left = add_exact(fma_exact(p, w, -z), ew);
+  return left != 0.f ? __uint_as_float(__float_as_uint(z) | 1u) : z;
 }
 
 // A row's weights stand still while rows come and go: vectors from L1.
@@ -324,19 +346,30 @@ __device__ __forceinline__ void weights16(const NormArgs& a, int k, float (&f)[1
   }
 }
 
+// The sum of two values and, of fp32 ones, what its rounding leaves out (sums of 16-bit values are exact but for far magnitudes).
+template <typename T>
+__device__ __forceinline__ void sum_of(float& h, float& lo, float x, float r) {
+  h = add_exact(x, r);
+  if constexpr (sizeof(T) == 4) {
+    const float b = add_exact(h, -x);
+    lo = add_exact(add_exact(x, -add_exact(h, -b)), add_exact(r, -b));
+    if (!(fabsf(h) < 3e38f)) lo = 0.f;
+  }
+}
+
 template <typename T, bool ALIGNED, int L>
 __device__ __forceinline__ void write_sum(const NormArgs& a, long long row, int k, const float (&v)[16], float* buf, int lane, unsigned mask) {
   T* to = reinterpret_cast<T*>(a.h) + row * a.K;
-  if constexpr (ALIGNED) store16(to, k, a.K, v);
+  if constexpr (ALIGNED) store16(to, k, a.K, a.wide, v);
   else store16_any<T, L>(to, k - lane * 16, a.K, v, buf, lane, mask);
 }
 
 template <typename T, int FMT, bool ALIGNED>
-__device__ __forceinline__ void write_norm(const NormArgs& a, long long row, int k, float (&v)[16], float rstd) {
+__device__ __forceinline__ void write_norm(const NormArgs& a, long long row, int k, float (&v)[16], const float (&lo)[16], const Root& root) {
   float w[16];
   weights16<T, ALIGNED>(a, k, w);
 #pragma unroll
-  for (int i = 0; i < 16; i++) v[i] = mul_exact(mul_exact(v[i], rstd), w[i]);
+  for (int i = 0; i < 16; i++) v[i] = normalized<sizeof(T) == 4>(v[i], lo[i], root, w[i]);
   uint32_t out[4];
   const int lane = threadIdx.x & 31;
   const uint32_t word = quantize16<FMT>(v, largest16(v), 0xffu << (lane & 24), lane, out);
@@ -344,8 +377,19 @@ __device__ __forceinline__ void write_norm(const NormArgs& a, long long row, int
   if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_word(row, k >> 7, a.pieces)) = word;
 }
 
+// The squares of sixteen values: two chains of eight in fp32, which an fp64 sum takes up.
+__device__ __forceinline__ double squares(const float (&v)[16]) {
+  float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+  for (int j = 0; j < 16; j += 2) {
+    s0 = fma_exact(v[j], v[j], s0);
+    s1 = fma_exact(v[j + 1], v[j + 1], s1);
+  }
+  return (double)s0 + (double)s1;
+}
+
 template <int G>
-__device__ __forceinline__ float row_sum(float s, float* red) {
+__device__ __forceinline__ double row_sum(double s, double* red) {
 #pragma unroll
   for (int o = (G < 32 ? G : 32) / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (G <= 32) return s;
@@ -353,7 +397,7 @@ __device__ __forceinline__ float row_sum(float s, float* red) {
   const int warp = threadIdx.x >> 5, first = (threadIdx.x / G) * (G / 32);
   if ((threadIdx.x & 31) == 0) red[warp] = s;
   __syncthreads();
-  s = 0.f;
+  s = 0.0;
 #pragma unroll
   for (int i = 0; i < G / 32; i++) s += red[first + i];
   __syncthreads();
@@ -364,8 +408,8 @@ __device__ __forceinline__ float row_sum(float s, float* red) {
 // of any length, read a second time for their codes.
 template <typename T, int FMT, int G, int VPT, bool ALIGNED>
 __global__ void __launch_bounds__(G > kThreads ? G : kThreads) mx_norm_kernel(const NormArgs a) {
-  constexpr int THREADS = G > kThreads ? G : kThreads, L = G < 32 ? G : 32, W = 4 * Elem<T>::SZ;
-  __shared__ float red[32];
+  constexpr int THREADS = G > kThreads ? G : kThreads, L = G < 32 ? G : 32, W = 4 * Elem<T>::SZ, F32 = sizeof(T) == 4;
+  __shared__ double red[32];
   __shared__ __align__(16) float bufs[ALIGNED ? 4 : THREADS * 16];
   pdl_trigger();
   pdl_wait();
@@ -380,9 +424,9 @@ __global__ void __launch_bounds__(G > kThreads ? G : kThreads) mx_norm_kernel(co
     const bool live = row < a.rows;
     const T* x = reinterpret_cast<const T*>(a.x) + row * a.ldx;
     const T* r = reinterpret_cast<const T*>(a.r) + row * a.ldr;
-    float s = 0.f;
+    double s = 0.0;
     if constexpr (VPT > 0) {
-      float v[VPT][16];
+      float v[VPT][16], lo[F32 ? VPT : 1][16];
       {
         uint32_t wx[VPT][W], wr[VPT][W];
 #pragma unroll
@@ -397,15 +441,12 @@ __global__ void __launch_bounds__(G > kThreads ? G : kThreads) mx_norm_kernel(co
         }
 #pragma unroll
         for (int i = 0; i < VPT; i++) {
+          float f[16];
           unpack16<T>(wx[i], v[i]);
-          if (sum) {
-            float f[16];
-            unpack16<T>(wr[i], f);
+          unpack16<T>(wr[i], f);                         // (zeros without a residual)
 #pragma unroll
-            for (int j = 0; j < 16; j++) v[i][j] = add_exact(v[i][j], f[j]);
-          }
-#pragma unroll
-          for (int j = 0; j < 16; j++) asm("fma.rn.f32 %0, %1, %1, %0;" : "+f"(s) : "f"(v[i][j]));
+          for (int j = 0; j < 16; j++) sum_of<T>(v[i][j], lo[F32 ? i : 0][j], v[i][j], f[j]);
+          s += squares(v[i]);
         }
       }
       if (sum) {
@@ -413,35 +454,35 @@ __global__ void __launch_bounds__(G > kThreads ? G : kThreads) mx_norm_kernel(co
         for (int i = 0; i < VPT; i++)
           if (live) write_sum<T, ALIGNED, L>(a, row, (t + i * G) * 16, v[i], buf, lane, mask);
       }
-      const float rstd = inverse_root(row_sum<G>(s, red), a.K, a.eps);
+      const Root root = inverse_root(row_sum<G>(s, red), a.inv_K, a.eps);
 #pragma unroll
       for (int i = 0; i < VPT; i++)
-        if (live && t + i * G < vecs) write_norm<T, FMT, ALIGNED>(a, row, (t + i * G) * 16, v[i], rstd);
+        if (live && t + i * G < vecs) write_norm<T, FMT, ALIGNED>(a, row, (t + i * G) * 16, v[i], lo[F32 ? i : 0], root);
     } else {
-      // (the row's threads take each step together: their stores do)
-      auto take = [&](int k, float (&v)[16]) {
+      auto take = [&](int k, float (&v)[16], float (&lo)[16]) {
         uint32_t u[W];
+        float f[16];
         load16<T, ALIGNED>(x, k, a.K, a.wide, a.ex, u);
         unpack16<T>(u, v);
-        if (!sum) return;
-        float f[16];
-        load16<T, ALIGNED>(r, k, a.K, a.wide, a.er, u);
+#pragma unroll
+        for (int j = 0; j < W; j++) u[j] = 0;
+        if (sum) load16<T, ALIGNED>(r, k, a.K, a.wide, a.er, u);
         unpack16<T>(u, f);
 #pragma unroll
-        for (int j = 0; j < 16; j++) v[j] = add_exact(v[j], f[j]);
+        for (int j = 0; j < 16; j++) sum_of<T>(v[j], lo[j], v[j], f[j]);
       };
+      // (a row's threads take each step together, as their stores of the sum do)
       for (int i = t; i - t < vecs; i += G) {
-        float v[16];
-        take(i * 16, v);
+        float v[16], lo[16];
+        take(i * 16, v, lo);
         if (sum) write_sum<T, ALIGNED, L>(a, row, i * 16, v, buf, lane, mask);
-#pragma unroll
-        for (int j = 0; j < 16; j++) asm("fma.rn.f32 %0, %1, %1, %0;" : "+f"(s) : "f"(v[j]));
+        s += squares(v);
       }
-      const float rstd = inverse_root(row_sum<G>(s, red), a.K, a.eps);
+      const Root root = inverse_root(row_sum<G>(s, red), a.inv_K, a.eps);
       for (int i = t; i < vecs; i += G) {
-        float v[16];
-        take(i * 16, v);
-        write_norm<T, FMT, ALIGNED>(a, row, i * 16, v, rstd);
+        float v[16], lo[16];
+        take(i * 16, v, lo);
+        write_norm<T, FMT, ALIGNED>(a, row, i * 16, v, lo, root);
       }
     }
   }
@@ -612,7 +653,7 @@ GB_EXPORT int gb_mx_dequantize(int dtype, int fmt, const void* data, const void*
   const int P = pieces((int)K, fmt), RB = row_bytes((int)K, fmt), size = dtype == DT_F32 ? 4 : 2;
   for (long long r0 = 0, n; r0 < rows; r0 += n) {
     n = rows_at_once(rows - r0, P);
-    DequantArgs a{(const uint8_t*)data + r0 * RB, (const uint8_t*)scales + r0 / 128 * P * 512, (uint8_t*)y + r0 * K * size, (int)n, (int)K, P, RB, FastDiv((uint32_t)P)};
+    DequantArgs a{(const uint8_t*)data + r0 * RB, (const uint8_t*)scales + r0 / 128 * P * 512, (uint8_t*)y + r0 * K * size, (int)n, (int)K, P, RB, wide_rows(y, K, K, size), FastDiv((uint32_t)P)};
     cudaError_t e = cudaSuccess;
     auto go = [&](auto kern) { e = gbh::launch(kern, dim3(grid_of(n * P, kThreads / 8, 8)), dim3(kThreads), 0, (cudaStream_t)stream, 1, a); };
     GB_MX_DISPATCH(dtype, fmt, aligned_rows(y, K, K, size), go(mx_dequantize_kernel<T, FMT, ALIGNED>))
@@ -621,10 +662,10 @@ GB_EXPORT int gb_mx_dequantize(int dtype, int fmt, const void* data, const void*
   return gbh::E_OK;
 }
 
-// h = x + r (r null: h is x, and is not written), codes and scales of h / sqrt(mean(h^2) + eps) * w.  x, r: rows ldx / ldr
+// h = x + r (r null: h is x, and is not written), codes and scales of (x + r) / sqrt(mean((x + r)^2) + eps) * w.  x, r: rows ldx / ldr
 // elements apart; w in x's type, or fp32 (w_f32); h contiguous.
 GB_EXPORT int gb_mx_add_rms_norm(int dtype, int fmt, const void* x, long long ldx, const void* r, long long ldr, const void* w, int w_f32, void* h, void* data,
-                                 void* scales, long long rows, long long K, float eps, void* stream) {
+                                 void* scales, long long rows, long long K, double eps, void* stream) {
   if (bad_shape("gb_mx_add_rms_norm", rows, K, ldx < ldr ? ldx : ldr, fmt, data, scales)) return gbh::E_BAD_ARG;
   if (dtype != DT_BF16 && dtype != DT_F16 && dtype != DT_F32) {
     gbh::set_error("gb_mx_add_rms_norm: unsupported dtype %d", dtype);
@@ -632,8 +673,8 @@ GB_EXPORT int gb_mx_add_rms_norm(int dtype, int fmt, const void* x, long long ld
   }
   const int size = dtype == DT_F32 ? 4 : 2;
   const bool aligned = aligned_rows(x, ldx, K, size) && aligned_rows(w, K, K, 2) && (r == nullptr || (aligned_rows(r, ldr, K, size) && aligned_rows(h, K, K, size)));
-  const bool wide = wide_rows(x, ldx, K, size) && (r == nullptr || wide_rows(r, ldr, K, size));
-  const NormArgs a{x, r, w, h, (uint8_t*)data, (uint8_t*)scales, ldx, ldr, (int)rows, (int)K, pieces((int)K, fmt), row_bytes((int)K, fmt), w_f32, wide, eps,
+  const bool wide = wide_rows(x, ldx, K, size) && (r == nullptr || (wide_rows(r, ldr, K, size) && wide_rows(h, K, K, size)));
+  const NormArgs a{x, r, w, h, (uint8_t*)data, (uint8_t*)scales, ldx, ldr, (int)rows, (int)K, pieces((int)K, fmt), row_bytes((int)K, fmt), w_f32, wide, eps, 1.0 / (double)K,
                    extent_of(x, rows, ldx, K, size), extent_of(r, rows, ldr, K, size), extent_of(w, 1, K, K, w_f32 ? 4 : size)};
   int rc = gbh::E_OK;
   GB_MX_DISPATCH(dtype, fmt, aligned, (rc = norm_launch<T, FMT, ALIGNED>(a, (cudaStream_t)stream)))

@@ -29,11 +29,11 @@ DT_BF16, DT_F16, DT_F32, DT_F64, DT_I8 = 0, 1, 2, 3, 4
 _DT = {torch.bfloat16: DT_BF16, torch.float16: DT_F16, torch.float32: DT_F32,
        torch.float64: DT_F64, torch.int8: DT_I8}
 
-# Argument types of entry points that are called with plain numbers and addresses (i int, L long long, f float, p pointer): a call of
+# Argument types of entry points that are called with plain numbers and addresses (i int, L long long, d double, p pointer): a call of
 # seventeen arguments takes the host 1 us so, 3 us with an object for each of them.
 _ARGUMENTS = {
     "gb_mx_quantize": "iipLppLLp", "gb_mx_quantize_both": "ipLppppppiLLp", "gb_mx_dequantize": "iipppLLp",
-    "gb_mx_add_rms_norm": "iipLpLpipppLLfp", "gb_mx_matmul": "ipppppLpiLLLiipLp", "gb_mx_linear": "iipLppppiLLLiipLp",
+    "gb_mx_add_rms_norm": "iipLpLpipppLLdp", "gb_mx_matmul": "ipppppLpiLLLiipLp", "gb_mx_linear": "iipLppppiLLLiipLp",
     "gb_mx_train_forward": "iipLpLppiLLLiipLpLp", "gb_mx_train_backward": "ipLppipipiLLLpLp",
     "gb_mx_plan": "LLLip", "gb_mx_linear_bytes": "LLLi", "gb_mx_train_bytes": "LLLiii",
 }
@@ -92,7 +92,7 @@ def lib() -> ctypes.CDLL:
             for name in ("gb_bench_matmul", "gb_bench_add", "gb_bench_flash_attn"):
                 getattr(l, name).restype = c_double
             for name, kinds in _ARGUMENTS.items():
-                getattr(l, name).argtypes = [{"i": c_int, "L": c_longlong, "f": c_float, "p": c_void_p}[k] for k in kinds]
+                getattr(l, name).argtypes = [{"i": c_int, "L": c_longlong, "d": c_double, "p": c_void_p}[k] for k in kinds]
             _lib = l
     return _lib
 

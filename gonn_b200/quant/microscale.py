@@ -16,7 +16,6 @@ this package; ``TrainLinearMX`` is differentiable.
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass
 from typing import Optional, Tuple, Union
 
 import torch
@@ -29,11 +28,12 @@ from ..ops.gemm import ACT, _act_ref
 from ..ops.linear import emit_grad, emit_vector_grad
 
 MXBlock = 32
+_FEW = 64                # rows up to which a product needs no workspace (gb_mx_plan)
 _FMT = {"mxfp8": 0, "mxfp4": 1}
+_NAMES = ("mxfp8", "mxfp4")
 _TYPES = {torch.bfloat16: _l.DT_BF16, torch.float16: _l.DT_F16, torch.float32: _l.DT_F32}
 
 
-@dataclass
 class QTensorMX:
     """Codes and scales of a tensor of ``Shape``, quantised along its last dimension.
 
@@ -41,10 +41,37 @@ class QTensorMX:
     128 rows by four blocks, the order in which the tensor core takes them: the pieces of 128 rows behind one another, row
     r of a piece at byte 16 (r % 32) + 4 (r // 32).  MXFP4 has an even number of pieces in a row of pieces.  Scales behind the
     last block of a row are zeros; those of rows behind the last one are never read into a result."""
-    Data: torch.Tensor
-    Scales: torch.Tensor
-    Format: str
-    Shape: tuple
+
+    __slots__ = ("_format", "_shape", "_data", "_scales", "_whole", "_rows")
+
+    def __init__(self, Data: torch.Tensor, Scales: torch.Tensor, Format: str, Shape: tuple):
+        self._format, self._shape = Format, tuple(Shape)
+        self._data, self._scales, self._whole, self._rows = Data, Scales, None, None
+
+    Format = property(lambda self: self._format)
+    Shape = property(lambda self: self._shape)
+
+    @classmethod
+    def _of(cls, whole: torch.Tensor, rows: int, fmt: int, shape: tuple) -> "QTensorMX":
+        """Codes and scales in one allocation, which the operators address as it is; ``Data`` and ``Scales`` become views of it when they are
+        asked for (two allocations and their checks are 5 of the 15 us that the host takes for a product)."""
+        q = cls(None, None, _NAMES[fmt], shape)
+        q._whole, q._rows = whole, rows
+        return q
+
+    def _views(self):
+        w, rows = self._whole, self._rows
+        if w is not None:
+            per = _row_bytes(self._shape[-1], _FMT[self._format])
+            self._data, self._scales = w[:rows * per].view(rows, per), w[_up16(rows * per):]
+            self._whole = None
+        return self._data, self._scales
+
+    Data = property(lambda self: self._views()[0])
+    Scales = property(lambda self: self._views()[1])
+
+    def __repr__(self) -> str:
+        return f"QTensorMX({self.Format}, {tuple(self.Shape)})"
 
     def Numel(self) -> int:
         return math.prod(self.Shape)
@@ -73,11 +100,17 @@ def _pieces(K: int, fmt: int) -> int:
     return -(-K // 128) if fmt == 0 else 2 * -(-K // 256)
 
 
-def _empty(rows: int, shape: tuple, fmt: int, like: torch.Tensor) -> QTensorMX:
+def _up16(n: int) -> int:
+    return (n + 15) & ~15
+
+
+def _empty(rows: int, shape: tuple, fmt: int, like: torch.Tensor):
+    """(an unwritten quantised tensor, the addresses of its codes and scales)."""
     K = shape[-1]
-    data = like.new_empty((rows, _row_bytes(K, fmt)), dtype=torch.uint8)
-    scales = like.new_empty(-(-rows // 128) * _pieces(K, fmt) * 512, dtype=torch.uint8)
-    return QTensorMX(data, scales, "mxfp4" if fmt else "mxfp8", shape)
+    n = _up16(rows * _row_bytes(K, fmt))
+    whole = like.new_empty(n + -(-rows // 128) * _pieces(K, fmt) * 512, dtype=torch.uint8)
+    at = whole.data_ptr()
+    return QTensorMX._of(whole, rows, fmt, shape), at, at + n
 
 
 def _rows(t: torch.Tensor, what: str) -> torch.Tensor:
@@ -175,9 +208,9 @@ def QuantizeMX(t: torch.Tensor, format: str = "mxfp8") -> QTensorMX:
     if not x.is_cuda:
         return _quantize_ref(x, fmt, shape)
     rows, K = x.shape
-    q = _empty(rows, shape, fmt, x)
+    q, codes, scales = _empty(rows, shape, fmt, x)
     if rows:
-        _call(x.get_device(), "gb_mx_quantize", _TYPES[x.dtype], fmt, x.data_ptr(), x.stride(0), q.Data.data_ptr(), q.Scales.data_ptr(), rows, K)
+        _call(x.get_device(), "gb_mx_quantize", _TYPES[x.dtype], fmt, x.data_ptr(), x.stride(0), codes, scales, rows, K)
     return q
 
 
@@ -191,47 +224,52 @@ def QuantizeMXPair(t: torch.Tensor) -> Tuple[QTensorMX, QTensorMX]:
         raise ValueError("QuantizeMXPair: at least one row is needed")
     if not x.is_cuda:
         return _quantize_ref(x, 0, shape), _quantize_ref(x.t(), 0, (K, rows))
-    q, qt = _empty(rows, shape, 0, x), _empty(K, (K, rows), 0, x)
-    _call(x.get_device(), "gb_mx_quantize_both", _TYPES[x.dtype], x.data_ptr(), x.stride(0), q.Data.data_ptr(), q.Scales.data_ptr(), qt.Data.data_ptr(),
-          qt.Scales.data_ptr(), None, None, 0, rows, K)
+    (q, codes, scales), (qt, codes_t, scales_t) = _empty(rows, shape, 0, x), _empty(K, (K, rows), 0, x)
+    _call(x.get_device(), "gb_mx_quantize_both", _TYPES[x.dtype], x.data_ptr(), x.stride(0), codes, scales, codes_t, scales_t, None, None, 0, rows, K)
     return q, qt
 
 
-def _checked(q: QTensorMX, what: str) -> int:
-    """The format's code, once codes and scales fit the shape."""
-    fmt, shape, d, s = _format(q.Format), q.Shape, q.Data, q.Scales
+def _checked(q: QTensorMX, what: str):
+    """(format's code, rows, K, a tensor of the device, address of the codes, of the scales), once codes and scales fit the shape."""
+    whole = q._whole
+    if whole is not None:
+        fmt, rows, K = _FMT[q._format], q._rows, q._shape[-1]
+        at = whole.data_ptr()
+        return fmt, rows, K, whole, at, at + _up16(rows * _row_bytes(K, fmt))
+    fmt, shape, d, s = _format(q._format), q._shape, q._data, q._scales
     if not shape or shape[-1] < 1:
         raise ValueError(f"{what}: a quantised tensor of shape {tuple(shape)}")
     rows, K = math.prod(shape[:-1]), shape[-1]
-    if d.dtype != torch.uint8 or s.dtype != torch.uint8 or d.device != s.device:
+    if d.dtype != torch.uint8 or s.dtype != torch.uint8 or d.get_device() != s.get_device():
         raise TypeError(f"{what}: codes and scales are uint8 tensors of one device")
     if d.shape != (rows, _row_bytes(K, fmt)) or s.numel() != -(-rows // 128) * _pieces(K, fmt) * 512:
         raise ValueError(f"{what}: codes {tuple(d.shape)} and {s.numel()} scales do not belong to shape {tuple(shape)} in {q.Format}")
     if not (d.is_contiguous() and s.is_contiguous()):
         raise ValueError(f"{what}: codes and scales must be contiguous")
-    if d.is_cuda and (d.data_ptr() | s.data_ptr()) & 15:
+    codes, scales = d.data_ptr(), s.data_ptr()
+    if d.is_cuda and (codes | scales) & 15:
         raise ValueError(f"{what}: codes and scales must be 16-byte aligned")
-    return fmt
+    return fmt, rows, K, d, codes, scales
 
 
 def DequantizeMX(q: QTensorMX, dtype=torch.float32) -> torch.Tensor:
     """The values that ``q`` stands for, rounded to ``dtype`` (exact in fp32)."""
-    fmt = _checked(q, "DequantizeMX")
-    if not q.Data.is_cuda:
+    fmt, rows, K, like, codes, scales = _checked(q, "DequantizeMX")
+    if not like.is_cuda:
         return _values_ref(q).to(dtype).reshape(q.Shape)
     if dtype not in _TYPES:
         raise TypeError(f"DequantizeMX: no CUDA kernel for dtype {dtype}")
-    y = q.Data.new_empty(q.Shape, dtype=dtype)
-    if y.numel():
-        _call(y.get_device(), "gb_mx_dequantize", _TYPES[dtype], fmt, q.Data.data_ptr(), q.Scales.data_ptr(), y.data_ptr(), q.Data.shape[0], q.Shape[-1])
+    y = like.new_empty(q.Shape, dtype=dtype)
+    if rows:
+        _call(like.get_device(), "gb_mx_dequantize", _TYPES[dtype], fmt, codes, scales, y.data_ptr(), rows, K)
     return y
 
 
 def AddRMSNormMX(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-6,
                  format: str = "mxfp8") -> Tuple[QTensorMX, torch.Tensor]:
     """``h = x + residual`` and the quantised ``h / sqrt(mean(h^2) + eps) * weight``: what a pre-norm block hands to its next
-    products, and the stream that goes on beside them.  Returns (codes and scales, h); the norm takes the sum in fp32, before it is
-    rounded to h's type.  Without a residual h is x itself."""
+    products, and the stream that goes on beside them.  Returns (codes and scales, h); the norm takes the sum before it is rounded to
+    h's type, and no rounding of its own moves a value to another code.  Without a residual h is x itself."""
     fmt, shape = _format(format), tuple(x.shape)
     a = _rows(x, "AddRMSNormMX")
     rows, K = a.shape
@@ -245,17 +283,15 @@ def AddRMSNormMX(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
     if weight.dtype not in (x.dtype, torch.float32):
         raise TypeError("AddRMSNormMX: weight dtype must equal the input dtype or be float32")
     if not x.is_cuda:
-        ct = torch.float64 if x.dtype == torch.float64 else torch.float32
-        h = a.to(ct) if r is None else a.to(ct) + r.to(ct)
-        y = h * torch.rsqrt(h.square().mean(-1, keepdim=True) + eps) * weight.detach().to(ct)
+        h = a.double() if r is None else a.double() + r.double()
+        y = h * torch.rsqrt(h.square().mean(-1, keepdim=True) + eps) * weight.detach().double()
         return _quantize_ref(y, fmt, shape), (x if r is None else h.to(x.dtype).reshape(shape))
     w = weight if weight.is_contiguous() else weight.contiguous()
-    q = _empty(rows, shape, fmt, a)
+    q, codes, scales = _empty(rows, shape, fmt, a)
     h = None if r is None else a.new_empty(shape)
     if rows:
         _call(a.get_device(), "gb_mx_add_rms_norm", _TYPES[x.dtype], fmt, a.data_ptr(), a.stride(0), None if r is None else r.data_ptr(),
-              K if r is None else r.stride(0), w.data_ptr(), w.dtype == torch.float32, None if h is None else h.data_ptr(), q.Data.data_ptr(),
-              q.Scales.data_ptr(), rows, K, eps)
+              K if r is None else r.stride(0), w.data_ptr(), w.dtype == torch.float32, None if h is None else h.data_ptr(), codes, scales, rows, K, eps)
     return q, (x if h is None else h)
 
 
@@ -278,33 +314,34 @@ def _epilogue(bias, N: int, device, dtype, act, what: str):
 def MatMulMX(a: QTensorMX, b: QTensorMX, bias: Optional[torch.Tensor] = None, dtype=torch.bfloat16, act: Optional[str] = None) -> torch.Tensor:
     """``act(A B^T + bias)`` in ``dtype`` (bf16, fp16 or fp32) for A (..., K) and B (N, K), both quantised along K in one format.
     ``act``: relu, gelu or geluexact, as ``nn.Linear`` takes it.  No gradients."""
-    fmt = _checked(a, "MatMulMX")
-    if _checked(b, "MatMulMX") != fmt:
+    fmt, M, K, like, codes, scales = _checked(a, "MatMulMX")
+    fmt_b, N, K_b, like_b, codes_b, scales_b = _checked(b, "MatMulMX")
+    if fmt != fmt_b:
         raise ValueError(f"MatMulMX: both operands have one format, got {a.Format} and {b.Format}")
-    ad, bd = a.Data, b.Data
-    if len(b.Shape) != 2 or a.Shape[-1] != b.Shape[-1]:
+    if len(b.Shape) != 2 or K != K_b:
         raise ValueError(f"MatMulMX: shapes {tuple(a.Shape)} and {tuple(b.Shape)} do not match (..., K) and (N, K)")
-    if ad.device != bd.device:
-        raise ValueError(f"MatMulMX: operands on {ad.device} and {bd.device}")
-    N, K = b.Shape
-    M = ad.shape[0]
-    bias, bias_at, bias_f32, code = _epilogue(bias, N, ad.device, dtype, act, "MatMulMX")
+    if like.device != like_b.device:
+        raise ValueError(f"MatMulMX: operands on {like.device} and {like_b.device}")
+    bias, bias_at, bias_f32, code = _epilogue(bias, N, like.device, dtype, act, "MatMulMX")
     shape = (*a.Shape[:-1], N)
-    if not ad.is_cuda:
+    if not like.is_cuda:
         y = _values_ref(a) @ _values_ref(b).t()
         if bias is not None:
             y = y + bias.detach().double()
         return _act_ref(y, act).to(dtype).reshape(shape)
     if dtype not in _TYPES:
         raise TypeError(f"MatMulMX: no CUDA kernel for dtype {dtype}")
-    y = ad.new_empty(shape, dtype=dtype)
+    y = like.new_empty(shape, dtype=dtype)
     if M == 0 or N == 0:
         return y
-    out = (_l.L * 4)()
-    _l.check(_l.lib().gb_mx_plan(M, N, K, fmt, out), "gb_mx_plan")
-    ws = ad.new_empty(out[3]) if out[3] else None
-    _call(ad.get_device(), "gb_mx_matmul", fmt, ad.data_ptr(), a.Scales.data_ptr(), bd.data_ptr(), b.Scales.data_ptr(), y.data_ptr(), N, bias_at, bias_f32,
-          M, N, K, _TYPES[dtype], code, None if ws is None else ws.data_ptr(), out[3])
+    need, ws = 0, None
+    if M > _FEW:
+        out = (_l.L * 4)()
+        _l.check(_l.lib().gb_mx_plan(M, N, K, fmt, out), "gb_mx_plan")
+        need = out[3]
+        ws = like.new_empty(need, dtype=torch.uint8) if need else None
+    _call(like.get_device(), "gb_mx_matmul", fmt, codes, scales, codes_b, scales_b, y.data_ptr(), N, bias_at, bias_f32, M, N, K, _TYPES[dtype], code,
+          None if ws is None else ws.data_ptr(), need)
     return y
 
 
@@ -316,25 +353,26 @@ def LinearMX(x: Union[torch.Tensor, QTensorMX], weight: QTensorMX, bias: Optiona
         return MatMulMX(x, weight, bias, dtype or torch.bfloat16, act)
     if not x.is_cuda:
         return MatMulMX(QuantizeMX(x, weight.Format), weight, bias, dtype or x.dtype, act)
-    fmt = _checked(weight, "LinearMX")
+    fmt, N, K, like, codes, scales = _checked(weight, "LinearMX")
     a = _rows(x, "LinearMX")
-    if len(weight.Shape) != 2 or a.shape[1] != weight.Shape[1]:
+    M = a.shape[0]
+    if len(weight.Shape) != 2 or a.shape[1] != K:
         raise ValueError(f"LinearMX: shapes {tuple(x.shape)} and {tuple(weight.Shape)} do not match (..., K) and (N, K)")
-    wd = weight.Data
-    if a.device != wd.device:
-        raise ValueError(f"LinearMX: x on {a.device}, weights on {wd.device}")
+    if a.device != like.device:
+        raise ValueError(f"LinearMX: x on {a.device}, weights on {like.device}")
     dtype = dtype or x.dtype
     if dtype not in _TYPES:
         raise TypeError(f"LinearMX: no CUDA kernel for dtype {dtype}")
-    (M, K), N = a.shape, weight.Shape[0]
     bias, bias_at, bias_f32, code = _epilogue(bias, N, a.device, dtype, act, "LinearMX")
-    y = wd.new_empty((*x.shape[:-1], N), dtype=dtype)
+    y = like.new_empty((*x.shape[:-1], N), dtype=dtype)
     if M == 0 or N == 0:
         return y
-    need = _l.lib().gb_mx_linear_bytes(M, N, K, fmt)
-    scratch = wd.new_empty(need)
-    _call(wd.get_device(), "gb_mx_linear", _TYPES[x.dtype], fmt, a.data_ptr(), a.stride(0), wd.data_ptr(), weight.Scales.data_ptr(), y.data_ptr(), bias_at,
-          bias_f32, M, N, K, _TYPES[dtype], code, scratch.data_ptr(), need)
+    need, scratch = 0, None
+    if M > 16:                   # (up to 16 rows are quantised within the product's kernel)
+        need = _l.lib().gb_mx_linear_bytes(M, N, K, fmt)
+        scratch = like.new_empty(need, dtype=torch.uint8)
+    _call(like.get_device(), "gb_mx_linear", _TYPES[x.dtype], fmt, a.data_ptr(), a.stride(0), codes, scales, y.data_ptr(), bias_at, bias_f32, M, N, K,
+          _TYPES[dtype], code, None if scratch is None else scratch.data_ptr(), need)
     return y
 
 

@@ -294,6 +294,39 @@ def test_train_linear(dtype, shape, N, status_ok):
         assert off(a.detach().reshape(e.shape), e) <= (length / 32 + 4) * 2.0 ** -23 + torch.finfo(dtype).eps / 2
 
 
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N,K", [(1, 5, 3), (1, 300, 1000), (2, 128, 32), (7, 2100, 700), (16, 130, 4097), (16, 64, 8192), (5, 40000, 96)])
+def test_few_rows_are_quantised_within_the_product(format, dtype, M, N, K, status_ok):
+    """The same bits as quantisation and product one after the other: rows of any address and pitch."""
+    w, bias = Q.QuantizeMX(torch.randn(N, K, device=DEV), format), torch.randn(N, device=DEV)
+    for offset, pitch in ((0, K), (1, K), (3, K + 5), (8, K + 8)):
+        flat = torch.full((offset + M * pitch + 16,), float("nan"), dtype=dtype, device=DEV)
+        x = flat.as_strided((M, K), (pitch, 1), offset)
+        x.copy_(wild(M, K, dtype=dtype))
+        for act in (None, "relu"):
+            assert torch.equal(Q.LinearMX(x, w, bias, act), Q.MatMulMX(Q.QuantizeMX(x, format), w, bias, dtype, act))
+    x = wild(M, K, dtype=dtype)
+    x[0, K // 2] = math.inf
+    y = Q.LinearMX(x.to(DEV), w)
+    assert torch.isnan(y[0]).all() and not torch.isnan(y[1:]).any()
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("kind", [1, 2])
+@pytest.mark.parametrize("splits", [1, 2, 3, 5, 8])
+def test_every_way_of_a_product(format, kind, splits, status_ok):
+    """Either kernel with any number of slices of K gives the exact sums; slices that K does not have are none."""
+    for M, N, K in ((70, 264, 1500), (300, 512, 4100), (3, 40, 64), (520, 1032, 700)):
+        _l.lib().gb_mx_tune(kind, splits)
+        try:
+            for dtype, act in ((torch.float32, None), (torch.bfloat16, "relu")):
+                y, want = product(M, N, K, format, dtype, True, act)
+                assert torch.equal(y, want)
+        finally:
+            _l.lib().gb_mx_tune(0, 0)
+
+
 def test_train_linear_broadcast_gradient(status_ok):
     """A gradient that is one value everywhere (y.sum()), a gradient of strided rows, and an input that appears twice."""
     x = torch.randint(-4, 5, (70, 64), device=DEV).float().requires_grad_()
