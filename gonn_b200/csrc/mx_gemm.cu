@@ -73,7 +73,10 @@ __device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t smem) {
 __device__ __forceinline__ float activate(float v, int act) {
   switch (act) {
     case ACT_RELU: return fmaxf(v, 0.f);
-    case ACT_GELU_TANH: return gelu_tanh_f(v);
+    case ACT_GELU_TANH: {                  // (gelu_tanh_f in five instructions and the tanh)
+      const float h = 0.5f * v, u = v * fmaf(v * v, 0.7978845608f * 0.044715f, 0.7978845608f);
+      return fmaf(h, tanh_fast(u), h);
+    }
     case ACT_GELU_ERF: return gelu_erf_f(v);
     default: return v;
   }
@@ -106,13 +109,14 @@ __device__ __forceinline__ void tile_at(int t, int num_m, int num_n, int& m, int
 // ---------------------------------------------------------------------------------------------------------------------------
 template <int FMT>
 struct PairCfg {
-  static constexpr int STAGES = 6, EW = 8, THREADS = 64 + 32 * EW;
+  static constexpr int STAGES = 6, EW = 8, THREADS = 96 + 32 * EW;
   static constexpr int A_BYTES = 128 * 128, B_BYTES = 128 * 128, TILE_BYTES = A_BYTES + B_BYTES;
   static constexpr int PIECE = 512, S_BYTES = 3 * Fmt<FMT>::PIECES * PIECE;      // A's row of pieces, B's two
   static constexpr int OFF_SCALES = STAGES * TILE_BYTES;
   static constexpr int OFF_OUT = OFF_SCALES + STAGES * S_BYTES;
-  static constexpr int OUT_BUF = 2048;                       // of an epilogue warp
-  static constexpr int OFF_BARS = OFF_OUT + EW * OUT_BUF;
+  static constexpr int OUT_BUF = 1024;                       // of an epilogue warp
+  static constexpr int OFF_BIAS = OFF_OUT + EW * OUT_BUF;    // two tiles' bias
+  static constexpr int OFF_BARS = OFF_BIAS + 2 * 1024;
   static constexpr int BYTES = OFF_BARS + 256;
   static constexpr int ACC1 = 128, SCALES = 384, SETS = 4, SET = 12 * Fmt<FMT>::PIECES;      // TMEM columns
   static_assert(BYTES <= 232448 && OFF_OUT % 16 == 0, "shared memory");
@@ -132,10 +136,11 @@ __device__ __forceinline__ void store32(uint32_t* to, bool wide, bool both, uint
 // 32 x 32 results of a warp (a lane has a row) into C.  Rows on 32-byte boundaries: 32 bytes a lane and store, whole sectors straight from the
 // registers (an SM stores 32 bytes a clock in any case; by way of shared memory and whole lines a tile took longer: FIGURES).  Other rows,
 // a sector at a time, would write each sector many times: they go through `buf`, a column a lane.
+template <bool VECTORS>
 __device__ __forceinline__ void store_chunk(const MxArgs& a, uint8_t* buf, int slice, int row0, int col0, const float (&v)[32]) {
   const int lane = threadIdx.x & 31;
   const long long first = (long long)slice * a.M + row0;
-  if (a.vectors) {
+  if constexpr (VECTORS) {
     if (row0 + lane >= a.M) return;
     const bool wide = a.vectors == 32;
     if (a.out == OUT_F32) {
@@ -153,61 +158,40 @@ __device__ __forceinline__ void store_chunk(const MxArgs& a, uint8_t* buf, int s
                                     pack_out(a, v[j + 12], v[j + 13]), pack_out(a, v[j + 14], v[j + 15]));
     }
     return;
-  }
-  const int rows = min(32, a.M - row0);
-  if (a.out == OUT_F32) {                                    // sixteen rows at a time
-    float* f = reinterpret_cast<float*>(buf);
+  } else {
+    const int rows = min(32, a.M - row0);
+    if (a.out == OUT_F32) {                                    // eight rows at a time
+      float* f = reinterpret_cast<float*>(buf);
+#pragma unroll 1
+      for (int h = 0; h < 4; h++) {
+        __syncwarp();
+        if (lane >> 3 == h) {
+#pragma unroll
+          for (int j = 0; j < 32; j++) f[(lane & 7) * 32 + (j ^ lane)] = v[j];
+        }
+        __syncwarp();
+        if (col0 + lane < a.N)
+          for (int r = 8 * h; r < min(rows, 8 * h + 8); r++) ((float*)a.C)[(first + r) * a.ldc + col0 + lane] = f[(r & 7) * 32 + (lane ^ r)];
+      }
+      return;
+    }
+    uint32_t* w = reinterpret_cast<uint32_t*>(buf);            // sixteen
 #pragma unroll 1
     for (int h = 0; h < 2; h++) {
       __syncwarp();
       if (lane >> 4 == h) {
 #pragma unroll
-        for (int j = 0; j < 32; j++) f[(lane & 15) * 32 + (j ^ lane)] = v[j];
+        for (int j = 0; j < 16; j++) w[(lane & 15) * 16 + (j ^ (lane & 15))] = pack_out(a, v[2 * j], v[2 * j + 1]);
       }
       __syncwarp();
       if (col0 + lane < a.N)
-        for (int r = 16 * h; r < min(rows, 16 * h + 16); r++) ((float*)a.C)[(first + r) * a.ldc + col0 + lane] = f[(r & 15) * 32 + (lane ^ r)];
+        for (int r = 16 * h; r < min(rows, 16 * h + 16); r++)
+          ((uint16_t*)a.C)[(first + r) * a.ldc + col0 + lane] = (uint16_t)(w[(r & 15) * 16 + (lane >> 1 ^ (r & 15))] >> (16 * (lane & 1)));
     }
-    return;
-  }
-  uint32_t* w = reinterpret_cast<uint32_t*>(buf);
-  __syncwarp();
-#pragma unroll
-  for (int j = 0; j < 16; j++) w[lane * 16 + (j ^ (lane & 15))] = pack_out(a, v[2 * j], v[2 * j + 1]);
-  __syncwarp();
-  if (col0 + lane < a.N)
-    for (int r = 0; r < rows; r++) ((uint16_t*)a.C)[(first + r) * a.ldc + col0 + lane] = (uint16_t)(w[r * 16 + (lane >> 1 ^ (r & 15))] >> (16 * (lane & 1)));
-}
-
-// The bias of 32 columns, the same in every lane.
-__device__ __forceinline__ void add_bias(const MxArgs& a, int col0, float (&v)[32]) {
-  if (a.bias == nullptr) return;
-  if (col0 + 32 <= a.N && ((uintptr_t)a.bias & 15) == 0) {
-    if (a.bias_f32) {
-#pragma unroll
-      for (int j = 0; j < 32; j += 4) {
-        const float4 b = __ldg(reinterpret_cast<const float4*>((const float*)a.bias + col0 + j));
-        v[j] += b.x; v[j + 1] += b.y; v[j + 2] += b.z; v[j + 3] += b.w;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; j += 8) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>((const uint16_t*)a.bias + col0 + j));
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float2 b = a.out == OUT_BF16 ? unpack_bf16(w[i]) : unpack_f16(w[i]);
-          v[j + 2 * i] += b.x; v[j + 2 * i + 1] += b.y;
-        }
-      }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; j++) v[j] += bias_at(a, col0 + j);
   }
 }
 
-template <int FMT>
+template <int FMT, bool VECTORS>
 __global__ void __launch_bounds__(PairCfg<FMT>::THREADS, 1)
 mx_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmSA,
                const __grid_constant__ CUtensorMap tmSB, const MxArgs args) {
@@ -222,7 +206,9 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
   uint64_t* empty = full + C::STAGES;                        // [STAGES]  per CTA
   uint64_t* ready = empty + C::STAGES;                       // [2]       per CTA: an accumulator is complete
   uint64_t* drained = ready + 2;                             //           used in CTA 0: the columns that the next tile needs are free
-  uint32_t* slot = (uint32_t*)(drained + 1);
+  uint64_t* bias_full = drained + 1;                         // [2]       per CTA
+  uint64_t* bias_empty = bias_full + 2;                      // [2]       per CTA
+  uint32_t* slot = (uint32_t*)(bias_empty + 2);
   volatile int* abort_flag = (volatile int*)(slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t cta = cluster_ctarank();
@@ -234,8 +220,11 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    mbar_init(&ready[0], 1);
-    mbar_init(&ready[1], 1);
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&ready[i], 1);
+      mbar_init(&bias_full[i], 1);
+      mbar_init(&bias_empty[i], C::EW);
+    }
     mbar_init(drained, 2 * C::EW);
     *abort_flag = 0;
     mbar_fence_init();
@@ -330,6 +319,24 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
       }
     }
     __syncwarp();
+  } else if (warp == 2 + C::EW) {
+    // the bias of the tiles' columns, a tile or two ahead (fetched where it is needed it kept the warps waiting: 16384 x 2304 x 768 52 us, so FIGURES)
+    if (args.bias != nullptr) {
+      int local = 0;
+      for (int u = pair; u < units; u += pairs, local++) {
+        const int which = local & 1;
+        int mb, nb;
+        tile_at(u % tiles, args.num_m, args.num_n, mb, nb);
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) f[i] = bias_at(args, nb * 256 + i * 32 + lane);
+        if (!__all_sync(0xffffffffu, mbar_wait(&bias_empty[which], ((local >> 1) & 1) ^ 1, abort_flag, args.status, ST_GEMM_TIMEOUT, 37))) break;
+#pragma unroll
+        for (int i = 0; i < 8; i++) reinterpret_cast<float*>(smem + C::OFF_BIAS)[which * 256 + i * 32 + lane] = f[i];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bias_full[which]);
+      }
+    }
   } else {
     const int q = warp & 3, half = (warp - 2) >> 2;
     uint8_t* buf = smem + C::OFF_OUT + (warp - 2) * C::OUT_BUF;
@@ -339,6 +346,7 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
       int mb, nb;
       tile_at(u - slice * tiles, args.num_m, args.num_n, mb, nb);
       const int row0 = mb * 256 + (int)cta * 128 + q * 32;
+      if (args.bias != nullptr && !mbar_wait(&bias_full[which], (local >> 1) & 1, abort_flag, args.status, ST_GEMM_TIMEOUT, 36)) break;
       if (!mbar_wait(&ready[which], (local >> 1) & 1, abort_flag, args.status, ST_GEMM_TIMEOUT, 35)) break;
       tc_fence_after();
       const uint32_t acc = tmem + which * C::ACC1 + ((uint32_t)(q * 32) << 16);
@@ -361,12 +369,23 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         float v[32];
 #pragma unroll
         for (int j = 0; j < 32; j++) v[j] = __uint_as_float(r[i & 1][j]);
-        add_bias(args, col0, v);
+        if (args.bias != nullptr) {
+          const float* b = reinterpret_cast<const float*>(smem + C::OFF_BIAS) + which * 256 + column(i);
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(b + j);
+            v[j] += f.x; v[j + 1] += f.y; v[j + 2] += f.z; v[j + 3] += f.w;
+          }
+        }
         if (args.act != ACT_NONE) {
 #pragma unroll
           for (int j = 0; j < 32; j++) v[j] = activate(v[j], args.act);
         }
-        store_chunk(args, buf, slice, row0, col0, v);
+        store_chunk<VECTORS>(args, buf, slice, row0, col0, v);
+      }
+      if (args.bias != nullptr) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bias_empty[which]);
       }
     }
   }
@@ -609,21 +628,33 @@ mx_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
   if (S > 1) cluster_sync_all();   // nobody leaves while another may still read its shared memory
 }
 
-// Slices of a product cut along K, summed in their order: C = act(sum + bias).
-__global__ void __launch_bounds__(256) mx_finish_kernel(const float* __restrict__ part, const MxArgs a, int slices) {
+// Slices of a product cut along K, summed in their order: C = act(sum + bias).  Four columns a thread; N is a multiple of 4.
+__global__ void __launch_bounds__(256) mx_finish_kernel(const float* __restrict__ part, const MxArgs a, int slices, FastDiv by_quads) {
   pdl_trigger();
   pdl_wait();
-  const long long total = (long long)a.M * a.N, stride = (long long)gridDim.x * blockDim.x * 4;
-  for (long long i = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 4; i < total; i += stride) {      // (N is a multiple of 4)
+  const int quads = a.N / 4, size = a.out == OUT_F32 ? 4 : 2;
+  const long long total = (long long)a.M * a.N;
+  const bool vector = (((uintptr_t)a.C | (uintptr_t)(a.ldc * size)) & (4 * size - 1)) == 0;
+  for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < (uint32_t)a.M * (uint32_t)quads; i += gridDim.x * 256) {
+    const uint32_t row = by_quads.div(i);
+    const int c = (int)(i - row * by_quads.d) * 4;
+    const float4* from = reinterpret_cast<const float4*>(part) + i;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
     for (int p = 0; p < slices; p++) {
-      const float4 u = __ldcs(reinterpret_cast<const float4*>(part + p * total + i));
+      const float4 u = __ldcs(from + p * (total / 4));
       s.x += u.x; s.y += u.y; s.z += u.z; s.w += u.w;
     }
-    const long long row = i / a.N;
-    const int c = (int)(i - row * a.N);
-    const float v[4] = {s.x, s.y, s.z, s.w};
-    for (int j = 0; j < 4; j++) store_out(a, row * a.ldc + c + j, activate(v[j] + bias_at(a, c + j), a.act));
+    const float y[4] = {activate(s.x + bias_at(a, c), a.act), activate(s.y + bias_at(a, c + 1), a.act), activate(s.z + bias_at(a, c + 2), a.act),
+                        activate(s.w + bias_at(a, c + 3), a.act)};
+    const long long to = row * a.ldc + c;
+    if (!vector) {
+      for (int j = 0; j < 4; j++) store_out(a, to + j, y[j]);
+    } else if (a.out == OUT_F32) {
+      *reinterpret_cast<float4*>((float*)a.C + to) = make_float4(y[0], y[1], y[2], y[3]);
+    } else {
+      *reinterpret_cast<uint2*>((uint16_t*)a.C + to) = make_uint2(pack_out(a, y[0], y[1]), pack_out(a, y[2], y[3]));
+    }
   }
 }
 
@@ -721,14 +752,14 @@ int map_scales(CUtensorMap* m, const void* p, long long rows, int P, int pieces,
   return gbh::encode_tmap(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, p, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-template <int FMT>
+template <int FMT, bool VECTORS>
 int launch_pair(const Maps& tm, const MxArgs& args, cudaStream_t st) {
   using C = PairCfg<FMT>;
   static std::atomic<uint32_t> done{0};
-  if (int rc = allow_shared(mx_pair_kernel<FMT>, C::BYTES, done)) return rc;
+  if (int rc = allow_shared(mx_pair_kernel<FMT, VECTORS>, C::BYTES, done)) return rc;
   const long long units = (long long)args.num_m * args.num_n * args.splits;
   const int pairs = units < 74 ? (int)units : 74;
-  GB_CUDA_OK(gbh::launch(mx_pair_kernel<FMT>, dim3(2 * pairs), dim3(C::THREADS), C::BYTES, st, 2, tm.a, tm.b, tm.sa, tm.sb, args));
+  GB_CUDA_OK(gbh::launch(mx_pair_kernel<FMT, VECTORS>, dim3(2 * pairs), dim3(C::THREADS), C::BYTES, st, 2, tm.a, tm.b, tm.sa, tm.sb, args));
   return gbh::E_OK;
 }
 template <int FMT, int BN, typename X = void>
@@ -807,10 +838,12 @@ GB_EXPORT int gb_mx_matmul(int fmt, const void* a, const void* sa, const void* b
     if (!rc) rc = map_codes(&tm.b, b, N, RB, 128);
     if (!rc) rc = map_scales(&tm.sa, sa, M, P, per, 1);
     if (!rc) rc = map_scales(&tm.sb, sb, N, P, per, 2);
-    if (!rc) rc = fmt == FP8 ? launch_pair<FP8>(tm, run, st) : launch_pair<FP4>(tm, run, st);
+    if (!rc && run.vectors) rc = fmt == FP8 ? launch_pair<FP8, true>(tm, run, st) : launch_pair<FP4, true>(tm, run, st);
+    else if (!rc) rc = fmt == FP8 ? launch_pair<FP8, false>(tm, run, st) : launch_pair<FP4, false>(tm, run, st);
     if (rc || p.splits == 1) return rc;
     const long long quads = M * N / 4;
-    GB_CUDA_OK(gbh::launch(mx_finish_kernel, dim3((unsigned)(quads / 256 + 1 < 148 * 8 ? quads / 256 + 1 : 148 * 8)), dim3(256), 0, st, 1, (const float*)workspace, args, p.splits));
+    GB_CUDA_OK(gbh::launch(mx_finish_kernel, dim3((unsigned)(quads / 256 + 1 < 148 * 8 ? quads / 256 + 1 : 148 * 8)), dim3(256), 0, st, 1, (const float*)workspace, args, p.splits,
+                           FastDiv((uint32_t)(N / 4))));
     return gbh::E_OK;
   }
   args.num_m = (int)((M + p.bn - 1) / p.bn);

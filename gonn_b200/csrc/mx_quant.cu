@@ -194,8 +194,10 @@ __global__ void __launch_bounds__(256) mx_column_sum_kernel(const float* __restr
   pdl_wait();
   const int c = blockIdx.x * 32 + (threadIdx.x & 31), strip = threadIdx.x >> 5;
   float s = 0.f;
-  if (c < K)
+  if (c < K) {
+#pragma unroll 8
     for (int i = strip; i < pieces; i += 8) s += __ldg(sums + (long long)i * K + c);
+  }
   part[strip][threadIdx.x & 31] = s;
   __syncthreads();
   if (strip == 0 && c < K) {
