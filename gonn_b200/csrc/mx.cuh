@@ -222,19 +222,6 @@ template <> __device__ __forceinline__ float to_type<float>(float v) { return v;
 template <> __device__ __forceinline__ __half to_type<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 to_type<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// The same for rows at any address: L lanes side by side hold 16 L consecutive values, from column `first` on, and write them one column
-// a lane, so that a store covers whole sectors.  buf: 16 L floats of shared memory.
-template <typename T, int L>
-__device__ __forceinline__ void store16_any(T* row, int first, int K, const float (&v)[16], float* buf, int lane, unsigned mask) {
-  __syncwarp(mask);
-#pragma unroll
-  for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(buf + lane * 16 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-  __syncwarp(mask);
-#pragma unroll
-  for (int i = 0; i < 16; i++)
-    if (first + i * L + lane < K) row[first + i * L + lane] = to_type<T>(buf[i * L + lane]);
-}
-
 // Bits of the largest magnitude of sixteen elements.  16-bit magnitudes compare in pairs, as whole numbers.
 template <typename T>
 __device__ __forceinline__ uint32_t largest16(const uint32_t (&w)[4 * Elem<T>::SZ]) {

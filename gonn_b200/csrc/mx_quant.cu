@@ -29,7 +29,7 @@ struct QuantArgs {
 };
 
 // A unit is 128 columns of a row; NU units of a lane are in flight.
-template <typename T, int FMT, bool ALIGNED>
+template <typename T, int FMT>
 __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const QuantArgs a) {
   constexpr int NU = Elem<T>::SZ == 2 ? 2 : 1;
   pdl_trigger();
@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const QuantArgs a
       const uint32_t u = min(u0 + i * stride, units - 1);
       row[i] = a.by_pieces.div(u);
       g[i] = (int)(u - row[i] * a.by_pieces.d);
-      load16<T, ALIGNED>(reinterpret_cast<const T*>(a.x) + row[i] * a.ld, g[i] * 128 + l8 * 16, a.K, a.wide, a.ext, w[i]);
+      load16<T, true>(reinterpret_cast<const T*>(a.x) + row[i] * a.ld, g[i] * 128 + l8 * 16, a.K, a.wide, a.ext, w[i]);
     }
 #pragma unroll
     for (int i = 0; i < NU; i++) {
@@ -58,6 +58,57 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const QuantArgs a
       store_codes<FMT>(a.data + (long long)row[i] * a.row_bytes, g[i] * 128 + l8 * 16, a.row_bytes, out);
       if (l8 == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_word(row[i], g[i], a.pieces)) = word;
     }
+  }
+}
+
+// Rows at any address: a column a lane, so that every load and store is of neighbours whatever they start on, and a block is a warp's.
+__device__ __forceinline__ float load_one(const __nv_bfloat16* p) { return __uint_as_float((uint32_t)__ldg(reinterpret_cast<const uint16_t*>(p)) << 16); }
+__device__ __forceinline__ float load_one(const __half* p) { return __half2float(__ushort_as_half(__ldg(reinterpret_cast<const uint16_t*>(p)))); }
+__device__ __forceinline__ float load_one(const float* p) { return __uint_as_float(__ldg(reinterpret_cast<const uint32_t*>(p))); }
+
+// The code of a lane's value of a block: a byte of columns k (FP8), or of columns k and k + 1 for even lanes (FP4).  Returns the block's scale code.
+template <int FMT>
+__device__ __forceinline__ uint32_t quantize1(float v, uint32_t& byte) {
+  const uint32_t code = scale_code(__reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu), FMT);
+  const float q = mul_exact(v, scale_inverse(code));
+  if (FMT == FP8) {
+    byte = e4m3x4(q, 0.f, 0.f, 0.f);
+  } else {
+    const float two[8] = {q, __shfl_xor_sync(0xffffffffu, q, 1), 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    byte = e2m1x8(two);
+  }
+  return code;
+}
+template <int FMT>
+__device__ __forceinline__ void store_byte(uint8_t* row, int k, int row_bytes, uint32_t byte) {
+  const int b = FMT == FP8 ? k : k / 2;
+  if (b < row_bytes && (FMT == FP8 || (k & 1) == 0)) row[b] = (uint8_t)byte;
+}
+
+template <typename T, int FMT>
+__global__ void __launch_bounds__(kThreads) mx_quantize_any_kernel(const QuantArgs a) {
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const uint32_t units = (uint32_t)a.rows * (uint32_t)a.pieces, stride = gridDim.x * (kThreads / 32);
+  for (uint32_t u = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); u < units; u += stride) {
+    const uint32_t row = a.by_pieces.div(u);
+    const int g = (int)(u - row * a.by_pieces.d);
+    const T* x = reinterpret_cast<const T*>(a.x) + row * a.ld;
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int k = g * 128 + i * 32 + lane;
+      v[i] = k < a.K ? load_one(x + k) : 0.f;
+    }
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      uint32_t byte;
+      word |= quantize1<FMT>(v[i], byte) << (8 * i);
+      store_byte<FMT>(a.data + (long long)row * a.row_bytes, g * 128 + i * 32 + lane, a.row_bytes, byte);
+    }
+    if (lane == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_word(row, g, a.pieces)) = word;
   }
 }
 
@@ -231,13 +282,12 @@ __device__ __forceinline__ void numbers16(const uint32_t (&c)[4], float (&v)[16]
   }
 }
 
-template <typename T, int FMT, bool ALIGNED>
+template <typename T, int FMT>
 __global__ void __launch_bounds__(kThreads) mx_dequantize_kernel(const DequantArgs a) {
   constexpr int NU = 2;
-  __shared__ __align__(16) float bufs[ALIGNED ? 4 : kThreads * 16];
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31, l8 = threadIdx.x & 7;
+  const int l8 = threadIdx.x & 7;
   const uint32_t units = (uint32_t)a.rows * (uint32_t)a.pieces, stride = gridDim.x * (kThreads / 8);
   for (uint32_t u0 = blockIdx.x * (kThreads / 8) + (threadIdx.x >> 3); u0 < units; u0 += NU * stride) {
     uint32_t c[NU][4], row[NU];
@@ -270,9 +320,46 @@ __global__ void __launch_bounds__(kThreads) mx_dequantize_kernel(const DequantAr
       const float scale = scale_value(s[i]);
 #pragma unroll
       for (int j = 0; j < 16; j++) v[j] = mul_exact(v[j], scale);
-      T* to = reinterpret_cast<T*>(a.y) + (long long)row[i] * a.K;
-      if constexpr (ALIGNED) store16(to, g[i] * 128 + l8 * 16, a.K, a.wide, v);
-      else store16_any<T, 8>(to, g[i] * 128, a.K, v, bufs + (threadIdx.x >> 3) * 128, l8, 0xffu << (lane & 24));
+      store16(reinterpret_cast<T*>(a.y) + (long long)row[i] * a.K, g[i] * 128 + l8 * 16, a.K, a.wide, v);
+    }
+  }
+}
+
+// Rows of values at any address: a column a lane.
+template <typename T, int FMT>
+__global__ void __launch_bounds__(kThreads) mx_dequantize_any_kernel(const DequantArgs a) {
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const uint32_t units = (uint32_t)a.rows * (uint32_t)a.pieces, stride = gridDim.x * (kThreads / 32);
+  for (uint32_t u = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); u < units; u += stride) {
+    const uint32_t row = a.by_pieces.div(u);
+    const int g = (int)(u - row * a.by_pieces.d);
+    const uint8_t* from = a.data + (long long)row * a.row_bytes;
+    uint32_t c[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int k = g * 128 + i * 32 + lane;
+      c[i] = 0;
+      if (FMT == FP8) {
+        if (k < a.K) c[i] = __ldg(from + k);
+      } else if (k / 2 < a.row_bytes) {      // (the eight codes around a lane's: rows are padded to whole blocks)
+        c[i] = __ldg(reinterpret_cast<const uint32_t*>(from) + k / 8) >> (4 * (k & 7));
+      }
+    }
+    const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(a.scales + scale_word(row, g, a.pieces)));
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int k = g * 128 + i * 32 + lane;
+      float v;
+      if (FMT == FP8) {
+        uint32_t h;
+        asm("{\n.reg .b16 t;\ncvt.u16.u32 t, %1;\ncvt.rn.f16x2.e4m3x2 %0, t;\n}" : "=r"(h) : "r"(c[i]));
+        v = unpack_f16(h).x;
+      } else {                               // exponent and fraction stand as they do in fp32, 126 exponents below (one half of a converted pair came out 0)
+        v = mul_exact(__uint_as_float((c[i] & 7u) << 22 | (c[i] & 8u) << 28), 0x1p126f);
+      }
+      if (k < a.K) reinterpret_cast<T*>(a.y)[(long long)row * a.K + k] = to_type<T>(mul_exact(v, scale_value(word >> (8 * i) & 255u)));
     }
   }
 }
@@ -293,7 +380,7 @@ struct NormArgs {
   Extent ex, er, ew;
 };
 
-// fp32 arithmetic that keeps subnormal numbers.
+// fp32 arithmetic that keeps subnormal numbers, alone and in pairs.
 __device__ __forceinline__ float add_exact(float a, float b) {
   float d;
   asm("add.rn.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
@@ -302,6 +389,27 @@ __device__ __forceinline__ float add_exact(float a, float b) {
 __device__ __forceinline__ float fma_exact(float a, float b, float c) {
   float d;
   asm("fma.rn.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ void parts_of(uint64_t p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
   return d;
 }
 
@@ -319,14 +427,18 @@ __device__ __forceinline__ Root inverse_root(double sum, double inv_K, double ep
   return {hi, (float)(r - (double)hi)};
 }
 
-// h (hi + lo) * root * w, rounded to odd: the last bit stands for all that lies behind it, so that the rounding to a code afterwards is that of
-// the product itself.  (A value next to the border between two codes falls on the side where it belongs: with three roundings of fp32 one in
-// a million fell on the other, a step of the code away.)
-template <bool LO>
-__device__ __forceinline__ float normalized(float h, float lo, const Root& root, float w) {
-  const float p = mul_exact(h, root.hi);
-  float e = fma_exact(h, root.lo, fma_exact(h, root.hi, -p));
-  if (LO) e = fma_exact(lo, root.hi, e);
+// A value next to the border between two codes has to fall on the side where it belongs: by three roundings of fp32 one in a million falls on
+// the other, a step of the code away.  Borders, and the powers of two at which a scale changes, have at most four leading bits of
+// a fraction (E4M3; E2M1 two), so the last 19 bits of a value in their neighbourhood are next to zero; four roundings move them by less
+// than eight.  Such values (one in 32 000; and zeros, infinities and NaN) are computed again, rounded to odd: the last bit stands for
+// all that lies behind it, so that the rounding to a code afterwards is that of the product itself.
+__device__ __forceinline__ uint32_t from_border(float y) { return (__float_as_uint(y) + 8u) & 0x7ffffu; }
+constexpr uint32_t kNear = 16;
+
+// h (hi + lo) * root * w, rounded to odd.
+__device__ __noinline__ float to_odd(float h, float lo, float root_hi, float root_lo, float w) {
+  const float p = mul_exact(h, root_hi);
+  const float e = fma_exact(lo, root_hi, fma_exact(h, root_lo, fma_exact(h, root_hi, -p)));
   const float ew = mul_exact(e, w);
   float z;
   asm("fma.rz.f32 %0, %1, %2, %3;" : "=f"(z) : "f"(p), "f"(w), "f"(ew));
@@ -334,64 +446,15 @@ __device__ __forceinline__ float normalized(float h, float lo, const Root& root,
   return left != 0.f ? __uint_as_float(__float_as_uint(z) | 1u) : z;
 }
 
-// A row's weights stand still while rows come and go: vectors from L1.
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ void weights16(const NormArgs& a, int k, float (&f)[16]) {
-  if (sizeof(T) == 2 && a.w_f32) {
-    uint32_t u[16];
-    load16<float, false>(reinterpret_cast<const float*>(a.w), k, a.K, false, a.ew, u);
-    unpack16<float>(u, f);
-  } else {
-    uint32_t u[4 * Elem<T>::SZ];
-    load16<T, ALIGNED>(reinterpret_cast<const T*>(a.w), k, a.K, false, a.ew, u);
-    unpack16<T>(u, f);
-  }
+// What the rounding of x + r to fp32 leaves out.  (Sums of 16-bit values are exact but for far magnitudes.)
+__device__ __forceinline__ float left_out(float h, float x, float r) {
+  const float b = add_exact(h, -x);
+  const float lo = add_exact(add_exact(x, -add_exact(h, -b)), add_exact(r, -b));
+  return fabsf(h) < 3e38f ? lo : 0.f;
 }
 
-// The sum of two values and, of fp32 ones, what its rounding leaves out (sums of 16-bit values are exact but for far magnitudes).
-template <typename T>
-__device__ __forceinline__ void sum_of(float& h, float& lo, float x, float r) {
-  h = add_exact(x, r);
-  if constexpr (sizeof(T) == 4) {
-    const float b = add_exact(h, -x);
-    lo = add_exact(add_exact(x, -add_exact(h, -b)), add_exact(r, -b));
-    if (!(fabsf(h) < 3e38f)) lo = 0.f;
-  }
-}
-
-template <typename T, bool ALIGNED, int L>
-__device__ __forceinline__ void write_sum(const NormArgs& a, long long row, int k, const float (&v)[16], float* buf, int lane, unsigned mask) {
-  T* to = reinterpret_cast<T*>(a.h) + row * a.K;
-  if constexpr (ALIGNED) store16(to, k, a.K, a.wide, v);
-  else store16_any<T, L>(to, k - lane * 16, a.K, v, buf, lane, mask);
-}
-
-template <typename T, int FMT, bool ALIGNED>
-__device__ __forceinline__ void write_norm(const NormArgs& a, long long row, int k, float (&v)[16], const float (&lo)[16], const Root& root) {
-  float w[16];
-  weights16<T, ALIGNED>(a, k, w);
-#pragma unroll
-  for (int i = 0; i < 16; i++) v[i] = normalized<sizeof(T) == 4>(v[i], lo[i], root, w[i]);
-  uint32_t out[4];
-  const int lane = threadIdx.x & 31;
-  const uint32_t word = quantize16<FMT>(v, largest16(v), 0xffu << (lane & 24), lane, out);
-  store_codes<FMT>(a.data + row * a.row_bytes, k, a.row_bytes, out);
-  if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_word(row, k >> 7, a.pieces)) = word;
-}
-
-// The squares of sixteen values: two chains of eight in fp32, which an fp64 sum takes up.
-__device__ __forceinline__ double squares(const float (&v)[16]) {
-  float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-  for (int j = 0; j < 16; j += 2) {
-    s0 = fma_exact(v[j], v[j], s0);
-    s1 = fma_exact(v[j + 1], v[j + 1], s1);
-  }
-  return (double)s0 + (double)s1;
-}
-
-template <int G>
-__device__ __forceinline__ double row_sum(double s, double* red) {
+template <int G, typename S>
+__device__ __forceinline__ double row_sum(double s, S* red) {
 #pragma unroll
   for (int o = (G < 32 ? G : 32) / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (G <= 32) return s;
@@ -406,18 +469,93 @@ __device__ __forceinline__ double row_sum(double s, double* red) {
   return s;
 }
 
-// G threads of a block take a row, VPT vectors of sixteen columns each, which stay in registers between the two passes.  VPT = 0: rows
-// of any length, read a second time for their codes.
-template <typename T, int FMT, int G, int VPT, bool ALIGNED>
+// Sixteen columns of x + r: in pairs, and what rounding leaves out of fp32 ones.
+template <typename T>
+__device__ __forceinline__ void sum16(const uint32_t (&wx)[4 * Elem<T>::SZ], const uint32_t (&wr)[4 * Elem<T>::SZ], uint64_t (&h)[8], float (&lo)[16]) {
+  float x[16], r[16];
+  unpack16<T>(wx, x);
+  unpack16<T>(wr, r);
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    h[j] = add_pair(pair_of(x[2 * j], x[2 * j + 1]), pair_of(r[2 * j], r[2 * j + 1]));
+    if constexpr (sizeof(T) == 4) {
+      float a, b;
+      parts_of(h[j], a, b);
+      lo[2 * j] = left_out(a, x[2 * j], r[2 * j]);
+      lo[2 * j + 1] = left_out(b, x[2 * j + 1], r[2 * j + 1]);
+    }
+  }
+}
+// Their squares: two chains of eight in fp32, which an fp64 sum takes up.
+__device__ __forceinline__ double squares(const uint64_t (&h)[8]) {
+  uint64_t s = 0;
+#pragma unroll
+  for (int j = 0; j < 8; j++) s = fma_pair(h[j], h[j], s);
+  float a, b;
+  parts_of(s, a, b);
+  return (double)a + (double)b;
+}
+
+template <typename T>
+__device__ __forceinline__ void write_sum(const NormArgs& a, long long row, int k, const uint64_t (&h)[8]) {
+  float v[16];
+#pragma unroll
+  for (int j = 0; j < 8; j++) parts_of(h[j], v[2 * j], v[2 * j + 1]);
+  store16(reinterpret_cast<T*>(a.h) + row * a.K, k, a.K, a.wide, v);
+}
+
+template <typename T, int FMT>
+__device__ __forceinline__ void write_norm(const NormArgs& a, long long row, int k, const uint64_t (&h)[8], const float (&lo)[16], const Root& root) {
+  float w[16], y[16];
+  if (sizeof(T) == 2 && a.w_f32) {
+    uint32_t u[16];
+    load16<float, false>(reinterpret_cast<const float*>(a.w), k, a.K, false, a.ew, u);
+    unpack16<float>(u, w);
+  } else {                               // (a row's weights stand still while rows come and go: vectors from L1)
+    uint32_t u[4 * Elem<T>::SZ];
+    load16<T, true>(reinterpret_cast<const T*>(a.w), k, a.K, false, a.ew, u);
+    unpack16<T>(u, w);
+  }
+  const uint64_t root2 = pair_of(root.hi, root.hi);
+  uint32_t near = ~0u;
+  float m = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    parts_of(mul_pair(mul_pair(h[j], root2), pair_of(w[2 * j], w[2 * j + 1])), y[2 * j], y[2 * j + 1]);
+    near = min(near, min(from_border(y[2 * j]), from_border(y[2 * j + 1])));
+    m = fmaxf(fmaxf(m, fabsf(y[2 * j])), fabsf(y[2 * j + 1]));
+  }
+  uint32_t amax = __float_as_uint(m);    // (a flushed subnormal number has the same scale; infinities and NaN take the branch)
+  if (near <= kNear) {
+    bool again = false;                  // (zeros alone: no)
+#pragma unroll
+    for (int j = 0; j < 16; j++) again |= y[j] != 0.f && from_border(y[j]) <= kNear;
+    if (again) {
+#pragma unroll
+      for (int j = 0; j < 16; j++) {
+        float p, q;
+        parts_of(h[j / 2], p, q);
+        y[j] = to_odd(j & 1 ? q : p, sizeof(T) == 4 ? lo[j] : 0.f, root.hi, root.lo, w[j]);
+      }
+      amax = largest16(y);
+    }
+  }
+  uint32_t out[4];
+  const int lane = threadIdx.x & 31;
+  const uint32_t word = quantize16<FMT>(y, amax, 0xffu << (lane & 24), lane, out);
+  store_codes<FMT>(a.data + row * a.row_bytes, k, a.row_bytes, out);
+  if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_word(row, k >> 7, a.pieces)) = word;
+}
+
+// Aligned rows.  G threads of a block take a row, VPT vectors of sixteen columns each, which stay in registers between the two passes.  VPT = 0:
+// rows of any length, read a second time for their codes.
+template <typename T, int FMT, int G, int VPT>
 __global__ void __launch_bounds__(G > kThreads ? G : kThreads) mx_norm_kernel(const NormArgs a) {
-  constexpr int THREADS = G > kThreads ? G : kThreads, L = G < 32 ? G : 32, W = 4 * Elem<T>::SZ, F32 = sizeof(T) == 4;
+  constexpr int THREADS = G > kThreads ? G : kThreads, W = 4 * Elem<T>::SZ, F32 = sizeof(T) == 4;
   __shared__ double red[32];
-  __shared__ __align__(16) float bufs[ALIGNED ? 4 : THREADS * 16];
   pdl_trigger();
   pdl_wait();
-  const int t = threadIdx.x % G, lane = threadIdx.x % L;
-  float* buf = bufs + (ALIGNED ? 0 : threadIdx.x / L * L * 16);
-  const unsigned mask = L == 32 ? 0xffffffffu : ((1u << L) - 1u) << (threadIdx.x & 31 & ~(L - 1));
+  const int t = threadIdx.x % G;
   const int vecs = a.pieces * 8;                         // whole pieces: eight lanes work together
   const bool sum = a.r != nullptr;
   constexpr int per = THREADS / G;
@@ -428,7 +566,8 @@ __global__ void __launch_bounds__(G > kThreads ? G : kThreads) mx_norm_kernel(co
     const T* r = reinterpret_cast<const T*>(a.r) + row * a.ldr;
     double s = 0.0;
     if constexpr (VPT > 0) {
-      float v[VPT][16], lo[F32 ? VPT : 1][16];
+      uint64_t h[VPT][8];
+      float lo[F32 ? VPT : 1][16];
       {
         uint32_t wx[VPT][W], wr[VPT][W];
 #pragma unroll
@@ -437,55 +576,115 @@ __global__ void __launch_bounds__(G > kThreads ? G : kThreads) mx_norm_kernel(co
 #pragma unroll
           for (int j = 0; j < W; j++) wx[i][j] = wr[i][j] = 0;
           if (live) {
-            load16<T, ALIGNED>(x, k, a.K, a.wide, a.ex, wx[i]);
-            if (sum) load16<T, ALIGNED>(r, k, a.K, a.wide, a.er, wr[i]);
+            load16<T, true>(x, k, a.K, a.wide, a.ex, wx[i]);
+            if (sum) load16<T, true>(r, k, a.K, a.wide, a.er, wr[i]);
           }
         }
 #pragma unroll
         for (int i = 0; i < VPT; i++) {
-          float f[16];
-          unpack16<T>(wx[i], v[i]);
-          unpack16<T>(wr[i], f);                         // (zeros without a residual)
-#pragma unroll
-          for (int j = 0; j < 16; j++) sum_of<T>(v[i][j], lo[F32 ? i : 0][j], v[i][j], f[j]);
-          s += squares(v[i]);
+          sum16<T>(wx[i], wr[i], h[i], lo[F32 ? i : 0]);     // (zeros without a residual)
+          s += squares(h[i]);
         }
       }
-      if (sum) {
+      if (sum && live) {
 #pragma unroll
-        for (int i = 0; i < VPT; i++)
-          if (live) write_sum<T, ALIGNED, L>(a, row, (t + i * G) * 16, v[i], buf, lane, mask);
+        for (int i = 0; i < VPT; i++) write_sum<T>(a, row, (t + i * G) * 16, h[i]);
       }
       const Root root = inverse_root(row_sum<G>(s, red), a.inv_K, a.eps);
 #pragma unroll
       for (int i = 0; i < VPT; i++)
-        if (live && t + i * G < vecs) write_norm<T, FMT, ALIGNED>(a, row, (t + i * G) * 16, v[i], lo[F32 ? i : 0], root);
+        if (live && t + i * G < vecs) write_norm<T, FMT>(a, row, (t + i * G) * 16, h[i], lo[F32 ? i : 0], root);
     } else {
-      auto take = [&](int k, float (&v)[16], float (&lo)[16]) {
-        uint32_t u[W];
-        float f[16];
-        load16<T, ALIGNED>(x, k, a.K, a.wide, a.ex, u);
-        unpack16<T>(u, v);
+      auto take = [&](int k, uint64_t (&h)[8], float (&lo)[16]) {
+        uint32_t u[W], v[W];
+        load16<T, true>(x, k, a.K, a.wide, a.ex, u);
 #pragma unroll
-        for (int j = 0; j < W; j++) u[j] = 0;
-        if (sum) load16<T, ALIGNED>(r, k, a.K, a.wide, a.er, u);
-        unpack16<T>(u, f);
-#pragma unroll
-        for (int j = 0; j < 16; j++) sum_of<T>(v[j], lo[j], v[j], f[j]);
+        for (int j = 0; j < W; j++) v[j] = 0;
+        if (sum) load16<T, true>(r, k, a.K, a.wide, a.er, v);
+        sum16<T>(u, v, h, lo);
       };
-      // (a row's threads take each step together, as their stores of the sum do)
-      for (int i = t; i - t < vecs; i += G) {
-        float v[16], lo[16];
-        take(i * 16, v, lo);
-        if (sum) write_sum<T, ALIGNED, L>(a, row, i * 16, v, buf, lane, mask);
-        s += squares(v);
+      for (int i = t; i < vecs; i += G) {
+        uint64_t h[8];
+        float lo[16];
+        take(i * 16, h, lo);
+        if (sum) write_sum<T>(a, row, i * 16, h);
+        s += squares(h);
       }
       const Root root = inverse_root(row_sum<G>(s, red), a.inv_K, a.eps);
       for (int i = t; i < vecs; i += G) {
-        float v[16], lo[16];
-        take(i * 16, v, lo);
-        write_norm<T, FMT, ALIGNED>(a, row, i * 16, v, lo, root);
+        uint64_t h[8];
+        float lo[16];
+        take(i * 16, h, lo);
+        write_norm<T, FMT>(a, row, i * 16, h, lo, root);
       }
+    }
+  }
+}
+
+// Rows at any address: a column a lane, a block a warp's.  G threads take a row, J blocks each warp (0: rows of any length, read twice).
+template <typename T, int FMT, int G, int J>
+__global__ void __launch_bounds__(G > kThreads ? G : kThreads) mx_norm_any_kernel(const NormArgs a) {
+  constexpr int THREADS = G > kThreads ? G : kThreads, per = THREADS / G, F32 = sizeof(T) == 4;
+  __shared__ double red[32];
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, w0 = (threadIdx.x % G) >> 5, blocks = a.pieces * 4;
+  const bool sum = a.r != nullptr;
+  for (long long first = (long long)blockIdx.x * per; first < a.rows; first += (long long)gridDim.x * per) {
+    const long long row = first + threadIdx.x / G;
+    const bool live = row < a.rows;
+    const T* x = reinterpret_cast<const T*>(a.x) + row * a.ldx;
+    const T* r = reinterpret_cast<const T*>(a.r) + row * a.ldr;
+    T* h_out = reinterpret_cast<T*>(a.h) + row * a.K;
+    auto take = [&](int k, float& h, float& lo) {
+      const bool there = live && k < a.K;
+      const float u = there ? load_one(x + k) : 0.f, v = there && sum ? load_one(r + k) : 0.f;
+      h = add_exact(u, v);
+      lo = F32 ? left_out(h, u, v) : 0.f;
+    };
+    auto give = [&](int b, float h, float lo, const Root& root) {
+      const int k = b * 32 + lane;
+      const float w = k >= a.K ? 0.f : a.w_f32 ? load_one(reinterpret_cast<const float*>(a.w) + k) : load_one(reinterpret_cast<const T*>(a.w) + k);
+      float y = mul_exact(mul_exact(h, root.hi), w);
+      if (y != 0.f && from_border(y) <= kNear) y = to_odd(h, lo, root.hi, root.lo, w);
+      uint32_t byte;
+      const uint32_t code = quantize1<FMT>(y, byte);
+      store_byte<FMT>(a.data + row * a.row_bytes, k, a.row_bytes, byte);
+      if (lane == 0) a.scales[scale_word(row, b >> 2, a.pieces) + (b & 3)] = (uint8_t)code;
+    };
+    double s = 0.0;
+    if constexpr (J > 0) {
+      float h[J], lo[J], q = 0.f;
+#pragma unroll
+      for (int j = 0; j < J; j++) take((w0 + j * (G / 32)) * 32 + lane, h[j], lo[j]);
+#pragma unroll
+      for (int j = 0; j < J; j++) {
+        const int k = (w0 + j * (G / 32)) * 32 + lane;
+        if (sum && live && k < a.K) h_out[k] = to_type<T>(h[j]);
+        q = fma_exact(h[j], h[j], q);
+        if ((j & 7) == 7 || j == J - 1) {
+          s += (double)q;
+          q = 0.f;
+        }
+      }
+      const Root root = inverse_root(row_sum<G>(s, red), a.inv_K, a.eps);
+#pragma unroll
+      for (int j = 0; j < J; j++)
+        if (live && w0 + j * (G / 32) < blocks) give(w0 + j * (G / 32), h[j], lo[j], root);
+    } else {
+      for (int b = w0; b < blocks; b += G / 32) {
+        float h, lo;
+        take(b * 32 + lane, h, lo);
+        if (sum && live && b * 32 + lane < a.K) h_out[b * 32 + lane] = to_type<T>(h);
+        s += (double)mul_exact(h, h);
+      }
+      const Root root = inverse_root(row_sum<G>(s, red), a.inv_K, a.eps);
+      if (live)
+        for (int b = w0; b < blocks; b += G / 32) {
+          float h, lo;
+          take(b * 32 + lane, h, lo);
+          give(b, h, lo, root);
+        }
     }
   }
 }
@@ -524,29 +723,37 @@ unsigned grid_of(long long units, int per_block, int blocks_per_sm) {
 bool aligned_rows(const void* p, long long ld, long long K, int size) { return ((uintptr_t)p & 15) == 0 && ld * size % 16 == 0 && K % 8 == 0; }
 bool wide_rows(const void* p, long long ld, long long K, int size) { return ((uintptr_t)p & 31) == 0 && ld * size % 32 == 0 && K % 16 == 0; }
 
-template <typename T, int FMT, bool ALIGNED>
-int norm_launch(const NormArgs& a, cudaStream_t st) {
-  const int vecs = a.pieces * 8;
+template <typename T, int FMT>
+int norm_launch(const NormArgs& a, bool aligned, cudaStream_t st) {
+  const int vecs = a.pieces * 8, blocks = a.pieces * 4;
   cudaError_t e = cudaSuccess;
   auto go = [&](auto kern, int G) {
     const int threads = G > kThreads ? G : kThreads, per = threads / G;
-    const long long blocks = ((long long)a.rows + per - 1) / per, most = 148LL * 8;
-    e = gbh::launch(kern, dim3((unsigned)(blocks < most ? blocks : most)), dim3(threads), 0, st, 1, a);
+    const long long ctas = ((long long)a.rows + per - 1) / per, most = 148LL * 8;
+    e = gbh::launch(kern, dim3((unsigned)(ctas < most ? ctas : most)), dim3(threads), 0, st, 1, a);
   };
-  if (a.rows <= 4 * 148 && vecs <= 512) {    // few rows: each over as many threads as it has vectors
-    if (vecs <= 32) go(mx_norm_kernel<T, FMT, 32, 1, ALIGNED>, 32);
-    else if (vecs <= 128) go(mx_norm_kernel<T, FMT, 128, 1, ALIGNED>, 128);
-    else go(mx_norm_kernel<T, FMT, 512, 1, ALIGNED>, 512);
-  } else if (vecs <= 16) go(mx_norm_kernel<T, FMT, 16, 1, ALIGNED>, 16);
-  else if (vecs <= 32) go(mx_norm_kernel<T, FMT, 16, 2, ALIGNED>, 16);
-  else if (vecs <= 48) go(mx_norm_kernel<T, FMT, 16, 3, ALIGNED>, 16);
-  else if (vecs <= 64) go(mx_norm_kernel<T, FMT, 32, 2, ALIGNED>, 32);
-  else if (vecs <= 96) go(mx_norm_kernel<T, FMT, 32, 3, ALIGNED>, 32);
-  else if (vecs <= 128) go(mx_norm_kernel<T, FMT, 64, 2, ALIGNED>, 64);
-  else if (vecs <= 256) go(mx_norm_kernel<T, FMT, 128, 2, ALIGNED>, 128);
-  else if (vecs <= 512) go(mx_norm_kernel<T, FMT, 256, 2, ALIGNED>, 256);
-  else if (vecs <= 1024) go(mx_norm_kernel<T, FMT, 512, 2, ALIGNED>, 512);
-  else go(mx_norm_kernel<T, FMT, 512, 0, ALIGNED>, 512);
+  if (!aligned) {
+    if (blocks <= 8) go(mx_norm_any_kernel<T, FMT, 32, 8>, 32);
+    else if (blocks <= 16) go(mx_norm_any_kernel<T, FMT, 64, 8>, 64);
+    else if (blocks <= 32) go(mx_norm_any_kernel<T, FMT, 128, 8>, 128);
+    else if (blocks <= 64) go(mx_norm_any_kernel<T, FMT, 256, 8>, 256);
+    else if (blocks <= 128) go(mx_norm_any_kernel<T, FMT, 512, 8>, 512);
+    else if (blocks <= 256) go(mx_norm_any_kernel<T, FMT, 1024, 8>, 1024);
+    else go(mx_norm_any_kernel<T, FMT, 1024, 0>, 1024);
+  } else if (a.rows <= 4 * 148 && vecs <= 512) {    // few rows: each over as many threads as it has vectors
+    if (vecs <= 32) go(mx_norm_kernel<T, FMT, 32, 1>, 32);
+    else if (vecs <= 128) go(mx_norm_kernel<T, FMT, 128, 1>, 128);
+    else go(mx_norm_kernel<T, FMT, 512, 1>, 512);
+  } else if (vecs <= 16) go(mx_norm_kernel<T, FMT, 16, 1>, 16);
+  else if (vecs <= 32) go(mx_norm_kernel<T, FMT, 16, 2>, 16);
+  else if (vecs <= 48) go(mx_norm_kernel<T, FMT, 16, 3>, 16);
+  else if (vecs <= 64) go(mx_norm_kernel<T, FMT, 32, 2>, 32);
+  else if (vecs <= 96) go(mx_norm_kernel<T, FMT, 32, 3>, 32);
+  else if (vecs <= 128) go(mx_norm_kernel<T, FMT, 64, 2>, 64);
+  else if (vecs <= 256) go(mx_norm_kernel<T, FMT, 128, 2>, 128);
+  else if (vecs <= 512) go(mx_norm_kernel<T, FMT, 256, 2>, 256);
+  else if (vecs <= 1024) go(mx_norm_kernel<T, FMT, 512, 2>, 512);
+  else go(mx_norm_kernel<T, FMT, 512, 0>, 512);
   GB_CUDA_OK(e);
   return gbh::E_OK;
 }
@@ -555,20 +762,17 @@ int norm_launch(const NormArgs& a, cudaStream_t st) {
 
 enum { DT_BF16 = 0, DT_F16 = 1, DT_F32 = 2 };
 
-// CALL with the type T, the format FMT and ALIGNED.
-#define GB_MX_PICK(TYPE, fmt, aligned, CALL)                                          \
-  {                                                                                   \
-    using T = TYPE;                                                                   \
-    if (fmt == FP8) { constexpr int FMT = FP8; GB_MX_PICK_ALIGNED(aligned, CALL) }    \
-    else { constexpr int FMT = FP4; GB_MX_PICK_ALIGNED(aligned, CALL) }               \
+// CALL with the type T and the format FMT.
+#define GB_MX_PICK(TYPE, fmt, CALL)                       \
+  {                                                       \
+    using T = TYPE;                                       \
+    if (fmt == FP8) { constexpr int FMT = FP8; CALL; }    \
+    else { constexpr int FMT = FP4; CALL; }               \
   }
-#define GB_MX_PICK_ALIGNED(aligned, CALL)                        \
-  if (aligned) { constexpr bool ALIGNED = true; CALL; }          \
-  else { constexpr bool ALIGNED = false; CALL; }
-#define GB_MX_DISPATCH(dtype, fmt, aligned, CALL)                        \
-  if (dtype == DT_BF16) GB_MX_PICK(__nv_bfloat16, fmt, aligned, CALL)    \
-  else if (dtype == DT_F16) GB_MX_PICK(__half, fmt, aligned, CALL)       \
-  else GB_MX_PICK(float, fmt, aligned, CALL)
+#define GB_MX_DISPATCH(dtype, fmt, CALL)                       \
+  if (dtype == DT_BF16) GB_MX_PICK(__nv_bfloat16, fmt, CALL)   \
+  else if (dtype == DT_F16) GB_MX_PICK(__half, fmt, CALL)      \
+  else GB_MX_PICK(float, fmt, CALL)
 
 // Bytes of a row of codes and of the scales of a matrix (fmt 0: MXFP8, 1: MXFP4).
 GB_EXPORT long long gb_mx_row_bytes(long long K, int fmt) { return K <= 0 || K > (1LL << 30) ? 0 : row_bytes((int)K, fmt); }
@@ -589,8 +793,9 @@ GB_EXPORT int gb_mx_quantize(int dtype, int fmt, const void* x, long long ld, vo
     QuantArgs a{(const uint8_t*)x + r0 * ld * size, (uint8_t*)data + r0 * RB, (uint8_t*)scales + r0 / 128 * P * 512, ld, (int)n, (int)K, P, RB,
                 wide_rows(x, ld, K, size), FastDiv((uint32_t)P), extent_of(x, rows, ld, K, size)};
     cudaError_t e = cudaSuccess;
-    auto go = [&](auto kern) { e = gbh::launch(kern, dim3(grid_of(n * P, kThreads / 8, 8)), dim3(kThreads), 0, (cudaStream_t)stream, 1, a); };
-    GB_MX_DISPATCH(dtype, fmt, aligned_rows(x, ld, K, size), go(mx_quantize_kernel<T, FMT, ALIGNED>))
+    const bool aligned = aligned_rows(x, ld, K, size);
+    auto go = [&](auto kern) { e = gbh::launch(kern, dim3(grid_of(n * P, aligned ? kThreads / 8 : kThreads / 32, 8)), dim3(kThreads), 0, (cudaStream_t)stream, 1, a); };
+    GB_MX_DISPATCH(dtype, fmt, aligned ? go(mx_quantize_kernel<T, FMT>) : go(mx_quantize_any_kernel<T, FMT>))
     GB_CUDA_OK(e);
   }
   return gbh::E_OK;
@@ -657,8 +862,9 @@ GB_EXPORT int gb_mx_dequantize(int dtype, int fmt, const void* data, const void*
     n = rows_at_once(rows - r0, P);
     DequantArgs a{(const uint8_t*)data + r0 * RB, (const uint8_t*)scales + r0 / 128 * P * 512, (uint8_t*)y + r0 * K * size, (int)n, (int)K, P, RB, wide_rows(y, K, K, size), FastDiv((uint32_t)P)};
     cudaError_t e = cudaSuccess;
-    auto go = [&](auto kern) { e = gbh::launch(kern, dim3(grid_of(n * P, kThreads / 8, 8)), dim3(kThreads), 0, (cudaStream_t)stream, 1, a); };
-    GB_MX_DISPATCH(dtype, fmt, aligned_rows(y, K, K, size), go(mx_dequantize_kernel<T, FMT, ALIGNED>))
+    const bool aligned = aligned_rows(y, K, K, size);
+    auto go = [&](auto kern) { e = gbh::launch(kern, dim3(grid_of(n * P, aligned ? kThreads / 8 : kThreads / 32, 8)), dim3(kThreads), 0, (cudaStream_t)stream, 1, a); };
+    GB_MX_DISPATCH(dtype, fmt, aligned ? go(mx_dequantize_kernel<T, FMT>) : go(mx_dequantize_any_kernel<T, FMT>))
     GB_CUDA_OK(e);
   }
   return gbh::E_OK;
@@ -679,6 +885,6 @@ GB_EXPORT int gb_mx_add_rms_norm(int dtype, int fmt, const void* x, long long ld
   const NormArgs a{x, r, w, h, (uint8_t*)data, (uint8_t*)scales, ldx, ldr, (int)rows, (int)K, pieces((int)K, fmt), row_bytes((int)K, fmt), w_f32, wide, eps, 1.0 / (double)K,
                    extent_of(x, rows, ldx, K, size), extent_of(r, rows, ldr, K, size), extent_of(w, 1, K, K, w_f32 ? 4 : size)};
   int rc = gbh::E_OK;
-  GB_MX_DISPATCH(dtype, fmt, aligned, (rc = norm_launch<T, FMT, ALIGNED>(a, (cudaStream_t)stream)))
+  GB_MX_DISPATCH(dtype, fmt, (rc = norm_launch<T, FMT>(a, aligned, (cudaStream_t)stream)))
   return rc;
 }
