@@ -12,6 +12,8 @@
 #pragma once
 #include "common.cuh"
 
+#include <type_traits>
+
 namespace gbmx {
 
 enum Format : int { FP8 = 0, FP4 = 1 };
@@ -28,6 +30,29 @@ __device__ __forceinline__ long long scale_word(long long row, int g, int P) {
 __device__ __forceinline__ float mul_exact(float a, float b) {
   float d;
   asm("mul.rn.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// Two numbers at a time.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ void parts_of(uint64_t p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
   return d;
 }
 
@@ -216,11 +241,56 @@ __device__ __forceinline__ void store16(T* row, int k, int K, bool wide, const f
     *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
-template <typename T>
-__device__ __forceinline__ T to_type(float v);
-template <> __device__ __forceinline__ float to_type<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half to_type<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 to_type<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+// Rows at any address, by way of shared memory: L lanes side by side hold 16 L consecutive columns, which come and go a column a lane and
+// step, so that loads and stores are of neighbours whatever they start on, and stand in shared memory as sixteen a lane, 16 bytes
+// between them (no bank is met twice).
+template <typename T, int L>
+struct Stage {
+  static constexpr int PITCH = 16 * sizeof(T) + 16, BYTES = L * PITCH;     // of a group of L lanes
+  using Bits = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
+  uint8_t* buf;
+  int lane;
+  unsigned mask;
+  // for a block's shared memory of THREADS / L groups
+  __device__ __forceinline__ explicit Stage(uint8_t* shared)
+      : buf(shared + threadIdx.x / L * BYTES), lane(threadIdx.x % L), mask(L == 32 ? 0xffffffffu : ((1u << L) - 1u) << (threadIdx.x & 31 & ~(L - 1))) {}
+  __device__ __forceinline__ uint8_t* at(int j) const { return buf + ((j * L + lane) >> 4) * PITCH + ((j * L + lane) & 15) * sizeof(T); }
+  // columns first + j L + lane of the group's row
+  static __device__ __forceinline__ void fetch(const T* row, int first, int K, int lane, Bits (&raw)[16]) {
+#pragma unroll
+    for (int j = 0; j < 16; j++) raw[j] = first + j * L + lane < K ? __ldg(reinterpret_cast<const Bits*>(row) + first + j * L + lane) : (Bits)0;
+  }
+  // into sixteen columns a lane, as load16 has them
+  __device__ __forceinline__ void turn(const Bits (&raw)[16], uint32_t (&w)[4 * Elem<T>::SZ]) const {
+    __syncwarp(mask);
+#pragma unroll
+    for (int j = 0; j < 16; j++) *reinterpret_cast<Bits*>(at(j)) = raw[j];
+    __syncwarp(mask);
+#pragma unroll
+    for (int i = 0; i < 4 * Elem<T>::SZ; i += 4) {
+      const uint4 u = *reinterpret_cast<const uint4*>(buf + lane * PITCH + i * 4);
+      w[i] = u.x; w[i + 1] = u.y; w[i + 2] = u.z; w[i + 3] = u.w;
+    }
+  }
+  // sixteen values a lane to the row's columns from `first` on
+  __device__ __forceinline__ void store(T* row, int first, int K, const float (&v)[16]) const {
+    __syncwarp(mask);
+#pragma unroll
+    for (int i = 0; i < 4 * Elem<T>::SZ; i += 4) {
+      uint32_t w[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        if constexpr (sizeof(T) == 4) w[k] = __float_as_uint(v[i + k]);
+        else w[k] = Elem<T>::pack(v[2 * (i + k)], v[2 * (i + k) + 1]);
+      }
+      *reinterpret_cast<uint4*>(buf + lane * PITCH + i * 4) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __syncwarp(mask);
+#pragma unroll
+    for (int j = 0; j < 16; j++)
+      if (first + j * L + lane < K) reinterpret_cast<Bits*>(row)[first + j * L + lane] = *reinterpret_cast<const Bits*>(at(j));
+  }
+};
 
 // Bits of the largest magnitude of sixteen elements.  16-bit magnitudes compare in pairs, as whole numbers.
 template <typename T>
@@ -252,10 +322,10 @@ template <int FMT>
 __device__ __forceinline__ uint32_t quantize16(const float (&v)[16], uint32_t amax, unsigned mask, int lane, uint32_t (&out)[4]) {
   amax = max(amax, __shfl_xor_sync(mask, amax, 1));
   const uint32_t code = scale_code(amax, FMT);
-  const float inv = scale_inverse(code);
+  const uint64_t inv = pair_of(scale_inverse(code), scale_inverse(code));
   float q[16];
 #pragma unroll
-  for (int i = 0; i < 16; i++) q[i] = mul_exact(v[i], inv);
+  for (int i = 0; i < 16; i += 2) parts_of(mul_pair(pair_of(v[i], v[i + 1]), inv), q[i], q[i + 1]);
   if (FMT == FP8) {
 #pragma unroll
     for (int i = 0; i < 4; i++) out[i] = e4m3x4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]);

@@ -24,29 +24,40 @@ struct QuantArgs {
   uint8_t* scales;
   long long ld;            // elements from row to row of x
   int rows, K, pieces, row_bytes, wide;
-  FastDiv by_pieces;
+  FastDiv by_units;
   Extent ext;
 };
 
-// A unit is 128 columns of a row; NU units of a lane are in flight.
-template <typename T, int FMT>
+// A unit is L / 8 times 128 columns of a row.  L = 0: aligned rows, eight lanes, NU units of a lane in flight.  Others (Stage): 32 lanes, or
+// eight of rows of up to 256.
+template <typename T, int FMT, int L>
 __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const QuantArgs a) {
-  constexpr int NU = Elem<T>::SZ == 2 ? 2 : 1;
+  constexpr int NU = Elem<T>::SZ == 2 && L == 0 ? 2 : 1, LANES = L ? L : 8;
+  __shared__ __align__(16) uint8_t shared[L ? kThreads / LANES * Stage<T, LANES>::BYTES : 16];
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31, l8 = threadIdx.x & 7;
+  const Stage<T, LANES> stage(shared);
+  const int lane = threadIdx.x & 31;
   const unsigned mask = 0xffu << (lane & 24);
-  const uint32_t units = (uint32_t)a.rows * (uint32_t)a.pieces, stride = gridDim.x * (kThreads / 8);
-  for (uint32_t u0 = blockIdx.x * (kThreads / 8) + (threadIdx.x >> 3); u0 < units; u0 += NU * stride) {
+  const uint32_t units = (uint32_t)a.rows * a.by_units.d, stride = gridDim.x * (kThreads / LANES);
+  for (uint32_t u0 = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES; u0 < units; u0 += NU * stride) {
     uint32_t w[NU][4 * Elem<T>::SZ];
     uint32_t row[NU];
-    int g[NU];
+    int k[NU];
 #pragma unroll
     for (int i = 0; i < NU; i++) {
       const uint32_t u = min(u0 + i * stride, units - 1);
-      row[i] = a.by_pieces.div(u);
-      g[i] = (int)(u - row[i] * a.by_pieces.d);
-      load16<T, true>(reinterpret_cast<const T*>(a.x) + row[i] * a.ld, g[i] * 128 + l8 * 16, a.K, a.wide, a.ext, w[i]);
+      row[i] = a.by_units.div(u);
+      const int first = (int)(u - row[i] * a.by_units.d) * (16 * LANES);
+      k[i] = first + stage.lane * 16;
+      const T* x = reinterpret_cast<const T*>(a.x) + row[i] * a.ld;
+      if constexpr (L == 0) {
+        load16<T, true>(x, k[i], a.K, a.wide, a.ext, w[i]);
+      } else {
+        typename Stage<T, LANES>::Bits raw[16];
+        stage.fetch(x, first, a.K, stage.lane, raw);
+        stage.turn(raw, w[i]);
+      }
     }
 #pragma unroll
     for (int i = 0; i < NU; i++) {
@@ -55,60 +66,9 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const QuantArgs a
       unpack16<T>(w[i], v);
       uint32_t out[4];
       const uint32_t word = quantize16<FMT>(v, largest16<T>(w[i]), mask, lane, out);
-      store_codes<FMT>(a.data + (long long)row[i] * a.row_bytes, g[i] * 128 + l8 * 16, a.row_bytes, out);
-      if (l8 == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_word(row[i], g[i], a.pieces)) = word;
+      store_codes<FMT>(a.data + (long long)row[i] * a.row_bytes, k[i], a.row_bytes, out);
+      if ((lane & 7) == 0 && k[i] >> 7 < a.pieces) *reinterpret_cast<uint32_t*>(a.scales + scale_word(row[i], k[i] >> 7, a.pieces)) = word;
     }
-  }
-}
-
-// Rows at any address: a column a lane, so that every load and store is of neighbours whatever they start on, and a block is a warp's.
-__device__ __forceinline__ float load_one(const __nv_bfloat16* p) { return __uint_as_float((uint32_t)__ldg(reinterpret_cast<const uint16_t*>(p)) << 16); }
-__device__ __forceinline__ float load_one(const __half* p) { return __half2float(__ushort_as_half(__ldg(reinterpret_cast<const uint16_t*>(p)))); }
-__device__ __forceinline__ float load_one(const float* p) { return __uint_as_float(__ldg(reinterpret_cast<const uint32_t*>(p))); }
-
-// The code of a lane's value of a block: a byte of columns k (FP8), or of columns k and k + 1 for even lanes (FP4).  Returns the block's scale code.
-template <int FMT>
-__device__ __forceinline__ uint32_t quantize1(float v, uint32_t& byte) {
-  const uint32_t code = scale_code(__reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu), FMT);
-  const float q = mul_exact(v, scale_inverse(code));
-  if (FMT == FP8) {
-    byte = e4m3x4(q, 0.f, 0.f, 0.f);
-  } else {
-    const float two[8] = {q, __shfl_xor_sync(0xffffffffu, q, 1), 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    byte = e2m1x8(two);
-  }
-  return code;
-}
-template <int FMT>
-__device__ __forceinline__ void store_byte(uint8_t* row, int k, int row_bytes, uint32_t byte) {
-  const int b = FMT == FP8 ? k : k / 2;
-  if (b < row_bytes && (FMT == FP8 || (k & 1) == 0)) row[b] = (uint8_t)byte;
-}
-
-template <typename T, int FMT>
-__global__ void __launch_bounds__(kThreads) mx_quantize_any_kernel(const QuantArgs a) {
-  pdl_trigger();
-  pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const uint32_t units = (uint32_t)a.rows * (uint32_t)a.pieces, stride = gridDim.x * (kThreads / 32);
-  for (uint32_t u = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); u < units; u += stride) {
-    const uint32_t row = a.by_pieces.div(u);
-    const int g = (int)(u - row * a.by_pieces.d);
-    const T* x = reinterpret_cast<const T*>(a.x) + row * a.ld;
-    float v[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int k = g * 128 + i * 32 + lane;
-      v[i] = k < a.K ? load_one(x + k) : 0.f;
-    }
-    uint32_t word = 0;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      uint32_t byte;
-      word |= quantize1<FMT>(v[i], byte) << (8 * i);
-      store_byte<FMT>(a.data + (long long)row * a.row_bytes, g * 128 + i * 32 + lane, a.row_bytes, byte);
-    }
-    if (lane == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_word(row, g, a.pieces)) = word;
   }
 }
 
@@ -237,6 +197,12 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_both_kernel(const BothAr
   }
 }
 
+template <typename T>
+__device__ __forceinline__ T to_type(float v);
+template <> __device__ __forceinline__ float to_type<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half to_type<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 to_type<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
 // Sums over the pieces of rows that mx_quantize_both_kernel left, in fp32 and in one order: 32 columns a block, eight strips of pieces.
 template <typename T>
 __global__ void __launch_bounds__(256) mx_column_sum_kernel(const float* __restrict__ sums, T* __restrict__ out, int pieces, int K) {
@@ -266,7 +232,7 @@ struct DequantArgs {
   const uint8_t* scales;
   void* y;                 // rows x K, contiguous
   int rows, K, pieces, row_bytes, wide;
-  FastDiv by_pieces;
+  FastDiv by_units;
 };
 
 template <int FMT>
@@ -282,25 +248,28 @@ __device__ __forceinline__ void numbers16(const uint32_t (&c)[4], float (&v)[16]
   }
 }
 
-template <typename T, int FMT>
+// L: as in mx_quantize_kernel, for the rows of values.
+template <typename T, int FMT, int L>
 __global__ void __launch_bounds__(kThreads) mx_dequantize_kernel(const DequantArgs a) {
-  constexpr int NU = 2;
+  constexpr int NU = L == 0 ? 2 : 1, LANES = L ? L : 8;
+  __shared__ __align__(16) uint8_t shared[L ? kThreads / LANES * Stage<T, LANES>::BYTES : 16];
   pdl_trigger();
   pdl_wait();
-  const int l8 = threadIdx.x & 7;
-  const uint32_t units = (uint32_t)a.rows * (uint32_t)a.pieces, stride = gridDim.x * (kThreads / 8);
-  for (uint32_t u0 = blockIdx.x * (kThreads / 8) + (threadIdx.x >> 3); u0 < units; u0 += NU * stride) {
+  const Stage<T, LANES> stage(shared);
+  const uint32_t units = (uint32_t)a.rows * a.by_units.d, stride = gridDim.x * (kThreads / LANES);
+  for (uint32_t u0 = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES; u0 < units; u0 += NU * stride) {
     uint32_t c[NU][4], row[NU];
-    int g[NU];
+    int first[NU];
     uint8_t s[NU];
 #pragma unroll
     for (int i = 0; i < NU; i++) {
       const uint32_t u = min(u0 + i * stride, units - 1);
-      row[i] = a.by_pieces.div(u);
-      g[i] = (int)(u - row[i] * a.by_pieces.d);
-      const int k = g[i] * 128 + l8 * 16, b = FMT == FP8 ? k : k / 2;
+      row[i] = a.by_units.div(u);
+      first[i] = (int)(u - row[i] * a.by_units.d) * (16 * LANES);
+      const int k = first[i] + stage.lane * 16, b = FMT == FP8 ? k : k / 2;
       const uint8_t* from = a.data + (long long)row[i] * a.row_bytes + b;
       c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0;
+      s[i] = 0;
       if (b < a.row_bytes) {
         if (FMT == FP8) {
           const uint4 q = __ldg(reinterpret_cast<const uint4*>(from));
@@ -309,57 +278,20 @@ __global__ void __launch_bounds__(kThreads) mx_dequantize_kernel(const DequantAr
           const uint2 q = __ldg(reinterpret_cast<const uint2*>(from));
           c[i][0] = q.x; c[i][1] = q.y;
         }
+        s[i] = __ldg(a.scales + scale_word(row[i], k >> 7, a.pieces) + (k >> 5 & 3));
       }
-      s[i] = __ldg(a.scales + scale_word(row[i], g[i], a.pieces) + (l8 >> 1));
     }
 #pragma unroll
     for (int i = 0; i < NU; i++) {
       if (u0 + i * stride >= units) break;
       float v[16];
       numbers16<FMT>(c[i], v);
-      const float scale = scale_value(s[i]);
+      const uint64_t scale = pair_of(scale_value(s[i]), scale_value(s[i]));
 #pragma unroll
-      for (int j = 0; j < 16; j++) v[j] = mul_exact(v[j], scale);
-      store16(reinterpret_cast<T*>(a.y) + (long long)row[i] * a.K, g[i] * 128 + l8 * 16, a.K, a.wide, v);
-    }
-  }
-}
-
-// Rows of values at any address: a column a lane.
-template <typename T, int FMT>
-__global__ void __launch_bounds__(kThreads) mx_dequantize_any_kernel(const DequantArgs a) {
-  pdl_trigger();
-  pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const uint32_t units = (uint32_t)a.rows * (uint32_t)a.pieces, stride = gridDim.x * (kThreads / 32);
-  for (uint32_t u = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); u < units; u += stride) {
-    const uint32_t row = a.by_pieces.div(u);
-    const int g = (int)(u - row * a.by_pieces.d);
-    const uint8_t* from = a.data + (long long)row * a.row_bytes;
-    uint32_t c[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int k = g * 128 + i * 32 + lane;
-      c[i] = 0;
-      if (FMT == FP8) {
-        if (k < a.K) c[i] = __ldg(from + k);
-      } else if (k / 2 < a.row_bytes) {      // (the eight codes around a lane's: rows are padded to whole blocks)
-        c[i] = __ldg(reinterpret_cast<const uint32_t*>(from) + k / 8) >> (4 * (k & 7));
-      }
-    }
-    const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(a.scales + scale_word(row, g, a.pieces)));
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int k = g * 128 + i * 32 + lane;
-      float v;
-      if (FMT == FP8) {
-        uint32_t h;
-        asm("{\n.reg .b16 t;\ncvt.u16.u32 t, %1;\ncvt.rn.f16x2.e4m3x2 %0, t;\n}" : "=r"(h) : "r"(c[i]));
-        v = unpack_f16(h).x;
-      } else {                               // exponent and fraction stand as they do in fp32, 126 exponents below (one half of a converted pair came out 0)
-        v = mul_exact(__uint_as_float((c[i] & 7u) << 22 | (c[i] & 8u) << 28), 0x1p126f);
-      }
-      if (k < a.K) reinterpret_cast<T*>(a.y)[(long long)row * a.K + k] = to_type<T>(mul_exact(v, scale_value(word >> (8 * i) & 255u)));
+      for (int j = 0; j < 16; j += 2) parts_of(mul_pair(pair_of(v[j], v[j + 1]), scale), v[j], v[j + 1]);
+      T* to = reinterpret_cast<T*>(a.y) + (long long)row[i] * a.K;
+      if constexpr (L == 0) store16(to, first[i] + stage.lane * 16, a.K, a.wide, v);
+      else stage.store(to, first[i], a.K, v);
     }
   }
 }
@@ -380,7 +312,7 @@ struct NormArgs {
   Extent ex, er, ew;
 };
 
-// fp32 arithmetic that keeps subnormal numbers, alone and in pairs.
+// fp32 arithmetic that keeps subnormal numbers.
 __device__ __forceinline__ float add_exact(float a, float b) {
   float d;
   asm("add.rn.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
@@ -391,28 +323,6 @@ __device__ __forceinline__ float fma_exact(float a, float b, float c) {
   asm("fma.rn.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-__device__ __forceinline__ uint64_t pair_of(float a, float b) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ void parts_of(uint64_t p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
-__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-
 // 1 / sqrt(sum / K + eps) in two parts: the approximation and a step of Newton's iteration in fp64.
 struct Root {
   float hi, lo;
@@ -432,8 +342,8 @@ __device__ __forceinline__ Root inverse_root(double sum, double inv_K, double ep
 // a fraction (E4M3; E2M1 two), so the last 19 bits of a value in their neighbourhood are next to zero; four roundings move them by less
 // than eight.  Such values (one in 32 000; and zeros, infinities and NaN) are computed again, rounded to odd: the last bit stands for
 // all that lies behind it, so that the rounding to a code afterwards is that of the product itself.
-__device__ __forceinline__ uint32_t from_border(float y) { return (__float_as_uint(y) + 8u) & 0x7ffffu; }
-constexpr uint32_t kNear = 16;
+__device__ __forceinline__ uint32_t from_border(float y) { return __float_as_uint(y) * 8192u + 8u * 8192u; }      // (the last 19 bits and 8, above zeros)
+constexpr uint32_t kNear = 16u * 8192u;
 
 // h (hi + lo) * root * w, rounded to odd.
 __device__ __noinline__ float to_odd(float h, float lo, float root_hi, float root_lo, float w) {
@@ -496,15 +406,17 @@ __device__ __forceinline__ double squares(const uint64_t (&h)[8]) {
   return (double)a + (double)b;
 }
 
-template <typename T>
-__device__ __forceinline__ void write_sum(const NormArgs& a, long long row, int k, const uint64_t (&h)[8]) {
+template <typename T, bool ALIGNED, int L>
+__device__ __forceinline__ void write_sum(const NormArgs& a, long long row, int k, const uint64_t (&h)[8], const Stage<T, L>& stage) {
   float v[16];
 #pragma unroll
   for (int j = 0; j < 8; j++) parts_of(h[j], v[2 * j], v[2 * j + 1]);
-  store16(reinterpret_cast<T*>(a.h) + row * a.K, k, a.K, a.wide, v);
+  T* to = reinterpret_cast<T*>(a.h) + row * a.K;
+  if constexpr (ALIGNED) store16(to, k, a.K, a.wide, v);
+  else stage.store(to, k - stage.lane * 16, a.K, v);
 }
 
-template <typename T, int FMT>
+template <typename T, int FMT, bool ALIGNED>
 __device__ __forceinline__ void write_norm(const NormArgs& a, long long row, int k, const uint64_t (&h)[8], const float (&lo)[16], const Root& root) {
   float w[16], y[16];
   if (sizeof(T) == 2 && a.w_f32) {
@@ -513,7 +425,7 @@ __device__ __forceinline__ void write_norm(const NormArgs& a, long long row, int
     unpack16<float>(u, w);
   } else {                               // (a row's weights stand still while rows come and go: vectors from L1)
     uint32_t u[4 * Elem<T>::SZ];
-    load16<T, true>(reinterpret_cast<const T*>(a.w), k, a.K, false, a.ew, u);
+    load16<T, ALIGNED>(reinterpret_cast<const T*>(a.w), k, a.K, false, a.ew, u);
     unpack16<T>(u, w);
   }
   const uint64_t root2 = pair_of(root.hi, root.hi);
@@ -547,14 +459,16 @@ __device__ __forceinline__ void write_norm(const NormArgs& a, long long row, int
   if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_word(row, k >> 7, a.pieces)) = word;
 }
 
-// Aligned rows.  G threads of a block take a row, VPT vectors of sixteen columns each, which stay in registers between the two passes.  VPT = 0:
-// rows of any length, read a second time for their codes.
-template <typename T, int FMT, int G, int VPT>
+// G threads of a block take a row, VPT vectors of sixteen columns each, which stay in registers between the two passes.  VPT = 0: rows of any
+// length, read a second time for their codes.
+template <typename T, int FMT, int G, int VPT, bool ALIGNED>
 __global__ void __launch_bounds__(G > kThreads ? G : kThreads) mx_norm_kernel(const NormArgs a) {
-  constexpr int THREADS = G > kThreads ? G : kThreads, W = 4 * Elem<T>::SZ, F32 = sizeof(T) == 4;
+  constexpr int THREADS = G > kThreads ? G : kThreads, W = 4 * Elem<T>::SZ, F32 = sizeof(T) == 4, L = G < 32 ? G : 32;
   __shared__ double red[32];
+  __shared__ __align__(16) uint8_t shared[ALIGNED ? 16 : THREADS / L * Stage<T, L>::BYTES];
   pdl_trigger();
   pdl_wait();
+  const Stage<T, L> stage(shared);
   const int t = threadIdx.x % G;
   const int vecs = a.pieces * 8;                         // whole pieces: eight lanes work together
   const bool sum = a.r != nullptr;
@@ -568,7 +482,7 @@ __global__ void __launch_bounds__(G > kThreads ? G : kThreads) mx_norm_kernel(co
     if constexpr (VPT > 0) {
       uint64_t h[VPT][8];
       float lo[F32 ? VPT : 1][16];
-      {
+      if constexpr (ALIGNED) {
         uint32_t wx[VPT][W], wr[VPT][W];
 #pragma unroll
         for (int i = 0; i < VPT; i++) {
@@ -585,106 +499,63 @@ __global__ void __launch_bounds__(G > kThreads ? G : kThreads) mx_norm_kernel(co
           sum16<T>(wx[i], wr[i], h[i], lo[F32 ? i : 0]);     // (zeros without a residual)
           s += squares(h[i]);
         }
+      } else {
+        typename Stage<T, L>::Bits bx[VPT][16], br[VPT][16];
+#pragma unroll
+        for (int i = 0; i < VPT; i++) {
+          const int k = (t - stage.lane + i * G) * 16, K = live ? a.K : 0;
+          stage.fetch(x, k, K, stage.lane, bx[i]);
+          stage.fetch(r, k, sum ? K : 0, stage.lane, br[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < VPT; i++) {
+          uint32_t wx[W], wr[W];
+          stage.turn(bx[i], wx);
+          stage.turn(br[i], wr);
+          sum16<T>(wx, wr, h[i], lo[F32 ? i : 0]);
+          s += squares(h[i]);
+        }
       }
       if (sum && live) {
 #pragma unroll
-        for (int i = 0; i < VPT; i++) write_sum<T>(a, row, (t + i * G) * 16, h[i]);
+        for (int i = 0; i < VPT; i++) write_sum<T, ALIGNED, L>(a, row, (t + i * G) * 16, h[i], stage);
       }
       const Root root = inverse_root(row_sum<G>(s, red), a.inv_K, a.eps);
 #pragma unroll
       for (int i = 0; i < VPT; i++)
-        if (live && t + i * G < vecs) write_norm<T, FMT>(a, row, (t + i * G) * 16, h[i], lo[F32 ? i : 0], root);
+        if (live && t + i * G < vecs) write_norm<T, FMT, ALIGNED>(a, row, (t + i * G) * 16, h[i], lo[F32 ? i : 0], root);
     } else {
-      auto take = [&](int k, uint64_t (&h)[8], float (&lo)[16]) {
+      // (a row's threads take each step together, for the way through shared memory)
+      auto take = [&](int i, uint64_t (&h)[8], float (&lo)[16]) {
         uint32_t u[W], v[W];
-        load16<T, true>(x, k, a.K, a.wide, a.ex, u);
 #pragma unroll
         for (int j = 0; j < W; j++) v[j] = 0;
-        if (sum) load16<T, true>(r, k, a.K, a.wide, a.er, v);
+        if constexpr (ALIGNED) {
+          load16<T, true>(x, i * 16, a.K, a.wide, a.ex, u);
+          if (sum) load16<T, true>(r, i * 16, a.K, a.wide, a.er, v);
+        } else {
+          typename Stage<T, L>::Bits raw[16];
+          stage.fetch(x, (i - stage.lane) * 16, a.K, stage.lane, raw);
+          stage.turn(raw, u);
+          stage.fetch(r, (i - stage.lane) * 16, sum ? a.K : 0, stage.lane, raw);
+          stage.turn(raw, v);
+        }
         sum16<T>(u, v, h, lo);
       };
-      for (int i = t; i < vecs; i += G) {
+      for (int i = t; i - t < vecs; i += G) {
         uint64_t h[8];
         float lo[16];
-        take(i * 16, h, lo);
-        if (sum) write_sum<T>(a, row, i * 16, h);
+        take(i, h, lo);
+        if (sum) write_sum<T, ALIGNED, L>(a, row, i * 16, h, stage);
         s += squares(h);
       }
       const Root root = inverse_root(row_sum<G>(s, red), a.inv_K, a.eps);
-      for (int i = t; i < vecs; i += G) {
+      for (int i = t; i - t < vecs; i += G) {
         uint64_t h[8];
         float lo[16];
-        take(i * 16, h, lo);
-        write_norm<T, FMT>(a, row, i * 16, h, lo, root);
+        take(i, h, lo);
+        if (i < vecs) write_norm<T, FMT, ALIGNED>(a, row, i * 16, h, lo, root);
       }
-    }
-  }
-}
-
-// Rows at any address: a column a lane, a block a warp's.  G threads take a row, J blocks each warp (0: rows of any length, read twice).
-template <typename T, int FMT, int G, int J>
-__global__ void __launch_bounds__(G > kThreads ? G : kThreads) mx_norm_any_kernel(const NormArgs a) {
-  constexpr int THREADS = G > kThreads ? G : kThreads, per = THREADS / G, F32 = sizeof(T) == 4;
-  __shared__ double red[32];
-  pdl_trigger();
-  pdl_wait();
-  const int lane = threadIdx.x & 31, w0 = (threadIdx.x % G) >> 5, blocks = a.pieces * 4;
-  const bool sum = a.r != nullptr;
-  for (long long first = (long long)blockIdx.x * per; first < a.rows; first += (long long)gridDim.x * per) {
-    const long long row = first + threadIdx.x / G;
-    const bool live = row < a.rows;
-    const T* x = reinterpret_cast<const T*>(a.x) + row * a.ldx;
-    const T* r = reinterpret_cast<const T*>(a.r) + row * a.ldr;
-    T* h_out = reinterpret_cast<T*>(a.h) + row * a.K;
-    auto take = [&](int k, float& h, float& lo) {
-      const bool there = live && k < a.K;
-      const float u = there ? load_one(x + k) : 0.f, v = there && sum ? load_one(r + k) : 0.f;
-      h = add_exact(u, v);
-      lo = F32 ? left_out(h, u, v) : 0.f;
-    };
-    auto give = [&](int b, float h, float lo, const Root& root) {
-      const int k = b * 32 + lane;
-      const float w = k >= a.K ? 0.f : a.w_f32 ? load_one(reinterpret_cast<const float*>(a.w) + k) : load_one(reinterpret_cast<const T*>(a.w) + k);
-      float y = mul_exact(mul_exact(h, root.hi), w);
-      if (y != 0.f && from_border(y) <= kNear) y = to_odd(h, lo, root.hi, root.lo, w);
-      uint32_t byte;
-      const uint32_t code = quantize1<FMT>(y, byte);
-      store_byte<FMT>(a.data + row * a.row_bytes, k, a.row_bytes, byte);
-      if (lane == 0) a.scales[scale_word(row, b >> 2, a.pieces) + (b & 3)] = (uint8_t)code;
-    };
-    double s = 0.0;
-    if constexpr (J > 0) {
-      float h[J], lo[J], q = 0.f;
-#pragma unroll
-      for (int j = 0; j < J; j++) take((w0 + j * (G / 32)) * 32 + lane, h[j], lo[j]);
-#pragma unroll
-      for (int j = 0; j < J; j++) {
-        const int k = (w0 + j * (G / 32)) * 32 + lane;
-        if (sum && live && k < a.K) h_out[k] = to_type<T>(h[j]);
-        q = fma_exact(h[j], h[j], q);
-        if ((j & 7) == 7 || j == J - 1) {
-          s += (double)q;
-          q = 0.f;
-        }
-      }
-      const Root root = inverse_root(row_sum<G>(s, red), a.inv_K, a.eps);
-#pragma unroll
-      for (int j = 0; j < J; j++)
-        if (live && w0 + j * (G / 32) < blocks) give(w0 + j * (G / 32), h[j], lo[j], root);
-    } else {
-      for (int b = w0; b < blocks; b += G / 32) {
-        float h, lo;
-        take(b * 32 + lane, h, lo);
-        if (sum && live && b * 32 + lane < a.K) h_out[b * 32 + lane] = to_type<T>(h);
-        s += (double)mul_exact(h, h);
-      }
-      const Root root = inverse_root(row_sum<G>(s, red), a.inv_K, a.eps);
-      if (live)
-        for (int b = w0; b < blocks; b += G / 32) {
-          float h, lo;
-          take(b * 32 + lane, h, lo);
-          give(b, h, lo, root);
-        }
     }
   }
 }
@@ -725,7 +596,7 @@ bool wide_rows(const void* p, long long ld, long long K, int size) { return ((ui
 
 template <typename T, int FMT>
 int norm_launch(const NormArgs& a, bool aligned, cudaStream_t st) {
-  const int vecs = a.pieces * 8, blocks = a.pieces * 4;
+  const int vecs = a.pieces * 8;
   cudaError_t e = cudaSuccess;
   auto go = [&](auto kern, int G) {
     const int threads = G > kThreads ? G : kThreads, per = threads / G;
@@ -733,27 +604,27 @@ int norm_launch(const NormArgs& a, bool aligned, cudaStream_t st) {
     e = gbh::launch(kern, dim3((unsigned)(ctas < most ? ctas : most)), dim3(threads), 0, st, 1, a);
   };
   if (!aligned) {
-    if (blocks <= 8) go(mx_norm_any_kernel<T, FMT, 32, 8>, 32);
-    else if (blocks <= 16) go(mx_norm_any_kernel<T, FMT, 64, 8>, 64);
-    else if (blocks <= 32) go(mx_norm_any_kernel<T, FMT, 128, 8>, 128);
-    else if (blocks <= 64) go(mx_norm_any_kernel<T, FMT, 256, 8>, 256);
-    else if (blocks <= 128) go(mx_norm_any_kernel<T, FMT, 512, 8>, 512);
-    else if (blocks <= 256) go(mx_norm_any_kernel<T, FMT, 1024, 8>, 1024);
-    else go(mx_norm_any_kernel<T, FMT, 1024, 0>, 1024);
+    if (vecs <= 16) go(mx_norm_kernel<T, FMT, 16, 1, false>, 16);
+    else if (vecs <= 32) go(mx_norm_kernel<T, FMT, 32, 1, false>, 32);
+    else if (vecs <= 64) go(mx_norm_kernel<T, FMT, 64, 1, false>, 64);
+    else if (vecs <= 128) go(mx_norm_kernel<T, FMT, 128, 1, false>, 128);
+    else if (vecs <= 256) go(mx_norm_kernel<T, FMT, 256, 1, false>, 256);
+    else if (vecs <= 512) go(mx_norm_kernel<T, FMT, 512, 1, false>, 512);
+    else go(mx_norm_kernel<T, FMT, 512, 0, false>, 512);
   } else if (a.rows <= 4 * 148 && vecs <= 512) {    // few rows: each over as many threads as it has vectors
-    if (vecs <= 32) go(mx_norm_kernel<T, FMT, 32, 1>, 32);
-    else if (vecs <= 128) go(mx_norm_kernel<T, FMT, 128, 1>, 128);
-    else go(mx_norm_kernel<T, FMT, 512, 1>, 512);
-  } else if (vecs <= 16) go(mx_norm_kernel<T, FMT, 16, 1>, 16);
-  else if (vecs <= 32) go(mx_norm_kernel<T, FMT, 16, 2>, 16);
-  else if (vecs <= 48) go(mx_norm_kernel<T, FMT, 16, 3>, 16);
-  else if (vecs <= 64) go(mx_norm_kernel<T, FMT, 32, 2>, 32);
-  else if (vecs <= 96) go(mx_norm_kernel<T, FMT, 32, 3>, 32);
-  else if (vecs <= 128) go(mx_norm_kernel<T, FMT, 64, 2>, 64);
-  else if (vecs <= 256) go(mx_norm_kernel<T, FMT, 128, 2>, 128);
-  else if (vecs <= 512) go(mx_norm_kernel<T, FMT, 256, 2>, 256);
-  else if (vecs <= 1024) go(mx_norm_kernel<T, FMT, 512, 2>, 512);
-  else go(mx_norm_kernel<T, FMT, 512, 0>, 512);
+    if (vecs <= 32) go(mx_norm_kernel<T, FMT, 32, 1, true>, 32);
+    else if (vecs <= 128) go(mx_norm_kernel<T, FMT, 128, 1, true>, 128);
+    else go(mx_norm_kernel<T, FMT, 512, 1, true>, 512);
+  } else if (vecs <= 16) go(mx_norm_kernel<T, FMT, 16, 1, true>, 16);
+  else if (vecs <= 32) go(mx_norm_kernel<T, FMT, 16, 2, true>, 16);
+  else if (vecs <= 48) go(mx_norm_kernel<T, FMT, 16, 3, true>, 16);
+  else if (vecs <= 64) go(mx_norm_kernel<T, FMT, 32, 2, true>, 32);
+  else if (vecs <= 96) go(mx_norm_kernel<T, FMT, 32, 3, true>, 32);
+  else if (vecs <= 128) go(mx_norm_kernel<T, FMT, 64, 2, true>, 64);
+  else if (vecs <= 256) go(mx_norm_kernel<T, FMT, 128, 2, true>, 128);
+  else if (vecs <= 512) go(mx_norm_kernel<T, FMT, 256, 2, true>, 256);
+  else if (vecs <= 1024) go(mx_norm_kernel<T, FMT, 512, 2, true>, 512);
+  else go(mx_norm_kernel<T, FMT, 512, 0, true>, 512);
   GB_CUDA_OK(e);
   return gbh::E_OK;
 }
@@ -788,14 +659,14 @@ GB_EXPORT int gb_mx_quantize(int dtype, int fmt, const void* x, long long ld, vo
     return gbh::E_BAD_ARG;
   }
   const int P = pieces((int)K, fmt), RB = row_bytes((int)K, fmt), size = dtype == DT_F32 ? 4 : 2;
+  const int lanes = aligned_rows(x, ld, K, size) ? 0 : K <= 256 ? 8 : 32;
   for (long long r0 = 0, n; r0 < rows; r0 += n) {
     n = rows_at_once(rows - r0, P);
     QuantArgs a{(const uint8_t*)x + r0 * ld * size, (uint8_t*)data + r0 * RB, (uint8_t*)scales + r0 / 128 * P * 512, ld, (int)n, (int)K, P, RB,
-                wide_rows(x, ld, K, size), FastDiv((uint32_t)P), extent_of(x, rows, ld, K, size)};
+                wide_rows(x, ld, K, size), FastDiv((uint32_t)(lanes == 32 ? (P + 3) / 4 : P)), extent_of(x, rows, ld, K, size)};
     cudaError_t e = cudaSuccess;
-    const bool aligned = aligned_rows(x, ld, K, size);
-    auto go = [&](auto kern) { e = gbh::launch(kern, dim3(grid_of(n * P, aligned ? kThreads / 8 : kThreads / 32, 8)), dim3(kThreads), 0, (cudaStream_t)stream, 1, a); };
-    GB_MX_DISPATCH(dtype, fmt, aligned ? go(mx_quantize_kernel<T, FMT>) : go(mx_quantize_any_kernel<T, FMT>))
+    auto go = [&](auto kern) { e = gbh::launch(kern, dim3(grid_of(n * a.by_units.d, kThreads / (lanes ? lanes : 8), 8)), dim3(kThreads), 0, (cudaStream_t)stream, 1, a); };
+    GB_MX_DISPATCH(dtype, fmt, lanes == 0 ? go(mx_quantize_kernel<T, FMT, 0>) : lanes == 8 ? go(mx_quantize_kernel<T, FMT, 8>) : go(mx_quantize_kernel<T, FMT, 32>))
     GB_CUDA_OK(e);
   }
   return gbh::E_OK;
@@ -858,13 +729,14 @@ GB_EXPORT int gb_mx_dequantize(int dtype, int fmt, const void* data, const void*
     return gbh::E_BAD_ARG;
   }
   const int P = pieces((int)K, fmt), RB = row_bytes((int)K, fmt), size = dtype == DT_F32 ? 4 : 2;
+  const int lanes = aligned_rows(y, K, K, size) ? 0 : K <= 256 ? 8 : 32;
   for (long long r0 = 0, n; r0 < rows; r0 += n) {
     n = rows_at_once(rows - r0, P);
-    DequantArgs a{(const uint8_t*)data + r0 * RB, (const uint8_t*)scales + r0 / 128 * P * 512, (uint8_t*)y + r0 * K * size, (int)n, (int)K, P, RB, wide_rows(y, K, K, size), FastDiv((uint32_t)P)};
+    DequantArgs a{(const uint8_t*)data + r0 * RB, (const uint8_t*)scales + r0 / 128 * P * 512, (uint8_t*)y + r0 * K * size, (int)n, (int)K, P, RB, wide_rows(y, K, K, size),
+                  FastDiv((uint32_t)(lanes == 32 ? (P + 3) / 4 : P))};
     cudaError_t e = cudaSuccess;
-    const bool aligned = aligned_rows(y, K, K, size);
-    auto go = [&](auto kern) { e = gbh::launch(kern, dim3(grid_of(n * P, aligned ? kThreads / 8 : kThreads / 32, 8)), dim3(kThreads), 0, (cudaStream_t)stream, 1, a); };
-    GB_MX_DISPATCH(dtype, fmt, aligned ? go(mx_dequantize_kernel<T, FMT>) : go(mx_dequantize_any_kernel<T, FMT>))
+    auto go = [&](auto kern) { e = gbh::launch(kern, dim3(grid_of(n * a.by_units.d, kThreads / (lanes ? lanes : 8), 8)), dim3(kThreads), 0, (cudaStream_t)stream, 1, a); };
+    GB_MX_DISPATCH(dtype, fmt, lanes == 0 ? go(mx_dequantize_kernel<T, FMT, 0>) : lanes == 8 ? go(mx_dequantize_kernel<T, FMT, 8>) : go(mx_dequantize_kernel<T, FMT, 32>))
     GB_CUDA_OK(e);
   }
   return gbh::E_OK;
