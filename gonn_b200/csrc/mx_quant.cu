@@ -339,11 +339,15 @@ __device__ __forceinline__ Root inverse_root(double sum, double inv_K, double ep
 
 // A value next to the border between two codes has to fall on the side where it belongs: by three roundings of fp32 one in a million falls on
 // the other, a step of the code away.  Borders, and the powers of two at which a scale changes, have at most four leading bits of
-// a fraction (E4M3; E2M1 two), so the last 19 bits of a value in their neighbourhood are next to zero; four roundings move them by less
-// than eight.  Such values (one in 32 000; and zeros, infinities and NaN) are computed again, rounded to odd: the last bit stands for
-// all that lies behind it, so that the rounding to a code afterwards is that of the product itself.
-__device__ __forceinline__ uint32_t from_border(float y) { return __float_as_uint(y) * 8192u + 8u * 8192u; }      // (the last 19 bits and 8, above zeros)
-constexpr uint32_t kNear = 16u * 8192u;
+// a fraction (E4M3; E2M1 two), so the last 19 (21) bits of a value in their neighbourhood are next to zero; four roundings, of 2^-24
+// each, move them by four at most.  Such values (one in 50 000 or 200 000; and infinities and NaN) are computed again, rounded to odd:
+// the last bit stands for all that lies behind it, so that the rounding to a code afterwards is that of the product itself.
+template <int FMT>
+__device__ __forceinline__ uint32_t from_border(float y) {       // those bits and 5, above zeros
+  constexpr uint32_t shift = FMT == FP8 ? 1u << 13 : 1u << 11;
+  return __float_as_uint(y) * shift + 5u * shift;
+}
+template <int FMT> constexpr uint32_t kNear = 10u << (FMT == FP8 ? 13 : 11);
 
 // h (hi + lo) * root * w, rounded to odd.
 __device__ __noinline__ float to_odd(float h, float lo, float root_hi, float root_lo, float w) {
@@ -363,14 +367,14 @@ __device__ __forceinline__ float left_out(float h, float x, float r) {
   return fabsf(h) < 3e38f ? lo : 0.f;
 }
 
-template <int G, typename S>
-__device__ __forceinline__ double row_sum(double s, S* red) {
+// The sum over the G threads of a row: a half-warp, or whole warps (their sums in one order, the same for every thread).
+template <int G>
+__device__ __forceinline__ double row_sum(double s, double* red) {
 #pragma unroll
   for (int o = (G < 32 ? G : 32) / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (G <= 32) return s;
-  // the row's warps: their sums in one order, the same for every thread
-  const int warp = threadIdx.x >> 5, first = (threadIdx.x / G) * (G / 32);
-  if ((threadIdx.x & 31) == 0) red[warp] = s;
+  const int first = (int)threadIdx.x / G * (G / 32);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
   __syncthreads();
   s = 0.0;
 #pragma unroll
@@ -429,28 +433,28 @@ __device__ __forceinline__ void write_norm(const NormArgs& a, long long row, int
     unpack16<T>(u, w);
   }
   const uint64_t root2 = pair_of(root.hi, root.hi);
+  // for the test, zeros become a number far from any border (sums of bf16 values are zero now and then) and others stay what they are
+  const uint64_t tiny = pair_of(__uint_as_float(0x00955555u), __uint_as_float(0x00955555u));
   uint32_t near = ~0u;
   float m = 0.f;
 #pragma unroll
   for (int j = 0; j < 8; j++) {
-    parts_of(mul_pair(mul_pair(h[j], root2), pair_of(w[2 * j], w[2 * j + 1])), y[2 * j], y[2 * j + 1]);
-    near = min(near, min(from_border(y[2 * j]), from_border(y[2 * j + 1])));
+    const uint64_t p = mul_pair(h[j], root2), w2 = pair_of(w[2 * j], w[2 * j + 1]);
+    float a, b;
+    parts_of(fma_pair(p, w2, tiny), a, b);
+    near = min(near, min(from_border<FMT>(a), from_border<FMT>(b)));
+    parts_of(mul_pair(p, w2), y[2 * j], y[2 * j + 1]);
     m = fmaxf(fmaxf(m, fabsf(y[2 * j])), fabsf(y[2 * j + 1]));
   }
   uint32_t amax = __float_as_uint(m);    // (a flushed subnormal number has the same scale; infinities and NaN take the branch)
-  if (near <= kNear) {
-    bool again = false;                  // (zeros alone: no)
+  if (near <= kNear<FMT>) {
 #pragma unroll
-    for (int j = 0; j < 16; j++) again |= y[j] != 0.f && from_border(y[j]) <= kNear;
-    if (again) {
-#pragma unroll
-      for (int j = 0; j < 16; j++) {
-        float p, q;
-        parts_of(h[j / 2], p, q);
-        y[j] = to_odd(j & 1 ? q : p, sizeof(T) == 4 ? lo[j] : 0.f, root.hi, root.lo, w[j]);
-      }
-      amax = largest16(y);
+    for (int j = 0; j < 16; j++) {
+      float p, q;
+      parts_of(h[j / 2], p, q);
+      y[j] = to_odd(j & 1 ? q : p, sizeof(T) == 4 ? lo[j] : 0.f, root.hi, root.lo, w[j]);
     }
+    amax = largest16(y);
   }
   uint32_t out[4];
   const int lane = threadIdx.x & 31;
@@ -459,11 +463,18 @@ __device__ __forceinline__ void write_norm(const NormArgs& a, long long row, int
   if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_word(row, k >> 7, a.pieces)) = word;
 }
 
-// G threads of a block take a row, VPT vectors of sixteen columns each, which stay in registers between the two passes.  VPT = 0: rows of any
-// length, read a second time for their codes.
+// G threads of a block take a row (sixteen, or whole warps), VPT vectors of sixteen columns each, which stay in registers between the two
+// passes.  VPT = 0: rows of any length, read a second time for their codes.  BLOCKS: on an SM.  What counts is how many warps there are to
+// hide each other's latency: with 14 of 124 registers on an SM, three vectors each, 16384 x 2048 bf16 took 51 us, with 24 of 80 44; rows that
+// bulk copies brought to 16 warps ahead of time 69.
+constexpr int norm_threads(int G) { return G >= 256 ? G : 256 / G * G; }
+constexpr int norm_blocks(int size, int vpt, int G) {
+  return (vpt == 1 ? (size == 4 ? 768 : 1024) : vpt == 2 ? (size == 4 ? 512 : 768) : 512) / norm_threads(G);
+}
+
 template <typename T, int FMT, int G, int VPT, bool ALIGNED>
-__global__ void __launch_bounds__(G > kThreads ? G : kThreads) mx_norm_kernel(const NormArgs a) {
-  constexpr int THREADS = G > kThreads ? G : kThreads, W = 4 * Elem<T>::SZ, F32 = sizeof(T) == 4, L = G < 32 ? G : 32;
+__global__ void __launch_bounds__(norm_threads(G), norm_blocks(sizeof(T), VPT, G)) mx_norm_kernel(const NormArgs a) {
+  constexpr int THREADS = norm_threads(G), W = 4 * Elem<T>::SZ, F32 = sizeof(T) == 4, L = G < 32 ? G : 32, per = THREADS / G;
   __shared__ double red[32];
   __shared__ __align__(16) uint8_t shared[ALIGNED ? 16 : THREADS / L * Stage<T, L>::BYTES];
   pdl_trigger();
@@ -472,7 +483,6 @@ __global__ void __launch_bounds__(G > kThreads ? G : kThreads) mx_norm_kernel(co
   const int t = threadIdx.x % G;
   const int vecs = a.pieces * 8;                         // whole pieces: eight lanes work together
   const bool sum = a.r != nullptr;
-  constexpr int per = THREADS / G;
   for (long long first = (long long)blockIdx.x * per; first < a.rows; first += (long long)gridDim.x * per) {
     const long long row = first + threadIdx.x / G;
     const bool live = row < a.rows;
@@ -594,39 +604,32 @@ unsigned grid_of(long long units, int per_block, int blocks_per_sm) {
 bool aligned_rows(const void* p, long long ld, long long K, int size) { return ((uintptr_t)p & 15) == 0 && ld * size % 16 == 0 && K % 8 == 0; }
 bool wide_rows(const void* p, long long ld, long long K, int size) { return ((uintptr_t)p & 31) == 0 && ld * size % 32 == 0 && K % 16 == 0; }
 
-template <typename T, int FMT>
-int norm_launch(const NormArgs& a, bool aligned, cudaStream_t st) {
+// How a row of `vecs` vectors is dealt out: two to a thread, or one where that leaves fewer threads without.  Few rows: one, for the shortest way.
+template <typename T, int FMT, bool ALIGNED>
+cudaError_t norm_launch(const NormArgs& a, cudaStream_t st) {
   const int vecs = a.pieces * 8;
-  cudaError_t e = cudaSuccess;
   auto go = [&](auto kern, int G) {
-    const int threads = G > kThreads ? G : kThreads, per = threads / G;
+    const int threads = norm_threads(G), per = threads / G;
     const long long ctas = ((long long)a.rows + per - 1) / per, most = 148LL * 8;
-    e = gbh::launch(kern, dim3((unsigned)(ctas < most ? ctas : most)), dim3(threads), 0, st, 1, a);
+    return gbh::launch(kern, dim3((unsigned)(ctas < most ? ctas : most)), dim3(threads), 0, st, 1, a);
   };
-  if (!aligned) {
-    if (vecs <= 16) go(mx_norm_kernel<T, FMT, 16, 1, false>, 16);
-    else if (vecs <= 32) go(mx_norm_kernel<T, FMT, 32, 1, false>, 32);
-    else if (vecs <= 64) go(mx_norm_kernel<T, FMT, 64, 1, false>, 64);
-    else if (vecs <= 128) go(mx_norm_kernel<T, FMT, 128, 1, false>, 128);
-    else if (vecs <= 256) go(mx_norm_kernel<T, FMT, 256, 1, false>, 256);
-    else if (vecs <= 512) go(mx_norm_kernel<T, FMT, 512, 1, false>, 512);
-    else go(mx_norm_kernel<T, FMT, 512, 0, false>, 512);
-  } else if (a.rows <= 4 * 148 && vecs <= 512) {    // few rows: each over as many threads as it has vectors
-    if (vecs <= 32) go(mx_norm_kernel<T, FMT, 32, 1, true>, 32);
-    else if (vecs <= 128) go(mx_norm_kernel<T, FMT, 128, 1, true>, 128);
-    else go(mx_norm_kernel<T, FMT, 512, 1, true>, 512);
-  } else if (vecs <= 16) go(mx_norm_kernel<T, FMT, 16, 1, true>, 16);
-  else if (vecs <= 32) go(mx_norm_kernel<T, FMT, 16, 2, true>, 16);
-  else if (vecs <= 48) go(mx_norm_kernel<T, FMT, 16, 3, true>, 16);
-  else if (vecs <= 64) go(mx_norm_kernel<T, FMT, 32, 2, true>, 32);
-  else if (vecs <= 96) go(mx_norm_kernel<T, FMT, 32, 3, true>, 32);
-  else if (vecs <= 128) go(mx_norm_kernel<T, FMT, 64, 2, true>, 64);
-  else if (vecs <= 256) go(mx_norm_kernel<T, FMT, 128, 2, true>, 128);
-  else if (vecs <= 512) go(mx_norm_kernel<T, FMT, 256, 2, true>, 256);
-  else if (vecs <= 1024) go(mx_norm_kernel<T, FMT, 512, 2, true>, 512);
-  else go(mx_norm_kernel<T, FMT, 512, 0, true>, 512);
-  GB_CUDA_OK(e);
-  return gbh::E_OK;
+  if (vecs <= 16) return go(mx_norm_kernel<T, FMT, 16, 1, ALIGNED>, 16);
+  if constexpr (ALIGNED) {
+    if (a.rows > 4 * 148) {
+      if (vecs > 32 && vecs <= 64) return go(mx_norm_kernel<T, FMT, 32, 2, true>, 32);
+      if (vecs > 64 && vecs <= 128) return go(mx_norm_kernel<T, FMT, 64, 2, true>, 64);
+      if (vecs > 128 && vecs <= 192) return go(mx_norm_kernel<T, FMT, 96, 2, true>, 96);
+      if (vecs > 192 && vecs <= 256) return go(mx_norm_kernel<T, FMT, 128, 2, true>, 128);
+      if (vecs > 256 && vecs <= 512) return go(mx_norm_kernel<T, FMT, 256, 2, true>, 256);
+    }
+    if (vecs > 512 && vecs <= 1024) return go(mx_norm_kernel<T, FMT, 512, 2, true>, 512);
+  }
+  if (vecs <= 32) return go(mx_norm_kernel<T, FMT, 32, 1, ALIGNED>, 32);
+  if (vecs <= 64) return go(mx_norm_kernel<T, FMT, 64, 1, ALIGNED>, 64);
+  if (vecs <= 128) return go(mx_norm_kernel<T, FMT, 128, 1, ALIGNED>, 128);
+  if (vecs <= 256) return go(mx_norm_kernel<T, FMT, 256, 1, ALIGNED>, 256);
+  if (vecs <= 512) return go(mx_norm_kernel<T, FMT, 512, 1, ALIGNED>, 512);
+  return go(mx_norm_kernel<T, FMT, 512, 0, ALIGNED>, 512);
 }
 
 }  // namespace
@@ -756,7 +759,8 @@ GB_EXPORT int gb_mx_add_rms_norm(int dtype, int fmt, const void* x, long long ld
   const bool wide = wide_rows(x, ldx, K, size) && (r == nullptr || (wide_rows(r, ldr, K, size) && wide_rows(h, K, K, size)));
   const NormArgs a{x, r, w, h, (uint8_t*)data, (uint8_t*)scales, ldx, ldr, (int)rows, (int)K, pieces((int)K, fmt), row_bytes((int)K, fmt), w_f32, wide, eps, 1.0 / (double)K,
                    extent_of(x, rows, ldx, K, size), extent_of(r, rows, ldr, K, size), extent_of(w, 1, K, K, w_f32 ? 4 : size)};
-  int rc = gbh::E_OK;
-  GB_MX_DISPATCH(dtype, fmt, (rc = norm_launch<T, FMT>(a, aligned, (cudaStream_t)stream)))
-  return rc;
+  cudaError_t e = cudaSuccess;
+  GB_MX_DISPATCH(dtype, fmt, (e = aligned ? norm_launch<T, FMT, true>(a, (cudaStream_t)stream) : norm_launch<T, FMT, false>(a, (cudaStream_t)stream)))
+  GB_CUDA_OK(e);
+  return gbh::E_OK;
 }
