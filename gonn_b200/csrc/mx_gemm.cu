@@ -13,8 +13,8 @@
 #include "mx.cuh"
 
 #include <atomic>
+
 #include <string.h>
-#include <type_traits>
 
 using namespace gb;
 using namespace gbmx;
@@ -134,8 +134,10 @@ __device__ __forceinline__ void store32(uint32_t* to, bool wide, bool both, uint
 }
 
 // 32 x 32 results of a warp (a lane has a row) into C.  Rows on 32-byte boundaries: 32 bytes a lane and store, whole sectors straight from the
-// registers (an SM stores 32 bytes a clock in any case; by way of shared memory and whole lines a tile took longer: FIGURES).  Other rows,
-// a sector at a time, would write each sector many times: they go through `buf`, a column a lane.
+// registers (an SM stores 32 bytes a clock in any case; by way of shared memory and whole lines it took as long, 25.8 against 26.1 us at
+// 16384 x 2304 x 768 in MXFP4, and that took the room of the sixth stage).  Other rows,
+// a sector at a time, would write each sector many times: they go through `buf`, a column a lane (which takes 72 us for the 31 of
+// vectors at 16384 x 2304 x 768 in MXFP8).
 template <bool VECTORS>
 __device__ __forceinline__ void store_chunk(const MxArgs& a, uint8_t* buf, int slice, int row0, int col0, const float (&v)[32]) {
   const int lane = threadIdx.x & 31;
@@ -320,7 +322,8 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     }
     __syncwarp();
   } else if (warp == 2 + C::EW) {
-    // the bias of the tiles' columns, a tile or two ahead (fetched where it is needed it kept the warps waiting: 16384 x 2304 x 768 52 us, so FIGURES)
+    // the bias of the tiles' columns, a tile or two ahead (fetched by the epilogue's warps before a tile's
+    // results it kept them waiting: 16384 x 2304 x 768 in MXFP8 37 us, so 32.4; without a bias 30.5)
     if (args.bias != nullptr) {
       int local = 0;
       for (int u = pair; u < units; u += pairs, local++) {
@@ -427,35 +430,49 @@ __device__ __forceinline__ void load_bulk(void* dst, const void* src, uint32_t b
 struct RowsArgs {
   const void* x;
   long long ld;
-  int K;
+  int K, aligned;          // rows on 16-byte boundaries, K a multiple of eight
   Extent ext;
 };
 
-// Codes and scales of one step's columns of the rows of x, from a warp into a stage's shared memory, in the order of the swizzle.
+// Codes and scales of one step's columns of the rows of x, from a warp into a stage's shared memory, in the order of the swizzle.  (With a
+// load in flight instead of four: 16 rows, 2048 -> 8192 in MXFP4, 10.7 against 8.6 us.)
 template <int FMT, typename X>
 __device__ __forceinline__ void stage_rows(const RowsArgs& x, int rows, int step, uint8_t* codes, uint8_t* scales) {
   constexpr int L = FMT == FP8 ? 8 : 16;                     // lanes of a row
+  constexpr int AT_ONCE = 32 / L, U = 4;                     // rows; and so many loads in flight
   const int lane = threadIdx.x & 31, l = lane % L, k = (step * L + l) * 16;
-  for (int r0 = 0; r0 < rows; r0 += 32 / L) {
-    const int r = r0 + lane / L;
-    uint32_t w[4 * Elem<X>::SZ];
+  for (int r0 = 0; r0 < rows; r0 += U * AT_ONCE) {
+    uint32_t w[U][4 * Elem<X>::SZ];
 #pragma unroll
-    for (int j = 0; j < 4 * Elem<X>::SZ; j++) w[j] = 0;
-    if (r < rows) load16<X, false>(reinterpret_cast<const X*>(x.x) + r * x.ld, k, x.K, false, x.ext, w);
-    float v[16];
-    unpack16<X>(w, v);
-    uint32_t c[4];
-    const uint32_t word = quantize16<FMT>(v, largest16<X>(w), 0xffu << (lane & 24), lane, c);
-    if (r >= rows) continue;
-    uint8_t* row = codes + r * 128;
-    if (FMT == FP8) *reinterpret_cast<uint4*>(row + ((l ^ (r & 7)) << 4)) = make_uint4(c[0], c[1], c[2], c[3]);
-    else *reinterpret_cast<uint2*>(row + ((l >> 1 ^ (r & 7)) << 4) + (l & 1) * 8) = make_uint2(c[0], c[1]);
-    if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(scales + (l >> 3) * 512 + r * 16) = word;
+    for (int i = 0; i < U; i++) {
+      const int r = r0 + i * AT_ONCE + lane / L;
+#pragma unroll
+      for (int j = 0; j < 4 * Elem<X>::SZ; j++) w[i][j] = 0;
+      if (r >= rows) continue;
+      const X* row = reinterpret_cast<const X*>(x.x) + r * x.ld;
+      if (x.aligned) load16<X, true>(row, k, x.K, false, x.ext, w[i]);
+      else load16<X, false>(row, k, x.K, false, x.ext, w[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < U; i++) {
+      if (r0 + i * AT_ONCE >= rows) break;
+      const int r = r0 + i * AT_ONCE + lane / L;
+      float v[16];
+      unpack16<X>(w[i], v);
+      uint32_t c[4];
+      const uint32_t word = quantize16<FMT>(v, largest16<X>(w[i]), 0xffu << (lane & 24), lane, c);
+      if (r >= rows) continue;
+      uint8_t* row = codes + r * 128;
+      if (FMT == FP8) *reinterpret_cast<uint4*>(row + ((l ^ (r & 7)) << 4)) = make_uint4(c[0], c[1], c[2], c[3]);
+      else *reinterpret_cast<uint2*>(row + ((l >> 1 ^ (r & 7)) << 4) + (l & 1) * 8) = make_uint2(c[0], c[1]);
+      if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(scales + (l >> 3) * 512 + r * 16) = word;
+    }
   }
 }
 
 // X: void, or the type of rows that come as they are (16 at most): the warps that wait for the results quantise them, each its steps, into the
-// ring.  Every CTA does so for its part of K, which costs less than a launch of their own: one token through 8192 -> 2048 in MXFP4, us, FIGURES.
+// ring.  Every CTA does so for its part of K.  As two kernels | so, bf16, us: 768 -> 2304 in MXFP8 1 row 5.2 | 4.2, 8 5.6 | 4.6, 16 6.0 | 5.8;
+// 2048 -> 8192 in MXFP4 1 row 6.0 | 5.0, 8 6.3 | 6.1, 16 6.7 | 8.6; of the host, 17 | 10.6 at any size, which is why the line is at 16.
 template <int FMT, int BN, typename X>
 __global__ void __launch_bounds__(ClusterCfg<FMT, BN>::THREADS, 2)
 mx_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const uint8_t* __restrict__ sA, const uint8_t* __restrict__ sB,
@@ -707,7 +724,9 @@ Choice best_pairs(long long M, long long N, long long tiles, int steps) {
   return c;
 }
 
-// Up to 64 rows run as clusters, without a workspace (pairs were the faster ones at none of the sizes above).
+// Up to 64 rows run as clusters, without a workspace (pairs were the faster ones at none of the sizes above).  A tile has as few rows of C as
+// hold them; with 128, us: 1 x 8192 x 2048 in MXFP4 6.9 instead of 5.0, 1 x 2048 x 8192 in MXFP8 7.1 instead of 6.4, 32 x 8192 x 2048 9.3 instead
+// of 7.9; from 16 to 60 rows of 2304 x 768 the same.
 Plan plan_of(long long M, long long N, long long K, int fmt) {
   Plan p{};
   p.steps = (int)((K + (fmt == FP8 ? 127 : 255)) / (fmt == FP8 ? 128 : 256));
@@ -735,6 +754,8 @@ int allow_shared(K kern, int bytes, std::atomic<uint32_t>& done) {
   if (dev < 32) done.fetch_or(1u << dev);
   return gbh::E_OK;
 }
+
+bool bad_operand(const void* p) { return p == nullptr || ((uintptr_t)p & 15) != 0; }
 
 struct Maps {
   CUtensorMap a, b, sa, sb;
@@ -809,9 +830,13 @@ GB_EXPORT int gb_mx_matmul(int fmt, const void* a, const void* sa, const void* b
     gbh::set_error("gb_mx_matmul: bad type %d, activation %d or row pitch %lld", out, act, ldc);
     return gbh::E_BAD_ARG;
   }
+  if (bad_operand(a) || bad_operand(sa) || bad_operand(b) || bad_operand(sb) || c == nullptr) {
+    gbh::set_error("gb_mx_matmul: codes and scales on 16-byte boundaries and a result are needed");
+    return gbh::E_BAD_ARG;
+  }
   const Plan p = plan_of(M, N, K, fmt);
-  if (p.workspace > 0 && (workspace == nullptr || workspace_bytes < p.workspace)) {
-    gbh::set_error("gb_mx_matmul: workspace of %lld bytes, %lld are needed", workspace_bytes, p.workspace);
+  if (p.workspace > 0 && (bad_operand(workspace) || workspace_bytes < p.workspace)) {
+    gbh::set_error("gb_mx_matmul: workspace of %lld bytes on a 16-byte boundary, %lld are needed", workspace_bytes, p.workspace);
     return gbh::E_BAD_ARG;
   }
   const int P = pieces((int)K, fmt), RB = row_bytes((int)K, fmt), per = fmt == FP8 ? 1 : 2;
@@ -872,6 +897,10 @@ GB_EXPORT int gb_mx_matmul_rows(int dtype, int fmt, const void* x, long long ld,
     gbh::set_error("gb_mx_matmul_rows: %lld rows (16 at most), types %d and %d, activation %d, row pitches %lld and %lld", M, dtype, out, act, ld, ldc);
     return gbh::E_BAD_ARG;
   }
+  if (x == nullptr || bad_operand(b) || bad_operand(sb) || c == nullptr) {
+    gbh::set_error("gb_mx_matmul_rows: rows, codes and scales on 16-byte boundaries and a result are needed");
+    return gbh::E_BAD_ARG;
+  }
   MxArgs args{};
   args.M = (int)M; args.N = (int)N;
   args.steps = (int)((K + (fmt == FP8 ? 127 : 255)) / (fmt == FP8 ? 128 : 256));
@@ -882,7 +911,7 @@ GB_EXPORT int gb_mx_matmul_rows(int dtype, int fmt, const void* x, long long ld,
   args.C = c; args.ldc = ldc; args.bias = bias; args.bias_f32 = bias_f32 || out == OUT_F32; args.act = act; args.out = out;
   args.status = gbh::status_ptr();
   const int size = dtype == 2 ? 4 : 2;
-  RowsArgs rows{x, ld, (int)K, {reinterpret_cast<uintptr_t>(x), reinterpret_cast<uintptr_t>(x) + (uintptr_t)(((M - 1) * ld + K) * size)}};
+  RowsArgs rows{x, ld, (int)K, ((uintptr_t)x & 15) == 0 && ld * size % 16 == 0 && K % 8 == 0, {reinterpret_cast<uintptr_t>(x), reinterpret_cast<uintptr_t>(x) + (uintptr_t)(((M - 1) * ld + K) * size)}};
   Maps tm;
   memset(&tm, 0, sizeof(tm));
   if (int rc = map_codes(&tm.a, b, N, row_bytes((int)K, fmt), 128)) return rc;

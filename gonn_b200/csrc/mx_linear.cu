@@ -126,6 +126,10 @@ GB_EXPORT int gb_mx_train_backward(int dtype, const void* dy, long long ld, cons
     gbh::set_error("gb_mx_train_backward: db comes with dw only");
     return gbh::E_BAD_ARG;
   }
+  if (kept == nullptr || ((uintptr_t)kept & 255)) {
+    gbh::set_error("gb_mx_train_backward: what the forward pass kept, on a 256-byte boundary, is needed");
+    return gbh::E_BAD_ARG;
+  }
   Carver c{(uint8_t*)scratch}, k{(uint8_t*)const_cast<void*>(kept)};
   const Packed g = c.packed(M, N, FP8), gt = c.packed(N, M, FP8);
   float* sums = (float*)c.bytes((M + 127) / 128 * N * 4);

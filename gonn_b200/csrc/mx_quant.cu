@@ -29,7 +29,8 @@ struct QuantArgs {
 };
 
 // A unit is L / 8 times 128 columns of a row.  L = 0: aligned rows, eight lanes, NU units of a lane in flight.  Others (Stage): 32 lanes, or
-// eight of rows of up to 256.
+// eight of rows of up to 256.  Directly | by way of Stage, us: 50304 x 2048 bf16 to MXFP4 44.5 | 63.6 (and back 48.3 | 58.1); eight lanes | 32, 40 M
+// values in rows of 33 117 | 294, 201 48 | 53, 257 57 | 45, 1003 46 | 29.
 template <typename T, int FMT, int L>
 __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const QuantArgs a) {
   constexpr int NU = Elem<T>::SZ == 2 && L == 0 ? 2 : 1, LANES = L ? L : 8;
@@ -577,13 +578,13 @@ Extent extent_of(const void* p, long long rows, long long ld, long long K, int s
   return e;
 }
 
-bool bad_shape(const char* what, long long rows, long long K, long long ld, int fmt, const void* data, const void* scales) {
+bool bad_shape(const char* what, const void* x, long long rows, long long K, long long ld, int fmt, const void* data, const void* scales) {
   if (rows <= 0 || K <= 0 || rows > 0x7fffffffLL || K > (1LL << 30) || ld < 0 || (fmt != FP8 && fmt != FP4)) {
     gbh::set_error("%s: bad extents %lld x %lld, row pitch %lld, format %d", what, rows, K, ld, fmt);
     return true;
   }
-  if (((uintptr_t)data & 15) || ((uintptr_t)scales & 15)) {
-    gbh::set_error("%s: codes and scales must be 16-byte aligned", what);
+  if (x == nullptr || data == nullptr || scales == nullptr || ((uintptr_t)data & 15) || ((uintptr_t)scales & 15)) {
+    gbh::set_error("%s: a tensor, and codes and scales on 16-byte boundaries are needed", what);
     return true;
   }
   return false;
@@ -604,7 +605,9 @@ unsigned grid_of(long long units, int per_block, int blocks_per_sm) {
 bool aligned_rows(const void* p, long long ld, long long K, int size) { return ((uintptr_t)p & 15) == 0 && ld * size % 16 == 0 && K % 8 == 0; }
 bool wide_rows(const void* p, long long ld, long long K, int size) { return ((uintptr_t)p & 31) == 0 && ld * size % 32 == 0 && K % 16 == 0; }
 
-// How a row of `vecs` vectors is dealt out: two to a thread, or one where that leaves fewer threads without.  Few rows: one, for the shortest way.
+// How a row of `vecs` vectors is dealt out: one to a thread, the shortest way, or two, which holds more in flight, for what does not stay in
+// L2.  One | two, bf16, us: 600 x 2048 4.0 | 5.2, 2400 x 2048 8.1 | 9.4, 8192 x 768 10.6 | 11.5, 2400 x 4096 13.6 | 13.7, 16384 x 768 21.5 | 19.1,
+// 16384 x 2048 44 | 43.5, 8192 x 8192 91 | 82; fp32, 8192 x 2048 42 | 42, 4096 x 8192 95 | 78.  Rows at any address: 16384 x 768 bf16 31, 16384 x 2048 66.
 template <typename T, int FMT, bool ALIGNED>
 cudaError_t norm_launch(const NormArgs& a, cudaStream_t st) {
   const int vecs = a.pieces * 8;
@@ -615,7 +618,7 @@ cudaError_t norm_launch(const NormArgs& a, cudaStream_t st) {
   };
   if (vecs <= 16) return go(mx_norm_kernel<T, FMT, 16, 1, ALIGNED>, 16);
   if constexpr (ALIGNED) {
-    if (a.rows > 4 * 148) {
+    if ((long long)a.rows * a.K > 9 << 20) {
       if (vecs > 32 && vecs <= 64) return go(mx_norm_kernel<T, FMT, 32, 2, true>, 32);
       if (vecs > 64 && vecs <= 128) return go(mx_norm_kernel<T, FMT, 64, 2, true>, 64);
       if (vecs > 128 && vecs <= 192) return go(mx_norm_kernel<T, FMT, 96, 2, true>, 96);
@@ -648,15 +651,9 @@ enum { DT_BF16 = 0, DT_F16 = 1, DT_F32 = 2 };
   else if (dtype == DT_F16) GB_MX_PICK(__half, fmt, CALL)      \
   else GB_MX_PICK(float, fmt, CALL)
 
-// Bytes of a row of codes and of the scales of a matrix (fmt 0: MXFP8, 1: MXFP4).
-GB_EXPORT long long gb_mx_row_bytes(long long K, int fmt) { return K <= 0 || K > (1LL << 30) ? 0 : row_bytes((int)K, fmt); }
-GB_EXPORT long long gb_mx_scale_bytes(long long rows, long long K, int fmt) {
-  return K <= 0 || K > (1LL << 30) ? 0 : (rows + 127) / 128 * pieces((int)K, fmt) * 512;
-}
-
 // Codes and scales of x (rows x K, rows `ld` elements apart).  The scales of rows up to the next multiple of 128 are left as they were.
 GB_EXPORT int gb_mx_quantize(int dtype, int fmt, const void* x, long long ld, void* data, void* scales, long long rows, long long K, void* stream) {
-  if (bad_shape("gb_mx_quantize", rows, K, ld, fmt, data, scales)) return gbh::E_BAD_ARG;
+  if (bad_shape("gb_mx_quantize", x, rows, K, ld, fmt, data, scales)) return gbh::E_BAD_ARG;
   if (dtype != DT_BF16 && dtype != DT_F16 && dtype != DT_F32) {
     gbh::set_error("gb_mx_quantize: unsupported dtype %d", dtype);
     return gbh::E_BAD_ARG;
@@ -679,12 +676,16 @@ GB_EXPORT int gb_mx_quantize(int dtype, int fmt, const void* x, long long ld, vo
 // fp32 scratch of (rows / 128, rounded up) x K, for the column sums of x in column_sums (of type sum_dtype).
 GB_EXPORT int gb_mx_quantize_both(int dtype, const void* x, long long ld, void* data, void* scales, void* data_t, void* scales_t, float* sums, void* column_sums,
                                   int sum_dtype, long long rows, long long K, void* stream) {
-  if (bad_shape("gb_mx_quantize_both", rows, K, ld, FP8, data, scales) || bad_shape("gb_mx_quantize_both", K, rows, ld, FP8, data_t, scales_t)) return gbh::E_BAD_ARG;
+  if (bad_shape("gb_mx_quantize_both", x, rows, K, ld, FP8, data, scales) || bad_shape("gb_mx_quantize_both", x, K, rows, ld, FP8, data_t, scales_t)) return gbh::E_BAD_ARG;
   const int P = pieces((int)K, FP8), PT = pieces((int)rows, FP8);
   const long long blocks = (long long)P * PT;
   if (blocks > 0x7fffffffLL) {
     gbh::set_error("gb_mx_quantize_both: %lld x %lld is too large", rows, K);
     return gbh::E_TOO_LARGE;
+  }
+  if (sums != nullptr && (column_sums == nullptr || sum_dtype < DT_BF16 || sum_dtype > DT_F32)) {
+    gbh::set_error("gb_mx_quantize_both: column sums of type %d", sum_dtype);
+    return gbh::E_BAD_ARG;
   }
   const int size = dtype == DT_F32 ? 4 : 2;
   const BothArgs a{x, (uint8_t*)data, (uint8_t*)scales, (uint8_t*)data_t, (uint8_t*)scales_t, ld, (int)rows, (int)K, P, row_bytes((int)K, FP8), PT,
@@ -716,17 +717,13 @@ GB_EXPORT int gb_mx_quantize_both(int dtype, const void* x, long long ld, void* 
   const dim3 grid((unsigned)((K + 31) / 32));
   if (sum_dtype == DT_BF16) GB_CUDA_OK(gbh::launch(mx_column_sum_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, 1, (const float*)sums, (__nv_bfloat16*)column_sums, PT, (int)K));
   else if (sum_dtype == DT_F16) GB_CUDA_OK(gbh::launch(mx_column_sum_kernel<__half>, grid, dim3(256), 0, st, 1, (const float*)sums, (__half*)column_sums, PT, (int)K));
-  else if (sum_dtype == DT_F32) GB_CUDA_OK(gbh::launch(mx_column_sum_kernel<float>, grid, dim3(256), 0, st, 1, (const float*)sums, (float*)column_sums, PT, (int)K));
-  else {
-    gbh::set_error("gb_mx_quantize_both: unsupported dtype %d of the sums", sum_dtype);
-    return gbh::E_BAD_ARG;
-  }
+  else GB_CUDA_OK(gbh::launch(mx_column_sum_kernel<float>, grid, dim3(256), 0, st, 1, (const float*)sums, (float*)column_sums, PT, (int)K));
   return gbh::E_OK;
 }
 
 // The values (rows x K, contiguous) that codes and scales stand for.
 GB_EXPORT int gb_mx_dequantize(int dtype, int fmt, const void* data, const void* scales, void* y, long long rows, long long K, void* stream) {
-  if (bad_shape("gb_mx_dequantize", rows, K, K, fmt, data, scales)) return gbh::E_BAD_ARG;
+  if (bad_shape("gb_mx_dequantize", y, rows, K, K, fmt, data, scales)) return gbh::E_BAD_ARG;
   if (dtype != DT_BF16 && dtype != DT_F16 && dtype != DT_F32) {
     gbh::set_error("gb_mx_dequantize: unsupported dtype %d", dtype);
     return gbh::E_BAD_ARG;
@@ -749,9 +746,13 @@ GB_EXPORT int gb_mx_dequantize(int dtype, int fmt, const void* data, const void*
 // elements apart; w in x's type, or fp32 (w_f32); h contiguous.
 GB_EXPORT int gb_mx_add_rms_norm(int dtype, int fmt, const void* x, long long ldx, const void* r, long long ldr, const void* w, int w_f32, void* h, void* data,
                                  void* scales, long long rows, long long K, double eps, void* stream) {
-  if (bad_shape("gb_mx_add_rms_norm", rows, K, ldx < ldr ? ldx : ldr, fmt, data, scales)) return gbh::E_BAD_ARG;
+  if (bad_shape("gb_mx_add_rms_norm", x, rows, K, ldx < ldr ? ldx : ldr, fmt, data, scales)) return gbh::E_BAD_ARG;
   if (dtype != DT_BF16 && dtype != DT_F16 && dtype != DT_F32) {
     gbh::set_error("gb_mx_add_rms_norm: unsupported dtype %d", dtype);
+    return gbh::E_BAD_ARG;
+  }
+  if (w == nullptr || (r != nullptr && h == nullptr)) {
+    gbh::set_error("gb_mx_add_rms_norm: a weight, and with a residual room for the sum are needed");
     return gbh::E_BAD_ARG;
   }
   const int size = dtype == DT_F32 ? 4 : 2;

@@ -26,6 +26,7 @@ from ..nn.module import Module
 from ..nn.norm import RMSNorm
 from ..ops.gemm import ACT, _act_ref
 from ..ops.linear import emit_grad, emit_vector_grad
+from ..ops.reduce import column_sum
 
 MXBlock = 32
 _FEW = 64                # rows up to which a product needs no workspace (gb_mx_plan)
@@ -268,8 +269,9 @@ def DequantizeMX(q: QTensorMX, dtype=torch.float32) -> torch.Tensor:
 def AddRMSNormMX(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-6,
                  format: str = "mxfp8") -> Tuple[QTensorMX, torch.Tensor]:
     """``h = x + residual`` and the quantised ``h / sqrt(mean(h^2) + eps) * weight``: what a pre-norm block hands to its next
-    products, and the stream that goes on beside them.  Returns (codes and scales, h); the norm takes the sum before it is rounded to
-    h's type, and no rounding of its own moves a value to another code.  Without a residual h is x itself."""
+    products, and the stream that goes on beside them.  Returns (codes and scales, h).  The norm takes the sum before it is rounded to
+    h's type; a value is rounded once, to its code, so that only the error of the mean (1e-8 or so of it) can move one that lies
+    between two codes to the other.  Squares are fp32: magnitudes from 1.8e19 on count as infinite.  Without a residual h is x itself."""
     fmt, shape = _format(format), tuple(x.shape)
     a = _rows(x, "AddRMSNormMX")
     rows, K = a.shape
@@ -439,7 +441,10 @@ class _TrainLinear(torch.autograd.Function):
                   0 if db is None else _TYPES[db.dtype], M, N, K, scratch.data_ptr(), n_scratch)
         # gradients go to their sinks last: a sink may start a step that rewrites the parameters
         if need_b:
-            db = emit_vector_grad(bias, g) if db is None else emit_grad(bias, db)
+            if db is None and bias.dtype in (g.dtype, torch.float32):
+                db = emit_vector_grad(bias, g)
+            else:                   # (summed beside dW's codes; or a bias of a type of its own)
+                db = emit_grad(bias, column_sum(g, out_dtype=torch.float32).to(bias.dtype) if db is None else db)
         if dw is not None:
             dw = emit_grad(weight, dw)
         return dx, dw, db
@@ -448,7 +453,8 @@ class _TrainLinear(torch.autograd.Function):
 def TrainLinearMX(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``Q(x) Q(W)^T + b`` in MXFP8 with gradients that go straight through the rounding; every product's operands are quantised
     along its contraction: dx = Q(dy) Q(W^T)^T, dW = Q(dy^T) Q(x^T)^T, db = column sums of dy.  For the backward pass the layer
-    keeps the codes of x^T and W^T, a byte a value."""
+    keeps the codes of x^T and W^T, a byte a value.  Into a CUDA graph, capture it with ``torch.autograd.grad`` or ``GraphedStep``
+    (``backward()`` adds to gradients on the stream that saw a parameter first, which a capture cannot follow)."""
     if weight.dim() != 2 or x.dim() == 0 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"TrainLinearMX: shapes {tuple(x.shape)} and {tuple(weight.shape)} do not match (..., K) and (N, K)")
     if weight.device != x.device:

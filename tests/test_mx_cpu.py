@@ -1,9 +1,12 @@
 """Microscaled formats on CPU tensors: the oracle against a plain restatement of the definition, layouts, refusals, layers."""
+import copy
 import math
+import pickle
 
 import pytest
 import torch
 
+from gonn_b200 import lib as _l
 from gonn_b200 import quant as Q
 from gonn_b200.nn import Linear, RMSNorm
 
@@ -229,3 +232,75 @@ def test_refusals():
         Q.TrainLinearMX(x, torch.zeros(8, 63))
     with pytest.raises(ValueError, match="activation"):
         Q.MXTrainLinear(Linear(4, 4, activation="relu"))
+
+
+A, ODD = 4096, 4104                   # addresses that are never read: on a 16-byte boundary, and not
+
+
+@pytest.mark.parametrize("name,args,what", [
+    ("gb_mx_quantize", (0, 0, None, 64, A, A, 4, 64, None), "needed"),
+    ("gb_mx_quantize", (0, 0, A, 64, ODD, A, 4, 64, None), "16-byte"),
+    ("gb_mx_quantize", (0, 0, A, 64, A, None, 4, 64, None), "needed"),
+    ("gb_mx_quantize", (3, 0, A, 64, A, A, 4, 64, None), "dtype"),
+    ("gb_mx_quantize", (0, 2, A, 64, A, A, 4, 64, None), "format"),
+    ("gb_mx_quantize", (0, 0, A, -1, A, A, 4, 64, None), "pitch"),
+    ("gb_mx_quantize", (0, 0, A, 64, A, A, 0, 64, None), "extents"),
+    ("gb_mx_quantize", (0, 0, A, 64, A, A, 4, (1 << 30) + 1, None), "extents"),
+    ("gb_mx_quantize_both", (0, A, 64, A, A, None, A, None, None, 0, 4, 64, None), "needed"),
+    ("gb_mx_quantize_both", (7, A, 64, A, A, A, A, None, None, 0, 4, 64, None), "dtype"),
+    ("gb_mx_quantize_both", (0, A, 64, A, A, A, A, A, None, 0, 4, 64, None), "column sums"),
+    ("gb_mx_quantize_both", (0, A, 64, A, A, A, A, A, A, 5, 4, 64, None), "column sums"),
+    ("gb_mx_dequantize", (0, 0, A, A, None, 4, 64, None), "needed"),
+    ("gb_mx_dequantize", (5, 0, A, A, A, 4, 64, None), "dtype"),
+    ("gb_mx_add_rms_norm", (0, 0, A, 64, None, 64, None, 0, None, A, A, 4, 64, 1e-6, None), "weight"),
+    ("gb_mx_add_rms_norm", (0, 0, A, 64, A, 64, A, 0, None, A, A, 4, 64, 1e-6, None), "room for the sum"),
+    ("gb_mx_matmul", (0, A, A, A, None, A, 8, None, 0, 4, 8, 64, 0, 0, None, 0, None), "boundaries"),
+    ("gb_mx_matmul", (0, A, A, A, ODD, A, 8, None, 0, 4, 8, 64, 0, 0, None, 0, None), "boundaries"),
+    ("gb_mx_matmul", (0, A, A, A, A, A, 7, None, 0, 4, 8, 64, 0, 0, None, 0, None), "pitch"),
+    ("gb_mx_matmul", (0, A, A, A, A, A, 8, None, 0, 4, 8, 64, 3, 0, None, 0, None), "type"),
+    ("gb_mx_matmul", (0, A, A, A, A, A, 8, None, 0, 4, 8, 64, 0, 4, None, 0, None), "activation"),
+    ("gb_mx_matmul", (0, A, A, A, A, A, 8, None, 0, 4, 0, 64, 0, 0, None, 0, None), "extents"),
+    ("gb_mx_matmul", (0, A, A, A, A, A, 768, None, 0, 2304, 768, 16384, 0, 0, None, 0, None), "workspace"),
+    ("gb_mx_matmul", (0, A, A, A, A, A, 768, None, 0, 2304, 768, 16384, 0, 0, ODD, 1 << 40, None), "workspace"),
+    ("gb_mx_matmul_rows", (0, 0, A, 64, A, A, A, 8, None, 0, 17, 8, 64, 0, 0, None), "16 at most"),
+    ("gb_mx_matmul_rows", (0, 0, None, 64, A, A, A, 8, None, 0, 4, 8, 64, 0, 0, None), "needed"),
+    ("gb_mx_linear", (0, 0, A, 64, A, A, A, None, 0, 40, 8, 64, 0, 0, None, 0, None), "scratch"),
+    ("gb_mx_linear", (0, 0, A, 64, A, A, A, None, 0, 0, 8, 64, 0, 0, None, 0, None), "extents"),
+    ("gb_mx_train_forward", (0, 0, A, 64, A, 64, A, None, 0, 4, 8, 64, 1, 1, A, 0, A, 1 << 30, None), "scratch"),
+    ("gb_mx_train_forward", (0, 0, A, 64, A, 64, A, None, 0, 4, 8, 1 << 31, 1, 1, A, 1 << 40, A, 1 << 40, None), "extents"),
+    ("gb_mx_train_backward", (0, A, 8, None, A, 0, A, 0, None, 0, 4, 8, 64, A, 1 << 30, None), "kept"),
+    ("gb_mx_train_backward", (0, A, 8, A, A, 0, None, 0, A, 0, 4, 8, 64, A, 1 << 30, None), "with dw only"),
+    ("gb_mx_tune", (3, 0), "kind"),
+])
+def test_native_refusals(name, args, what):
+    """Every entry of the library looks at its arguments before it touches a device."""
+    with pytest.raises(RuntimeError, match=what):
+        _l.check(getattr(_l.lib(), name)(*args), name)
+
+
+def test_copies_keep_their_values():
+    t = torch.randn(5, 70)
+    for q in (Q.QuantizeMX(t, "mxfp4"), Q.QTensorMX(*(lambda p: (p.Data, p.Scales, p.Format, p.Shape))(Q.QuantizeMX(t)))):
+        for other in (copy.copy(q), copy.deepcopy(q), pickle.loads(pickle.dumps(q))):
+            assert torch.equal(Q.DequantizeMX(other), Q.DequantizeMX(q)) and other.Shape == (5, 70) and other.Format == q.Format
+        assert q.Numel() == 350 and repr(q) == f"QTensorMX({q.Format}, (5, 70))"
+    with pytest.raises(AttributeError):
+        q.Shape = (70, 5)
+
+
+def test_a_layer_moves_and_keeps_its_codes():
+    m = Q.NewMXLinearFrom(Linear(40, 24), "mxfp4")
+    x = torch.randn(3, 40)
+    want = m(x)
+    again = copy.deepcopy(m).half()                   # codes and scales are bytes, whatever the layer's type
+    assert again.codes.dtype == torch.uint8 and again.bias.dtype == torch.float16
+    assert torch.equal(again.float().codes, m.codes) and torch.equal(copy.deepcopy(m)(x), want)
+
+
+@pytest.mark.parametrize("xt,wt,bt", [(torch.float32, torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32, torch.float32), (torch.float32, torch.bfloat16, torch.float32)])
+def test_train_linear_mixed_types(xt, wt, bt):
+    x, w, b = torch.randn(6, 40).to(xt).requires_grad_(), torch.randn(9, 40).to(wt).requires_grad_(), torch.randn(9).to(bt).requires_grad_()
+    y = Q.TrainLinearMX(x, w, b)
+    grads = torch.autograd.grad(y.sum(), (x, w, b))
+    assert y.dtype == xt and [g.dtype for g in grads] == [xt, wt, bt]
+    assert torch.equal(grads[2].float(), torch.full((9,), 6.0))

@@ -146,6 +146,22 @@ def test_norm(format, dtype, shape, residual, status_ok):
     nearly(cpu(q), y, 4 + chain / 2 + 12)
 
 
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("K", [520, 768, 2048, 2304, 4096, 8192])
+def test_norm_of_many_rows(format, dtype, K, status_ok):
+    """More than L2 keeps; a hundred of the rows are compared."""
+    rows = (9 << 20) // K + 7
+    x, r, w = torch.randn(rows, K, device=DEV).to(dtype), torch.randn(rows, K, device=DEV).to(dtype), (torch.rand(K, device=DEV) + 0.5).to(dtype)
+    q, h = Q.AddRMSNormMX(x, r, w, 1e-6, format)
+    assert torch.equal(h, (x.float() + r.float()).to(dtype))
+    some = torch.cat((torch.arange(0, rows, rows // 98)[:98], torch.tensor([rows - 2, rows - 1])))
+    total = x.cpu()[some].double() + r.cpu()[some].double()
+    y = total / torch.sqrt(total.square().mean(-1, keepdim=True) + 1e-6) * w.cpu().double()
+    part = Q.QTensorMX(q.Data.cpu()[some], Q.microscale._pack_scales(q.ScaleCodes().cpu()[some], int(format == "mxfp4")), format, (100, K))
+    nearly(part, y, 4 + 16 + 12)
+
+
 def cpu(q):
     return Q.QTensorMX(q.Data.cpu(), q.Scales.cpu(), q.Format, q.Shape)
 
@@ -444,3 +460,131 @@ def test_refusals_on_the_device(status_ok):
     off_by_one = torch.empty(q.Scales.numel() + 1, dtype=torch.uint8, device=DEV)[1:]
     with pytest.raises(ValueError, match="aligned"):
         Q.DequantizeMX(Q.QTensorMX(q.Data, off_by_one, "mxfp8", (4, 64)))
+
+
+def test_empty_on_the_device(status_ok):
+    w = Q.QuantizeMX(torch.randn(5, 40, device=DEV))
+    q = Q.QuantizeMX(torch.zeros(0, 40, device=DEV))
+    assert Q.DequantizeMX(q).shape == (0, 40) and q.Data.shape == (0, 64) and q.ScaleCodes().shape == (0, 2)
+    assert Q.MatMulMX(q, w).shape == (0, 5) and Q.LinearMX(torch.zeros(2, 0, 40, device=DEV), w).shape == (2, 0, 5)
+    assert Q.MatMulMX(w, q).shape == (5, 0)
+    n, h = Q.AddRMSNormMX(torch.zeros(0, 40, device=DEV), torch.zeros(0, 40, device=DEV), torch.ones(40, device=DEV))
+    assert h.shape == (0, 40) and n.Shape == (0, 40)
+    x, p, b = torch.zeros(0, 40, device=DEV, requires_grad=True), torch.randn(5, 40, device=DEV, requires_grad=True), torch.randn(5, device=DEV, requires_grad=True)
+    grads = torch.autograd.grad(Q.TrainLinearMX(x, p, b).sum(), (x, p, b))
+    assert [tuple(g.shape) for g in grads] == [(0, 40), (5, 40), (5,)] and not any(g.any() for g in grads)
+
+
+@pytest.mark.parametrize("xt,wt,bt", [(torch.float32, torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32, torch.float32),
+                                      (torch.float16, torch.bfloat16, torch.float64), (torch.float32, torch.float16, None)])
+@pytest.mark.parametrize("M", [7, 700])
+def test_train_linear_mixed_types_and_orders(xt, wt, bt, M, status_ok):
+    """Parameters in types of their own; x a slice, the weight a transpose, the gradient's rows one row.  Equal to the products by hand."""
+    N, K = 200, 300
+    x = torch.randn(M, 2 * K, device=DEV).to(xt)[:, 3:3 + K].requires_grad_()
+    w = torch.randn(K, N, device=DEV).to(wt).t().requires_grad_()
+    b = None if bt is None else torch.randn(N, device=DEV).to(bt).requires_grad_()
+    dy = torch.randn(1, N, device=DEV).to(xt).expand(M, N)
+    y = Q.TrainLinearMX(x, w, b)
+    leaves = [t for t in (x, w, b) if t is not None]
+    grads = torch.autograd.grad(y, leaves, dy)
+    q = Q.QuantizeMX
+    with torch.no_grad():
+        assert torch.equal(y, Q.MatMulMX(q(x), q(w), b, xt))
+        assert torch.equal(grads[0], Q.MatMulMX(q(dy), q(w.t()), None, xt)) and torch.equal(grads[1], Q.MatMulMX(q(dy.t()), q(x.t()), None, wt))
+    assert [(g.dtype, g.shape) for g in grads] == [(t.dtype, t.shape) for t in leaves]
+    if b is not None:
+        assert off(grads[2], dy.double().sum(0)) <= (M / 128 + 40) * 2.0 ** -24 + torch.finfo(grads[2].dtype).eps / 2
+
+
+@pytest.mark.parametrize("needs", [(True, False, False), (False, True, False), (False, False, True), (True, False, True), (False, True, True)])
+def test_train_linear_asks_for_what_is_needed(needs, status_ok):
+    t = [torch.randn(300, 128, device=DEV), torch.randn(64, 128, device=DEV), torch.randn(64, device=DEV)]
+    every = [v.clone().requires_grad_() for v in t]
+    some = [v.clone().requires_grad_(n) for v, n in zip(t, needs)]
+    dy = torch.randn(300, 64, device=DEV)
+    want = torch.autograd.grad(Q.TrainLinearMX(*every), every, dy)
+    y = Q.TrainLinearMX(*some)
+    for _ in range(2):                                 # a graph that is kept gives the same again
+        got = torch.autograd.grad(y, [v for v, n in zip(some, needs) if n], dy, retain_graph=True)
+        assert all(off(g, w.double()) <= 310 * 2.0 ** -24 for g, w in zip(got, [w for w, n in zip(want, needs) if n]))
+
+
+def test_two_graphs_replayed_at_once(status_ok):
+    """Captured training steps of their own buffers, on two streams at a time, give what each gives alone."""
+    torch.manual_seed(2)
+    steps = []
+    for N, K in ((768, 512), (520, 1000)):
+        x, dy = torch.randn(2000, K, device=DEV, dtype=torch.bfloat16), torch.randn(2000, N, device=DEV, dtype=torch.bfloat16)
+        w, b = torch.randn(N, K, device=DEV, dtype=torch.bfloat16, requires_grad=True), torch.randn(N, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+        wq = Q.QuantizeMX(w.detach(), "mxfp4")
+
+        def step(x=x, w=w, b=b, dy=dy, wq=wq):
+            y = Q.TrainLinearMX(x, w, b)
+            return (*torch.autograd.grad(y, (w, b), dy), y.detach(), Q.LinearMX(x, wq, b))
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            want = step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        steps.append((graph, out, want, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for graph, _, _, stream in steps:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, out, want, _ in steps:
+        assert all(torch.equal(a, c) for a, c in zip(out, want))
+
+
+def test_training_with_gradient_sinks(status_ok):
+    """A model of these layers under the data-parallel wrapper, whose flat buffers take the gradients: the first gradients are autograd's own,
+    and a captured step gives the same losses and parameters as one that runs eagerly."""
+    from gonn_b200 import nn
+    from gonn_b200.distributed.ddp import DistributedDataParallel
+    from gonn_b200.utils.graph import GraphedStep
+    x = torch.randn(5, 256, 96, device=DEV).bfloat16()
+
+    def model():
+        torch.manual_seed(4)
+        return nn.Sequential(*(Q.NewMXTrainLinearFrom(nn.Linear(i, o, dtype=torch.bfloat16, device=torch.device(DEV, 0))) for i, o in ((96, 200), (200, 64))))
+
+    def run(graph):
+        net = model()
+        ddp = DistributedDataParallel(net, optimizer=dict(kind="sgd", lr=1e-3))
+
+        def step(x):
+            out = net(x).float().square().mean()
+            out.backward()
+            ddp.step()
+            return out
+
+        if graph:
+            step = GraphedStep(step, ddp, (x[0],), warmup=2)
+        else:
+            step(x[0]), step(x[0])
+        losses = [float(step(v)) for v in x]
+        return losses, ddp.flat_params.clone()
+
+    (le, pe), (lg, pg) = run(False), run(True)
+    assert le == lg and torch.equal(pe, pg)
+    net = model()
+    net(x[0]).float().square().mean().backward()
+    assert all(p.grad is not None and p.grad.shape == p.shape and bool(p.grad.any()) for p in net.parameters())
+
+
+def test_layers_between_devices_and_files(status_ok, tmp_path):
+    m = Q.NewMXLinearFrom(Linear(100, 60), "mxfp4")
+    x = torch.randn(9, 100)
+    want = m(x)
+    m.to(DEV)
+    torch.save(m.state_dict(), tmp_path / "layer.pt")
+    other = Q.NewMXLinearFrom(Linear(100, 60), "mxfp4").to(DEV)
+    other.load_state_dict(torch.load(tmp_path / "layer.pt"))
+    assert torch.equal(other(x.to(DEV)), m(x.to(DEV)))
+    assert off(m(x.to(DEV)).cpu(), want.double()) <= (100 / 64 + 4) * 2.0 ** -23 + 2.0 ** -24
