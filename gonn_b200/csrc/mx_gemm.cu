@@ -404,12 +404,13 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
 
 // ---------------------------------------------------------------------------------------------------------------------------
 // Clusters.  The 128 rows of an instruction are rows of B (columns of C), so that a few rows of A cost no more of the tensor core
-// than they need.  A tile's rows of A start at a multiple of 128, as the scale pieces do.
+// than they need.  Where a tile's rows of A start within a scale piece, those of its 32, 64 or 96 first rows are turned to the front in
+// shared memory.
 // ---------------------------------------------------------------------------------------------------------------------------
 template <int FMT, int BN>
 struct ClusterCfg {
   // at most half of an SM's shared memory, so that the next kernel's CTAs set up beside this one's
-  static constexpr int STAGES = BN <= 32 ? 5 : BN == 64 ? 4 : 3, THREADS = BN >= 64 ? 320 : 192;     // (more hands for the results)
+  static constexpr int STAGES = BN <= 32 ? 5 : BN == 64 ? 4 : 3, THREADS = BN >= 32 ? 320 : 192;     // (more hands for the results)
   static constexpr int A_BYTES = 128 * 128, B_BYTES = BN * 128, TILE_BYTES = A_BYTES + B_BYTES;
   static constexpr int PIECE = 512, S_BYTES = 2 * Fmt<FMT>::PIECES * PIECE;
   static constexpr int OFF_SCALES = STAGES * TILE_BYTES;
@@ -489,15 +490,17 @@ mx_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
   }
   uint64_t* full = (uint64_t*)(smem + C::OFF_BARS);
   uint64_t* empty = full + C::STAGES;
-  uint64_t* done = empty + C::STAGES;
+  uint64_t* turned = empty + C::STAGES;        // the step's scales of rows of C start at its first row
+  uint64_t* done = turned + C::STAGES;
   uint32_t* slot = (uint32_t*)(done + 1);
   volatile int* abort_flag = (volatile int*)(slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int S = args.splits, tile = blockIdx.x / S, rank = blockIdx.x - tile * S;
   const int c0 = (tile % args.num_n) * 128, r0 = (tile / args.num_n) * BN;       // columns and rows of C
   const int k0 = rank * args.steps_per, k1 = min(args.steps, k0 + args.steps_per);
+  const int sub = r0 >> 5 & 3;                 // the tile's first 32 rows among the four of a scale piece
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::STAGES; s++) { mbar_init(&full[s], ROWS ? 2 : 1); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < C::STAGES; s++) { mbar_init(&full[s], ROWS ? 2 : 1); mbar_init(&empty[s], 1); mbar_init(&turned[s], 1); }
     mbar_init(done, 1);
     *abort_flag = 0;
     mbar_fence_init();
@@ -542,6 +545,7 @@ mx_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
       for (int k = k0, n = 0; k < k1; k++, n++) {
         const int stage = n % C::STAGES;
         if (!mbar_wait(&full[stage], (n / C::STAGES) & 1, abort_flag, args.status, ST_GEMM_TIMEOUT, 42)) break;
+        if (sub != 0 && !mbar_wait(&turned[stage], (n / C::STAGES) & 1, abort_flag, args.status, ST_GEMM_TIMEOUT, 43)) break;
         tc_fence_after();
         const uint32_t sa = smem_u32(smem + stage * C::TILE_BYTES), sb = sa + C::A_BYTES;
         const uint32_t ss = smem_u32(smem + C::OFF_SCALES + stage * C::S_BYTES);
@@ -566,6 +570,21 @@ mx_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&full[stage]);
+      }
+    }
+    if (!ROWS && sub != 0 && warp < 6) {       // the warps that wait for the results take turns
+      for (int k = k0 + warp - 2, i = warp - 2; k < k1; k += 4, i += 4) {
+        const int stage = i % C::STAGES;
+        if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], (i / C::STAGES) & 1, abort_flag, args.status, ST_GEMM_TIMEOUT, 46))) break;
+        uint4* s = reinterpret_cast<uint4*>(smem + C::OFF_SCALES + stage * C::S_BYTES + F::PIECES * C::PIECE);
+#pragma unroll
+        for (int p = 0; p < F::PIECES; p++) {
+          const uint4 v = s[p * 32 + lane];
+          s[p * 32 + lane] = sub == 1 ? make_uint4(v.y, v.z, v.w, v.x) : sub == 2 ? make_uint4(v.z, v.w, v.x, v.y) : make_uint4(v.w, v.x, v.y, v.z);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&turned[stage]);
       }
     }
     // the accumulator into the ring, transposed (every load has been consumed by then): rows of C of 128 fp32 columns
@@ -683,61 +702,66 @@ struct Plan {
   long long workspace;     // bytes: fp32 slices of a cut product of the pair kernel
 };
 
-thread_local int g_kind = 0, g_splits = 0;       // gb_mx_tune
+thread_local int g_kind = 0, g_rows = 0, g_splits = 0;       // gb_mx_tune
 
-// Microseconds that a product takes in either kernel, by what was measured of them.  A step takes 0.3 of either (an SM's 32 KB; or the 1.6 us
-// of a load over the 100 KB that a cluster's CTA has in flight).  Pairs: 4 for the launch, the first loads and the last results, 1.5 for a
-// tile's own, and for slices a second launch and their values' way through L2.  Clusters: 2.5 and what a tile's rows cost; from two CTAs
-// on the exchange, whose values the more CTAs share the way of, the longer they take.  us, measured | so, of 64 steps (MXFP8, N = 2048, K = 8192):
-//   clusters of 1, 2, 4, 8: 1 row 20.6, 12.4, 7.9, 6.2 | 20.4, 12.5, 8.1, 6.1; 64 rows 22.2, 14.5, 10.8, 13.3 | 21.6, 14.6, 11.2, 13.7;
-//   128 rows 23.0, 15.9, 13.9, 20.4 | 22.7, 16.7, 14.2, 23.7; 200 rows in clusters of 4 17.8 | 18.1;  pairs: 128 rows 23.6 | 24.7, 384 in 4 slices 16.5 | 15.9
-// and 2304 x 768 x 16384 as pairs in 1, 2, 5 slices 43.7, 32.7, 34.8 | 43.9, 30.7, 34.5; 1 x 2304 x 768 as clusters of 1, 2, 4 4.2, 4.4, 4.0 | 4.2, 4.4, 4.2.
+// Microseconds that a product takes in either kernel, by what was measured of them.  Pairs: a step takes 0.3 (an SM's 32 KB), 4 go by for the
+// launch, the first loads and the last results, 1.5 for a tile's own, and for slices a second launch and their values' way through L2.
+// Clusters: a step takes 0.33 (the 1.6 us of a load over the 100 KB that a CTA has in flight) and more where CTAs share an SM, a launch 2.45, each
+// of a tile's rows 0.026, the turning of scales 0.25; from two CTAs on the exchange, the longer the more CTAs share the way of its values;
+// CTAs beyond those that fit at a time a third more.  The fit is off by 6 % of 645 runs (root of the mean square), and what it chooses takes 1.7 %
+// longer than the best of them (geometric mean).  us, measured | so, MXFP8: 1 x 2048 x 8192 in clusters of 1, 2, 4, 8 20.6, 12.4, 7.9, 6.2 |
+// 23.6, 13.9, 9.0, 7.0; 128 x 2304 x 768 in tiles of 32, 64, 128 rows 5.6, 6.1, 7.7 | 5.5, 6.3, 7.8, as pairs 7.0 | 7.3; 512 x 2048 x 8192: 64 rows in
+// clusters of 2 18.4 | 19.4, 128 in 4 21.0 | 20.2, pairs in 1, 2, 4 slices 24.1, 20.1, 16.1 | 24.7, 19.7, 17.0; 2304 x 768 x 16384 as pairs in 1, 2, 5
+// slices 43.7, 32.7, 34.8 | 43.9, 30.7, 34.5.
 double pair_us(long long M, long long N, long long tiles, int steps, int splits) {
   const long long units = tiles * splits, waves = (units + 73) / 74;
   const int per = (steps + splits - 1) / splits;
   return 4.0 + waves * (per * 0.3 + 1.5) + (splits > 1 ? 2.5 + splits * 1e-6 * M * N : 0.0);
 }
 double cluster_us(long long M, int bn, long long tiles, int steps, int splits) {
-  const double ctas = (double)tiles * splits, rows = M < bn ? M : bn, waves = ctas > 296 ? ctas / 296 : 1.0;      // (two CTAs on an SM)
-  return 1.0 + waves * (1.5 + rows * 0.018) + (steps + splits - 1) / splits * 0.28 * (ctas > 148 ? ctas / 148 : 1.0) +
-         (splits > 1 ? 0.9 + 0.05 * splits + 0.0075 * splits * rows * (ctas > 64 ? ctas / 64 : 1.0) : 0.0);
+  const double ctas = (double)tiles * splits, rows = M < bn ? M : bn, load = ctas > 148 ? ctas / 148 - 1.0 : 0.0;      // (two CTAs on an SM)
+  const double once = 2.45 + 0.026 * rows + 0.65 * load + (steps + splits - 1) / splits * 0.33 * (1.0 + 0.19 * load) + (M > bn && bn < 128 ? 0.25 : 0.0) +
+                      (splits > 1 ? 0.56 + 0.16 * splits + 0.0033 * splits * rows * (ctas > 64 ? ctas / 64 : 1.0) : 0.0);
+  return once * (ctas > 296 ? 1.0 + 0.36 * (ceil(ctas / 296) - 1.0) : 1.0);
 }
 
 struct Choice {
-  int splits;
+  int rows, splits;
   double us;
 };
-Choice best_clusters(long long M, int bn, long long tiles, int steps) {
-  Choice c{0, 1e30};
-  for (int s = 1; s <= 8; s *= 2) {
-    if (g_splits ? s != (g_splits < 8 ? g_splits : 8) : (s > 1 && (s > steps || tiles * s > 296))) continue;
-    const double us = cluster_us(M, bn, tiles, steps, s);
-    if (us < c.us) c = {s, us};
+// Tiles of 16 rows for as many at most (scales of 32 rows stay together), else of 32, 64 or 128.
+Choice best_clusters(long long M, long long N, int steps) {
+  Choice c{0, 0, 1e300};
+  for (int bn = M <= 16 ? 16 : 32; bn <= (M <= 16 ? 16 : 128); bn *= 2) {
+    if (g_rows && M > 16 && bn != g_rows) continue;
+    const long long tiles = ((M + bn - 1) / bn) * ((N + 127) / 128);
+    for (int s = 1; s <= 8; s *= 2) {
+      if (g_splits ? s != (g_splits < 8 ? g_splits : 8) : (s > 1 && (s > steps || tiles * s > 296))) continue;
+      const double us = cluster_us(M, bn, tiles, steps, s);
+      if (us < c.us) c = {bn, s, us};
+    }
   }
-  if (c.splits == 0) c.splits = 1;       // (slices were asked for that there are not)
+  if (c.rows == 0) c = {g_rows && M > 16 ? g_rows : M <= 16 ? 16 : 128, 1, 1e300};       // (slices were asked for that there are not)
   return c;
 }
-Choice best_pairs(long long M, long long N, long long tiles, int steps) {
-  Choice c{1, pair_us(M, N, tiles, steps, 1)};
+Choice best_pairs(long long M, long long N, int steps) {
+  const long long tiles = ((M + 255) / 256) * ((N + 255) / 256);
+  Choice c{256, 1, pair_us(M, N, tiles, steps, 1)};
   for (int s = 2; s <= 8 && s <= steps && N % 4 == 0 && tiles < 74; s++)
-    if (g_splits ? s == g_splits : pair_us(M, N, tiles, steps, s) < c.us) c = {s, pair_us(M, N, tiles, steps, s)};
+    if (g_splits ? s == g_splits : pair_us(M, N, tiles, steps, s) < c.us) c = {256, s, pair_us(M, N, tiles, steps, s)};
   return c;
 }
 
-// Up to 64 rows run as clusters, without a workspace (pairs were the faster ones at none of the sizes above).  A tile has as few rows of C as
-// hold them; with 128, us: 1 x 8192 x 2048 in MXFP4 6.9 instead of 5.0, 1 x 2048 x 8192 in MXFP8 7.1 instead of 6.4, 32 x 8192 x 2048 9.3 instead
-// of 7.9; from 16 to 60 rows of 2304 x 768 the same.
+// Up to 64 rows run as clusters, without a workspace (pairs were the faster ones at none of the sizes above).
 Plan plan_of(long long M, long long N, long long K, int fmt) {
   Plan p{};
   p.steps = (int)((K + (fmt == FP8 ? 127 : 255)) / (fmt == FP8 ? 128 : 256));
-  p.bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-  const Choice pairs = best_pairs(M, N, ((M + 255) / 256) * ((N + 255) / 256), p.steps);
-  const Choice clusters = best_clusters(M, p.bn, ((M + p.bn - 1) / p.bn) * ((N + 127) / 128), p.steps);
+  const Choice pairs = best_pairs(M, N, p.steps), clusters = best_clusters(M, N, p.steps);
   p.pair = g_kind ? g_kind == 1 : M > 64 && pairs.us < clusters.us;
+  p.bn = p.pair ? 256 : clusters.rows;
   p.splits = p.pair ? pairs.splits : clusters.splits;
   p.steps_per = (p.steps + p.splits - 1) / p.splits;
   if (p.pair) {
-    p.bn = 256;
     p.splits = (p.steps + p.steps_per - 1) / p.steps_per;      // no empty slice
     p.workspace = p.splits > 1 ? M * N * 4 * p.splits : 0;
   }
@@ -795,13 +819,15 @@ int launch_cluster(const Maps& tm, const void* sa, const void* sb, const MxArgs&
 
 }  // namespace
 
-// The kernel of products from this thread: kind 0 by size, 1 pairs, 2 clusters; splits 0 by size, else that many slices of K.
+// The kernel of products from this thread: kind 0 by size, 1 pairs, 2 clusters, 32, 64 or 128 clusters with tiles of so many rows (above 16 rows
+// of C); splits 0 by size, else that many slices of K.
 GB_EXPORT int gb_mx_tune(int kind, int splits) {
-  if (kind < 0 || kind > 2 || splits < 0 || splits > 64) {
+  if (((kind < 0 || kind > 2) && kind != 32 && kind != 64 && kind != 128) || splits < 0 || splits > 64) {
     gbh::set_error("gb_mx_tune: kind %d, splits %d", kind, splits);
     return gbh::E_BAD_ARG;
   }
-  g_kind = kind;
+  g_kind = kind > 2 ? 2 : kind;
+  g_rows = kind > 2 ? kind : 0;
   g_splits = splits;
   return gbh::E_OK;
 }
@@ -906,7 +932,7 @@ GB_EXPORT int gb_mx_matmul_rows(int dtype, int fmt, const void* x, long long ld,
   args.steps = (int)((K + (fmt == FP8 ? 127 : 255)) / (fmt == FP8 ? 128 : 256));
   args.num_m = 1;
   args.num_n = (int)((N + 127) / 128);
-  args.splits = best_clusters(M, 16, args.num_n, args.steps).splits;
+  args.splits = best_clusters(M, N, args.steps).splits;
   args.steps_per = (args.steps + args.splits - 1) / args.splits;
   args.C = c; args.ldc = ldc; args.bias = bias; args.bias_f32 = bias_f32 || out == OUT_F32; args.act = act; args.out = out;
   args.status = gbh::status_ptr();

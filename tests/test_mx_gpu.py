@@ -329,10 +329,10 @@ def test_few_rows_are_quantised_within_the_product(format, dtype, M, N, K, statu
 
 
 @pytest.mark.parametrize("format", FORMATS)
-@pytest.mark.parametrize("kind", [1, 2])
+@pytest.mark.parametrize("kind", [1, 2, 32, 64, 128])
 @pytest.mark.parametrize("splits", [1, 2, 3, 5, 8])
 def test_every_way_of_a_product(format, kind, splits, status_ok):
-    """Either kernel with any number of slices of K gives the exact sums; slices that K does not have are none."""
+    """Either kernel with any number of slices of K, and tiles of any number of rows, give the exact sums; slices that K does not have are none."""
     for M, N, K in ((70, 264, 1500), (300, 512, 4100), (3, 40, 64), (520, 1032, 700)):
         _l.lib().gb_mx_tune(kind, splits)
         try:
