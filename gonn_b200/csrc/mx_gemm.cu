@@ -7,7 +7,7 @@
 // is written again once the step that read it has ended.
 //
 // Two kernels.  Pairs: a cluster of two CTAs per 256 x 256 tile (cta_group::2), persistent, for products with tiles enough to fill
-// the SMs.  Clusters: one tile of 128 columns of C (rows of B: the 128 rows of an instruction) by 16 to 128 rows of C per cluster of up to
+// the SMs, or two pairs per tile that share K.  Clusters: one tile of 128 columns of C (rows of B: the 128 rows of an instruction) by 16 to 128 rows of C per cluster of up to
 // eight CTAs, each of which takes a part of K; the parts meet in distributed shared memory in the order of the CTAs.
 #include "pair.cuh"
 #include "mx.cuh"
@@ -27,7 +27,7 @@ enum Out : int { OUT_BF16 = 0, OUT_F16 = 1, OUT_F32 = 2 };
 struct MxArgs {
   int M, N, steps;         // steps of the main loop over all of K
   int num_m, num_n;        // tiles
-  int splits, steps_per;   // slice s takes steps [s * steps_per, (s + 1) * steps_per)
+  int splits, steps_per;   // slice s of a tile takes steps [s * steps_per, (s + 1) * steps_per)
   void* C;                 // rows ldc elements apart
   long long ldc;
   const void* bias;        // N values in C's type, or fp32; null: none
@@ -139,9 +139,9 @@ __device__ __forceinline__ void store32(uint32_t* to, bool wide, bool both, uint
 // a sector at a time, would write each sector many times: they go through `buf`, a column a lane (which takes 72 us for the 31 of
 // vectors at 16384 x 2304 x 768 in MXFP8).
 template <bool VECTORS>
-__device__ __forceinline__ void store_chunk(const MxArgs& a, uint8_t* buf, int slice, int row0, int col0, const float (&v)[32]) {
+__device__ __forceinline__ void store_chunk(const MxArgs& a, uint8_t* buf, int row0, int col0, const float (&v)[32]) {
   const int lane = threadIdx.x & 31;
-  const long long first = (long long)slice * a.M + row0;
+  const long long first = row0;
   if constexpr (VECTORS) {
     if (row0 + lane >= a.M) return;
     const bool wide = a.vectors == 32;
@@ -193,7 +193,33 @@ __device__ __forceinline__ void store_chunk(const MxArgs& a, uint8_t* buf, int s
   }
 }
 
-template <int FMT, bool VECTORS>
+__device__ __forceinline__ uint32_t address_in(uint32_t smem, uint32_t rank) {      // of the CTA `rank` of the cluster
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem), "r"(rank));
+  return r;
+}
+
+// Bias, activation and 32 x 32 results of a warp into C; b: the columns' bias in shared memory.
+template <bool VECTORS>
+__device__ __forceinline__ void finish_chunk(const MxArgs& a, uint8_t* buf, int row0, int col0, const float* b, float (&v)[32]) {
+  if (a.bias != nullptr) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const float4 f = *reinterpret_cast<const float4*>(b + j);
+      v[j] += f.x; v[j + 1] += f.y; v[j + 2] += f.z; v[j + 3] += f.w;
+    }
+  }
+  if (a.act != ACT_NONE) {
+#pragma unroll
+    for (int j = 0; j < 32; j++) v[j] = activate(v[j], a.act);
+  }
+  store_chunk<VECTORS>(a, buf, row0, col0, v);
+}
+
+// SLICED: a tile per cluster of two pairs, each of which takes half of K; a pair finishes 128 of the columns, of which the other
+// sends it its sums through distributed shared memory.  (2304 x 768 x 16384 in MXFP8: 43.8 us whole, 32.3 as two slices that a second kernel
+// added, 28.6 so.  Four pairs were slower than clusters of smaller tiles wherever they fit: 256 x 2048 x 8192 15.7 against 14.6 us.)
+template <int FMT, bool VECTORS, bool SLICED>
 __global__ void __launch_bounds__(PairCfg<FMT>::THREADS, 1)
 mx_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmSA,
                const __grid_constant__ CUtensorMap tmSB, const MxArgs args) {
@@ -212,10 +238,14 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
   uint64_t* bias_empty = bias_full + 2;                      // [2]       per CTA
   uint32_t* slot = (uint32_t*)(bias_empty + 2);
   volatile int* abort_flag = (volatile int*)(slot + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t cta = cluster_ctarank();
-  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const int tiles = args.num_m * args.num_n, units = tiles * args.splits;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = warp & 3, half = (warp - 2) >> 2;      // (of the warps with the results)
+  uint8_t* buf = smem + C::OFF_OUT + (warp - 2) * C::OUT_BUF;
+  const uint32_t rank = cluster_ctarank(), cta = rank & 1;
+  constexpr int S = SLICED ? 2 : 1;
+  const int slice = SLICED ? (int)(rank >> 1) : 0, k0 = slice * args.steps_per, k1 = min(args.steps, k0 + args.steps_per);
+  const int tiles = args.num_m * args.num_n, pair = blockIdx.x / (2 * S), pairs = gridDim.x / (2 * S);      // (SLICED: one tile for each cluster)
+  const auto leaders = [&](uint32_t at) { return SLICED ? address_in(at, rank & ~1u) : at & ~kPeerBit; };   // an address in the pair's CTA 0, in its CTA 1
+  const auto peers = [&](uint32_t at) { return SLICED ? address_in(at, rank | 1u) : at | kPeerBit; };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; s++) {
@@ -252,18 +282,16 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int u = pair; u < units && ok; u += pairs) {
-        const int slice = u / tiles;
+      for (int u = pair; u < tiles && ok; u += pairs) {
         int mb, nb;
-        tile_at(u - slice * tiles, args.num_m, args.num_n, mb, nb);
+        tile_at(u, args.num_m, args.num_n, mb, nb);
         const int m0 = mb * 256 + (int)cta * 128, n0 = nb * 256 + (int)cta * 128;
-        const int k1 = min(args.steps, (slice + 1) * args.steps_per);
-        for (int k = slice * args.steps_per; k < k1; k++) {
+        for (int k = k0; k < k1; k++) {
           ok = mbar_wait(&empty[stage], phase ^ 1, abort_flag, args.status, ST_GEMM_TIMEOUT, 31);
           if (!ok) break;
           uint8_t* sa = smem + stage * C::TILE_BYTES;
           uint8_t* ss = smem + C::OFF_SCALES + stage * C::S_BYTES;
-          const uint32_t fb = smem_u32(&full[stage]) & ~kPeerBit;        // what lands in either CTA counts on the leader's barrier
+          const uint32_t fb = leaders(smem_u32(&full[stage]));        // what lands in either CTA counts on the leader's barrier
           if (cta == 0) mbar_expect_tx(&full[stage], 2 * (C::TILE_BYTES + C::S_BYTES));
           tma_load_3d_2sm(ss, &tmSA, fb, 0, k * F::PIECES, m0 >> 7);
           tma_load_3d_2sm(ss + F::PIECES * C::PIECE, &tmSB, fb, 0, k * F::PIECES, nb * 2);
@@ -281,14 +309,13 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     if (cta == 0 && elect_one()) {
       int n = 0, local = 0;              // steps and tiles so far
       bool ok = true;
-      for (int u = pair; u < units && ok; u += pairs, local++) {
+      for (int u = pair; u < tiles && ok; u += pairs, local++) {
         if (local > 0) {
           ok = mbar_wait(drained, (local - 1) & 1, abort_flag, args.status, ST_GEMM_TIMEOUT, 32);
           if (!ok) break;
           tc_fence_after();
         }
         const uint32_t acc = tmem + (local & 1) * C::ACC1;
-        const int slice = u / tiles, k0 = slice * args.steps_per, k1 = min(args.steps, k0 + args.steps_per);
         for (int k = k0; k < k1; k++, n++) {
           const int stage = n % C::STAGES;
           ok = mbar_wait(&full[stage], (n / C::STAGES) & 1, abort_flag, args.status, ST_GEMM_TIMEOUT, 33);
@@ -311,11 +338,11 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
                                scaled_idesc(F::ELEM, 256, 256, F::byte(i)), ta + 4 * F::piece(i), tb + 8 * F::piece(i), k > k0 || i != 0);
           const uint32_t eb = smem_u32(&empty[stage]);
           tc_commit_2sm(eb);
-          tc_commit_2sm(eb | kPeerBit);
+          tc_commit_2sm(peers(eb));
           if (k == k1 - 1) {
             const uint32_t rb = smem_u32(&ready[local & 1]);
             tc_commit_2sm(rb);
-            tc_commit_2sm(rb | kPeerBit);
+            tc_commit_2sm(peers(rb));
           }
         }
       }
@@ -326,10 +353,10 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     // results it kept them waiting: 16384 x 2304 x 768 in MXFP8 37 us, so 32.4; without a bias 30.5)
     if (args.bias != nullptr) {
       int local = 0;
-      for (int u = pair; u < units; u += pairs, local++) {
+      for (int u = pair; u < tiles; u += pairs, local++) {
         const int which = local & 1;
         int mb, nb;
-        tile_at(u % tiles, args.num_m, args.num_n, mb, nb);
+        tile_at(u, args.num_m, args.num_n, mb, nb);
         float f[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) f[i] = bias_at(args, nb * 256 + i * 32 + lane);
@@ -340,14 +367,12 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         if (lane == 0) mbar_arrive(&bias_full[which]);
       }
     }
-  } else {
-    const int q = warp & 3, half = (warp - 2) >> 2;
-    uint8_t* buf = smem + C::OFF_OUT + (warp - 2) * C::OUT_BUF;
+  } else if (!SLICED) {
     int local = 0;
-    for (int u = pair; u < units; u += pairs, local++) {
-      const int slice = u / tiles, which = local & 1;
+    for (int u = pair; u < tiles; u += pairs, local++) {
+      const int which = local & 1;
       int mb, nb;
-      tile_at(u - slice * tiles, args.num_m, args.num_n, mb, nb);
+      tile_at(u, args.num_m, args.num_n, mb, nb);
       const int row0 = mb * 256 + (int)cta * 128 + q * 32;
       if (args.bias != nullptr && !mbar_wait(&bias_full[which], (local >> 1) & 1, abort_flag, args.status, ST_GEMM_TIMEOUT, 36)) break;
       if (!mbar_wait(&ready[which], (local >> 1) & 1, abort_flag, args.status, ST_GEMM_TIMEOUT, 35)) break;
@@ -365,30 +390,66 @@ mx_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
           tmem_ld_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster_relaxed(smem_u32(drained) & ~kPeerBit);
+          if (lane == 0) mbar_arrive_cluster_relaxed(leaders(smem_u32(drained)));
         }
         const int col0 = nb * 256 + column(i);
         if (row0 >= args.M || col0 >= args.N) continue;
         float v[32];
 #pragma unroll
         for (int j = 0; j < 32; j++) v[j] = __uint_as_float(r[i & 1][j]);
-        if (args.bias != nullptr) {
-          const float* b = reinterpret_cast<const float*>(smem + C::OFF_BIAS) + which * 256 + column(i);
-#pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(b + j);
-            v[j] += f.x; v[j + 1] += f.y; v[j + 2] += f.z; v[j + 3] += f.w;
-          }
-        }
-        if (args.act != ACT_NONE) {
-#pragma unroll
-          for (int j = 0; j < 32; j++) v[j] = activate(v[j], args.act);
-        }
-        store_chunk<VECTORS>(args, buf, slice, row0, col0, v);
+        finish_chunk<VECTORS>(args, buf, row0, col0, reinterpret_cast<const float*>(smem + C::OFF_BIAS) + which * 256 + column(i), v);
       }
       if (args.bias != nullptr) {
         __syncwarp();
         if (lane == 0) mbar_arrive(&bias_empty[which]);
+      }
+    }
+  }
+  if constexpr (SLICED) {
+    constexpr int W = 256 / S;             // columns that a pair finishes
+    const bool works = warp >= 2 && warp < 2 + C::EW;
+    __syncwarp();
+    const bool ok = works && __all_sync(0xffffffffu, mbar_wait(&ready[0], 0, abort_flag, args.status, ST_GEMM_TIMEOUT, 38));
+    tc_fence_after();
+    __syncthreads();
+    cluster_sync_all();                    // the products of every pair have been taken: their rings are free
+    const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16);
+    // sums lie in the ring as [columns / 4][row of 128][4]
+    const auto at = [&](int c) { return (uint32_t)((c / 4 * 128 + q * 32 + lane) * 16); };
+    if (ok) {
+      const uint32_t to = address_in(smem_u32(smem), rank ^ 2);
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const int c = half * 64 + i * 32;
+        uint32_t r[32];
+        tmem_ld32(acc + (slice ^ 1) * W + c, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; j += 4)
+          asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + at(c + j)), "r"(r[j]), "r"(r[j + 1]), "r"(r[j + 2]), "r"(r[j + 3]) : "memory");
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();
+    if (ok) {
+      int mb, nb;
+      tile_at(pair, args.num_m, args.num_n, mb, nb);
+      const int row0 = mb * 256 + (int)cta * 128 + q * 32;
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const int c = half * 64 + i * 32;
+        uint32_t r[32];
+        tmem_ld32(acc + slice * W + c, r);
+        tmem_ld_wait();
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {      // (the same sum in either order)
+          const float4 f = *reinterpret_cast<const float4*>(smem + at(c + j));
+          v[j] = __uint_as_float(r[j]) + f.x; v[j + 1] = __uint_as_float(r[j + 1]) + f.y;
+          v[j + 2] = __uint_as_float(r[j + 2]) + f.z; v[j + 3] = __uint_as_float(r[j + 3]) + f.w;
+        }
+        const int col0 = nb * 256 + slice * W + c;
+        if (row0 < args.M && col0 < args.N) finish_chunk<VECTORS>(args, buf, row0, col0, reinterpret_cast<const float*>(smem + C::OFF_BIAS) + slice * W + c, v);
       }
     }
   }
@@ -664,59 +725,26 @@ mx_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
   if (S > 1) cluster_sync_all();   // nobody leaves while another may still read its shared memory
 }
 
-// Slices of a product cut along K, summed in their order: C = act(sum + bias).  Four columns a thread; N is a multiple of 4.
-__global__ void __launch_bounds__(256) mx_finish_kernel(const float* __restrict__ part, const MxArgs a, int slices, FastDiv by_quads) {
-  pdl_trigger();
-  pdl_wait();
-  const int quads = a.N / 4, size = a.out == OUT_F32 ? 4 : 2;
-  const long long total = (long long)a.M * a.N;
-  const bool vector = (((uintptr_t)a.C | (uintptr_t)(a.ldc * size)) & (4 * size - 1)) == 0;
-  for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < (uint32_t)a.M * (uint32_t)quads; i += gridDim.x * 256) {
-    const uint32_t row = by_quads.div(i);
-    const int c = (int)(i - row * by_quads.d) * 4;
-    const float4* from = reinterpret_cast<const float4*>(part) + i;
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int p = 0; p < slices; p++) {
-      const float4 u = __ldcs(from + p * (total / 4));
-      s.x += u.x; s.y += u.y; s.z += u.z; s.w += u.w;
-    }
-    const float y[4] = {activate(s.x + bias_at(a, c), a.act), activate(s.y + bias_at(a, c + 1), a.act), activate(s.z + bias_at(a, c + 2), a.act),
-                        activate(s.w + bias_at(a, c + 3), a.act)};
-    const long long to = row * a.ldc + c;
-    if (!vector) {
-      for (int j = 0; j < 4; j++) store_out(a, to + j, y[j]);
-    } else if (a.out == OUT_F32) {
-      *reinterpret_cast<float4*>((float*)a.C + to) = make_float4(y[0], y[1], y[2], y[3]);
-    } else {
-      *reinterpret_cast<uint2*>((uint16_t*)a.C + to) = make_uint2(pack_out(a, y[0], y[1]), pack_out(a, y[2], y[3]));
-    }
-  }
-}
-
 // ---------------------------------------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------------------------------------
 struct Plan {
   int pair, bn, splits, steps, steps_per;
-  long long workspace;     // bytes: fp32 slices of a cut product of the pair kernel
 };
 
 thread_local int g_kind = 0, g_rows = 0, g_splits = 0;       // gb_mx_tune
 
 // Microseconds that a product takes in either kernel, by what was measured of them.  Pairs: a step takes 0.3 (an SM's 32 KB), 4 go by for the
-// launch, the first loads and the last results, 1.5 for a tile's own, and for slices a second launch and their values' way through L2.
+// launch, the first loads and the last results, 1.5 for a tile's own; two slices exchange their sums, and 33 clusters of two pairs fit at a time.
 // Clusters: a step takes 0.33 (the 1.6 us of a load over the 100 KB that a CTA has in flight) and more where CTAs share an SM, a launch 2.45, each
 // of a tile's rows 0.026, the turning of scales 0.25; from two CTAs on the exchange, the longer the more CTAs share the way of its values;
 // CTAs beyond those that fit at a time a third more.  The fit is off by 6 % of 645 runs (root of the mean square), and what it chooses takes 1.7 %
 // longer than the best of them (geometric mean).  us, measured | so, MXFP8: 1 x 2048 x 8192 in clusters of 1, 2, 4, 8 20.6, 12.4, 7.9, 6.2 |
 // 23.6, 13.9, 9.0, 7.0; 128 x 2304 x 768 in tiles of 32, 64, 128 rows 5.6, 6.1, 7.7 | 5.5, 6.3, 7.8, as pairs 7.0 | 7.3; 512 x 2048 x 8192: 64 rows in
-// clusters of 2 18.4 | 19.4, 128 in 4 21.0 | 20.2, pairs in 1, 2, 4 slices 24.1, 20.1, 16.1 | 24.7, 19.7, 17.0; 2304 x 768 x 16384 as pairs in 1, 2, 5
-// slices 43.7, 32.7, 34.8 | 43.9, 30.7, 34.5.
-double pair_us(long long M, long long N, long long tiles, int steps, int splits) {
-  const long long units = tiles * splits, waves = (units + 73) / 74;
-  const int per = (steps + splits - 1) / splits;
-  return 4.0 + waves * (per * 0.3 + 1.5) + (splits > 1 ? 2.5 + splits * 1e-6 * M * N : 0.0);
+// clusters of 2 18.4 | 19.4, 128 in 4 21.0 | 20.2, pairs whole 24.1 | 24.7, in two slices 17.0 | 17.4; 2304 x 768 x 16384 43.8 | 43.9, 28.6 | 28.1.
+double pair_us(long long tiles, int steps, int splits) {
+  const long long at_once = splits == 1 ? 74 : 33, waves = (tiles + at_once - 1) / at_once;
+  return 4.0 + waves * ((steps + splits - 1) / splits * 0.3 + 1.5 + (splits > 1 ? 0.7 + 0.1 * (tiles < 33 ? tiles : 33) : 0.0));
 }
 double cluster_us(long long M, int bn, long long tiles, int steps, int splits) {
   const double ctas = (double)tiles * splits, rows = M < bn ? M : bn, load = ctas > 148 ? ctas / 148 - 1.0 : 0.0;      // (two CTAs on an SM)
@@ -746,25 +774,20 @@ Choice best_clusters(long long M, long long N, int steps) {
 }
 Choice best_pairs(long long M, long long N, int steps) {
   const long long tiles = ((M + 255) / 256) * ((N + 255) / 256);
-  Choice c{256, 1, pair_us(M, N, tiles, steps, 1)};
-  for (int s = 2; s <= 8 && s <= steps && N % 4 == 0 && tiles < 74; s++)
-    if (g_splits ? s == g_splits : pair_us(M, N, tiles, steps, s) < c.us) c = {256, s, pair_us(M, N, tiles, steps, s)};
+  Choice c{256, 1, pair_us(tiles, steps, 1)};
+  const double two = pair_us(tiles, steps, 2);
+  if (steps > 1 && tiles < 0xffffff && (g_splits ? g_splits == 2 : two < c.us)) c = {256, 2, two};
   return c;
 }
 
-// Up to 64 rows run as clusters, without a workspace (pairs were the faster ones at none of the sizes above).
 Plan plan_of(long long M, long long N, long long K, int fmt) {
   Plan p{};
   p.steps = (int)((K + (fmt == FP8 ? 127 : 255)) / (fmt == FP8 ? 128 : 256));
   const Choice pairs = best_pairs(M, N, p.steps), clusters = best_clusters(M, N, p.steps);
-  p.pair = g_kind ? g_kind == 1 : M > 64 && pairs.us < clusters.us;
+  p.pair = g_kind ? g_kind == 1 : pairs.us < clusters.us;
   p.bn = p.pair ? 256 : clusters.rows;
   p.splits = p.pair ? pairs.splits : clusters.splits;
   p.steps_per = (p.steps + p.splits - 1) / p.splits;
-  if (p.pair) {
-    p.splits = (p.steps + p.steps_per - 1) / p.steps_per;      // no empty slice
-    p.workspace = p.splits > 1 ? M * N * 4 * p.splits : 0;
-  }
   return p;
 }
 
@@ -797,14 +820,14 @@ int map_scales(CUtensorMap* m, const void* p, long long rows, int P, int pieces,
   return gbh::encode_tmap(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, p, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-template <int FMT, bool VECTORS>
+template <int FMT, bool VECTORS, bool SLICED>
 int launch_pair(const Maps& tm, const MxArgs& args, cudaStream_t st) {
   using C = PairCfg<FMT>;
   static std::atomic<uint32_t> done{0};
-  if (int rc = allow_shared(mx_pair_kernel<FMT, VECTORS>, C::BYTES, done)) return rc;
-  const long long units = (long long)args.num_m * args.num_n * args.splits;
-  const int pairs = units < 74 ? (int)units : 74;
-  GB_CUDA_OK(gbh::launch(mx_pair_kernel<FMT, VECTORS>, dim3(2 * pairs), dim3(C::THREADS), C::BYTES, st, 2, tm.a, tm.b, tm.sa, tm.sb, args));
+  if (int rc = allow_shared(mx_pair_kernel<FMT, VECTORS, SLICED>, C::BYTES, done)) return rc;
+  const long long tiles = (long long)args.num_m * args.num_n, clusters = SLICED || tiles < 74 ? tiles : 74;
+  const unsigned size = SLICED ? 4 : 2;
+  GB_CUDA_OK(gbh::launch(mx_pair_kernel<FMT, VECTORS, SLICED>, dim3((unsigned)clusters * size), dim3(C::THREADS), C::BYTES, st, size, tm.a, tm.b, tm.sa, tm.sb, args));
   return gbh::E_OK;
 }
 template <int FMT, int BN, typename X = void>
@@ -832,26 +855,24 @@ GB_EXPORT int gb_mx_tune(int kind, int splits) {
   return gbh::E_OK;
 }
 
-// How a product runs (for tests): 1 pairs, 2 clusters; rows of a tile; slices of K; workspace bytes.
-GB_EXPORT int gb_mx_plan(long long M, long long N, long long K, int fmt, long long* out4) {
+// How a product runs (for tests): 1 pairs, 2 clusters; rows of a tile; slices of K.
+GB_EXPORT int gb_mx_plan(long long M, long long N, long long K, int fmt, long long* out3) {
   if (M <= 0 || N <= 0 || K <= 0 || M > 0x7fffffffLL || N > 0x7fffffffLL || K > (1LL << 30) || (fmt != FP8 && fmt != FP4)) {
     gbh::set_error("gb_mx_plan: bad extents %lld x %lld x %lld, format %d", M, N, K, fmt);
     return gbh::E_BAD_ARG;
   }
   const Plan p = plan_of(M, N, K, fmt);
-  out4[0] = p.pair ? 1 : 2;
-  out4[1] = p.bn;
-  out4[2] = p.splits;
-  out4[3] = p.workspace;
+  out3[0] = p.pair ? 1 : 2;
+  out3[1] = p.bn;
+  out3[2] = p.splits;
   return gbh::E_OK;
 }
 
 // C (M x N, rows ldc apart) = act(A B^T + bias).  out: DT_BF16, DT_F16 or DT_F32; bias in C's type or fp32 (bias_f32), or null.
-// workspace: as many bytes as gb_mx_plan says.
 GB_EXPORT int gb_mx_matmul(int fmt, const void* a, const void* sa, const void* b, const void* sb, void* c, long long ldc, const void* bias, int bias_f32, long long M,
-                           long long N, long long K, int out, int act, void* workspace, long long workspace_bytes, void* stream) {
-  long long p4[4];
-  if (int rc = gb_mx_plan(M, N, K, fmt, p4)) return rc;
+                           long long N, long long K, int out, int act, void* stream) {
+  long long p3[3];
+  if (int rc = gb_mx_plan(M, N, K, fmt, p3)) return rc;
   if (out < 0 || out > 2 || act < 0 || act > 3 || ldc < N) {
     gbh::set_error("gb_mx_matmul: bad type %d, activation %d or row pitch %lld", out, act, ldc);
     return gbh::E_BAD_ARG;
@@ -861,10 +882,6 @@ GB_EXPORT int gb_mx_matmul(int fmt, const void* a, const void* sa, const void* b
     return gbh::E_BAD_ARG;
   }
   const Plan p = plan_of(M, N, K, fmt);
-  if (p.workspace > 0 && (bad_operand(workspace) || workspace_bytes < p.workspace)) {
-    gbh::set_error("gb_mx_matmul: workspace of %lld bytes on a 16-byte boundary, %lld are needed", workspace_bytes, p.workspace);
-    return gbh::E_BAD_ARG;
-  }
   const int P = pieces((int)K, fmt), RB = row_bytes((int)K, fmt), per = fmt == FP8 ? 1 : 2;
   MxArgs args{};
   args.M = (int)M; args.N = (int)N; args.steps = p.steps;
@@ -874,28 +891,24 @@ GB_EXPORT int gb_mx_matmul(int fmt, const void* a, const void* sa, const void* b
   cudaStream_t st = (cudaStream_t)stream;
   Maps tm;
   memset(&tm, 0, sizeof(tm));
-  int rc = 0;
   if (p.pair) {
+    int rc = 0;
     args.num_m = (int)((M + 255) / 256);
     args.num_n = (int)((N + 255) / 256);
-    MxArgs run = args;
-    if (p.splits > 1) {
-      run.C = workspace; run.ldc = N; run.out = OUT_F32; run.bias = nullptr; run.act = ACT_NONE;
-    }
-    const int size = run.out == OUT_F32 ? 4 : 2;
-    const auto whole = [&](int bytes) { return (uintptr_t)run.C % bytes == 0 && run.ldc * size % bytes == 0 && N * size % bytes == 0; };
-    run.vectors = whole(32) ? 32 : whole(16) ? 16 : 0;
+    const int size = out == OUT_F32 ? 4 : 2;
+    const auto whole = [&](int bytes) { return (uintptr_t)c % bytes == 0 && ldc * size % bytes == 0 && N * size % bytes == 0; };
+    args.vectors = whole(32) ? 32 : whole(16) ? 16 : 0;
     if (!rc) rc = map_codes(&tm.a, a, M, RB, 128);
     if (!rc) rc = map_codes(&tm.b, b, N, RB, 128);
     if (!rc) rc = map_scales(&tm.sa, sa, M, P, per, 1);
     if (!rc) rc = map_scales(&tm.sb, sb, N, P, per, 2);
-    if (!rc && run.vectors) rc = fmt == FP8 ? launch_pair<FP8, true>(tm, run, st) : launch_pair<FP4, true>(tm, run, st);
-    else if (!rc) rc = fmt == FP8 ? launch_pair<FP8, false>(tm, run, st) : launch_pair<FP4, false>(tm, run, st);
-    if (rc || p.splits == 1) return rc;
-    const long long quads = M * N / 4;
-    GB_CUDA_OK(gbh::launch(mx_finish_kernel, dim3((unsigned)(quads / 256 + 1 < 148 * 8 ? quads / 256 + 1 : 148 * 8)), dim3(256), 0, st, 1, (const float*)workspace, args, p.splits,
-                           FastDiv((uint32_t)(N / 4))));
-    return gbh::E_OK;
+    if (rc) return rc;
+    if (p.splits > 1) {
+      if (args.vectors) return fmt == FP8 ? launch_pair<FP8, true, true>(tm, args, st) : launch_pair<FP4, true, true>(tm, args, st);
+      return fmt == FP8 ? launch_pair<FP8, false, true>(tm, args, st) : launch_pair<FP4, false, true>(tm, args, st);
+    }
+    if (args.vectors) return fmt == FP8 ? launch_pair<FP8, true, false>(tm, args, st) : launch_pair<FP4, true, false>(tm, args, st);
+    return fmt == FP8 ? launch_pair<FP8, false, false>(tm, args, st) : launch_pair<FP4, false, false>(tm, args, st);
   }
   args.num_m = (int)((M + p.bn - 1) / p.bn);
   args.num_n = (int)((N + 127) / 128);
@@ -903,9 +916,8 @@ GB_EXPORT int gb_mx_matmul(int fmt, const void* a, const void* sa, const void* b
     gbh::set_error("gb_mx_matmul: %lld x %lld has too many tiles", M, N);
     return gbh::E_TOO_LARGE;
   }
-  rc = map_codes(&tm.a, b, N, RB, 128);
-  if (!rc) rc = map_codes(&tm.b, a, M, RB, p.bn);
-  if (rc) return rc;
+  if (int rc = map_codes(&tm.a, b, N, RB, 128)) return rc;
+  if (int rc = map_codes(&tm.b, a, M, RB, p.bn)) return rc;
   switch (p.bn) {
     case 16: return fmt == FP8 ? launch_cluster<FP8, 16>(tm, sb, sa, args, st) : launch_cluster<FP4, 16>(tm, sb, sa, args, st);
     case 32: return fmt == FP8 ? launch_cluster<FP8, 32>(tm, sb, sa, args, st) : launch_cluster<FP4, 32>(tm, sb, sa, args, st);
@@ -917,8 +929,8 @@ GB_EXPORT int gb_mx_matmul(int fmt, const void* a, const void* sa, const void* b
 // The same for up to 16 rows of x as they are (bf16, fp16 or fp32, K elements, ld apart), quantised within the product's kernel.
 GB_EXPORT int gb_mx_matmul_rows(int dtype, int fmt, const void* x, long long ld, const void* b, const void* sb, void* c, long long ldc, const void* bias, int bias_f32,
                                 long long M, long long N, long long K, int out, int act, void* stream) {
-  long long p4[4];
-  if (int rc = gb_mx_plan(M, N, K, fmt, p4)) return rc;
+  long long p3[3];
+  if (int rc = gb_mx_plan(M, N, K, fmt, p3)) return rc;
   if (M > 16 || dtype < 0 || dtype > 2 || out < 0 || out > 2 || act < 0 || act > 3 || ldc < N || ld < 0) {
     gbh::set_error("gb_mx_matmul_rows: %lld rows (16 at most), types %d and %d, activation %d, row pitches %lld and %lld", M, dtype, out, act, ld, ldc);
     return gbh::E_BAD_ARG;

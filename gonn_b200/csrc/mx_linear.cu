@@ -7,9 +7,8 @@ using namespace gbmx;
 GB_EXPORT int gb_mx_quantize(int dtype, int fmt, const void* x, long long ld, void* data, void* scales, long long rows, long long K, void* stream);
 GB_EXPORT int gb_mx_quantize_both(int dtype, const void* x, long long ld, void* data, void* scales, void* data_t, void* scales_t, float* sums, void* column_sums,
                                   int sum_dtype, long long rows, long long K, void* stream);
-GB_EXPORT int gb_mx_plan(long long M, long long N, long long K, int fmt, long long* out4);
 GB_EXPORT int gb_mx_matmul(int fmt, const void* a, const void* sa, const void* b, const void* sb, void* c, long long ldc, const void* bias, int bias_f32, long long M,
-                           long long N, long long K, int out, int act, void* workspace, long long workspace_bytes, void* stream);
+                           long long N, long long K, int out, int act, void* stream);
 GB_EXPORT int gb_mx_matmul_rows(int dtype, int fmt, const void* x, long long ld, const void* b, const void* sb, void* c, long long ldc, const void* bias, int bias_f32,
                                 long long M, long long N, long long K, int out, int act, void* stream);
 
@@ -21,10 +20,6 @@ long long up256(long long n) { return (n + 255) & ~255LL; }
 bool fits(long long rows, long long K) { return rows > 0 && K > 0 && rows <= 0x7fffffffLL && K <= (1LL << 30); }
 long long code_bytes(long long rows, long long K, int fmt) { return up256(rows * row_bytes((int)K, fmt)); }
 long long packed_bytes(long long rows, long long K, int fmt) { return code_bytes(rows, K, fmt) + up256((rows + 127) / 128 * pieces((int)K, fmt) * 512); }
-long long workspace_of(long long M, long long N, long long K, int fmt) {
-  long long p[4] = {0, 0, 0, 0};
-  return gb_mx_plan(M, N, K, fmt, p) ? 0 : up256(p[3]);
-}
 
 // Pieces of a buffer, each on a 256-byte boundary.
 struct Packed {
@@ -44,13 +39,11 @@ struct Carver {
   }
 };
 
-long long max2(long long a, long long b) { return a > b ? a : b; }
-
 // Bytes of a training layer's buffers: what it keeps from forward to backward, and the scratch of either.
 long long kept_bytes(long long M, long long N, long long K, int need_x, int need_w) { return (need_w ? packed_bytes(K, M, FP8) : 0) + (need_x ? packed_bytes(K, N, FP8) : 0); }
-long long forward_bytes(long long M, long long N, long long K) { return packed_bytes(M, K, FP8) + packed_bytes(N, K, FP8) + workspace_of(M, N, K, FP8); }
+long long forward_bytes(long long M, long long N, long long K) { return packed_bytes(M, K, FP8) + packed_bytes(N, K, FP8); }
 long long backward_bytes(long long M, long long N, long long K) {
-  return packed_bytes(M, N, FP8) + packed_bytes(N, M, FP8) + up256((M + 127) / 128 * N * 4) + max2(workspace_of(M, K, N, FP8), workspace_of(N, K, M, FP8));
+  return packed_bytes(M, N, FP8) + packed_bytes(N, M, FP8) + up256((M + 127) / 128 * N * 4);
 }
 
 // need: bytes of scratch, 0 where the extents are bad.
@@ -70,7 +63,7 @@ bool bad(const char* what, long long M, long long N, long long K, const void* sc
 
 // Scratch bytes of gb_mx_linear, 0 for none (16 rows at most) and for bad extents.
 GB_EXPORT long long gb_mx_linear_bytes(long long M, long long N, long long K, int fmt) {
-  return M > kFew && fits(M, K) && fits(N, K) ? packed_bytes(M, K, fmt) + workspace_of(M, N, K, fmt) : 0;
+  return M > kFew && fits(M, K) && fits(N, K) ? packed_bytes(M, K, fmt) : 0;
 }
 
 // y (M x N, of x's type or `out`) = act(Q(x) W^T + bias): x M x K, rows `ld` apart; W quantised (N, K).
@@ -81,8 +74,7 @@ GB_EXPORT int gb_mx_linear(int dtype, int fmt, const void* x, long long ld, cons
   Carver c{(uint8_t*)scratch};
   const Packed q = c.packed(M, K, fmt);
   if (int rc = gb_mx_quantize(dtype, fmt, x, ld, q.codes, q.scales, M, K, stream)) return rc;
-  const long long ws = workspace_of(M, N, K, fmt);
-  return gb_mx_matmul(fmt, q.codes, q.scales, w, sw, y, N, bias, bias_f32, M, N, K, out, act, c.bytes(ws), ws, stream);
+  return gb_mx_matmul(fmt, q.codes, q.scales, w, sw, y, N, bias, bias_f32, M, N, K, out, act, stream);
 }
 
 // Bytes of a training layer: which 0: kept from forward to backward, 1: forward's scratch, 2: backward's.  0 for bad extents.
@@ -113,8 +105,7 @@ GB_EXPORT int gb_mx_train_forward(int dtype, int wdtype, const void* x, long lon
     rc = gb_mx_quantize(wdtype, FP8, w, ldw, wq.codes, wq.scales, N, K, stream);
   }
   if (rc) return rc;
-  const long long ws = workspace_of(M, N, K, FP8);
-  return gb_mx_matmul(FP8, xq.codes, xq.scales, wq.codes, wq.scales, y, N, bias, bias_f32, M, N, K, dtype, 0, c.bytes(ws), ws, stream);
+  return gb_mx_matmul(FP8, xq.codes, xq.scales, wq.codes, wq.scales, y, N, bias, bias_f32, M, N, K, dtype, 0, stream);
 }
 
 // dx (M x K, of type dtype_x) = Q(dy) Q(W^T)^T, dw (N x K, dtype_w) = Q(dy^T) Q(x^T)^T, db (N, dtype_b) = column sums of dy; null: not
@@ -133,8 +124,6 @@ GB_EXPORT int gb_mx_train_backward(int dtype, const void* dy, long long ld, cons
   Carver c{(uint8_t*)scratch}, k{(uint8_t*)const_cast<void*>(kept)};
   const Packed g = c.packed(M, N, FP8), gt = c.packed(N, M, FP8);
   float* sums = (float*)c.bytes((M + 127) / 128 * N * 4);
-  const long long wsx = workspace_of(M, K, N, FP8), wsw = workspace_of(N, K, M, FP8);
-  uint8_t* ws = c.bytes(max2(wsx, wsw));
   int rc = 0;
   if (dw != nullptr) rc = gb_mx_quantize_both(dtype, dy, ld, g.codes, g.scales, gt.codes, gt.scales, db != nullptr ? sums : nullptr, db, dtype_b, M, N, stream);
   else if (dx != nullptr) rc = gb_mx_quantize(dtype, FP8, dy, ld, g.codes, g.scales, M, N, stream);
@@ -143,8 +132,8 @@ GB_EXPORT int gb_mx_train_backward(int dtype, const void* dy, long long ld, cons
   if (dw != nullptr) xt = k.packed(K, M, FP8);
   if (dx != nullptr) {
     const Packed wt = k.packed(K, N, FP8);
-    if ((rc = gb_mx_matmul(FP8, g.codes, g.scales, wt.codes, wt.scales, dx, K, nullptr, 0, M, K, N, dtype_x, 0, ws, wsx, stream))) return rc;
+    if ((rc = gb_mx_matmul(FP8, g.codes, g.scales, wt.codes, wt.scales, dx, K, nullptr, 0, M, K, N, dtype_x, 0, stream))) return rc;
   }
-  if (dw != nullptr) rc = gb_mx_matmul(FP8, gt.codes, gt.scales, xt.codes, xt.scales, dw, K, nullptr, 0, N, K, M, dtype_w, 0, ws, wsw, stream);
+  if (dw != nullptr) rc = gb_mx_matmul(FP8, gt.codes, gt.scales, xt.codes, xt.scales, dw, K, nullptr, 0, N, K, M, dtype_w, 0, stream);
   return rc;
 }

@@ -33,7 +33,7 @@ _DT = {torch.bfloat16: DT_BF16, torch.float16: DT_F16, torch.float32: DT_F32,
 # seventeen arguments takes the host 1 us so, 3 us with an object for each of them.
 _ARGUMENTS = {
     "gb_mx_quantize": "iipLppLLp", "gb_mx_quantize_both": "ipLppppppiLLp", "gb_mx_dequantize": "iipppLLp",
-    "gb_mx_add_rms_norm": "iipLpLpipppLLdp", "gb_mx_matmul": "ipppppLpiLLLiipLp", "gb_mx_matmul_rows": "iipLpppLpiLLLiip",
+    "gb_mx_add_rms_norm": "iipLpLpipppLLdp", "gb_mx_matmul": "ipppppLpiLLLiip", "gb_mx_matmul_rows": "iipLpppLpiLLLiip",
     "gb_mx_linear": "iipLppppiLLLiipLp",
     "gb_mx_train_forward": "iipLpLppiLLLiipLpLp", "gb_mx_train_backward": "ipLppipipiLLLpLp",
     "gb_mx_plan": "LLLip", "gb_mx_linear_bytes": "LLLi", "gb_mx_train_bytes": "LLLiii",

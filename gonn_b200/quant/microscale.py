@@ -29,7 +29,6 @@ from ..ops.linear import emit_grad, emit_vector_grad
 from ..ops.reduce import column_sum
 
 MXBlock = 32
-_FEW = 64                # rows up to which a product needs no workspace (gb_mx_plan)
 _FMT = {"mxfp8": 0, "mxfp4": 1}
 _NAMES = ("mxfp8", "mxfp4")
 _TYPES = {torch.bfloat16: _l.DT_BF16, torch.float16: _l.DT_F16, torch.float32: _l.DT_F32}
@@ -336,14 +335,7 @@ def MatMulMX(a: QTensorMX, b: QTensorMX, bias: Optional[torch.Tensor] = None, dt
     y = like.new_empty(shape, dtype=dtype)
     if M == 0 or N == 0:
         return y
-    need, ws = 0, None
-    if M > _FEW:
-        out = (_l.L * 4)()
-        _l.check(_l.lib().gb_mx_plan(M, N, K, fmt, out), "gb_mx_plan")
-        need = out[3]
-        ws = like.new_empty(need, dtype=torch.uint8) if need else None
-    _call(like.get_device(), "gb_mx_matmul", fmt, codes, scales, codes_b, scales_b, y.data_ptr(), N, bias_at, bias_f32, M, N, K, _TYPES[dtype], code,
-          None if ws is None else ws.data_ptr(), need)
+    _call(like.get_device(), "gb_mx_matmul", fmt, codes, scales, codes_b, scales_b, y.data_ptr(), N, bias_at, bias_f32, M, N, K, _TYPES[dtype], code)
     return y
 
 

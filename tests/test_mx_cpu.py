@@ -254,14 +254,12 @@ A, ODD = 4096, 4104                   # addresses that are never read: on a 16-b
     ("gb_mx_dequantize", (5, 0, A, A, A, 4, 64, None), "dtype"),
     ("gb_mx_add_rms_norm", (0, 0, A, 64, None, 64, None, 0, None, A, A, 4, 64, 1e-6, None), "weight"),
     ("gb_mx_add_rms_norm", (0, 0, A, 64, A, 64, A, 0, None, A, A, 4, 64, 1e-6, None), "room for the sum"),
-    ("gb_mx_matmul", (0, A, A, A, None, A, 8, None, 0, 4, 8, 64, 0, 0, None, 0, None), "boundaries"),
-    ("gb_mx_matmul", (0, A, A, A, ODD, A, 8, None, 0, 4, 8, 64, 0, 0, None, 0, None), "boundaries"),
-    ("gb_mx_matmul", (0, A, A, A, A, A, 7, None, 0, 4, 8, 64, 0, 0, None, 0, None), "pitch"),
-    ("gb_mx_matmul", (0, A, A, A, A, A, 8, None, 0, 4, 8, 64, 3, 0, None, 0, None), "type"),
-    ("gb_mx_matmul", (0, A, A, A, A, A, 8, None, 0, 4, 8, 64, 0, 4, None, 0, None), "activation"),
-    ("gb_mx_matmul", (0, A, A, A, A, A, 8, None, 0, 4, 0, 64, 0, 0, None, 0, None), "extents"),
-    ("gb_mx_matmul", (0, A, A, A, A, A, 768, None, 0, 2304, 768, 16384, 0, 0, None, 0, None), "workspace"),
-    ("gb_mx_matmul", (0, A, A, A, A, A, 768, None, 0, 2304, 768, 16384, 0, 0, ODD, 1 << 40, None), "workspace"),
+    ("gb_mx_matmul", (0, A, A, A, None, A, 8, None, 0, 4, 8, 64, 0, 0, None), "boundaries"),
+    ("gb_mx_matmul", (0, A, A, A, ODD, A, 8, None, 0, 4, 8, 64, 0, 0, None), "boundaries"),
+    ("gb_mx_matmul", (0, A, A, A, A, A, 7, None, 0, 4, 8, 64, 0, 0, None), "pitch"),
+    ("gb_mx_matmul", (0, A, A, A, A, A, 8, None, 0, 4, 8, 64, 3, 0, None), "type"),
+    ("gb_mx_matmul", (0, A, A, A, A, A, 8, None, 0, 4, 8, 64, 0, 4, None), "activation"),
+    ("gb_mx_matmul", (0, A, A, A, A, A, 8, None, 0, 4, 0, 64, 0, 0, None), "extents"),
     ("gb_mx_matmul_rows", (0, 0, A, 64, A, A, A, 8, None, 0, 17, 8, 64, 0, 0, None), "16 at most"),
     ("gb_mx_matmul_rows", (0, 0, None, 64, A, A, A, 8, None, 0, 4, 8, 64, 0, 0, None), "needed"),
     ("gb_mx_linear", (0, 0, A, 64, A, A, A, None, 0, 40, 8, 64, 0, 0, None, 0, None), "scratch"),
