@@ -633,8 +633,9 @@ mx_cluster_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         if (lane == 0) mbar_arrive(&full[stage]);
       }
     }
-    if (!ROWS && sub != 0 && warp < 6) {       // the warps that wait for the results take turns
-      for (int k = k0 + warp - 2, i = warp - 2; k < k1; k += 4, i += 4) {
+    // (One warp, step by step: loads land in any order, and a warp that had not seen a stage's last phase end would take that for the next one's.)
+    if (!ROWS && sub != 0 && warp == 2) {
+      for (int i = 0; i < k1 - k0; i++) {
         const int stage = i % C::STAGES;
         if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], (i / C::STAGES) & 1, abort_flag, args.status, ST_GEMM_TIMEOUT, 46))) break;
         uint4* s = reinterpret_cast<uint4*>(smem + C::OFF_SCALES + stage * C::S_BYTES + F::PIECES * C::PIECE);

@@ -329,6 +329,25 @@ def test_few_rows_are_quantised_within_the_product(format, dtype, M, N, K, statu
 
 
 @pytest.mark.parametrize("format", FORMATS)
+def test_loads_that_land_in_any_order(format, status_ok):
+    """More weights than L2 holds, rows of C in tiles that start within a scale piece: loads wait for memory and overtake one another."""
+    M, N, K = 100, 50304, 3000
+    a, b = (torch.randint(-3, 4, (rows, K), device=DEV).float() * torch.exp2(torch.randint(0, 4, (rows, K // 8 // 3), device=DEV).float()).repeat_interleave(24, 1) for rows in (M, N))
+    qa, qb = Q.QuantizeMX(a, format), Q.QuantizeMX(b, format)
+    want = (Q.DequantizeMX(qa).double() @ Q.DequantizeMX(qb).double().T).float()
+    for kind in (0, 32, 64):
+        for splits in (1, 2):
+            _l.lib().gb_mx_tune(kind, splits if kind else 0)
+            try:
+                for _ in range(3):
+                    y = Q.MatMulMX(qa, qb, None, torch.float32)
+                    _l.assert_status_ok()
+                    assert torch.equal(y, want)
+            finally:
+                _l.lib().gb_mx_tune(0, 0)
+
+
+@pytest.mark.parametrize("format", FORMATS)
 @pytest.mark.parametrize("kind", [1, 2, 32, 64, 128])
 @pytest.mark.parametrize("splits", [1, 2, 3, 5, 8])
 def test_every_way_of_a_product(format, kind, splits, status_ok):
