@@ -739,8 +739,7 @@ thread_local int g_kind = 0, g_rows = 0, g_splits = 0;       // gb_mx_tune
 // launch, the first loads and the last results, 1.5 for a tile's own; two slices exchange their sums, and 33 clusters of two pairs fit at a time.
 // Clusters: a step takes 0.33 (the 1.6 us of a load over the 100 KB that a CTA has in flight) and more where CTAs share an SM, a launch 2.45, each
 // of a tile's rows 0.026, the turning of scales 0.25; from two CTAs on the exchange, the longer the more CTAs share the way of its values;
-// CTAs beyond those that fit at a time a third more.  The fit is off by 6 % of 645 runs (root of the mean square), and what it chooses takes 1.7 %
-// longer than the best of them (geometric mean).  us, measured | so, MXFP8: 1 x 2048 x 8192 in clusters of 1, 2, 4, 8 20.6, 12.4, 7.9, 6.2 |
+// CTAs beyond those that fit at a time three quarters more.  What it chooses takes 1.2 % longer than the best (geometric mean over 116 sizes, 757 runs).  us, measured | so, MXFP8: 1 x 2048 x 8192 in clusters of 1, 2, 4, 8 20.6, 12.4, 7.9, 6.2 |
 // 23.6, 13.9, 9.0, 7.0; 128 x 2304 x 768 in tiles of 32, 64, 128 rows 5.6, 6.1, 7.7 | 5.5, 6.3, 7.8, as pairs 7.0 | 7.3; 512 x 2048 x 8192: 64 rows in
 // clusters of 2 18.4 | 19.4, 128 in 4 21.0 | 20.2, pairs whole 24.1 | 24.7, in two slices 17.0 | 17.4; 2304 x 768 x 16384 43.8 | 43.9, 28.6 | 28.1.
 double pair_us(long long tiles, int steps, int splits) {
@@ -751,7 +750,7 @@ double cluster_us(long long M, int bn, long long tiles, int steps, int splits) {
   const double ctas = (double)tiles * splits, rows = M < bn ? M : bn, load = ctas > 148 ? ctas / 148 - 1.0 : 0.0;      // (two CTAs on an SM)
   const double once = 2.45 + 0.026 * rows + 0.65 * load + (steps + splits - 1) / splits * 0.33 * (1.0 + 0.19 * load) + (M > bn && bn < 128 ? 0.25 : 0.0) +
                       (splits > 1 ? 0.56 + 0.16 * splits + 0.0033 * splits * rows * (ctas > 64 ? ctas / 64 : 1.0) : 0.0);
-  return once * (ctas > 296 ? 1.0 + 0.36 * (ceil(ctas / 296) - 1.0) : 1.0);
+  return once * (ctas > 296 ? 1.0 + 0.75 * (ceil(ctas / 296) - 1.0) : 1.0);
 }
 
 struct Choice {
