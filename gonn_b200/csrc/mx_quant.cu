@@ -347,8 +347,10 @@ __device__ __forceinline__ Root inverse_root(double sum, double inv_K, double ep
   const double v = fma(sum, inv_K, eps);
   float r0;
   asm("rsqrt.approx.f32 %0, %1;" : "=f"(r0) : "f"((float)v));
-  if (!(v > 1e-36 && v < 1e36)) return {r0, 0.f};
-  const double r = fma(0.5 * (double)r0, fma(-v * (double)r0, (double)r0, 1.0), (double)r0);
+  double r;
+  if (v > 1e-36 && v < 1e36) r = fma(0.5 * (double)r0, fma(-v * (double)r0, (double)r0, 1.0), (double)r0);
+  else if (v > 0.0 && v < 1e300) r = 1.0 / sqrt(v);
+  else return {r0, 0.f};
   const float hi = (float)r;
   return {hi, (float)(r - (double)hi)};
 }
@@ -356,14 +358,15 @@ __device__ __forceinline__ Root inverse_root(double sum, double inv_K, double ep
 // A value next to the border between two codes has to fall on the side where it belongs: by three roundings of fp32 one in a million falls on
 // the other, a step of the code away.  Borders, and the powers of two at which a scale changes, have at most four leading bits of
 // a fraction (E4M3; E2M1 two), so the last 19 (21) bits of a value in their neighbourhood are next to zero; four roundings, of 2^-24
-// each, move them by four at most.  Such values (one in 50 000 or 200 000; and infinities and NaN) are computed again, rounded to odd:
-// the last bit stands for all that lies behind it, so that the rounding to a code afterwards is that of the product itself.
+// each, and the error of the sum of squares in fp32, half of eight roundings, move them by eight at most.  A row with such a value (one value
+// in 30 000 or 120 000; and infinities and NaN) gets its sum again, in fp64, and the blocks with such values are computed again, rounded
+// to odd: the last bit stands for all that lies behind it, so that the rounding to a code afterwards is that of the product itself.
 template <int FMT>
-__device__ __forceinline__ uint32_t from_border(float y) {       // those bits and 5, above zeros
+__device__ __forceinline__ uint32_t from_border(float y) {       // those bits and 8, above zeros
   constexpr uint32_t shift = FMT == FP8 ? 1u << 13 : 1u << 11;
-  return __float_as_uint(y) * shift + 5u * shift;
+  return __float_as_uint(y) * shift + 8u * shift;
 }
-template <int FMT> constexpr uint32_t kNear = 10u << (FMT == FP8 ? 13 : 11);
+template <int FMT> constexpr uint32_t kNear = 16u << (FMT == FP8 ? 13 : 11);
 
 // h (hi + lo) * root * w, rounded to odd.
 __device__ __noinline__ float to_odd(float h, float lo, float root_hi, float root_lo, float w) {
@@ -395,8 +398,13 @@ __device__ __forceinline__ double row_sum(double s, double* red) {
   s = 0.0;
 #pragma unroll
   for (int i = 0; i < G / 32; i++) s += red[first + i];
-  __syncthreads();
-  return s;
+  return s;                              // (a barrier has to follow before the next: row_any's)
+}
+// Whether one of a warp's threads, or of a block's where a row takes more than a warp, says so.
+template <int G>
+__device__ __forceinline__ bool row_any(bool says) {
+  if (G <= 32) return __any_sync(0xffffffffu, says);
+  return __syncthreads_or(says);
 }
 
 // Sixteen columns of x + r: in pairs, and what rounding leaves out of fp32 ones.
@@ -426,6 +434,22 @@ __device__ __forceinline__ double squares(const uint64_t (&h)[8]) {
   return (double)a + (double)b;
 }
 
+// The same in fp64, of what was added (lo: of fp32 sums).
+template <bool F32>
+__device__ __forceinline__ double squares_exact(const uint64_t (&h)[8], const float (&lo)[16]) {
+  double s = 0.0;
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    float a, b;
+    parts_of(h[j], a, b);
+    const double x = F32 ? (double)a + (double)lo[2 * j] : (double)a, y = F32 ? (double)b + (double)lo[2 * j + 1] : (double)b;
+    s = fma(x, x, fma(y, y, s));
+  }
+  return s;
+}
+// Sums of squares that fp32 cannot be trusted with.
+__device__ __forceinline__ bool far_out(double s) { return !(s > 1e-25 && s < 1e38); }
+
 template <typename T, bool ALIGNED, int L>
 __device__ __forceinline__ void write_sum(const NormArgs& a, long long row, int k, const uint64_t (&h)[8], const Stage<T, L>& stage) {
   float v[16];
@@ -436,8 +460,9 @@ __device__ __forceinline__ void write_sum(const NormArgs& a, long long row, int 
   else stage.store(to, k - stage.lane * 16, a.K, v);
 }
 
-template <typename T, int FMT, bool ALIGNED>
-__device__ __forceinline__ void write_norm(const NormArgs& a, long long row, int k, const uint64_t (&h)[8], const float (&lo)[16], const Root& root) {
+// Codes of sixteen columns; whether one of the values may lie on the other side of a border (EXACT: it does not any more).
+template <typename T, int FMT, bool ALIGNED, bool EXACT>
+__device__ __forceinline__ bool write_norm(const NormArgs& a, long long row, int k, const uint64_t (&h)[8], const float (&lo)[16], const Root& root) {
   float w[16], y[16];
   if (sizeof(T) == 2 && a.w_f32) {
     uint32_t u[16];
@@ -462,8 +487,8 @@ __device__ __forceinline__ void write_norm(const NormArgs& a, long long row, int
     parts_of(mul_pair(p, w2), y[2 * j], y[2 * j + 1]);
     m = fmaxf(fmaxf(m, fabsf(y[2 * j])), fabsf(y[2 * j + 1]));
   }
-  uint32_t amax = __float_as_uint(m);    // (a flushed subnormal number has the same scale; infinities and NaN take the branch)
-  if (near <= kNear<FMT>) {
+  uint32_t amax = __float_as_uint(m);    // (a flushed subnormal number has the same scale; infinities and NaN come again)
+  if (EXACT && near <= kNear<FMT>) {
 #pragma unroll
     for (int j = 0; j < 16; j++) {
       float p, q;
@@ -477,6 +502,7 @@ __device__ __forceinline__ void write_norm(const NormArgs& a, long long row, int
   const uint32_t word = quantize16<FMT>(y, amax, 0xffu << (lane & 24), lane, out);
   store_codes<FMT>(a.data + row * a.row_bytes, k, a.row_bytes, out);
   if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_word(row, k >> 7, a.pieces)) = word;
+  return near <= kNear<FMT>;
 }
 
 // G threads of a block take a row (sixteen, or whole warps), VPT vectors of sixteen columns each, which stay in registers between the two
@@ -546,10 +572,25 @@ __global__ void __launch_bounds__(norm_threads(G), norm_blocks(sizeof(T), VPT, G
 #pragma unroll
         for (int i = 0; i < VPT; i++) write_sum<T, ALIGNED, L>(a, row, (t + i * G) * 16, h[i], stage);
       }
-      const Root root = inverse_root(row_sum<G>(s, red), a.inv_K, a.eps);
+      s = row_sum<G>(s, red);
+      const Root root = inverse_root(s, a.inv_K, a.eps);
+      bool near[VPT], any = live && far_out(s);
 #pragma unroll
-      for (int i = 0; i < VPT; i++)
-        if (live && t + i * G < vecs) write_norm<T, FMT, ALIGNED>(a, row, (t + i * G) * 16, h[i], lo[F32 ? i : 0], root);
+      for (int i = 0; i < VPT; i++) {
+        near[i] = false;
+        if (live && t + i * G < vecs) near[i] = write_norm<T, FMT, ALIGNED, false>(a, row, (t + i * G) * 16, h[i], lo[F32 ? i : 0], root) || far_out(s);
+        any |= near[i];
+      }
+      if (row_any<G>(any)) {
+        double exact = 0.0;
+#pragma unroll
+        for (int i = 0; i < VPT; i++) exact += squares_exact<F32>(h[i], lo[F32 ? i : 0]);
+        const Root again = inverse_root(row_sum<G>(exact, red), a.inv_K, a.eps);
+#pragma unroll
+        for (int i = 0; i < VPT; i++)
+          if (__ballot_sync(0xffffffffu, near[i]) & 0xffu << (threadIdx.x & 24)) write_norm<T, FMT, ALIGNED, true>(a, row, (t + i * G) * 16, h[i], lo[F32 ? i : 0], again);
+        if (G > 32) __syncthreads();
+      }
     } else {
       // (a row's threads take each step together, for the way through shared memory)
       auto take = [&](int i, uint64_t (&h)[8], float (&lo)[16]) {
@@ -575,12 +616,31 @@ __global__ void __launch_bounds__(norm_threads(G), norm_blocks(sizeof(T), VPT, G
         if (sum) write_sum<T, ALIGNED, L>(a, row, i * 16, h, stage);
         s += squares(h);
       }
-      const Root root = inverse_root(row_sum<G>(s, red), a.inv_K, a.eps);
+      s = row_sum<G>(s, red);
+      const Root root = inverse_root(s, a.inv_K, a.eps);
+      bool any = far_out(s);
       for (int i = t; i - t < vecs; i += G) {
         uint64_t h[8];
         float lo[16];
         take(i, h, lo);
-        if (i < vecs) write_norm<T, FMT, ALIGNED>(a, row, i * 16, h, lo, root);
+        if (i < vecs) any |= write_norm<T, FMT, ALIGNED, false>(a, row, i * 16, h, lo, root);
+      }
+      if (row_any<G>(any)) {
+        double exact = 0.0;
+        for (int i = t; i - t < vecs; i += G) {
+          uint64_t h[8];
+          float lo[16];
+          take(i, h, lo);
+          exact += squares_exact<F32>(h, lo);
+        }
+        const Root again = inverse_root(row_sum<G>(exact, red), a.inv_K, a.eps);
+        for (int i = t; i - t < vecs; i += G) {
+          uint64_t h[8];
+          float lo[16];
+          take(i, h, lo);
+          if (i < vecs) write_norm<T, FMT, ALIGNED, true>(a, row, i * 16, h, lo, again);
+        }
+        __syncthreads();
       }
     }
   }

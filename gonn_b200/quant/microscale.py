@@ -269,8 +269,8 @@ def AddRMSNormMX(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
                  format: str = "mxfp8") -> Tuple[QTensorMX, torch.Tensor]:
     """``h = x + residual`` and the quantised ``h / sqrt(mean(h^2) + eps) * weight``: what a pre-norm block hands to its next
     products, and the stream that goes on beside them.  Returns (codes and scales, h).  The norm takes the sum before it is rounded to
-    h's type; a value is rounded once, to its code, so that only the error of the mean (1e-8 or so of it) can move one that lies
-    between two codes to the other.  Squares are fp32: magnitudes from 1.8e19 on count as infinite.  Without a residual h is x itself."""
+    h's type; a value is rounded once, to its code: none of the arithmetic before moves one that lies next to the border between two
+    codes to the other.  Without a residual h is x itself."""
     fmt, shape = _format(format), tuple(x.shape)
     a = _rows(x, "AddRMSNormMX")
     rows, K = a.shape

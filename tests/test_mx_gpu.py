@@ -162,6 +162,24 @@ def test_norm_of_many_rows(format, dtype, K, status_ok):
     nearly(part, y, 4 + 16 + 12)
 
 
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,K", [(40000, 160), (8000, 776), (3000, 2304), (4100, 1003), (100, 20000), (600, 8200)])
+def test_norm_codes_are_those_of_64_bits(format, dtype, rows, K, status_ok):
+    """Millions of values, some of which lie within a rounding of fp32 of the border between two codes; and rows whose squares fp32 does not
+    hold.  (fp64 on the device: its own error, some 1e-15, is a millionth of the distance at which a border was ever met.)"""
+    x, r, w = torch.randn(rows, K, device=DEV).to(dtype), torch.randn(rows, K, device=DEV).to(dtype), (torch.rand(K, device=DEV) + 0.5).to(dtype)
+    if dtype == torch.float32:
+        x[1], r[1] = x[1] * 2.0 ** 70, r[1] * 2.0 ** 70
+        x[2], r[2] = x[2] * 2.0 ** -70, r[2] * 2.0 ** -70
+    eps = 0.0
+    q, _ = Q.AddRMSNormMX(x, r, w, eps, format)
+    total = x.double() + r.double()
+    y = total / torch.sqrt(total.square().mean(-1, keepdim=True) + eps) * w.double()
+    want = Q.microscale._quantize_ref(y.cpu(), int(format == "mxfp4"), (rows, K))
+    equal(q, want)
+
+
 def cpu(q):
     return Q.QTensorMX(q.Data.cpu(), q.Scales.cpu(), q.Format, q.Shape)
 
