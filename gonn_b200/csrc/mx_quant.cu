@@ -682,7 +682,8 @@ bool wide_rows(const void* p, long long ld, long long K, int size) { return ((ui
 
 // How a row of `vecs` vectors is dealt out: one to a thread, the shortest way, or two, which holds more in flight, for what does not stay in
 // L2.  One | two, bf16, us: 600 x 2048 4.0 | 5.2, 2400 x 2048 8.1 | 9.4, 8192 x 768 10.6 | 11.5, 2400 x 4096 13.6 | 13.7, 16384 x 768 21.5 | 19.1,
-// 16384 x 2048 44 | 43.5, 8192 x 8192 91 | 82; fp32, 8192 x 2048 42 | 42, 4096 x 8192 95 | 78.  Rows at any address: 16384 x 768 bf16 31, 16384 x 2048 66.
+// 16384 x 2048 44 | 43.5, 8192 x 8192 91 | 82; fp32, 8192 x 2048 42 | 42, 4096 x 8192 95 | 78 (before rows with a value next to a border took
+// their sum again, which costs 5 to 10 % of either).  Rows at any address: 16384 x 768 bf16 31, 16384 x 2048 66.
 template <typename T, int FMT, bool ALIGNED>
 cudaError_t norm_launch(const NormArgs& a, cudaStream_t st) {
   const int vecs = a.pieces * 8;
