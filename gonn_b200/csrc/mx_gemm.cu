@@ -72,7 +72,11 @@ __device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t smem) {
 
 __device__ __forceinline__ float activate(float v, int act) {
   switch (act) {
-    case ACT_RELU: return fmaxf(v, 0.f);
+    case ACT_RELU: {                       // (NaN stays NaN: a block with a NaN or an infinity is one, and its products are)
+      float y;
+      asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(v));
+      return y;
+    }
     case ACT_GELU_TANH: {                  // (gelu_tanh_f in five instructions and the tanh)
       const float h = 0.5f * v, u = v * fmaf(v * v, 0.7978845608f * 0.044715f, 0.7978845608f);
       return fmaf(h, tanh_fast(u), h);

@@ -625,3 +625,21 @@ def test_layers_between_devices_and_files(status_ok, tmp_path):
     other.load_state_dict(torch.load(tmp_path / "layer.pt"))
     assert torch.equal(other(x.to(DEV)), m(x.to(DEV)))
     assert off(m(x.to(DEV)).cpu(), want.double()) <= (100 / 64 + 4) * 2.0 ** -23 + 2.0 ** -24
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("act", ["relu", "gelu", "geluexact"])
+@pytest.mark.parametrize("M,N", [(3, 200), (40, 200), (2000, 2100)])
+def test_activations_keep_nan(format, act, M, N, status_ok):
+    """NaN and infinities of the operands, behind every activation and in every kernel: as on the CPU."""
+    K = 333
+    a, b = torch.randn(M, K), torch.randn(N, K)
+    a[1, 70] = math.nan
+    b[130, 5] = math.inf
+    nan = torch.zeros(M, N, dtype=torch.bool)
+    nan[1] = nan[:, 130] = True
+    w = Q.QuantizeMX(b.to(DEV), format)
+    for dtype in DTYPES:
+        assert torch.equal(torch.isnan(Q.LinearMX(a.to(DEV), w, None, act, dtype)).cpu(), nan)
+        assert torch.equal(torch.isnan(Q.MatMulMX(Q.QuantizeMX(a.to(DEV), format), w, torch.ones(N, device=DEV), dtype, act)).cpu(), nan)
+    assert torch.equal(torch.isnan(Q.LinearMX(a[:9], cpu(w), None, act)), nan[:9])
