@@ -643,3 +643,35 @@ def test_activations_keep_nan(format, act, M, N, status_ok):
         assert torch.equal(torch.isnan(Q.LinearMX(a.to(DEV), w, None, act, dtype)).cpu(), nan)
         assert torch.equal(torch.isnan(Q.MatMulMX(Q.QuantizeMX(a.to(DEV), format), w, torch.ones(N, device=DEV), dtype, act)).cpu(), nan)
     assert torch.equal(torch.isnan(Q.LinearMX(a[:9], cpu(w), None, act)), nan[:9])
+
+
+def activated(act, dtype, rows):
+    """(v, the activation of v as a product's epilogue computes it): products of zeros, v as the bias."""
+    v = torch.linspace(-6, 6, 24001, device=DEV)
+    zero = Q.QuantizeMX(torch.zeros(rows, 32, device=DEV))
+    y = Q.MatMulMX(zero, Q.QuantizeMX(torch.zeros(v.numel(), 32, device=DEV)), v, dtype, act)
+    assert all(torch.equal(r, y[0]) for r in y[1:])
+    return v.double(), y[0].double()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 300])
+def test_gelu_value_by_value(dtype, rows, status_ok):
+    """v / (1 + exp(-2u)), relative to each value.  The exponent is rounded five times (two of them constants), each of which moves the result by
+    2 |u| 2^-24; the exponential is off by two units, the reciprocal by one, and five operations follow: twelve roundings of 2^-24.  Then
+    the rounding to the type, and for fp16 half a step of its subnormal numbers."""
+    v, y = activated("gelu", dtype, rows)
+    u = math.sqrt(2 / math.pi) * (v + 0.044715 * v ** 3)
+    want = v / (1 + torch.exp(-2 * u))
+    rel = (10 * u.abs() + 12) * 2.0 ** -24 + (0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2)
+    least = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    assert bool(((y - want).abs() <= rel * 1.001 * want.abs() + least).all())
+
+
+def test_gelu_of_far_values(status_ok):
+    """Nothing is left below, everything above, and a NaN stays where it is."""
+    v = torch.tensor([-1e30, -3e4, -20.0, math.nan, 9.0, 20.0, math.nan, 3e4, 1e30, -0.0], device=DEV)
+    zero, w = Q.QuantizeMX(torch.zeros(1, 32, device=DEV)), Q.QuantizeMX(torch.zeros(10, 32, device=DEV))
+    y = Q.MatMulMX(zero, w, v, torch.float32, "gelu")[0]
+    assert torch.isnan(y[[3, 6]]).all() and y[:3].abs().max() < 1e-15
+    assert torch.equal(y[[4, 5, 7, 8, 9]], v[[4, 5, 7, 8, 9]])
