@@ -675,3 +675,23 @@ def test_gelu_of_far_values(status_ok):
     y = Q.MatMulMX(zero, w, v, torch.float32, "gelu")[0]
     assert torch.isnan(y[[3, 6]]).all() and y[:3].abs().max() < 1e-15
     assert torch.equal(y[[4, 5, 7, 8, 9]], v[[4, 5, 7, 8, 9]])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 300])
+def test_exact_gelu_value_by_value(dtype, rows, status_ok):
+    """v / 2 erfc(-v / sqrt 2), relative to each value, in roundings of 2^-24: the exponent -v^2 / 2 takes three, each of which moves the result by v^2 / 2;
+    the exponential four; the polynomial's fit two; its argument, off by five, moves it by up to 2.7 times that; its sums eight; products four."""
+    v, y = activated("geluexact", dtype, rows)
+    want = v / 2 * torch.special.erfc(-v / math.sqrt(2))
+    rel = (1.5 * v ** 2 + 32) * 2.0 ** -24 + (0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2)
+    least = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    assert bool(((y - want).abs() <= rel * 1.001 * want.abs() + least).all())
+
+
+def test_exact_gelu_of_far_values(status_ok):
+    v = torch.tensor([-1e30, -3e4, -20.0, math.nan, 9.0, 20.0, math.nan, 3e4, 1e30, -0.0], device=DEV)
+    zero, w = Q.QuantizeMX(torch.zeros(1, 32, device=DEV)), Q.QuantizeMX(torch.zeros(10, 32, device=DEV))
+    y = Q.MatMulMX(zero, w, v, torch.float32, "geluexact")[0]
+    assert torch.isnan(y[[3, 6]]).all() and y[:3].abs().max() < 1e-15
+    assert torch.equal(y[[4, 5, 7, 8, 9]], v[[4, 5, 7, 8, 9]])
