@@ -104,6 +104,7 @@ template <> struct Elem<__nv_bfloat16> {     // (not by way of fp32 arithmetic, 
   static __device__ __forceinline__ float2 pair(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return gb::pack_bf16(a, b); }
   static __device__ __forceinline__ uint32_t bits(uint32_t h) { return h << 16; }
+  static __device__ __forceinline__ float one(uint32_t h) { return __uint_as_float(bits(h)); }
 };
 template <> struct Elem<__half> {
   static constexpr int SZ = 2;
@@ -114,6 +115,7 @@ template <> struct Elem<__half> {
   static __device__ __forceinline__ float2 pair(uint32_t w) { return gb::unpack_f16(w); }
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return gb::pack_f16(a, b); }
   static __device__ __forceinline__ uint32_t bits(uint32_t h) { return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h))); }
+  static __device__ __forceinline__ float one(uint32_t h) { return __uint_as_float(bits(h)); }
 };
 template <> struct Elem<float> {
   static constexpr int SZ = 4;
@@ -121,6 +123,7 @@ template <> struct Elem<float> {
 #pragma unroll
     for (int i = 0; i < 8; i++) f[i] = __uint_as_float(w[i]);
   }
+  static __device__ __forceinline__ float one(uint32_t w) { return __uint_as_float(w); }
 };
 
 // Extent of a matrix in memory: vectors are read as long as they lie within it.

@@ -328,39 +328,29 @@ struct NormArgs {
   Extent ex, er, ew;
 };
 
-// fp32 arithmetic that keeps subnormal numbers.
-__device__ __forceinline__ float add_exact(float a, float b) {
-  float d;
-  asm("add.rn.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+// fp64 of fp32, subnormal numbers too.
+__device__ __forceinline__ double to_double(float v) {
+  double d;
+  asm("cvt.f64.f32 %0, %1;" : "=d"(d) : "f"(v));
   return d;
 }
-__device__ __forceinline__ float fma_exact(float a, float b, float c) {
-  float d;
-  asm("fma.rn.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-// 1 / sqrt(sum / K + eps) in two parts: the approximation and a step of Newton's iteration in fp64.
-struct Root {
-  float hi, lo;
-};
-__device__ __forceinline__ Root inverse_root(double sum, double inv_K, double eps) {
-  const double v = fma(sum, inv_K, eps);
+// 1 / sqrt(v) to a rounding of fp32: the approximation and a step of Newton's iteration in fp64.
+__device__ __forceinline__ float inverse_root(double v) {
   float r0;
   asm("rsqrt.approx.f32 %0, %1;" : "=f"(r0) : "f"((float)v));
-  double r;
-  if (v > 1e-36 && v < 1e36) r = fma(0.5 * (double)r0, fma(-v * (double)r0, (double)r0, 1.0), (double)r0);
-  else if (v > 0.0 && v < 1e300) r = 1.0 / sqrt(v);
-  else return {r0, 0.f};
-  const float hi = (float)r;
-  return {hi, (float)(r - (double)hi)};
+  return (float)fma(0.5 * (double)r0, fma(-v * (double)r0, (double)r0, 1.0), (double)r0);
 }
+// A row whose sum of squares s or mean square v = s / K + eps fp32 cannot be trusted with (its values are all taken as next to a border).
+__device__ __forceinline__ bool far_out(double s, double v) { return !(s > 1e-25 && s < 1e38 && v > 1e-36 && v < 1e36); }
 
 // A value next to the border between two codes has to fall on the side where it belongs: by three roundings of fp32 one in a million falls on
 // the other, a step of the code away.  Borders, and the powers of two at which a scale changes, have at most four leading bits of
-// a fraction (E4M3; E2M1 two), so the last 19 (21) bits of a value in their neighbourhood are next to zero; four roundings, of 2^-24
-// each, and the error of the sum of squares in fp32, half of eight roundings, move them by eight at most.  A row with such a value (one value
-// in 30 000 or 120 000; and infinities and NaN) gets its sum again, in fp64, and the blocks with such values are computed again, rounded
-// to odd: the last bit stands for all that lies behind it, so that the rounding to a code afterwards is that of the product itself.
+// a fraction (E4M3; E2M1 two), so the last 19 (21) bits of a value in their neighbourhood are next to zero.  Eight roundings of 2^-24 each (the
+// sum, in its square too, where it is not exact; half of the eight of a chain of squares; 1 / rms; its product) and the value's own move them by
+// less than nine units of the last place, 4.25 times two for the largest fraction and half a unit.  A row with such a value (one value
+// in 30 000 or 120 000; and infinities and NaN) gets its sum again, in fp64, and the blocks of such values are computed again in fp64, from
+// what was added, and rounded to odd: the last bit stands for all that lies behind it, so that the rounding to a code afterwards is that of the
+// value itself.
 template <int FMT>
 __device__ __forceinline__ uint32_t from_border(float y) {       // those bits and 8, above zeros
   constexpr uint32_t shift = FMT == FP8 ? 1u << 13 : 1u << 11;
@@ -368,22 +358,12 @@ __device__ __forceinline__ uint32_t from_border(float y) {       // those bits a
 }
 template <int FMT> constexpr uint32_t kNear = 16u << (FMT == FP8 ? 13 : 11);
 
-// h (hi + lo) * root * w, rounded to odd.
-__device__ __noinline__ float to_odd(float h, float lo, float root_hi, float root_lo, float w) {
-  const float p = mul_exact(h, root_hi);
-  const float e = fma_exact(lo, root_hi, fma_exact(h, root_lo, fma_exact(h, root_hi, -p)));
-  const float ew = mul_exact(e, w);
+// (x + r) / rms * w * by, rounded to odd; what is above the largest number of fp32 becomes that (an odd one).
+__device__ __forceinline__ float to_odd(float x, float r, float w, double rms, double by) {
+  const double y = (to_double(x) + to_double(r)) / rms * to_double(w) * by;
   float z;
-  asm("fma.rz.f32 %0, %1, %2, %3;" : "=f"(z) : "f"(p), "f"(w), "f"(ew));
-  const float left = add_exact(fma_exact(p, w, -z), ew);
-  return left != 0.f ? __uint_as_float(__float_as_uint(z) | 1u) : z;
-}
-
-// What the rounding of x + r to fp32 leaves out.  (Sums of 16-bit values are exact but for far magnitudes.)
-__device__ __forceinline__ float left_out(float h, float x, float r) {
-  const float b = add_exact(h, -x);
-  const float lo = add_exact(add_exact(x, -add_exact(h, -b)), add_exact(r, -b));
-  return fabsf(h) < 3e38f ? lo : 0.f;
+  asm("cvt.rz.f32.f64 %0, %1;" : "=f"(z) : "d"(y));
+  return to_double(z) != y ? __uint_as_float(__float_as_uint(z) | 1u) : z;
 }
 
 // The sum over the G threads of a row: a half-warp, or whole warps (their sums in one order, the same for every thread).
@@ -407,22 +387,14 @@ __device__ __forceinline__ bool row_any(bool says) {
   return __syncthreads_or(says);
 }
 
-// Sixteen columns of x + r: in pairs, and what rounding leaves out of fp32 ones.
+// Sixteen columns of x + r, in pairs.
 template <typename T>
-__device__ __forceinline__ void sum16(const uint32_t (&wx)[4 * Elem<T>::SZ], const uint32_t (&wr)[4 * Elem<T>::SZ], uint64_t (&h)[8], float (&lo)[16]) {
+__device__ __forceinline__ void sum16(const uint32_t (&wx)[4 * Elem<T>::SZ], const uint32_t (&wr)[4 * Elem<T>::SZ], uint64_t (&h)[8]) {
   float x[16], r[16];
   unpack16<T>(wx, x);
   unpack16<T>(wr, r);
 #pragma unroll
-  for (int j = 0; j < 8; j++) {
-    h[j] = add_pair(pair_of(x[2 * j], x[2 * j + 1]), pair_of(r[2 * j], r[2 * j + 1]));
-    if constexpr (sizeof(T) == 4) {
-      float a, b;
-      parts_of(h[j], a, b);
-      lo[2 * j] = left_out(a, x[2 * j], r[2 * j]);
-      lo[2 * j + 1] = left_out(b, x[2 * j + 1], r[2 * j + 1]);
-    }
-  }
+  for (int j = 0; j < 8; j++) h[j] = add_pair(pair_of(x[2 * j], x[2 * j + 1]), pair_of(r[2 * j], r[2 * j + 1]));
 }
 // Their squares: two chains of eight in fp32, which an fp64 sum takes up.
 __device__ __forceinline__ double squares(const uint64_t (&h)[8]) {
@@ -434,21 +406,20 @@ __device__ __forceinline__ double squares(const uint64_t (&h)[8]) {
   return (double)a + (double)b;
 }
 
-// The same in fp64, of what was added (lo: of fp32 sums).
-template <bool F32>
-__device__ __forceinline__ double squares_exact(const uint64_t (&h)[8], const float (&lo)[16]) {
+// The same in fp64, of x + r as it is before any rounding to fp32.
+template <typename T>
+__device__ __forceinline__ double squares_exact(const uint32_t (&wx)[4 * Elem<T>::SZ], const uint32_t (&wr)[4 * Elem<T>::SZ]) {
+  float x[16], r[16];
+  unpack16<T>(wx, x);
+  unpack16<T>(wr, r);
   double s = 0.0;
 #pragma unroll
-  for (int j = 0; j < 8; j++) {
-    float a, b;
-    parts_of(h[j], a, b);
-    const double x = F32 ? (double)a + (double)lo[2 * j] : (double)a, y = F32 ? (double)b + (double)lo[2 * j + 1] : (double)b;
-    s = fma(x, x, fma(y, y, s));
+  for (int j = 0; j < 16; j++) {
+    const double h = to_double(x[j]) + to_double(r[j]);
+    s = fma(h, h, s);
   }
   return s;
 }
-// Sums of squares that fp32 cannot be trusted with.
-__device__ __forceinline__ bool far_out(double s) { return !(s > 1e-25 && s < 1e38); }
 
 template <typename T, bool ALIGNED, int L>
 __device__ __forceinline__ void write_sum(const NormArgs& a, long long row, int k, const uint64_t (&h)[8], const Stage<T, L>& stage) {
@@ -460,10 +431,9 @@ __device__ __forceinline__ void write_sum(const NormArgs& a, long long row, int 
   else stage.store(to, k - stage.lane * 16, a.K, v);
 }
 
-// Codes of sixteen columns; whether one of the values may lie on the other side of a border (EXACT: it does not any more).
-template <typename T, int FMT, bool ALIGNED, bool EXACT>
-__device__ __forceinline__ bool write_norm(const NormArgs& a, long long row, int k, const uint64_t (&h)[8], const float (&lo)[16], const Root& root) {
-  float w[16], y[16];
+// The weights of sixteen columns.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void weights16(const NormArgs& a, int k, float (&w)[16]) {
   if (sizeof(T) == 2 && a.w_f32) {
     uint32_t u[16];
     load16<float, false>(reinterpret_cast<const float*>(a.w), k, a.K, false, a.ew, u);
@@ -473,7 +443,14 @@ __device__ __forceinline__ bool write_norm(const NormArgs& a, long long row, int
     load16<T, ALIGNED>(reinterpret_cast<const T*>(a.w), k, a.K, false, a.ew, u);
     unpack16<T>(u, w);
   }
-  const uint64_t root2 = pair_of(root.hi, root.hi);
+}
+
+// Codes of sixteen columns; whether one of the values may lie on the other side of a border.
+template <typename T, int FMT, bool ALIGNED>
+__device__ __forceinline__ bool write_norm(const NormArgs& a, long long row, int k, const uint64_t (&h)[8], float root) {
+  float w[16], y[16];
+  weights16<T, ALIGNED>(a, k, w);
+  const uint64_t root2 = pair_of(root, root);
   // for the test, zeros become a number far from any border (sums of bf16 values are zero now and then) and others stay what they are
   const uint64_t tiny = pair_of(__uint_as_float(0x00955555u), __uint_as_float(0x00955555u));
   uint32_t near = ~0u;
@@ -487,36 +464,59 @@ __device__ __forceinline__ bool write_norm(const NormArgs& a, long long row, int
     parts_of(mul_pair(p, w2), y[2 * j], y[2 * j + 1]);
     m = fmaxf(fmaxf(m, fabsf(y[2 * j])), fabsf(y[2 * j + 1]));
   }
-  uint32_t amax = __float_as_uint(m);    // (a flushed subnormal number has the same scale; infinities and NaN come again)
-  if (EXACT && near <= kNear<FMT>) {
-#pragma unroll
-    for (int j = 0; j < 16; j++) {
-      float p, q;
-      parts_of(h[j / 2], p, q);
-      y[j] = to_odd(j & 1 ? q : p, sizeof(T) == 4 ? lo[j] : 0.f, root.hi, root.lo, w[j]);
-    }
-    amax = largest16(y);
-  }
   uint32_t out[4];
-  const int lane = threadIdx.x & 31;
-  const uint32_t word = quantize16<FMT>(y, amax, 0xffu << (lane & 24), lane, out);
+  const int lane = threadIdx.x & 31;     // (a flushed subnormal number has the same scale; infinities and NaN come again)
+  const uint32_t word = quantize16<FMT>(y, __float_as_uint(m), 0xffu << (lane & 24), lane, out);
   store_codes<FMT>(a.data + row * a.row_bytes, k, a.row_bytes, out);
   if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_word(row, k >> 7, a.pieces)) = word;
   return near <= kNear<FMT>;
+}
+template <typename T> __device__ __forceinline__ float element(const T* from, long long i) {
+  return Elem<T>::one(__ldg(reinterpret_cast<const typename Stage<T, 32>::Bits*>(from) + i));
+}
+// Codes and scale of the block from column k on, in fp64, a column a lane (a lane that computes its sixteen one after the other takes 3 us for
+// them: 600 x 2048 bf16 5.5 | 8.5).  A block that holds more than fp32 does is taken 2^16 times smaller (a norm's values are below 2^15
+// times the weight).
+template <typename T, int FMT>
+__device__ __forceinline__ void write_block_exact(const NormArgs& a, long long row, int k, double rms) {
+  const int lane = threadIdx.x & 31, c = k + lane;
+  float x = 0.f, r = 0.f, w = 0.f;
+  if (c < a.K) {
+    x = element(reinterpret_cast<const T*>(a.x), row * a.ldx + c);
+    if (a.r != nullptr) r = element(reinterpret_cast<const T*>(a.r), row * a.ldr + c);
+    w = a.w_f32 ? __ldg(reinterpret_cast<const float*>(a.w) + c) : element(reinterpret_cast<const T*>(a.w), c);
+  }
+  float y;
+  uint32_t amax = 0, up = 0;
+  for (double by = 1.0;; by = 0x1p-16, up = 16) {
+    y = c < a.K ? to_odd(x, r, w, rms, by) : 0.f;        // (zeros behind the end of a row of NaN too)
+    amax = __reduce_max_sync(0xffffffffu, __float_as_uint(y) & 0x7fffffffu);
+    if (up != 0 || amax != 0x7f7fffffu) break;
+  }
+  const uint32_t code = up == 0 ? scale_code(amax, FMT) : min(scale_code(amax, FMT) + up, 254u);
+  const float q = mul_exact(y, scale_inverse(code - up)), next = __shfl_down_sync(0xffffffffu, q, 1);
+  uint8_t* to = a.data + row * a.row_bytes;
+  if (FMT == FP8) {
+    if (c < a.row_bytes) to[c] = (uint8_t)e4m3x4(q, 0.f, 0.f, 0.f);
+  } else {
+    const float v[8] = {q, next, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (c / 2 < a.row_bytes && (lane & 1) == 0) to[c / 2] = (uint8_t)e2m1x8(v);
+  }
+  if (lane == 0) a.scales[scale_word(row, k >> 7, a.pieces) + (k >> 5 & 3)] = (uint8_t)code;
 }
 
 // G threads of a block take a row (sixteen, or whole warps), VPT vectors of sixteen columns each, which stay in registers between the two
 // passes.  VPT = 0: rows of any length, read a second time for their codes.  BLOCKS: on an SM.  What counts is how many warps there are to
 // hide each other's latency: with 14 of 124 registers on an SM, three vectors each, 16384 x 2048 bf16 took 51 us, with 24 of 80 44; rows that
-// bulk copies brought to 16 warps ahead of time 69.
+// bulk copies brought to 16 warps ahead of time 69.  Rows at any address spill from 64 registers: 5003 x 2001 bf16 28.2 us, with 80 26.9.
 constexpr int norm_threads(int G) { return G >= 256 ? G : 256 / G * G; }
-constexpr int norm_blocks(int size, int vpt, int G) {
-  return (vpt == 1 ? (size == 4 ? 768 : 1024) : vpt == 2 ? (size == 4 ? 512 : 768) : 512) / norm_threads(G);
+constexpr int norm_blocks(int size, int vpt, int G, bool aligned) {
+  return (vpt == 1 ? (size == 4 || !aligned ? 768 : 1024) : vpt == 2 ? (size == 4 ? 512 : 768) : 512) / norm_threads(G);
 }
 
 template <typename T, int FMT, int G, int VPT, bool ALIGNED>
-__global__ void __launch_bounds__(norm_threads(G), norm_blocks(sizeof(T), VPT, G)) mx_norm_kernel(const NormArgs a) {
-  constexpr int THREADS = norm_threads(G), W = 4 * Elem<T>::SZ, F32 = sizeof(T) == 4, L = G < 32 ? G : 32, per = THREADS / G;
+__global__ void __launch_bounds__(norm_threads(G), norm_blocks(sizeof(T), VPT, G, ALIGNED)) mx_norm_kernel(const NormArgs a) {
+  constexpr int THREADS = norm_threads(G), W = 4 * Elem<T>::SZ, L = G < 32 ? G : 32, per = THREADS / G;
   __shared__ double red[32];
   __shared__ __align__(16) uint8_t shared[ALIGNED ? 16 : THREADS / L * Stage<T, L>::BYTES];
   pdl_trigger();
@@ -528,43 +528,54 @@ __global__ void __launch_bounds__(norm_threads(G), norm_blocks(sizeof(T), VPT, G
   for (long long first = (long long)blockIdx.x * per; first < a.rows; first += (long long)gridDim.x * per) {
     const long long row = first + threadIdx.x / G;
     const bool live = row < a.rows;
+    const int K = live ? a.K : 0, KR = sum ? K : 0;
     const T* x = reinterpret_cast<const T*>(a.x) + row * a.ldx;
     const T* r = reinterpret_cast<const T*>(a.r) + row * a.ldr;
-    double s = 0.0;
+    // vector i of x and r (a row's threads take each step together, for the way through shared memory)
+    auto take = [&](int i, uint32_t (&wx)[W], uint32_t (&wr)[W]) {
+      if constexpr (ALIGNED) {
+#pragma unroll
+        for (int j = 0; j < W; j++) wx[j] = wr[j] = 0;
+        if (live) {
+          load16<T, true>(x, i * 16, a.K, a.wide, a.ex, wx);
+          if (sum) load16<T, true>(r, i * 16, a.K, a.wide, a.er, wr);
+        }
+      } else {
+        typename Stage<T, L>::Bits bx[16], br[16];
+        stage.fetch(x, (i - stage.lane) * 16, K, stage.lane, bx);
+        stage.fetch(r, (i - stage.lane) * 16, KR, stage.lane, br);
+        stage.turn(bx, wx);
+        stage.turn(br, wr);
+      }
+    };
+    double s = 0.0, v;
+    float root;
+    uint32_t near = 0;                                   // which of the thread's vectors have to come again (the last bit: from the 32nd on)
     if constexpr (VPT > 0) {
       uint64_t h[VPT][8];
-      float lo[F32 ? VPT : 1][16];
       if constexpr (ALIGNED) {
         uint32_t wx[VPT][W], wr[VPT][W];
 #pragma unroll
-        for (int i = 0; i < VPT; i++) {
-          const int k = (t + i * G) * 16;
-#pragma unroll
-          for (int j = 0; j < W; j++) wx[i][j] = wr[i][j] = 0;
-          if (live) {
-            load16<T, true>(x, k, a.K, a.wide, a.ex, wx[i]);
-            if (sum) load16<T, true>(r, k, a.K, a.wide, a.er, wr[i]);
-          }
-        }
+        for (int i = 0; i < VPT; i++) take(t + i * G, wx[i], wr[i]);
 #pragma unroll
         for (int i = 0; i < VPT; i++) {
-          sum16<T>(wx[i], wr[i], h[i], lo[F32 ? i : 0]);     // (zeros without a residual)
+          sum16<T>(wx[i], wr[i], h[i]);                  // (zeros without a residual)
           s += squares(h[i]);
         }
       } else {
         typename Stage<T, L>::Bits bx[VPT][16], br[VPT][16];
 #pragma unroll
         for (int i = 0; i < VPT; i++) {
-          const int k = (t - stage.lane + i * G) * 16, K = live ? a.K : 0;
+          const int k = (t - stage.lane + i * G) * 16;
           stage.fetch(x, k, K, stage.lane, bx[i]);
-          stage.fetch(r, k, sum ? K : 0, stage.lane, br[i]);
+          stage.fetch(r, k, KR, stage.lane, br[i]);
         }
 #pragma unroll
         for (int i = 0; i < VPT; i++) {
           uint32_t wx[W], wr[W];
           stage.turn(bx[i], wx);
           stage.turn(br[i], wr);
-          sum16<T>(wx, wr, h[i], lo[F32 ? i : 0]);
+          sum16<T>(wx, wr, h[i]);
           s += squares(h[i]);
         }
       }
@@ -573,75 +584,67 @@ __global__ void __launch_bounds__(norm_threads(G), norm_blocks(sizeof(T), VPT, G
         for (int i = 0; i < VPT; i++) write_sum<T, ALIGNED, L>(a, row, (t + i * G) * 16, h[i], stage);
       }
       s = row_sum<G>(s, red);
-      const Root root = inverse_root(s, a.inv_K, a.eps);
-      bool near[VPT], any = live && far_out(s);
+      v = fma(s, a.inv_K, a.eps);
+      root = inverse_root(v);
 #pragma unroll
-      for (int i = 0; i < VPT; i++) {
-        near[i] = false;
-        if (live && t + i * G < vecs) near[i] = write_norm<T, FMT, ALIGNED, false>(a, row, (t + i * G) * 16, h[i], lo[F32 ? i : 0], root) || far_out(s);
-        any |= near[i];
-      }
-      if (row_any<G>(any)) {
-        double exact = 0.0;
-#pragma unroll
-        for (int i = 0; i < VPT; i++) exact += squares_exact<F32>(h[i], lo[F32 ? i : 0]);
-        const Root again = inverse_root(row_sum<G>(exact, red), a.inv_K, a.eps);
-#pragma unroll
-        for (int i = 0; i < VPT; i++)
-          if (__ballot_sync(0xffffffffu, near[i]) & 0xffu << (threadIdx.x & 24)) write_norm<T, FMT, ALIGNED, true>(a, row, (t + i * G) * 16, h[i], lo[F32 ? i : 0], again);
-        if (G > 32) __syncthreads();
-      }
+      for (int i = 0; i < VPT; i++)
+        if (live && t + i * G < vecs && (write_norm<T, FMT, ALIGNED>(a, row, (t + i * G) * 16, h[i], root) || far_out(s, v))) near |= 1u << i;
     } else {
-      // (a row's threads take each step together, for the way through shared memory)
-      auto take = [&](int i, uint64_t (&h)[8], float (&lo)[16]) {
-        uint32_t u[W], v[W];
-#pragma unroll
-        for (int j = 0; j < W; j++) v[j] = 0;
-        if constexpr (ALIGNED) {
-          load16<T, true>(x, i * 16, a.K, a.wide, a.ex, u);
-          if (sum) load16<T, true>(r, i * 16, a.K, a.wide, a.er, v);
-        } else {
-          typename Stage<T, L>::Bits raw[16];
-          stage.fetch(x, (i - stage.lane) * 16, a.K, stage.lane, raw);
-          stage.turn(raw, u);
-          stage.fetch(r, (i - stage.lane) * 16, sum ? a.K : 0, stage.lane, raw);
-          stage.turn(raw, v);
-        }
-        sum16<T>(u, v, h, lo);
-      };
       for (int i = t; i - t < vecs; i += G) {
+        uint32_t wx[W], wr[W];
         uint64_t h[8];
-        float lo[16];
-        take(i, h, lo);
+        take(i, wx, wr);
+        sum16<T>(wx, wr, h);
         if (sum) write_sum<T, ALIGNED, L>(a, row, i * 16, h, stage);
         s += squares(h);
       }
       s = row_sum<G>(s, red);
-      const Root root = inverse_root(s, a.inv_K, a.eps);
-      bool any = far_out(s);
-      for (int i = t; i - t < vecs; i += G) {
+      v = fma(s, a.inv_K, a.eps);
+      root = inverse_root(v);
+      for (int i = t, n = 0; i - t < vecs; i += G, n++) {
+        uint32_t wx[W], wr[W];
         uint64_t h[8];
-        float lo[16];
-        take(i, h, lo);
-        if (i < vecs) any |= write_norm<T, FMT, ALIGNED, false>(a, row, i * 16, h, lo, root);
+        take(i, wx, wr);
+        sum16<T>(wx, wr, h);
+        if (i < vecs && (write_norm<T, FMT, ALIGNED>(a, row, i * 16, h, root) || far_out(s, v))) near |= 1u << min(n, 31);
       }
-      if (row_any<G>(any)) {
-        double exact = 0.0;
-        for (int i = t; i - t < vecs; i += G) {
-          uint64_t h[8];
-          float lo[16];
-          take(i, h, lo);
-          exact += squares_exact<F32>(h, lo);
+    }
+    if (row_any<G>(near != 0)) {
+      double exact = 0.0;
+      if constexpr (ALIGNED) {
+        for (int i = t; i < vecs; i += G) {
+          uint32_t wx[W], wr[W];
+          take(i, wx, wr);
+          exact += squares_exact<T>(wx, wr);
         }
-        const Root again = inverse_root(row_sum<G>(exact, red), a.inv_K, a.eps);
-        for (int i = t; i - t < vecs; i += G) {
-          uint64_t h[8];
-          float lo[16];
-          take(i, h, lo);
-          if (i < vecs) write_norm<T, FMT, ALIGNED, true>(a, row, i * 16, h, lo, again);
+      } else {
+        const auto from = [&](const T* p, int k, int K) { return k < K ? element(p, k) : 0.f; };
+#pragma unroll 1
+        for (int k = t; k < K; k += 8 * G) {             // (a sum has any order; eight columns of a thread in flight)
+          float ex[8], er[8];
+#pragma unroll
+          for (int j = 0; j < 8; j++) ex[j] = from(x, k + j * G, K), er[j] = from(r, k + j * G, KR);
+#pragma unroll
+          for (int j = 0; j < 8; j++) {
+            const double h = to_double(ex[j]) + to_double(er[j]);
+            exact = fma(h, h, exact);
+          }
         }
-        __syncthreads();
       }
+      const double rms = sqrt(row_sum<G>(exact, red) / a.K + a.eps);
+      __syncwarp();                                      // the blocks' first codes, of any lane of the warp, are there
+      const int lane = threadIdx.x & 31;
+      const int steps = VPT > 0 ? VPT : (vecs + G - 1) / G;
+#pragma unroll 1
+      for (int n = 0; n < steps; n++) {
+        const unsigned those = __ballot_sync(0xffffffffu, t + n * G < vecs && (near >> min(n, 31) & 1));
+        for (unsigned pairs = (those | those >> 1) & 0x55555555u; pairs != 0; pairs &= pairs - 1) {
+          const int from = __ffs(pairs) - 1;             // the first lane of a block: its row, its columns
+          const double its = G < 32 ? __shfl_sync(0xffffffffu, rms, from) : rms;
+          write_block_exact<T, FMT>(a, first + (threadIdx.x - lane + from) / G, ((threadIdx.x - lane + from) % G + n * G) * 16, its);
+        }
+      }
+      if (G > 32) __syncthreads();
     }
   }
 }

@@ -285,7 +285,7 @@ def AddRMSNormMX(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
         raise TypeError("AddRMSNormMX: weight dtype must equal the input dtype or be float32")
     if not x.is_cuda:
         h = a.double() if r is None else a.double() + r.double()
-        y = h * torch.rsqrt(h.square().mean(-1, keepdim=True) + eps) * weight.detach().double()
+        y = h / torch.sqrt(h.square().sum(-1, keepdim=True) / K + eps) * weight.detach().double()
         return _quantize_ref(y, fmt, shape), (x if r is None else h.to(x.dtype).reshape(shape))
     w = weight if weight.is_contiguous() else weight.contiguous()
     q, codes, scales = _empty(rows, shape, fmt, a)

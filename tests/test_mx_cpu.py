@@ -302,3 +302,14 @@ def test_train_linear_mixed_types(xt, wt, bt):
     grads = torch.autograd.grad(y.sum(), (x, w, b))
     assert y.dtype == xt and [g.dtype for g in grads] == [xt, wt, bt]
     assert torch.equal(grads[2].float(), torch.full((9,), 6.0))
+
+
+@pytest.mark.parametrize("format", FORMATS)
+def test_norm_of_rows_of_one_value(format):
+    """Without eps a value's quotient is 1 and the norm the weight, ties between two codes among them."""
+    c = torch.arange(1, 201, dtype=torch.float64)
+    for K in (32, 48, 1001):
+        w = torch.randint(16, 32, (K,)).double() / 16
+        q, _ = Q.AddRMSNormMX(c[:, None].expand(200, K), None, w, 0.0, format)
+        want = Q.QuantizeMX(w.expand(200, K), format)
+        assert torch.equal(q.Data, want.Data) and torch.equal(q.ScaleCodes(), want.ScaleCodes())

@@ -695,3 +695,84 @@ def test_exact_gelu_of_far_values(status_ok):
     y = Q.MatMulMX(zero, w, v, torch.float32, "geluexact")[0]
     assert torch.isnan(y[[3, 6]]).all() and y[:3].abs().max() < 1e-15
     assert torch.equal(y[[4, 5, 7, 8, 9]], v[[4, 5, 7, 8, 9]])
+
+
+def norm64(x, r, w, eps):
+    """The definition.  (K as a tensor: by a number, ``mean`` and ``/`` multiply with a rounded 1 / K on the device; 1003 x 1.0 / 1003 is not 1 then, and
+    in rows of one value what are ties would not be any.)"""
+    t = x.double() if r is None else x.double() + r.double()
+    K = torch.tensor(float(t.shape[-1]), dtype=torch.float64, device=t.device)
+    return t / torch.sqrt(t.square().sum(-1, keepdim=True) / K + eps) * w.double()
+
+
+def norm_codes(x, r, w, eps, format):
+    """Codes and scales have to be those of the definition in 64 bits."""
+    q, _ = Q.AddRMSNormMX(x, r, w, eps, format)
+    equal(q, Q.microscale._quantize_ref(norm64(x, r, w, eps).cpu(), int(format == "mxfp4"), tuple(x.shape)))
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("K", [96, 768, 1003, 2304, 20000])
+def test_norm_of_far_rows(format, dtype, K, status_ok):
+    """Rows whose 1 / rms, or the sum of x and the residual, fp32 does not hold, and rows of subnormal numbers."""
+    w = (torch.rand(K, device=DEV) + 0.5).to(dtype)
+    for e in (-130, -140, -100, 60, 120):
+        x, r = (torch.randn(40, K, device=DEV) * 2.0 ** (e + 20) * 2.0 ** -20 for _ in range(2))
+        for eps in (0.0, 1e-6):
+            norm_codes(x.to(dtype), r.to(dtype), w, eps, format)
+    x = torch.full((3, K), 3e38, device=DEV).to(dtype)
+    norm_codes(x, x, w, 0.0, format)
+    norm_codes(torch.randn(40, K, device=DEV).to(dtype), None, w, 1e40, format)
+
+
+@pytest.mark.parametrize("format", FORMATS)
+def test_norm_of_rows_of_one_value(format, status_ok):
+    """Without eps a value's quotient is 1, and its product a tie between two codes where the weight is one."""
+    c = torch.arange(1, 2001, device=DEV).float()
+    for K in (32, 48, 768, 1001):
+        w = torch.randint(16, 32, (K,), device=DEV).float() / 16
+        norm_codes(c[:, None].expand(2000, K), None, w, 0.0, format)
+        norm_codes(c[:, None].expand(2000, K).bfloat16().float(), None, -w, 0.0, format)
+
+
+@pytest.mark.parametrize("format", FORMATS)
+def test_norm_with_far_weights(format, status_ok):
+    """Products with the weight that fp32 does not hold are values of blocks with larger scales."""
+    x = torch.zeros(4, 96, device=DEV)
+    x[0, 3], x[1], x[2, 40:], x[3, 60] = 1, 1, 5, -7
+    for w in (3e38, 2e38, 1e37, 1e-38):
+        norm_codes(x, None, torch.full((96,), w, device=DEV), 1e-6, format)
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("K", [1, 40, 200, 1001, 20001])
+def test_norm_pads_rows_of_nan_with_zeros(format, K, status_ok):
+    """Codes and scales behind the last value and the last block are zeros whatever the row holds."""
+    x = torch.randn(5, K, device=DEV)
+    x[1, K // 2] = math.nan
+    x[2] = 0
+    x[3, K // 3] = math.inf
+    q = cpu(Q.AddRMSNormMX(x, None, torch.ones(K, device=DEV), 0.0, format)[0])
+    assert (q.ScaleCodes()[1:3] == 255).all()
+    used = K if format == "mxfp8" else (K + 1) // 2
+    assert not q.Data[:, used:].any() and (format == "mxfp8" or K % 2 == 0 or not (q.Data[:, used - 1] >> 4).any())
+    s = q.Scales.view(1, -1, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(128, -1)
+    assert not s[:5, -(-K // 32):].any()
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("K", [262144, 300001])
+def test_norm_of_very_long_rows(format, K, status_ok):
+    """More than 32 vectors of a thread, the last of them not of every thread; what lies behind the result stays as it was."""
+    x, r, w = torch.randn(3, K, device=DEV), torch.randn(3, K, device=DEV), torch.rand(K, device=DEV) + 0.5
+    x[1] *= 2.0 ** -70
+    r[1] *= 2.0 ** -70
+    norm_codes(x, r, w, 1e-30, format)
+    norm_codes(x.bfloat16(), None, w.bfloat16(), 1e-30, format)
+    fmt = int(format == "mxfp4")
+    codes, scales = 3 * Q.microscale._row_bytes(K, fmt), Q.microscale._pieces(K, fmt) * 512
+    data, s = torch.full((codes + 64,), 77, dtype=torch.uint8, device=DEV), torch.full((scales + 64,), 77, dtype=torch.uint8, device=DEV)
+    h = torch.empty_like(x)
+    _l.call("gb_mx_add_rms_norm", 2, fmt, x.data_ptr(), K, r.data_ptr(), K, w.data_ptr(), 1, h.data_ptr(), data.data_ptr(), s.data_ptr(), 3, K, 1e-30, _l.current_stream_handle())
+    assert (data[codes:] == 77).all() and (s[scales:] == 77).all() and (s[:scales].view(-1, 32, 4, 4)[:, :, 1:] == 77).all()
