@@ -451,7 +451,9 @@ __device__ __forceinline__ bool write_norm(const NormArgs& a, long long row, int
   float w[16], y[16];
   weights16<T, ALIGNED>(a, k, w);
   const uint64_t root2 = pair_of(root, root);
-  // for the test, zeros become a number far from any border (sums of bf16 values are zero now and then) and others stay what they are
+  // for the test, zeros become a number far from any border (sums of bf16 values are zero now and then) and others from 2^-101 on stay what they
+  // are; lanes whose largest value is so small that the others count come again whole.  (What this does not see: a product with 1 / rms that is
+  // subnormal, of a value 2^126 times below the row's, and comes back through a weight above 2^27.)
   const uint64_t tiny = pair_of(__uint_as_float(0x00955555u), __uint_as_float(0x00955555u));
   uint32_t near = ~0u;
   float m = 0.f;
@@ -469,6 +471,12 @@ __device__ __forceinline__ bool write_norm(const NormArgs& a, long long row, int
   const uint32_t word = quantize16<FMT>(y, __float_as_uint(m), 0xffu << (lane & 24), lane, out);
   store_codes<FMT>(a.data + row * a.row_bytes, k, a.row_bytes, out);
   if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_word(row, k >> 7, a.pieces)) = word;
+  if (m < 0x1p-80f) {                    // (a block's borders go down to 2^-19 of its largest value)
+    uint32_t some = 0;
+#pragma unroll
+    for (int j = 0; j < 16; j++) some |= __float_as_uint(y[j]) & 0x7fffffffu;
+    return some != 0;
+  }
   return near <= kNear<FMT>;
 }
 template <typename T> __device__ __forceinline__ float element(const T* from, long long i) {

@@ -270,7 +270,7 @@ def AddRMSNormMX(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
     """``h = x + residual`` and the quantised ``h / sqrt(mean(h^2) + eps) * weight``: what a pre-norm block hands to its next
     products, and the stream that goes on beside them.  Returns (codes and scales, h).  The norm takes the sum before it is rounded to
     h's type; a value is rounded once, to its code: none of the arithmetic before moves one that lies next to the border between two
-    codes to the other.  Without a residual h is x itself."""
+    codes to the other (for weights up to 2^27).  Without a residual h is x itself."""
     fmt, shape = _format(format), tuple(x.shape)
     a = _rows(x, "AddRMSNormMX")
     rows, K = a.shape

@@ -776,3 +776,43 @@ def test_norm_of_very_long_rows(format, K, status_ok):
     h = torch.empty_like(x)
     _l.call("gb_mx_add_rms_norm", 2, fmt, x.data_ptr(), K, r.data_ptr(), K, w.data_ptr(), 1, h.data_ptr(), data.data_ptr(), s.data_ptr(), 3, K, 1e-30, _l.current_stream_handle())
     assert (data[codes:] == 77).all() and (s[scales:] == 77).all() and (s[:scales].view(-1, 32, 4, 4)[:, :, 1:] == 77).all()
+
+
+def power(e):
+    """2^e in 64 bits from its bits (a library's power is off by one)."""
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
+def nearest64(y, format):
+    """The values that codes and scales of y stand for, in 64 bits and where y is."""
+    mant, least, top, largest = (3, -6, 8, 448.0) if format == "mxfp8" else (1, 0, 2, 6.0)
+    rows, K = y.shape
+    v = torch.nn.functional.pad(y, (0, -K % 32)).view(rows, -1, 32)
+    big = v.abs().amax(-1, keepdim=True)
+    e = torch.where(big == 0, -127, torch.frexp(big).exponent - 1 - top).clamp(-127, 127)
+    v = v * power(-e)
+    step = power((torch.frexp(v).exponent - 1).clamp(min=least) - mant)
+    return ((torch.round(v / step) * step).clamp(-largest, largest) * power(e)).view(rows, -1)[:, :K]
+
+
+def norm_values(x, r, w, eps, format):
+    """As norm_codes, on the device."""
+    q, _ = Q.AddRMSNormMX(x, r, w, eps, format)
+    assert torch.equal(Q.DequantizeMX(q).double(), nearest64(norm64(x, r, w, eps), format))
+
+
+def test_nearest_is_the_oracle():
+    for format in FORMATS:
+        y = torch.randn(50, 333, dtype=torch.float64) * torch.exp2(torch.randint(-90, 90, (50, 1)).double())
+        assert torch.equal(nearest64(y, format), Q.DequantizeMX(Q.QuantizeMX(y, format), torch.float64))
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("e", [-85, -100, -110, -118])
+def test_norm_of_small_blocks(format, e, status_ok):
+    """Blocks of values far below the row's others, whose borders count as well: 28 million, of which fp32's roundings move some."""
+    x, w = torch.randn(40000, 768, device=DEV), torch.rand(768, device=DEV) + 0.5
+    x[:, 64:] *= 2.0 ** e
+    norm_values(x, None, w, 1e-6, format)
+    x[:, 70::32] = 0
+    norm_values(x[:20000], x[20000:], w, 1e-6, format)
