@@ -810,13 +810,12 @@ Choice best_clusters(long long M, long long N, int steps) {
   for (int bn = M <= 16 ? 16 : 32; bn <= (M <= 16 ? 16 : 128); bn *= 2) {
     if (g_rows && M > 16 && bn != g_rows) continue;
     const long long tiles = ((M + bn - 1) / bn) * ((N + 127) / 128);
-    for (int s = 1; s <= 8; s *= 2) {
-      if (g_splits ? s != (g_splits < 8 ? g_splits : 8) : (s > 1 && (s > steps || tiles * s > 296))) continue;
+    for (int s = g_splits ? g_splits : 1; s <= 8; s *= 2) {
+      if (g_splits ? s != g_splits : s > 1 && (s > steps || tiles * s > 296)) break;
       const double us = cluster_us(M, bn, tiles, steps, s);
       if (us < c.us) c = {bn, s, us};
     }
   }
-  if (c.rows == 0) c = {g_rows && M > 16 ? g_rows : M <= 16 ? 16 : 128, 1, 1e300};       // (slices were asked for that there are not)
   return c;
 }
 Choice best_pairs(long long M, long long N, int steps) {
@@ -890,9 +889,10 @@ int launch_cluster(const Maps& tm, const void* sa, const void* sb, const MxArgs&
 }  // namespace
 
 // The kernel of products from this thread: kind 0 by size, 1 pairs, 2 clusters, 32, 64 or 128 clusters with tiles of so many rows (above 16 rows
-// of C); splits 0 by size, else that many slices of K.
+// of C); splits 0 by size, else that many slices of K: up to two of pairs, eight of clusters.  (Of a single step of K a pair takes no half.)
 GB_EXPORT int gb_mx_tune(int kind, int splits) {
-  if (((kind < 0 || kind > 2) && kind != 32 && kind != 64 && kind != 128) || splits < 0 || splits > 64) {
+  const int most = kind == 0 ? 0 : kind == 1 ? 2 : 8;
+  if (((kind < 0 || kind > 2) && kind != 32 && kind != 64 && kind != 128) || splits < 0 || splits > most) {
     gbh::set_error("gb_mx_tune: kind %d, splits %d", kind, splits);
     return gbh::E_BAD_ARG;
   }
@@ -902,12 +902,15 @@ GB_EXPORT int gb_mx_tune(int kind, int splits) {
   return gbh::E_OK;
 }
 
+static bool bad_extents(const char* what, long long M, long long N, long long K, int fmt) {
+  if (M > 0 && N > 0 && K > 0 && M <= 0x7fffffffLL && N <= 0x7fffffffLL && K <= (1LL << 30) && (fmt == FP8 || fmt == FP4)) return false;
+  gbh::set_error("%s: bad extents %lld x %lld x %lld, format %d", what, M, N, K, fmt);
+  return true;
+}
+
 // How a product runs (for tests): 1 pairs, 2 clusters; rows of a tile; slices of K.
 GB_EXPORT int gb_mx_plan(long long M, long long N, long long K, int fmt, long long* out3) {
-  if (M <= 0 || N <= 0 || K <= 0 || M > 0x7fffffffLL || N > 0x7fffffffLL || K > (1LL << 30) || (fmt != FP8 && fmt != FP4)) {
-    gbh::set_error("gb_mx_plan: bad extents %lld x %lld x %lld, format %d", M, N, K, fmt);
-    return gbh::E_BAD_ARG;
-  }
+  if (bad_extents("gb_mx_plan", M, N, K, fmt)) return gbh::E_BAD_ARG;
   const Plan p = plan_of(M, N, K, fmt);
   out3[0] = p.pair ? 1 : 2;
   out3[1] = p.bn;
@@ -918,8 +921,7 @@ GB_EXPORT int gb_mx_plan(long long M, long long N, long long K, int fmt, long lo
 // C (M x N, rows ldc apart) = act(A B^T + bias).  out: DT_BF16, DT_F16 or DT_F32; bias in C's type or fp32 (bias_f32), or null.
 GB_EXPORT int gb_mx_matmul(int fmt, const void* a, const void* sa, const void* b, const void* sb, void* c, long long ldc, const void* bias, int bias_f32, long long M,
                            long long N, long long K, int out, int act, void* stream) {
-  long long p3[3];
-  if (int rc = gb_mx_plan(M, N, K, fmt, p3)) return rc;
+  if (bad_extents("gb_mx_matmul", M, N, K, fmt)) return gbh::E_BAD_ARG;
   if (out < 0 || out > 2 || act < 0 || act > 3 || ldc < N) {
     gbh::set_error("gb_mx_matmul: bad type %d, activation %d or row pitch %lld", out, act, ldc);
     return gbh::E_BAD_ARG;
@@ -931,6 +933,12 @@ GB_EXPORT int gb_mx_matmul(int fmt, const void* a, const void* sa, const void* b
   const Plan p = plan_of(M, N, K, fmt);
   const int P = pieces((int)K, fmt), RB = row_bytes((int)K, fmt), per = fmt == FP8 ? 1 : 2;
   MxArgs args{};
+  args.num_m = (int)((M + p.bn - 1) / p.bn);
+  args.num_n = (int)(p.pair ? (N + 255) / 256 : (N + 127) / 128);
+  if ((long long)args.num_m * args.num_n * p.splits * (p.pair ? 2 : 1) > 0x7fffffffLL) {
+    gbh::set_error("gb_mx_matmul: %lld x %lld has too many tiles", M, N);
+    return gbh::E_TOO_LARGE;
+  }
   args.M = (int)M; args.N = (int)N; args.steps = p.steps;
   args.splits = p.splits; args.steps_per = p.steps_per;
   args.C = c; args.ldc = ldc; args.bias = bias; args.bias_f32 = bias_f32 || out == OUT_F32; args.act = act; args.out = out;
@@ -940,8 +948,6 @@ GB_EXPORT int gb_mx_matmul(int fmt, const void* a, const void* sa, const void* b
   memset(&tm, 0, sizeof(tm));
   if (p.pair) {
     int rc = 0;
-    args.num_m = (int)((M + 255) / 256);
-    args.num_n = (int)((N + 255) / 256);
     const int size = out == OUT_F32 ? 4 : 2;
     const auto whole = [&](int bytes) { return (uintptr_t)c % bytes == 0 && ldc * size % bytes == 0 && N * size % bytes == 0; };
     args.vectors = whole(32) ? 32 : whole(16) ? 16 : 0;
@@ -957,12 +963,6 @@ GB_EXPORT int gb_mx_matmul(int fmt, const void* a, const void* sa, const void* b
     if (args.vectors) return fmt == FP8 ? launch_pair<FP8, true, false>(tm, args, st) : launch_pair<FP4, true, false>(tm, args, st);
     return fmt == FP8 ? launch_pair<FP8, false, false>(tm, args, st) : launch_pair<FP4, false, false>(tm, args, st);
   }
-  args.num_m = (int)((M + p.bn - 1) / p.bn);
-  args.num_n = (int)((N + 127) / 128);
-  if ((long long)args.num_m * args.num_n * p.splits > 0x7fffffffLL) {
-    gbh::set_error("gb_mx_matmul: %lld x %lld has too many tiles", M, N);
-    return gbh::E_TOO_LARGE;
-  }
   if (int rc = map_codes(&tm.a, b, N, RB, 128)) return rc;
   if (int rc = map_codes(&tm.b, a, M, RB, p.bn)) return rc;
   switch (p.bn) {
@@ -976,8 +976,7 @@ GB_EXPORT int gb_mx_matmul(int fmt, const void* a, const void* sa, const void* b
 // The same for up to 16 rows of x as they are (bf16, fp16 or fp32, K elements, ld apart), quantised within the product's kernel.
 GB_EXPORT int gb_mx_matmul_rows(int dtype, int fmt, const void* x, long long ld, const void* b, const void* sb, void* c, long long ldc, const void* bias, int bias_f32,
                                 long long M, long long N, long long K, int out, int act, void* stream) {
-  long long p3[3];
-  if (int rc = gb_mx_plan(M, N, K, fmt, p3)) return rc;
+  if (bad_extents("gb_mx_matmul_rows", M, N, K, fmt)) return gbh::E_BAD_ARG;
   if (M > 16 || dtype < 0 || dtype > 2 || out < 0 || out > 2 || act < 0 || act > 3 || ldc < N || ld < 0) {
     gbh::set_error("gb_mx_matmul_rows: %lld rows (16 at most), types %d and %d, activation %d, row pitches %lld and %lld", M, dtype, out, act, ld, ldc);
     return gbh::E_BAD_ARG;

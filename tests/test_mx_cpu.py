@@ -1,5 +1,6 @@
 """Microscaled formats on CPU tensors: the oracle against a plain restatement of the definition, layouts, refusals, layers."""
 import copy
+import ctypes
 import math
 import pickle
 
@@ -313,3 +314,43 @@ def test_norm_of_rows_of_one_value(format):
         q, _ = Q.AddRMSNormMX(c[:, None].expand(200, K), None, w, 0.0, format)
         want = Q.QuantizeMX(w.expand(200, K), format)
         assert torch.equal(q.Data, want.Data) and torch.equal(q.ScaleCodes(), want.ScaleCodes())
+
+
+def plan(M, N, K, format):
+    out = (ctypes.c_longlong * 3)()
+    _l.check(_l.lib().gb_mx_plan(M, N, K, FORMATS.index(format), ctypes.addressof(out)), "gb_mx_plan")
+    return tuple(out)
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("M,N,K", [(3, 40, 1500), (70, 264, 1500), (520, 1032, 700), (5000, 4000, 4100)])
+def test_a_product_runs_as_it_is_told(format, M, N, K):
+    """Every kernel, tile and number of slices that gb_mx_tune takes is the one that runs; others are refused, and leave things as they were."""
+    tune = _l.lib().gb_mx_tune
+    try:
+        for kind, most in ((0, 0), (1, 2), (2, 8), (32, 8), (64, 8), (128, 8)):
+            for splits in range(1, 10):
+                _l.check(tune(0, 0))
+                if splits > most:
+                    with pytest.raises(RuntimeError, match="splits"):
+                        _l.check(tune(kind, splits))
+                    continue
+                by_size = plan(M, N, K, format)
+                _l.check(tune(kind, splits))
+                got = plan(M, N, K, format)
+                rows = 256 if kind == 1 else 16 if M <= 16 else kind if kind > 2 else got[1]
+                assert got == (1 if kind == 1 else 2, rows, splits) and rows in (16, 32, 64, 128, 256)
+                _l.check(tune(0, 0))
+                assert plan(M, N, K, format) == by_size
+    finally:
+        tune(0, 0)
+
+
+def test_products_that_no_launch_holds():
+    for kind in (1, 2):
+        try:
+            _l.check(_l.lib().gb_mx_tune(kind, 1))
+            with pytest.raises(RuntimeError, match="too many tiles"):
+                _l.check(_l.lib().gb_mx_matmul(0, A, A, A, A, A, 1 << 31, None, 0, (1 << 31) - 1, (1 << 31) - 1, 64, 0, 0, None))
+        finally:
+            _l.lib().gb_mx_tune(0, 0)

@@ -816,3 +816,20 @@ def test_norm_of_small_blocks(format, e, status_ok):
     norm_values(x, None, w, 1e-6, format)
     x[:, 70::32] = 0
     norm_values(x[:20000], x[20000:], w, 1e-6, format)
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("splits", range(1, 9))
+def test_every_number_of_slices(format, splits, status_ok):
+    """Slices of K over clusters of so many CTAs, some of which have none."""
+    for kind in (2, 32, 64, 128):
+        for M, N, K in ((5, 200, 1700), (70, 264, 1500), (300, 512, 260)):
+            _l.check(_l.lib().gb_mx_tune(kind, splits))
+            try:
+                y, want = product(M, N, K, format, torch.float32, True, None)
+                assert torch.equal(y, want)
+                if M <= 16:
+                    x, w = whole(M, K, format).to(DEV), Q.QuantizeMX(whole(N, K, format).to(DEV), format)
+                    assert torch.equal(Q.LinearMX(x, w), Q.MatMulMX(Q.QuantizeMX(x, format), w, dtype=torch.float32))
+            finally:
+                _l.lib().gb_mx_tune(0, 0)
