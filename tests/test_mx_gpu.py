@@ -3,6 +3,7 @@
 Quantised codes have to be equal: rounding is part of the format.  Products are first taken of values whose sums the fp32
 accumulator holds exactly (whole numbers times powers of two, every partial sum below 2^24 units), so that results have to be
 equal as well; random operands follow with tolerances that count roundings."""
+import ctypes
 import math
 
 import pytest
@@ -833,3 +834,51 @@ def test_every_number_of_slices(format, splits, status_ok):
                     assert torch.equal(Q.LinearMX(x, w), Q.MatMulMX(Q.QuantizeMX(x, format), w, dtype=torch.float32))
             finally:
                 _l.lib().gb_mx_tune(0, 0)
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("M,N,K", [(4600, 4900, 300), (4600, 4904, 1100), (4599, 4901, 300), (9000, 9000, 40)])
+def test_pairs_of_many_tiles(format, M, N, K, status_ok):
+    """Four tiles and more a pair of CTAs: accumulators, barriers and the bias' buffers come round more than once.  A bias of its own in every column."""
+    a, b = whole(M, K, format).to(DEV), whole(N, K, format).to(DEV)
+    qa, qb = Q.QuantizeMX(a, format), Q.QuantizeMX(b, format)
+    bias = torch.arange(N, device=DEV).float() - N // 2
+    want = a.double() @ b.double().T
+    _l.check(_l.lib().gb_mx_tune(1, 1))
+    try:
+        out = (ctypes.c_longlong * 3)()
+        _l.check(_l.lib().gb_mx_plan(M, N, K, FORMATS.index(format), ctypes.addressof(out)))
+        assert tuple(out) == (1, 256, 1) and -(-M // 256) * -(-N // 256) >= 4 * 74
+        for dtype, v, act in ((torch.float32, bias, None), (torch.bfloat16, None, None), (torch.float16, bias.half(), "relu"), (torch.bfloat16, bias.bfloat16(), None)):
+            full = want if v is None else want + v.double()
+            full = (full.relu() if act else full).to(dtype)
+            for _ in range(3):
+                y = Q.MatMulMX(qa, qb, v, dtype, act)
+                _l.assert_status_ok()
+                assert torch.equal(y, full)
+    finally:
+        _l.lib().gb_mx_tune(0, 0)
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("K", [768, 776, 1536, 2304, 4096, 8192])
+def test_norm_codes_of_many_rows(format, dtype, K, status_ok):
+    """Every way of dealing out rows that L2 does not keep, every value: with and without a residual, weights of the rows' type and of fp32."""
+    rows = (9 << 20) // K + 7
+    x, r = torch.randn(rows, K, device=DEV).to(dtype), torch.randn(rows, K, device=DEV).to(dtype)
+    w = torch.rand(K, device=DEV) + 0.5
+    norm_values(x, r, w.to(dtype), 1e-6, format)
+    norm_values(x, None, w, 1e-6, format)
+    norm_values(x, r, w, 1e-6, format)
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,K", [(60000, 100), (60000, 256), (20000, 300), (8000, 1003), (4000, 2001), (2000, 4100), (2000, 8001), (300, 40001)])
+def test_norm_codes_of_either_way(format, dtype, rows, K, status_ok):
+    """The same for rows of any length that stay in L2, and at any address."""
+    x, r = torch.randn(rows, K, device=DEV).to(dtype), torch.randn(rows, K, device=DEV).to(dtype)
+    w = torch.rand(K, device=DEV) + 0.5
+    norm_values(x, r, w.to(dtype), 1e-6, format)
+    norm_values(x, None, w, 1e-6, format)
