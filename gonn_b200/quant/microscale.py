@@ -372,9 +372,9 @@ def LinearMX(x: Union[torch.Tensor, QTensorMX], weight: QTensorMX, bias: Optiona
 
 class _TrainLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias):
+    def forward(ctx, x, weight, bias, taped):
         N, K = weight.shape
-        need_x, need_w, _ = ctx.needs_input_grad
+        need_x, need_w = (taped and n for n in ctx.needs_input_grad[:2])      # (parameters ask for gradients without a tape too)
         a, w = _rows(x, "TrainLinearMX"), _rows(weight, "TrainLinearMX")
         M = a.shape[0]
         ctx.meta = (x.shape, x.dtype, M, N, K, need_x, need_w)
@@ -383,9 +383,8 @@ class _TrainLinear(torch.autograd.Function):
         if M == 0:
             return y
         if not x.is_cuda:
-            xq, xt = QuantizeMXPair(a)
-            wq, wt = QuantizeMXPair(w)
-            ctx.save_for_backward(xt.Data, xt.Scales, wt.Data, wt.Scales)
+            (xq, xt), (wq, wt) = (QuantizeMXPair(t) if need else (QuantizeMX(t), None) for t, need in ((a, need_w), (w, need_x)))
+            ctx.save_for_backward(*(v for t in (xt, wt) for v in ((None, None) if t is None else (t.Data, t.Scales))))
             return MatMulMX(xq, wq, bias, x.dtype).view(y.shape)
         sizes = _l.lib().gb_mx_train_bytes
         kept = scratch = None
@@ -409,7 +408,7 @@ class _TrainLinear(torch.autograd.Function):
         dx = dw = db = None
         if M == 0:
             return (dy.new_zeros(xshape, dtype=xdtype) if need_x else None, emit_grad(weight, torch.zeros_like(weight)) if need_w else None,
-                    emit_grad(bias, torch.zeros_like(bias)) if need_b else None)
+                    emit_grad(bias, torch.zeros_like(bias)) if need_b else None, None)
         g = _rows(dy, "TrainLinearMX")
         if not dy.is_cuda:
             xt, xs, wt, ws = ctx.saved_tensors
@@ -439,13 +438,13 @@ class _TrainLinear(torch.autograd.Function):
                 db = emit_grad(bias, column_sum(g, out_dtype=torch.float32).to(bias.dtype) if db is None else db)
         if dw is not None:
             dw = emit_grad(weight, dw)
-        return dx, dw, db
+        return dx, dw, db, None
 
 
 def TrainLinearMX(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``Q(x) Q(W)^T + b`` in MXFP8 with gradients that go straight through the rounding; every product's operands are quantised
     along its contraction: dx = Q(dy) Q(W^T)^T, dW = Q(dy^T) Q(x^T)^T, db = column sums of dy.  For the backward pass the layer
-    keeps the codes of x^T and W^T, a byte a value.  Into a CUDA graph, capture it with ``torch.autograd.grad`` or ``GraphedStep``
+    keeps the codes of x^T and W^T, a byte a value; without a tape it neither makes nor keeps them.  Into a CUDA graph, capture it with ``torch.autograd.grad`` or ``GraphedStep``
     (``backward()`` adds to gradients on the stream that saw a parameter first, which a capture cannot follow)."""
     if weight.dim() != 2 or x.dim() == 0 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"TrainLinearMX: shapes {tuple(x.shape)} and {tuple(weight.shape)} do not match (..., K) and (N, K)")
@@ -455,7 +454,7 @@ def TrainLinearMX(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
         raise ValueError("TrainLinearMX: a layer needs outputs")
     if bias is not None and (bias.shape != weight.shape[:1] or bias.device != x.device):
         raise ValueError(f"TrainLinearMX: bias must have shape ({weight.shape[0]},) on {x.device}")
-    return _TrainLinear.apply(x, weight, bias)
+    return _TrainLinear.apply(x, weight, bias, torch.is_grad_enabled())
 
 
 # ---------------------------------------------------------------------------------------

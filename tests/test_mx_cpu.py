@@ -354,3 +354,18 @@ def test_products_that_no_launch_holds():
                 _l.check(_l.lib().gb_mx_matmul(0, A, A, A, A, A, 1 << 31, None, 0, (1 << 31) - 1, (1 << 31) - 1, 64, 0, 0, None))
         finally:
             _l.lib().gb_mx_tune(0, 0)
+
+
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+def test_a_training_layer_without_a_tape_keeps_nothing(mode, monkeypatch):
+    layer, x = Q.NewMXTrainLinearFrom(Linear(40, 24)), torch.randn(6, 40, requires_grad=True)
+    want = layer(x).detach()
+    monkeypatch.setattr(Q.microscale, "QuantizeMXPair", lambda t: pytest.fail("quantised for gradients that nobody asks for"))
+    with mode():
+        y = layer(x)
+    assert torch.equal(y, want) and not y.requires_grad
+    monkeypatch.undo()
+    pairs = []
+    monkeypatch.setattr(Q.microscale, "QuantizeMXPair", lambda t, f=Q.QuantizeMXPair: (pairs.append(tuple(t.shape)), f(t))[1])
+    layer(x.detach()).sum().backward()                 # x, whose transpose dW takes; the gradient of y
+    assert pairs == [(6, 40), (6, 24)]

@@ -882,3 +882,30 @@ def test_norm_codes_of_either_way(format, dtype, rows, K, status_ok):
     w = torch.rand(K, device=DEV) + 0.5
     norm_values(x, r, w.to(dtype), 1e-6, format)
     norm_values(x, None, w, 1e-6, format)
+
+
+def native_calls(run):
+    """(name, arguments) of the native calls of run()."""
+    calls = []
+
+    def hook(name, fn, args):
+        calls.append((name, args))
+        return fn(*args)
+
+    _l.set_call_hook(hook)
+    try:
+        run()
+    finally:
+        _l.set_call_hook(None)
+    return calls
+
+
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+def test_a_training_layer_without_a_tape_keeps_nothing(mode, status_ok):
+    layer, x = Q.NewMXTrainLinearFrom(Linear(512, 256)).to(DEV), torch.randn(100, 512, device=DEV, requires_grad=True)
+    want = layer(x).detach()
+    with mode():
+        ((name, args),) = native_calls(lambda: layer(x))
+        assert name == "gb_mx_train_forward" and args[12:16] == (False, False, None, 0)
+        y = layer(x)
+    assert torch.equal(y, want) and not y.requires_grad
