@@ -49,7 +49,10 @@ KERNELS_PER_CALL = {
     "gb_norm_bwd": 2, "gb_channel_sum": 2, "gb_ce_fwd": 2, "gb_ce_fused": 2, "gb_flash_bwd": 2, "gb_flash_bwd_ws": 2, "gb_embedding_bwd": 5,
     "gb_status_read": 0, "gb_comm_alloc": 0, "gb_comm_open": 0, "gb_comm_emulate": 0,
     "gb_comm_free": 0, "gb_reduce": 1, "gb_gemm_f32x3": 3, "gb_conv_wgrad": 2, "gb_conv_cl_fwd": 2, "gb_conv_cl_bwd": 4, "gb_stack_fwd": 0, "gb_set_words": 1, "gb_norm_bwd_res": 2, "gb_q_dynamic": 2,
-    "gb_mx_linear": 2, "gb_mx_train_forward": 3, "gb_mx_train_backward": 4,
+    # by the arguments: up to 16 rows take one; of dX, dW and db those that there are, and the gradient's quantisation
+    "gb_mx_linear": lambda a: 1 if a[9] <= 16 else 2,
+    "gb_mx_train_forward": 3,
+    "gb_mx_train_backward": lambda a: 1 + sum(a[i] is not None for i in (4, 6, 8)),
 }
 
 
@@ -152,7 +155,8 @@ def call(name: str, *args) -> None:
         fn = _fn_cache[name] = getattr(lib(), name)
     rc = fn(*args) if _call_hook is None else _call_hook(name, fn, args)
     launch_count += 1
-    kernel_count += KERNELS_PER_CALL.get(name, 1)
+    n = KERNELS_PER_CALL.get(name, 1)
+    kernel_count += n if n.__class__ is int else n(args)
     if rc != 0:
         check(rc, name)
 

@@ -369,3 +369,20 @@ def test_a_training_layer_without_a_tape_keeps_nothing(mode, monkeypatch):
     monkeypatch.setattr(Q.microscale, "QuantizeMXPair", lambda t, f=Q.QuantizeMXPair: (pairs.append(tuple(t.shape)), f(t))[1])
     layer(x.detach()).sum().backward()                 # x, whose transpose dW takes; the gradient of y
     assert pairs == [(6, 40), (6, 24)]
+
+
+@pytest.mark.parametrize("name,args,kernels", [
+    ("gb_mx_linear", (0, 0, A, 64, A, A, A, None, 0, 16, 8, 64, 0, 0, None, 0, None), 1),
+    ("gb_mx_linear", (0, 0, A, 64, A, A, A, None, 0, 17, 8, 64, 0, 0, A, 4096, None), 2),
+    ("gb_mx_train_backward", (0, A, 8, A, A, 0, A, 0, A, 0, 4, 8, 64, A, 4096, None), 4),
+    ("gb_mx_train_backward", (0, A, 8, A, A, 0, A, 0, None, 0, 4, 8, 64, A, 4096, None), 3),
+    ("gb_mx_train_backward", (0, A, 8, A, A, 0, None, 0, None, 0, 4, 8, 64, A, 4096, None), 2),
+    ("gb_mx_train_forward", (0, 0, A, 64, A, 64, A, None, 0, 4, 8, 64, 1, 1, A, 4096, A, 4096, None), 3),
+    ("gb_mx_quantize", (0, 0, A, 64, A, A, 4, 64, None), 1),
+])
+def test_kernels_that_a_call_launches(name, args, kernels, monkeypatch):
+    """The count goes by the arguments (nothing is launched here)."""
+    monkeypatch.setitem(_l._fn_cache, name, lambda *a: 0)
+    before = _l.kernel_count
+    _l.call(name, *args)
+    assert _l.kernel_count - before == kernels
