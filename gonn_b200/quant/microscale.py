@@ -265,12 +265,26 @@ def DequantizeMX(q: QTensorMX, dtype=torch.float32) -> torch.Tensor:
     return y
 
 
+class _OnTape(torch.autograd.Function):
+    """h, which a kernel wrote, as the sum of x and the residual."""
+
+    @staticmethod
+    def forward(ctx, x, residual, h):
+        return h
+
+    @staticmethod
+    def backward(ctx, dh):
+        need_x, need_r, _ = ctx.needs_input_grad
+        return dh if need_x else None, dh if need_r else None, None
+
+
 def AddRMSNormMX(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-6,
                  format: str = "mxfp8") -> Tuple[QTensorMX, torch.Tensor]:
     """``h = x + residual`` and the quantised ``h / sqrt(mean(h^2) + eps) * weight``: what a pre-norm block hands to its next
     products, and the stream that goes on beside them.  Returns (codes and scales, h).  The norm takes the sum before it is rounded to
     h's type; a value is rounded once, to its code: none of the arithmetic before moves one that lies next to the border between two
-    codes to the other (for weights up to 2^27).  Without a residual h is x itself."""
+    codes to the other (for weights up to 2^27).  Without a residual h is x itself.  Gradients go through the sum alone: the quantised rows
+    have none, like all that is computed from them here."""
     fmt, shape = _format(format), tuple(x.shape)
     a = _rows(x, "AddRMSNormMX")
     rows, K = a.shape
@@ -286,14 +300,22 @@ def AddRMSNormMX(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
     if not x.is_cuda:
         h = a.double() if r is None else a.double() + r.double()
         y = h / torch.sqrt(h.square().sum(-1, keepdim=True) / K + eps) * weight.detach().double()
-        return _quantize_ref(y, fmt, shape), (x if r is None else h.to(x.dtype).reshape(shape))
+        return _quantize_ref(y, fmt, shape), _sum_of(x, residual, None if r is None else h.to(x.dtype).reshape(shape))
     w = weight if weight.is_contiguous() else weight.contiguous()
     q, codes, scales = _empty(rows, shape, fmt, a)
     h = None if r is None else a.new_empty(shape)
     if rows:
         _call(a.get_device(), "gb_mx_add_rms_norm", _TYPES[x.dtype], fmt, a.data_ptr(), a.stride(0), None if r is None else r.data_ptr(),
               K if r is None else r.stride(0), w.data_ptr(), w.dtype == torch.float32, None if h is None else h.data_ptr(), codes, scales, rows, K, eps)
-    return q, (x if h is None else h)
+    return q, _sum_of(x, residual, h)
+
+
+def _sum_of(x, residual, h):
+    if h is None:
+        return x
+    if torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad):
+        return _OnTape.apply(x, residual, h)
+    return h
 
 
 def _epilogue(bias, N: int, device, dtype, act, what: str):

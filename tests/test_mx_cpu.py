@@ -386,3 +386,21 @@ def test_kernels_that_a_call_launches(name, args, kernels, monkeypatch):
     before = _l.kernel_count
     _l.call(name, *args)
     assert _l.kernel_count - before == kernels
+
+
+def test_norm_keeps_the_sum_on_the_tape():
+    """h is x + residual for gradients as well; without a tape, or leaves that ask for them, it has none."""
+    x, r, w = (torch.randn(*s) for s in ((3, 5, 40), (3, 5, 40), (40,)))
+    for need in ((True, True), (True, False), (False, True)):
+        leaves = [t.clone().requires_grad_(n) for t, n in zip((x, r), need)]
+        dy = torch.randn_like(x)
+        h = Q.AddRMSNormMX(*leaves, w)[1]
+        assert torch.equal(h, x + r)
+        asked = [t for t, n in zip(leaves, need) if n]
+        assert all(torch.equal(g, 2 * dy) for g in torch.autograd.grad(h * 2, asked, dy))
+        with torch.no_grad():
+            assert not Q.AddRMSNormMX(*leaves, w)[1].requires_grad
+    assert not Q.AddRMSNormMX(x, r, w.requires_grad_())[1].requires_grad
+    leaf = x.clone().requires_grad_()
+    assert Q.AddRMSNormMX(leaf, None, w)[1] is leaf
+    assert not Q.MXRMSNorm(RMSNorm(40))(leaf, r)[1].requires_grad

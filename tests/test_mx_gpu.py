@@ -909,3 +909,21 @@ def test_a_training_layer_without_a_tape_keeps_nothing(mode, status_ok):
         assert name == "gb_mx_train_forward" and args[12:16] == (False, False, None, 0)
         y = layer(x)
     assert torch.equal(y, want) and not y.requires_grad
+
+
+def test_norm_keeps_the_sum_on_the_tape(status_ok):
+    """h is x + residual for gradients as well; without a tape, or leaves that ask for them, it has none."""
+    x, r, w = (torch.randn(*s, device=DEV) for s in ((3, 5, 40), (3, 5, 40), (40,)))
+    for need in ((True, True), (True, False), (False, True)):
+        leaves = [t.clone().requires_grad_(n) for t, n in zip((x, r), need)]
+        dy = torch.randn_like(x)
+        h = Q.AddRMSNormMX(*leaves, w)[1]
+        assert torch.equal(h, x + r)
+        asked = [t for t, n in zip(leaves, need) if n]
+        assert all(torch.equal(g, 2 * dy) for g in torch.autograd.grad(h * 2, asked, dy))
+        with torch.no_grad():
+            assert not Q.AddRMSNormMX(*leaves, w)[1].requires_grad
+    assert not Q.AddRMSNormMX(x, r, w.requires_grad_())[1].requires_grad
+    leaf = x.clone().requires_grad_()
+    assert Q.AddRMSNormMX(leaf, None, w)[1] is leaf
+    assert not Q.MXRMSNorm(RMSNorm(40).to(DEV))(leaf, r)[1].requires_grad
