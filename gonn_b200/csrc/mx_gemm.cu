@@ -150,7 +150,8 @@ __device__ __forceinline__ void tile_at(int t, int num_m, int num_n, int& m, int
 // these (its half of the accumulator has all columns); CTA 0 issues.  Two accumulators of 256 columns and the scales do not fit into TMEM's
 // 512, so the two overlap in columns 128 to 255: the epilogue drains those first, and then the next tile starts.  (Tiles of 192 columns,
 // whose accumulators do not overlap, were no faster for a K of 768, 24 against 25 us at 16384 x 2304 in MXFP4, and slower for longer ones:
-// 8192^3 437 against 358 us in MXFP8.)  Four sets of scale columns take turns.
+// 8192^3 437 against 358 us in MXFP8, bursts on one box; on others this one takes up to 387, and 440 at the power cap.)  Four sets of scale
+// columns take turns.
 // ---------------------------------------------------------------------------------------------------------------------------
 template <int FMT>
 struct PairCfg {

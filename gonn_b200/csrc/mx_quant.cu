@@ -30,7 +30,8 @@ struct QuantArgs {
 
 // A unit is L / 8 times 128 columns of a row.  L = 0: aligned rows, eight lanes, NU units of a lane in flight.  Others (Stage): 32 lanes, or
 // eight of rows of up to 256.  Directly | by way of Stage, us: 50304 x 2048 bf16 to MXFP4 44.5 | 63.6 (and back 48.3 | 58.1); eight lanes | 32, 40 M
-// values in rows of 33 117 | 294, 201 48 | 53, 257 57 | 45, 1003 46 | 29.
+// bf16 values to MXFP8 in rows of 33 117 | 294, 201 48 | 53, 257 57 | 45, 1003 46 | 29.  (To MXFP4, whose scale pieces come in twos, rows of 33 220; of
+// fp32, 136, 55, 53 and 35.)  What bounds the narrow ones is a load and a store into shared memory for each element.
 template <typename T, int FMT, int L>
 __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const QuantArgs a) {
   constexpr int NU = Elem<T>::SZ == 2 && L == 0 ? 2 : 1, LANES = L ? L : 8;
@@ -93,7 +94,7 @@ struct BothArgs {
 // then stands in shared memory, a thread quantises two columns of 32 rows, and their codes leave by way of shared memory as
 // 128-byte pieces of the transpose's rows.  Pieces of 16 bytes are exchanged within a lane's (swapped) so that no bank is met twice.
 // As many CTAs as the registers allow load, compute and store in turn: 16384 x 2304 bf16 36.2 us with two of them on an SM and banks met
-// twice to eight times, 35.0 so (floor 23.4), 16384 x 768 fp32 21.5 and 17.3 (11.7).  Half of the issue slots are in use, 39 % of DRAM's rate.
+// twice to eight times, 35.0 so (floor 23.4), 16384 x 768 fp32 21.5 and 17.3 (11.7); rows at any address, 16384 x 2303 bf16 52, 16384 x 767 fp32 28.  Half of the issue slots are in use, 39 % of DRAM's rate.
 template <typename T>
 struct BothCfg {
   static constexpr int TILE = 128 * 128 * Elem<T>::SZ, PITCH = 128 + 16;
@@ -694,7 +695,8 @@ bool wide_rows(const void* p, long long ld, long long K, int size) { return ((ui
 // How a row of `vecs` vectors is dealt out: one to a thread, the shortest way, or two, which holds more in flight, for what does not stay in
 // L2.  One | two, bf16, us: 600 x 2048 4.0 | 5.2, 2400 x 2048 8.1 | 9.4, 8192 x 768 10.6 | 11.5, 2400 x 4096 13.6 | 13.7, 16384 x 768 21.5 | 19.1,
 // 16384 x 2048 44 | 43.5, 8192 x 8192 91 | 82; fp32, 8192 x 2048 42 | 42, 4096 x 8192 95 | 78 (before rows with a value next to a border took
-// their sum again, which costs 5 to 10 % of either).  Rows at any address: 16384 x 768 bf16 31, 16384 x 2048 66.
+// their sum again, which costs 5 to 10 % of either).  Now, with inputs in turn beyond L2: 16384 x 768 21.4, 16384 x 2048 50, 8192 x 8192 94, fp32
+// 16384 x 768 33.7, 8192 x 8192 167; rows at any address, 16384 x 1003 42.9, fp32 53.
 template <typename T, int FMT, bool ALIGNED>
 cudaError_t norm_launch(const NormArgs& a, cudaStream_t st) {
   const int vecs = a.pieces * 8;

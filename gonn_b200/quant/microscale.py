@@ -11,7 +11,8 @@ every product with them.  Sums of products are kept in fp32 by the tensor core, 
 
 CUDA tensors run on ``csrc/mx_quant.cu`` and ``csrc/mx_gemm.cu`` (tcgen05 with block scales), CPU tensors on the same formulas
 with tensor operations.  ``QuantizeMX``, ``AddRMSNormMX``, ``MatMulMX`` and ``LinearMX`` serve evaluation, like the int8 layers of
-this package; ``TrainLinearMX`` is differentiable.
+this package; ``TrainLinearMX`` is differentiable.  The modules stand wherever a module is called; the blocks of ``models`` and ``nn.Transformer``
+read the parameters of their ``Linear`` layers for fused kernels and take neither these nor the int8 layers in their place.
 """
 from __future__ import annotations
 

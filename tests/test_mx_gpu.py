@@ -927,3 +927,20 @@ def test_norm_keeps_the_sum_on_the_tape(status_ok):
     leaf = x.clone().requires_grad_()
     assert Q.AddRMSNormMX(leaf, None, w)[1] is leaf
     assert not Q.MXRMSNorm(RMSNorm(40).to(DEV))(leaf, r)[1].requires_grad
+
+
+def test_head_of_a_model(status_ok):
+    """A model whose closing projection keeps its weights quantised: the logits are the layer's of the model's own hidden rows."""
+    from gonn_b200.models.lm import GPT
+    torch.manual_seed(3)
+    model = GPT(vocab=100, d_model=64, n_layers=2, n_heads=2, d_ff=128, max_seq=16).to(DEV)
+    ids = torch.randint(0, 100, (2, 16)).to(DEV)
+    hidden = []
+    hook = model.norm.register_forward_hook(lambda m, i, o: hidden.append(o.detach()))
+    with torch.no_grad():
+        full = model(ids)
+        weight = Q.QuantizeMX(model.head.weight)
+        model.head = Q.NewMXLinearFrom(model.head)
+        y = model(ids)
+    assert torch.equal(y, Q.LinearMX(hidden[-1], weight)) and torch.equal(hidden[0], hidden[1])
+    assert y.shape == full.shape and y.dtype == full.dtype
