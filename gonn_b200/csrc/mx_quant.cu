@@ -446,9 +446,9 @@ __device__ __forceinline__ void weights16(const NormArgs& a, int k, float (&w)[1
   }
 }
 
-// Codes of sixteen columns; whether one of the values may lie on the other side of a border.
+// Codes of sixteen columns; whether one of the values may lie on the other side of a border.  far: the row's sum cannot be trusted.
 template <typename T, int FMT, bool ALIGNED>
-__device__ __forceinline__ bool write_norm(const NormArgs& a, long long row, int k, const uint64_t (&h)[8], float root) {
+__device__ __forceinline__ bool write_norm(const NormArgs& a, long long row, int k, const uint64_t (&h)[8], float root, bool far) {
   float w[16], y[16];
   weights16<T, ALIGNED>(a, k, w);
   const uint64_t root2 = pair_of(root, root);
@@ -472,10 +472,10 @@ __device__ __forceinline__ bool write_norm(const NormArgs& a, long long row, int
   const uint32_t word = quantize16<FMT>(y, __float_as_uint(m), 0xffu << (lane & 24), lane, out);
   store_codes<FMT>(a.data + row * a.row_bytes, k, a.row_bytes, out);
   if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(a.scales + scale_word(row, k >> 7, a.pieces)) = word;
-  if (m < 0x1p-80f) {                    // (a block's borders go down to 2^-19 of its largest value)
-    uint32_t some = 0;
+  if (far || m < 0x1p-80f) {             // (a block's borders go down to 2^-19 of its largest value)
+    uint64_t some = 0;                   // zeros are what they are, unless the root makes NaN of them
 #pragma unroll
-    for (int j = 0; j < 16; j++) some |= __float_as_uint(y[j]) & 0x7fffffffu;
+    for (int j = 0; j < 8; j++) some |= (h[j] | pair_of(y[2 * j], y[2 * j + 1])) & 0x7fffffff7fffffffull;
     return some != 0;
   }
   return near <= kNear<FMT>;
@@ -597,7 +597,7 @@ __global__ void __launch_bounds__(norm_threads(G), norm_blocks(sizeof(T), VPT, G
       root = inverse_root(v);
 #pragma unroll
       for (int i = 0; i < VPT; i++)
-        if (live && t + i * G < vecs && (write_norm<T, FMT, ALIGNED>(a, row, (t + i * G) * 16, h[i], root) || far_out(s, v))) near |= 1u << i;
+        if (live && t + i * G < vecs && write_norm<T, FMT, ALIGNED>(a, row, (t + i * G) * 16, h[i], root, far_out(s, v))) near |= 1u << i;
     } else {
       for (int i = t; i - t < vecs; i += G) {
         uint32_t wx[W], wr[W];
@@ -615,7 +615,7 @@ __global__ void __launch_bounds__(norm_threads(G), norm_blocks(sizeof(T), VPT, G
         uint64_t h[8];
         take(i, wx, wr);
         sum16<T>(wx, wr, h);
-        if (i < vecs && (write_norm<T, FMT, ALIGNED>(a, row, i * 16, h, root) || far_out(s, v))) near |= 1u << min(n, 31);
+        if (i < vecs && write_norm<T, FMT, ALIGNED>(a, row, i * 16, h, root, far_out(s, v))) near |= 1u << min(n, 31);
       }
     }
     if (row_any<G>(near != 0)) {

@@ -944,3 +944,28 @@ def test_head_of_a_model(status_ok):
         y = model(ids)
     assert torch.equal(y, Q.LinearMX(hidden[-1], weight)) and torch.equal(hidden[0], hidden[1])
     assert y.shape == full.shape and y.dtype == full.dtype
+
+
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("K", [40, 768, 1003, 2304, 20001])
+def test_norm_of_rows_of_zeros(format, dtype, K, status_ok):
+    """Padded batches: rows of zeros between others, also with eps 0 (NaN), and beside weights that are not finite.  (In a block with the scale of NaN
+    the finite values' codes say nothing: scales and values are compared.)"""
+    def compare(x, r, w, eps):
+        q, want = cpu(Q.AddRMSNormMX(x, r, w, eps, format)[0]), Q.microscale._quantize_ref(norm64(x, r, w, eps).cpu(), int(format == "mxfp4"), (50, K))
+        assert torch.equal(q.ScaleCodes(), want.ScaleCodes())
+        a, b = Q.DequantizeMX(q), Q.DequantizeMX(want)
+        assert bool(((a == b) | torch.isnan(a) & torch.isnan(b)).all())
+
+    x, r = torch.randn(50, K, device=DEV).to(dtype), torch.randn(50, K, device=DEV).to(dtype)
+    x[::3] = r[::3] = 0
+    x[1::9, K // 2:] = r[1::9, K // 2:] = 0
+    r[2::9] = -x[2::9]
+    w = (torch.rand(K, device=DEV) + 0.5).to(dtype)
+    for bad in (None, math.inf, -math.inf, math.nan, 0.0):
+        if bad is not None:
+            w[K // 2] = bad
+        for eps in (1e-6, 0.0):
+            compare(x, r, w, eps)
+            compare(x, None, w, eps)
