@@ -267,11 +267,12 @@ def DequantizeMX(q: QTensorMX, dtype=torch.float32) -> torch.Tensor:
 
 
 class _OnTape(torch.autograd.Function):
-    """h, which a kernel wrote, as the sum of x and the residual."""
+    """h, which a kernel wrote, as the sum of x and the residual.  (In a list: a tensor that went in would come out as a view, which nothing may be
+    added to in place.)"""
 
     @staticmethod
     def forward(ctx, x, residual, h):
-        return h
+        return h[0]
 
     @staticmethod
     def backward(ctx, dh):
@@ -301,7 +302,7 @@ def AddRMSNormMX(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
     if not x.is_cuda:
         h = a.double() if r is None else a.double() + r.double()
         y = h / torch.sqrt(h.square().sum(-1, keepdim=True) / K + eps) * weight.detach().double()
-        return _quantize_ref(y, fmt, shape), _sum_of(x, residual, None if r is None else h.to(x.dtype).reshape(shape))
+        return _quantize_ref(y, fmt, shape), _sum_of(x, residual, None if r is None else h.reshape(shape).to(x.dtype, copy=True))
     w = weight if weight.is_contiguous() else weight.contiguous()
     q, codes, scales = _empty(rows, shape, fmt, a)
     h = None if r is None else a.new_empty(shape)
@@ -315,7 +316,7 @@ def _sum_of(x, residual, h):
     if h is None:
         return x
     if torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad):
-        return _OnTape.apply(x, residual, h)
+        return _OnTape.apply(x, residual, [h])
     return h
 
 

@@ -421,3 +421,12 @@ def test_head_of_a_model():
         y = model(ids)
     assert torch.equal(y, Q.LinearMX(hidden[-1], weight)) and torch.equal(hidden[0], hidden[1])
     assert y.shape == full.shape and y.dtype == full.dtype
+
+
+def test_the_sum_on_the_tape_takes_more_in_place():
+    """h += what a layer returned, as a residual stream runs on."""
+    x, r, y, dy = (torch.randn(6, 40, requires_grad=n) for n in (True, True, True, False))
+    h = Q.AddRMSNormMX(x * 2, r, torch.ones(40))[1]
+    h += y
+    grads = torch.autograd.grad(h, (x, r, y), dy)
+    assert torch.equal(grads[0], 2 * dy) and torch.equal(grads[1], dy) and torch.equal(grads[2], dy)

@@ -969,3 +969,12 @@ def test_norm_of_rows_of_zeros(format, dtype, K, status_ok):
         for eps in (1e-6, 0.0):
             compare(x, r, w, eps)
             compare(x, None, w, eps)
+
+
+def test_the_sum_on_the_tape_takes_more_in_place(status_ok):
+    """h += what a layer returned, as a residual stream runs on."""
+    x, r, y, dy = (torch.randn(6, 40, device=DEV, requires_grad=n) for n in (True, True, True, False))
+    h = Q.AddRMSNormMX(x * 2, r, torch.ones(40, device=DEV))[1]
+    h += y
+    grads = torch.autograd.grad(h, (x, r, y), dy)
+    assert torch.equal(grads[0], 2 * dy) and torch.equal(grads[1], dy) and torch.equal(grads[2], dy)
