@@ -409,7 +409,7 @@ class _TrainLinear(torch.autograd.Function):
         if not x.is_cuda:
             (xq, xt), (wq, wt) = (QuantizeMXPair(t) if need else (QuantizeMX(t), None) for t, need in ((a, need_w), (w, need_x)))
             ctx.save_for_backward(*(v for t in (xt, wt) for v in ((None, None) if t is None else (t.Data, t.Scales))))
-            return MatMulMX(xq, wq, bias, x.dtype).view(y.shape)
+            return y.copy_(MatMulMX(xq, wq, bias, x.dtype).view(y.shape))
         sizes = _l.lib().gb_mx_train_bytes
         kept = scratch = None
         n_kept, n_scratch = sizes(M, N, K, need_x, need_w, 0), sizes(M, N, K, need_x, need_w, 1)

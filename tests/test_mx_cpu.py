@@ -430,3 +430,12 @@ def test_the_sum_on_the_tape_takes_more_in_place():
     h += y
     grads = torch.autograd.grad(h, (x, r, y), dy)
     assert torch.equal(grads[0], 2 * dy) and torch.equal(grads[1], dy) and torch.equal(grads[2], dy)
+
+
+def test_a_training_layers_result_takes_more_in_place():
+    layer, x = Q.NewMXTrainLinearFrom(Linear(40, 24)), torch.randn(6, 40, requires_grad=True)
+    y = layer(x)
+    want = torch.autograd.grad(y.sum(), x)[0]
+    y = layer(x)
+    y += 1
+    assert torch.equal(torch.autograd.grad(y.sum(), x)[0], want)
