@@ -987,3 +987,37 @@ def test_a_training_layers_result_takes_more_in_place(status_ok):
     y = layer(x)
     y += 1
     assert torch.equal(torch.autograd.grad(y.sum(), x)[0], want)
+
+
+@pytest.mark.parametrize("format", FORMATS)
+def test_offsets_beyond_32_bits(format, status_ok):
+    """More than 2^31 values (and 2^32 bytes) of rows, codes and results: the last rows are those of the same rows alone."""
+    R, K, N, last = 1060000, 2050, 2060, 300
+    x = torch.randn(R, K, device=DEV, dtype=torch.bfloat16)
+    assert x.numel() > 2 ** 31
+    end, w = x[-last:].clone(), torch.rand(K, device=DEV).bfloat16() + 0.5
+
+    def same(q, alone, rows=slice(-last, None)):
+        assert torch.equal(q.Data[rows], alone.Data) and torch.equal(Q.DequantizeMX(part(q, rows)), Q.DequantizeMX(alone))
+
+    def part(q, rows):
+        return Q.QTensorMX(q.Data[rows].contiguous(), Q.microscale._pack_scales(q.ScaleCodes()[rows].cpu(), FORMATS.index(format)).to(DEV), format, (last, K))
+
+    q = Q.QuantizeMX(x, format)
+    same(q, Q.QuantizeMX(end, format))
+    assert torch.equal(Q.DequantizeMX(q, torch.bfloat16)[-last:], Q.DequantizeMX(Q.QuantizeMX(end, format), torch.bfloat16))
+    n, h = Q.AddRMSNormMX(x, x, w, 1e-6, format)
+    m, g = Q.AddRMSNormMX(end, end, w, 1e-6, format)
+    same(n, m)
+    assert torch.equal(h[-last:], g)
+    del h, n
+    b, bias = Q.QuantizeMX(torch.randn(N, K, device=DEV), format), torch.randn(N, device=DEV)
+    y = Q.MatMulMX(q, b, bias)
+    assert y.numel() > 2 ** 31 and torch.equal(y[-last:], Q.MatMulMX(part(q, slice(-last, None)), b, bias))
+    del y
+    if format == "mxfp8":
+        p, t = Q.QuantizeMXPair(x)
+        same(p, Q.QuantizeMX(end))
+        first = R - R % 128 - 256
+        tail = Q.QuantizeMX(x[first:].t())
+        assert torch.equal(t.Data[:, first:], tail.Data)
