@@ -341,7 +341,7 @@ __device__ __forceinline__ float inverse_root(double v) {
   asm("rsqrt.approx.f32 %0, %1;" : "=f"(r0) : "f"((float)v));
   return (float)fma(0.5 * (double)r0, fma(-v * (double)r0, (double)r0, 1.0), (double)r0);
 }
-// A row whose sum of squares s or mean square v = s / K + eps fp32 cannot be trusted with (its values are all taken as next to a border).
+// A row whose sum of squares s or mean square v = s / K + eps fp32 cannot be trusted with (all of its values but zeros are taken as next to a border).
 __device__ __forceinline__ bool far_out(double s, double v) { return !(s > 1e-25 && s < 1e38 && v > 1e-36 && v < 1e36); }
 
 // A value next to the border between two codes has to fall on the side where it belongs: by three roundings of fp32 one in a million falls on
