@@ -1,0 +1,833 @@
+// Attention of new tokens over a paged cache of keys and values, and of a batch whose first pages are shared.
+//
+// Token t < counts[b] of sequence b sits at position lengths[b] + t and sees the positions up to its own:
+// o = sum_j p_j v_j / sum_j p_j with p_j = exp(scale q . k_j - m).  One pass over the keys with the running maximum m and sum l of
+// each row, in fp32; H / Hkv query heads share a key head and are rows of one tile.  The weights p are at most 1 and are rounded to the
+// inputs' type for the second product (2^-9 of each, as in csrc/flash_attn.cu); their sum is taken before that.
+//
+// What bounds it: every key and value is read once for a few rows of queries, so memory does.  The work is a list of tiles of kTile keys:
+// sequence by sequence, key head by key head.  Its length is known on the device alone (lengths[]), so every CTA adds the
+// lengths up itself and takes an equal share of the list, across sequences and heads: no plan, no host, no idle SM with ragged
+// lengths.  A (sequence, head) whose tiles fall to several CTAs leaves partial rows (m, l, o) behind, which a second kernel joins in
+// the list's order; no atomics.
+//
+// A shared prefix is one more entry at the head of the list whose rows are the queries of all sequences: its keys are read once for
+// every 16, 32 or 64 rows.  The sequences' own entries then start behind it, and all rows are joined by the second kernel.
+//
+// A CTA: four warps that multiply (mma.sync for 16-bit types, FMA for fp32) and one that copies (cp.async, 16 bytes a lane, a page looked
+// up for every key, so a page may have any size) through a ring of stages.
+#include "common.cuh"
+
+#include <atomic>
+
+using namespace gb;
+
+namespace {
+
+constexpr int kThreads = 160;
+constexpr int kConsumers = 4;
+
+struct CacheArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;                               // (B, T, H, D), contiguous
+  long long q_sb, q_st, q_sh;
+  long long k_sp, k_sh, k_sr, v_sp, v_sh, v_sr;
+  const int* table;
+  long long table_stride;
+  int columns, pages, page, room;          // room: columns page
+  const int* lengths;
+  const int* counts;
+  int B, T, H, Hkv, G, D;
+  int prefix;                              // shared positions (whole pages)
+  float scale_log2;
+  int own_tiles, prefix_tiles;             // row tiles of a sequence, of the prefix
+  int ctas;
+  float* part;                             // [slots][rows of a tile][D] unscaled sums
+  float2* stat;                            // [slots][rows of a tile] (m, l)
+  int2* owner;                             // [(prefix tiles + B own_tiles) Hkv] first and last CTA
+  int* status;
+};
+
+template <typename T> struct Elem;
+template <> struct Elem<__nv_bfloat16> {
+  static constexpr bool kMma = true;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16(a, b); }
+};
+template <> struct Elem<__half> {
+  static constexpr bool kMma = true;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_f16(a, b); }
+};
+template <> struct Elem<float> { static constexpr bool kMma = false; };
+
+// Rows of a tile: 16 RG.  Row groups of 16 rows times key groups of a quarter, a half or all of the keys are the four warps of the
+// 16-bit kernel; in fp32 a warp takes four rows and all keys.
+template <typename T, int HD_, int RG_>
+struct Cfg {
+  static constexpr int HD = HD_, RG = RG_;
+  static constexpr bool kMma = Elem<T>::kMma;
+  static constexpr int ROWS = 16 * RG;
+  static constexpr int TILE = kMma ? 64 : 32;
+  static constexpr int KG = kMma ? 4 / RG : 1;
+  static constexpr int SUB = TILE * HD * (int)sizeof(T);          // one K or V tile
+  static constexpr int STAGES = HD == 64 ? 6 : 3;
+  static constexpr int CHUNKS = HD * (int)sizeof(T) / 16;         // 16-byte chunks of a row
+  static constexpr int EXTRA = kMma ? (KG > 1 ? KG / 2 * ROWS * (HD * 4 + 8) : 0) : ROWS * HD * 4 + ROWS * TILE * 4;   // joined groups; queries and weights
+  static constexpr int SMEM = 2 * STAGES * SUB + EXTRA + 256 + 1024;
+};
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// the list of tiles
+// ---------------------------------------------------------------------------------------------------------------------------
+struct Entry {                // rows of queries over a range of keys, for every key head
+  int b;                      // -1: all sequences, over the prefix
+  int row0;                   // first row
+  int begin, end;             // keys
+  int tiles;                  // of one key head
+};
+
+__device__ __forceinline__ int count_of(const CacheArgs& a, int b) {
+  const int c = a.counts ? a.counts[b] : a.T;
+  return c < 0 ? 0 : c < a.T ? c : a.T;
+}
+
+template <int ROWS, int TILE>
+__device__ __forceinline__ Entry entry_of(const CacheArgs& a, int e) {
+  Entry x;
+  x.begin = a.prefix;
+  if (e < a.prefix_tiles) {
+    x.b = -1;
+    x.row0 = e * ROWS;
+    x.begin = 0;
+    x.end = a.prefix;
+  } else {
+    e -= a.prefix_tiles;
+    x.b = a.own_tiles == 1 ? e : e / a.own_tiles;
+    const int rt = e - x.b * a.own_tiles;
+    x.row0 = rt * ROWS;
+    const int c = count_of(a, x.b), last = min(a.T * a.G, x.row0 + ROWS) - 1;
+    const int seen = min(c, last / a.G + 1);                         // tokens of these rows that count, and those before them
+    const long long end = x.row0 / a.G < c ? (long long)a.lengths[x.b] + seen : 0;
+    x.end = (int)(end < a.room ? end : (long long)a.room);
+  }
+  x.tiles = x.end > x.begin ? (x.end - x.begin + TILE - 1) / TILE : 0;
+  return x;
+}
+
+// Position in the list.
+template <int ROWS, int TILE>
+struct Cursor {
+  Entry x;
+  int e, h, entries, tile;
+  // to the entry e (or the first one after it that has tiles), `tile` tiles into it
+  __device__ __forceinline__ void start(const CacheArgs& a, int e_, long long into) {
+    entries = a.prefix_tiles + a.B * a.own_tiles;
+    e = e_;
+    x = entry_of<ROWS, TILE>(a, e);
+    h = x.tiles ? (int)(into / x.tiles) : 0;
+    tile = x.tiles ? (int)(into - (long long)h * x.tiles) : 0;
+  }
+  __device__ __forceinline__ void next_segment(const CacheArgs& a) {
+    tile = 0;
+    if (++h < a.Hkv) return;
+    h = 0;
+    do {
+      if (++e >= entries) return;
+      x = entry_of<ROWS, TILE>(a, e);
+    } while (x.tiles == 0);
+  }
+};
+
+struct Share {
+  long long first, count, total;     // of this CTA's tiles, of all
+  int e;                             // the entry of the first one
+  long long into;                    // tiles of that entry before it
+};
+
+// Adds up the tiles of all entries and finds this CTA's share.  By the threads of a CTA, through shared memory.
+template <int ROWS, int TILE>
+__device__ __forceinline__ Share share_of(const CacheArgs& a, long long* s_sum, Share* s_share) {
+  const int entries = a.prefix_tiles + a.B * a.own_tiles, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (entries + kThreads - 1) / kThreads, lo = min(entries, tid * per), hi = min(entries, lo + per);
+  long long mine = 0;
+  for (int e = lo; e < hi; e++) mine += entry_of<ROWS, TILE>(a, e).tiles;
+  mine *= a.Hkv;
+  long long sum = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long up = __shfl_up_sync(0xffffffffu, sum, d);
+    if (lane >= d) sum += up;
+  }
+  if (lane == 31) s_sum[warp] = sum;
+  __syncthreads();
+  long long before = 0, total = 0;
+  for (int w = 0; w < kThreads / 32; w++) {
+    if (w < warp) before += s_sum[w];
+    total += s_sum[w];
+  }
+  before += sum - mine;
+  const long long first = total * blockIdx.x / a.ctas, end = total * (blockIdx.x + 1) / a.ctas;
+  if (end > first && first >= before && first < before + mine) {
+    int e = lo;
+    long long at = before;
+    for (;; e++) {
+      const long long n = (long long)entry_of<ROWS, TILE>(a, e).tiles * a.Hkv;
+      if (first < at + n) break;
+      at += n;
+    }
+    *s_share = {first, end - first, total, e, first - at};
+  }
+  if (tid == 0 && end == first) *s_share = {first, 0, total, 0, 0};
+  __syncthreads();
+  return *s_share;
+}
+
+__device__ __forceinline__ int cta_of(long long tile, long long total, int ctas) { return (int)(((tile + 1) * ctas - 1) / total); }
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// matrix instructions
+// ---------------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldm4t(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (sizeof(T) == 2 && __is_same(T, __nv_bfloat16))
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Byte of a 16-byte chunk in a tile: 16-bit rows lie in columns of 64 elements (128 bytes), fp32 rows whole; the chunk's last three
+// bits are exchanged by the row's, so that eight rows' chunks lie in eight different banks.
+template <typename T, int HD, int TILE>
+__device__ __forceinline__ uint32_t chunk_at(int row, int chunk) {
+  if constexpr (sizeof(T) == 2) return (uint32_t)((chunk >> 3) * (TILE * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+  else return (uint32_t)(row * (HD * 4) + ((chunk ^ (row & 7)) << 4));
+}
+
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// A row of a tile: its query, its output row and how many keys it sees.
+struct Row {
+  int b, t, g;
+  bool there;            // a row of the entry
+  bool counts;           // of a token that counts
+  int sees;
+};
+
+__device__ __forceinline__ Row row_of(const CacheArgs& a, const Entry& x, int r) {
+  Row w;
+  int i = x.row0 + r;
+  const int per = a.T * a.G;
+  w.there = i < (x.b < 0 ? a.B * per : per);
+  if (!w.there) i = 0;
+  w.b = x.b;
+  if (x.b < 0) {
+    w.b = i / per;
+    i -= w.b * per;
+  }
+  w.t = i / a.G;
+  w.g = i - w.t * a.G;
+  w.counts = w.there && w.t < count_of(a, w.b);
+  const long long sees = w.counts ? (long long)a.lengths[w.b] + w.t + 1 : 0;
+  w.sees = (int)(sees < 0x7fffffffLL ? sees : 0x7fffffffLL);
+  return w;
+}
+
+template <typename T, int HD, int RG>
+__global__ void __launch_bounds__(kThreads, 2) cache_attn_kernel(const CacheArgs a) {
+  using C = Cfg<T, HD, RG>;
+  constexpr int ROWS = C::ROWS, TILE = C::TILE, STAGES = C::STAGES, SUB = C::SUB;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* s_k = smem;
+  uint8_t* s_v = smem + STAGES * SUB;
+  uint8_t* s_extra = s_v + STAGES * SUB;
+  uint64_t* full = (uint64_t*)(s_extra + C::EXTRA);
+  uint64_t* empty = full + STAGES;
+  long long* s_sum = (long long*)(empty + STAGES);
+  Share* s_share = (Share*)(s_sum + kThreads / 32);
+  volatile int* abort_flag = (volatile int*)(s_share + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; i++) {
+      mbar_init(&full[i], 32);
+      mbar_init(&empty[i], kConsumers);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  pdl_wait();
+  const Share share = share_of<ROWS, TILE>(a, s_sum, s_share);      // (ends with a barrier of the CTA)
+  pdl_trigger();
+  if (share.count == 0) return;
+  Cursor<ROWS, TILE> at;
+  at.start(a, share.e, share.into);
+
+  if (warp == kConsumers) {
+    // ---------------- copies ----------------
+    constexpr int LOOK = TILE / 32;                                  // keys that a lane looks up
+    constexpr int PER = 32 / C::CHUNKS < 1 ? 1 : 32 / C::CHUNKS;     // rows of one instruction of the warp
+    constexpr int SPAN = C::CHUNKS < 32 ? C::CHUNKS : 32;
+    const int sub = lane / SPAN, chunk = lane % SPAN;
+    const bool inside = chunk * 16 < a.D * (int)sizeof(T);
+    int page[LOOK], in_page[LOOK];
+    auto look_up = [&]() {
+      const int* row = a.table + (at.x.b < 0 ? 0 : at.x.b) * a.table_stride;
+#pragma unroll
+      for (int i = 0; i < LOOK; i++) {
+        const int key = at.x.begin + at.tile * TILE + i * 32 + lane;
+        page[i] = -1;
+        in_page[i] = 0;
+        if (key < at.x.end) {
+          const unsigned p = (unsigned)key / (unsigned)a.page;
+          in_page[i] = (int)((unsigned)key - p * (unsigned)a.page);
+          page[i] = row[p];
+          if (page[i] < 0 || page[i] >= a.pages) {
+            set_status(a.status, ST_BAD_INDEX, at.x.b);
+            page[i] = -1;
+          }
+        }
+      }
+    };
+    look_up();
+    int st = 0;
+    uint32_t ph = 0;
+    for (long long n = 0; n < share.count; n++) {
+      long long k_off[LOOK], v_off[LOOK];
+#pragma unroll
+      for (int i = 0; i < LOOK; i++) {
+        k_off[i] = page[i] < 0 ? -1 : page[i] * a.k_sp + at.h * a.k_sh + in_page[i] * a.k_sr;
+        v_off[i] = page[i] < 0 ? -1 : page[i] * a.v_sp + at.h * a.v_sh + in_page[i] * a.v_sr;
+      }
+      if (++at.tile == at.x.tiles) at.next_segment(a);
+      if (n + 1 < share.count) look_up();                            // on their way while this stage is waited for
+      if (!mbar_wait(&empty[st], ph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 20)) break;
+      uint8_t* dk = s_k + st * SUB;
+      uint8_t* dv = s_v + st * SUB;
+#pragma unroll
+      for (int i = 0; i < LOOK; i++) {
+#pragma unroll 4
+        for (int r = 0; r < 32; r += PER) {
+          const long long ko = __shfl_sync(0xffffffffu, k_off[i], r + sub), vo = __shfl_sync(0xffffffffu, v_off[i], r + sub);
+          const int bytes = ko >= 0 && inside ? 16 : 0;
+          const uint32_t to = chunk_at<T, HD, TILE>(i * 32 + r + sub, chunk);
+          cp_async16(dk + to, (const T*)a.k + (bytes ? ko + chunk * (16 / (int)sizeof(T)) : 0), bytes);
+          cp_async16(dv + to, (const T*)a.v + (bytes ? vo + chunk * (16 / (int)sizeof(T)) : 0), bytes);
+        }
+      }
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[st])) : "memory");
+      if (++st == STAGES) { st = 0; ph ^= 1; }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    return;
+  }
+
+  // ---------------- products ----------------
+  int st = 0;
+  uint32_t ph = 0;
+  long long left = share.count, tile_no = share.first;
+  bool first_segment = true, dead = false;       // dead: a wait has given up; the barriers among the warps are kept all the same
+  while (left > 0) {
+    const int n = (int)min(left, (long long)(at.x.tiles - at.tile));
+    const long long segment0 = tile_no - at.tile;                    // the list's number of this segment's first tile
+    const bool whole = n == at.x.tiles;
+    const int seg = at.e * a.Hkv + at.h;
+    // Where its rows go: straight to the output, to the partial rows of a whole segment (in the output's order, those of the prefix
+    // behind the sequences'), or to this CTA's first or last ones.
+    const int slot = 2 * blockIdx.x + (first_segment ? 0 : 1);
+    if (at.tile == 0 && threadIdx.x == 0) a.owner[seg] = make_int2(slot, cta_of(segment0 + at.x.tiles - 1, share.total, a.ctas));
+    const bool direct = whole && a.prefix_tiles == 0;
+    auto part_row = [&](const Row& w, int r) -> long long {
+      if (!whole) return (long long)slot * ROWS + r;
+      const long long bt = (long long)w.b * a.T + w.t;
+      return 2LL * a.ctas * ROWS + ((at.x.b < 0 ? (long long)a.B * a.T : 0) + bt) * a.H + at.h * a.G + w.g;
+    };
+
+    if constexpr (C::kMma) {
+      const int rg = warp / C::KG, kg = warp % C::KG;
+      constexpr int NK = TILE / C::KG;                               // keys of this warp
+      const int r0 = rg * 16 + (lane >> 2), r1 = r0 + 8;
+      const Row w0 = row_of(a, at.x, r0), w1 = row_of(a, at.x, r1);
+      const bool idle = !__any_sync(0xffffffffu, w0.counts || w1.counts);
+      uint32_t qf[HD / 16][4];
+      {
+        const T* q0 = (const T*)a.q + w0.b * a.q_sb + w0.t * a.q_st + (long long)(at.h * a.G + w0.g) * a.q_sh;
+        const T* q1 = (const T*)a.q + w1.b * a.q_sb + w1.t * a.q_st + (long long)(at.h * a.G + w1.g) * a.q_sh;
+#pragma unroll
+        for (int s = 0; s < HD / 16; s++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int col = s * 16 + (i >> 1) * 8 + (lane & 3) * 2;
+            const bool ok = col < a.D && ((i & 1) ? w1.counts : w0.counts);
+            qf[s][i] = ok ? *reinterpret_cast<const uint32_t*>(((i & 1) ? q1 : q0) + col) : 0u;
+          }
+      }
+      // rows of nothing are masked nowhere: what they add up to is not used
+      const int sees0 = w0.counts ? w0.sees : 0x7fffffff, sees1 = w1.counts ? w1.sees : 0x7fffffff;
+      float o[HD / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+#pragma unroll
+      for (int j = 0; j < HD / 8; j++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[j][i] = 0.f;
+
+      for (int i = 0; i < n; i++) {
+        dead = dead || !mbar_wait(&full[st], ph, abort_flag, a.status, ST_ATTN_TIMEOUT, 21);
+        if (dead) break;
+        if (!idle) {
+          const uint32_t ka = smem_u32(s_k + st * SUB), va = smem_u32(s_v + st * SUB);
+          const int key0 = at.x.begin + (at.tile + i) * TILE + kg * NK;
+          float s[NK / 8][4];
+#pragma unroll
+          for (int j = 0; j < NK / 8; j++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) s[j][c] = 0.f;
+#pragma unroll
+          for (int j = 0; j < NK / 16; j++) {                        // 16 keys: two n8 tiles
+            const int row = kg * NK + j * 16 + (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+            for (int x = 0; x < HD / 16; x++) {
+              uint32_t b[4];
+              ldm4(b, ka + chunk_at<T, HD, TILE>(row, x * 2 + ((lane >> 3) & 1)));
+              mma16<T>(s[2 * j], qf[x], b[0], b[1]);
+              mma16<T>(s[2 * j + 1], qf[x], b[2], b[3]);
+            }
+          }
+          const int low = min(min(sees0, sees1), at.x.end);          // (zeros stand in for keys behind the last one)
+          if (__any_sync(0xffffffffu, low - key0 < NK)) {
+#pragma unroll
+            for (int j = 0; j < NK / 8; j++)
+#pragma unroll
+              for (int c = 0; c < 4; c++) {
+                const int key = key0 + j * 8 + (lane & 3) * 2 + (c & 1);
+                if (key >= min((c & 2) ? sees1 : sees0, at.x.end)) s[j][c] = -INFINITY;
+              }
+          }
+          float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < NK / 8; j++) {
+            x0 = fmaxf(x0, fmaxf(s[j][0], s[j][1]));
+            x1 = fmaxf(x1, fmaxf(s[j][2], s[j][3]));
+          }
+#pragma unroll
+          for (int d = 1; d < 4; d <<= 1) {
+            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
+            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+          }
+          x0 *= a.scale_log2;
+          x1 *= a.scale_log2;
+          const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+          if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
+            const float f0 = m0 == -INFINITY ? 0.f : exp2f(m0 - n0), f1 = m1 == -INFINITY ? 0.f : exp2f(m1 - n1);
+            m0 = n0;
+            m1 = n1;
+            l0 *= f0;
+            l1 *= f1;
+#pragma unroll
+            for (int j = 0; j < HD / 8; j++) {
+              o[j][0] *= f0;
+              o[j][1] *= f0;
+              o[j][2] *= f1;
+              o[j][3] *= f1;
+            }
+          }
+          const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
+#pragma unroll
+          for (int j = 0; j < NK / 8; j++) {
+            s[j][0] = exp2f(fmaf(s[j][0], a.scale_log2, -z0));
+            s[j][1] = exp2f(fmaf(s[j][1], a.scale_log2, -z0));
+            s[j][2] = exp2f(fmaf(s[j][2], a.scale_log2, -z1));
+            s[j][3] = exp2f(fmaf(s[j][3], a.scale_log2, -z1));
+            l0 += s[j][0] + s[j][1];
+            l1 += s[j][2] + s[j][3];
+          }
+#pragma unroll
+          for (int j = 0; j < NK / 16; j++) {
+            const uint32_t p[4] = {Elem<T>::pack(s[2 * j][0], s[2 * j][1]), Elem<T>::pack(s[2 * j][2], s[2 * j][3]),
+                                   Elem<T>::pack(s[2 * j + 1][0], s[2 * j + 1][1]), Elem<T>::pack(s[2 * j + 1][2], s[2 * j + 1][3])};
+            const int row = kg * NK + j * 16 + (lane & 15);
+#pragma unroll
+            for (int x = 0; x < HD / 16; x++) {                      // 16 columns
+              uint32_t b[4];
+              ldm4t(b, va + chunk_at<T, HD, TILE>(row, x * 2 + (lane >> 4)));
+              mma16<T>(o[2 * x], p, b[0], b[1]);
+              mma16<T>(o[2 * x + 1], p, b[2], b[3]);
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[st]);
+        if (++st == STAGES) { st = 0; ph ^= 1; }
+      }
+#pragma unroll
+      for (int d = 1; d < 4; d <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, d);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, d);
+      }
+      // key groups joined by twos
+      if constexpr (C::KG > 1) {
+        float* buf = reinterpret_cast<float*>(s_extra);
+        float2* stats = reinterpret_cast<float2*>(buf + C::KG / 2 * ROWS * HD);
+#pragma unroll
+        for (int half = C::KG / 2; half >= 1; half >>= 1) {
+          consumers_sync();                                          // the buffer's last use is over
+          if (kg >= half && kg < 2 * half) {
+            float* p0 = buf + ((kg - half) * ROWS + r0) * HD + (lane & 3) * 2;
+#pragma unroll
+            for (int j = 0; j < HD / 8; j++) {
+              *reinterpret_cast<float2*>(p0 + j * 8) = make_float2(o[j][0], o[j][1]);
+              *reinterpret_cast<float2*>(p0 + 8 * HD + j * 8) = make_float2(o[j][2], o[j][3]);
+            }
+            if ((lane & 3) == 0) {
+              stats[(kg - half) * ROWS + r0] = make_float2(m0, l0);
+              stats[(kg - half) * ROWS + r1] = make_float2(m1, l1);
+            }
+          }
+          consumers_sync();
+          if (kg < half) {
+            const float2 y0 = stats[kg * ROWS + r0], y1 = stats[kg * ROWS + r1];
+            const float n0 = fmaxf(m0, y0.x), n1 = fmaxf(m1, y1.x);
+            const float f0 = m0 == -INFINITY ? 0.f : exp2f(m0 - n0), f1 = m1 == -INFINITY ? 0.f : exp2f(m1 - n1);
+            const float g0 = y0.x == -INFINITY ? 0.f : exp2f(y0.x - n0), g1 = y1.x == -INFINITY ? 0.f : exp2f(y1.x - n1);
+            m0 = n0;
+            m1 = n1;
+            l0 = l0 * f0 + y0.y * g0;
+            l1 = l1 * f1 + y1.y * g1;
+            const float* p0 = buf + (kg * ROWS + r0) * HD + (lane & 3) * 2;
+#pragma unroll
+            for (int j = 0; j < HD / 8; j++) {
+              const float2 u = *reinterpret_cast<const float2*>(p0 + j * 8), w = *reinterpret_cast<const float2*>(p0 + 8 * HD + j * 8);
+              o[j][0] = o[j][0] * f0 + u.x * g0;
+              o[j][1] = o[j][1] * f0 + u.y * g0;
+              o[j][2] = o[j][2] * f1 + w.x * g1;
+              o[j][3] = o[j][3] * f1 + w.y * g1;
+            }
+          }
+        }
+      }
+      if (kg == 0) {
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+          const Row& w = half ? w1 : w0;
+          const float m = half ? m1 : m0, l = half ? l1 : l0;
+          const int r = half ? r1 : r0;
+          if (direct) {
+            if (w.there) {
+              const float f = w.counts && l != 0.f ? __frcp_rn(l) : 0.f;
+              T* to = (T*)a.out + (((long long)w.b * a.T + w.t) * a.H + at.h * a.G + w.g) * a.D + (lane & 3) * 2;
+#pragma unroll
+              for (int j = 0; j < HD / 8; j++)
+                if (j * 8 < a.D)
+                  *reinterpret_cast<uint32_t*>(to + j * 8) =
+                      f == 0.f ? 0u : Elem<T>::pack(o[j][2 * half] * f, o[j][2 * half + 1] * f);
+            }
+          } else if (w.there) {
+            const long long row = part_row(w, r);
+            float* to = a.part + row * a.D + (lane & 3) * 2;
+#pragma unroll
+            for (int j = 0; j < HD / 8; j++)
+              if (j * 8 < a.D) *reinterpret_cast<float2*>(to + j * 8) = make_float2(o[j][2 * half], o[j][2 * half + 1]);
+            if ((lane & 3) == 0) a.stat[row] = make_float2(m, l);
+          }
+        }
+      }
+    } else {
+      // fp32: a warp's four rows over all keys of a tile.  Scores: a lane is a key; products with the values: a lane is HD / 32 columns.
+      static_assert(RG == 1, "16 rows");
+      constexpr int CPL = HD / 32;
+      float* s_q = reinterpret_cast<float*>(s_extra);                // [ROWS][HD]
+      float* s_p = s_q + ROWS * HD + warp * (4 * TILE);              // [TILE][4] of this warp
+      Row w[4];
+      int sees[4];
+      bool any = false;
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        w[r] = row_of(a, at.x, warp * 4 + r);
+        any |= w[r].counts;
+        sees[r] = w[r].counts ? w[r].sees : 0x7fffffff;
+        const float* q = (const float*)a.q + w[r].b * a.q_sb + w[r].t * a.q_st + (long long)(at.h * a.G + w[r].g) * a.q_sh;
+#pragma unroll
+        for (int c = lane; c < HD; c += 32) s_q[(warp * 4 + r) * HD + c] = w[r].counts && c < a.D ? q[c] : 0.f;
+      }
+      __syncwarp();
+      float o[4][CPL], m[4], l[4];
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+#pragma unroll
+        for (int c = 0; c < CPL; c++) o[r][c] = 0.f;
+      }
+      for (int i = 0; i < n; i++) {
+        dead = dead || !mbar_wait(&full[st], ph, abort_flag, a.status, ST_ATTN_TIMEOUT, 22);
+        if (dead) break;
+        if (any) {
+          const uint8_t* kt = s_k + st * SUB;
+          const uint8_t* vt = s_v + st * SUB;
+          const int key = at.x.begin + (at.tile + i) * TILE + lane;
+          float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+          for (int c = 0; c < HD / 4; c++) {
+            const float4 kk = *reinterpret_cast<const float4*>(kt + chunk_at<T, HD, TILE>(lane, c));
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+              const float4 qq = *reinterpret_cast<const float4*>(s_q + (warp * 4 + r) * HD + c * 4);
+              s[r] = fmaf(qq.x, kk.x, s[r]);
+              s[r] = fmaf(qq.y, kk.y, s[r]);
+              s[r] = fmaf(qq.z, kk.z, s[r]);
+              s[r] = fmaf(qq.w, kk.w, s[r]);
+            }
+          }
+          float4 p4;
+          float* p = &p4.x;
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const float x = key < sees[r] && key < at.x.end ? s[r] * a.scale_log2 : -INFINITY;
+            const float top = fmaxf(m[r], warp_max(x));
+            if (top > m[r]) {
+              const float f = m[r] == -INFINITY ? 0.f : exp2f(m[r] - top);
+              m[r] = top;
+              l[r] *= f;
+#pragma unroll
+              for (int c = 0; c < CPL; c++) o[r][c] *= f;
+            }
+            p[r] = exp2f(x - (m[r] == -INFINITY ? 0.f : m[r]));
+            l[r] += p[r];                                            // this lane's keys; summed over lanes at the end
+          }
+          __syncwarp();
+          *reinterpret_cast<float4*>(s_p + lane * 4) = p4;
+          __syncwarp();
+#pragma unroll 4
+          for (int j = 0; j < TILE; j++) {
+            const float4 pj = *reinterpret_cast<const float4*>(s_p + j * 4);
+            float v[CPL];
+            const uint8_t* vr = vt + chunk_at<T, HD, TILE>(j, lane * CPL / 4);
+            if constexpr (CPL == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(vr);
+            else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(vr + (lane & 1) * 8);
+#pragma unroll
+            for (int c = 0; c < CPL; c++) {
+              o[0][c] = fmaf(pj.x, v[c], o[0][c]);
+              o[1][c] = fmaf(pj.y, v[c], o[1][c]);
+              o[2][c] = fmaf(pj.z, v[c], o[2][c]);
+              o[3][c] = fmaf(pj.w, v[c], o[3][c]);
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[st]);
+        if (++st == STAGES) { st = 0; ph ^= 1; }
+      }
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const float sum = warp_sum(l[r]);
+        const int col = lane * CPL;
+        if (!w[r].there || col >= a.D) {
+          // a column behind the head's last one
+        } else if (direct) {
+          const float f = w[r].counts && sum != 0.f ? __frcp_rn(sum) : 0.f;
+          float* to = (float*)a.out + (((long long)w[r].b * a.T + w[r].t) * a.H + at.h * a.G + w[r].g) * a.D + col;
+#pragma unroll
+          for (int c = 0; c < CPL; c++) to[c] = f == 0.f ? 0.f : o[r][c] * f;
+        } else {
+          float* to = a.part + part_row(w[r], warp * 4 + r) * a.D + col;
+#pragma unroll
+          for (int c = 0; c < CPL; c++) to[c] = o[r][c];
+        }
+        if (w[r].there && !direct && lane == 0) a.stat[part_row(w[r], warp * 4 + r)] = make_float2(m[r], sum);
+      }
+      __syncwarp();
+    }
+    first_segment = false;
+    left -= n;
+    tile_no += n;
+    at.next_segment(a);
+  }
+}
+
+// Joins the partial rows of a query row in the order of the list, prefix first: a warp a row, a lane every 32nd column.  Rows that the
+// first kernel has written are left alone; rows that see nothing become zeros.
+template <typename T, int ROWS, int TILE>
+__global__ void __launch_bounds__(256) cache_join_kernel(const CacheArgs a) {
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const long long rows = (long long)a.B * a.T * a.H;
+  const long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (i >= rows) return;
+  const int head = (int)(i % a.H), h = head / a.G, g = head - h * a.G;
+  const long long bt = i / a.H;
+  const int b = (int)(bt / a.T), t = (int)(bt - (long long)b * a.T);
+  T* out = (T*)a.out + i * a.D;
+  float top = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  bool done = false;
+  auto take = [&](long long row) {
+    const float2 s = a.stat[row];
+    const float* p = a.part + row * a.D;
+    const float n = fmaxf(top, s.x);
+    const float f = top == -INFINITY ? 0.f : exp2f(top - n);
+    const float w = s.x == -INFINITY ? (s.y == 0.f ? 0.f : 1.f) : exp2f(s.x - n);     // (scores of NaN leave no maximum, but a sum)
+    top = n;
+    sum = sum * f + s.y * w;
+#pragma unroll
+    for (int c = 0; c < 4; c++)
+      if (c * 32 + lane < a.D) o[c] = o[c] * f + p[c * 32 + lane] * w;
+  };
+  auto gather = [&](int e, int r, long long whole) {
+    if (entry_of<ROWS, TILE>(a, e).tiles == 0) return;
+    const int2 c = a.owner[e * a.Hkv + h];
+    if (c.x >> 1 == c.y) {                       // one CTA had all of it
+      if (a.prefix_tiles == 0) done = true;
+      else take(2LL * a.ctas * ROWS + whole);
+      return;
+    }
+    take((long long)c.x * ROWS + r);
+    for (int k = (c.x >> 1) + 1; k <= c.y; k++) take(2LL * k * ROWS + r);
+  };
+  if (t < count_of(a, b)) {
+    const int r = t * a.G + g;
+    if (a.prefix_tiles) {
+      const int all = b * a.T * a.G + r;
+      gather(all / ROWS, all % ROWS, rows + i);
+    }
+    gather(a.prefix_tiles + b * a.own_tiles + r / ROWS, r % ROWS, i);
+  }
+  if (done) return;
+  const float f = sum != 0.f ? __frcp_rn(sum) : 0.f;
+#pragma unroll
+  for (int c = 0; c < 4; c++)
+    if (c * 32 + lane < a.D) out[c * 32 + lane] = (T)(f == 0.f ? 0.f : o[c] * f);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------------------------------------
+constexpr int kCtas = 2 * 148;
+
+struct Sizes {
+  int rows;                      // of a tile
+  int own_tiles, prefix_tiles;
+  long long entries, slot_rows, part, stat, owner, total;      // bytes of the workspace's parts
+};
+
+bool plan(Sizes& z, int dtype, long long B, long long T, long long H, long long Hkv, long long D, bool prefix) {
+  const long long own = T * (H / Hkv), all = B * own, most = prefix ? all : own;
+  z.rows = dtype == 2 || most <= 16 ? 16 : most <= 32 ? 32 : 64;
+  const long long ot = (own + z.rows - 1) / z.rows, pt = prefix ? (all + z.rows - 1) / z.rows : 0;
+  z.entries = pt + B * ot;
+  if (z.entries * Hkv >= 0x7fffffffLL || all >= 0x7fffffffLL) return false;
+  z.own_tiles = (int)ot;
+  z.prefix_tiles = (int)pt;
+  z.slot_rows = 2LL * kCtas * z.rows + (prefix ? 2 * B * T * H : 0);
+  auto up = [](long long n) { return (n + 255) / 256 * 256; };
+  z.part = up(z.slot_rows * D * 4);
+  z.stat = up(z.slot_rows * 8);
+  z.owner = up(z.entries * Hkv * 8);
+  z.total = z.part + z.stat + z.owner;
+  return true;
+}
+
+template <typename T, int HD, int RG>
+int launch_attn(CacheArgs& a, cudaStream_t s) {
+  using C = Cfg<T, HD, RG>;
+  static std::atomic<uint32_t> done{0};
+  int dev = 0;
+  GB_CUDA_OK(cudaGetDevice(&dev));
+  if (dev >= 32 || !(done.load() >> dev & 1u)) {
+    GB_CUDA_OK(cudaFuncSetAttribute(cache_attn_kernel<T, HD, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    if (dev < 32) done.fetch_or(1u << dev);
+  }
+  GB_CUDA_OK(gbh::launch(cache_attn_kernel<T, HD, RG>, dim3(a.ctas), dim3(kThreads), C::SMEM, s, 1, a));
+  const long long rows = (long long)a.B * a.T * a.H;
+  GB_CUDA_OK(gbh::launch(cache_join_kernel<T, C::ROWS, C::TILE>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, 1, a));
+  return gbh::E_OK;
+}
+
+template <typename T>
+int launch_type(CacheArgs& a, int rows, cudaStream_t s) {
+  if constexpr (Elem<T>::kMma) {
+    if (a.D <= 64) return rows == 16 ? launch_attn<T, 64, 1>(a, s) : rows == 32 ? launch_attn<T, 64, 2>(a, s) : launch_attn<T, 64, 4>(a, s);
+    return rows == 16 ? launch_attn<T, 128, 1>(a, s) : rows == 32 ? launch_attn<T, 128, 2>(a, s) : launch_attn<T, 128, 4>(a, s);
+  } else {
+    return a.D <= 64 ? launch_attn<T, 64, 1>(a, s) : launch_attn<T, 128, 1>(a, s);
+  }
+}
+
+}  // namespace
+
+// Bytes of the workspace of gb_cache_attn, or a negative error.
+GB_EXPORT long long gb_cache_attn_bytes(int dtype, long long B, long long T, long long H, long long Hkv, long long D, int prefix) {
+  Sizes z;
+  if (B < 0 || T < 1 || H < 1 || Hkv < 1 || H % Hkv || D < 1 || D > 128 || !plan(z, dtype, B, T, H, Hkv, D, prefix > 0)) {
+    gbh::set_error("gb_cache_attn: too many rows, or bad sizes (%lld sequences, %lld tokens, %lld and %lld heads of %lld)", B, T, H, Hkv, D);
+    return gbh::E_TOO_LARGE;
+  }
+  return z.total;
+}
+
+// out (B, T, H, D) = attention of q over the pages of its sequences.  strides: of q (batch, token, head), of both caches (page, head, row),
+// in elements; rows of q aligned to 4 bytes, those of the caches to 16.  prefix: positions, a multiple of the page, that all sequences have in
+// the pages of the first one's.  The workspace belongs to this call until its kernels have run.
+GB_EXPORT int gb_cache_attn(int dtype, const void* q, const void* k, const void* v, void* out, const long long* strides, int B, int T, int H,
+                            int Hkv, int D, const void* table, long long table_stride, int columns, int pages, int page, const void* lengths,
+                            const void* counts, int prefix, double scale, void* ws, long long ws_bytes, void* stream) {
+  const int size = dtype == 2 ? 4 : 2;
+  if (dtype < 0 || dtype > 2 || B < 0 || T < 0 || H < 1 || Hkv < 1 || H % Hkv || D < 1 || D > 128 || D * size % 16) {
+    gbh::set_error("gb_cache_attn: bad type or sizes (type %d, %d sequences, %d tokens, %d and %d heads of %d)", dtype, B, T, H, Hkv, D);
+    return gbh::E_BAD_ARG;
+  }
+  if (B == 0 || T == 0) return gbh::E_OK;
+  if (!q || !k || !v || !out || !table || !lengths || !ws || page < 1 || columns < 1 || pages < 1) {
+    gbh::set_error("gb_cache_attn: null pointer or empty cache");
+    return gbh::E_BAD_ARG;
+  }
+  if ((long long)columns * page >= 0x7fffffffLL || prefix < 0 || prefix > (long long)columns * page || prefix % page || !(scale > 0)) {
+    gbh::set_error("gb_cache_attn: a table of %d pages of %d positions, %d of them shared, scale %g", columns, page, prefix, scale);
+    return gbh::E_BAD_ARG;
+  }
+  long long cache = 0;
+  for (int i = 3; i < 9; i++) cache |= strides[i];
+  if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)ws) & 15 || cache * size % 16 || (uintptr_t)q & 3 || (strides[0] | strides[1] | strides[2]) * size % 4 ||
+      (uintptr_t)out & 3) {
+    gbh::set_error("gb_cache_attn: misaligned tensor");
+    return gbh::E_BAD_ARG;
+  }
+  Sizes z;
+  if (!plan(z, dtype, B, T, H, Hkv, D, prefix > 0) || ws_bytes < z.total) {
+    gbh::set_error("gb_cache_attn: workspace of %lld bytes is too small, or too many rows", ws_bytes);
+    return gbh::E_TOO_LARGE;
+  }
+  const long long join = ((long long)B * T * H + 7) / 8;
+  if (join >= 0x7fffffffLL) {
+    gbh::set_error("gb_cache_attn: too many rows");
+    return gbh::E_TOO_LARGE;
+  }
+  CacheArgs a = {};
+  a.q = q; a.k = k; a.v = v; a.out = out;
+  a.q_sb = strides[0]; a.q_st = strides[1]; a.q_sh = strides[2];
+  a.k_sp = strides[3]; a.k_sh = strides[4]; a.k_sr = strides[5];
+  a.v_sp = strides[6]; a.v_sh = strides[7]; a.v_sr = strides[8];
+  a.table = (const int*)table; a.table_stride = table_stride;
+  a.columns = columns; a.pages = pages; a.page = page; a.room = columns * page;
+  a.lengths = (const int*)lengths; a.counts = (const int*)counts;
+  a.B = B; a.T = T; a.H = H; a.Hkv = Hkv; a.G = H / Hkv; a.D = D;
+  a.prefix = prefix;
+  a.scale_log2 = (float)(scale * 1.4426950408889634);
+  a.own_tiles = z.own_tiles; a.prefix_tiles = z.prefix_tiles;
+  a.ctas = kCtas;
+  a.part = (float*)ws;
+  a.stat = (float2*)((uint8_t*)ws + z.part);
+  a.owner = (int2*)((uint8_t*)ws + z.part + z.stat);
+  a.status = gbh::status_ptr();
+  cudaStream_t s = (cudaStream_t)stream;
+  if (dtype == 0) return launch_type<__nv_bfloat16>(a, z.rows, s);
+  if (dtype == 1) return launch_type<__half>(a, z.rows, s);
+  return launch_type<float>(a, z.rows, s);
+}

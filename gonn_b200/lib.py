@@ -36,6 +36,8 @@ _ARGUMENTS = {
     "gb_mx_add_rms_norm": "iipLpLpipppLLdp", "gb_mx_matmul": "ipppppLpiLLLiip", "gb_mx_matmul_rows": "iipLpppLpiLLLiip",
     "gb_mx_linear": "iipLppppiLLLiipLp",
     "gb_mx_train_forward": "iipLpLppiLLLiipLpLp", "gb_mx_train_backward": "ipLppipipiLLLpLp",
+    "gb_rotary": "ipLLLpiiiiiipdipiLLp", "gb_cache_append": "ipppppppiiiiiiipdpLiiippp",
+    "gb_cache_attn": "ipppppiiiiipLiiippidpLp", "gb_cache_attn_bytes": "iLLLLLi",
     "gb_mx_plan": "LLLip", "gb_mx_linear_bytes": "LLLi", "gb_mx_train_bytes": "LLLiii",
 }
 
@@ -49,6 +51,7 @@ KERNELS_PER_CALL = {
     "gb_norm_bwd": 2, "gb_channel_sum": 2, "gb_ce_fwd": 2, "gb_ce_fused": 2, "gb_flash_bwd": 2, "gb_flash_bwd_ws": 2, "gb_embedding_bwd": 5,
     "gb_status_read": 0, "gb_comm_alloc": 0, "gb_comm_open": 0, "gb_comm_emulate": 0,
     "gb_comm_free": 0, "gb_reduce": 1, "gb_gemm_f32x3": 3, "gb_conv_wgrad": 2, "gb_conv_cl_fwd": 2, "gb_conv_cl_bwd": 4, "gb_stack_fwd": 0, "gb_set_words": 1, "gb_norm_bwd_res": 2, "gb_q_dynamic": 2,
+    "gb_cache_attn": 2, "gb_cache_attn_bytes": 0,
     # by the arguments: up to 16 rows take one; of dX, dW and db those that there are, and the gradient's quantisation
     "gb_mx_linear": lambda a: 1 if a[9] <= 16 else 2,
     "gb_mx_train_forward": 3,
@@ -91,7 +94,7 @@ def lib() -> ctypes.CDLL:
             l.gb_gemm_f32x3_workspace.restype = c_longlong
             l.gb_gemm_f32x3_workspace.argtypes = [c_int, c_int, c_int, c_int]
             for name in ("gb_conv_cl_fwd_ws", "gb_conv_cl_bwd_ws", "gb_conv_cl_part", "gb_block_ws", "gb_lstm_seq_bwd_words",
-                         "gb_mx_linear_bytes", "gb_mx_train_bytes"):
+                         "gb_mx_linear_bytes", "gb_mx_train_bytes", "gb_cache_attn_bytes"):
                 getattr(l, name).restype = c_longlong
             for name in ("gb_bench_matmul", "gb_bench_add", "gb_bench_flash_attn"):
                 getattr(l, name).restype = c_double
@@ -159,6 +162,15 @@ def call(name: str, *args) -> None:
     kernel_count += n if n.__class__ is int else n(args)
     if rc != 0:
         check(rc, name)
+
+
+def call_on(device: int, name: str, *args) -> None:
+    """``call`` with plain numbers and addresses, on the current stream of a device, whichever is the current one."""
+    if device == (_raw_device() if _raw_device is not None else torch.cuda.current_device()):
+        call(name, *args, current_stream_handle())
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, current_stream_handle())
 
 
 def read_status(clear: bool = True):

@@ -7,6 +7,7 @@ from .activation import *  # noqa
 from .embedding import Embedding, EmbeddingBag  # noqa
 from .dropout import Dropout, Dropout1d, Dropout2d, Dropout3d, AlphaDropout, FeatureAlphaDropout  # noqa
 from .attention import MultiHeadAttention  # noqa
+from .cache import KVCache, RotaryEmbedding  # noqa
 from .transformer import (TransformerEncoderLayer, TransformerEncoder, TransformerDecoderLayer,  # noqa
                           TransformerDecoder, Transformer)
 from . import init  # noqa

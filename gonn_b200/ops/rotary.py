@@ -1,0 +1,111 @@
+"""Rotary positions: pairs of a head's columns turned by an angle that grows with the token's position.
+
+CUDA: ``csrc/rotary.cu``, where angles are exact to a float's last bit at any position.  CPU: the same formulas with tensor
+operations, angles in fp64."""
+from __future__ import annotations
+
+import math
+from typing import Optional, Sequence
+
+import torch
+
+from .. import lib as _l
+
+_TYPES = {torch.bfloat16: _l.DT_BF16, torch.float16: _l.DT_F16, torch.float32: _l.DT_F32}
+
+
+def frequencies(dim: int, base: float, scaling: str = "none", factor: float = 1.0, original: int = 0, low: float = 1.0,
+                high: float = 32.0) -> Sequence[float]:
+    """The angle w_i that pair i < dim / 2 is turned by a position (see ``nn.RotaryEmbedding``)."""
+    if scaling == "base":
+        base = base * factor ** (dim / (dim - 2))
+    w = [base ** (-2.0 * i / dim) for i in range(dim // 2)]
+    if scaling == "linear":
+        w = [f / factor for f in w]
+    elif scaling == "bands":
+        def part(f):
+            g = min(1.0, max(0.0, (original * f / (2 * math.pi) - low) / (high - low)))
+            return f * (g + (1.0 - g) / factor)
+        w = [part(f) for f in w]
+    return w
+
+
+def turns_of(w: Sequence[float]) -> torch.Tensor:
+    """Fractions of a turn in 64 bits of fixed point, as int64."""
+    t = [round(f / (2 * math.pi) * 2.0 ** 64) % 2 ** 64 for f in w]
+    return torch.tensor([v - 2 ** 64 if v >= 2 ** 63 else v for v in t], dtype=torch.int64)
+
+
+def rotate_ref(x: torch.Tensor, positions: torch.Tensor, w: Sequence[float], interleaved: bool, amplitude: float, back: bool = False):
+    """Oracle: x (batch, tokens, heads, width), positions (batch, tokens) or (tokens,); in fp32 (fp64 for fp64)."""
+    ct = torch.float64 if x.dtype == torch.float64 else torch.float32
+    half = len(w)
+    angle = positions.to(torch.float64)[..., None] * torch.tensor(w, dtype=torch.float64, device=x.device)
+    cos, sin = ((amplitude * f(angle)).to(ct)[..., None, :] for f in (torch.cos, torch.sin))
+    if back:
+        sin = -sin
+    y = x.to(ct)
+    part, rest = y[..., :2 * half], y[..., 2 * half:]
+    a, b = (part[..., 0::2], part[..., 1::2]) if interleaved else (part[..., :half], part[..., half:])
+    u, v = a * cos - b * sin, a * sin + b * cos
+    part = torch.stack((u, v), -1).flatten(-2) if interleaved else torch.cat((u, v), -1)
+    return torch.cat((part, rest), -1).to(x.dtype)
+
+
+def _launch(x, positions, turns, interleaved, amplitude, back):
+    batch, tokens, heads, width = x.shape
+    if x.stride(3) != 1 and width > 1:
+        x = x.contiguous()
+    y = torch.empty((batch, tokens, heads, width), dtype=x.dtype, device=x.device)
+    if positions is None:
+        at, wide, pb, pt = None, 0, 0, 0
+    else:
+        at, wide = positions.data_ptr(), positions.dtype == torch.int64
+        pb, pt = (0, positions.stride(0)) if positions.dim() == 1 else positions.stride()
+    sb, st, sh, _ = x.stride()
+    _l.call_on(x.get_device(), "gb_rotary", _TYPES[x.dtype], x.data_ptr(), sb, st, sh, y.data_ptr(), batch, tokens, heads, width,
+               2 * turns.shape[0], interleaved, turns.data_ptr(), amplitude, back, at, wide, pb, pt)
+    return y
+
+
+class _Rotary(torch.autograd.Function):
+    """A turn; its gradient is the turn back (with a gradient of its own)."""
+
+    @staticmethod
+    def forward(ctx, x, positions, turns, interleaved, amplitude, back):
+        ctx.rest = positions, turns, interleaved, amplitude, not back
+        return _launch(x, positions, turns, interleaved, amplitude, back)
+
+    @staticmethod
+    def backward(ctx, dy):
+        return _Rotary.apply(dy, *ctx.rest), None, None, None, None, None
+
+
+def rotary(x: torch.Tensor, positions: Optional[torch.Tensor], w: Sequence[float], turns: torch.Tensor, interleaved: bool = False,
+           amplitude: float = 1.0) -> torch.Tensor:
+    """x (batch, tokens, heads, width), any strides; positions: int32 or int64, (tokens,) or (batch, tokens), or None for 0, 1, ...;
+    differentiable in x."""
+    if x.dim() != 4:
+        raise ValueError(f"rotary: expected (batch, tokens, heads, width), got shape {tuple(x.shape)}")
+    batch, tokens, _, width = x.shape
+    if 2 * len(w) > width:
+        raise ValueError(f"rotary: {2 * len(w)} columns are turned, but a head has {width}")
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"rotary: positions are int32 or int64, not {positions.dtype}")
+        if tuple(positions.shape) not in ((tokens,), (batch, tokens)):
+            raise ValueError(f"rotary: positions must have shape ({tokens},) or ({batch}, {tokens}), got {tuple(positions.shape)}")
+        if positions.device != x.device:
+            raise ValueError(f"rotary: positions are on {positions.device}, x on {x.device}")
+    if not x.is_cuda:
+        if not x.is_floating_point():
+            raise TypeError(f"rotary: a floating point tensor is needed, got {x.dtype}")
+        at = torch.arange(tokens, device=x.device) if positions is None else positions
+        return rotate_ref(x, at, w, interleaved, amplitude)
+    if x.dtype not in _TYPES:
+        raise TypeError(f"rotary: no CUDA kernel for dtype {x.dtype}")
+    if turns.device != x.device:
+        raise ValueError(f"rotary: the frequencies are on {turns.device}, x on {x.device}; move the module there")
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _Rotary.apply(x, positions, turns, interleaved, amplitude, False)
+    return _launch(x, positions, turns, interleaved, amplitude, False)

@@ -1,0 +1,149 @@
+"""Rotary positions and the paged cache: the CPU path, and what calls refuse."""
+import math
+
+import pytest
+import torch
+
+from gonn_b200 import nn
+from gonn_b200.ops.rotary import turns_of
+
+
+def test_fixed_point_angles():
+    """p times the fraction of a turn, modulo 2^64, against the exact product."""
+    from fractions import Fraction
+    w = nn.RotaryEmbedding(64, 500000.0)._w
+    for f, t in zip(w, turns_of(w).tolist()):
+        turn = Fraction(f / (2 * math.pi))
+        for p in (0, 1, 4095, 131071, 2 ** 31 - 1, -5):
+            got = Fraction(t * p % 2 ** 64, 2 ** 64)
+            want = turn * p % 1
+            d = abs(got - want)
+            assert min(d, 1 - d) <= Fraction(abs(p) + 1, 2 ** 65)
+
+
+@pytest.mark.parametrize("inter", [False, True])
+def test_rotary_keeps_lengths_and_relative_positions(inter):
+    rope = nn.RotaryEmbedding(6, interleaved=inter)
+    x, y = torch.randn(2, 1, 1, 1, 8, dtype=torch.float64)
+    at = torch.arange(50)
+    a, b = rope(x.expand(1, 50, 1, 8), at)[0, :, 0], rope(y.expand(1, 50, 1, 8), at)[0, :, 0]
+    assert torch.allclose(a.norm(dim=-1), x.norm().expand(50))
+    assert torch.allclose((a[3:] * b[:-3]).sum(-1), (a[3] * b[0]).sum().expand(47))
+    assert torch.equal(a[:, 6:], x.view(8)[6:].expand(50, 2))
+    assert torch.equal(a[0], x.view(8))
+
+
+def test_rotary_gradient():
+    rope = nn.RotaryEmbedding(4, interleaved=True, scaling="linear", factor=3.0, amplitude=1.2)
+    x = torch.randn(2, 3, 2, 5, dtype=torch.float64, requires_grad=True)
+    assert torch.autograd.gradcheck(lambda t: rope(t, torch.tensor([5, 9, 100])), (x,))
+
+
+def test_scalings():
+    plain = nn.RotaryEmbedding(64)._w
+    assert nn.RotaryEmbedding(64, scaling="linear", factor=4.0)._w == [f / 4 for f in plain]
+    base = nn.RotaryEmbedding(64, scaling="base", factor=4.0)._w
+    assert base[0] == plain[0] and math.isclose(base[-1], plain[-1] / 4)
+    bands = nn.RotaryEmbedding(64, scaling="bands", factor=4.0, original=4096)._w
+    for f, g in zip(plain, bands):
+        turns = 4096 * f / (2 * math.pi)
+        assert g == f if turns >= 32 else math.isclose(g, f / 4) if turns <= 1 else f / 4 < g < f
+
+
+def test_module():
+    rope = nn.NewRotaryEmbedding(8)
+    assert not list(rope.parameters()) and not rope.state_dict()
+    assert rope.to(torch.bfloat16).turns.dtype == torch.int64
+
+
+def steps(B, kv, H, D, page, pieces, shared=0, dtype=torch.float64):
+    """Tokens appended and attended piece by piece, and the same by attention over all of them at once."""
+    T = sum(pieces)
+    columns = -(-T // page)
+    cache = nn.KVCache(B * columns + shared, page, kv, D, dtype=dtype)
+    table = torch.randperm(B * columns).view(B, columns).to(torch.int32)
+    q, k, v = (torch.randn(B, T, h, D, dtype=dtype) for h in (H, kv, kv))
+    if shared:
+        table[1:, :shared] = table[0, :shared]
+        k[1:, :shared * page], v[1:, :shared * page] = k[0, :shared * page], v[0, :shared * page]
+    rope = nn.RotaryEmbedding(D // 2 * 2)
+    lengths, outs = torch.zeros(B, dtype=torch.int32), []
+    for n in pieces:
+        at = int(lengths[0])
+        piece = slice(at, at + n)
+        x = cache.Append(k[:, piece], v[:, piece], table, lengths, rotary=rope, q=q[:, piece])
+        outs.append(cache.Attend(x, table, lengths, shared_pages=shared if at >= shared * page else 0))
+        lengths += n
+    qr, kr = rope(q), rope(k).repeat_interleave(H // kv, 2)
+    s = torch.einsum("bthd,bnhd->bhtn", qr, kr) / math.sqrt(D)
+    s = s.masked_fill(torch.ones(T, T, dtype=torch.bool).triu(1), -math.inf)
+    want = torch.einsum("bhtn,bnhd->bthd", torch.softmax(s, -1), v.repeat_interleave(H // kv, 2))
+    return torch.cat(outs, 1), want
+
+
+@pytest.mark.parametrize("pieces", [[1] * 9, [5, 1, 1, 4], [20], [16, 3]])
+def test_pieces(pieces):
+    got, want = steps(2, 2, 6, 8, 4, pieces)
+    assert torch.allclose(got, want)
+
+
+def test_shared_pages():
+    got, want = steps(3, 1, 2, 6, 4, [8, 1, 2], shared=2)
+    assert torch.allclose(got, want)
+
+
+def test_padded_batch():
+    cache = nn.KVCache(6, 4, 1, 4)
+    table, lengths = torch.arange(6, dtype=torch.int32).view(3, 2), torch.tensor([0, 3, 1], dtype=torch.int32)
+    counts = torch.tensor([2, 0, 3], dtype=torch.int32)
+    q, k, v = (torch.randn(3, 3, 1, 4) for _ in range(3))
+    before = cache.Keys.clone()
+    out = cache.Append(k, v, table, lengths, counts=counts, q=q)
+    assert torch.equal(out[0, :2], q[0, :2]) and not bool(out[0, 2:].any()) and not bool(out[1].any())
+    assert torch.equal(cache.Keys[0, 0, :2], k[0, :2, 0]) and torch.equal(cache.Keys[2:4], before[2:4]) and not bool(cache.Keys[0, 0, 2:].any())
+    y = cache.Attend(q, table, lengths, counts=counts)
+    assert not bool(y[1].any()) and not bool(y[0, 2].any()) and bool(y[2].any())
+    assert torch.allclose(y[0, 0], v[0, 0])                    # the first position sees itself alone
+
+
+def test_refusals():
+    i32 = dict(dtype=torch.int32)
+    cache = nn.KVCache(4, 16, 2, 8)
+    k, q = torch.zeros(2, 1, 2, 8), torch.zeros(2, 1, 4, 8)
+    table, at = torch.zeros(2, 1, **i32), torch.zeros(2, **i32)
+    for bad in (dict(dim=0), dict(dim=3), dict(dim=2050), dict(dim=4, scaling="other"), dict(dim=2, scaling="base"), dict(dim=4, factor=0.0),
+                dict(dim=4, scaling="bands"), dict(dim=4, scaling="bands", original=8, low=4, high=4), dict(dim=4, base=-1.0)):
+        with pytest.raises(ValueError):
+            nn.RotaryEmbedding(**bad)
+    rope = nn.RotaryEmbedding(8)
+    for x, p, error in ((torch.zeros(2, 8), None, ValueError), (torch.zeros(1, 1, 1, 6), None, ValueError), (k, torch.zeros(2, 2, **i32), ValueError),
+                        (k, torch.zeros(1), TypeError), (k.int(), None, TypeError)):
+        with pytest.raises(error):
+            rope(x, p)
+    for shape in ((0, 1, 1, 1), (1, 0, 1, 1)):
+        with pytest.raises(ValueError):
+            nn.KVCache(*shape)
+    with pytest.raises(ValueError):
+        nn.KVCache.Over(torch.zeros(1, 2, 3, 4), torch.zeros(1, 2, 3, 5))
+    with pytest.raises(TypeError):
+        nn.KVCache(1, 1, 1, 1, dtype=torch.int8)
+    for args, error in (((k[..., :4], k[..., :4], table, at), ValueError), ((k[:, :, :1], k, table, at), ValueError), ((k.double(), k, table, at), TypeError),
+                        ((k, k, table.long(), at), TypeError), ((k, k, table, at[:1]), ValueError), ((k, k, table[:, :0], at), ValueError),
+                        ((k, k, table, at + 16), ValueError), ((k, k, table, at - 1), ValueError), ((k, k, table + 4, at), ValueError),
+                        ((k, k, torch.zeros(2, 2 ** 27, **i32).expand(2, 2 ** 27), at), ValueError)):
+        with pytest.raises(error):
+            cache.Append(*args)
+    with pytest.raises(ValueError):
+        cache.Append(k, k, table, at, rotary=nn.RotaryEmbedding(10))
+    with pytest.raises(ValueError):
+        cache.Append(k, k, table, at, q=q[:1])
+    for kw, error in ((dict(q=q[:, :, :3]), ValueError), (dict(q=q[..., :4]), ValueError), (dict(q=q.half()), TypeError), (dict(shared_pages=2), ValueError),
+                      (dict(shared_pages=-1), ValueError), (dict(scale=0.0), ValueError), (dict(scale=-1.0), ValueError), (dict(scale=math.inf), ValueError),
+                      (dict(lengths=at + 16), ValueError), (dict(table=table - 1), ValueError), (dict(counts=at.long()), TypeError)):
+        with pytest.raises(error):
+            cache.Attend(**{**dict(q=q, table=table, lengths=at), **kw})
+    grad = q.clone().requires_grad_()
+    with pytest.raises(RuntimeError):
+        cache.Attend(grad, table, at)
+    with torch.no_grad():
+        cache.Attend(grad, table, at)
