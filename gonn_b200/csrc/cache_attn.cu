@@ -141,6 +141,7 @@ struct Cursor {
 
 struct Share {
   long long first, count, total;     // of this CTA's tiles, of all
+  int ctas;                          // that have any
   int e;                             // the entry of the first one
   long long into;                    // tiles of that entry before it
 };
@@ -167,7 +168,8 @@ __device__ __forceinline__ Share share_of(const CacheArgs& a, long long* s_sum, 
     total += s_sum[w];
   }
   before += sum - mine;
-  const long long first = total * blockIdx.x / a.ctas, end = total * (blockIdx.x + 1) / a.ctas;
+  const int ctas = (int)min((long long)a.ctas, total);               // so that none between two others has nothing
+  const long long first = blockIdx.x < ctas ? total * blockIdx.x / ctas : 0, end = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : 0;
   if (end > first && first >= before && first < before + mine) {
     int e = lo;
     long long at = before;
@@ -176,9 +178,9 @@ __device__ __forceinline__ Share share_of(const CacheArgs& a, long long* s_sum, 
       if (first < at + n) break;
       at += n;
     }
-    *s_share = {first, end - first, total, e, first - at};
+    *s_share = {first, end - first, total, ctas, e, first - at};
   }
-  if (tid == 0 && end == first) *s_share = {first, 0, total, 0, 0};
+  if (tid == 0 && end == first) *s_share = {first, 0, total, ctas, 0, 0};
   __syncthreads();
   return *s_share;
 }
@@ -344,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_kernel(const CacheArgs
     // Where its rows go: straight to the output, to the partial rows of a whole segment (in the output's order, those of the prefix
     // behind the sequences'), or to this CTA's first or last ones.
     const int slot = 2 * blockIdx.x + (first_segment ? 0 : 1);
-    if (at.tile == 0 && threadIdx.x == 0) a.owner[seg] = make_int2(slot, cta_of(segment0 + at.x.tiles - 1, share.total, a.ctas));
+    if (at.tile == 0 && threadIdx.x == 0) a.owner[seg] = make_int2(slot, cta_of(segment0 + at.x.tiles - 1, share.total, share.ctas));
     const bool direct = whole && a.prefix_tiles == 0;
     auto part_row = [&](const Row& w, int r) -> long long {
       if (!whole) return (long long)slot * ROWS + r;

@@ -318,7 +318,8 @@ def test_bad_tables_are_reported():
 
 def test_other_streams_and_graphs():
     """Two captured calls replayed on different streams, with lengths that change between replays; none shares a workspace."""
-    cache, table, at, c, (q, k, v) = batch(6, 1, 8, 2, 128, 16, [100, 0, 64, 63, 500, 31], BF)
+    cache, table, at, c, new = batch(6, 2, 8, 2, 128, 16, [100, 0, 64, 63, 500, 31], BF)          # pages for the second token too
+    q, k, v = (t[:, :1] for t in new)
     rope = nn.RotaryEmbedding(128, device="cuda")
     other, table2, at2, c2, (q2, k2, v2) = batch(4, 2, 4, 4, 64, 24, [700, 3, 64, 90], F16, prefix=0)
     rope2 = nn.RotaryEmbedding(32, interleaved=True, device="cuda")
