@@ -14,9 +14,13 @@
 // A shared prefix is one more entry at the head of the list whose rows are the queries of all sequences: its keys are read once for
 // every 16, 32 or 64 rows.  The sequences' own entries then start behind it, and all rows are joined by the second kernel.
 //
-// A CTA: four warps that multiply (mma.sync for 16-bit types, FMA for fp32) and one that copies (cp.async, 16 bytes a lane, a page looked
-// up for every key, so a page may have any size) through a ring of stages.
+// A CTA: four warps that multiply (mma.sync for 16-bit types, FMA for fp32) and one that copies through a ring of stages: by TMA, a box of
+// as many rows as divide both a page and a tile, where these are at least eight (a multiple of the swizzle's period); else with cp.async,
+// 16 bytes a lane, a page looked up for every key.  What stands behind a sequence's last key in its last page may be anything, NaN
+// too: those scores are masked, and those rows of V become zeros in shared memory.
 #include "common.cuh"
+
+#include <string.h>
 
 #include <atomic>
 
@@ -46,6 +50,7 @@ struct CacheArgs {
   int ctas;
   float* part;                             // [slots][rows of a tile][D] unscaled sums
   float2* stat;                            // [slots][rows of a tile] (m, l)
+  int box;                                 // rows of a TMA box
   int2* owner;                             // [(prefix tiles + B own_tiles) Hkv] first and last CTA
   int* status;
 };
@@ -74,7 +79,8 @@ struct Cfg {
   static constexpr int STAGES = HD == 64 ? 6 : 3;
   static constexpr int CHUNKS = HD * (int)sizeof(T) / 16;         // 16-byte chunks of a row
   static constexpr int EXTRA = kMma ? (KG > 1 ? KG / 2 * ROWS * (HD * 4 + 8) : 0) : ROWS * HD * 4 + ROWS * TILE * 4;   // joined groups; queries and weights
-  static constexpr int SMEM = 2 * STAGES * SUB + EXTRA + 256 + 1024;
+  static constexpr int COLS = HD * (int)sizeof(T) / 128;          // columns of 128 bytes
+  static constexpr int SMEM = 2 * STAGES * SUB + EXTRA + 256 + 1024 + 2 * TILE * 8;
 };
 
 // ---------------------------------------------------------------------------------------------------------------------------
@@ -206,12 +212,20 @@ __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uin
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Byte of a 16-byte chunk in a tile: 16-bit rows lie in columns of 64 elements (128 bytes), fp32 rows whole; the chunk's last three
-// bits are exchanged by the row's, so that eight rows' chunks lie in eight different banks.
-template <typename T, int HD, int TILE>
+// Byte of a 16-byte chunk in a tile: rows lie in columns of 128 bytes, and a chunk's place in its row is exchanged by the row's last three
+// bits, so that eight rows' chunks lie in eight different banks (the 128-byte swizzle of TMA).
+template <int TILE>
 __device__ __forceinline__ uint32_t chunk_at(int row, int chunk) {
-  if constexpr (sizeof(T) == 2) return (uint32_t)((chunk >> 3) * (TILE * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
-  else return (uint32_t)(row * (HD * 4) + ((chunk ^ (row & 7)) << 4));
+  return (uint32_t)((chunk >> 3) * (TILE * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+}
+
+// Zeros in place of the rows from..to of V.  By a warp.
+template <int TILE, int CHUNKS>
+__device__ __forceinline__ void clear_rows(uint8_t* tile, int from, int to, int lane) {
+  for (int i = from * CHUNKS + lane; i < to * CHUNKS; i += 32)
+    *reinterpret_cast<uint4*>(tile + chunk_at<TILE>(i / CHUNKS, i % CHUNKS)) = make_uint4(0u, 0u, 0u, 0u);
+  fence_proxy_async_smem();                // before a copy overwrites them
+  __syncwarp();
 }
 
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
@@ -243,8 +257,9 @@ __device__ __forceinline__ Row row_of(const CacheArgs& a, const Entry& x, int r)
   return w;
 }
 
-template <typename T, int HD, int RG>
-__global__ void __launch_bounds__(kThreads, 2) cache_attn_kernel(const CacheArgs a) {
+template <typename T, int HD, int RG, bool TMA>
+__global__ void __launch_bounds__(kThreads, 2)
+cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const CacheArgs a) {
   using C = Cfg<T, HD, RG>;
   constexpr int ROWS = C::ROWS, TILE = C::TILE, STAGES = C::STAGES, SUB = C::SUB;
   extern __shared__ uint8_t smem_raw[];
@@ -257,11 +272,12 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_kernel(const CacheArgs
   long long* s_sum = (long long*)(empty + STAGES);
   Share* s_share = (Share*)(s_sum + kThreads / 32);
   volatile int* abort_flag = (volatile int*)(s_share + 1);
+  long long* s_off = (long long*)(s_extra + C::EXTRA + 256);        // where the keys and values of a tile start
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; i++) {
-      mbar_init(&full[i], 32);
+      mbar_init(&full[i], TMA ? 1 : 32);
       mbar_init(&empty[i], kConsumers);
     }
     *abort_flag = 0;
@@ -276,10 +292,48 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_kernel(const CacheArgs
 
   if (warp == kConsumers) {
     // ---------------- copies ----------------
+    if constexpr (TMA) {
+      // lane i: column i % COLS of box i / COLS of keys and of values
+      const int box = lane / C::COLS, col = lane % C::COLS * (128 / (int)sizeof(T));
+      const bool mine = box * a.box < TILE;                          // (columns behind the head's last one: zeros)
+      int page = 0, in_page = 0;
+      auto look_up = [&]() {
+        if (!mine) return;
+        const int key = at.x.begin + at.tile * TILE + box * a.box;
+        page = a.pages;                                              // behind the last one: zeros
+        in_page = 0;
+        if (key < at.x.end) {
+          const unsigned p = (unsigned)key / (unsigned)a.page;
+          in_page = (int)((unsigned)key - p * (unsigned)a.page);
+          page = a.table[(at.x.b < 0 ? 0 : at.x.b) * a.table_stride + p];
+          if (page < 0 || page >= a.pages) {
+            set_status(a.status, ST_BAD_INDEX, at.x.b);
+            page = a.pages;
+          }
+        }
+      };
+      look_up();
+      int st = 0;
+      uint32_t ph = 0;
+      for (long long n = 0; n < share.count; n++) {
+        const int h = at.h, pg = page, row = in_page;
+        if (++at.tile == at.x.tiles) at.next_segment(a);
+        if (n + 1 < share.count) look_up();                          // on its way while this stage is waited for
+        if (!mbar_wait(&empty[st], ph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 20)) break;
+        if (lane == 0) mbar_expect_tx(&full[st], 2 * SUB);
+        __syncwarp();
+        if (mine) {
+          const int to = st * SUB + lane % C::COLS * (TILE * 128) + box * a.box * 128;
+          tma_load_4d(s_k + to, &tm_k, &full[st], col, row, h, pg);
+          tma_load_4d(s_v + to, &tm_v, &full[st], col, row, h, pg);
+        }
+        if (++st == STAGES) { st = 0; ph ^= 1; }
+      }
+      return;
+    }
     constexpr int LOOK = TILE / 32;                                  // keys that a lane looks up
-    constexpr int PER = 32 / C::CHUNKS < 1 ? 1 : 32 / C::CHUNKS;     // rows of one instruction of the warp
-    constexpr int SPAN = C::CHUNKS < 32 ? C::CHUNKS : 32;
-    const int sub = lane / SPAN, chunk = lane % SPAN;
+    constexpr int PER = 32 / C::CHUNKS;                              // rows of one instruction of the warp
+    const int sub = lane / C::CHUNKS, chunk = lane % C::CHUNKS;
     const bool inside = chunk * 16 < a.D * (int)sizeof(T);
     int page[LOOK], in_page[LOOK];
     auto look_up = [&]() {
@@ -304,28 +358,26 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_kernel(const CacheArgs
     int st = 0;
     uint32_t ph = 0;
     for (long long n = 0; n < share.count; n++) {
-      long long k_off[LOOK], v_off[LOOK];
 #pragma unroll
       for (int i = 0; i < LOOK; i++) {
-        k_off[i] = page[i] < 0 ? -1 : page[i] * a.k_sp + at.h * a.k_sh + in_page[i] * a.k_sr;
-        v_off[i] = page[i] < 0 ? -1 : page[i] * a.v_sp + at.h * a.v_sh + in_page[i] * a.v_sr;
+        s_off[i * 32 + lane] = page[i] < 0 ? -1 : page[i] * a.k_sp + at.h * a.k_sh + in_page[i] * a.k_sr;
+        s_off[TILE + i * 32 + lane] = page[i] < 0 ? -1 : page[i] * a.v_sp + at.h * a.v_sh + in_page[i] * a.v_sr;
       }
+      __syncwarp();
       if (++at.tile == at.x.tiles) at.next_segment(a);
-      if (n + 1 < share.count) look_up();                            // on their way while this stage is waited for
+      if (n + 1 < share.count) look_up();
       if (!mbar_wait(&empty[st], ph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 20)) break;
       uint8_t* dk = s_k + st * SUB;
       uint8_t* dv = s_v + st * SUB;
-#pragma unroll
-      for (int i = 0; i < LOOK; i++) {
-#pragma unroll 4
-        for (int r = 0; r < 32; r += PER) {
-          const long long ko = __shfl_sync(0xffffffffu, k_off[i], r + sub), vo = __shfl_sync(0xffffffffu, v_off[i], r + sub);
-          const int bytes = ko >= 0 && inside ? 16 : 0;
-          const uint32_t to = chunk_at<T, HD, TILE>(i * 32 + r + sub, chunk);
-          cp_async16(dk + to, (const T*)a.k + (bytes ? ko + chunk * (16 / (int)sizeof(T)) : 0), bytes);
-          cp_async16(dv + to, (const T*)a.v + (bytes ? vo + chunk * (16 / (int)sizeof(T)) : 0), bytes);
-        }
+#pragma unroll 8
+      for (int r = 0; r < TILE; r += PER) {
+        const long long ko = s_off[r + sub], vo = s_off[TILE + r + sub];
+        const int bytes = ko >= 0 && inside ? 16 : 0;
+        const uint32_t to = chunk_at<TILE>(r + sub, chunk);
+        cp_async16(dk + to, (const T*)a.k + (bytes ? ko + chunk * (16 / (int)sizeof(T)) : 0), bytes);
+        cp_async16(dv + to, (const T*)a.v + (bytes ? vo + chunk * (16 / (int)sizeof(T)) : 0), bytes);
       }
+      __syncwarp();
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[st])) : "memory");
       if (++st == STAGES) { st = 0; ph ^= 1; }
     }
@@ -358,10 +410,15 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_kernel(const CacheArgs
       const int rg = warp / C::KG, kg = warp % C::KG;
       constexpr int NK = TILE / C::KG;                               // keys of this warp
       const int r0 = rg * 16 + (lane >> 2), r1 = r0 + 8;
-      const Row w0 = row_of(a, at.x, r0), w1 = row_of(a, at.x, r1);
-      const bool idle = !__any_sync(0xffffffffu, w0.counts || w1.counts);
       uint32_t qf[HD / 16][4];
+      int sees0, sees1;
+      bool idle;
       {
+        const Row w0 = row_of(a, at.x, r0), w1 = row_of(a, at.x, r1);
+        idle = !__any_sync(0xffffffffu, w0.counts || w1.counts);
+        // rows of nothing are masked nowhere: what they add up to is not used
+        sees0 = w0.counts ? w0.sees : 0x7fffffff;
+        sees1 = w1.counts ? w1.sees : 0x7fffffff;
         const T* q0 = (const T*)a.q + w0.b * a.q_sb + w0.t * a.q_st + (long long)(at.h * a.G + w0.g) * a.q_sh;
         const T* q1 = (const T*)a.q + w1.b * a.q_sb + w1.t * a.q_st + (long long)(at.h * a.G + w1.g) * a.q_sh;
 #pragma unroll
@@ -373,8 +430,6 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_kernel(const CacheArgs
             qf[s][i] = ok ? *reinterpret_cast<const uint32_t*>(((i & 1) ? q1 : q0) + col) : 0u;
           }
       }
-      // rows of nothing are masked nowhere: what they add up to is not used
-      const int sees0 = w0.counts ? w0.sees : 0x7fffffff, sees1 = w1.counts ? w1.sees : 0x7fffffff;
       float o[HD / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 #pragma unroll
       for (int j = 0; j < HD / 8; j++)
@@ -398,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_kernel(const CacheArgs
 #pragma unroll
             for (int x = 0; x < HD / 16; x++) {
               uint32_t b[4];
-              ldm4(b, ka + chunk_at<T, HD, TILE>(row, x * 2 + ((lane >> 3) & 1)));
+              ldm4(b, ka + chunk_at<TILE>(row, x * 2 + ((lane >> 3) & 1)));
               mma16<T>(s[2 * j], qf[x], b[0], b[1]);
               mma16<T>(s[2 * j + 1], qf[x], b[2], b[3]);
             }
@@ -413,6 +468,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_kernel(const CacheArgs
                 if (key >= min((c & 2) ? sees1 : sees0, at.x.end)) s[j][c] = -INFINITY;
               }
           }
+          if (TMA && at.x.end - key0 < NK) clear_rows<TILE, C::CHUNKS>(s_v + st * SUB, kg * NK + max(at.x.end - key0, 0), kg * NK + NK, lane);
           float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
           for (int j = 0; j < NK / 8; j++) {
@@ -459,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_kernel(const CacheArgs
 #pragma unroll
             for (int x = 0; x < HD / 16; x++) {                      // 16 columns
               uint32_t b[4];
-              ldm4t(b, va + chunk_at<T, HD, TILE>(row, x * 2 + (lane >> 4)));
+              ldm4t(b, va + chunk_at<TILE>(row, x * 2 + (lane >> 4)));
               mma16<T>(o[2 * x], p, b[0], b[1]);
               mma16<T>(o[2 * x + 1], p, b[2], b[3]);
             }
@@ -518,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_kernel(const CacheArgs
       if (kg == 0) {
 #pragma unroll
         for (int half = 0; half < 2; half++) {
-          const Row& w = half ? w1 : w0;
+          const Row w = row_of(a, at.x, half ? r1 : r0);
           const float m = half ? m1 : m0, l = half ? l1 : l0;
           const int r = half ? r1 : r0;
           if (direct) {
@@ -578,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_kernel(const CacheArgs
           float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
           for (int c = 0; c < HD / 4; c++) {
-            const float4 kk = *reinterpret_cast<const float4*>(kt + chunk_at<T, HD, TILE>(lane, c));
+            const float4 kk = *reinterpret_cast<const float4*>(kt + chunk_at<TILE>(lane, c));
 #pragma unroll
             for (int r = 0; r < 4; r++) {
               const float4 qq = *reinterpret_cast<const float4*>(s_q + (warp * 4 + r) * HD + c * 4);
@@ -588,6 +644,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_kernel(const CacheArgs
               s[r] = fmaf(qq.w, kk.w, s[r]);
             }
           }
+          if (TMA && at.x.end - key + lane < TILE) clear_rows<TILE, C::CHUNKS>(s_v + st * SUB, at.x.end - key + lane, TILE, lane);
           float4 p4;
           float* p = &p4.x;
 #pragma unroll
@@ -611,7 +668,7 @@ __global__ void __launch_bounds__(kThreads, 2) cache_attn_kernel(const CacheArgs
           for (int j = 0; j < TILE; j++) {
             const float4 pj = *reinterpret_cast<const float4*>(s_p + j * 4);
             float v[CPL];
-            const uint8_t* vr = vt + chunk_at<T, HD, TILE>(j, lane * CPL / 4);
+            const uint8_t* vr = vt + chunk_at<TILE>(j, lane * CPL / 4);
             if constexpr (CPL == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(vr);
             else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(vr + (lane & 1) * 8);
 #pragma unroll
@@ -736,30 +793,56 @@ bool plan(Sizes& z, int dtype, long long B, long long T, long long H, long long 
   return true;
 }
 
-template <typename T, int HD, int RG>
-int launch_attn(CacheArgs& a, cudaStream_t s) {
+template <typename T, int HD, int RG, bool TMA>
+int launch_attn(const CUtensorMap& tk, const CUtensorMap& tv, CacheArgs& a, cudaStream_t s) {
   using C = Cfg<T, HD, RG>;
+  const auto kernel = cache_attn_kernel<T, HD, RG, TMA>;
   static std::atomic<uint32_t> done{0};
   int dev = 0;
   GB_CUDA_OK(cudaGetDevice(&dev));
   if (dev >= 32 || !(done.load() >> dev & 1u)) {
-    GB_CUDA_OK(cudaFuncSetAttribute(cache_attn_kernel<T, HD, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    GB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     if (dev < 32) done.fetch_or(1u << dev);
   }
-  GB_CUDA_OK(gbh::launch(cache_attn_kernel<T, HD, RG>, dim3(a.ctas), dim3(kThreads), C::SMEM, s, 1, a));
+  GB_CUDA_OK(gbh::launch(kernel, dim3(a.ctas), dim3(kThreads), C::SMEM, s, 1, tk, tv, a));
   const long long rows = (long long)a.B * a.T * a.H;
   GB_CUDA_OK(gbh::launch(cache_join_kernel<T, C::ROWS, C::TILE>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, 1, a));
   return gbh::E_OK;
 }
 
-template <typename T>
-int launch_type(CacheArgs& a, int rows, cudaStream_t s) {
+// (columns, rows of a page, heads, pages) in boxes of 128 bytes by `rows` rows
+int cache_map(CUtensorMap* m, int dtype, const void* base, int D, int page, int heads, int pages, const long long* strides, int rows) {
+  const int size = dtype == 2 ? 4 : 2;
+  const uint64_t dims[4] = {(uint64_t)D, (uint64_t)page, (uint64_t)heads, (uint64_t)pages};
+  const uint64_t st[3] = {(uint64_t)strides[2] * size, (uint64_t)strides[1] * size, (uint64_t)strides[0] * size};
+  const uint32_t box[4] = {128u / size, (uint32_t)rows, 1u, 1u};
+  const CUtensorMapDataType type = dtype == 0 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  return gbh::encode_tmap(m, type, 4, base, dims, st, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// Rows of a TMA box, 0 where there can be none: a power of two that divides a page and a tile; strides that a tensor map holds.
+int box_of(int page, int tile, const long long* strides, int size) {
+  int rows = tile;
+  while (rows > 1 && page % rows) rows >>= 1;
+  for (int i = 0; i < 6; i++)
+    if (strides[i] <= 0 || strides[i] * size >= (1LL << 40)) return 0;
+  return rows >= 8 ? rows : 0;
+}
+
+template <typename T, bool TMA>
+int launch_type(const CUtensorMap& k, const CUtensorMap& v, CacheArgs& a, int rows, cudaStream_t s) {
   if constexpr (Elem<T>::kMma) {
-    if (a.D <= 64) return rows == 16 ? launch_attn<T, 64, 1>(a, s) : rows == 32 ? launch_attn<T, 64, 2>(a, s) : launch_attn<T, 64, 4>(a, s);
-    return rows == 16 ? launch_attn<T, 128, 1>(a, s) : rows == 32 ? launch_attn<T, 128, 2>(a, s) : launch_attn<T, 128, 4>(a, s);
+    if (a.D <= 64)
+      return rows == 16 ? launch_attn<T, 64, 1, TMA>(k, v, a, s) : rows == 32 ? launch_attn<T, 64, 2, TMA>(k, v, a, s) : launch_attn<T, 64, 4, TMA>(k, v, a, s);
+    return rows == 16 ? launch_attn<T, 128, 1, TMA>(k, v, a, s) : rows == 32 ? launch_attn<T, 128, 2, TMA>(k, v, a, s) : launch_attn<T, 128, 4, TMA>(k, v, a, s);
   } else {
-    return a.D <= 64 ? launch_attn<T, 64, 1>(a, s) : launch_attn<T, 128, 1>(a, s);
+    return a.D <= 64 ? launch_attn<T, 64, 1, TMA>(k, v, a, s) : launch_attn<T, 128, 1, TMA>(k, v, a, s);
   }
+}
+
+template <typename T>
+int launch_any(const CUtensorMap& k, const CUtensorMap& v, CacheArgs& a, int rows, cudaStream_t s) {
+  return a.box ? launch_type<T, true>(k, v, a, rows, s) : launch_type<T, false>(k, v, a, rows, s);
 }
 
 }  // namespace
@@ -829,7 +912,16 @@ GB_EXPORT int gb_cache_attn(int dtype, const void* q, const void* k, const void*
   a.owner = (int2*)((uint8_t*)ws + z.part + z.stat);
   a.status = gbh::status_ptr();
   cudaStream_t s = (cudaStream_t)stream;
-  if (dtype == 0) return launch_type<__nv_bfloat16>(a, z.rows, s);
-  if (dtype == 1) return launch_type<__half>(a, z.rows, s);
-  return launch_type<float>(a, z.rows, s);
+  CUtensorMap tk, tv;
+  memset(&tk, 0, sizeof(tk));
+  memset(&tv, 0, sizeof(tv));
+  a.box = box_of(page, dtype == 2 ? 32 : 64, strides + 3, size);
+  if (a.box) {
+    int rc;
+    if ((rc = cache_map(&tk, dtype, k, D, page, Hkv, pages, strides + 3, a.box))) return rc;
+    if ((rc = cache_map(&tv, dtype, v, D, page, Hkv, pages, strides + 6, a.box))) return rc;
+  }
+  if (dtype == 0) return launch_any<__nv_bfloat16>(tk, tv, a, z.rows, s);
+  if (dtype == 1) return launch_any<__half>(tk, tv, a, z.rows, s);
+  return launch_any<float>(tk, tv, a, z.rows, s);
 }
