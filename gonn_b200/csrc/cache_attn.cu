@@ -51,6 +51,10 @@ struct CacheArgs {
   float* part;                             // [slots][rows of a tile][D] unscaled sums
   float2* stat;                            // [slots][rows of a tile] (m, l)
   int box;                                 // rows of a TMA box
+  int shared;                              // a prefix is joined to the sequences' own keys
+  int wide_prefix, wide_own;               // which of them the kernel for many rows takes
+  int wide_tiles, splits;                  // its row tiles, of a sequence or of the prefix; runs of keys
+  int slot_rows;                           // rows of the other kernel's tiles
   int2* owner;                             // [(prefix tiles + B own_tiles) Hkv] first and last CTA
   int* status;
 };
@@ -91,6 +95,7 @@ struct Entry {                // rows of queries over a range of keys, for every
   int row0;                   // first row
   int begin, end;             // keys
   int tiles;                  // of one key head
+  bool cut;                   // keys behind the end of its table were asked for
 };
 
 __device__ __forceinline__ int count_of(const CacheArgs& a, int b) {
@@ -102,6 +107,7 @@ template <int ROWS, int TILE>
 __device__ __forceinline__ Entry entry_of(const CacheArgs& a, int e) {
   Entry x;
   x.begin = a.prefix;
+  x.cut = false;
   if (e < a.prefix_tiles) {
     x.b = -1;
     x.row0 = e * ROWS;
@@ -115,7 +121,8 @@ __device__ __forceinline__ Entry entry_of(const CacheArgs& a, int e) {
     const int c = count_of(a, x.b), last = min(a.T * a.G, x.row0 + ROWS) - 1;
     const int seen = min(c, last / a.G + 1);                         // tokens of these rows that count, and those before them
     const long long end = x.row0 / a.G < c ? (long long)a.lengths[x.b] + seen : 0;
-    x.end = (int)(end < a.room ? end : (long long)a.room);
+    x.cut = end > a.room;
+    x.end = (int)(x.cut ? (long long)a.room : end > 0 ? end : 0);
   }
   x.tiles = x.end > x.begin ? (x.end - x.begin + TILE - 1) / TILE : 0;
   return x;
@@ -158,7 +165,11 @@ __device__ __forceinline__ Share share_of(const CacheArgs& a, long long* s_sum, 
   const int entries = a.prefix_tiles + a.B * a.own_tiles, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (entries + kThreads - 1) / kThreads, lo = min(entries, tid * per), hi = min(entries, lo + per);
   long long mine = 0;
-  for (int e = lo; e < hi; e++) mine += entry_of<ROWS, TILE>(a, e).tiles;
+  for (int e = lo; e < hi; e++) {
+    const Entry x = entry_of<ROWS, TILE>(a, e);
+    mine += x.tiles;
+    if (x.cut && blockIdx.x == 0) set_status(a.status, ST_BAD_INDEX, x.b);
+  }
   mine *= a.Hkv;
   long long sum = mine;
 #pragma unroll
@@ -210,6 +221,26 @@ __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uin
   else
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ unsigned long long pair(uint32_t lo, uint32_t hi) { return (unsigned long long)hi << 32 | lo; }
+__device__ __forceinline__ unsigned long long pairf(float lo, float hi) { return pair(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ float lo_of(unsigned long long v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi_of(unsigned long long v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ unsigned long long fmul2(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ unsigned long long ffma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ unsigned long long fadd2(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 
 // Byte of a 16-byte chunk in a tile: rows lie in columns of 128 bytes, and a chunk's place in its row is exchanged by the row's last three
@@ -399,7 +430,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     // behind the sequences'), or to this CTA's first or last ones.
     const int slot = 2 * blockIdx.x + (first_segment ? 0 : 1);
     if (at.tile == 0 && threadIdx.x == 0) a.owner[seg] = make_int2(slot, cta_of(segment0 + at.x.tiles - 1, share.total, share.ctas));
-    const bool direct = whole && a.prefix_tiles == 0;
+    const bool direct = whole && !a.shared;
     auto part_row = [&](const Row& w, int r) -> long long {
       if (!whole) return (long long)slot * ROWS + r;
       const long long bt = (long long)w.b * a.T + w.t;
@@ -711,8 +742,338 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   }
 }
 
-// Joins the partial rows of a query row in the order of the list, prefix first: a warp a row, a lane every 32nd column.  Rows that the
-// first kernel has written are left alone; rows that see nothing become zeros.
+// ---------------------------------------------------------------------------------------------------------------------------
+// many rows of 16 bits: tcgen05
+// ---------------------------------------------------------------------------------------------------------------------------
+// More than 64 rows share their keys: a batch over its shared prefix, or several tokens of a sequence.  Then the products count and not the keys'
+// bytes, and a CTA takes 128 rows over a run of keys: scores and sums in TMEM, Q in shared memory, K and V by TMA in sub-tiles of 64
+// keys, weights written over their scores as the second product's operand; two score buffers, so that the next scores are computed while
+// a softmax warp (a row a thread) works.  The sum is rescaled only when the maximum has moved by more than 2^8.  Where the row tiles are too few
+// for the SMs, the keys are cut into `splits` runs, which leave partial rows.
+constexpr int kWideRows = 128, kWideKeys = 64, kWideThreads = 192;
+
+template <int HD>
+struct Wide {
+  static constexpr int CH = HD / 64, Q_BYTES = CH * kWideRows * 128, SUB = CH * kWideKeys * 128;
+  static constexpr int STAGES = HD == 64 ? 3 : 2;
+  static constexpr int SMEM = Q_BYTES + 2 * STAGES * SUB + 1024 + 256;
+  static constexpr int COLS = 256, COL_O = 128;
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kWideThreads, 2)
+cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const CacheArgs a) {
+  using C = Wide<HD>;
+  constexpr int STAGES = C::STAGES, SUB = C::SUB;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* s_q = smem;
+  uint8_t* s_k = s_q + C::Q_BYTES;
+  uint8_t* s_v = s_k + STAGES * SUB;
+  uint64_t* q_full = (uint64_t*)(s_v + STAGES * SUB);
+  uint64_t* k_full = q_full + 1;
+  uint64_t* k_empty = k_full + STAGES;
+  uint64_t* v_full = k_empty + STAGES;
+  uint64_t* v_empty = v_full + STAGES;
+  uint64_t* s_full = v_empty + STAGES;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* pv_done = p_full + 2;
+  uint32_t* tmem_slot = (uint32_t*)(pv_done + 2);
+  volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 4);
+    for (int i = 0; i < STAGES; i++) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&pv_done[i], 1);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_trigger();
+
+  // Row tiles of a sequence run from its last one, which sees the most keys, to its first.
+  unsigned idx = blockIdx.x;
+  const int rank = idx % a.wide_tiles;
+  idx /= a.wide_tiles;
+  const int split = idx % a.splits;
+  idx /= a.splits;
+  const int h = idx % a.Hkv;
+  Entry x;
+  x.b = a.wide_prefix ? -1 : (int)(idx / a.Hkv);
+  x.row0 = (a.wide_prefix ? rank : a.wide_tiles - 1 - rank) * kWideRows;
+  x.begin = 0;
+  if (a.wide_prefix) {
+    x.end = a.prefix;
+  } else {
+    const int c = count_of(a, x.b), last = min(a.T * a.G, x.row0 + kWideRows) - 1;
+    const long long end = x.row0 / a.G < c ? (long long)a.lengths[x.b] + min(c, last / a.G + 1) : 0;
+    x.end = (int)max(0LL, min(end, (long long)a.room));
+    if (end > a.room && threadIdx.x == 0 && split == 0) set_status(a.status, ST_BAD_INDEX, x.b);
+  }
+  x.tiles = (x.end + kWideKeys - 1) / kWideKeys;
+  const int first = (int)((long long)x.tiles * split / a.splits), n_kv = (int)((long long)x.tiles * (split + 1) / a.splits) - first;
+
+  if (warp == 0) {
+    // lane i: columns i % CH of box i / CH
+    const int box = lane / C::CH, col = lane % C::CH * 64;
+    const bool mine = box * a.box < kWideKeys;
+    int page = 0, in_page = 0;
+    auto look_up = [&](int j) {
+      if (!mine) return;
+      const int key = (first + j) * kWideKeys + box * a.box;
+      page = a.pages;
+      in_page = 0;
+      if (key < x.end) {
+        const unsigned p = (unsigned)key / (unsigned)a.page;
+        in_page = (int)((unsigned)key - p * (unsigned)a.page);
+        page = a.table[(key < a.prefix ? 0 : x.b) * a.table_stride + p];
+        if (page < 0 || page >= a.pages) {
+          set_status(a.status, ST_BAD_INDEX, x.b);
+          page = a.pages;
+        }
+      }
+    };
+    if (n_kv > 0) look_up(0);
+    int st = 0;
+    uint32_t ph = 0;
+    const int to = lane % C::CH * (kWideKeys * 128) + box * a.box * 128;
+    for (int j = 0; j < n_kv; j++) {
+      const int pg = page, row = in_page;
+      if (j + 1 < n_kv) look_up(j + 1);
+      if (!mbar_wait(&k_empty[st], ph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 30)) break;
+      if (lane == 0) mbar_expect_tx(&k_full[st], SUB);
+      __syncwarp();
+      if (mine) tma_load_4d(s_k + st * SUB + to, &tm_k, &k_full[st], col, row, h, pg);
+      if (!mbar_wait(&v_empty[st], ph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 31)) break;
+      if (lane == 0) mbar_expect_tx(&v_full[st], SUB);
+      __syncwarp();
+      if (mine) tma_load_4d(s_v + st * SUB + to, &tm_v, &v_full[st], col, row, h, pg);
+      if (++st == STAGES) { st = 0; ph ^= 1; }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint32_t fmt = __is_same(T, __nv_bfloat16) ? 1u : 0u;
+      const uint32_t idesc_s = make_idesc(1u, fmt, false, false, kWideRows, kWideKeys);
+      const uint32_t idesc_o = make_idesc(1u, fmt, false, true, kWideRows, HD);
+      const uint32_t qa = smem_u32(s_q);
+      bool ok = n_kv > 0 && mbar_wait(q_full, 0, abort_flag, a.status, ST_ATTN_TIMEOUT, 32);
+      int st_s = 0, st = 0;
+      uint32_t ph_s = 0, ph = 0;
+      auto issue_s = [&](int j) {
+        if (!mbar_wait(&k_full[st_s], ph_s, abort_flag, a.status, ST_ATTN_TIMEOUT, 33)) return false;
+        tc_fence_after();
+        const uint32_t ka = smem_u32(s_k + st_s * SUB);
+#pragma unroll
+        for (int k = 0; k < HD / 16; k++)
+          tc_mma_f16(tmem + (j & 1) * kWideKeys, make_smem_desc_sw128(qa + (k / 4) * (kWideRows * 128) + (k % 4) * 32, 16, 1024),
+                     make_smem_desc_sw128(ka + (k / 4) * (kWideKeys * 128) + (k % 4) * 32, 16, 1024), idesc_s, k != 0);
+        tc_commit(&k_empty[st_s]);
+        tc_commit(&s_full[j & 1]);
+        if (++st_s == STAGES) { st_s = 0; ph_s ^= 1; }
+        return true;
+      };
+      if (ok) ok = issue_s(0);
+      for (int j = 0; j < n_kv && ok; j++) {
+        if (j + 1 < n_kv) ok = issue_s(j + 1);
+        ok = ok && mbar_wait(&p_full[j & 1], (j >> 1) & 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 34);
+        ok = ok && mbar_wait(&v_full[st], ph, abort_flag, a.status, ST_ATTN_TIMEOUT, 35);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t va = smem_u32(s_v + st * SUB), p_tmem = tmem + (j & 1) * kWideKeys;
+#pragma unroll
+        for (int k = 0; k < kWideKeys / 16; k++)
+          tc_mma_f16_ts(tmem + C::COL_O, p_tmem + (k >> 1) * 32 + (k & 1) * 8, make_smem_desc_sw128(va + k * 16 * 128, kWideKeys * 128, 1024), idesc_o,
+                        (j | k) != 0);
+        tc_commit(&v_empty[st]);
+        tc_commit(&pv_done[j & 1]);
+        if (++st == STAGES) { st = 0; ph ^= 1; }
+      }
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3, r = quarter * 32 + lane;
+    const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
+    const Row w = row_of(a, x, r);
+    bool ok = true;
+    if (n_kv > 0) {
+      // this row of Q, zeros where there is none
+      const uint4* q = reinterpret_cast<const uint4*>((const T*)a.q + w.b * a.q_sb + w.t * a.q_st + (long long)(h * a.G + w.g) * a.q_sh);
+#pragma unroll
+      for (int c = 0; c < HD / 8; c++)
+        *reinterpret_cast<uint4*>(s_q + chunk_at<kWideRows>(r, c)) = w.counts && c * 8 < a.D ? __ldg(q + c) : make_uint4(0u, 0u, 0u, 0u);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    }
+    // keys that this row, all rows and any row of the warp see; a row of nothing is masked nowhere
+    const int sees = w.counts ? min(w.sees, x.end) : x.end;
+    const int sees_all = __reduce_min_sync(0xffffffffu, sees), sees_any = __reduce_max_sync(0xffffffffu, w.counts ? sees : 0);
+    float m = -INFINITY;
+    unsigned long long l2 = 0ull;
+    const unsigned long long sl2 = pairf(a.scale_log2, a.scale_log2);
+    uint32_t s[2][32];
+    for (int j = 0; j < n_kv; j++) {
+      ok = mbar_wait(&s_full[j & 1], (j >> 1) & 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 36);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t at = lane_addr + (j & 1) * kWideKeys;
+      const int kv0 = (first + j) * kWideKeys;
+      if (kv0 + kWideKeys > x.end) {
+        // the last keys of all: zeros behind them in V, whose copy has to be there first
+        ok = mbar_wait(&v_full[j % STAGES], (j / STAGES) & 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 37);
+        if (!ok) break;
+        const int from = x.end - kv0, each = (kWideKeys - from + 3) / 4;
+        clear_rows<kWideKeys, HD / 8>(s_v + j % STAGES * SUB, min(kWideKeys, from + quarter * each), min(kWideKeys, from + (quarter + 1) * each), lane);
+      }
+      if (kv0 >= sees_any) {                      // none of this warp's rows sees any of them
+        uint32_t zero[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) zero[i] = 0u;
+        tmem_st16(at, zero);
+        tmem_st16(at + 32, zero);
+      } else {
+        tmem_ld32(at, s[0]);
+        tmem_ld32(at + 32, s[1]);
+        tmem_ld_wait();
+        if (kv0 + kWideKeys > sees_all) {
+#pragma unroll
+          for (int c = 0; c < 64; c++)
+            if (kv0 + c >= sees) s[c / 32][c % 32] = 0xff800000u;
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 64; c++) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(s[c / 32][c % 32]));
+        const float next = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2);
+        const bool need = m == -INFINITY ? next > m : next - m > 8.f;
+        if (__any_sync(0xffffffffu, need)) {
+          float f = 1.f;
+          if (need) {
+            f = m == -INFINITY ? 0.f : exp2f(m - next);
+            m = next;
+            l2 = fmul2(l2, pairf(f, f));
+          }
+          if (j > 0) {
+            ok = mbar_wait(&pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 38);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < HD / 16; c++) {
+              uint32_t ro[16];
+              tmem_ld16(lane_addr + C::COL_O + c * 16, ro);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; i++) ro[i] = __float_as_uint(__uint_as_float(ro[i]) * f);
+              tmem_st16(lane_addr + C::COL_O + c * 16, ro);
+            }
+            tmem_st_wait();
+          }
+        }
+        const float z = m == -INFINITY ? 0.f : m;
+        const unsigned long long nz = pairf(-z, -z);
+#pragma unroll
+        for (int g = 1; g >= 0; g--) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const unsigned long long y = ffma2(pair(s[g][2 * i], s[g][2 * i + 1]), sl2, nz);
+            const float p0 = exp2f(lo_of(y)), p1 = exp2f(hi_of(y));
+            l2 = fadd2(l2, pairf(p0, p1));
+            pk[i] = Elem<T>::pack(p0, p1);
+          }
+          tmem_st16(at + g * 32, pk);
+        }
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[j & 1]);
+    }
+    if (ok && n_kv > 0) ok = mbar_wait(&pv_done[(n_kv - 1) & 1], ((n_kv - 1) >> 1) & 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 39);
+    if (ok) {
+      tc_fence_after();
+      const float l = lo_of(l2) + hi_of(l2);
+      const bool direct = !a.wide_prefix && a.splits == 1;
+      const float f = direct ? (w.counts && l != 0.f ? __frcp_rn(l) : 0.f) : 1.f;
+      const long long all = (long long)a.B * a.T * a.H;
+      const long long here = w.there ? ((long long)w.b * a.T + w.t) * a.H + h * a.G + w.g : -1;
+      const long long row = here < 0 || direct ? here : (a.wide_prefix ? 2LL * a.ctas * a.slot_rows + all : 0) + split * all + here;
+      if (row >= 0 && !direct) a.stat[row] = make_float2(m, l);
+      // through this warp's part of Q's tile (all products have read it), so that a row leaves in whole lines: 32 rows of 64 fp32 or HD 16-bit values
+      uint8_t* buf = s_q + quarter * (32 * 128) * C::CH;
+      constexpr int PIECE = HD == 128 ? 64 : 32;                     // fp32 columns at a time
+#pragma unroll
+      for (int half = 0; half < HD / PIECE; half++) {
+        const bool last_half = half == HD / PIECE - 1;
+#pragma unroll
+        for (int c = 0; c < PIECE / 16; c++) {
+          uint32_t ro[16];
+          if (n_kv > 0) {
+            tmem_ld16(lane_addr + C::COL_O + half * PIECE + c * 16, ro);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; i++) ro[i] = 0u;
+          }
+          if (direct) {
+            uint32_t o[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) o[i] = f == 0.f ? 0u : Elem<T>::pack(__uint_as_float(ro[2 * i]) * f, __uint_as_float(ro[2 * i + 1]) * f);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              const int chunk = half * (PIECE / 8) + c * 2 + i;
+              *reinterpret_cast<uint4*>(buf + (lane * (HD / 8) + (chunk ^ (lane & 7))) * 16) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              *reinterpret_cast<uint4*>(buf + (lane * (PIECE / 4) + ((c * 4 + i) ^ (lane & 7))) * 16) = make_uint4(ro[4 * i], ro[4 * i + 1], ro[4 * i + 2], ro[4 * i + 3]);
+          }
+        }
+        if (direct && !last_half) continue;
+        __syncwarp();
+        const int chunks = direct ? HD / 8 : PIECE / 4, per = direct ? 8 : 4, from = direct ? 0 : half * PIECE;
+        const int size = direct ? (int)sizeof(T) : 4;
+        uint8_t* base = direct ? (uint8_t*)a.out : (uint8_t*)a.part;
+        for (int i = lane; i < 32 * chunks; i += 32) {
+          const int rr = i / chunks, chunk = i % chunks;
+          const long long to = __shfl_sync(0xffffffffu, row, rr);
+          if (to >= 0 && from + chunk * per < a.D)
+            *reinterpret_cast<uint4*>(base + (to * a.D + from + chunk * per) * size) = *reinterpret_cast<const uint4*>(buf + (rr * chunks + (chunk ^ (rr & 7))) * 16);
+        }
+        __syncwarp();
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::COLS);
+  }
+}
+
+// Joins the partial rows of a query row: those of the prefix and those of its own sequence, each in the order of the keys.  A warp a row, a
+// lane every 32nd column.  First the statistics, a part a lane, so that they are one wait and not one for each part; then the sums with their
+// weights, eight parts on their way at a time.  Rows that the first kernel has written are left alone; rows that see nothing become zeros.
 template <typename T, int ROWS, int TILE>
 __global__ void __launch_bounds__(256) cache_join_kernel(const CacheArgs a) {
   pdl_trigger();
@@ -725,40 +1086,59 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const CacheArgs a) {
   const long long bt = i / a.H;
   const int b = (int)(bt / a.T), t = (int)(bt - (long long)b * a.T);
   T* out = (T*)a.out + i * a.D;
-  float top = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  bool done = false;
-  auto take = [&](long long row) {
-    const float2 s = a.stat[row];
-    const float* p = a.part + row * a.D;
-    const float n = fmaxf(top, s.x);
-    const float f = top == -INFINITY ? 0.f : exp2f(top - n);
-    const float w = s.x == -INFINITY ? (s.y == 0.f ? 0.f : 1.f) : exp2f(s.x - n);     // (scores of NaN leave no maximum, but a sum)
-    top = n;
-    sum = sum * f + s.y * w;
-#pragma unroll
-    for (int c = 0; c < 4; c++)
-      if (c * 32 + lane < a.D) o[c] = o[c] * f + p[c * 32 + lane] * w;
-  };
-  auto gather = [&](int e, int r, long long whole) {
-    if (entry_of<ROWS, TILE>(a, e).tiles == 0) return;
+  // parts: row `first`, then rest + k step, 0 < k < n
+  struct Parts { long long first, rest, step; int n; };
+  Parts pre = {0, 0, 0, 0}, own = {0, 0, 0, 0};
+  const long long whole = 2LL * a.ctas * ROWS;
+  auto find = [&](Parts& p, int e, int r, long long at) {
+    if (entry_of<ROWS, TILE>(a, e).tiles == 0) return true;
     const int2 c = a.owner[e * a.Hkv + h];
-    if (c.x >> 1 == c.y) {                       // one CTA had all of it
-      if (a.prefix_tiles == 0) done = true;
-      else take(2LL * a.ctas * ROWS + whole);
-      return;
+    const int cta = c.x >> 1;
+    if (cta == c.y) {                             // one CTA had all of it
+      p = {at, at, 0, 1};
+      return a.shared != 0;
     }
-    take((long long)c.x * ROWS + r);
-    for (int k = (c.x >> 1) + 1; k <= c.y; k++) take(2LL * k * ROWS + r);
+    // The first part may be that CTA's second one (slot 2 cta + 1); the others are the first ones of theirs.
+    p = {(long long)c.x * ROWS + r, 2LL * cta * ROWS + r, 2 * ROWS, c.y - cta + 1};
+    return true;
   };
+  const int per = a.T * a.G, r = t * a.G + g;
   if (t < count_of(a, b)) {
-    const int r = t * a.G + g;
-    if (a.prefix_tiles) {
-      const int all = b * a.T * a.G + r;
-      gather(all / ROWS, all % ROWS, rows + i);
+    if (a.wide_prefix) {
+      pre = {whole + rows + i, whole + rows + i, rows, a.splits};
+    } else if (a.prefix_tiles) {
+      const int all = b * per + r;
+      find(pre, all / ROWS, all % ROWS, whole + rows + i);
     }
-    gather(a.prefix_tiles + b * a.own_tiles + r / ROWS, r % ROWS, i);
+    if (a.wide_own) own = {i, i, rows, a.splits};
+    else if (!find(own, a.prefix_tiles + b * a.own_tiles + r / ROWS, r % ROWS, whole + i)) return;
   }
-  if (done) return;
+  const int n = pre.n + own.n;
+  float top = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int k0 = 0; k0 < n; k0 += 32) {
+    const int k = k0 + lane;
+    long long row = 0;
+    float2 st = make_float2(-INFINITY, 0.f);
+    if (k < n) {
+      row = k < pre.n ? (k == 0 ? pre.first : pre.rest + k * pre.step) : (k == pre.n ? own.first : own.rest + (k - pre.n) * own.step);
+      st = a.stat[row];
+    }
+    const float next = fmaxf(top, warp_max(st.x)), f = top == -INFINITY ? 0.f : exp2f(top - next);
+    const float w = st.x == -INFINITY ? (st.y == 0.f ? 0.f : 1.f) : exp2f(st.x - next);     // (scores of NaN leave no maximum, but a sum)
+    top = next;
+    sum = sum * f + warp_sum(st.y * w);
+#pragma unroll
+    for (int c = 0; c < 4; c++) o[c] *= f;
+    const int m = min(32, n - k0);
+#pragma unroll 8
+    for (int j = 0; j < m; j++) {
+      const float* p = a.part + __shfl_sync(0xffffffffu, row, j) * a.D;
+      const float wj = __shfl_sync(0xffffffffu, w, j);
+#pragma unroll
+      for (int c = 0; c < 4; c++)
+        if (c * 32 + lane < a.D) o[c] += p[c * 32 + lane] * wj;
+    }
+  }
   const float f = sum != 0.f ? __frcp_rn(sum) : 0.f;
 #pragma unroll
   for (int c = 0; c < 4; c++)
@@ -771,26 +1151,81 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const CacheArgs a) {
 constexpr int kCtas = 2 * 148;
 
 struct Sizes {
-  int rows;                      // of a tile
+  int rows;                      // of a tile of the kernel for few rows
   int own_tiles, prefix_tiles;
-  long long entries, slot_rows, part, stat, owner, total;      // bytes of the workspace's parts
+  int wide_prefix, wide_own, wide_tiles, splits;
+  long long entries, part, stat, owner, total;      // bytes of the workspace's parts
 };
 
-bool plan(Sizes& z, int dtype, long long B, long long T, long long H, long long Hkv, long long D, bool prefix) {
-  const long long own = T * (H / Hkv), all = B * own, most = prefix ? all : own;
+// Which kernel takes what, and the workspace.  box: rows of a TMA box (0: none).
+bool plan(Sizes& z, int dtype, long long B, long long T, long long H, long long Hkv, long long D, int prefix, int box) {
+  const long long own = T * (H / Hkv), all = B * own;
+  z = Sizes{};
+  if (all >= 0x7fffffffLL) return false;
+  // Many rows of a sequence: its keys with the prefix among them, nothing is gained by sharing.  Many rows of the batch alone: its prefix.
+  const bool wide = dtype != 2 && box > 0;
+  z.wide_own = wide && own > 64;
+  const bool shared = prefix > 0 && !z.wide_own;
+  z.wide_prefix = shared && wide && all > 64;
+  if (z.wide_own || z.wide_prefix) {
+    z.wide_tiles = (int)(((z.wide_own ? own : all) + kWideRows - 1) / kWideRows);
+    const long long items = z.wide_tiles * Hkv * (z.wide_own ? B : 1);
+    // Runs of keys, so that the CTAs (two to an SM) come out in whole rounds: of up to 16, the number whose rounds are shortest, the smaller one
+    // where a larger gains less than a twentieth (partial rows have to be written and joined); runs of 256 keys at least in a prefix.
+    z.splits = 1;
+    double best = 0;
+    for (int n = 1; n <= 16; n++) {
+      if (z.wide_prefix && n > 1 && prefix / n < 256) break;
+      const double rounds = (double)((items * n + kCtas - 1) / kCtas) / n;
+      if (n == 1 || rounds < 0.95 * best) {
+        best = rounds;
+        z.splits = n;
+      }
+    }
+  }
+  const long long most = shared && !z.wide_prefix ? all : own;
   z.rows = dtype == 2 || most <= 16 ? 16 : most <= 32 ? 32 : 64;
-  const long long ot = (own + z.rows - 1) / z.rows, pt = prefix ? (all + z.rows - 1) / z.rows : 0;
+  const long long ot = z.wide_own ? 0 : (own + z.rows - 1) / z.rows, pt = shared && !z.wide_prefix ? (all + z.rows - 1) / z.rows : 0;
   z.entries = pt + B * ot;
-  if (z.entries * Hkv >= 0x7fffffffLL || all >= 0x7fffffffLL) return false;
+  if (z.entries * Hkv >= 0x7fffffffLL) return false;
   z.own_tiles = (int)ot;
   z.prefix_tiles = (int)pt;
-  z.slot_rows = 2LL * kCtas * z.rows + (prefix ? 2 * B * T * H : 0);
+  const long long rows = z.wide_own ? (z.splits > 1 ? z.splits * B * T * H : 0)
+                                    : 2LL * kCtas * z.rows + (shared ? B * T * H * (1 + (z.wide_prefix ? z.splits : 1)) : 0);
   auto up = [](long long n) { return (n + 255) / 256 * 256; };
-  z.part = up(z.slot_rows * D * 4);
-  z.stat = up(z.slot_rows * 8);
+  z.part = up(rows * D * 4);
+  z.stat = up(rows * 8);
   z.owner = up(z.entries * Hkv * 8);
-  z.total = z.part + z.stat + z.owner;
+  z.total = z.part + z.stat + z.owner + 256;
   return true;
+}
+
+template <typename K>
+int allow_shared(K kernel, int bytes, std::atomic<uint32_t>& done) {
+  int dev = 0;
+  GB_CUDA_OK(cudaGetDevice(&dev));
+  if (dev < 32 && (done.load() >> dev & 1u)) return gbh::E_OK;
+  GB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (dev < 32) done.fetch_or(1u << dev);
+  return gbh::E_OK;
+}
+
+template <typename T, int HD>
+int launch_wide(const CUtensorMap& tk, const CUtensorMap& tv, const CacheArgs& a, cudaStream_t s) {
+  using C = Wide<HD>;
+  static std::atomic<uint32_t> done{0};
+  const int rc = allow_shared(cache_wide_kernel<T, HD>, C::SMEM, done);
+  if (rc) return rc;
+  const long long ctas = (long long)a.wide_tiles * a.splits * a.Hkv * (a.wide_prefix ? 1 : a.B);
+  GB_CUDA_OK(gbh::launch(cache_wide_kernel<T, HD>, dim3((unsigned)ctas), dim3(kWideThreads), C::SMEM, s, 1, tk, tv, a));
+  return gbh::E_OK;
+}
+
+template <typename T, int ROWS, int TILE>
+int launch_join(const CacheArgs& a, cudaStream_t s) {
+  const long long rows = (long long)a.B * a.T * a.H;
+  GB_CUDA_OK(gbh::launch(cache_join_kernel<T, ROWS, TILE>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, 1, a));
+  return gbh::E_OK;
 }
 
 template <typename T, int HD, int RG, bool TMA>
@@ -798,16 +1233,10 @@ int launch_attn(const CUtensorMap& tk, const CUtensorMap& tv, CacheArgs& a, cuda
   using C = Cfg<T, HD, RG>;
   const auto kernel = cache_attn_kernel<T, HD, RG, TMA>;
   static std::atomic<uint32_t> done{0};
-  int dev = 0;
-  GB_CUDA_OK(cudaGetDevice(&dev));
-  if (dev >= 32 || !(done.load() >> dev & 1u)) {
-    GB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-    if (dev < 32) done.fetch_or(1u << dev);
-  }
+  const int rc = allow_shared(kernel, C::SMEM, done);
+  if (rc) return rc;
   GB_CUDA_OK(gbh::launch(kernel, dim3(a.ctas), dim3(kThreads), C::SMEM, s, 1, tk, tv, a));
-  const long long rows = (long long)a.B * a.T * a.H;
-  GB_CUDA_OK(gbh::launch(cache_join_kernel<T, C::ROWS, C::TILE>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, 1, a));
-  return gbh::E_OK;
+  return launch_join<T, C::ROWS, C::TILE>(a, s);
 }
 
 // (columns, rows of a page, heads, pages) in boxes of 128 bytes by `rows` rows
@@ -842,15 +1271,24 @@ int launch_type(const CUtensorMap& k, const CUtensorMap& v, CacheArgs& a, int ro
 
 template <typename T>
 int launch_any(const CUtensorMap& k, const CUtensorMap& v, CacheArgs& a, int rows, cudaStream_t s) {
+  if constexpr (Elem<T>::kMma) {
+    if (a.wide_own || a.wide_prefix) {
+      const int rc = a.D <= 64 ? launch_wide<T, 64>(k, v, a, s) : launch_wide<T, 128>(k, v, a, s);
+      if (rc) return rc;
+      if (a.wide_own) return a.splits > 1 ? launch_join<T, 64, 64>(a, s) : gbh::E_OK;
+    }
+  }
   return a.box ? launch_type<T, true>(k, v, a, rows, s) : launch_type<T, false>(k, v, a, rows, s);
 }
 
 }  // namespace
 
-// Bytes of the workspace of gb_cache_attn, or a negative error.
-GB_EXPORT long long gb_cache_attn_bytes(int dtype, long long B, long long T, long long H, long long Hkv, long long D, int prefix) {
+// Bytes of the workspace of gb_cache_attn, or a negative error.  strides: as there.
+GB_EXPORT long long gb_cache_attn_bytes(int dtype, long long B, long long T, long long H, long long Hkv, long long D, int page, int prefix,
+                                        const long long* strides) {
   Sizes z;
-  if (B < 0 || T < 1 || H < 1 || Hkv < 1 || H % Hkv || D < 1 || D > 128 || !plan(z, dtype, B, T, H, Hkv, D, prefix > 0)) {
+  if (dtype < 0 || dtype > 2 || B < 0 || T < 1 || H < 1 || Hkv < 1 || H % Hkv || D < 1 || D > 128 || page < 1 || !strides ||
+      !plan(z, dtype, B, T, H, Hkv, D, prefix, box_of(page, dtype == 2 ? 32 : 64, strides + 3, dtype == 2 ? 4 : 2))) {
     gbh::set_error("gb_cache_attn: too many rows, or bad sizes (%lld sequences, %lld tokens, %lld and %lld heads of %lld)", B, T, H, Hkv, D);
     return gbh::E_TOO_LARGE;
   }
@@ -858,7 +1296,7 @@ GB_EXPORT long long gb_cache_attn_bytes(int dtype, long long B, long long T, lon
 }
 
 // out (B, T, H, D) = attention of q over the pages of its sequences.  strides: of q (batch, token, head), of both caches (page, head, row),
-// in elements; rows of q aligned to 4 bytes, those of the caches to 16.  prefix: positions, a multiple of the page, that all sequences have in
+// in elements; rows aligned to 16 bytes.  prefix: positions, a multiple of the page, that all sequences have in
 // the pages of the first one's.  The workspace belongs to this call until its kernels have run.
 GB_EXPORT int gb_cache_attn(int dtype, const void* q, const void* k, const void* v, void* out, const long long* strides, int B, int T, int H,
                             int Hkv, int D, const void* table, long long table_stride, int columns, int pages, int page, const void* lengths,
@@ -879,22 +1317,22 @@ GB_EXPORT int gb_cache_attn(int dtype, const void* q, const void* k, const void*
   }
   long long cache = 0;
   for (int i = 3; i < 9; i++) cache |= strides[i];
-  if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)ws) & 15 || cache * size % 16 || (uintptr_t)q & 3 || (strides[0] | strides[1] | strides[2]) * size % 4 ||
-      (uintptr_t)out & 3) {
+  if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)ws) & 15 || cache * size % 16 || (uintptr_t)q & 15 || (strides[0] | strides[1] | strides[2]) * size % 16 ||
+      (uintptr_t)out & 15) {
     gbh::set_error("gb_cache_attn: misaligned tensor");
     return gbh::E_BAD_ARG;
   }
+  CacheArgs a = {};
+  a.box = box_of(page, dtype == 2 ? 32 : 64, strides + 3, size);
   Sizes z;
-  if (!plan(z, dtype, B, T, H, Hkv, D, prefix > 0) || ws_bytes < z.total) {
+  if (!plan(z, dtype, B, T, H, Hkv, D, prefix, a.box) || ws_bytes < z.total) {
     gbh::set_error("gb_cache_attn: workspace of %lld bytes is too small, or too many rows", ws_bytes);
     return gbh::E_TOO_LARGE;
   }
-  const long long join = ((long long)B * T * H + 7) / 8;
-  if (join >= 0x7fffffffLL) {
+  if (((long long)B * T * H + 7) / 8 >= 0x7fffffffLL || (long long)z.wide_tiles * z.splits * Hkv * B >= 0x7fffffffLL) {
     gbh::set_error("gb_cache_attn: too many rows");
     return gbh::E_TOO_LARGE;
   }
-  CacheArgs a = {};
   a.q = q; a.k = k; a.v = v; a.out = out;
   a.q_sb = strides[0]; a.q_st = strides[1]; a.q_sh = strides[2];
   a.k_sp = strides[3]; a.k_sh = strides[4]; a.k_sr = strides[5];
@@ -906,6 +1344,9 @@ GB_EXPORT int gb_cache_attn(int dtype, const void* q, const void* k, const void*
   a.prefix = prefix;
   a.scale_log2 = (float)(scale * 1.4426950408889634);
   a.own_tiles = z.own_tiles; a.prefix_tiles = z.prefix_tiles;
+  a.shared = prefix > 0 && !z.wide_own;
+  a.wide_prefix = z.wide_prefix; a.wide_own = z.wide_own; a.wide_tiles = z.wide_tiles; a.splits = z.splits;
+  a.slot_rows = z.rows;
   a.ctas = kCtas;
   a.part = (float*)ws;
   a.stat = (float2*)((uint8_t*)ws + z.part);
@@ -915,7 +1356,6 @@ GB_EXPORT int gb_cache_attn(int dtype, const void* q, const void* k, const void*
   CUtensorMap tk, tv;
   memset(&tk, 0, sizeof(tk));
   memset(&tv, 0, sizeof(tv));
-  a.box = box_of(page, dtype == 2 ? 32 : 64, strides + 3, size);
   if (a.box) {
     int rc;
     if ((rc = cache_map(&tk, dtype, k, D, page, Hkv, pages, strides + 3, a.box))) return rc;

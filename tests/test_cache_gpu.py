@@ -310,9 +310,9 @@ def test_bad_tables_are_reported():
         cache.Append(k, k, table, at)
         assert lib.read_status()[0] == 5
         assert torch.equal(cache.Keys, before)
-        if int(table[0, 0]) != 0:
-            cache.Attend(q, table, at)
-            assert lib.read_status()[0] == 5
+        for tokens in (1, 70):                                          # few rows, many
+            cache.Attend(q.expand(2, tokens, 4, 64), table, at)
+            assert lib.read_status()[0] == (0 if int(at[0]) < 0 and tokens == 1 else 5)
     lib.assert_status_ok()
 
 
