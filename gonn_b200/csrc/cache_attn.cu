@@ -71,8 +71,8 @@ template <> struct Elem<__half> {
 template <> struct Elem<float> { static constexpr bool kMma = false; };
 
 // Rows of a tile: 16 RG.  Row groups of 16 rows times key groups of a quarter, a half or all of the keys are the four warps of the
-// 16-bit kernel; in fp32 a warp takes four rows and all keys.
-template <typename T, int HD_, int RG_>
+// 16-bit kernel; in fp32 a warp takes four rows and all keys.  Two CTAs to an SM: while one waits, joins or stores, the other multiplies.
+template <typename T, int HD_, int RG_, bool TMA>
 struct Cfg {
   static constexpr int HD = HD_, RG = RG_;
   static constexpr bool kMma = Elem<T>::kMma;
@@ -80,11 +80,16 @@ struct Cfg {
   static constexpr int TILE = kMma ? 64 : 32;
   static constexpr int KG = kMma ? 4 / RG : 1;
   static constexpr int SUB = TILE * HD * (int)sizeof(T);          // one K or V tile
-  static constexpr int STAGES = HD == 64 ? 6 : 3;
+  static constexpr int STAGES = HD == 64 ? 4 : 2;
+  static constexpr int SEGS = RG == 1 && kMma && TMA ? 3 : 2;           // segments (queries, rows) on their way
+  static constexpr int Q_BYTES = ROWS * HD * (int)sizeof(T);
   static constexpr int CHUNKS = HD * (int)sizeof(T) / 16;         // 16-byte chunks of a row
-  static constexpr int EXTRA = kMma ? (KG > 1 ? KG / 2 * ROWS * (HD * 4 + 8) : 0) : ROWS * HD * 4 + ROWS * TILE * 4;   // joined groups; queries and weights
   static constexpr int COLS = HD * (int)sizeof(T) / 128;          // columns of 128 bytes
-  static constexpr int SMEM = 2 * STAGES * SUB + EXTRA + 256 + 1024 + 2 * TILE * 8;
+  static constexpr int PAD = HD + 8;                              // floats of a row of sums: eight rows' columns in different banks
+  // sums of the key groups that are joined (all four, or the second of two), or the weights of fp32
+  static constexpr int JOIN = kMma ? (RG == 1 ? 4 : RG == 2 ? 1 : 0) * ROWS * (PAD * 4 + 8) : ROWS * TILE * 4;
+  static constexpr int SMEM = 2 * STAGES * SUB + SEGS * Q_BYTES + JOIN + 1024 + SEGS * (ROWS * 12 + 32) + 256 + (TMA ? 0 : 2 * TILE * 8);
+  static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs to an SM");
 };
 
 // ---------------------------------------------------------------------------------------------------------------------------
@@ -115,12 +120,19 @@ __device__ __forceinline__ Entry entry_of(const CacheArgs& a, int e) {
     x.end = a.prefix;
   } else {
     e -= a.prefix_tiles;
-    x.b = a.own_tiles == 1 ? e : e / a.own_tiles;
-    const int rt = e - x.b * a.own_tiles;
-    x.row0 = rt * ROWS;
-    const int c = count_of(a, x.b), last = min(a.T * a.G, x.row0 + ROWS) - 1;
-    const int seen = min(c, last / a.G + 1);                         // tokens of these rows that count, and those before them
-    const long long end = x.row0 / a.G < c ? (long long)a.lengths[x.b] + seen : 0;
+    long long end;
+    if (a.own_tiles == 1) {
+      x.b = e;
+      x.row0 = 0;
+      const int c = count_of(a, e);
+      end = c > 0 ? (long long)a.lengths[e] + c : 0;
+    } else {
+      x.b = e / a.own_tiles;
+      x.row0 = (e - x.b * a.own_tiles) * ROWS;
+      const int c = count_of(a, x.b), last = min(a.T * a.G, x.row0 + ROWS) - 1;
+      const int seen = min(c, last / a.G + 1);                       // tokens of these rows that count, and those before them
+      end = x.row0 / a.G < c ? (long long)a.lengths[x.b] + seen : 0;
+    }
     x.cut = end > a.room;
     x.end = (int)(x.cut ? (long long)a.room : end > 0 ? end : 0);
   }
@@ -128,20 +140,77 @@ __device__ __forceinline__ Entry entry_of(const CacheArgs& a, int e) {
   return x;
 }
 
-// Position in the list.
+// The list cut into equal shares: `per` tiles for every CTA and one more for the first `rem`.
+struct Shares {
+  unsigned per, rem;
+  __device__ __forceinline__ unsigned first(unsigned cta) const { return cta * per + min(cta, rem); }
+  __device__ __forceinline__ unsigned cta_of(unsigned tile) const {
+    const unsigned longer = rem * (per + 1);
+    return tile < longer ? tile / (per + 1) : rem + (tile - longer) / per;
+  }
+};
+
+// A CTA's place in the list, held by the warp that copies.
 template <int ROWS, int TILE>
 struct Cursor {
+  Shares shares;
   Entry x;
   int e, h, entries, tile;
-  // to the entry e (or the first one after it that has tiles), `tile` tiles into it
-  __device__ __forceinline__ void start(const CacheArgs& a, int e_, long long into) {
+  unsigned left, segment0;           // tiles to go; the list's number of the segment's first tile
+
+  // Adds up the tiles of all entries, an entry or a run of them a lane, and finds this CTA's share.  (Totals stay below 2^31.)
+  __device__ __forceinline__ void start(const CacheArgs& a, int lane) {
     entries = a.prefix_tiles + a.B * a.own_tiles;
-    e = e_;
-    x = entry_of<ROWS, TILE>(a, e);
-    h = x.tiles ? (int)(into / x.tiles) : 0;
-    tile = x.tiles ? (int)(into - (long long)h * x.tiles) : 0;
+    const int per = (entries + 31) / 32, lo = min(entries, lane * per), hi = min(entries, lo + per);
+    unsigned mine = 0;
+    Entry first_entry;
+#pragma unroll 4
+    for (int k = lo; k < hi; k++) {
+      const Entry y = entry_of<ROWS, TILE>(a, k);
+      if (k == lo) first_entry = y;
+      mine += y.tiles;
+      if (y.cut && blockIdx.x == 0) set_status(a.status, ST_BAD_INDEX, y.b);
+    }
+    mine *= a.Hkv;
+    unsigned sum = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const unsigned up = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += up;
+    }
+    const unsigned total = __shfl_sync(0xffffffffu, sum, 31), before = sum - mine;
+    const unsigned ctas = min((unsigned)a.ctas, total);              // so that none between two others has nothing
+    left = 0;
+    if (blockIdx.x >= ctas) return;
+    shares.per = total / ctas;
+    shares.rem = total - shares.per * ctas;
+    const unsigned first = shares.first(blockIdx.x);
+    left = shares.per + (blockIdx.x < shares.rem);
+    const unsigned owner = __ffs(__ballot_sync(0xffffffffu, first >= before && first < sum)) - 1;
+    unsigned at = before;
+    if (lane == owner) {
+      x = first_entry;
+      for (e = lo;; ) {
+        const unsigned n = (unsigned)x.tiles * a.Hkv;
+        if (first < at + n) break;
+        at += n;
+        x = entry_of<ROWS, TILE>(a, ++e);
+      }
+      h = (first - at) / x.tiles;
+      at += h * x.tiles;
+    }
+    e = __shfl_sync(0xffffffffu, e, owner);
+    h = __shfl_sync(0xffffffffu, h, owner);
+    segment0 = __shfl_sync(0xffffffffu, at, owner);
+    x.b = __shfl_sync(0xffffffffu, x.b, owner);
+    x.row0 = __shfl_sync(0xffffffffu, x.row0, owner);
+    x.begin = __shfl_sync(0xffffffffu, x.begin, owner);
+    x.end = __shfl_sync(0xffffffffu, x.end, owner);
+    x.tiles = __shfl_sync(0xffffffffu, x.tiles, owner);
+    tile = first - segment0;
   }
   __device__ __forceinline__ void next_segment(const CacheArgs& a) {
+    segment0 += x.tiles;
     tile = 0;
     if (++h < a.Hkv) return;
     h = 0;
@@ -151,58 +220,6 @@ struct Cursor {
     } while (x.tiles == 0);
   }
 };
-
-struct Share {
-  long long first, count, total;     // of this CTA's tiles, of all
-  int ctas;                          // that have any
-  int e;                             // the entry of the first one
-  long long into;                    // tiles of that entry before it
-};
-
-// Adds up the tiles of all entries and finds this CTA's share.  By the threads of a CTA, through shared memory.
-template <int ROWS, int TILE>
-__device__ __forceinline__ Share share_of(const CacheArgs& a, long long* s_sum, Share* s_share) {
-  const int entries = a.prefix_tiles + a.B * a.own_tiles, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int per = (entries + kThreads - 1) / kThreads, lo = min(entries, tid * per), hi = min(entries, lo + per);
-  long long mine = 0;
-  for (int e = lo; e < hi; e++) {
-    const Entry x = entry_of<ROWS, TILE>(a, e);
-    mine += x.tiles;
-    if (x.cut && blockIdx.x == 0) set_status(a.status, ST_BAD_INDEX, x.b);
-  }
-  mine *= a.Hkv;
-  long long sum = mine;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const long long up = __shfl_up_sync(0xffffffffu, sum, d);
-    if (lane >= d) sum += up;
-  }
-  if (lane == 31) s_sum[warp] = sum;
-  __syncthreads();
-  long long before = 0, total = 0;
-  for (int w = 0; w < kThreads / 32; w++) {
-    if (w < warp) before += s_sum[w];
-    total += s_sum[w];
-  }
-  before += sum - mine;
-  const int ctas = (int)min((long long)a.ctas, total);               // so that none between two others has nothing
-  const long long first = blockIdx.x < ctas ? total * blockIdx.x / ctas : 0, end = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : 0;
-  if (end > first && first >= before && first < before + mine) {
-    int e = lo;
-    long long at = before;
-    for (;; e++) {
-      const long long n = (long long)entry_of<ROWS, TILE>(a, e).tiles * a.Hkv;
-      if (first < at + n) break;
-      at += n;
-    }
-    *s_share = {first, end - first, total, ctas, e, first - at};
-  }
-  if (tid == 0 && end == first) *s_share = {first, 0, total, ctas, 0, 0};
-  __syncthreads();
-  return *s_share;
-}
-
-__device__ __forceinline__ int cta_of(long long tile, long long total, int ctas) { return (int)(((tile + 1) * ctas - 1) / total); }
 
 // ---------------------------------------------------------------------------------------------------------------------------
 // matrix instructions
@@ -259,8 +276,6 @@ __device__ __forceinline__ void clear_rows(uint8_t* tile, int from, int to, int 
   __syncwarp();
 }
 
-__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
-
 // A row of a tile: its query, its output row and how many keys it sees.
 struct Row {
   int b, t, g;
@@ -288,22 +303,34 @@ __device__ __forceinline__ Row row_of(const CacheArgs& a, const Entry& x, int r)
   return w;
 }
 
+// What the copying warp hands to the others with a segment (the tiles of one entry and key head that fall to this CTA).
+struct Segment {
+  int tiles, key0, end;      // 0 tiles: no more segments; the first tile's first key; the entry's end of keys
+  int rows;                  // rows that there are
+  int direct;                // rows go to the output, else to partial rows
+};
+
 template <typename T, int HD, int RG, bool TMA>
 __global__ void __launch_bounds__(kThreads, 2)
 cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const CacheArgs a) {
-  using C = Cfg<T, HD, RG>;
-  constexpr int ROWS = C::ROWS, TILE = C::TILE, STAGES = C::STAGES, SUB = C::SUB;
+  using C = Cfg<T, HD, RG, TMA>;
+  constexpr int ROWS = C::ROWS, TILE = C::TILE, STAGES = C::STAGES, SUB = C::SUB, SEGS = C::SEGS, KG = C::KG;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* s_k = smem;
-  uint8_t* s_v = smem + STAGES * SUB;
-  uint8_t* s_extra = s_v + STAGES * SUB;
-  uint64_t* full = (uint64_t*)(s_extra + C::EXTRA);
+  uint8_t* s_v = s_k + STAGES * SUB;
+  uint8_t* s_q = s_v + STAGES * SUB;
+  float* s_join = reinterpret_cast<float*>(s_q + SEGS * C::Q_BYTES);
+  long long* s_dst = reinterpret_cast<long long*>((uint8_t*)s_join + C::JOIN);       // [SEGS][ROWS] where a row goes
+  long long* s_off = s_dst + SEGS * ROWS;                                            // where the keys and values of a tile start (cp.async)
+  int* s_sees = reinterpret_cast<int*>(s_off + (TMA ? 0 : 2 * TILE));                          // [SEGS][ROWS] keys that a row sees, 0: it does not count
+  Segment* s_seg = reinterpret_cast<Segment*>(s_sees + SEGS * ROWS);
+  uint64_t* full = reinterpret_cast<uint64_t*>(((uintptr_t)(s_seg + SEGS) + 7) & ~(uintptr_t)7);
   uint64_t* empty = full + STAGES;
-  long long* s_sum = (long long*)(empty + STAGES);
-  Share* s_share = (Share*)(s_sum + kThreads / 32);
-  volatile int* abort_flag = (volatile int*)(s_share + 1);
-  long long* s_off = (long long*)(s_extra + C::EXTRA + 256);        // where the keys and values of a tile start
+  uint64_t* seg_full = empty + STAGES;
+  uint64_t* seg_empty = seg_full + SEGS;
+  uint64_t* joined = seg_empty + SEGS;                                               // sums written, sums read
+  volatile int* abort_flag = (volatile int*)(joined + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -311,155 +338,171 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       mbar_init(&full[i], TMA ? 1 : 32);
       mbar_init(&empty[i], kConsumers);
     }
+    for (int i = 0; i < SEGS; i++) {
+      mbar_init(&seg_full[i], 33);               // every lane's copies, and the first one's arrival behind all other stores
+      mbar_init(&seg_empty[i], kConsumers);
+    }
+    mbar_init(&joined[0], kConsumers);
+    mbar_init(&joined[1], kConsumers);
     *abort_flag = 0;
     mbar_fence_init();
   }
+  __syncthreads();
   pdl_wait();
-  const Share share = share_of<ROWS, TILE>(a, s_sum, s_share);      // (ends with a barrier of the CTA)
   pdl_trigger();
-  if (share.count == 0) return;
-  Cursor<ROWS, TILE> at;
-  at.start(a, share.e, share.into);
 
   if (warp == kConsumers) {
     // ---------------- copies ----------------
-    if constexpr (TMA) {
-      // lane i: column i % COLS of box i / COLS of keys and of values
-      const int box = lane / C::COLS, col = lane % C::COLS * (128 / (int)sizeof(T));
-      const bool mine = box * a.box < TILE;                          // (columns behind the head's last one: zeros)
-      int page = 0, in_page = 0;
-      auto look_up = [&]() {
-        if (!mine) return;
-        const int key = at.x.begin + at.tile * TILE + box * a.box;
-        page = a.pages;                                              // behind the last one: zeros
-        in_page = 0;
-        if (key < at.x.end) {
-          const unsigned p = (unsigned)key / (unsigned)a.page;
-          in_page = (int)((unsigned)key - p * (unsigned)a.page);
-          page = a.table[(at.x.b < 0 ? 0 : at.x.b) * a.table_stride + p];
-          if (page < 0 || page >= a.pages) {
-            set_status(a.status, ST_BAD_INDEX, at.x.b);
-            page = a.pages;
-          }
-        }
-      };
-      look_up();
-      int st = 0;
-      uint32_t ph = 0;
-      for (long long n = 0; n < share.count; n++) {
-        const int h = at.h, pg = page, row = in_page;
-        if (++at.tile == at.x.tiles) at.next_segment(a);
-        if (n + 1 < share.count) look_up();                          // on its way while this stage is waited for
-        if (!mbar_wait(&empty[st], ph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 20)) break;
-        if (lane == 0) mbar_expect_tx(&full[st], 2 * SUB);
-        __syncwarp();
-        if (mine) {
-          const int to = st * SUB + lane % C::COLS * (TILE * 128) + box * a.box * 128;
-          tma_load_4d(s_k + to, &tm_k, &full[st], col, row, h, pg);
-          tma_load_4d(s_v + to, &tm_v, &full[st], col, row, h, pg);
-        }
-        if (++st == STAGES) { st = 0; ph ^= 1; }
-      }
-      return;
-    }
-    constexpr int LOOK = TILE / 32;                                  // keys that a lane looks up
+    Cursor<ROWS, TILE> at;
+    at.start(a, lane);
+    // lane i: column i % COLS of box i / COLS of keys and of values
+    const int box = lane / C::COLS, col = lane % C::COLS * (128 / (int)sizeof(T));
+    const bool mine = box * a.box < TILE;                            // (columns behind the head's last one: zeros)
+    constexpr int LOOK = TILE / 32;                                  // keys that a lane looks up for cp.async
     constexpr int PER = 32 / C::CHUNKS;                              // rows of one instruction of the warp
     const int sub = lane / C::CHUNKS, chunk = lane % C::CHUNKS;
     const bool inside = chunk * 16 < a.D * (int)sizeof(T);
+    // Pages of the next tile, asked for while this one is copied and looked at when its turn comes.  -1: behind the last key.
     int page[LOOK], in_page[LOOK];
     auto look_up = [&]() {
       const int* row = a.table + (at.x.b < 0 ? 0 : at.x.b) * a.table_stride;
 #pragma unroll
-      for (int i = 0; i < LOOK; i++) {
-        const int key = at.x.begin + at.tile * TILE + i * 32 + lane;
+      for (int i = 0; i < (TMA ? 1 : LOOK); i++) {
+        const int key = at.x.begin + at.tile * TILE + (TMA ? box * a.box : i * 32 + lane);
         page[i] = -1;
         in_page[i] = 0;
-        if (key < at.x.end) {
+        if ((!TMA || mine) && key < at.x.end) {
           const unsigned p = (unsigned)key / (unsigned)a.page;
           in_page[i] = (int)((unsigned)key - p * (unsigned)a.page);
-          page[i] = row[p];
-          if (page[i] < 0 || page[i] >= a.pages) {
-            set_status(a.status, ST_BAD_INDEX, at.x.b);
-            page[i] = -1;
-          }
+          const int got = row[p];
+          page[i] = got == -1 ? -2 : got;
         }
       }
     };
-    look_up();
-    int st = 0;
-    uint32_t ph = 0;
-    for (long long n = 0; n < share.count; n++) {
+    auto checked = [&](int i) {
+      if (page[i] < -1 || page[i] >= a.pages) {
+        set_status(a.status, ST_BAD_INDEX, at.x.b);
+        page[i] = -1;
+      }
+    };
+    int st = 0, sg = 0;
+    uint32_t ph = 0, sph = 0;
+    bool first_segment = true;
+    const int per = a.T * a.G;
+    while (true) {
+      // the segment: its description, where its rows go, its queries
+      if (at.left) look_up();
+      if (!mbar_wait(&seg_empty[sg], sph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 23)) break;
+      const int n = (int)min(at.left, (unsigned)(at.x.tiles - at.tile));
+      if (at.left) {
+        const bool whole = n == at.x.tiles, direct = whole && !a.shared;
+        const int slot = 2 * blockIdx.x + (first_segment ? 0 : 1);
+        const int rows = min(ROWS, (at.x.b < 0 ? a.B * per : per) - at.x.row0);
+        if (lane == 0) {
+          s_seg[sg] = Segment{n, at.x.begin + at.tile * TILE, at.x.end, rows, direct};
+          if (at.tile == 0) a.owner[at.e * a.Hkv + at.h] = make_int2(slot, (int)at.shares.cta_of(at.segment0 + at.x.tiles - 1));
+        }
+        // Whole segments of a batch with a shared prefix leave partial rows too: in the output's order, those of the prefix behind the sequences'.
 #pragma unroll
-      for (int i = 0; i < LOOK; i++) {
-        s_off[i * 32 + lane] = page[i] < 0 ? -1 : page[i] * a.k_sp + at.h * a.k_sh + in_page[i] * a.k_sr;
-        s_off[TILE + i * 32 + lane] = page[i] < 0 ? -1 : page[i] * a.v_sp + at.h * a.v_sh + in_page[i] * a.v_sr;
+        for (int r = lane; r < ROWS; r += 32) {
+          const Row w = row_of(a, at.x, r);
+          const long long row = ((long long)w.b * a.T + w.t) * a.H + at.h * a.G + w.g;
+          s_sees[sg * ROWS + r] = w.counts ? max(w.sees, 0) : 0;
+          s_dst[sg * ROWS + r] = direct ? row : !whole ? (long long)slot * ROWS + r
+                                              : 2LL * a.ctas * ROWS + (at.x.b < 0 ? (long long)a.B * a.T * a.H : 0) + row;
+        }
+        uint8_t* dq = s_q + sg * C::Q_BYTES;
+        for (int r0 = 0; r0 < rows; r0 += PER) {                     // (rows behind the last one: anything, nothing comes of them)
+          const int r = r0 + sub;
+          const Row w = row_of(a, at.x, r);
+          const int bytes = w.counts && inside ? 16 : 0;
+          const T* from = (const T*)a.q + w.b * a.q_sb + w.t * a.q_st + (long long)(at.h * a.G + w.g) * a.q_sh;
+          cp_async16(dq + chunk_at<ROWS>(r, chunk), bytes ? from + chunk * (16 / (int)sizeof(T)) : (const T*)a.q, bytes);
+        }
+      } else if (lane == 0) {
+        s_seg[sg] = Segment{0, 0, 0, 0, 0};
       }
       __syncwarp();
-      if (++at.tile == at.x.tiles) at.next_segment(a);
-      if (n + 1 < share.count) look_up();
-      if (!mbar_wait(&empty[st], ph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 20)) break;
-      uint8_t* dk = s_k + st * SUB;
-      uint8_t* dv = s_v + st * SUB;
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&seg_full[sg])) : "memory");
+      if (lane == 0) mbar_arrive(&seg_full[sg]);
+      if (++sg == SEGS) { sg = 0; sph ^= 1; }
+      if (at.left == 0) break;
+      first_segment = false;
+      at.left -= n;
+      bool ok = true;
+      for (int i = 0; i < n && ok; i++) {
+        if constexpr (TMA) {
+          checked(0);
+          const int pg = page[0] < 0 ? a.pages : page[0], row = in_page[0];        // behind the last page: zeros
+          at.tile++;
+          if (i + 1 < n) look_up();
+          ok = mbar_wait(&empty[st], ph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 20);
+          if (!ok) break;
+          if (lane == 0) mbar_expect_tx(&full[st], 2 * SUB);
+          __syncwarp();
+          if (mine) {
+            const int to = st * SUB + lane % C::COLS * (TILE * 128) + box * a.box * 128;
+            tma_load_4d(s_k + to, &tm_k, &full[st], col, row, at.h, pg);
+            tma_load_4d(s_v + to, &tm_v, &full[st], col, row, at.h, pg);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < LOOK; k++) {
+            checked(k);
+            s_off[k * 32 + lane] = page[k] < 0 ? -1 : page[k] * a.k_sp + at.h * a.k_sh + in_page[k] * a.k_sr;
+            s_off[TILE + k * 32 + lane] = page[k] < 0 ? -1 : page[k] * a.v_sp + at.h * a.v_sh + in_page[k] * a.v_sr;
+          }
+          __syncwarp();
+          at.tile++;
+          if (i + 1 < n) look_up();
+          ok = mbar_wait(&empty[st], ph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 20);
+          if (!ok) break;
+          uint8_t* dk = s_k + st * SUB;
+          uint8_t* dv = s_v + st * SUB;
 #pragma unroll 8
-      for (int r = 0; r < TILE; r += PER) {
-        const long long ko = s_off[r + sub], vo = s_off[TILE + r + sub];
-        const int bytes = ko >= 0 && inside ? 16 : 0;
-        const uint32_t to = chunk_at<TILE>(r + sub, chunk);
-        cp_async16(dk + to, (const T*)a.k + (bytes ? ko + chunk * (16 / (int)sizeof(T)) : 0), bytes);
-        cp_async16(dv + to, (const T*)a.v + (bytes ? vo + chunk * (16 / (int)sizeof(T)) : 0), bytes);
+          for (int r = 0; r < TILE; r += PER) {
+            const long long ko = s_off[r + sub], vo = s_off[TILE + r + sub];
+            const int bytes = ko >= 0 && inside ? 16 : 0;
+            const uint32_t to = chunk_at<TILE>(r + sub, chunk);
+            cp_async16(dk + to, (const T*)a.k + (bytes ? ko + chunk * (16 / (int)sizeof(T)) : 0), bytes);
+            cp_async16(dv + to, (const T*)a.v + (bytes ? vo + chunk * (16 / (int)sizeof(T)) : 0), bytes);
+          }
+          __syncwarp();
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[st])) : "memory");
+        }
+        if (++st == STAGES) { st = 0; ph ^= 1; }
       }
-      __syncwarp();
-      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[st])) : "memory");
-      if (++st == STAGES) { st = 0; ph ^= 1; }
+      if (!ok) break;
+      if (at.left) at.next_segment(a);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     return;
   }
 
   // ---------------- products ----------------
-  int st = 0;
-  uint32_t ph = 0;
-  long long left = share.count, tile_no = share.first;
-  bool first_segment = true, dead = false;       // dead: a wait has given up; the barriers among the warps are kept all the same
-  while (left > 0) {
-    const int n = (int)min(left, (long long)(at.x.tiles - at.tile));
-    const long long segment0 = tile_no - at.tile;                    // the list's number of this segment's first tile
-    const bool whole = n == at.x.tiles;
-    const int seg = at.e * a.Hkv + at.h;
-    // Where its rows go: straight to the output, to the partial rows of a whole segment (in the output's order, those of the prefix
-    // behind the sequences'), or to this CTA's first or last ones.
-    const int slot = 2 * blockIdx.x + (first_segment ? 0 : 1);
-    if (at.tile == 0 && threadIdx.x == 0) a.owner[seg] = make_int2(slot, cta_of(segment0 + at.x.tiles - 1, share.total, share.ctas));
-    const bool direct = whole && !a.shared;
-    auto part_row = [&](const Row& w, int r) -> long long {
-      if (!whole) return (long long)slot * ROWS + r;
-      const long long bt = (long long)w.b * a.T + w.t;
-      return 2LL * a.ctas * ROWS + ((at.x.b < 0 ? (long long)a.B * a.T : 0) + bt) * a.H + at.h * a.G + w.g;
-    };
+  int st = 0, sg = 0;
+  uint32_t ph = 0, sph = 0, jph = 0;
+  const int rg = warp / KG, kg = warp % KG;      // (fp32: rows 4 warp .. 4 warp + 3)
+  for (;;) {
+    if (!mbar_wait(&seg_full[sg], sph, abort_flag, a.status, ST_ATTN_TIMEOUT, 24)) return;
+    const Segment seg = s_seg[sg];
+    if (seg.tiles == 0) return;
+    const int* sees_of = s_sees + sg * ROWS;
+    const long long* dst_of = s_dst + sg * ROWS;
 
     if constexpr (C::kMma) {
-      const int rg = warp / C::KG, kg = warp % C::KG;
-      constexpr int NK = TILE / C::KG;                               // keys of this warp
+      constexpr int NK = TILE / KG;                                  // keys of this warp
       const int r0 = rg * 16 + (lane >> 2), r1 = r0 + 8;
+      // rows of nothing are masked nowhere: what they add up to is not used
+      int sees0 = sees_of[r0], sees1 = sees_of[r1];
+      const bool idle = !__any_sync(0xffffffffu, sees0 | sees1);
+      sees0 = sees0 ? sees0 : 0x7fffffff;
+      sees1 = sees1 ? sees1 : 0x7fffffff;
       uint32_t qf[HD / 16][4];
-      int sees0, sees1;
-      bool idle;
       {
-        const Row w0 = row_of(a, at.x, r0), w1 = row_of(a, at.x, r1);
-        idle = !__any_sync(0xffffffffu, w0.counts || w1.counts);
-        // rows of nothing are masked nowhere: what they add up to is not used
-        sees0 = w0.counts ? w0.sees : 0x7fffffff;
-        sees1 = w1.counts ? w1.sees : 0x7fffffff;
-        const T* q0 = (const T*)a.q + w0.b * a.q_sb + w0.t * a.q_st + (long long)(at.h * a.G + w0.g) * a.q_sh;
-        const T* q1 = (const T*)a.q + w1.b * a.q_sb + w1.t * a.q_st + (long long)(at.h * a.G + w1.g) * a.q_sh;
+        const uint32_t qa = smem_u32(s_q + sg * C::Q_BYTES);
 #pragma unroll
-        for (int s = 0; s < HD / 16; s++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const int col = s * 16 + (i >> 1) * 8 + (lane & 3) * 2;
-            const bool ok = col < a.D && ((i & 1) ? w1.counts : w0.counts);
-            qf[s][i] = ok ? *reinterpret_cast<const uint32_t*>(((i & 1) ? q1 : q0) + col) : 0u;
-          }
+        for (int x = 0; x < HD / 16; x++) ldm4(qf[x], qa + chunk_at<ROWS>(rg * 16 + (lane & 15), x * 2 + (lane >> 4)));
       }
       float o[HD / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 #pragma unroll
@@ -467,12 +510,11 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 #pragma unroll
         for (int i = 0; i < 4; i++) o[j][i] = 0.f;
 
-      for (int i = 0; i < n; i++) {
-        dead = dead || !mbar_wait(&full[st], ph, abort_flag, a.status, ST_ATTN_TIMEOUT, 21);
-        if (dead) break;
-        if (!idle) {
+      for (int i = 0; i < seg.tiles; i++) {
+        if (!mbar_wait(&full[st], ph, abort_flag, a.status, ST_ATTN_TIMEOUT, 21)) return;
+        const int key0 = seg.key0 + i * TILE + kg * NK;
+        if (!idle && key0 < seg.end) {
           const uint32_t ka = smem_u32(s_k + st * SUB), va = smem_u32(s_v + st * SUB);
-          const int key0 = at.x.begin + (at.tile + i) * TILE + kg * NK;
           float s[NK / 8][4];
 #pragma unroll
           for (int j = 0; j < NK / 8; j++)
@@ -489,17 +531,17 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
               mma16<T>(s[2 * j + 1], qf[x], b[2], b[3]);
             }
           }
-          const int low = min(min(sees0, sees1), at.x.end);          // (zeros stand in for keys behind the last one)
+          const int low = min(min(sees0, sees1), seg.end);           // (zeros stand in for keys behind the last one)
           if (__any_sync(0xffffffffu, low - key0 < NK)) {
 #pragma unroll
             for (int j = 0; j < NK / 8; j++)
 #pragma unroll
               for (int c = 0; c < 4; c++) {
                 const int key = key0 + j * 8 + (lane & 3) * 2 + (c & 1);
-                if (key >= min((c & 2) ? sees1 : sees0, at.x.end)) s[j][c] = -INFINITY;
+                if (key >= min((c & 2) ? sees1 : sees0, seg.end)) s[j][c] = -INFINITY;
               }
           }
-          if (TMA && at.x.end - key0 < NK) clear_rows<TILE, C::CHUNKS>(s_v + st * SUB, kg * NK + max(at.x.end - key0, 0), kg * NK + NK, lane);
+          if (TMA && seg.end - key0 < NK) clear_rows<TILE, C::CHUNKS>(s_v + st * SUB, kg * NK + seg.end - key0, kg * NK + NK, lane);
           float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
           for (int j = 0; j < NK / 8; j++) {
@@ -511,9 +553,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
             x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
             x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
           }
-          x0 *= a.scale_log2;
-          x1 *= a.scale_log2;
-          const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+          const float n0 = fmaxf(m0, x0 * a.scale_log2), n1 = fmaxf(m1, x1 * a.scale_log2);
           if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
             const float f0 = m0 == -INFINITY ? 0.f : exp2f(m0 - n0), f1 = m1 == -INFINITY ? 0.f : exp2f(m1 - n1);
             m0 = n0;
@@ -561,70 +601,98 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         l0 += __shfl_xor_sync(0xffffffffu, l0, d);
         l1 += __shfl_xor_sync(0xffffffffu, l1, d);
       }
-      // key groups joined by twos
-      if constexpr (C::KG > 1) {
-        float* buf = reinterpret_cast<float*>(s_extra);
-        float2* stats = reinterpret_cast<float2*>(buf + C::KG / 2 * ROWS * HD);
+      // The key groups' sums meet in shared memory: one of two hands them to the other, four to all of them, a quarter of the columns each.
+      if constexpr (KG > 1) {
+        float2* s_stat = reinterpret_cast<float2*>(s_join + (RG == 1 ? 4 : 1) * ROWS * C::PAD);
+        const int mine = RG == 1 ? kg * ROWS : 0;
+        if (!mbar_wait(&joined[1], jph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 25)) return;      // (the last segment's have been read)
+        if (RG == 1 || kg == 1) {
 #pragma unroll
-        for (int half = C::KG / 2; half >= 1; half >>= 1) {
-          consumers_sync();                                          // the buffer's last use is over
-          if (kg >= half && kg < 2 * half) {
-            float* p0 = buf + ((kg - half) * ROWS + r0) * HD + (lane & 3) * 2;
+          for (int half = 0; half < 2; half++) {
+            const int r = half ? r1 : r0;
+            if (r < seg.rows) {
+              float* to = s_join + (mine + r) * C::PAD + (lane & 3) * 2;
 #pragma unroll
-            for (int j = 0; j < HD / 8; j++) {
-              *reinterpret_cast<float2*>(p0 + j * 8) = make_float2(o[j][0], o[j][1]);
-              *reinterpret_cast<float2*>(p0 + 8 * HD + j * 8) = make_float2(o[j][2], o[j][3]);
-            }
-            if ((lane & 3) == 0) {
-              stats[(kg - half) * ROWS + r0] = make_float2(m0, l0);
-              stats[(kg - half) * ROWS + r1] = make_float2(m1, l1);
-            }
-          }
-          consumers_sync();
-          if (kg < half) {
-            const float2 y0 = stats[kg * ROWS + r0], y1 = stats[kg * ROWS + r1];
-            const float n0 = fmaxf(m0, y0.x), n1 = fmaxf(m1, y1.x);
-            const float f0 = m0 == -INFINITY ? 0.f : exp2f(m0 - n0), f1 = m1 == -INFINITY ? 0.f : exp2f(m1 - n1);
-            const float g0 = y0.x == -INFINITY ? 0.f : exp2f(y0.x - n0), g1 = y1.x == -INFINITY ? 0.f : exp2f(y1.x - n1);
-            m0 = n0;
-            m1 = n1;
-            l0 = l0 * f0 + y0.y * g0;
-            l1 = l1 * f1 + y1.y * g1;
-            const float* p0 = buf + (kg * ROWS + r0) * HD + (lane & 3) * 2;
-#pragma unroll
-            for (int j = 0; j < HD / 8; j++) {
-              const float2 u = *reinterpret_cast<const float2*>(p0 + j * 8), w = *reinterpret_cast<const float2*>(p0 + 8 * HD + j * 8);
-              o[j][0] = o[j][0] * f0 + u.x * g0;
-              o[j][1] = o[j][1] * f0 + u.y * g0;
-              o[j][2] = o[j][2] * f1 + w.x * g1;
-              o[j][3] = o[j][3] * f1 + w.y * g1;
+              for (int j = 0; j < HD / 8; j++) *reinterpret_cast<float2*>(to + j * 8) = make_float2(o[j][2 * half], o[j][2 * half + 1]);
+              if ((lane & 3) == 0) s_stat[mine + r] = half ? make_float2(m1, l1) : make_float2(m0, l0);
             }
           }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&joined[0]);
+        if (!mbar_wait(&joined[0], jph, abort_flag, a.status, ST_ATTN_TIMEOUT, 26)) return;
+        jph ^= 1;
+        if constexpr (RG == 1) {
+          constexpr int CPW = HD / 4, STEP = 32 / CPW;               // columns of a warp, rows at a time
+          const int col = warp * CPW + lane % CPW;
+#pragma unroll 2
+          for (int r = lane / CPW; r < seg.rows; r += STEP) {
+            float2 y[4];
+            float top = -INFINITY, l = 0.f, sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              y[k] = s_stat[k * ROWS + r];
+              top = fmaxf(top, y[k].x);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              const float w = y[k].x == -INFINITY ? (y[k].y == 0.f ? 0.f : 1.f) : exp2f(y[k].x - top);   // (scores of NaN leave no maximum, but a sum)
+              l += y[k].y * w;
+              sum += s_join[(k * ROWS + r) * C::PAD + col] * w;
+            }
+            const long long row = dst_of[r];
+            if (col < a.D) {
+              if (seg.direct) ((T*)a.out)[row * a.D + col] = (T)(sees_of[r] && l != 0.f ? sum * __frcp_rn(l) : 0.f);
+              else a.part[row * a.D + col] = sum;
+            }
+            if (!seg.direct && col == 0) a.stat[row] = make_float2(top, l);
+          }
+        } else if (kg == 0) {
+#pragma unroll
+          for (int half = 0; half < 2; half++) {
+            const int r = half ? r1 : r0;
+            float& m = half ? m1 : m0;
+            float& l = half ? l1 : l0;
+            if (r < seg.rows) {
+              const float2 y = s_stat[r];
+              const float top = fmaxf(m, y.x);
+              const float f = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2f(m - top), w = y.x == -INFINITY ? (y.y == 0.f ? 0.f : 1.f) : exp2f(y.x - top);
+              m = top;
+              l = l * f + y.y * w;
+              const float* from = s_join + r * C::PAD + (lane & 3) * 2;
+#pragma unroll
+              for (int j = 0; j < HD / 8; j++) {
+                const float2 v = *reinterpret_cast<const float2*>(from + j * 8);
+                o[j][2 * half] = o[j][2 * half] * f + v.x * w;
+                o[j][2 * half + 1] = o[j][2 * half + 1] * f + v.y * w;
+              }
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&joined[1]);
       }
-      if (kg == 0) {
+      if (RG > 1 && kg == 0) {
 #pragma unroll
         for (int half = 0; half < 2; half++) {
-          const Row w = row_of(a, at.x, half ? r1 : r0);
           const float m = half ? m1 : m0, l = half ? l1 : l0;
           const int r = half ? r1 : r0;
-          if (direct) {
-            if (w.there) {
-              const float f = w.counts && l != 0.f ? __frcp_rn(l) : 0.f;
-              T* to = (T*)a.out + (((long long)w.b * a.T + w.t) * a.H + at.h * a.G + w.g) * a.D + (lane & 3) * 2;
+          if (r < seg.rows) {
+            const long long row = dst_of[r];
+            if (seg.direct) {
+              const float f = sees_of[r] && l != 0.f ? __frcp_rn(l) : 0.f;
+              T* to = (T*)a.out + row * a.D + (lane & 3) * 2;
 #pragma unroll
               for (int j = 0; j < HD / 8; j++)
                 if (j * 8 < a.D)
-                  *reinterpret_cast<uint32_t*>(to + j * 8) =
-                      f == 0.f ? 0u : Elem<T>::pack(o[j][2 * half] * f, o[j][2 * half + 1] * f);
-            }
-          } else if (w.there) {
-            const long long row = part_row(w, r);
-            float* to = a.part + row * a.D + (lane & 3) * 2;
+                  *reinterpret_cast<uint32_t*>(to + j * 8) = f == 0.f ? 0u : Elem<T>::pack(o[j][2 * half] * f, o[j][2 * half + 1] * f);
+            } else {
+              float* to = a.part + row * a.D + (lane & 3) * 2;
 #pragma unroll
-            for (int j = 0; j < HD / 8; j++)
-              if (j * 8 < a.D) *reinterpret_cast<float2*>(to + j * 8) = make_float2(o[j][2 * half], o[j][2 * half + 1]);
-            if ((lane & 3) == 0) a.stat[row] = make_float2(m, l);
+              for (int j = 0; j < HD / 8; j++)
+                if (j * 8 < a.D) *reinterpret_cast<float2*>(to + j * 8) = make_float2(o[j][2 * half], o[j][2 * half + 1]);
+              if ((lane & 3) == 0) a.stat[row] = make_float2(m, l);
+            }
           }
         }
       }
@@ -632,21 +700,16 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       // fp32: a warp's four rows over all keys of a tile.  Scores: a lane is a key; products with the values: a lane is HD / 32 columns.
       static_assert(RG == 1, "16 rows");
       constexpr int CPL = HD / 32;
-      float* s_q = reinterpret_cast<float*>(s_extra);                // [ROWS][HD]
-      float* s_p = s_q + ROWS * HD + warp * (4 * TILE);              // [TILE][4] of this warp
-      Row w[4];
+      const uint8_t* q = s_q + sg * C::Q_BYTES;
+      float* s_p = s_join + warp * (4 * TILE);                       // [TILE][4] of this warp
       int sees[4];
       bool any = false;
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        w[r] = row_of(a, at.x, warp * 4 + r);
-        any |= w[r].counts;
-        sees[r] = w[r].counts ? w[r].sees : 0x7fffffff;
-        const float* q = (const float*)a.q + w[r].b * a.q_sb + w[r].t * a.q_st + (long long)(at.h * a.G + w[r].g) * a.q_sh;
-#pragma unroll
-        for (int c = lane; c < HD; c += 32) s_q[(warp * 4 + r) * HD + c] = w[r].counts && c < a.D ? q[c] : 0.f;
+        sees[r] = sees_of[warp * 4 + r];
+        any |= sees[r] > 0;
+        sees[r] = sees[r] ? sees[r] : 0x7fffffff;
       }
-      __syncwarp();
       float o[4][CPL], m[4], l[4];
 #pragma unroll
       for (int r = 0; r < 4; r++) {
@@ -655,32 +718,31 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 #pragma unroll
         for (int c = 0; c < CPL; c++) o[r][c] = 0.f;
       }
-      for (int i = 0; i < n; i++) {
-        dead = dead || !mbar_wait(&full[st], ph, abort_flag, a.status, ST_ATTN_TIMEOUT, 22);
-        if (dead) break;
+      for (int i = 0; i < seg.tiles; i++) {
+        if (!mbar_wait(&full[st], ph, abort_flag, a.status, ST_ATTN_TIMEOUT, 22)) return;
         if (any) {
           const uint8_t* kt = s_k + st * SUB;
           const uint8_t* vt = s_v + st * SUB;
-          const int key = at.x.begin + (at.tile + i) * TILE + lane;
+          const int key0 = seg.key0 + i * TILE, key = key0 + lane;
           float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
           for (int c = 0; c < HD / 4; c++) {
             const float4 kk = *reinterpret_cast<const float4*>(kt + chunk_at<TILE>(lane, c));
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-              const float4 qq = *reinterpret_cast<const float4*>(s_q + (warp * 4 + r) * HD + c * 4);
+              const float4 qq = *reinterpret_cast<const float4*>(q + chunk_at<ROWS>(warp * 4 + r, c));
               s[r] = fmaf(qq.x, kk.x, s[r]);
               s[r] = fmaf(qq.y, kk.y, s[r]);
               s[r] = fmaf(qq.z, kk.z, s[r]);
               s[r] = fmaf(qq.w, kk.w, s[r]);
             }
           }
-          if (TMA && at.x.end - key + lane < TILE) clear_rows<TILE, C::CHUNKS>(s_v + st * SUB, at.x.end - key + lane, TILE, lane);
+          if (TMA && seg.end - key0 < TILE) clear_rows<TILE, C::CHUNKS>(s_v + st * SUB, seg.end - key0, TILE, lane);
           float4 p4;
           float* p = &p4.x;
 #pragma unroll
           for (int r = 0; r < 4; r++) {
-            const float x = key < sees[r] && key < at.x.end ? s[r] * a.scale_log2 : -INFINITY;
+            const float x = key < min(sees[r], seg.end) ? s[r] * a.scale_log2 : -INFINITY;
             const float top = fmaxf(m[r], warp_max(x));
             if (top > m[r]) {
               const float f = m[r] == -INFINITY ? 0.f : exp2f(m[r] - top);
@@ -718,27 +780,22 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         const float sum = warp_sum(l[r]);
-        const int col = lane * CPL;
-        if (!w[r].there || col >= a.D) {
-          // a column behind the head's last one
-        } else if (direct) {
-          const float f = w[r].counts && sum != 0.f ? __frcp_rn(sum) : 0.f;
-          float* to = (float*)a.out + (((long long)w[r].b * a.T + w[r].t) * a.H + at.h * a.G + w[r].g) * a.D + col;
+        const int col = lane * CPL, rr = warp * 4 + r;
+        if (rr < seg.rows) {
+          const long long row = dst_of[rr];
+          const float f = seg.direct ? (sees_of[rr] && sum != 0.f ? __frcp_rn(sum) : 0.f) : 1.f;
+          float* to = (seg.direct ? (float*)a.out : a.part) + row * a.D + col;
+          if (col < a.D) {
 #pragma unroll
-          for (int c = 0; c < CPL; c++) to[c] = f == 0.f ? 0.f : o[r][c] * f;
-        } else {
-          float* to = a.part + part_row(w[r], warp * 4 + r) * a.D + col;
-#pragma unroll
-          for (int c = 0; c < CPL; c++) to[c] = o[r][c];
+            for (int c = 0; c < CPL; c++) to[c] = f == 0.f ? 0.f : o[r][c] * f;
+          }
+          if (!seg.direct && lane == 0) a.stat[row] = make_float2(m[r], sum);
         }
-        if (w[r].there && !direct && lane == 0) a.stat[part_row(w[r], warp * 4 + r)] = make_float2(m[r], sum);
       }
-      __syncwarp();
     }
-    first_segment = false;
-    left -= n;
-    tile_no += n;
-    at.next_segment(a);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&seg_empty[sg]);
+    if (++sg == SEGS) { sg = 0; sph ^= 1; }
   }
 }
 
@@ -1072,27 +1129,25 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 }
 
 // Joins the partial rows of a query row: those of the prefix and those of its own sequence, each in the order of the keys.  A warp a row, a
-// lane every 32nd column.  First the statistics, a part a lane, so that they are one wait and not one for each part; then the sums with their
+// lane four columns.  First the statistics, a part a lane, so that they are one wait and not one for each part; then the sums with their
 // weights, eight parts on their way at a time.  Rows that the first kernel has written are left alone; rows that see nothing become zeros.
 template <typename T, int ROWS, int TILE>
 __global__ void __launch_bounds__(256) cache_join_kernel(const CacheArgs a) {
   pdl_trigger();
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const long long rows = (long long)a.B * a.T * a.H;
-  const long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const unsigned rows = (unsigned)a.B * a.T * a.H, i = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (i >= rows) return;
-  const int head = (int)(i % a.H), h = head / a.G, g = head - h * a.G;
-  const long long bt = i / a.H;
-  const int b = (int)(bt / a.T), t = (int)(bt - (long long)b * a.T);
-  T* out = (T*)a.out + i * a.D;
+  const unsigned bt = i / a.H;
+  const int head = i - bt * a.H, h = head / a.G, g = head - h * a.G, b = bt / a.T, t = bt - b * a.T;
+  T* out = (T*)a.out + (long long)i * a.D;
   // parts: row `first`, then rest + k step, 0 < k < n
   struct Parts { long long first, rest, step; int n; };
   Parts pre = {0, 0, 0, 0}, own = {0, 0, 0, 0};
   const long long whole = 2LL * a.ctas * ROWS;
   auto find = [&](Parts& p, int e, int r, long long at) {
+    const int2 c = a.owner[e * a.Hkv + h];                           // (of an entry without tiles: anything)
     if (entry_of<ROWS, TILE>(a, e).tiles == 0) return true;
-    const int2 c = a.owner[e * a.Hkv + h];
     const int cta = c.x >> 1;
     if (cta == c.y) {                             // one CTA had all of it
       p = {at, at, 0, 1};
@@ -1134,15 +1189,22 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const CacheArgs a) {
     for (int j = 0; j < m; j++) {
       const float* p = a.part + __shfl_sync(0xffffffffu, row, j) * a.D;
       const float wj = __shfl_sync(0xffffffffu, w, j);
-#pragma unroll
-      for (int c = 0; c < 4; c++)
-        if (c * 32 + lane < a.D) o[c] += p[c * 32 + lane] * wj;
+      if (4 * lane < a.D) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(p) + lane);
+        o[0] += v.x * wj;
+        o[1] += v.y * wj;
+        o[2] += v.z * wj;
+        o[3] += v.w * wj;
+      }
     }
   }
   const float f = sum != 0.f ? __frcp_rn(sum) : 0.f;
+  if (4 * lane < a.D) {
 #pragma unroll
-  for (int c = 0; c < 4; c++)
-    if (c * 32 + lane < a.D) out[c * 32 + lane] = (T)(f == 0.f ? 0.f : o[c] * f);
+    for (int c = 0; c < 4; c++) o[c] = f == 0.f ? 0.f : o[c] * f;
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out + 4 * lane) = make_float4(o[0], o[1], o[2], o[3]);
+    else *reinterpret_cast<uint2*>(out + 4 * lane) = make_uint2(Elem<T>::pack(o[0], o[1]), Elem<T>::pack(o[2], o[3]));
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------
@@ -1159,6 +1221,7 @@ struct Sizes {
 
 // Which kernel takes what, and the workspace.  box: rows of a TMA box (0: none).
 bool plan(Sizes& z, int dtype, long long B, long long T, long long H, long long Hkv, long long D, int prefix, int box) {
+  if (B * T * H >= 0x7fffffffLL) return false;
   const long long own = T * (H / Hkv), all = B * own;
   z = Sizes{};
   if (all >= 0x7fffffffLL) return false;
@@ -1170,18 +1233,10 @@ bool plan(Sizes& z, int dtype, long long B, long long T, long long H, long long 
   if (z.wide_own || z.wide_prefix) {
     z.wide_tiles = (int)(((z.wide_own ? own : all) + kWideRows - 1) / kWideRows);
     const long long items = z.wide_tiles * Hkv * (z.wide_own ? B : 1);
-    // Runs of keys, so that the CTAs (two to an SM) come out in whole rounds: of up to 16, the number whose rounds are shortest, the smaller one
-    // where a larger gains less than a twentieth (partial rows have to be written and joined); runs of 256 keys at least in a prefix.
-    z.splits = 1;
-    double best = 0;
-    for (int n = 1; n <= 16; n++) {
-      if (z.wide_prefix && n > 1 && prefix / n < 256) break;
-      const double rounds = (double)((items * n + kCtas - 1) / kCtas) / n;
-      if (n == 1 || rounds < 0.95 * best) {
-        best = rounds;
-        z.splits = n;
-      }
-    }
+    // Runs of keys, as many as one round of CTAs (two to an SM) holds, 16 at most and of 256 keys at least in a prefix.
+    z.splits = items >= kCtas ? 1 : (int)(kCtas / items);
+    if (z.splits > 16) z.splits = 16;
+    if (z.wide_prefix && z.splits > prefix / 256) z.splits = prefix / 256 < 1 ? 1 : prefix / 256;
   }
   const long long most = shared && !z.wide_prefix ? all : own;
   z.rows = dtype == 2 || most <= 16 ? 16 : most <= 32 ? 32 : 64;
@@ -1230,7 +1285,7 @@ int launch_join(const CacheArgs& a, cudaStream_t s) {
 
 template <typename T, int HD, int RG, bool TMA>
 int launch_attn(const CUtensorMap& tk, const CUtensorMap& tv, CacheArgs& a, cudaStream_t s) {
-  using C = Cfg<T, HD, RG>;
+  using C = Cfg<T, HD, RG, TMA>;
   const auto kernel = cache_attn_kernel<T, HD, RG, TMA>;
   static std::atomic<uint32_t> done{0};
   const int rc = allow_shared(kernel, C::SMEM, done);
@@ -1329,7 +1384,9 @@ GB_EXPORT int gb_cache_attn(int dtype, const void* q, const void* k, const void*
     gbh::set_error("gb_cache_attn: workspace of %lld bytes is too small, or too many rows", ws_bytes);
     return gbh::E_TOO_LARGE;
   }
-  if (((long long)B * T * H + 7) / 8 >= 0x7fffffffLL || (long long)z.wide_tiles * z.splits * Hkv * B >= 0x7fffffffLL) {
+  // (the list of tiles is numbered in 32 bits)
+  const long long tiles = ((long long)columns * page + 31) / 32 * Hkv * (z.entries > 0 ? z.entries : 1);
+  if (tiles >= 0x7fffffffLL || (long long)z.wide_tiles * z.splits * Hkv * B >= 0x7fffffffLL) {
     gbh::set_error("gb_cache_attn: too many rows");
     return gbh::E_TOO_LARGE;
   }
