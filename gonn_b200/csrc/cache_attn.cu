@@ -28,8 +28,8 @@ using namespace gb;
 
 namespace {
 
-constexpr int kThreads = 160;
-constexpr int kConsumers = 4;
+constexpr int kThreads = 256;
+constexpr int kConsumers = 4, kCopiers = 4;      // warps
 
 struct CacheArgs {
   const void* q;
@@ -77,18 +77,18 @@ struct Cfg {
   static constexpr int HD = HD_, RG = RG_;
   static constexpr bool kMma = Elem<T>::kMma;
   static constexpr int ROWS = 16 * RG;
-  static constexpr int TILE = kMma ? 64 : 32;
+  static constexpr int TILE = kMma ? (HD == 64 ? 128 : 64) : HD == 64 ? 64 : 32;      // 16 KB of keys
   static constexpr int KG = kMma ? 4 / RG : 1;
   static constexpr int SUB = TILE * HD * (int)sizeof(T);          // one K or V tile
-  static constexpr int STAGES = HD == 64 ? 4 : 2;
+  static constexpr int STAGES = 2;
   static constexpr int SEGS = RG == 1 && kMma && TMA ? 3 : 2;           // segments (queries, rows) on their way
   static constexpr int Q_BYTES = ROWS * HD * (int)sizeof(T);
   static constexpr int CHUNKS = HD * (int)sizeof(T) / 16;         // 16-byte chunks of a row
   static constexpr int COLS = HD * (int)sizeof(T) / 128;          // columns of 128 bytes
   static constexpr int PAD = HD + 8;                              // floats of a row of sums: eight rows' columns in different banks
   // sums of the key groups that are joined (all four, or the second of two), or the weights of fp32
-  static constexpr int JOIN = kMma ? (RG == 1 ? 4 : RG == 2 ? 1 : 0) * ROWS * (PAD * 4 + 8) : ROWS * TILE * 4;
-  static constexpr int SMEM = 2 * STAGES * SUB + SEGS * Q_BYTES + JOIN + 1024 + SEGS * (ROWS * 12 + 32) + 256 + (TMA ? 0 : 2 * TILE * 8);
+  static constexpr int JOIN = kMma ? (RG == 1 ? 4 : RG == 2 ? 1 : 0) * ROWS * (PAD * 4 + 8) : ROWS * 32 * 4;
+  static constexpr int SMEM = 2 * STAGES * SUB + SEGS * Q_BYTES + JOIN + 1024 + SEGS * (ROWS * 12 + 32) + ROWS * 8 + 256 + (TMA ? 0 : 2 * TILE * 8);
   static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs to an SM");
 };
 
@@ -169,7 +169,7 @@ struct Cursor {
       const Entry y = entry_of<ROWS, TILE>(a, k);
       if (k == lo) first_entry = y;
       mine += y.tiles;
-      if (y.cut && blockIdx.x == 0) set_status(a.status, ST_BAD_INDEX, y.b);
+      if (y.cut && blockIdx.x == 0 && threadIdx.x < 32 * (kConsumers + 1)) set_status(a.status, ST_BAD_INDEX, y.b);
     }
     mine *= a.Hkv;
     unsigned sum = mine;
@@ -322,7 +322,8 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   uint8_t* s_q = s_v + STAGES * SUB;
   float* s_join = reinterpret_cast<float*>(s_q + SEGS * C::Q_BYTES);
   long long* s_dst = reinterpret_cast<long long*>((uint8_t*)s_join + C::JOIN);       // [SEGS][ROWS] where a row goes
-  long long* s_off = s_dst + SEGS * ROWS;                                            // where the keys and values of a tile start (cp.async)
+  long long* s_from = s_dst + SEGS * ROWS;                                           // [ROWS] where a row's query is, for the copying warp
+  long long* s_off = s_from + ROWS;                                                  // where the keys and values of a tile start (cp.async)
   int* s_sees = reinterpret_cast<int*>(s_off + (TMA ? 0 : 2 * TILE));                          // [SEGS][ROWS] keys that a row sees, 0: it does not count
   Segment* s_seg = reinterpret_cast<Segment*>(s_sees + SEGS * ROWS);
   uint64_t* full = reinterpret_cast<uint64_t*>(((uintptr_t)(s_seg + SEGS) + 7) & ~(uintptr_t)7);
@@ -335,11 +336,11 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; i++) {
-      mbar_init(&full[i], TMA ? 1 : 32);
+      mbar_init(&full[i], TMA ? kCopiers : 32 * kCopiers);
       mbar_init(&empty[i], kConsumers);
     }
     for (int i = 0; i < SEGS; i++) {
-      mbar_init(&seg_full[i], 33);               // every lane's copies, and the first one's arrival behind all other stores
+      mbar_init(&seg_full[i], 33 * kCopiers);    // every lane's copies, and a warp's first one's arrival behind all other stores
       mbar_init(&seg_empty[i], kConsumers);
     }
     mbar_init(&joined[0], kConsumers);
@@ -351,135 +352,144 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   pdl_wait();
   pdl_trigger();
 
-  if (warp == kConsumers) {
+  // Registers: 128 a thread at launch, of which the copying warps hand 64 to those that multiply.
+  if (warp >= kConsumers) {
     // ---------------- copies ----------------
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    const int me = warp - kConsumers;
     Cursor<ROWS, TILE> at;
     at.start(a, lane);
-    // lane i: column i % COLS of box i / COLS of keys and of values
-    const int box = lane / C::COLS, col = lane % C::COLS * (128 / (int)sizeof(T));
-    const bool mine = box * a.box < TILE;                            // (columns behind the head's last one: zeros)
-    constexpr int LOOK = TILE / 32;                                  // keys that a lane looks up for cp.async
+    constexpr int MINE = TILE / kCopiers;                            // keys of this warp for cp.async
     constexpr int PER = 32 / C::CHUNKS;                              // rows of one instruction of the warp
     const int sub = lane / C::CHUNKS, chunk = lane % C::CHUNKS;
     const bool inside = chunk * 16 < a.D * (int)sizeof(T);
-    // Pages of the next tile, asked for while this one is copied and looked at when its turn comes.  -1: behind the last key.
-    int page[LOOK], in_page[LOOK];
+    // A TMA copy is a box of rows by 128 bytes of keys or of values; they are dealt out to the warps and to their lanes, which take turns at
+    // 60 ns a copy.
+    const int units = TMA ? TILE / a.box * C::COLS * 2 : 0, unit = lane * kCopiers + me;
+    const int box = unit / (2 * C::COLS), col = unit / 2 % C::COLS;  // (columns behind the head's last one: zeros)
+    const int bytes = units > me ? (units - me + kCopiers - 1) / kCopiers * a.box * 128 : 0;
+    const int unit_to = col * (TILE * 128) + box * a.box * 128;
+    // Pages of the next tile, asked for while this one is copied and looked at when its turn comes: of a box a lane, or of a key a lane.
+    // -1: behind the last key.
+    int page, in_page;
     auto look_up = [&]() {
-      const int* row = a.table + (at.x.b < 0 ? 0 : at.x.b) * a.table_stride;
-#pragma unroll
-      for (int i = 0; i < (TMA ? 1 : LOOK); i++) {
-        const int key = at.x.begin + at.tile * TILE + (TMA ? box * a.box : i * 32 + lane);
-        page[i] = -1;
-        in_page[i] = 0;
-        if ((!TMA || mine) && key < at.x.end) {
-          const unsigned p = (unsigned)key / (unsigned)a.page;
-          in_page[i] = (int)((unsigned)key - p * (unsigned)a.page);
-          const int got = row[p];
-          page[i] = got == -1 ? -2 : got;
-        }
-      }
-    };
-    auto checked = [&](int i) {
-      if (page[i] < -1 || page[i] >= a.pages) {
-        set_status(a.status, ST_BAD_INDEX, at.x.b);
-        page[i] = -1;
+      const int key = at.x.begin + at.tile * TILE + (TMA ? box * a.box : me * MINE + lane);
+      page = -1;
+      in_page = 0;
+      if ((TMA ? unit < units : lane < MINE) && key < at.x.end) {
+        const unsigned p = (unsigned)key / (unsigned)a.page;
+        in_page = (int)((unsigned)key - p * (unsigned)a.page);
+        const int got = a.table[(at.x.b < 0 ? 0 : at.x.b) * a.table_stride + p];
+        page = got == -1 ? -2 : got;
       }
     };
     int st = 0, sg = 0;
     uint32_t ph = 0, sph = 0;
+    // Copies the tile whose pages have been looked up, and asks for the next one's if there is one in the segment.
+    auto copy_tile = [&](bool more) {
+      if (page < -1 || page >= a.pages) {
+        set_status(a.status, ST_BAD_INDEX, at.x.b);
+        page = -1;
+      }
+      if constexpr (TMA) {
+        const int pg = page < 0 ? a.pages : page, row = in_page;                     // behind the last page: zeros
+        at.tile++;
+        if (more) look_up();
+        if (!mbar_wait(&empty[st], ph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 20)) return false;
+        if (lane == 0) {
+          if (bytes) mbar_expect_tx(&full[st], bytes);
+          else mbar_arrive(&full[st]);
+        }
+        __syncwarp();
+        if (unit < units) {
+          const bool v = unit & 1;
+          tma_load_4d((v ? s_v : s_k) + st * SUB + unit_to, v ? &tm_v : &tm_k, &full[st], col * (128 / (int)sizeof(T)), row, at.h, pg);
+        }
+        __syncwarp();
+      } else {
+        long long* off = s_off + me * 2 * MINE;
+        if (lane < MINE) {
+          off[lane] = page < 0 ? -1 : page * a.k_sp + at.h * a.k_sh + in_page * a.k_sr;
+          off[MINE + lane] = page < 0 ? -1 : page * a.v_sp + at.h * a.v_sh + in_page * a.v_sr;
+        }
+        __syncwarp();
+        at.tile++;
+        if (more) look_up();
+        if (!mbar_wait(&empty[st], ph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 20)) return false;
+        uint8_t* dk = s_k + st * SUB;
+        uint8_t* dv = s_v + st * SUB;
+#pragma unroll 4
+        for (int r = 0; r < MINE; r += PER) {
+          const long long ko = off[r + sub], vo = off[MINE + r + sub];
+          const int size = ko >= 0 && inside ? 16 : 0;
+          const uint32_t to = chunk_at<TILE>(me * MINE + r + sub, chunk);
+          cp_async16(dk + to, (const T*)a.k + (size ? ko + chunk * (16 / (int)sizeof(T)) : 0), size);
+          cp_async16(dv + to, (const T*)a.v + (size ? vo + chunk * (16 / (int)sizeof(T)) : 0), size);
+        }
+        __syncwarp();
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[st])) : "memory");
+      }
+      if (++st == STAGES) { st = 0; ph ^= 1; }
+      return true;
+    };
     bool first_segment = true;
     const int per = a.T * a.G;
-    while (true) {
-      // the segment: its description, where its rows go, its queries
-      if (at.left) look_up();
+    while (at.left) {
+      // The first tile is on its way before the segment is described: where its rows go, its queries.
+      const int n = (int)min(at.left, (unsigned)(at.x.tiles - at.tile)), tile0 = at.tile;
+      look_up();
+      if (!copy_tile(n > 1)) break;
       if (!mbar_wait(&seg_empty[sg], sph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 23)) break;
-      const int n = (int)min(at.left, (unsigned)(at.x.tiles - at.tile));
-      if (at.left) {
-        const bool whole = n == at.x.tiles, direct = whole && !a.shared;
-        const int slot = 2 * blockIdx.x + (first_segment ? 0 : 1);
-        const int rows = min(ROWS, (at.x.b < 0 ? a.B * per : per) - at.x.row0);
-        if (lane == 0) {
-          s_seg[sg] = Segment{n, at.x.begin + at.tile * TILE, at.x.end, rows, direct};
-          if (at.tile == 0) a.owner[at.e * a.Hkv + at.h] = make_int2(slot, (int)at.shares.cta_of(at.segment0 + at.x.tiles - 1));
-        }
-        // Whole segments of a batch with a shared prefix leave partial rows too: in the output's order, those of the prefix behind the sequences'.
-#pragma unroll
-        for (int r = lane; r < ROWS; r += 32) {
-          const Row w = row_of(a, at.x, r);
-          const long long row = ((long long)w.b * a.T + w.t) * a.H + at.h * a.G + w.g;
-          s_sees[sg * ROWS + r] = w.counts ? max(w.sees, 0) : 0;
-          s_dst[sg * ROWS + r] = direct ? row : !whole ? (long long)slot * ROWS + r
-                                              : 2LL * a.ctas * ROWS + (at.x.b < 0 ? (long long)a.B * a.T * a.H : 0) + row;
-        }
-        uint8_t* dq = s_q + sg * C::Q_BYTES;
-        for (int r0 = 0; r0 < rows; r0 += PER) {                     // (rows behind the last one: anything, nothing comes of them)
-          const int r = r0 + sub;
-          const Row w = row_of(a, at.x, r);
-          const int bytes = w.counts && inside ? 16 : 0;
-          const T* from = (const T*)a.q + w.b * a.q_sb + w.t * a.q_st + (long long)(at.h * a.G + w.g) * a.q_sh;
-          cp_async16(dq + chunk_at<ROWS>(r, chunk), bytes ? from + chunk * (16 / (int)sizeof(T)) : (const T*)a.q, bytes);
-        }
-      } else if (lane == 0) {
-        s_seg[sg] = Segment{0, 0, 0, 0, 0};
+      const bool whole = n == at.x.tiles, direct = whole && !a.shared;
+      const int slot = 2 * blockIdx.x + (first_segment ? 0 : 1);
+      const int rows = min(ROWS, (at.x.b < 0 ? a.B * per : per) - at.x.row0);
+      if (lane == 0 && me == 0) {
+        s_seg[sg] = Segment{n, at.x.begin + tile0 * TILE, at.x.end, rows, direct};
+        if (tile0 == 0) a.owner[at.e * a.Hkv + at.h] = make_int2(slot, (int)at.shares.cta_of(at.segment0 + at.x.tiles - 1));
+      }
+      // Whole segments of a batch with a shared prefix leave partial rows too: in the output's order, those of the prefix behind the sequences'.
+      // The warps take a quarter of the rows each.
+      constexpr int RW = ROWS / kCopiers;
+      if (lane < RW) {
+        const int r = me * RW + lane;
+        const Row w = row_of(a, at.x, r);
+        const long long row = ((long long)w.b * a.T + w.t) * a.H + at.h * a.G + w.g;
+        s_sees[sg * ROWS + r] = w.counts ? max(w.sees, 0) : 0;
+        s_dst[sg * ROWS + r] = direct ? row : !whole ? (long long)slot * ROWS + r
+                                            : 2LL * a.ctas * ROWS + (at.x.b < 0 ? (long long)a.B * a.T * a.H : 0) + row;
+        s_from[r] = w.counts ? w.b * a.q_sb + w.t * a.q_st + (long long)(at.h * a.G + w.g) * a.q_sh : -1;
+      }
+      __syncwarp();
+      uint8_t* dq = s_q + sg * C::Q_BYTES;
+#pragma unroll 4
+      for (int r0 = me * RW; r0 < min(rows, me * RW + RW); r0 += PER) {      // (rows behind the last one: anything, nothing comes of them)
+        const long long from = s_from[r0 + sub];
+        const int bytes = from >= 0 && inside ? 16 : 0;
+        cp_async16(dq + chunk_at<ROWS>(r0 + sub, chunk), (const T*)a.q + (bytes ? from + chunk * (16 / (int)sizeof(T)) : 0), bytes);
       }
       __syncwarp();
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&seg_full[sg])) : "memory");
       if (lane == 0) mbar_arrive(&seg_full[sg]);
       if (++sg == SEGS) { sg = 0; sph ^= 1; }
-      if (at.left == 0) break;
       first_segment = false;
       at.left -= n;
       bool ok = true;
-      for (int i = 0; i < n && ok; i++) {
-        if constexpr (TMA) {
-          checked(0);
-          const int pg = page[0] < 0 ? a.pages : page[0], row = in_page[0];        // behind the last page: zeros
-          at.tile++;
-          if (i + 1 < n) look_up();
-          ok = mbar_wait(&empty[st], ph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 20);
-          if (!ok) break;
-          if (lane == 0) mbar_expect_tx(&full[st], 2 * SUB);
-          __syncwarp();
-          if (mine) {
-            const int to = st * SUB + lane % C::COLS * (TILE * 128) + box * a.box * 128;
-            tma_load_4d(s_k + to, &tm_k, &full[st], col, row, at.h, pg);
-            tma_load_4d(s_v + to, &tm_v, &full[st], col, row, at.h, pg);
-          }
-        } else {
-#pragma unroll
-          for (int k = 0; k < LOOK; k++) {
-            checked(k);
-            s_off[k * 32 + lane] = page[k] < 0 ? -1 : page[k] * a.k_sp + at.h * a.k_sh + in_page[k] * a.k_sr;
-            s_off[TILE + k * 32 + lane] = page[k] < 0 ? -1 : page[k] * a.v_sp + at.h * a.v_sh + in_page[k] * a.v_sr;
-          }
-          __syncwarp();
-          at.tile++;
-          if (i + 1 < n) look_up();
-          ok = mbar_wait(&empty[st], ph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 20);
-          if (!ok) break;
-          uint8_t* dk = s_k + st * SUB;
-          uint8_t* dv = s_v + st * SUB;
-#pragma unroll 8
-          for (int r = 0; r < TILE; r += PER) {
-            const long long ko = s_off[r + sub], vo = s_off[TILE + r + sub];
-            const int bytes = ko >= 0 && inside ? 16 : 0;
-            const uint32_t to = chunk_at<TILE>(r + sub, chunk);
-            cp_async16(dk + to, (const T*)a.k + (bytes ? ko + chunk * (16 / (int)sizeof(T)) : 0), bytes);
-            cp_async16(dv + to, (const T*)a.v + (bytes ? vo + chunk * (16 / (int)sizeof(T)) : 0), bytes);
-          }
-          __syncwarp();
-          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[st])) : "memory");
-        }
-        if (++st == STAGES) { st = 0; ph ^= 1; }
-      }
+      for (int i = 1; i < n && ok; i++) ok = copy_tile(i + 1 < n);
       if (!ok) break;
       if (at.left) at.next_segment(a);
+    }
+    if (at.left == 0 && mbar_wait(&seg_empty[sg], sph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 23)) {
+      if (lane == 0 && me == 0) s_seg[sg] = Segment{0, 0, 0, 0, 0};  // no more
+      __syncwarp();
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&seg_full[sg])) : "memory");
+      if (lane == 0) mbar_arrive(&seg_full[sg]);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     return;
   }
 
   // ---------------- products ----------------
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
   int st = 0, sg = 0;
   uint32_t ph = 0, sph = 0, jph = 0;
   const int rg = warp / KG, kg = warp % KG;      // (fp32: rows 4 warp .. 4 warp + 3)
@@ -515,11 +525,15 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         const int key0 = seg.key0 + i * TILE + kg * NK;
         if (!idle && key0 < seg.end) {
           const uint32_t ka = smem_u32(s_k + st * SUB), va = smem_u32(s_v + st * SUB);
-          float s[NK / 8][4];
+          float s[NK / 8][4], odd[2][4];
 #pragma unroll
           for (int j = 0; j < NK / 8; j++)
 #pragma unroll
             for (int c = 0; c < 4; c++) s[j][c] = 0.f;
+          // A warp with few keys has few chains of dependent products: two of half the length for each.
+          constexpr bool kHalves = NK == 16;
+#pragma unroll
+          for (int c = 0; c < 8; c++) odd[c / 4][c % 4] = 0.f;
 #pragma unroll
           for (int j = 0; j < NK / 16; j++) {                        // 16 keys: two n8 tiles
             const int row = kg * NK + j * 16 + (lane & 7) + ((lane >> 4) << 3);
@@ -527,9 +541,13 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
             for (int x = 0; x < HD / 16; x++) {
               uint32_t b[4];
               ldm4(b, ka + chunk_at<TILE>(row, x * 2 + ((lane >> 3) & 1)));
-              mma16<T>(s[2 * j], qf[x], b[0], b[1]);
-              mma16<T>(s[2 * j + 1], qf[x], b[2], b[3]);
+              mma16<T>(kHalves && x % 2 ? odd[0] : s[2 * j], qf[x], b[0], b[1]);
+              mma16<T>(kHalves && x % 2 ? odd[1] : s[2 * j + 1], qf[x], b[2], b[3]);
             }
+          }
+          if (kHalves) {
+#pragma unroll
+            for (int c = 0; c < 8; c++) s[c / 4][c % 4] += odd[c / 4][c % 4];
           }
           const int low = min(min(sees0, sees1), seg.end);           // (zeros stand in for keys behind the last one)
           if (__any_sync(0xffffffffu, low - key0 < NK)) {
@@ -701,7 +719,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       static_assert(RG == 1, "16 rows");
       constexpr int CPL = HD / 32;
       const uint8_t* q = s_q + sg * C::Q_BYTES;
-      float* s_p = s_join + warp * (4 * TILE);                       // [TILE][4] of this warp
+      float* s_p = s_join + warp * (4 * 32);                         // [32 keys][4] of this warp
       int sees[4];
       bool any = false;
 #pragma unroll
@@ -723,11 +741,15 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         if (any) {
           const uint8_t* kt = s_k + st * SUB;
           const uint8_t* vt = s_v + st * SUB;
-          const int key0 = seg.key0 + i * TILE, key = key0 + lane;
+          const int key0 = seg.key0 + i * TILE;
+          if (TMA && seg.end - key0 < TILE) clear_rows<TILE, C::CHUNKS>(s_v + st * SUB, seg.end - key0, TILE, lane);
+#pragma unroll 1
+          for (int j0 = 0; j0 < min(TILE, seg.end - key0); j0 += 32) {   // 32 keys at a time
+          const int key = key0 + j0 + lane;
           float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
           for (int c = 0; c < HD / 4; c++) {
-            const float4 kk = *reinterpret_cast<const float4*>(kt + chunk_at<TILE>(lane, c));
+            const float4 kk = *reinterpret_cast<const float4*>(kt + chunk_at<TILE>(j0 + lane, c));
 #pragma unroll
             for (int r = 0; r < 4; r++) {
               const float4 qq = *reinterpret_cast<const float4*>(q + chunk_at<ROWS>(warp * 4 + r, c));
@@ -737,7 +759,6 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
               s[r] = fmaf(qq.w, kk.w, s[r]);
             }
           }
-          if (TMA && seg.end - key0 < TILE) clear_rows<TILE, C::CHUNKS>(s_v + st * SUB, seg.end - key0, TILE, lane);
           float4 p4;
           float* p = &p4.x;
 #pragma unroll
@@ -758,10 +779,10 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           *reinterpret_cast<float4*>(s_p + lane * 4) = p4;
           __syncwarp();
 #pragma unroll 4
-          for (int j = 0; j < TILE; j++) {
+          for (int j = 0; j < 32; j++) {
             const float4 pj = *reinterpret_cast<const float4*>(s_p + j * 4);
             float v[CPL];
-            const uint8_t* vr = vt + chunk_at<TILE>(j, lane * CPL / 4);
+            const uint8_t* vr = vt + chunk_at<TILE>(j0 + j, lane * CPL / 4);
             if constexpr (CPL == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(vr);
             else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(vr + (lane & 1) * 8);
 #pragma unroll
@@ -771,6 +792,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
               o[2][c] = fmaf(pj.z, v[c], o[2][c]);
               o[3][c] = fmaf(pj.w, v[c], o[3][c]);
             }
+          }
           }
         }
         __syncwarp();
@@ -807,17 +829,18 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 // keys, weights written over their scores as the second product's operand; two score buffers, so that the next scores are computed while
 // a softmax warp (a row a thread) works.  The sum is rescaled only when the maximum has moved by more than 2^8.  Where the row tiles are too few
 // for the SMs, the keys are cut into `splits` runs, which leave partial rows.
-constexpr int kWideRows = 128, kWideKeys = 64, kWideThreads = 192;
+constexpr int kWideRows = 128, kWideKeys = 64, kWideThreads = 256, kWideCopiers = 3;
 
 template <int HD>
 struct Wide {
   static constexpr int CH = HD / 64, Q_BYTES = CH * kWideRows * 128, SUB = CH * kWideKeys * 128;
   static constexpr int STAGES = HD == 64 ? 3 : 2;
-  static constexpr int SMEM = Q_BYTES + 2 * STAGES * SUB + 1024 + 256;
+  static constexpr int SMEM = Q_BYTES + 2 * STAGES * SUB + 1024 + 256 + 2 * kWideKeys * 8;
   static constexpr int COLS = 256, COL_O = 128;
+  static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs to an SM");
 };
 
-template <typename T, int HD>
+template <typename T, int HD, bool TMA>
 __global__ void __launch_bounds__(kWideThreads, 2)
 cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const CacheArgs a) {
   using C = Wide<HD>;
@@ -835,16 +858,17 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   uint64_t* s_full = v_empty + STAGES;
   uint64_t* p_full = s_full + 2;
   uint64_t* pv_done = p_full + 2;
-  uint32_t* tmem_slot = (uint32_t*)(pv_done + 2);
+  long long* s_off = (long long*)(pv_done + 2);                      // where the keys and values of a sub-tile start (cp.async)
+  uint32_t* tmem_slot = (uint32_t*)(s_off + 2 * kWideKeys);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 4);
     for (int i = 0; i < STAGES; i++) {
-      mbar_init(&k_full[i], 1);
+      mbar_init(&k_full[i], kWideCopiers);
       mbar_init(&k_empty[i], 1);
-      mbar_init(&v_full[i], 1);
+      mbar_init(&v_full[i], kWideCopiers);
       mbar_init(&v_empty[i], 1);
     }
     for (int i = 0; i < 2; i++) {
@@ -855,7 +879,7 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     *abort_flag = 0;
     mbar_fence_init();
   }
-  if (warp == 1) {
+  if (warp == kWideCopiers) {
     tmem_alloc(tmem_slot, C::COLS);
     tmem_relinquish();
   }
@@ -888,45 +912,104 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   x.tiles = (x.end + kWideKeys - 1) / kWideKeys;
   const int first = (int)((long long)x.tiles * split / a.splits), n_kv = (int)((long long)x.tiles * (split + 1) / a.splits) - first;
 
-  if (warp == 0) {
-    // lane i: columns i % CH of box i / CH
-    const int box = lane / C::CH, col = lane % C::CH * 64;
-    const bool mine = box * a.box < kWideKeys;
-    int page = 0, in_page = 0;
-    auto look_up = [&](int j) {
-      if (!mine) return;
-      const int key = (first + j) * kWideKeys + box * a.box;
-      page = a.pages;
+  if (warp < kWideCopiers) {
+    int st = 0;
+    uint32_t ph = 0;
+    // the page of a key, for sub-tile j; -1: behind the last key
+    int page = -1, in_page = 0;
+    auto look_up = [&](int key, bool mine) {
+      page = -1;
       in_page = 0;
-      if (key < x.end) {
+      if (mine && key < x.end) {
         const unsigned p = (unsigned)key / (unsigned)a.page;
         in_page = (int)((unsigned)key - p * (unsigned)a.page);
         page = a.table[(key < a.prefix ? 0 : x.b) * a.table_stride + p];
-        if (page < 0 || page >= a.pages) {
-          set_status(a.status, ST_BAD_INDEX, x.b);
-          page = a.pages;
-        }
+        page = page == -1 ? -2 : page;
       }
     };
-    if (n_kv > 0) look_up(0);
-    int st = 0;
-    uint32_t ph = 0;
-    const int to = lane % C::CH * (kWideKeys * 128) + box * a.box * 128;
-    for (int j = 0; j < n_kv; j++) {
-      const int pg = page, row = in_page;
-      if (j + 1 < n_kv) look_up(j + 1);
-      if (!mbar_wait(&k_empty[st], ph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 30)) break;
-      if (lane == 0) mbar_expect_tx(&k_full[st], SUB);
-      __syncwarp();
-      if (mine) tma_load_4d(s_k + st * SUB + to, &tm_k, &k_full[st], col, row, h, pg);
-      if (!mbar_wait(&v_empty[st], ph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 31)) break;
-      if (lane == 0) mbar_expect_tx(&v_full[st], SUB);
-      __syncwarp();
-      if (mine) tma_load_4d(s_v + st * SUB + to, &tm_v, &v_full[st], col, row, h, pg);
-      if (++st == STAGES) { st = 0; ph ^= 1; }
+    auto check = [&]() {
+      if (page < -1 || page >= a.pages) {
+        set_status(a.status, ST_BAD_INDEX, x.b);
+        page = -1;
+      }
+    };
+    if constexpr (TMA) {
+      // boxes of rows by 64 columns, dealt out to the warps and their lanes
+      const int units = kWideKeys / a.box * C::CH, unit = lane * kWideCopiers + warp, box = unit / C::CH, col = unit % C::CH;
+      const bool mine = unit < units;
+      const int bytes = units > warp ? (units - warp + kWideCopiers - 1) / kWideCopiers * a.box * 128 : 0;
+      const int to = col * (kWideKeys * 128) + box * a.box * 128;
+      auto copy = [&](uint8_t* tile, const CUtensorMap* map, uint64_t* bar, int pg, int row) {
+        if (lane == 0) {
+          if (bytes) mbar_expect_tx(bar, bytes);
+          else mbar_arrive(bar);
+        }
+        __syncwarp();
+        if (mine) tma_load_4d(tile + to, map, bar, col * 64, row, h, pg);
+        __syncwarp();
+      };
+      if (n_kv > 0) look_up(first * kWideKeys + box * a.box, mine);
+      for (int j = 0; j < n_kv; j++) {
+        check();
+        const int pg = page < 0 ? a.pages : page, row = in_page;     // behind the last page: zeros
+        if (j + 1 < n_kv) look_up((first + j + 1) * kWideKeys + box * a.box, mine);
+        if (!mbar_wait(&k_empty[st], ph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 30)) break;
+        copy(s_k + st * SUB, &tm_k, &k_full[st], pg, row);
+        if (!mbar_wait(&v_empty[st], ph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 31)) break;
+        copy(s_v + st * SUB, &tm_v, &v_full[st], pg, row);
+        if (++st == STAGES) { st = 0; ph ^= 1; }
+      }
+    } else {
+      // Key by key with cp.async, which the tensor core sees after a fence of the thread that copied: a sub-tile is handed on when the next copy is
+      // on its way.
+      constexpr int CHUNKS = HD / 8, PER = 32 / CHUNKS, MOST = (kWideKeys + kWideCopiers - 1) / kWideCopiers;
+      const int row0 = warp * MOST, rows = min(MOST, kWideKeys - row0), sub = lane / CHUNKS, chunk = lane % CHUNKS;
+      const bool inside = chunk * 8 < a.D;
+      long long* off = s_off + 2 * row0;
+      uint64_t* waiting = nullptr;
+      auto hand_on = [&](uint64_t* next) {
+        if (next) asm volatile("cp.async.commit_group;\ncp.async.wait_group 1;" ::: "memory");
+        else asm volatile("cp.async.wait_all;" ::: "memory");
+        if (waiting) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(waiting);
+        }
+        waiting = next;
+      };
+      auto copy = [&](uint8_t* tile, const T* from, const long long* at) {
+#pragma unroll 4
+        for (int r = 0; r < rows; r += PER) {
+          const long long o = r + sub < rows ? at[r + sub] : -1;
+          const int size = o >= 0 && inside ? 16 : 0;
+          if (r + sub < rows) cp_async16(tile + chunk_at<kWideKeys>(row0 + r + sub, chunk), from + (size ? o + chunk * 8 : 0), size);
+        }
+      };
+      if (n_kv > 0) look_up(first * kWideKeys + row0 + lane, lane < rows);
+      bool ok = true;
+      for (int j = 0; j < n_kv; j++) {
+        check();
+        __syncwarp();
+        if (lane < rows) {
+          off[lane] = page < 0 ? -1 : page * a.k_sp + h * a.k_sh + in_page * a.k_sr;
+          off[rows + lane] = page < 0 ? -1 : page * a.v_sp + h * a.v_sh + in_page * a.v_sr;
+        }
+        __syncwarp();
+        if (j + 1 < n_kv) look_up((first + j + 1) * kWideKeys + row0 + lane, lane < rows);
+        ok = mbar_wait(&k_empty[st], ph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 30);
+        if (!ok) break;
+        copy(s_k + st * SUB, (const T*)a.k, off);
+        hand_on(&k_full[st]);
+        ok = mbar_wait(&v_empty[st], ph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 31);
+        if (!ok) break;
+        copy(s_v + st * SUB, (const T*)a.v, off + rows);
+        hand_on(&v_full[st]);
+        if (++st == STAGES) { st = 0; ph ^= 1; }
+      }
+      hand_on(nullptr);
     }
     __syncwarp();
-  } else if (warp == 1) {
+  } else if (warp == kWideCopiers) {
     if (elect_one()) {
       const uint32_t fmt = __is_same(T, __nv_bfloat16) ? 1u : 0u;
       const uint32_t idesc_s = make_idesc(1u, fmt, false, false, kWideRows, kWideKeys);
@@ -1122,7 +1205,7 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) {
+  if (warp == kWideCopiers) {
     tc_fence_after();
     tmem_dealloc(tmem, C::COLS);
   }
@@ -1185,16 +1268,20 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const CacheArgs a) {
 #pragma unroll
     for (int c = 0; c < 4; c++) o[c] *= f;
     const int m = min(32, n - k0);
-#pragma unroll 8
-    for (int j = 0; j < m; j++) {
-      const float* p = a.part + __shfl_sync(0xffffffffu, row, j) * a.D;
-      const float wj = __shfl_sync(0xffffffffu, w, j);
-      if (4 * lane < a.D) {
-        const float4 v = __ldg(reinterpret_cast<const float4*>(p) + lane);
-        o[0] += v.x * wj;
-        o[1] += v.y * wj;
-        o[2] += v.z * wj;
-        o[3] += v.w * wj;
+    for (int j0 = 0; j0 < m; j0 += 8) {
+      float4 v[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const long long at = __shfl_sync(0xffffffffu, row, j0 + j) * a.D + 4 * lane;
+        v[j] = j0 + j < m && 4 * lane < a.D ? __ldg(reinterpret_cast<const float4*>(a.part + at)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float wj = j0 + j < m ? __shfl_sync(0xffffffffu, w, j0 + j) : 0.f;
+        o[0] += v[j].x * wj;
+        o[1] += v[j].y * wj;
+        o[2] += v[j].z * wj;
+        o[3] += v[j].w * wj;
       }
     }
   }
@@ -1219,14 +1306,14 @@ struct Sizes {
   long long entries, part, stat, owner, total;      // bytes of the workspace's parts
 };
 
-// Which kernel takes what, and the workspace.  box: rows of a TMA box (0: none).
-bool plan(Sizes& z, int dtype, long long B, long long T, long long H, long long Hkv, long long D, int prefix, int box) {
+// Which kernel takes what, and the workspace.
+bool plan(Sizes& z, int dtype, long long B, long long T, long long H, long long Hkv, long long D, int prefix) {
   if (B * T * H >= 0x7fffffffLL) return false;
   const long long own = T * (H / Hkv), all = B * own;
   z = Sizes{};
   if (all >= 0x7fffffffLL) return false;
   // Many rows of a sequence: its keys with the prefix among them, nothing is gained by sharing.  Many rows of the batch alone: its prefix.
-  const bool wide = dtype != 2 && box > 0;
+  const bool wide = dtype != 2;
   z.wide_own = wide && own > 64;
   const bool shared = prefix > 0 && !z.wide_own;
   z.wide_prefix = shared && wide && all > 64;
@@ -1265,14 +1352,14 @@ int allow_shared(K kernel, int bytes, std::atomic<uint32_t>& done) {
   return gbh::E_OK;
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool TMA>
 int launch_wide(const CUtensorMap& tk, const CUtensorMap& tv, const CacheArgs& a, cudaStream_t s) {
   using C = Wide<HD>;
   static std::atomic<uint32_t> done{0};
-  const int rc = allow_shared(cache_wide_kernel<T, HD>, C::SMEM, done);
+  const int rc = allow_shared(cache_wide_kernel<T, HD, TMA>, C::SMEM, done);
   if (rc) return rc;
   const long long ctas = (long long)a.wide_tiles * a.splits * a.Hkv * (a.wide_prefix ? 1 : a.B);
-  GB_CUDA_OK(gbh::launch(cache_wide_kernel<T, HD>, dim3((unsigned)ctas), dim3(kWideThreads), C::SMEM, s, 1, tk, tv, a));
+  GB_CUDA_OK(gbh::launch(cache_wide_kernel<T, HD, TMA>, dim3((unsigned)ctas), dim3(kWideThreads), C::SMEM, s, 1, tk, tv, a));
   return gbh::E_OK;
 }
 
@@ -1305,8 +1392,9 @@ int cache_map(CUtensorMap* m, int dtype, const void* base, int D, int page, int 
 }
 
 // Rows of a TMA box, 0 where there can be none: a power of two that divides a page and a tile; strides that a tensor map holds.
-int box_of(int page, int tile, const long long* strides, int size) {
-  int rows = tile;
+int box_of(int page, int dtype, int D, const long long* strides) {
+  const int size = dtype == 2 ? 4 : 2;
+  int rows = dtype == 2 && D > 64 ? 32 : 64;
   while (rows > 1 && page % rows) rows >>= 1;
   for (int i = 0; i < 6; i++)
     if (strides[i] <= 0 || strides[i] * size >= (1LL << 40)) return 0;
@@ -1328,7 +1416,8 @@ template <typename T>
 int launch_any(const CUtensorMap& k, const CUtensorMap& v, CacheArgs& a, int rows, cudaStream_t s) {
   if constexpr (Elem<T>::kMma) {
     if (a.wide_own || a.wide_prefix) {
-      const int rc = a.D <= 64 ? launch_wide<T, 64>(k, v, a, s) : launch_wide<T, 128>(k, v, a, s);
+      const int rc = a.box ? (a.D <= 64 ? launch_wide<T, 64, true>(k, v, a, s) : launch_wide<T, 128, true>(k, v, a, s))
+                           : (a.D <= 64 ? launch_wide<T, 64, false>(k, v, a, s) : launch_wide<T, 128, false>(k, v, a, s));
       if (rc) return rc;
       if (a.wide_own) return a.splits > 1 ? launch_join<T, 64, 64>(a, s) : gbh::E_OK;
     }
@@ -1338,12 +1427,11 @@ int launch_any(const CUtensorMap& k, const CUtensorMap& v, CacheArgs& a, int row
 
 }  // namespace
 
-// Bytes of the workspace of gb_cache_attn, or a negative error.  strides: as there.
-GB_EXPORT long long gb_cache_attn_bytes(int dtype, long long B, long long T, long long H, long long Hkv, long long D, int page, int prefix,
-                                        const long long* strides) {
+// Bytes of the workspace of gb_cache_attn, or a negative error.
+GB_EXPORT long long gb_cache_attn_bytes(int dtype, long long B, long long T, long long H, long long Hkv, long long D, int prefix) {
   Sizes z;
-  if (dtype < 0 || dtype > 2 || B < 0 || T < 1 || H < 1 || Hkv < 1 || H % Hkv || D < 1 || D > 128 || page < 1 || !strides ||
-      !plan(z, dtype, B, T, H, Hkv, D, prefix, box_of(page, dtype == 2 ? 32 : 64, strides + 3, dtype == 2 ? 4 : 2))) {
+  if (dtype < 0 || dtype > 2 || B < 0 || T < 1 || H < 1 || Hkv < 1 || H % Hkv || D < 1 || D > 128 ||
+      !plan(z, dtype, B, T, H, Hkv, D, prefix)) {
     gbh::set_error("gb_cache_attn: too many rows, or bad sizes (%lld sequences, %lld tokens, %lld and %lld heads of %lld)", B, T, H, Hkv, D);
     return gbh::E_TOO_LARGE;
   }
@@ -1378,9 +1466,9 @@ GB_EXPORT int gb_cache_attn(int dtype, const void* q, const void* k, const void*
     return gbh::E_BAD_ARG;
   }
   CacheArgs a = {};
-  a.box = box_of(page, dtype == 2 ? 32 : 64, strides + 3, size);
+  a.box = box_of(page, dtype, D, strides + 3);
   Sizes z;
-  if (!plan(z, dtype, B, T, H, Hkv, D, prefix, a.box) || ws_bytes < z.total) {
+  if (!plan(z, dtype, B, T, H, Hkv, D, prefix) || ws_bytes < z.total) {
     gbh::set_error("gb_cache_attn: workspace of %lld bytes is too small, or too many rows", ws_bytes);
     return gbh::E_TOO_LARGE;
   }

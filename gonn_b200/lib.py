@@ -37,7 +37,7 @@ _ARGUMENTS = {
     "gb_mx_linear": "iipLppppiLLLiipLp",
     "gb_mx_train_forward": "iipLpLppiLLLiipLpLp", "gb_mx_train_backward": "ipLppipipiLLLpLp",
     "gb_rotary": "ipLLLpiiiiiipdipiLLp", "gb_cache_append": "ipppppppiiiiiiipdpLiiippp",
-    "gb_cache_attn": "ipppppiiiiipLiiippidpLp", "gb_cache_attn_bytes": "iLLLLLiip",
+    "gb_cache_attn": "ipppppiiiiipLiiippidpLp", "gb_cache_attn_bytes": "iLLLLLi",
     "gb_mx_plan": "LLLip", "gb_mx_linear_bytes": "LLLi", "gb_mx_train_bytes": "LLLiii",
 }
 

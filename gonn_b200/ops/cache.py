@@ -130,8 +130,8 @@ def _append_ref(k_cache, v_cache, k, v, table, lengths, counts, w, interleaved, 
 
 
 @lru_cache(maxsize=1024)
-def _workspace(code, batch, tokens, heads, kv, width, page, prefix, *strides):
-    n = _l.lib().gb_cache_attn_bytes(code, batch, tokens, heads, kv, width, page, prefix, (c_longlong * 9)(0, 0, 0, *strides))
+def _workspace(code, batch, tokens, heads, kv, width, prefix):
+    n = _l.lib().gb_cache_attn_bytes(code, batch, tokens, heads, kv, width, prefix)
     _l.check(min(n, 0), "gb_cache_attn_bytes")
     return n
 
@@ -166,7 +166,7 @@ def attend(k_cache, v_cache, q, table, lengths, counts=None, scale: Optional[flo
         table = table.contiguous()
     code = _TYPES[q.dtype]
     ks, vs = k_cache.stride()[:3], v_cache.stride()[:3]
-    need = _workspace(code, batch, tokens, heads, kv, width, page, shared_pages * page, *ks, *vs)
+    need = _workspace(code, batch, tokens, heads, kv, width, shared_pages * page)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device)
     strides = (c_longlong * 9)(sb, st, sh, *ks, *vs)
     _l.call_on(q.get_device(), "gb_cache_attn", code, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), strides, batch, tokens,
