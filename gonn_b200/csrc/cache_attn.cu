@@ -70,25 +70,26 @@ template <> struct Elem<__half> {
 };
 template <> struct Elem<float> { static constexpr bool kMma = false; };
 
-// Rows of a tile: 16 RG.  Row groups of 16 rows times key groups of a quarter, a half or all of the keys are the four warps of the
-// 16-bit kernel; in fp32 a warp takes four rows and all keys.  Two CTAs to an SM: while one waits, joins or stores, the other multiplies.
+// Rows of a tile: 16 RG, or 4 (RG = 0, fp32).  Row groups of 16 rows times key groups of a quarter, a half or all of the keys are the four
+// warps of the 16-bit kernel; in fp32 a warp takes a quarter of the keys and all rows.  Two CTAs to an SM: while one waits, joins or stores, the other multiplies.
 template <typename T, int HD_, int RG_, bool TMA>
 struct Cfg {
   static constexpr int HD = HD_, RG = RG_;
   static constexpr bool kMma = Elem<T>::kMma;
-  static constexpr int ROWS = 16 * RG;
+  static constexpr int ROWS = RG ? 16 * RG : 4;
   static constexpr int TILE = kMma ? (HD == 64 ? 128 : 64) : HD == 64 ? 64 : 32;      // 16 KB of keys
-  static constexpr int KG = kMma ? 4 / RG : 1;
+  static constexpr int KG = kMma ? 4 / (RG ? RG : 1) : 4;
   static constexpr int SUB = TILE * HD * (int)sizeof(T);          // one K or V tile
   static constexpr int STAGES = 2;
-  static constexpr int SEGS = RG == 1 && kMma && TMA ? 3 : 2;           // segments (queries, rows) on their way
+  static constexpr int SEGS = RG <= 1 && TMA && ROWS * HD * (int)sizeof(T) <= 4096 ? 3 : 2;           // segments (queries, rows) on their way
   static constexpr int Q_BYTES = ROWS * HD * (int)sizeof(T);
   static constexpr int CHUNKS = HD * (int)sizeof(T) / 16;         // 16-byte chunks of a row
   static constexpr int COLS = HD * (int)sizeof(T) / 128;          // columns of 128 bytes
   static constexpr int PAD = HD + 8;                              // floats of a row of sums: eight rows' columns in different banks
-  // sums of the key groups that are joined (all four, or the second of two), or the weights of fp32
-  static constexpr int JOIN = kMma ? (RG == 1 ? 4 : RG == 2 ? 1 : 0) * ROWS * (PAD * 4 + 8) : ROWS * 32 * 4;
-  static constexpr int SMEM = 2 * STAGES * SUB + SEGS * Q_BYTES + JOIN + 1024 + SEGS * (ROWS * 12 + 32) + ROWS * 8 + 256 + (TMA ? 0 : 2 * TILE * 8);
+  static constexpr int RJ = ROWS < 16 || kMma ? ROWS : 8;         // rows whose four sums are joined at a time
+  static constexpr int JOIN = (KG == 4 ? 4 * RJ : KG == 2 ? ROWS : 0) * (PAD * 4 + 8);      // of two key groups one hands its sums to the other
+  static constexpr int WEIGHTS = kMma ? 0 : TILE * ROWS * 4;      // fp32: the weights of a tile
+  static constexpr int SMEM = 2 * STAGES * SUB + SEGS * Q_BYTES + JOIN + WEIGHTS + 1024 + SEGS * (ROWS * 12 + 32) + ROWS * 8 + 256 + (TMA ? 0 : 2 * TILE * 8);
   static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs to an SM");
 };
 
@@ -321,7 +322,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   uint8_t* s_v = s_k + STAGES * SUB;
   uint8_t* s_q = s_v + STAGES * SUB;
   float* s_join = reinterpret_cast<float*>(s_q + SEGS * C::Q_BYTES);
-  long long* s_dst = reinterpret_cast<long long*>((uint8_t*)s_join + C::JOIN);       // [SEGS][ROWS] where a row goes
+  long long* s_dst = reinterpret_cast<long long*>((uint8_t*)s_join + C::JOIN + C::WEIGHTS);       // [SEGS][ROWS] where a row goes
   long long* s_from = s_dst + SEGS * ROWS;                                           // [ROWS] where a row's query is, for the copying warp
   long long* s_off = s_from + ROWS;                                                  // where the keys and values of a tile start (cp.async)
   int* s_sees = reinterpret_cast<int*>(s_off + (TMA ? 0 : 2 * TILE));                          // [SEGS][ROWS] keys that a row sees, 0: it does not count
@@ -450,6 +451,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       // Whole segments of a batch with a shared prefix leave partial rows too: in the output's order, those of the prefix behind the sequences'.
       // The warps take a quarter of the rows each.
       constexpr int RW = ROWS / kCopiers;
+      static_assert(RW >= 1, "rows of a warp");
       if (lane < RW) {
         const int r = me * RW + lane;
         const Row w = row_of(a, at.x, r);
@@ -463,6 +465,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       uint8_t* dq = s_q + sg * C::Q_BYTES;
 #pragma unroll 4
       for (int r0 = me * RW; r0 < min(rows, me * RW + RW); r0 += PER) {      // (rows behind the last one: anything, nothing comes of them)
+        if (RW < PER && sub >= RW) break;
         const long long from = s_from[r0 + sub];
         const int bytes = from >= 0 && inside ? 16 : 0;
         cp_async16(dq + chunk_at<ROWS>(r0 + sub, chunk), (const T*)a.q + (bytes ? from + chunk * (16 / (int)sizeof(T)) : 0), bytes);
@@ -492,7 +495,42 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
   int st = 0, sg = 0;
   uint32_t ph = 0, sph = 0, jph = 0;
-  const int rg = warp / KG, kg = warp % KG;      // (fp32: rows 4 warp .. 4 warp + 3)
+  const int rg = warp / KG, kg = warp % KG;
+  float2* s_stat = reinterpret_cast<float2*>(s_join + (KG == 4 ? 4 * C::RJ : KG == 2 ? ROWS : 0) * C::PAD);
+  // Four key groups' sums of the rows from..from + RJ - 1 meet in shared memory; a warp joins a quarter of the columns.
+  auto join_rows = [&](const Segment& seg, int from) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&joined[0]);
+    if (!mbar_wait(&joined[0], jph, abort_flag, a.status, ST_ATTN_TIMEOUT, 26)) return false;
+    jph ^= 1;
+    constexpr int CPW = HD / 4, STEP = 32 / CPW;                     // columns of a warp, rows at a time
+    const int col = warp * CPW + lane % CPW;
+#pragma unroll 2
+    for (int r = lane / CPW; r < min(C::RJ, seg.rows - from); r += STEP) {
+      float2 y[4];
+      float top = -INFINITY, l = 0.f, sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        y[k] = s_stat[k * C::RJ + r];
+        top = fmaxf(top, y[k].x);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const float w = y[k].x == -INFINITY ? (y[k].y == 0.f ? 0.f : 1.f) : exp2f(y[k].x - top);   // (scores of NaN leave no maximum, but a sum)
+        l += y[k].y * w;
+        sum += s_join[(k * C::RJ + r) * C::PAD + col] * w;
+      }
+      const long long row = s_dst[sg * ROWS + from + r];
+      if (col < a.D) {
+        if (seg.direct) ((T*)a.out)[row * a.D + col] = (T)(s_sees[sg * ROWS + from + r] && l != 0.f ? sum * __frcp_rn(l) : 0.f);
+        else a.part[row * a.D + col] = sum;
+      }
+      if (!seg.direct && col == 0) a.stat[row] = make_float2(top, l);
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&joined[1]);
+    return true;
+  };
   for (;;) {
     if (!mbar_wait(&seg_full[sg], sph, abort_flag, a.status, ST_ATTN_TIMEOUT, 24)) return;
     const Segment seg = s_seg[sg];
@@ -619,9 +657,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         l0 += __shfl_xor_sync(0xffffffffu, l0, d);
         l1 += __shfl_xor_sync(0xffffffffu, l1, d);
       }
-      // The key groups' sums meet in shared memory: one of two hands them to the other, four to all of them, a quarter of the columns each.
       if constexpr (KG > 1) {
-        float2* s_stat = reinterpret_cast<float2*>(s_join + (RG == 1 ? 4 : 1) * ROWS * C::PAD);
         const int mine = RG == 1 ? kg * ROWS : 0;
         if (!mbar_wait(&joined[1], jph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 25)) return;      // (the last segment's have been read)
         if (RG == 1 || kg == 1) {
@@ -636,36 +672,15 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
             }
           }
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&joined[0]);
-        if (!mbar_wait(&joined[0], jph, abort_flag, a.status, ST_ATTN_TIMEOUT, 26)) return;
-        jph ^= 1;
         if constexpr (RG == 1) {
-          constexpr int CPW = HD / 4, STEP = 32 / CPW;               // columns of a warp, rows at a time
-          const int col = warp * CPW + lane % CPW;
-#pragma unroll 2
-          for (int r = lane / CPW; r < seg.rows; r += STEP) {
-            float2 y[4];
-            float top = -INFINITY, l = 0.f, sum = 0.f;
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-              y[k] = s_stat[k * ROWS + r];
-              top = fmaxf(top, y[k].x);
-            }
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-              const float w = y[k].x == -INFINITY ? (y[k].y == 0.f ? 0.f : 1.f) : exp2f(y[k].x - top);   // (scores of NaN leave no maximum, but a sum)
-              l += y[k].y * w;
-              sum += s_join[(k * ROWS + r) * C::PAD + col] * w;
-            }
-            const long long row = dst_of[r];
-            if (col < a.D) {
-              if (seg.direct) ((T*)a.out)[row * a.D + col] = (T)(sees_of[r] && l != 0.f ? sum * __frcp_rn(l) : 0.f);
-              else a.part[row * a.D + col] = sum;
-            }
-            if (!seg.direct && col == 0) a.stat[row] = make_float2(top, l);
-          }
-        } else if (kg == 0) {
+          if (!join_rows(seg, 0)) return;
+        } else {
+          // of two key groups one hands its sums to the other
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&joined[0]);
+          if (!mbar_wait(&joined[0], jph, abort_flag, a.status, ST_ATTN_TIMEOUT, 26)) return;
+          jph ^= 1;
+          if (kg == 0) {
 #pragma unroll
           for (int half = 0; half < 2; half++) {
             const int r = half ? r1 : r0;
@@ -686,9 +701,10 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
               }
             }
           }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&joined[1]);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&joined[1]);
       }
       if (RG > 1 && kg == 0) {
 #pragma unroll
@@ -715,22 +731,15 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         }
       }
     } else {
-      // fp32: a warp's four rows over all keys of a tile.  Scores: a lane is a key; products with the values: a lane is HD / 32 columns.
-      static_assert(RG == 1, "16 rows");
-      constexpr int CPL = HD / 32;
+      // fp32: a warp's quarter of the keys of a tile for all rows.  Scores: LPK lanes share a key, every LPK-th chunk of its columns each; products with
+      // the values: a lane is HD / 32 columns.
+      constexpr int KW = TILE / 4, LPK = 32 / KW, CPL = HD / 32;
       const uint8_t* q = s_q + sg * C::Q_BYTES;
-      float* s_p = s_join + warp * (4 * 32);                         // [32 keys][4] of this warp
-      int sees[4];
-      bool any = false;
+      float* s_p = reinterpret_cast<float*>((uint8_t*)s_join + C::JOIN) + warp * (KW * ROWS);      // [KW][ROWS] of this warp
+      const int mykey = lane / LPK, slice = lane % LPK;
+      float o[ROWS][CPL], m[ROWS], l[ROWS];
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        sees[r] = sees_of[warp * 4 + r];
-        any |= sees[r] > 0;
-        sees[r] = sees[r] ? sees[r] : 0x7fffffff;
-      }
-      float o[4][CPL], m[4], l[4];
-#pragma unroll
-      for (int r = 0; r < 4; r++) {
+      for (int r = 0; r < ROWS; r++) {
         m[r] = -INFINITY;
         l[r] = 0.f;
 #pragma unroll
@@ -738,33 +747,35 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       }
       for (int i = 0; i < seg.tiles; i++) {
         if (!mbar_wait(&full[st], ph, abort_flag, a.status, ST_ATTN_TIMEOUT, 22)) return;
-        if (any) {
+        const int key0 = seg.key0 + i * TILE + warp * KW, there = min(KW, seg.end - key0);
+        if (there > 0) {
           const uint8_t* kt = s_k + st * SUB;
           const uint8_t* vt = s_v + st * SUB;
-          const int key0 = seg.key0 + i * TILE;
-          if (TMA && seg.end - key0 < TILE) clear_rows<TILE, C::CHUNKS>(s_v + st * SUB, seg.end - key0, TILE, lane);
-#pragma unroll 1
-          for (int j0 = 0; j0 < min(TILE, seg.end - key0); j0 += 32) {   // 32 keys at a time
-          const int key = key0 + j0 + lane;
-          float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-          for (int c = 0; c < HD / 4; c++) {
-            const float4 kk = *reinterpret_cast<const float4*>(kt + chunk_at<TILE>(j0 + lane, c));
+          const int key = key0 + mykey;
+          float s[ROWS];
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-              const float4 qq = *reinterpret_cast<const float4*>(q + chunk_at<ROWS>(warp * 4 + r, c));
+          for (int r = 0; r < ROWS; r++) s[r] = 0.f;
+#pragma unroll 2
+          for (int c = slice; c < HD / 4; c += LPK) {
+            const float4 kk = *reinterpret_cast<const float4*>(kt + chunk_at<TILE>(warp * KW + mykey, c));
+#pragma unroll
+            for (int r = 0; r < ROWS; r++) {
+              const float4 qq = *reinterpret_cast<const float4*>(q + chunk_at<ROWS>(r, c));
               s[r] = fmaf(qq.x, kk.x, s[r]);
               s[r] = fmaf(qq.y, kk.y, s[r]);
               s[r] = fmaf(qq.z, kk.z, s[r]);
               s[r] = fmaf(qq.w, kk.w, s[r]);
             }
           }
-          float4 p4;
-          float* p = &p4.x;
 #pragma unroll
-          for (int r = 0; r < 4; r++) {
-            const float x = key < min(sees[r], seg.end) ? s[r] * a.scale_log2 : -INFINITY;
-            const float top = fmaxf(m[r], warp_max(x));
+          for (int r = 0; r < ROWS; r++) {
+#pragma unroll
+            for (int d = 1; d < LPK; d <<= 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], d);
+            const int sees = s_sees[sg * ROWS + r];
+            const float x = key < min(sees ? sees : 0x7fffffff, seg.end) ? s[r] * a.scale_log2 : -INFINITY;
+            float top = x;
+#pragma unroll
+            for (int d = LPK; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             if (top > m[r]) {
               const float f = m[r] == -INFINITY ? 0.f : exp2f(m[r] - top);
               m[r] = top;
@@ -772,27 +783,30 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 #pragma unroll
               for (int c = 0; c < CPL; c++) o[r][c] *= f;
             }
-            p[r] = exp2f(x - (m[r] == -INFINITY ? 0.f : m[r]));
-            l[r] += p[r];                                            // this lane's keys; summed over lanes at the end
+            s[r] = exp2f(x - (m[r] == -INFINITY ? 0.f : m[r]));
+            l[r] += slice == 0 ? s[r] : 0.f;                         // this lane's keys; summed over lanes at the end
+          }
+          if (slice == 0) {
+#pragma unroll
+            for (int r = 0; r < ROWS; r += 4) *reinterpret_cast<float4*>(s_p + mykey * ROWS + r) = make_float4(s[r], s[r + 1], s[r + 2], s[r + 3]);
           }
           __syncwarp();
-          *reinterpret_cast<float4*>(s_p + lane * 4) = p4;
-          __syncwarp();
-#pragma unroll 4
-          for (int j = 0; j < 32; j++) {
-            const float4 pj = *reinterpret_cast<const float4*>(s_p + j * 4);
+          for (int j = 0; j < there; j++) {                          // (rows of V behind the last key are not read)
             float v[CPL];
-            const uint8_t* vr = vt + chunk_at<TILE>(j0 + j, lane * CPL / 4);
+            const uint8_t* vr = vt + chunk_at<TILE>(warp * KW + j, lane * CPL / 4);
             if constexpr (CPL == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(vr);
             else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(vr + (lane & 1) * 8);
 #pragma unroll
-            for (int c = 0; c < CPL; c++) {
-              o[0][c] = fmaf(pj.x, v[c], o[0][c]);
-              o[1][c] = fmaf(pj.y, v[c], o[1][c]);
-              o[2][c] = fmaf(pj.z, v[c], o[2][c]);
-              o[3][c] = fmaf(pj.w, v[c], o[3][c]);
+            for (int r = 0; r < ROWS; r += 4) {
+              const float4 p = *reinterpret_cast<const float4*>(s_p + j * ROWS + r);
+#pragma unroll
+              for (int c = 0; c < CPL; c++) {
+                o[r][c] = fmaf(p.x, v[c], o[r][c]);
+                o[r + 1][c] = fmaf(p.y, v[c], o[r + 1][c]);
+                o[r + 2][c] = fmaf(p.z, v[c], o[r + 2][c]);
+                o[r + 3][c] = fmaf(p.w, v[c], o[r + 3][c]);
+              }
             }
-          }
           }
         }
         __syncwarp();
@@ -800,19 +814,17 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         if (++st == STAGES) { st = 0; ph ^= 1; }
       }
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const float sum = warp_sum(l[r]);
-        const int col = lane * CPL, rr = warp * 4 + r;
-        if (rr < seg.rows) {
-          const long long row = dst_of[rr];
-          const float f = seg.direct ? (sees_of[rr] && sum != 0.f ? __frcp_rn(sum) : 0.f) : 1.f;
-          float* to = (seg.direct ? (float*)a.out : a.part) + row * a.D + col;
-          if (col < a.D) {
+      for (int from = 0; from < ROWS; from += C::RJ) {
+        if (!mbar_wait(&joined[1], jph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 25)) return;      // (the last rows have been read)
 #pragma unroll
-            for (int c = 0; c < CPL; c++) to[c] = f == 0.f ? 0.f : o[r][c] * f;
-          }
-          if (!seg.direct && lane == 0) a.stat[row] = make_float2(m[r], sum);
+        for (int r = 0; r < C::RJ; r++) {
+          const float sum = warp_sum(l[from + r]);
+          float* to = s_join + (warp * C::RJ + r) * C::PAD + lane * CPL;
+#pragma unroll
+          for (int c = 0; c < CPL; c++) to[c] = o[from + r][c];
+          if (lane == 0) s_stat[warp * C::RJ + r] = make_float2(m[from + r], sum);
         }
+        if (!join_rows(seg, from)) return;
       }
     }
     __syncwarp();
@@ -1326,7 +1338,7 @@ bool plan(Sizes& z, int dtype, long long B, long long T, long long H, long long 
     if (z.wide_prefix && z.splits > prefix / 256) z.splits = prefix / 256 < 1 ? 1 : prefix / 256;
   }
   const long long most = shared && !z.wide_prefix ? all : own;
-  z.rows = dtype == 2 || most <= 16 ? 16 : most <= 32 ? 32 : 64;
+  z.rows = dtype == 2 ? (most <= 4 ? 4 : 16) : most <= 16 ? 16 : most <= 32 ? 32 : 64;
   const long long ot = z.wide_own ? 0 : (own + z.rows - 1) / z.rows, pt = shared && !z.wide_prefix ? (all + z.rows - 1) / z.rows : 0;
   z.entries = pt + B * ot;
   if (z.entries * Hkv >= 0x7fffffffLL) return false;
@@ -1408,6 +1420,7 @@ int launch_type(const CUtensorMap& k, const CUtensorMap& v, CacheArgs& a, int ro
       return rows == 16 ? launch_attn<T, 64, 1, TMA>(k, v, a, s) : rows == 32 ? launch_attn<T, 64, 2, TMA>(k, v, a, s) : launch_attn<T, 64, 4, TMA>(k, v, a, s);
     return rows == 16 ? launch_attn<T, 128, 1, TMA>(k, v, a, s) : rows == 32 ? launch_attn<T, 128, 2, TMA>(k, v, a, s) : launch_attn<T, 128, 4, TMA>(k, v, a, s);
   } else {
+    if (rows == 4) return a.D <= 64 ? launch_attn<T, 64, 0, TMA>(k, v, a, s) : launch_attn<T, 128, 0, TMA>(k, v, a, s);
     return a.D <= 64 ? launch_attn<T, 64, 1, TMA>(k, v, a, s) : launch_attn<T, 128, 1, TMA>(k, v, a, s);
   }
 }
