@@ -11,6 +11,9 @@
 // lengths.  A (sequence, head) whose tiles fall to several CTAs leaves partial rows (m, l, o) behind, which a second kernel joins in
 // the list's order; no atomics.
 //
+// Where few (sequence, head) pairs have short tables, a cluster of up to eight CTAs takes each of them, and their sums meet in distributed shared
+// memory instead: no second kernel, which is half of such a call's time.
+//
 // A shared prefix is one more entry at the head of the list whose rows are the queries of all sequences: its keys are read once for
 // every 16, 32 or 64 rows.  The sequences' own entries then start behind it, and all rows are joined by the second kernel.
 //
@@ -19,6 +22,7 @@
 // 16 bytes a lane, a page looked up for every key.  What stands behind a sequence's last key in its last page may be anything, NaN
 // too: those scores are masked, and those rows of V become zeros in shared memory.
 #include "common.cuh"
+#include "pair.cuh"
 
 #include <string.h>
 
@@ -30,6 +34,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kConsumers = 4, kCopiers = 4;      // warps
+constexpr int kPeers = 8;                        // most CTAs of a cluster
 
 struct CacheArgs {
   const void* q;
@@ -51,6 +56,7 @@ struct CacheArgs {
   float* part;                             // [slots][rows of a tile][D] unscaled sums
   float2* stat;                            // [slots][rows of a tile] (m, l)
   int box;                                 // rows of a TMA box
+  int peers;                               // CTAs of a cluster, 0: the list is dealt out
   int shared;                              // a prefix is joined to the sequences' own keys
   int wide_prefix, wide_own;               // which of them the kernel for many rows takes
   int wide_tiles, splits;                  // its row tiles, of a sequence or of the prefix; runs of keys
@@ -70,26 +76,28 @@ template <> struct Elem<__half> {
 };
 template <> struct Elem<float> { static constexpr bool kMma = false; };
 
-// Rows of a tile: 16 RG, or 4 (RG = 0, fp32).  Row groups of 16 rows times key groups of a quarter, a half or all of the keys are the four
+// Rows of a tile: 16 RG in 16 bits, 4, 16 or 8 (RG = 0, 1, 2) in fp32.  Row groups of 16 rows times key groups of a quarter, a half or all of the keys are the four
 // warps of the 16-bit kernel; in fp32 a warp takes a quarter of the keys and all rows.  Two CTAs to an SM: while one waits, joins or stores, the other multiplies.
 template <typename T, int HD_, int RG_, bool TMA>
 struct Cfg {
   static constexpr int HD = HD_, RG = RG_;
   static constexpr bool kMma = Elem<T>::kMma;
-  static constexpr int ROWS = RG ? 16 * RG : 4;
+  static constexpr int ROWS = kMma ? 16 * RG : RG == 0 ? 4 : RG == 1 ? 16 : 8;
   static constexpr int TILE = kMma ? (HD == 64 ? 128 : 64) : HD == 64 ? 64 : 32;      // 16 KB of keys
   static constexpr int KG = kMma ? 4 / (RG ? RG : 1) : 4;
   static constexpr int SUB = TILE * HD * (int)sizeof(T);          // one K or V tile
   static constexpr int STAGES = 2;
-  static constexpr int SEGS = RG <= 1 && TMA && ROWS * HD * (int)sizeof(T) <= 4096 ? 3 : 2;           // segments (queries, rows) on their way
+  static constexpr int SEGS = ROWS * HD * (int)sizeof(T) <= 4096 ? 3 : 2;           // segments (queries, rows) on their way
   static constexpr int Q_BYTES = ROWS * HD * (int)sizeof(T);
   static constexpr int CHUNKS = HD * (int)sizeof(T) / 16;         // 16-byte chunks of a row
   static constexpr int COLS = HD * (int)sizeof(T) / 128;          // columns of 128 bytes
   static constexpr int PAD = HD + 8;                              // floats of a row of sums: eight rows' columns in different banks
-  static constexpr int RJ = ROWS < 16 || kMma ? ROWS : 8;         // rows whose four sums are joined at a time
+  static constexpr int RJ = ROWS < 8 ? ROWS : 8;                  // rows whose four sums are joined at a time
   static constexpr int JOIN = (KG == 4 ? 4 * RJ : KG == 2 ? ROWS : 0) * (PAD * 4 + 8);      // of two key groups one hands its sums to the other
   static constexpr int WEIGHTS = kMma ? 0 : TILE * ROWS * 4;      // fp32: the weights of a tile
-  static constexpr int SMEM = 2 * STAGES * SUB + SEGS * Q_BYTES + JOIN + WEIGHTS + 1024 + SEGS * (ROWS * 12 + 32) + ROWS * 8 + 256 + (TMA ? 0 : 2 * TILE * 8);
+  static constexpr int PEERS = KG == 4 ? kPeers * ROWS * 8 : 0;   // statistics of a cluster's CTAs; their sums lie in the second buffer for queries
+  static_assert(KG < 4 || (SEGS - 1) * Q_BYTES >= ROWS * HD * 4, "sums of a cluster");
+  static constexpr int SMEM = 2 * STAGES * SUB + SEGS * Q_BYTES + JOIN + WEIGHTS + PEERS + 1024 + SEGS * (ROWS * 12 + 32) + ROWS * 8 + 256 + (TMA ? 0 : 2 * TILE * 8);
   static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs to an SM");
 };
 
@@ -151,7 +159,7 @@ struct Shares {
   }
 };
 
-// A CTA's place in the list, held by the warp that copies.
+// A CTA's place in the list, held by the warps that copy.
 template <int ROWS, int TILE>
 struct Cursor {
   Shares shares;
@@ -209,6 +217,16 @@ struct Cursor {
     x.end = __shfl_sync(0xffffffffu, x.end, owner);
     x.tiles = __shfl_sync(0xffffffffu, x.tiles, owner);
     tile = first - segment0;
+  }
+  // The share of a CTA whose cluster has one entry and key head for itself.
+  __device__ __forceinline__ void start_cluster(const CacheArgs& a, int peers, int rank) {
+    const int seg = blockIdx.x / peers;
+    e = seg / a.Hkv;
+    h = seg - e * a.Hkv;
+    x = entry_of<ROWS, TILE>(a, e);
+    if (x.cut && rank == 0 && threadIdx.x == 32 * kConsumers) set_status(a.status, ST_BAD_INDEX, x.b);
+    tile = x.tiles * rank / peers;
+    left = x.tiles * (rank + 1) / peers - tile;
   }
   __device__ __forceinline__ void next_segment(const CacheArgs& a) {
     segment0 += x.tiles;
@@ -304,14 +322,33 @@ __device__ __forceinline__ Row row_of(const CacheArgs& a, const Entry& x, int r)
   return w;
 }
 
-// What the copying warp hands to the others with a segment (the tiles of one entry and key head that fall to this CTA).
+__device__ __forceinline__ uint32_t peer_address(uint32_t smem, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void st_peer(uint32_t at, float x, float y) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(x), "f"(y) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void load_floats(float* v, const float* from) {
+  if constexpr (N == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(from);
+  else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(from);
+}
+template <int N>
+__device__ __forceinline__ void store_floats(float* to, const float* v) {
+  if constexpr (N == 4) *reinterpret_cast<float4*>(to) = *reinterpret_cast<const float4*>(v);
+  else *reinterpret_cast<float2*>(to) = *reinterpret_cast<const float2*>(v);
+}
+
+// What the copying warps hand to the others with a segment (the tiles of one entry and key head that fall to this CTA).
 struct Segment {
   int tiles, key0, end;      // 0 tiles: no more segments; the first tile's first key; the entry's end of keys
   int rows;                  // rows that there are
   int direct;                // rows go to the output, else to partial rows
 };
 
-template <typename T, int HD, int RG, bool TMA>
+template <typename T, int HD, int RG, bool TMA, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, 2)
 cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const CacheArgs a) {
   using C = Cfg<T, HD, RG, TMA>;
@@ -322,7 +359,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   uint8_t* s_v = s_k + STAGES * SUB;
   uint8_t* s_q = s_v + STAGES * SUB;
   float* s_join = reinterpret_cast<float*>(s_q + SEGS * C::Q_BYTES);
-  long long* s_dst = reinterpret_cast<long long*>((uint8_t*)s_join + C::JOIN + C::WEIGHTS);       // [SEGS][ROWS] where a row goes
+  long long* s_dst = reinterpret_cast<long long*>((uint8_t*)s_join + C::JOIN + C::WEIGHTS + C::PEERS);       // [SEGS][ROWS] where a row goes
   long long* s_from = s_dst + SEGS * ROWS;                                           // [ROWS] where a row's query is, for the copying warp
   long long* s_off = s_from + ROWS;                                                  // where the keys and values of a tile start (cp.async)
   int* s_sees = reinterpret_cast<int*>(s_off + (TMA ? 0 : 2 * TILE));                          // [SEGS][ROWS] keys that a row sees, 0: it does not count
@@ -349,17 +386,26 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     *abort_flag = 0;
     mbar_fence_init();
   }
-  __syncthreads();
+  // Sums and statistics of the cluster's CTAs, for the columns that this one joins.
+  const int peers = CLUSTER ? a.peers : 1, rank = CLUSTER ? (int)cluster_ctarank() : 0, slice = HD / peers;
+  float* x_sum = reinterpret_cast<float*>(s_q + C::Q_BYTES);                         // [peers][ROWS][slice]
+  float2* x_stat = reinterpret_cast<float2*>((uint8_t*)s_join + C::JOIN + C::WEIGHTS);      // [peers][ROWS]
+  if constexpr (CLUSTER) {
+    for (int i = threadIdx.x; i < kPeers * ROWS; i += kThreads) x_stat[i] = make_float2(-INFINITY, 0.f);
+    cluster_sync_all();                          // all of them are there before one writes to another
+  } else {
+    __syncthreads();
+  }
   pdl_wait();
   pdl_trigger();
 
   // Registers: 128 a thread at launch, of which the copying warps hand 64 to those that multiply.
-  if (warp >= kConsumers) {
-    // ---------------- copies ----------------
+  auto copies = [&]() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     const int me = warp - kConsumers;
     Cursor<ROWS, TILE> at;
-    at.start(a, lane);
+    if constexpr (CLUSTER) at.start_cluster(a, peers, rank);
+    else at.start(a, lane);
     constexpr int MINE = TILE / kCopiers;                            // keys of this warp for cp.async
     constexpr int PER = 32 / C::CHUNKS;                              // rows of one instruction of the warp
     const int sub = lane / C::CHUNKS, chunk = lane % C::CHUNKS;
@@ -435,18 +481,17 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     };
     bool first_segment = true;
     const int per = a.T * a.G;
-    while (at.left) {
-      // The first tile is on its way before the segment is described: where its rows go, its queries.
+    while (CLUSTER || at.left) {
+      // While the pages of the first tile are looked up, the segment is described: where its rows go; its queries are copied behind that tile.
       const int n = (int)min(at.left, (unsigned)(at.x.tiles - at.tile)), tile0 = at.tile;
-      look_up();
-      if (!copy_tile(n > 1)) break;
+      if (n > 0) look_up();
       if (!mbar_wait(&seg_empty[sg], sph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 23)) break;
       const bool whole = n == at.x.tiles, direct = whole && !a.shared;
       const int slot = 2 * blockIdx.x + (first_segment ? 0 : 1);
       const int rows = min(ROWS, (at.x.b < 0 ? a.B * per : per) - at.x.row0);
       if (lane == 0 && me == 0) {
         s_seg[sg] = Segment{n, at.x.begin + tile0 * TILE, at.x.end, rows, direct};
-        if (tile0 == 0) a.owner[at.e * a.Hkv + at.h] = make_int2(slot, (int)at.shares.cta_of(at.segment0 + at.x.tiles - 1));
+        if (!CLUSTER && tile0 == 0) a.owner[at.e * a.Hkv + at.h] = make_int2(slot, (int)at.shares.cta_of(at.segment0 + at.x.tiles - 1));
       }
       // Whole segments of a batch with a shared prefix leave partial rows too: in the output's order, those of the prefix behind the sequences'.
       // The warps take a quarter of the rows each.
@@ -457,11 +502,12 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         const Row w = row_of(a, at.x, r);
         const long long row = ((long long)w.b * a.T + w.t) * a.H + at.h * a.G + w.g;
         s_sees[sg * ROWS + r] = w.counts ? max(w.sees, 0) : 0;
-        s_dst[sg * ROWS + r] = direct ? row : !whole ? (long long)slot * ROWS + r
-                                            : 2LL * a.ctas * ROWS + (at.x.b < 0 ? (long long)a.B * a.T * a.H : 0) + row;
+        s_dst[sg * ROWS + r] = CLUSTER || direct ? row : !whole ? (long long)slot * ROWS + r
+                                                      : 2LL * a.ctas * ROWS + (at.x.b < 0 ? (long long)a.B * a.T * a.H : 0) + row;
         s_from[r] = w.counts ? w.b * a.q_sb + w.t * a.q_st + (long long)(at.h * a.G + w.g) * a.q_sh : -1;
       }
       __syncwarp();
+      if (n > 0 && !copy_tile(n > 1)) break;
       uint8_t* dq = s_q + sg * C::Q_BYTES;
 #pragma unroll 4
       for (int r0 = me * RW; r0 < min(rows, me * RW + RW); r0 += PER) {      // (rows behind the last one: anything, nothing comes of them)
@@ -478,54 +524,77 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       at.left -= n;
       bool ok = true;
       for (int i = 1; i < n && ok; i++) ok = copy_tile(i + 1 < n);
-      if (!ok) break;
+      if (!ok || CLUSTER) break;
       if (at.left) at.next_segment(a);
     }
-    if (at.left == 0 && mbar_wait(&seg_empty[sg], sph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 23)) {
+    if (!CLUSTER && at.left == 0 && mbar_wait(&seg_empty[sg], sph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 23)) {
       if (lane == 0 && me == 0) s_seg[sg] = Segment{0, 0, 0, 0, 0};  // no more
       __syncwarp();
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&seg_full[sg])) : "memory");
       if (lane == 0) mbar_arrive(&seg_full[sg]);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-    return;
-  }
+  };
 
-  // ---------------- products ----------------
+  auto products = [&]() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
   int st = 0, sg = 0;
   uint32_t ph = 0, sph = 0, jph = 0;
   const int rg = warp / KG, kg = warp % KG;
   float2* s_stat = reinterpret_cast<float2*>(s_join + (KG == 4 ? 4 * C::RJ : KG == 2 ? ROWS : 0) * C::PAD);
-  // Four key groups' sums of the rows from..from + RJ - 1 meet in shared memory; a warp joins a quarter of the columns.
+  // Four key groups' sums of the rows from..from + RJ - 1 meet in shared memory; a warp joins every fourth row.
   auto join_rows = [&](const Segment& seg, int from) {
     __syncwarp();
     if (lane == 0) mbar_arrive(&joined[0]);
     if (!mbar_wait(&joined[0], jph, abort_flag, a.status, ST_ATTN_TIMEOUT, 26)) return false;
     jph ^= 1;
-    constexpr int CPW = HD / 4, STEP = 32 / CPW;                     // columns of a warp, rows at a time
-    const int col = warp * CPW + lane % CPW;
-#pragma unroll 2
-    for (int r = lane / CPW; r < min(C::RJ, seg.rows - from); r += STEP) {
-      float2 y[4];
-      float top = -INFINITY, l = 0.f, sum = 0.f;
+    constexpr int CPL = HD / 32;                                     // columns of a lane
+    const int col = lane * CPL;
+#pragma unroll
+    for (int i = 0; i < C::RJ / 4; i++) {
+      const int r = i * 4 + warp;
+      if (r >= seg.rows - from) break;
+      float w[4], top = -INFINITY, l = 0.f, sum[CPL];
+#pragma unroll
+      for (int k = 0; k < 4; k++) top = fmaxf(top, s_stat[k * C::RJ + r].x);
+#pragma unroll
+      for (int c = 0; c < CPL; c++) sum[c] = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; k++) {
-        y[k] = s_stat[k * C::RJ + r];
-        top = fmaxf(top, y[k].x);
-      }
+        const float2 y = s_stat[k * C::RJ + r];
+        w[k] = y.x == -INFINITY ? (y.y == 0.f ? 0.f : 1.f) : exp2f(y.x - top);     // (scores of NaN leave no maximum, but a sum)
+        l += y.y * w[k];
+        float v[CPL];
+        load_floats<CPL>(v, s_join + (k * C::RJ + r) * C::PAD + col);
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const float w = y[k].x == -INFINITY ? (y[k].y == 0.f ? 0.f : 1.f) : exp2f(y[k].x - top);   // (scores of NaN leave no maximum, but a sum)
-        l += y[k].y * w;
-        sum += s_join[(k * C::RJ + r) * C::PAD + col] * w;
+        for (int c = 0; c < CPL; c++) sum[c] += v[c] * w[k];
       }
-      const long long row = s_dst[sg * ROWS + from + r];
-      if (col < a.D) {
-        if (seg.direct) ((T*)a.out)[row * a.D + col] = (T)(s_sees[sg * ROWS + from + r] && l != 0.f ? sum * __frcp_rn(l) : 0.f);
-        else a.part[row * a.D + col] = sum;
+      if constexpr (CLUSTER) {
+        const int to = col / slice, at = col - to * slice;
+        const uint32_t p = peer_address(smem_u32(x_sum + (rank * ROWS + from + r) * slice + at), to);
+#pragma unroll
+        for (int c = 0; c < CPL; c += 2) st_peer(p + 4 * c, sum[c], sum[c + 1]);
+        if (at == 0) st_peer(peer_address(smem_u32(x_stat + rank * ROWS + from + r), to), top, l);
+      } else {
+        const long long row = s_dst[sg * ROWS + from + r];
+        const bool counts = s_sees[sg * ROWS + from + r] && l != 0.f;
+        if (col < a.D) {
+          if (!seg.direct) {
+            store_floats<CPL>(a.part + row * a.D + col, sum);
+          } else {
+            const float f = counts ? __frcp_rn(l) : 0.f;
+#pragma unroll
+            for (int c = 0; c < CPL; c++) sum[c] = counts ? sum[c] * f : 0.f;
+            if constexpr (C::kMma) {
+#pragma unroll
+              for (int c = 0; c < CPL; c += 2) *reinterpret_cast<uint32_t*>((T*)a.out + row * a.D + col + c) = Elem<T>::pack(sum[c], sum[c + 1]);
+            } else {
+              store_floats<CPL>((float*)a.out + row * a.D + col, sum);
+            }
+          }
+        }
+        if (!seg.direct && lane == 0) a.stat[row] = make_float2(top, l);
       }
-      if (!seg.direct && col == 0) a.stat[row] = make_float2(top, l);
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&joined[1]);
@@ -534,7 +603,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   for (;;) {
     if (!mbar_wait(&seg_full[sg], sph, abort_flag, a.status, ST_ATTN_TIMEOUT, 24)) return;
     const Segment seg = s_seg[sg];
-    if (seg.tiles == 0) return;
+    if (seg.tiles == 0) return;                  // no more; of a cluster, none for this CTA
     const int* sees_of = s_sees + sg * ROWS;
     const long long* dst_of = s_dst + sg * ROWS;
 
@@ -658,24 +727,31 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         l1 += __shfl_xor_sync(0xffffffffu, l1, d);
       }
       if constexpr (KG > 1) {
-        const int mine = RG == 1 ? kg * ROWS : 0;
-        if (!mbar_wait(&joined[1], jph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 25)) return;      // (the last segment's have been read)
-        if (RG == 1 || kg == 1) {
+        auto hand_over = [&](int half, int to_row) {
+          const int r = half ? r1 : r0;
+          if (r < seg.rows) {
+            float* to = s_join + to_row * C::PAD + (lane & 3) * 2;
+#pragma unroll
+            for (int j = 0; j < HD / 8; j++) *reinterpret_cast<float2*>(to + j * 8) = make_float2(o[j][2 * half], o[j][2 * half + 1]);
+            if ((lane & 3) == 0) s_stat[to_row] = half ? make_float2(m1, l1) : make_float2(m0, l0);
+          }
+        };
+        if constexpr (RG == 1) {
+          static_assert(C::RJ == 8, "a half of a warp's rows");
 #pragma unroll
           for (int half = 0; half < 2; half++) {
-            const int r = half ? r1 : r0;
-            if (r < seg.rows) {
-              float* to = s_join + (mine + r) * C::PAD + (lane & 3) * 2;
-#pragma unroll
-              for (int j = 0; j < HD / 8; j++) *reinterpret_cast<float2*>(to + j * 8) = make_float2(o[j][2 * half], o[j][2 * half + 1]);
-              if ((lane & 3) == 0) s_stat[mine + r] = half ? make_float2(m1, l1) : make_float2(m0, l0);
-            }
+            if (half && seg.rows <= 8) break;
+            if (!mbar_wait(&joined[1], jph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 25)) return;      // (the last rows have been read)
+            hand_over(half, kg * 8 + (lane >> 2));
+            if (!join_rows(seg, half * 8)) return;
           }
-        }
-        if constexpr (RG == 1) {
-          if (!join_rows(seg, 0)) return;
         } else {
           // of two key groups one hands its sums to the other
+          if (!mbar_wait(&joined[1], jph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 25)) return;
+          if (kg == 1) {
+            hand_over(0, r0);
+            hand_over(1, r1);
+          }
           __syncwarp();
           if (lane == 0) mbar_arrive(&joined[0]);
           if (!mbar_wait(&joined[0], jph, abort_flag, a.status, ST_ATTN_TIMEOUT, 26)) return;
@@ -815,6 +891,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       }
 #pragma unroll
       for (int from = 0; from < ROWS; from += C::RJ) {
+        if (from >= seg.rows) break;
         if (!mbar_wait(&joined[1], jph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 25)) return;      // (the last rows have been read)
 #pragma unroll
         for (int r = 0; r < C::RJ; r++) {
@@ -827,9 +904,35 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         if (!join_rows(seg, from)) return;
       }
     }
+    if constexpr (CLUSTER) return;
     __syncwarp();
     if (lane == 0) mbar_arrive(&seg_empty[sg]);
     if (++sg == SEGS) { sg = 0; sph ^= 1; }
+  }
+  };
+
+  if (warp >= kConsumers) copies();
+  else products();
+  if constexpr (CLUSTER) {
+    __syncwarp();
+    cluster_sync_all();                          // (every wait before it ends, and none reads or writes another's memory behind it)
+    if (warp < kConsumers && !*abort_flag) {
+      const int rows = s_seg[0].rows;
+      for (int i = threadIdx.x; i < rows * slice; i += 32 * kConsumers) {
+        const int r = i / slice, col = i - r * slice;
+        float top = -INFINITY, l = 0.f, sum = 0.f;
+        for (int p = 0; p < peers; p++) top = fmaxf(top, x_stat[p * ROWS + r].x);
+        for (int p = 0; p < peers; p++) {
+          const float2 y = x_stat[p * ROWS + r];
+          if (y.x == -INFINITY && y.y == 0.f) continue;                              // (of a CTA without keys)
+          const float w = y.x == -INFINITY ? 1.f : exp2f(y.x - top);
+          l += y.y * w;
+          sum += x_sum[(p * ROWS + r) * slice + col] * w;
+        }
+        const int to = rank * slice + col;
+        if (to < a.D) ((T*)a.out)[s_dst[r] * a.D + to] = (T)(s_sees[r] && l != 0.f ? sum * __frcp_rn(l) : 0.f);
+      }
+    }
   }
 }
 
@@ -1223,16 +1326,19 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   }
 }
 
-// Joins the partial rows of a query row: those of the prefix and those of its own sequence, each in the order of the keys.  A warp a row, a
-// lane four columns.  First the statistics, a part a lane, so that they are one wait and not one for each part; then the sums with their
-// weights, eight parts on their way at a time.  Rows that the first kernel has written are left alone; rows that see nothing become zeros.
-template <typename T, int ROWS, int TILE>
+// Joins the partial rows of a query row: those of the prefix and those of its own sequence.  WPR warps a row, a lane four columns.  First the
+// statistics, a part a lane, so that they are one wait and not one for each part; then the sums with their weights, eight parts on their
+// way at a time.  With eight warps to a row, every eighth part is a warp's, and they meet in shared memory: where rows are few and parts many,
+// which a warp alone would wait for by eights.  Rows that the first kernel has written are left alone; rows that see nothing become zeros.
+template <typename T, int ROWS, int TILE, int WPR>
 __global__ void __launch_bounds__(256) cache_join_kernel(const CacheArgs a) {
+  __shared__ float s_o[WPR > 1 ? 8 : 1][128];
+  __shared__ float2 s_st[8];
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const unsigned rows = (unsigned)a.B * a.T * a.H, i = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (i >= rows) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % WPR;
+  const unsigned rows = (unsigned)a.B * a.T * a.H, i = blockIdx.x * (8 / WPR) + warp / WPR;
+  if (i >= rows) return;                         // (with eight warps to a row: none)
   const unsigned bt = i / a.H;
   const int head = i - bt * a.H, h = head / a.G, g = head - h * a.G, b = bt / a.T, t = bt - b * a.T;
   T* out = (T*)a.out + (long long)i * a.D;
@@ -1265,8 +1371,8 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const CacheArgs a) {
   }
   const int n = pre.n + own.n;
   float top = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int k0 = 0; k0 < n; k0 += 32) {
-    const int k = k0 + lane;
+  for (int k0 = 0; k0 < n; k0 += 32 * WPR) {
+    const int k = k0 + lane * WPR + sub;
     long long row = 0;
     float2 st = make_float2(-INFINITY, 0.f);
     if (k < n) {
@@ -1279,7 +1385,7 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const CacheArgs a) {
     sum = sum * f + warp_sum(st.y * w);
 #pragma unroll
     for (int c = 0; c < 4; c++) o[c] *= f;
-    const int m = min(32, n - k0);
+    const int m = min(32, (n - k0 - sub + WPR - 1) / WPR);
     for (int j0 = 0; j0 < m; j0 += 8) {
       float4 v[8];
 #pragma unroll
@@ -1297,6 +1403,24 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const CacheArgs a) {
       }
     }
   }
+  if constexpr (WPR > 1) {
+    *reinterpret_cast<float4*>(&s_o[sub][4 * lane]) = make_float4(o[0], o[1], o[2], o[3]);
+    if (lane == 0) s_st[sub] = make_float2(top, sum);
+    __syncthreads();
+    if (sub) return;
+    top = -INFINITY;
+    sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < 4; c++) o[c] = 0.f;
+    for (int k = 0; k < WPR; k++) top = fmaxf(top, s_st[k].x);
+    for (int k = 0; k < WPR; k++) {
+      const float2 st = s_st[k];
+      const float w = st.x == -INFINITY ? (st.y == 0.f ? 0.f : 1.f) : exp2f(st.x - top);
+      sum += st.y * w;
+#pragma unroll
+      for (int c = 0; c < 4; c++) o[c] += s_o[k][4 * lane + c] * w;
+    }
+  }
   const float f = sum != 0.f ? __frcp_rn(sum) : 0.f;
   if (4 * lane < a.D) {
 #pragma unroll
@@ -1310,16 +1434,18 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const CacheArgs a) {
 // host side
 // ---------------------------------------------------------------------------------------------------------------------------
 constexpr int kCtas = 2 * 148;
+constexpr int kClusterTiles = 8;
+constexpr long long kFewRows = 148 * 8;          // rows that are joined by eight warps each: those CTAs all fit at a time
 
 struct Sizes {
   int rows;                      // of a tile of the kernel for few rows
   int own_tiles, prefix_tiles;
-  int wide_prefix, wide_own, wide_tiles, splits;
+  int wide_prefix, wide_own, wide_tiles, splits, peers;
   long long entries, part, stat, owner, total;      // bytes of the workspace's parts
 };
 
 // Which kernel takes what, and the workspace.
-bool plan(Sizes& z, int dtype, long long B, long long T, long long H, long long Hkv, long long D, int prefix) {
+bool plan(Sizes& z, int dtype, long long B, long long T, long long H, long long Hkv, long long D, int prefix, long long room) {
   if (B * T * H >= 0x7fffffffLL) return false;
   const long long own = T * (H / Hkv), all = B * own;
   z = Sizes{};
@@ -1338,19 +1464,28 @@ bool plan(Sizes& z, int dtype, long long B, long long T, long long H, long long 
     if (z.wide_prefix && z.splits > prefix / 256) z.splits = prefix / 256 < 1 ? 1 : prefix / 256;
   }
   const long long most = shared && !z.wide_prefix ? all : own;
-  z.rows = dtype == 2 ? (most <= 4 ? 4 : 16) : most <= 16 ? 16 : most <= 32 ? 32 : 64;
+  z.rows = dtype == 2 ? (most <= 4 ? 4 : most <= 8 ? 8 : 16) : most <= 16 ? 16 : most <= 32 ? 32 : 64;
   const long long ot = z.wide_own ? 0 : (own + z.rows - 1) / z.rows, pt = shared && !z.wide_prefix ? (all + z.rows - 1) / z.rows : 0;
   z.entries = pt + B * ot;
   if (z.entries * Hkv >= 0x7fffffffLL) return false;
   z.own_tiles = (int)ot;
   z.prefix_tiles = (int)pt;
+  // A cluster for each (sequence, row tile, key head): as many CTAs, up to eight, as leave all of them on the SMs at a time.  Where a full table
+  // would be more than kClusterTiles tiles for one of them, the list is dealt out, which balances lengths.
+  if (!shared && !z.wide_own && z.rows <= 16 && z.entries * Hkv <= kCtas) {
+    const long long tile = 16384 / ((D <= 64 ? 64 : 128) * (dtype == 2 ? 4 : 2)), tiles = (room + tile - 1) / tile;
+    z.peers = kPeers;
+    while (z.peers > 1 && z.entries * Hkv * z.peers > kCtas) z.peers >>= 1;
+    if (tiles > (long long)kClusterTiles * z.peers) z.peers = 0;
+    if (z.peers) return true;                                        // without a workspace
+  }
   const long long rows = z.wide_own ? (z.splits > 1 ? z.splits * B * T * H : 0)
                                     : 2LL * kCtas * z.rows + (shared ? B * T * H * (1 + (z.wide_prefix ? z.splits : 1)) : 0);
   auto up = [](long long n) { return (n + 255) / 256 * 256; };
   z.part = up(rows * D * 4);
   z.stat = up(rows * 8);
   z.owner = up(z.entries * Hkv * 8);
-  z.total = z.part + z.stat + z.owner + 256;
+  z.total = z.part + z.stat + z.owner;
   return true;
 }
 
@@ -1378,19 +1513,35 @@ int launch_wide(const CUtensorMap& tk, const CUtensorMap& tv, const CacheArgs& a
 template <typename T, int ROWS, int TILE>
 int launch_join(const CacheArgs& a, cudaStream_t s) {
   const long long rows = (long long)a.B * a.T * a.H;
-  GB_CUDA_OK(gbh::launch(cache_join_kernel<T, ROWS, TILE>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, 1, a));
+  // about as many parts as the CTAs are times the segments: above eight, which a warp fetches at a time
+  const bool many_parts = a.wide_own || a.wide_prefix ? a.splits > 8 : kCtas > 8LL * a.Hkv * (a.prefix_tiles + (long long)a.B * a.own_tiles);
+  if (rows <= kFewRows && many_parts) GB_CUDA_OK(gbh::launch(cache_join_kernel<T, ROWS, TILE, 8>, dim3((unsigned)rows), dim3(256), 0, s, 1, a));
+  else GB_CUDA_OK(gbh::launch(cache_join_kernel<T, ROWS, TILE, 1>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, 1, a));
   return gbh::E_OK;
+}
+
+template <typename T, int HD, int RG, bool TMA, bool CLUSTER>
+int launch_kernel(const CUtensorMap& tk, const CUtensorMap& tv, CacheArgs& a, cudaStream_t s) {
+  using C = Cfg<T, HD, RG, TMA>;
+  const auto kernel = cache_attn_kernel<T, HD, RG, TMA, CLUSTER>;
+  static std::atomic<uint32_t> done{0};
+  const int rc = allow_shared(kernel, C::SMEM, done);
+  if (rc) return rc;
+  if constexpr (CLUSTER) {
+    GB_CUDA_OK(gbh::launch(kernel, dim3((unsigned)(a.peers * a.B * a.own_tiles * a.Hkv)), dim3(kThreads), C::SMEM, s, a.peers, tk, tv, a));
+    return gbh::E_OK;
+  } else {
+    GB_CUDA_OK(gbh::launch(kernel, dim3(a.ctas), dim3(kThreads), C::SMEM, s, 1, tk, tv, a));
+    return launch_join<T, C::ROWS, C::TILE>(a, s);
+  }
 }
 
 template <typename T, int HD, int RG, bool TMA>
 int launch_attn(const CUtensorMap& tk, const CUtensorMap& tv, CacheArgs& a, cudaStream_t s) {
-  using C = Cfg<T, HD, RG, TMA>;
-  const auto kernel = cache_attn_kernel<T, HD, RG, TMA>;
-  static std::atomic<uint32_t> done{0};
-  const int rc = allow_shared(kernel, C::SMEM, done);
-  if (rc) return rc;
-  GB_CUDA_OK(gbh::launch(kernel, dim3(a.ctas), dim3(kThreads), C::SMEM, s, 1, tk, tv, a));
-  return launch_join<T, C::ROWS, C::TILE>(a, s);
+  if constexpr (Cfg<T, HD, RG, TMA>::KG == 4) {
+    if (a.peers) return launch_kernel<T, HD, RG, TMA, true>(tk, tv, a, s);
+  }
+  return launch_kernel<T, HD, RG, TMA, false>(tk, tv, a, s);
 }
 
 // (columns, rows of a page, heads, pages) in boxes of 128 bytes by `rows` rows
@@ -1421,6 +1572,7 @@ int launch_type(const CUtensorMap& k, const CUtensorMap& v, CacheArgs& a, int ro
     return rows == 16 ? launch_attn<T, 128, 1, TMA>(k, v, a, s) : rows == 32 ? launch_attn<T, 128, 2, TMA>(k, v, a, s) : launch_attn<T, 128, 4, TMA>(k, v, a, s);
   } else {
     if (rows == 4) return a.D <= 64 ? launch_attn<T, 64, 0, TMA>(k, v, a, s) : launch_attn<T, 128, 0, TMA>(k, v, a, s);
+    if (rows == 8) return a.D <= 64 ? launch_attn<T, 64, 2, TMA>(k, v, a, s) : launch_attn<T, 128, 2, TMA>(k, v, a, s);
     return a.D <= 64 ? launch_attn<T, 64, 1, TMA>(k, v, a, s) : launch_attn<T, 128, 1, TMA>(k, v, a, s);
   }
 }
@@ -1440,21 +1592,30 @@ int launch_any(const CUtensorMap& k, const CUtensorMap& v, CacheArgs& a, int row
 
 }  // namespace
 
-// Bytes of the workspace of gb_cache_attn, or a negative error.
-GB_EXPORT long long gb_cache_attn_bytes(int dtype, long long B, long long T, long long H, long long Hkv, long long D, int prefix) {
+// Bytes of the workspace of gb_cache_attn (0: none), or a negative error.  room: positions that a row of the table holds.
+GB_EXPORT long long gb_cache_attn_bytes(int dtype, long long B, long long T, long long H, long long Hkv, long long D, int prefix,
+                                        long long room) {
   Sizes z;
   if (dtype < 0 || dtype > 2 || B < 0 || T < 1 || H < 1 || Hkv < 1 || H % Hkv || D < 1 || D > 128 ||
-      !plan(z, dtype, B, T, H, Hkv, D, prefix)) {
+      !plan(z, dtype, B, T, H, Hkv, D, prefix, room)) {
     gbh::set_error("gb_cache_attn: too many rows, or bad sizes (%lld sequences, %lld tokens, %lld and %lld heads of %lld)", B, T, H, Hkv, D);
     return gbh::E_TOO_LARGE;
   }
   return z.total;
 }
 
-// out (B, T, H, D) = attention of q over the pages of its sequences.  strides: of q (batch, token, head), of both caches (page, head, row),
-// in elements; rows aligned to 16 bytes.  prefix: positions, a multiple of the page, that all sequences have in
+// Kernels that gb_cache_attn launches.
+GB_EXPORT int gb_cache_attn_kernels(int dtype, long long B, long long T, long long H, long long Hkv, long long D, int prefix, long long room) {
+  Sizes z;
+  if (B < 1 || T < 1 || H < 1 || Hkv < 1 || !plan(z, dtype, B, T, H, Hkv, D, prefix, room)) return 0;
+  return z.peers ? 1 : z.wide_own ? 1 + (z.splits > 1) : 2 + z.wide_prefix;
+}
+
+// out (B, T, H, D) = attention of q over the pages of its sequences.  Strides in elements, of q (batch, token, head) and of both caches (page,
+// head, row: strides[0..5]); rows aligned to 16 bytes.  prefix: positions, a multiple of the page, that all sequences have in
 // the pages of the first one's.  The workspace belongs to this call until its kernels have run.
-GB_EXPORT int gb_cache_attn(int dtype, const void* q, const void* k, const void* v, void* out, const long long* strides, int B, int T, int H,
+GB_EXPORT int gb_cache_attn(int dtype, const void* q, long long q_sb, long long q_st, long long q_sh, const void* k, const void* v,
+                            const long long* strides, void* out, int B, int T, int H,
                             int Hkv, int D, const void* table, long long table_stride, int columns, int pages, int page, const void* lengths,
                             const void* counts, int prefix, double scale, void* ws, long long ws_bytes, void* stream) {
   const int size = dtype == 2 ? 4 : 2;
@@ -1463,7 +1624,7 @@ GB_EXPORT int gb_cache_attn(int dtype, const void* q, const void* k, const void*
     return gbh::E_BAD_ARG;
   }
   if (B == 0 || T == 0) return gbh::E_OK;
-  if (!q || !k || !v || !out || !table || !lengths || !ws || page < 1 || columns < 1 || pages < 1) {
+  if (!q || !k || !v || !out || !table || !lengths || !strides || page < 1 || columns < 1 || pages < 1) {
     gbh::set_error("gb_cache_attn: null pointer or empty cache");
     return gbh::E_BAD_ARG;
   }
@@ -1472,16 +1633,16 @@ GB_EXPORT int gb_cache_attn(int dtype, const void* q, const void* k, const void*
     return gbh::E_BAD_ARG;
   }
   long long cache = 0;
-  for (int i = 3; i < 9; i++) cache |= strides[i];
-  if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)ws) & 15 || cache * size % 16 || (uintptr_t)q & 15 || (strides[0] | strides[1] | strides[2]) * size % 16 ||
+  for (int i = 0; i < 6; i++) cache |= strides[i];
+  if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)ws) & 15 || cache * size % 16 || (uintptr_t)q & 15 || (q_sb | q_st | q_sh) * size % 16 ||
       (uintptr_t)out & 15) {
     gbh::set_error("gb_cache_attn: misaligned tensor");
     return gbh::E_BAD_ARG;
   }
   CacheArgs a = {};
-  a.box = box_of(page, dtype, D, strides + 3);
+  a.box = box_of(page, dtype, D, strides);
   Sizes z;
-  if (!plan(z, dtype, B, T, H, Hkv, D, prefix) || ws_bytes < z.total) {
+  if (!plan(z, dtype, B, T, H, Hkv, D, prefix, (long long)columns * page) || ws_bytes < z.total || (z.total && !ws)) {
     gbh::set_error("gb_cache_attn: workspace of %lld bytes is too small, or too many rows", ws_bytes);
     return gbh::E_TOO_LARGE;
   }
@@ -1492,9 +1653,9 @@ GB_EXPORT int gb_cache_attn(int dtype, const void* q, const void* k, const void*
     return gbh::E_TOO_LARGE;
   }
   a.q = q; a.k = k; a.v = v; a.out = out;
-  a.q_sb = strides[0]; a.q_st = strides[1]; a.q_sh = strides[2];
-  a.k_sp = strides[3]; a.k_sh = strides[4]; a.k_sr = strides[5];
-  a.v_sp = strides[6]; a.v_sh = strides[7]; a.v_sr = strides[8];
+  a.q_sb = q_sb; a.q_st = q_st; a.q_sh = q_sh;
+  a.k_sp = strides[0]; a.k_sh = strides[1]; a.k_sr = strides[2];
+  a.v_sp = strides[3]; a.v_sh = strides[4]; a.v_sr = strides[5];
   a.table = (const int*)table; a.table_stride = table_stride;
   a.columns = columns; a.pages = pages; a.page = page; a.room = columns * page;
   a.lengths = (const int*)lengths; a.counts = (const int*)counts;
@@ -1505,6 +1666,7 @@ GB_EXPORT int gb_cache_attn(int dtype, const void* q, const void* k, const void*
   a.shared = prefix > 0 && !z.wide_own;
   a.wide_prefix = z.wide_prefix; a.wide_own = z.wide_own; a.wide_tiles = z.wide_tiles; a.splits = z.splits;
   a.slot_rows = z.rows;
+  a.peers = z.peers;
   a.ctas = kCtas;
   a.part = (float*)ws;
   a.stat = (float2*)((uint8_t*)ws + z.part);
@@ -1516,8 +1678,8 @@ GB_EXPORT int gb_cache_attn(int dtype, const void* q, const void* k, const void*
   memset(&tv, 0, sizeof(tv));
   if (a.box) {
     int rc;
-    if ((rc = cache_map(&tk, dtype, k, D, page, Hkv, pages, strides + 3, a.box))) return rc;
-    if ((rc = cache_map(&tv, dtype, v, D, page, Hkv, pages, strides + 6, a.box))) return rc;
+    if ((rc = cache_map(&tk, dtype, k, D, page, Hkv, pages, strides, a.box))) return rc;
+    if ((rc = cache_map(&tv, dtype, v, D, page, Hkv, pages, strides + 3, a.box))) return rc;
   }
   if (dtype == 0) return launch_any<__nv_bfloat16>(tk, tv, a, z.rows, s);
   if (dtype == 1) return launch_any<__half>(tk, tv, a, z.rows, s);

@@ -113,6 +113,54 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
     const long long i = b * a.pb + t * a.pt;
     return a.positions64 ? reinterpret_cast<const long long*>(a.positions)[i] : reinterpret_cast<const int*>(a.positions)[i];
   };
+  // A head is half / V turned items of two vectors, then items of up to two vectors of the rest.
+  const int turned = a.half / V, rest = a.width - a.dim, items = turned + (rest + 2 * V - 1) / (2 * V);
+  const int flat = (a.width + 2 * V - 1) / (2 * V);       // items of a head of values
+  const int per_token = APPEND ? (a.q.heads + a.k.heads) * items + a.v.heads * flat : a.q.heads * items;
+  struct Item {
+    int k, which, h, at, second, cs;      // token of the CTA; queries, keys, values; first columns of the two vectors; first angle, -1: copied
+    Pack<T, V> u, w;
+  };
+  auto fetch = [&](int i, Item& x) {
+    x.k = i / per_token;
+    int j = i - x.k * per_token;
+    const int token = n0 + x.k, b = token / a.tokens, t = token - b * a.tokens;
+    const Part* part = &a.q;
+    x.which = 0;
+    int width_items = items, first = turned;
+    if constexpr (APPEND) {
+      if (j >= a.q.heads * items) {
+        j -= a.q.heads * items;
+        part = &a.k;
+        x.which = 1;
+        if (j >= a.k.heads * items) {
+          j -= a.k.heads * items;
+          part = &a.v;
+          x.which = 2;
+          width_items = flat;
+          first = 0;
+        }
+      }
+    }
+    x.h = j / width_items;
+    const int item = j - x.h * width_items;
+    if (item < first) {
+      x.at = INTER ? item * 2 * V : item * V;
+      x.second = INTER ? x.at + V : x.at + a.half;
+      x.cs = item * V;
+    } else {
+      x.at = (x.which == 2 ? 0 : a.dim) + (item - first) * 2 * V;
+      x.second = x.at + V;
+      x.cs = -1;
+    }
+    const T* src = (const T*)part->src + b * part->sb + t * part->st + x.h * part->sh;
+    x.u.load(src + x.at);
+    if (x.second < a.width) x.w.load(src + x.second);
+  };
+  // The first item is on its way while the angles are computed, and each one while the one before it is turned.
+  const int total = n * per_token;
+  Item x;
+  if ((int)threadIdx.x < total) fetch(threadIdx.x, x);
   for (int i = threadIdx.x; i < n * a.half; i += kThreads) {
     const int k = i / a.half;
     bool live;
@@ -141,59 +189,27 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
     }
   }
   __syncthreads();
-  // A head is half / V turned items of two vectors, then items of up to two vectors of the rest.
-  const int turned = a.half / V, rest = a.width - a.dim, items = turned + (rest + 2 * V - 1) / (2 * V);
-  const int flat = (a.width + 2 * V - 1) / (2 * V);       // items of a head of values
-  const int per_token = APPEND ? (a.q.heads + a.k.heads) * items + a.v.heads * flat : a.q.heads * items;
-  for (int i = threadIdx.x; i < n * per_token; i += kThreads) {
-    const int k = i / per_token;
-    int j = i - k * per_token;
-    const int token = n0 + k, b = token / a.tokens, t = token - b * a.tokens;
-    const Part* part = &a.q;
-    int which = 0, width_items = items, first = turned;
-    if constexpr (APPEND) {
-      if (j >= a.q.heads * items) {
-        j -= a.q.heads * items;
-        part = &a.k;
-        which = 1;
-        if (j >= a.k.heads * items) {
-          j -= a.k.heads * items;
-          part = &a.v;
-          which = 2;
-          width_items = flat;
-          first = 0;
-        }
-      }
-    }
-    const int h = j / width_items, item = j - h * width_items;
-    const T* src = (const T*)part->src + b * part->sb + t * part->st + h * part->sh;
-    T* dst;
-    if (!APPEND || which == 0) {
-      dst = (T*)part->dst + ((long long)token * part->heads + h) * a.width;
+  for (int i = threadIdx.x; i < total; i += kThreads) {
+    Item y;
+    if (i + kThreads < total) fetch(i + kThreads, y);
+    T* dst = nullptr;
+    if (!APPEND || x.which == 0) {
+      dst = (T*)a.q.dst + ((long long)(n0 + x.k) * a.q.heads + x.h) * a.width;
     } else {
-      const long long row = s_row[which - 1][k];
-      if (row < 0) continue;
-      dst = (T*)part->dst + row + h * part->dh;
+      const Part& part = x.which == 1 ? a.k : a.v;
+      const long long row = s_row[x.which - 1][x.k];
+      if (row >= 0) dst = (T*)part.dst + row + x.h * part.dh;
     }
-    int at, second;
-    if (item < first) {
-      at = INTER ? item * 2 * V : item * V;
-      second = INTER ? at + V : at + a.half;
-    } else {
-      at = (which == 2 ? 0 : a.dim) + (item - first) * 2 * V;
-      second = at + V;
-    }
-    const bool both = second < a.width;
-    Pack<T, V> u, w;
-    u.load(src + at);
-    if (both) w.load(src + second);
-    if (item < first) turn<T, V, INTER>(u, w, s_cs + k * a.half + item * V);
-    if (APPEND && which == 0 && !s_live[k]) {
+    if (dst) {
+      if (x.cs >= 0) turn<T, V, INTER>(x.u, x.w, s_cs + x.k * a.half + x.cs);
+      if (APPEND && x.which == 0 && !s_live[x.k]) {
 #pragma unroll
-      for (int e = 0; e < V; e++) u.e[e] = w.e[e] = (T)0.f;
+        for (int e = 0; e < V; e++) x.u.e[e] = x.w.e[e] = (T)0.f;
+      }
+      x.u.store(dst + x.at);
+      if (x.second < a.width) x.w.store(dst + x.second);
     }
-    u.store(dst + at);
-    if (both) w.store(dst + second);
+    x = y;
   }
 }
 
@@ -299,16 +315,17 @@ GB_EXPORT int gb_rotary(int dtype, const void* x, long long sb, long long st, lo
 }
 
 // k and v (batch, tokens, heads, width) into the pages of their sequences, k turned (dim 0: as it is); q, where there is one, turned
-// into q_out.  strides: of q, k, v (batch, token, head), of both caches (page, head, row).
-GB_EXPORT int gb_cache_append(int dtype, const void* q, void* q_out, const void* k, const void* v, void* k_cache, void* v_cache,
-                              const long long* strides, int batch, int tokens, int q_heads, int heads, int width, int dim, int interleaved,
+// into q_out.  Strides in elements: of q, k, v (batch, token, head), of both caches (page, head, row: strides[0..5]).
+GB_EXPORT int gb_cache_append(int dtype, const void* q, long long q_sb, long long q_st, long long q_sh, void* q_out, const void* k, long long k_sb,
+                              long long k_st, long long k_sh, const void* v, long long v_sb, long long v_st, long long v_sh, void* k_cache,
+                              void* v_cache, const long long* strides, int batch, int tokens, int q_heads, int heads, int width, int dim, int interleaved,
                               const void* turns, double amplitude, const void* table, long long table_stride, int columns, int pages, int page,
                               const void* lengths, const void* counts, void* stream) {
   RotaryArgs a = {};
-  const long long* s = strides;
-  a.q = {q, q_out, s[0], s[1], s[2], 0, 0, 0, q ? q_heads : 0};
-  a.k = {k, k_cache, s[3], s[4], s[5], s[9], s[10], s[11], heads};
-  a.v = {v, v_cache, s[6], s[7], s[8], s[12], s[13], s[14], heads};
+  const long long zero[6] = {0, 0, 0, 0, 0, 0}, *s = strides ? strides : zero;
+  a.q = {q, q_out, q_sb, q_st, q_sh, 0, 0, 0, q ? q_heads : 0};
+  a.k = {k, k_cache, k_sb, k_st, k_sh, s[0], s[1], s[2], heads};
+  a.v = {v, v_cache, v_sb, v_st, v_sh, s[3], s[4], s[5], heads};
   a.batch = batch; a.tokens = tokens; a.width = width; a.dim = dim; a.half = dim / 2;
   a.turns = (const unsigned long long*)turns;
   a.amplitude = (float)amplitude;
@@ -318,7 +335,7 @@ GB_EXPORT int gb_cache_append(int dtype, const void* q, void* q_out, const void*
   const int rc = checked("gb_cache_append", dtype, a);
   if (rc != gbh::E_OK) return rc;
   if (batch == 0 || tokens == 0) return gbh::E_OK;
-  if (!k || !v || !k_cache || !v_cache || !table || !lengths || (q && !q_out) || page < 1 || columns < 1 || pages < 1 || heads < 1) {
+  if (!k || !v || !k_cache || !v_cache || !strides || !table || !lengths || (q && !q_out) || page < 1 || columns < 1 || pages < 1 || heads < 1) {
     gbh::set_error("gb_cache_append: null pointer or empty cache");
     return gbh::E_BAD_ARG;
   }

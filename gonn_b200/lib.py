@@ -36,8 +36,8 @@ _ARGUMENTS = {
     "gb_mx_add_rms_norm": "iipLpLpipppLLdp", "gb_mx_matmul": "ipppppLpiLLLiip", "gb_mx_matmul_rows": "iipLpppLpiLLLiip",
     "gb_mx_linear": "iipLppppiLLLiipLp",
     "gb_mx_train_forward": "iipLpLppiLLLiipLpLp", "gb_mx_train_backward": "ipLppipipiLLLpLp",
-    "gb_rotary": "ipLLLpiiiiiipdipiLLp", "gb_cache_append": "ipppppppiiiiiiipdpLiiippp",
-    "gb_cache_attn": "ipppppiiiiipLiiippidpLp", "gb_cache_attn_bytes": "iLLLLLi",
+    "gb_rotary": "ipLLLpiiiiiipdipiLLp", "gb_cache_append": "ipLLLppLLLpLLLpppiiiiiiipdpLiiippp",
+    "gb_cache_attn": "ipLLLppppiiiiipLiiippidpLp", "gb_cache_attn_bytes": "iLLLLLiL", "gb_cache_attn_kernels": "iLLLLLiL",
     "gb_mx_plan": "LLLip", "gb_mx_linear_bytes": "LLLi", "gb_mx_train_bytes": "LLLiii",
 }
 
@@ -51,7 +51,6 @@ KERNELS_PER_CALL = {
     "gb_norm_bwd": 2, "gb_channel_sum": 2, "gb_ce_fwd": 2, "gb_ce_fused": 2, "gb_flash_bwd": 2, "gb_flash_bwd_ws": 2, "gb_embedding_bwd": 5,
     "gb_status_read": 0, "gb_comm_alloc": 0, "gb_comm_open": 0, "gb_comm_emulate": 0,
     "gb_comm_free": 0, "gb_reduce": 1, "gb_gemm_f32x3": 3, "gb_conv_wgrad": 2, "gb_conv_cl_fwd": 2, "gb_conv_cl_bwd": 4, "gb_stack_fwd": 0, "gb_set_words": 1, "gb_norm_bwd_res": 2, "gb_q_dynamic": 2,
-    "gb_cache_attn": 2, "gb_cache_attn_bytes": 0,
     # by the arguments: up to 16 rows take one; of dX, dW and db those that there are, and the gradient's quantisation
     "gb_mx_linear": lambda a: 1 if a[9] <= 16 else 2,
     "gb_mx_train_forward": 3,

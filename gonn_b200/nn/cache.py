@@ -63,24 +63,23 @@ class KVCache:
         if min(pages, page_size, num_heads, head_dim) < 1:
             raise ValueError("KVCache: pages, page_size, num_heads and head_dim must be >= 1")
         shape = (pages, num_heads, page_size, head_dim)
-        self._set(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device))
+        self._of = _cache.Layout(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device))
 
     @classmethod
     def Over(cls, keys: torch.Tensor, values: torch.Tensor) -> "KVCache":
         """A cache in tensors that are there already."""
         c = cls.__new__(cls)
-        c._set(keys, values)
+        c._of = _cache.Layout(keys, values)
         return c
 
-    def _set(self, keys, values):
-        _cache.check_cache(keys, values)
-        self.Keys, self.Values = keys, values
+    Keys = property(lambda self: self._of.keys)
+    Values = property(lambda self: self._of.values)
 
     def Append(self, k, v, table, lengths, counts=None, rotary: Optional[RotaryEmbedding] = None, q=None):
         """Writes k and v (batch, tokens, heads, head size), any strides, to the pages of their sequences: k turned by ``rotary`` at its
         positions, if one is given.  ``q`` (batch, tokens, its heads, head size) is turned on the way and returned (zeros where a token does
         not count).  No two sequences may write the same row."""
-        return _cache.append(self.Keys, self.Values, k, v, table, lengths, counts, None if rotary is None else rotary._plan(), q)
+        return _cache.append(self._of, k, v, table, lengths, counts, None if rotary is None else rotary._plan(), q)
 
     def Attend(self, q, table, lengths, counts=None, scale: Optional[float] = None, shared_pages: int = 0):
         """softmax(scale q K^T) V of q (batch, tokens, heads, head size) over its sequence's positions up to its own, keys and values of
@@ -89,4 +88,4 @@ class KVCache:
 
         ``shared_pages``: all sequences have the same first pages (a common prompt), which are taken from the table's first row and read
         once for many sequences."""
-        return _cache.attend(self.Keys, self.Values, q, table, lengths, counts, scale, shared_pages)
+        return _cache.attend(self._of, q, table, lengths, counts, scale, shared_pages)

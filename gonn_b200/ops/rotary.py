@@ -78,7 +78,8 @@ class _Rotary(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        return _Rotary.apply(dy, *ctx.rest), None, None, None, None, None
+        dx = _Rotary.apply(dy, *ctx.rest) if torch.is_grad_enabled() else _launch(dy, *ctx.rest)
+        return dx, None, None, None, None, None
 
 
 def rotary(x: torch.Tensor, positions: Optional[torch.Tensor], w: Sequence[float], turns: torch.Tensor, interleaved: bool = False,
@@ -90,21 +91,22 @@ def rotary(x: torch.Tensor, positions: Optional[torch.Tensor], w: Sequence[float
     batch, tokens, _, width = x.shape
     if 2 * len(w) > width:
         raise ValueError(f"rotary: {2 * len(w)} columns are turned, but a head has {width}")
+    device = x.get_device()
     if positions is not None:
         if positions.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"rotary: positions are int32 or int64, not {positions.dtype}")
-        if tuple(positions.shape) not in ((tokens,), (batch, tokens)):
+        if positions.shape != (tokens,) and positions.shape != (batch, tokens):
             raise ValueError(f"rotary: positions must have shape ({tokens},) or ({batch}, {tokens}), got {tuple(positions.shape)}")
-        if positions.device != x.device:
+        if positions.get_device() != device:
             raise ValueError(f"rotary: positions are on {positions.device}, x on {x.device}")
-    if not x.is_cuda:
+    if device < 0:
         if not x.is_floating_point():
             raise TypeError(f"rotary: a floating point tensor is needed, got {x.dtype}")
         at = torch.arange(tokens, device=x.device) if positions is None else positions
         return rotate_ref(x, at, w, interleaved, amplitude)
     if x.dtype not in _TYPES:
         raise TypeError(f"rotary: no CUDA kernel for dtype {x.dtype}")
-    if turns.device != x.device:
+    if turns.get_device() != device:
         raise ValueError(f"rotary: the frequencies are on {turns.device}, x on {x.device}; move the module there")
     if torch.is_grad_enabled() and x.requires_grad:
         return _Rotary.apply(x, positions, turns, interleaved, amplitude, False)
