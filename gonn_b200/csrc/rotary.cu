@@ -6,10 +6,12 @@
 // Angles.  p w in fp32 is off by p 2^-24: by 0.008 at position 131 072, twice a bf16's last bit.  So a frequency is held as the fraction
 // w / 2 pi of a turn in 64 bits of fixed point, and p times it, modulo 2^64, is the fraction of a turn that is left: an integer
 // product whose overflow is the reduction, off by p 2^-65 turns.  Its upper 32 bits become a float in half turns (off by 2^-25) for
-// sincospif.  No table: sine and cosine of a token are taken once per CTA, in shared memory, and serve all of its heads.
+// sincospif.
 //
-// What bounds it: memory, every element read and written once.  A CTA takes a few tokens with all of their heads, a thread two
-// vectors of 16 bytes (narrower ones where a size or an address is odd): the two halves of its pairs.
+// What bounds it: memory, every element read and written once.  A thread takes an item, two vectors of 16 bytes (narrower ones where a size or an
+// address is odd) with the two halves of its pairs, of several heads of one token: their loads and the position's are on their way at once, and sines and
+// cosines serve all of these heads.  No table, no shared memory, no barrier.  (A CTA that computed the angles of a few tokens in shared memory for
+// all of their heads: 16 x 1024 x 24 heads of 64 in bf16 21 to 25 us, of which the floor is 15; so: see launch_rotary.)
 #include "common.cuh"
 
 using namespace gb;
@@ -17,8 +19,7 @@ using namespace gb;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kAngles = 1024;         // sines and cosines that a CTA holds
-constexpr int kMaxTokens = 16;
+constexpr int kHeads = 4;              // whose loads a thread has on their way
 
 struct Part {                         // a tensor (batch, tokens, heads, width) and where its rows go
   const void* src;
@@ -46,7 +47,7 @@ struct RotaryArgs {
   const int* lengths;
   const int* counts;                  // null: all tokens count
   int* status;
-  int per_cta;                        // tokens of a CTA
+  int groups;                         // threads that share a token's heads of an item
   int early;
 };
 
@@ -63,10 +64,19 @@ struct Pack {
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<typename VecOf<V * sizeof(T)>::type*>(p) = *reinterpret_cast<const typename VecOf<V * sizeof(T)>::type*>(e); }
 };
 
+// Cosine and sine of a position's angle.  For fp32 rows sincospif; for 16-bit rows the hardware's functions, off by 2^-21 at most within half a turn,
+// where the rows themselves are off by 2^-12 or 2^-9 (four prompts of 2048 tokens appended, 48 heads of 128: 40.9 us with sincospif).
+template <typename T>
 __device__ __forceinline__ float2 angle_of(unsigned long long turns, long long position, float amplitude, bool back) {
   const unsigned long long phase = turns * (unsigned long long)position;
+  const float x = (float)(int)(phase >> 32) * 4.656612873077393e-10f;          // 2^-31: half turns in [-1, 1)
   float s, c;
-  sincospif((float)(int)(phase >> 32) * 4.656612873077393e-10f, &s, &c);       // 2^-31: half turns in [-1, 1)
+  if constexpr (sizeof(T) == 4) {
+    sincospif(x, &s, &c);
+  } else {
+    s = __sinf(x * 3.14159265358979f);
+    c = __cosf(x * 3.14159265358979f);
+  }
   return make_float2(c * amplitude, (back ? -s : s) * amplitude);
 }
 
@@ -94,139 +104,119 @@ __device__ __forceinline__ void turn(Pack<T, V>& u, Pack<T, V>& w, const float2*
   }
 }
 
+// A head of any part is `items` items of two vectors: half / V turned ones, then the rest (of values: all of it) as it lies.
 template <typename T, int V, bool INTER, bool APPEND>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
-  __shared__ __align__(16) float2 s_cs[kAngles];
-  __shared__ long long s_row[2][kMaxTokens];     // where a token's row starts in either cache, -1: nowhere
-  __shared__ int s_live[kMaxTokens];
   if (a.early) pdl_trigger();
+  const int items = (a.width + 2 * V - 1) / (2 * V), heads = APPEND ? a.q.heads + 2 * a.k.heads : a.q.heads;
+  const unsigned i = blockIdx.x * kThreads + threadIdx.x, per_token = (unsigned)a.groups * items, token = i / per_token;
+  const unsigned in_token = i - token * per_token, group = in_token / items;
+  const int item = in_token - group * items, b = token / a.tokens, t = token - b * a.tokens;
   pdl_wait();
-  const int n_all = a.batch * a.tokens, n0 = blockIdx.x * a.per_cta, n = min(a.per_cta, n_all - n0);
-  auto position_of = [&](int token, bool& live) -> long long {
-    const int b = token / a.tokens, t = token - b * a.tokens;
-    live = true;
-    if constexpr (APPEND) {
-      live = a.counts == nullptr || t < a.counts[b];
-      return (long long)a.lengths[b] + t;
-    }
-    if (a.positions == nullptr) return t;
-    const long long i = b * a.pb + t * a.pt;
-    return a.positions64 ? reinterpret_cast<const long long*>(a.positions)[i] : reinterpret_cast<const int*>(a.positions)[i];
-  };
-  // A head is half / V turned items of two vectors, then items of up to two vectors of the rest.
-  const int turned = a.half / V, rest = a.width - a.dim, items = turned + (rest + 2 * V - 1) / (2 * V);
-  const int flat = (a.width + 2 * V - 1) / (2 * V);       // items of a head of values
-  const int per_token = APPEND ? (a.q.heads + a.k.heads) * items + a.v.heads * flat : a.q.heads * items;
-  struct Item {
-    int k, which, h, at, second, cs;      // token of the CTA; queries, keys, values; first columns of the two vectors; first angle, -1: copied
+  if (b >= a.batch) return;
+  const bool turns = item < a.half / V;
+  const int flat = item * 2 * V, first = turns && !INTER ? item * V : flat, second = turns && !INTER ? first + a.half : first + V;
+  struct Pair {
     Pack<T, V> u, w;
+    int which, h;                         // queries, keys, values; the head
   };
-  auto fetch = [&](int i, Item& x) {
-    x.k = i / per_token;
-    int j = i - x.k * per_token;
-    const int token = n0 + x.k, b = token / a.tokens, t = token - b * a.tokens;
-    const Part* part = &a.q;
+  // (values chosen one by one: a pointer to a part of the arguments would have them copied to local memory)
+  auto of = [&](int which, auto q, auto k, auto v) { return !APPEND || which == 0 ? q : which == 1 ? k : v; };
+  auto fetch = [&](Pair& x, int h) {
     x.which = 0;
-    int width_items = items, first = turned;
-    if constexpr (APPEND) {
-      if (j >= a.q.heads * items) {
-        j -= a.q.heads * items;
-        part = &a.k;
-        x.which = 1;
-        if (j >= a.k.heads * items) {
-          j -= a.k.heads * items;
-          part = &a.v;
-          x.which = 2;
-          width_items = flat;
-          first = 0;
-        }
+    if (APPEND && h >= a.q.heads) {
+      x.which = 1;
+      h -= a.q.heads;
+      if (h >= a.k.heads) {
+        x.which = 2;
+        h -= a.k.heads;
       }
     }
-    x.h = j / width_items;
-    const int item = j - x.h * width_items;
-    if (item < first) {
-      x.at = INTER ? item * 2 * V : item * V;
-      x.second = INTER ? x.at + V : x.at + a.half;
-      x.cs = item * V;
-    } else {
-      x.at = (x.which == 2 ? 0 : a.dim) + (item - first) * 2 * V;
-      x.second = x.at + V;
-      x.cs = -1;
-    }
-    const T* src = (const T*)part->src + b * part->sb + t * part->st + x.h * part->sh;
-    x.u.load(src + x.at);
-    if (x.second < a.width) x.w.load(src + x.second);
+    x.h = h;
+    const bool value = APPEND && x.which == 2;
+    const T* src = (const T*)of(x.which, a.q.src, a.k.src, a.v.src) + b * of(x.which, a.q.sb, a.k.sb, a.v.sb) +
+                   t * of(x.which, a.q.st, a.k.st, a.v.st) + h * of(x.which, a.q.sh, a.k.sh, a.v.sh);
+    const int at = value ? flat : first, to = value ? flat + V : second;
+    x.u.load(src + at);
+    if (to < a.width) x.w.load(src + to);
   };
-  // The first item is on its way while the angles are computed, and each one while the one before it is turned.
-  const int total = n * per_token;
-  Item x;
-  if ((int)threadIdx.x < total) fetch(threadIdx.x, x);
-  for (int i = threadIdx.x; i < n * a.half; i += kThreads) {
-    const int k = i / a.half;
-    bool live;
-    s_cs[i] = angle_of(a.turns[i - k * a.half], position_of(n0 + k, live), a.amplitude, a.back);
-  }
-  if constexpr (APPEND) {
-    if (threadIdx.x < n) {
-      bool live;
-      const long long p = position_of(n0 + threadIdx.x, live);
-      long long rk = -1, rv = -1;
-      if (live) {
-        const int b = (n0 + threadIdx.x) / a.tokens;
-        int page = -1;
-        if (p >= 0 && p < (long long)a.columns * a.page) page = a.table[b * a.table_stride + p / a.page];
-        if (page < 0 || page >= a.pages) {
-          set_status(a.status, ST_BAD_INDEX, b);
-        } else {
-          const long long r = p % a.page;
-          rk = page * a.k.dp + r * a.k.dr;
-          rv = page * a.v.dp + r * a.v.dr;
-        }
-      }
-      s_row[0][threadIdx.x] = rk;
-      s_row[1][threadIdx.x] = rv;
-      s_live[threadIdx.x] = live;
-    }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < total; i += kThreads) {
-    Item y;
-    if (i + kThreads < total) fetch(i + kThreads, y);
-    T* dst = nullptr;
-    if (!APPEND || x.which == 0) {
-      dst = (T*)a.q.dst + ((long long)(n0 + x.k) * a.q.heads + x.h) * a.width;
-    } else {
-      const Part& part = x.which == 1 ? a.k : a.v;
-      const long long row = s_row[x.which - 1][x.k];
-      if (row >= 0) dst = (T*)part.dst + row + x.h * part.dh;
-    }
-    if (dst) {
-      if (x.cs >= 0) turn<T, V, INTER>(x.u, x.w, s_cs + x.k * a.half + x.cs);
-      if (APPEND && x.which == 0 && !s_live[x.k]) {
+  // kHeads heads at a time, the first ones on their way before anything else is known.
+  Pair x[kHeads];
+  int h = group;
 #pragma unroll
-        for (int e = 0; e < V; e++) x.u.e[e] = x.w.e[e] = (T)0.f;
+  for (int k = 0; k < kHeads; k++)
+    if (h + k * a.groups < heads) fetch(x[k], h + k * a.groups);
+  long long position = t;
+  if constexpr (APPEND) {
+    position = (long long)a.lengths[b] + t;
+  } else if (a.positions != nullptr) {
+    const long long at = b * a.pb + t * a.pt;
+    position = a.positions64 ? reinterpret_cast<const long long*>(a.positions)[at] : reinterpret_cast<const int*>(a.positions)[at];
+  }
+  bool live = true;
+  int page = -1, in_page = 0;
+  if constexpr (APPEND) {
+    live = a.counts == nullptr || t < a.counts[b];
+    if (live) {
+      if (position >= 0 && position < (long long)a.columns * a.page) {
+        const unsigned column = (unsigned)position / (unsigned)a.page;
+        in_page = (int)((unsigned)position - column * (unsigned)a.page);
+        page = a.table[b * a.table_stride + column];
       }
-      x.u.store(dst + x.at);
-      if (x.second < a.width) x.w.store(dst + x.second);
+      if (page < 0 || page >= a.pages) {
+        if (in_token == 0) set_status(a.status, ST_BAD_INDEX, b);
+        page = -1;
+      }
     }
-    x = y;
+  }
+  float2 cs[V];
+  if (turns) {
+#pragma unroll
+    for (int k = 0; k < V; k++) cs[k] = angle_of<T>(a.turns[item * V + k], position, a.amplitude, a.back);
+  }
+  for (; h < heads; h += kHeads * a.groups) {
+#pragma unroll
+    for (int k = 0; k < kHeads; k++) {
+      if (h + k * a.groups >= heads) break;
+      const bool value = APPEND && x[k].which == 2;
+      if (turns && !value) turn<T, V, INTER>(x[k].u, x[k].w, cs);
+      T* dst;
+      if (!APPEND || x[k].which == 0) {
+        dst = (T*)a.q.dst + ((long long)token * a.q.heads + x[k].h) * a.width;
+        if (APPEND && !live) {
+#pragma unroll
+          for (int e = 0; e < V; e++) x[k].u.e[e] = x[k].w.e[e] = (T)0.f;
+        }
+      } else {
+        if (page < 0) continue;
+        dst = value ? (T*)a.v.dst + page * a.v.dp + x[k].h * a.v.dh + in_page * a.v.dr
+                    : (T*)a.k.dst + page * a.k.dp + x[k].h * a.k.dh + in_page * a.k.dr;
+      }
+      const int at = value ? flat : first, to = value ? flat + V : second;
+      x[k].u.store(dst + at);
+      if (to < a.width) x[k].w.store(dst + to);
+    }
+#pragma unroll
+    for (int k = 0; k < kHeads; k++)
+      if (h + (k + kHeads) * a.groups < heads) fetch(x[k], h + (k + kHeads) * a.groups);
   }
 }
 
 template <typename T, int V, bool APPEND>
 int launch_rotary(RotaryArgs& a, int inter, cudaStream_t s) {
-  const int n = a.batch * a.tokens;
-  // Tokens of a CTA: as many as keep every thread busy with four items, as their angles fit, and as leave two CTAs for every SM.
-  const long long items = (long long)(a.q.heads + (APPEND ? 2 * a.k.heads : 0)) * ((a.width + 2 * V - 1) / (2 * V));
-  long long per = (4 * kThreads + items - 1) / items;
-  per = per < kMaxTokens ? per : kMaxTokens;
-  if (per * a.half > kAngles) per = kAngles / a.half;
-  const long long spread = (n + 2 * 148 - 1) / (2 * 148);
-  per = per < spread ? per : spread;
-  if (per < 1) per = 1;
-  a.per_cta = (int)per;
-  const unsigned ctas = (unsigned)((n + per - 1) / per);
-  a.early = starts_early(per * items * 4 * V * sizeof(T), ctas);
+  const unsigned long long tokens = (unsigned long long)a.batch * a.tokens;
+  const int heads = a.q.heads + (APPEND ? 2 * a.k.heads : 0), items = (a.width + 2 * V - 1) / (2 * V);
+  // Heads of a thread: four where that leaves the SMs full twice over, two where it does so once, else one.
+  int per = 4;
+  while (per > 1 && tokens * items * ((heads + per - 1) / per) < (per > 2 ? 2ull : 1ull) * 148 * 1024) per >>= 1;
+  a.groups = (heads + per - 1) / per;
+  const unsigned long long threads = tokens * items * a.groups;
+  if (threads >= 0xffff0000ull) {
+    gbh::set_error("rotary: %llu tokens of %d heads are too many for one call", tokens, heads);
+    return gbh::E_TOO_LARGE;
+  }
+  const unsigned ctas = (unsigned)((threads + kThreads - 1) / kThreads);
+  a.early = starts_early((long long)kThreads * per * 4 * V * sizeof(T), ctas);
   if (inter) GB_CUDA_OK(gbh::launch_if(a.early, rotary_kernel<T, V, true, APPEND>, dim3(ctas), dim3(kThreads), 0, s, a));
   else GB_CUDA_OK(gbh::launch_if(a.early, rotary_kernel<T, V, false, APPEND>, dim3(ctas), dim3(kThreads), 0, s, a));
   return gbh::E_OK;
@@ -276,14 +266,13 @@ int checked(const char* what, int dtype, const RotaryArgs& a) {
     gbh::set_error("%s: bad dtype %d", what, dtype);
     return gbh::E_BAD_ARG;
   }
-  if (a.batch < 0 || a.tokens < 0 || a.width < 1 || a.dim < 0 || a.dim > a.width || a.dim % 2 || a.half > kAngles || a.q.heads < 0 ||
+  if (a.batch < 0 || a.tokens < 0 || a.width < 1 || a.dim < 0 || a.dim > a.width || a.dim % 2 || a.q.heads < 0 ||
       a.k.heads < 0 || (a.half && !a.turns)) {
     gbh::set_error("%s: bad sizes (batch %d, tokens %d, width %d, dim %d)", what, a.batch, a.tokens, a.width, a.dim);
     return gbh::E_BAD_ARG;
   }
-  const long long n = (long long)a.batch * a.tokens, wide = (long long)(a.q.heads + 2LL * a.k.heads) * a.width;
-  if (n >= 0x7fffffffLL || wide * kMaxTokens >= 0x7fffffffLL) {
-    gbh::set_error("%s: %lld tokens of %lld columns are too many for one call", what, n, wide);
+  if ((long long)a.batch * a.tokens >= 0x7fffffffLL || (long long)a.columns * a.page >= 0x7fffffffLL) {
+    gbh::set_error("%s: %d x %d tokens or a table of %d pages of %d positions are too many for one call", what, a.batch, a.tokens, a.columns, a.page);
     return gbh::E_TOO_LARGE;
   }
   return gbh::E_OK;
