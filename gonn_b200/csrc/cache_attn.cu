@@ -59,7 +59,7 @@ struct CacheArgs {
   int peers;                               // CTAs of a cluster, 0: the list is dealt out
   int shared;                              // a prefix is joined to the sequences' own keys
   int wide_prefix, wide_own;               // which of them the kernel for many rows takes
-  int wide_tiles, splits;                  // its row tiles, of a sequence or of the prefix; runs of keys
+  int wide_tiles, splits, wide_group;      // its row tiles, of a sequence or of the prefix; runs of keys; runs whose tiles go together
   int slot_rows;                           // rows of the other kernel's tiles
   int2* owner;                             // [(prefix tiles + B own_tiles) Hkv] first and last CTA
   int* status;
@@ -1002,13 +1002,17 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_wait();
+  // Beside the kernel for few rows, which was launched first and has waited for all that came before: this one waits for that one's end alone, and at
+  // its own, so that what follows it follows both.
+  if (!a.wide_prefix) pdl_wait();
   pdl_trigger();
 
-  // Row tiles of a sequence run from its last one, which sees the most keys, to its first.
-  unsigned idx = blockIdx.x;
-  const int rank = idx % a.wide_tiles;
-  idx /= a.wide_tiles;
+  // Row tiles of a sequence run from its last one, which sees the most keys, to its first: over the heads of a group, so that the kernel ends on
+  // the shortest ones.  (sequence, head, run of keys) by groups, in a group by row tiles.
+  const unsigned runs = (unsigned)a.splits * a.Hkv * (a.wide_prefix ? 1 : a.B), per_group = (unsigned)a.wide_group * a.wide_tiles;
+  const unsigned group = blockIdx.x / per_group, in_group = blockIdx.x - group * per_group, size = min((unsigned)a.wide_group, runs - group * a.wide_group);
+  const int rank = in_group / size;
+  unsigned idx = group * a.wide_group + in_group - rank * size;
   const int split = idx % a.splits;
   idx /= a.splits;
   const int h = idx % a.Hkv;
@@ -1324,6 +1328,7 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     tc_fence_after();
     tmem_dealloc(tmem, C::COLS);
   }
+  if (a.wide_prefix) pdl_wait();
 }
 
 // Joins the partial rows of a query row: those of the prefix and those of its own sequence.  WPR warps a row, a lane four columns.  First the
@@ -1470,13 +1475,15 @@ bool plan(Sizes& z, int dtype, long long B, long long T, long long H, long long 
   if (z.entries * Hkv >= 0x7fffffffLL) return false;
   z.own_tiles = (int)ot;
   z.prefix_tiles = (int)pt;
-  // A cluster for each (sequence, row tile, key head): as many CTAs, up to eight, as leave all of them on the SMs at a time.  Where a full table
-  // would be more than kClusterTiles tiles for one of them, the list is dealt out, which balances lengths.
+  // A cluster for each (sequence, row tile, key head): as many CTAs, up to eight, as leave all of them on the SMs at a time.  The list is dealt out
+  // instead, which balances lengths over all CTAs but takes the second kernel (worth about kClusterTiles tiles), where that is less than what the longest
+  // sequence, a full table, costs more here than one of half its length with all CTAs at work.
   if (!shared && !z.wide_own && z.rows <= 16 && z.entries * Hkv <= kCtas) {
     const long long tile = 16384 / ((D <= 64 ? 64 : 128) * (dtype == 2 ? 4 : 2)), tiles = (room + tile - 1) / tile;
     z.peers = kPeers;
     while (z.peers > 1 && z.entries * Hkv * z.peers > kCtas) z.peers >>= 1;
-    if (tiles > (long long)kClusterTiles * z.peers) z.peers = 0;
+    const long long each = (tiles + z.peers - 1) / z.peers, ctas = z.entries * Hkv * z.peers;
+    if (each * (2 * kCtas - ctas) > 2LL * kCtas * kClusterTiles) z.peers = 0;
     if (z.peers) return true;                                        // without a workspace
   }
   const long long rows = z.wide_own ? (z.splits > 1 ? z.splits * B * T * H : 0)
@@ -1532,6 +1539,13 @@ int launch_kernel(const CUtensorMap& tk, const CUtensorMap& tv, CacheArgs& a, cu
     return gbh::E_OK;
   } else {
     GB_CUDA_OK(gbh::launch(kernel, dim3(a.ctas), dim3(kThreads), C::SMEM, s, 1, tk, tv, a));
+    if constexpr (C::kMma) {
+      if (a.wide_prefix) {
+        const int rc = a.box ? (a.D <= 64 ? launch_wide<T, 64, true>(tk, tv, a, s) : launch_wide<T, 128, true>(tk, tv, a, s))
+                             : (a.D <= 64 ? launch_wide<T, 64, false>(tk, tv, a, s) : launch_wide<T, 128, false>(tk, tv, a, s));
+        if (rc) return rc;
+      }
+    }
     return launch_join<T, C::ROWS, C::TILE>(a, s);
   }
 }
@@ -1580,11 +1594,11 @@ int launch_type(const CUtensorMap& k, const CUtensorMap& v, CacheArgs& a, int ro
 template <typename T>
 int launch_any(const CUtensorMap& k, const CUtensorMap& v, CacheArgs& a, int rows, cudaStream_t s) {
   if constexpr (Elem<T>::kMma) {
-    if (a.wide_own || a.wide_prefix) {
+    if (a.wide_own) {
       const int rc = a.box ? (a.D <= 64 ? launch_wide<T, 64, true>(k, v, a, s) : launch_wide<T, 128, true>(k, v, a, s))
                            : (a.D <= 64 ? launch_wide<T, 64, false>(k, v, a, s) : launch_wide<T, 128, false>(k, v, a, s));
       if (rc) return rc;
-      if (a.wide_own) return a.splits > 1 ? launch_join<T, 64, 64>(a, s) : gbh::E_OK;
+      return a.splits > 1 ? launch_join<T, 64, 64>(a, s) : gbh::E_OK;
     }
   }
   return a.box ? launch_type<T, true>(k, v, a, rows, s) : launch_type<T, false>(k, v, a, rows, s);
@@ -1666,6 +1680,13 @@ GB_EXPORT int gb_cache_attn(int dtype, const void* q, long long q_sb, long long 
   a.shared = prefix > 0 && !z.wide_own;
   a.wide_prefix = z.wide_prefix; a.wide_own = z.wide_own; a.wide_tiles = z.wide_tiles; a.splits = z.splits;
   a.slot_rows = z.rows;
+  // Groups of one size, about a round of CTAs each, whose keys and values stay in L2 (of 126 MB) while their tiles run.  Four prompts of 2048
+  // tokens behind 2048 others, 64 heads of 16 row tiles: in groups of 16 191 us, 19 212, 32 201, all 212, one by one 211.
+  if (z.wide_own || z.wide_prefix) {
+    const long long runs = (long long)z.splits * Hkv * (z.wide_own ? B : 1), groups = (runs * z.wide_tiles + kCtas - 1) / kCtas;
+    const long long run = (long long)a.room * D * 4 / z.splits, fit = run > 0 ? (64LL << 20) / run : runs, size = (runs + groups - 1) / groups;
+    a.wide_group = (int)(size < fit ? size : fit > 1 ? fit : 1);
+  }
   a.peers = z.peers;
   a.ctas = kCtas;
   a.part = (float*)ws;
