@@ -23,9 +23,9 @@ constexpr int kHeads = 4;              // whose loads a thread has on their way
 
 struct Part {                         // a tensor (batch, tokens, heads, width) and where its rows go
   const void* src;
-  void* dst;                          // (batch, tokens, heads, width), contiguous; a cache for keys and values
+  void* dst;                          // (batch, tokens, heads, width), src itself perhaps; a cache for keys and values
   long long sb, st, sh;               // strides of src in elements
-  long long dp, dh, dr;               // strides of a cache: page, head, row
+  long long dp, dh, dr;               // strides of dst: batch, head, token; of a cache: page, head, row
   int heads;
 };
 
@@ -60,7 +60,7 @@ template <> struct VecOf<2> { using type = uint16_t; };
 template <typename T, int V>
 struct Pack {
   T e[V];
-  __device__ __forceinline__ void load(const T* p) { *reinterpret_cast<typename VecOf<V * sizeof(T)>::type*>(e) = __ldg(reinterpret_cast<const typename VecOf<V * sizeof(T)>::type*>(p)); }
+  __device__ __forceinline__ void load(const T* p) { *reinterpret_cast<typename VecOf<V * sizeof(T)>::type*>(e) = *reinterpret_cast<const typename VecOf<V * sizeof(T)>::type*>(p); }
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<typename VecOf<V * sizeof(T)>::type*>(p) = *reinterpret_cast<const typename VecOf<V * sizeof(T)>::type*>(e); }
 };
 
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
       if (turns && !value) turn<T, V, INTER>(x[k].u, x[k].w, cs);
       T* dst;
       if (!APPEND || x[k].which == 0) {
-        dst = (T*)a.q.dst + ((long long)token * a.q.heads + x[k].h) * a.width;
+        dst = (T*)a.q.dst + b * a.q.dp + t * a.q.dr + x[k].h * a.q.dh;
         if (APPEND && !live) {
 #pragma unroll
           for (int e = 0; e < V; e++) x[k].u.e[e] = x[k].w.e[e] = (T)0.f;
@@ -248,16 +248,15 @@ int dispatch(int dtype, RotaryArgs& a, int inter, cudaStream_t s) {
 }
 
 // The widest vector (elements) that divides every size, stride and address.
-int vector_of(int size, const RotaryArgs& a, int extra) {
+int vector_of(int size, const RotaryArgs& a) {
   int v = 16 / size;
-  auto fits = [&](const Part& p, bool cache) {
+  auto fits = [&](const Part& p) {
     if (!p.src) return true;
     const uintptr_t at = (uintptr_t)p.src | (uintptr_t)p.dst;
-    long long s = p.sb | p.st | p.sh;
-    if (cache) s |= p.dp | p.dh | p.dr;
+    const long long s = p.sb | p.st | p.sh | p.dp | p.dh | p.dr;
     return at % (v * size) == 0 && s % v == 0;
   };
-  while (v > 1 && !(a.half % v == 0 && a.width % v == 0 && fits(a.q, false) && fits(a.k, extra) && fits(a.v, extra))) v >>= 1;
+  while (v > 1 && !(a.half % v == 0 && a.width % v == 0 && fits(a.q) && fits(a.k) && fits(a.v))) v >>= 1;
   return v;
 }
 
@@ -280,13 +279,13 @@ int checked(const char* what, int dtype, const RotaryArgs& a) {
 
 }  // namespace
 
-// y = x turned: x (batch, tokens, heads, width) with strides (elements), y contiguous.  positions: int32 or int64 with strides (0 where
+// y = x turned, both (batch, tokens, heads, width) with strides (batch, token, head, in elements); y may be x.  positions: int32 or int64 with strides (0 where
 // shared), or null for 0, 1, ...
-GB_EXPORT int gb_rotary(int dtype, const void* x, long long sb, long long st, long long sh, void* y, int batch, int tokens, int heads, int width,
+GB_EXPORT int gb_rotary(int dtype, const void* x, long long sb, long long st, long long sh, void* y, long long yb, long long yt, long long yh, int batch, int tokens, int heads, int width,
                         int dim, int interleaved, const void* turns, double amplitude, int back, const void* positions, int positions64,
                         long long pb, long long pt, void* stream) {
   RotaryArgs a = {};
-  a.q = {x, y, sb, st, sh, 0, 0, 0, heads};
+  a.q = {x, y, sb, st, sh, yb, yh, yt, heads};
   a.batch = batch; a.tokens = tokens; a.width = width; a.dim = dim; a.half = dim / 2;
   a.turns = (const unsigned long long*)turns;
   a.amplitude = (float)amplitude;
@@ -299,7 +298,7 @@ GB_EXPORT int gb_rotary(int dtype, const void* x, long long sb, long long st, lo
     gbh::set_error("gb_rotary: null pointer");
     return gbh::E_BAD_ARG;
   }
-  a.vec = vector_of(dtype == 2 ? 4 : 2, a, 0);
+  a.vec = vector_of(dtype == 2 ? 4 : 2, a);
   return dispatch<false>(dtype, a, interleaved, (cudaStream_t)stream);
 }
 
@@ -312,7 +311,7 @@ GB_EXPORT int gb_cache_append(int dtype, const void* q, long long q_sb, long lon
                               const void* lengths, const void* counts, void* stream) {
   RotaryArgs a = {};
   const long long zero[6] = {0, 0, 0, 0, 0, 0}, *s = strides ? strides : zero;
-  a.q = {q, q_out, q_sb, q_st, q_sh, 0, 0, 0, q ? q_heads : 0};
+  a.q = {q, q_out, q_sb, q_st, q_sh, (long long)tokens * q_heads * width, width, (long long)q_heads * width, q ? q_heads : 0};
   a.k = {k, k_cache, k_sb, k_st, k_sh, s[0], s[1], s[2], heads};
   a.v = {v, v_cache, v_sb, v_st, v_sh, s[3], s[4], s[5], heads};
   a.batch = batch; a.tokens = tokens; a.width = width; a.dim = dim; a.half = dim / 2;
@@ -329,6 +328,6 @@ GB_EXPORT int gb_cache_append(int dtype, const void* q, long long q_sb, long lon
     return gbh::E_BAD_ARG;
   }
   a.status = gbh::status_ptr();
-  a.vec = vector_of(dtype == 2 ? 4 : 2, a, 1);
+  a.vec = vector_of(dtype == 2 ? 4 : 2, a);
   return dispatch<true>(dtype, a, interleaved, (cudaStream_t)stream);
 }

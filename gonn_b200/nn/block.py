@@ -90,6 +90,8 @@ def _block_words(B, S, E, dt, dev, parts):
         return None
     code = _ACT.get(kind)
     ad = attn.__dict__
+    if ad.get("rotary", _ABSENT) is not None:
+        return None                # (its queries and keys are turned between the products)
     H = ad["num_heads"]
     D = E // H
     if (code is None or not E == ad["embed_dim"] == ad["kdim"] == ad["vdim"] or E % 8 or D % 8 or not 8 <= D <= 128

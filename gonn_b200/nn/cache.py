@@ -42,10 +42,10 @@ class RotaryEmbedding(Module):
     def forward(self, x, positions: Optional[torch.Tensor] = None):
         """x (batch, tokens, heads, width) with any strides, bf16, fp16 or fp32 on CUDA; positions int32 or int64, (tokens,) or
         (batch, tokens), None for 0, 1, ...  Differentiable in x."""
-        return rotary(x, positions, self._w, self.turns, self.interleaved, self.amplitude)
+        return rotary(x, positions, self._w, self._buffers["turns"], self.interleaved, self.amplitude)
 
     def _plan(self):
-        return self._w, self.turns, self.interleaved, self.amplitude
+        return self._w, self._buffers["turns"], self.interleaved, self.amplitude
 
 
 class KVCache:

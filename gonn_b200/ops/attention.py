@@ -20,6 +20,7 @@ from typing import Optional
 import torch
 
 from .. import lib as _l
+from .rotary import rotate_in_place
 
 
 def attention_ref(q, k, v, causal: bool = False, scale: Optional[float] = None):
@@ -378,17 +379,19 @@ def _emit_fused(params, grad_fn_into, grad_fn_new):
 
 class _SelfAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, wq, wk, wv, bq, bk, bv, wqkv, bqkv, H, causal, scale):
+    def forward(ctx, x, wq, wk, wv, bq, bk, bv, wqkv, bqkv, H, causal, scale, rope=None):
         from .gemm import gemm
         B, S, E = x.shape
         D = E // H
         x2 = x.reshape(B * S, E)
         qkv = gemm(x2, wqkv, trans_b=True, bias=bqkv)          # (B*S, 3E)
         qkv5 = qkv.view(B, S, 3, H, D)
+        if rope is not None:            # queries and keys turned where they lie
+            rotate_in_place(qkv.view(B, S, 3 * H, D)[:, :, :2 * H], rope)
         out, lse = flash_fwd(qkv5[:, :, 0], qkv5[:, :, 1], qkv5[:, :, 2], causal, scale)
         ctx.save_for_backward(x2, wqkv, qkv, out, lse)
         ctx.params = (wq, wk, wv, bq, bk, bv)
-        ctx.meta = (B, S, E, H, D, causal, scale)
+        ctx.meta = (B, S, E, H, D, causal, scale, rope)
         return out.view(B, S, E)
 
     @staticmethod
@@ -397,10 +400,12 @@ class _SelfAttention(torch.autograd.Function):
         from .reduce import column_sum
         x2, wqkv, qkv, out, lse = ctx.saved_tensors
         wq, wk, wv, bq, bk, bv = ctx.params
-        B, S, E, H, D, causal, scale = ctx.meta
+        B, S, E, H, D, causal, scale, rope = ctx.meta
         qkv5 = qkv.view(B, S, 3, H, D)
         dq, dk, dv, dqkv = flash_bwd(qkv5[:, :, 0], qkv5[:, :, 1], qkv5[:, :, 2], out,
                                      dout.reshape(B, S, H, D), lse, causal, scale)
+        if rope is not None:            # and their gradients back
+            rotate_in_place(dqkv.view(B, S, 3 * H, D)[:, :, :2 * H], rope, back=True)
         d2 = dqkv.view(B * S, 3 * E)
         dx = gemm(d2, wqkv).view(B, S, E) if ctx.needs_input_grad[0] else None
         gw = _emit_fused([wq, wk, wv],
@@ -412,12 +417,13 @@ class _SelfAttention(torch.autograd.Function):
                              lambda: column_sum(d2))
         else:
             gb = [None, None, None]
-        return (dx, gw[0], gw[1], gw[2], gb[0], gb[1], gb[2], None, None, None, None, None)
+        return (dx, gw[0], gw[1], gw[2], gb[0], gb[1], gb[2], None, None, None, None, None, None)
 
 
-def self_attention_qkv(x, wq, wk, wv, bq, bk, bv, num_heads: int, causal: bool, scale=None):
+def self_attention_qkv(x, wq, wk, wv, bq, bk, bv, num_heads: int, causal: bool, scale=None, rope=None):
     """``flash(x Wq^T + bq, x Wk^T + bk, x Wv^T + bv)`` for (B, S, E) input.
 
+    ``rope``: the plan of a RotaryEmbedding that turns queries and keys, positions 0, 1, ...
     Takes the one-GEMM path when the three weights (and biases) are adjacent in memory,
     bf16/fp16 on CUDA and head_dim is 64 or 128; returns None when that path does not
     apply so that the caller can fall back to separate projections.
@@ -436,4 +442,4 @@ def self_attention_qkv(x, wq, wk, wv, bq, bk, bv, num_heads: int, causal: bool, 
             return None
     scale = (1.0 / math.sqrt(D)) if scale is None else float(scale)
     return _SelfAttention.apply(x, wq, wk, wv, bq, bk, bv, wqkv.detach(), None if bqkv is None else bqkv.detach(),
-                                num_heads, bool(causal), scale)
+                                num_heads, bool(causal), scale, rope)

@@ -52,20 +52,30 @@ def rotate_ref(x: torch.Tensor, positions: torch.Tensor, w: Sequence[float], int
     return torch.cat((part, rest), -1).to(x.dtype)
 
 
-def _launch(x, positions, turns, interleaved, amplitude, back):
+def _launch(x, positions, turns, interleaved, amplitude, back, out=None):
     batch, tokens, heads, width = x.shape
     if x.stride(3) != 1 and width > 1:
         x = x.contiguous()
-    y = torch.empty((batch, tokens, heads, width), dtype=x.dtype, device=x.device)
+    y = torch.empty((batch, tokens, heads, width), dtype=x.dtype, device=x.device) if out is None else out
     if positions is None:
         at, wide, pb, pt = None, 0, 0, 0
     else:
         at, wide = positions.data_ptr(), positions.dtype == torch.int64
         pb, pt = (0, positions.stride(0)) if positions.dim() == 1 else positions.stride()
     sb, st, sh, _ = x.stride()
-    _l.call_on(x.get_device(), "gb_rotary", _TYPES[x.dtype], x.data_ptr(), sb, st, sh, y.data_ptr(), batch, tokens, heads, width,
+    yb, yt, yh, _ = y.stride()
+    _l.call_on(x.get_device(), "gb_rotary", _TYPES[x.dtype], x.data_ptr(), sb, st, sh, y.data_ptr(), yb, yt, yh, batch, tokens, heads, width,
                2 * turns.shape[0], interleaved, turns.data_ptr(), amplitude, back, at, wide, pb, pt)
     return y
+
+
+def rotate_in_place(x: torch.Tensor, plan, back: bool = False) -> None:
+    """Turns a (batch, tokens, heads, width) view of a CUDA buffer where it lies, positions 0, 1, ...; ``plan``: of a RotaryEmbedding.  For buffers
+    that their caller owns: no tape."""
+    _, turns, interleaved, amplitude = plan
+    if turns.get_device() != x.get_device():
+        raise ValueError(f"rotary: the frequencies are on {turns.device}, x on {x.device}; move the module there")
+    _launch(x, None, turns, interleaved, amplitude, back, x)
 
 
 class _Rotary(torch.autograd.Function):

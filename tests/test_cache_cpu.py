@@ -147,3 +147,61 @@ def test_refusals():
         cache.Attend(grad, table, at)
     with torch.no_grad():
         cache.Attend(grad, table, at)
+
+
+# ------------------------------------------------------------------------------------------------------------------ layers and models
+def test_attention_with_rotary():
+    """The layer with rotary positions: relative to each other, gradients by differences, in pieces from a cache."""
+    torch.manual_seed(1)
+    mha = nn.MultiHeadAttention(12, 2, rotary=nn.RotaryEmbedding(4, interleaved=True), dtype=torch.float64)
+    x = torch.randn(2, 5, 12, dtype=torch.float64)
+    whole = mha(x, causal=True)
+    assert not torch.allclose(whole, nn.MultiHeadAttention.forward(_without_rotary(mha), x, causal=True))
+    assert torch.allclose(mha.ForwardMasked(x, causal=True), whole)
+    assert torch.autograd.gradcheck(lambda t: mha(t, causal=True), (x[:1, :3].clone().requires_grad_(),))
+    cache = nn.KVCache(4, 4, 2, 6, dtype=torch.float64)
+    table, at, outs = torch.tensor([[3, 0], [1, 2]], dtype=torch.int32), torch.zeros(2, dtype=torch.int32), []
+    with torch.no_grad():
+        for piece in x.split([2, 1, 2], 1):
+            outs.append(mha.ForwardCached(piece, cache, table, at))
+            at += piece.shape[1]
+    assert torch.allclose(torch.cat(outs, 1), whole)
+    with pytest.raises(ValueError):
+        nn.MultiHeadAttention(12, 2, rotary=nn.RotaryEmbedding(8))
+
+
+def _without_rotary(mha):
+    import copy
+    other = copy.deepcopy(mha)
+    other.__dict__["rotary"] = None
+    return other
+
+
+@pytest.mark.parametrize("rotary", [None, True, dict(dim=4, interleaved=True, scaling="linear", factor=2.0)])
+def test_generate(rotary):
+    """Greedy continuation from the cache is that of the whole sequence computed anew for every token."""
+    from gonn_b200.models import GPT
+    torch.manual_seed(2)
+    model = GPT(vocab=31, d_model=16, n_layers=2, n_heads=2, d_ff=24, max_seq=32, rotary=rotary, dtype=torch.float64)
+    assert (model.pos is None) == (rotary is not None)
+    with torch.no_grad():
+        for p in model.parameters():
+            if p.dim() > 1:
+                p.normal_(0, 0.5)
+    ids = torch.randint(0, 31, (2, 7))
+    want = ids
+    with torch.no_grad():
+        for _ in range(9):
+            want = torch.cat((want, model(want)[:, -1].argmax(-1, keepdim=True)), 1)
+    assert torch.equal(model.Generate(ids, 9, page_size=4), want)
+    assert torch.equal(model.Generate(ids[:1], 9, samples=3, page_size=4), want[:1].expand(3, -1))
+    assert torch.equal(model.Generate(ids[:1], 9, samples=3, page_size=7), want[:1].expand(3, -1))
+    drawn = model.Generate(ids[:1], 5, samples=4, temperature=1.0, page_size=4)
+    assert drawn.shape == (4, 12) and torch.equal(drawn[:, :7], ids[:1].expand(4, -1))
+    assert torch.equal(model.Generate(ids, 0), ids)
+    for bad in (dict(new_tokens=-1), dict(new_tokens=1, samples=2), dict(new_tokens=1, samples=0)):
+        with pytest.raises(ValueError):
+            model.Generate(ids, **bad)
+    if rotary is None:
+        with pytest.raises(ValueError):
+            model.Generate(ids, 26)

@@ -1,7 +1,8 @@
 """Rotary positions and the paged cache on the GPU, against the formulas in fp64.
 
-Tolerances.  Rotation: (a cos - b sin) with cos and sin off by 2e-7 of the amplitude (an angle in 32 bits of a turn, pi 2^-25, and the function's
-own 2 units) plus three fp32 roundings, then one rounding to the type: eps / 2 of the value.  Attention: a score's sum of D products is off by
+Tolerances.  Rotation: (a cos - b sin) with cos and sin off by 2e-7 of the amplitude (an angle in 32 bits of a turn, pi 2^-25 = 9.4e-8, and the
+function's own 2 units) in fp32 and by 6e-7 in 16 bits (the same angle, and 2^-21 of the hardware's functions within half a turn, as documented: 4.8e-7),
+plus three fp32 roundings, then one rounding to the type: eps / 2 of the value.  Attention: a score's sum of D products is off by
 at most D 2^-24 of the sum of its magnitudes, its scaling and exponential by 2^-21 of it and 2^-22: together at most d of a weight.  Weights in 16
 bits are rounded by eps / 2 each.  With A = sum p |v| / sum p the result is off by at most 2 d A + n 2^-24 A (sums of n terms) + eps / 2 A (16
 bits) + eps / 2 of the result (its own rounding)."""
@@ -35,7 +36,7 @@ def turned(x, at, rope, back=False):
     part, err = (torch.stack((p, q), -1).flatten(-2) if rope.interleaved else torch.cat((p, q), -1) for p, q in ((u, v), (size, size)))
     y = torch.cat((part, rest), -1)
     # the angle itself, p w in fp64: 2^-53 of it
-    slack = 2e-7 + 3 * 2.0 ** -24 + float(at.abs().max()) * 2.0 ** -52 if at.numel() else 0.0
+    slack = (2e-7 if x.dtype == F32 else 6e-7) + 3 * 2.0 ** -24 + float(at.abs().max()) * 2.0 ** -52 if at.numel() else 0.0
     return y, torch.cat((err * slack, torch.zeros_like(rest)), -1) + y.abs() * half(x.dtype) * 1.001 + 1e-7 * (x.dtype == F16) + 1e-37
 
 
@@ -283,6 +284,19 @@ def test_beyond_32_bits():
     close(cache.Attend(q, table, at), attended(cache, q, table, at, None))
 
 
+def test_calls_of_a_new_thread():
+    """A thread whose first CUDA call is this one."""
+    import threading
+    cache, table, at, c, (q, k, v) = batch(2, 1, 4, 2, 64, 64, [100, 3], BF)
+    cache.Append(k, v, table, at)
+    outs = []
+    thread = threading.Thread(target=lambda: outs.append(cache.Attend(q, table, at)))
+    thread.start()
+    thread.join()
+    torch.cuda.synchronize()
+    close(outs[0], attended(cache, q, table, at, c))
+
+
 def test_empty_calls():
     cache = nn.KVCache(4, 16, 2, 64, dtype=BF, device="cuda")
     table, at = torch.zeros(0, 1, device="cuda", dtype=torch.int32), torch.zeros(0, device="cuda", dtype=torch.int32)
@@ -375,3 +389,84 @@ def test_refusals():
     wide = nn.KVCache(4, 16, 1, 136, dtype=BF, device="cuda")
     with pytest.raises(ValueError):
         wide.Attend(torch.zeros(2, 1, 1, 136, device="cuda", dtype=BF), table, at)
+
+
+# ------------------------------------------------------------------------------------------------------------------ layers and models
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("inter", [False, True])
+def test_attention_layer_with_rotary(dtype, inter):
+    """Forward, gradients, masks and pieces from a cache, against the layer in fp64 on the CPU.  Every result is a chain of a few roundings of values
+    of about the result's size: eight of them, at the size of its largest value, are allowed.  In fp32 the sums' own errors are no smaller than that: a
+    sum of n products is off by up to n 2^-24 of its terms' magnitudes, which add up to at least the result; n is 256 here (columns; 140 rows in the
+    gradients of weights), where in 16 bits it hides behind the rounding of the result."""
+    import copy
+    torch.manual_seed(3)
+    mha = nn.MultiHeadAttention(256, 4, rotary=nn.RotaryEmbedding(48, interleaved=inter), dtype=dtype, device="cuda")
+    mha = mha.to("cuda")                                                # the frequencies follow
+    exact = copy.deepcopy(mha).cpu().double()
+    x = torch.randn(2, 70, 256, device="cuda").to(dtype).requires_grad_()
+    x64 = x.detach().cpu().double().requires_grad_()
+    dy = torch.randn(2, 70, 256, device="cuda").to(dtype)
+
+    def near(got, want):
+        err = float((got.detach().cpu().double() - want).abs().max())
+        assert err <= (8 + (256 if dtype == F32 else 0)) * half(dtype) * float(want.detach().abs().max()), (err, float(want.detach().abs().max()))
+
+    y, want = mha(x, causal=True), exact(x64, causal=True)
+    near(y, want)
+    params, params64 = list(mha.parameters()), list(exact.parameters())
+    for g, w in zip(torch.autograd.grad(y, [x, *params], dy), torch.autograd.grad(want, [x64, *params64], dy.cpu().double())):
+        if float(w.abs().max()) > 1e-9:                                 # (the key projection's bias has none)
+            near(g, w)
+    with torch.no_grad():
+        near(mha.ForwardMasked(x, causal=True), want)
+        cache = nn.KVCache(6, 32, 4, 64, dtype=dtype, device="cuda")
+        table, at, outs = torch.tensor([[3, 0, 4], [1, 2, 5]], device="cuda", dtype=torch.int32), torch.zeros(2, device="cuda", dtype=torch.int32), []
+        for piece in x.split([40, 1, 1, 28], 1):
+            outs.append(mha.ForwardCached(piece, cache, table, at))
+            at += piece.shape[1]
+        near(torch.cat(outs, 1), want)
+
+
+def test_model_steps_in_a_graph():
+    """A step of a model captured once and replayed token by token, against the whole sequence at once in fp64 on the CPU."""
+    import copy
+    from gonn_b200.models import GPT
+    torch.manual_seed(4)
+    model = GPT(vocab=61, d_model=128, n_layers=2, n_heads=2, d_ff=256, max_seq=64, rotary=dict(scaling="linear", factor=2.0), device="cuda")
+    ids = torch.randint(0, 61, (3, 20), device="cuda")
+    with torch.no_grad():
+        want = copy.deepcopy(model).cpu().double()(ids.cpu())
+        whole = float((model(ids).cpu().double() - want).abs().max())
+        caches = model.Caches(6, 16)
+        table, at = torch.arange(6, device="cuda", dtype=torch.int32).view(3, 2), torch.zeros(3, device="cuda", dtype=torch.int32)
+        first = model.Step(ids[:, :12], caches, table, at)
+        at += 12
+        token = ids[:, 12:13].clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            model.Step(token, caches, table, at)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            logits = model.Step(token, caches, table, at)
+            at += 1
+        outs = [first]
+        for t in range(12, 20):
+            token.copy_(ids[:, t:t + 1])
+            graph.replay()
+            outs.append(logits.clone())
+        steps = float((torch.cat(outs, 1).cpu().double() - want).abs().max())
+    # two ways through the same fp32 products: neither is off by much more than the other
+    assert steps <= 4 * whole + 2.0 ** -20 * float(want.abs().max()), (steps, whole)
+
+
+def test_samples_share_the_prompt():
+    """Continuations of one prompt, in bf16: the first token of every sample is the prompt's, and equal draws stay equal."""
+    from gonn_b200.models import GPT
+    torch.manual_seed(5)
+    model = GPT(vocab=61, d_model=128, n_layers=2, n_heads=2, d_ff=256, max_seq=512, rotary=True, dtype=BF, device="cuda")
+    ids = torch.randint(0, 61, (1, 150), device="cuda")
+    out = model.Generate(ids, 6, samples=80, page_size=16)
+    assert out.shape == (80, 156) and torch.equal(out, out[:1].expand(80, -1)) and torch.equal(out[:, :150], ids.expand(80, -1))
