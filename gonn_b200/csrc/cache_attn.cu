@@ -1351,9 +1351,8 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const CacheArgs a) {
   struct Parts { long long first, rest, step; int n; };
   Parts pre = {0, 0, 0, 0}, own = {0, 0, 0, 0};
   const long long whole = 2LL * a.ctas * ROWS;
-  auto find = [&](Parts& p, int e, int r, long long at) {
-    const int2 c = a.owner[e * a.Hkv + h];                           // (of an entry without tiles: anything)
-    if (entry_of<ROWS, TILE>(a, e).tiles == 0) return true;
+  auto find = [&](Parts& p, int e, const int2 c, int r, long long at) {
+    if (entry_of<ROWS, TILE>(a, e).tiles == 0) return true;          // (whose owner is anything)
     const int cta = c.x >> 1;
     if (cta == c.y) {                             // one CTA had all of it
       p = {at, at, 0, 1};
@@ -1364,15 +1363,14 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const CacheArgs a) {
     return true;
   };
   const int per = a.T * a.G, r = t * a.G + g;
+  const int all = b * per + r, e_pre = all / ROWS, e_own = a.prefix_tiles + b * a.own_tiles + r / ROWS;
+  // (asked for at once, before it is known whether they matter)
+  const int2 c_pre = a.prefix_tiles ? a.owner[e_pre * a.Hkv + h] : make_int2(0, 0), c_own = a.wide_own ? make_int2(0, 0) : a.owner[e_own * a.Hkv + h];
   if (t < count_of(a, b)) {
-    if (a.wide_prefix) {
-      pre = {whole + rows + i, whole + rows + i, rows, a.splits};
-    } else if (a.prefix_tiles) {
-      const int all = b * per + r;
-      find(pre, all / ROWS, all % ROWS, whole + rows + i);
-    }
+    if (a.wide_prefix) pre = {whole + rows + i, whole + rows + i, rows, a.splits};
+    else if (a.prefix_tiles) find(pre, e_pre, c_pre, all % ROWS, whole + rows + i);
     if (a.wide_own) own = {i, i, rows, a.splits};
-    else if (!find(own, a.prefix_tiles + b * a.own_tiles + r / ROWS, r % ROWS, whole + i)) return;
+    else if (!find(own, e_own, c_own, r % ROWS, whole + i)) return;
   }
   const int n = pre.n + own.n;
   float top = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
@@ -1384,27 +1382,34 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const CacheArgs a) {
       row = k < pre.n ? (k == 0 ? pre.first : pre.rest + k * pre.step) : (k == pre.n ? own.first : own.rest + (k - pre.n) * own.step);
       st = a.stat[row];
     }
-    const float next = fmaxf(top, warp_max(st.x)), f = top == -INFINITY ? 0.f : exp2f(top - next);
-    const float w = st.x == -INFINITY ? (st.y == 0.f ? 0.f : 1.f) : exp2f(st.x - next);     // (scores of NaN leave no maximum, but a sum)
-    top = next;
-    sum = sum * f + warp_sum(st.y * w);
-#pragma unroll
-    for (int c = 0; c < 4; c++) o[c] *= f;
     const int m = min(32, (n - k0 - sub + WPR - 1) / WPR);
-    for (int j0 = 0; j0 < m; j0 += 8) {
-      float4 v[8];
+    float4 v[8];
+    auto fetch = [&](int j0) {
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        const long long at = __shfl_sync(0xffffffffu, row, j0 + j) * a.D + 4 * lane;
+        const long long at = __shfl_sync(0xffffffffu, row, (j0 + j) & 31) * a.D + 4 * lane;
         v[j] = j0 + j < m && 4 * lane < a.D ? __ldg(reinterpret_cast<const float4*>(a.part + at)) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
+    };
+    fetch(0);                                    // beside the statistics
+    const bool none = st.x == -INFINITY && st.y == 0.f;                                     // no key of this part is seen: nothing of it counts
+    const float next = fmaxf(top, warp_max(st.x)), f = top == -INFINITY ? 0.f : exp2f(top - next);
+    const float w = none ? -1.f : st.x == -INFINITY ? 1.f : exp2f(st.x - next);             // (scores of NaN leave no maximum, but a sum)
+    top = next;
+    sum = sum * f + warp_sum(none ? 0.f : st.y * w);
+#pragma unroll
+    for (int c = 0; c < 4; c++) o[c] *= f;
+    for (int j0 = 0; j0 < m; j0 += 8) {
+      if (j0) fetch(j0);
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        const float wj = j0 + j < m ? __shfl_sync(0xffffffffu, w, j0 + j) : 0.f;
-        o[0] += v[j].x * wj;
-        o[1] += v[j].y * wj;
-        o[2] += v[j].z * wj;
-        o[3] += v[j].w * wj;
+        const float wj = __shfl_sync(0xffffffffu, w, (j0 + j) & 31);
+        if (j0 + j < m && wj >= 0.f) {
+          o[0] += v[j].x * wj;
+          o[1] += v[j].y * wj;
+          o[2] += v[j].z * wj;
+          o[3] += v[j].w * wj;
+        }
       }
     }
   }
@@ -1625,20 +1630,26 @@ GB_EXPORT int gb_cache_attn_kernels(int dtype, long long B, long long T, long lo
   return z.peers ? 1 : z.wide_own ? 1 + (z.splits > 1) : 2 + z.wide_prefix;
 }
 
-// out (B, T, H, D) = attention of q over the pages of its sequences.  Strides in elements, of q (batch, token, head) and of both caches (page,
-// head, row: strides[0..5]); rows aligned to 16 bytes.  prefix: positions, a multiple of the page, that all sequences have in
-// the pages of the first one's.  The workspace belongs to this call until its kernels have run.
-GB_EXPORT int gb_cache_attn(int dtype, const void* q, long long q_sb, long long q_st, long long q_sh, const void* k, const void* v,
-                            const long long* strides, void* out, int B, int T, int H,
-                            int Hkv, int D, const void* table, long long table_stride, int columns, int pages, int page, const void* lengths,
-                            const void* counts, int prefix, double scale, void* ws, long long ws_bytes, void* stream) {
+// out (B, T, H, D) = attention of q over the pages of its sequences.  sizes (64-bit words; strides in elements, rows aligned to 16 bytes): [0..2]
+// strides of q (batch, token, head), [3..8] of both caches (page, head, row), [9..13] B, T, H, Hkv, D, [14] the table's stride, [15] its columns, [16] pages,
+// [17] positions of a page, [18] positions, a multiple of the page, that all sequences have in the pages of the first one's.  The workspace belongs to this
+// call until its kernels have run.
+GB_EXPORT int gb_cache_attn(int dtype, const void* q, const void* k, const void* v, void* out, const long long* sizes, const void* table,
+                            const void* lengths, const void* counts, double scale, void* ws, long long ws_bytes, void* stream) {
+  if (!sizes) {
+    gbh::set_error("gb_cache_attn: null pointer");
+    return gbh::E_BAD_ARG;
+  }
+  const long long q_sb = sizes[0], q_st = sizes[1], q_sh = sizes[2], *strides = sizes + 3, table_stride = sizes[14];
+  const int B = (int)sizes[9], T = (int)sizes[10], H = (int)sizes[11], Hkv = (int)sizes[12], D = (int)sizes[13], columns = (int)sizes[15];
+  const int pages = (int)sizes[16], page = (int)sizes[17], prefix = (int)sizes[18];
   const int size = dtype == 2 ? 4 : 2;
   if (dtype < 0 || dtype > 2 || B < 0 || T < 0 || H < 1 || Hkv < 1 || H % Hkv || D < 1 || D > 128 || D * size % 16) {
     gbh::set_error("gb_cache_attn: bad type or sizes (type %d, %d sequences, %d tokens, %d and %d heads of %d)", dtype, B, T, H, Hkv, D);
     return gbh::E_BAD_ARG;
   }
   if (B == 0 || T == 0) return gbh::E_OK;
-  if (!q || !k || !v || !out || !table || !lengths || !strides || page < 1 || columns < 1 || pages < 1) {
+  if (!q || !k || !v || !out || !table || !lengths || page < 1 || columns < 1 || pages < 1) {
     gbh::set_error("gb_cache_attn: null pointer or empty cache");
     return gbh::E_BAD_ARG;
   }

@@ -60,7 +60,12 @@ template <> struct VecOf<2> { using type = uint16_t; };
 template <typename T, int V>
 struct Pack {
   T e[V];
-  __device__ __forceinline__ void load(const T* p) { *reinterpret_cast<typename VecOf<V * sizeof(T)>::type*>(e) = *reinterpret_cast<const typename VecOf<V * sizeof(T)>::type*>(p); }
+  // CONST: nothing writes there meanwhile.  Four prompts appended: 38.4 us so, 48.1 with loads that might see a store.
+  template <bool CONST>
+  __device__ __forceinline__ void load(const T* p) {
+    using U = typename VecOf<V * sizeof(T)>::type;
+    *reinterpret_cast<U*>(e) = CONST ? __ldg(reinterpret_cast<const U*>(p)) : *reinterpret_cast<const U*>(p);
+  }
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<typename VecOf<V * sizeof(T)>::type*>(p) = *reinterpret_cast<const typename VecOf<V * sizeof(T)>::type*>(e); }
 };
 
@@ -105,7 +110,7 @@ __device__ __forceinline__ void turn(Pack<T, V>& u, Pack<T, V>& w, const float2*
 }
 
 // A head of any part is `items` items of two vectors: half / V turned ones, then the rest (of values: all of it) as it lies.
-template <typename T, int V, bool INTER, bool APPEND>
+template <typename T, int V, bool INTER, bool APPEND, bool IN_PLACE>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
   if (a.early) pdl_trigger();
   const int items = (a.width + 2 * V - 1) / (2 * V), heads = APPEND ? a.q.heads + 2 * a.k.heads : a.q.heads;
@@ -137,8 +142,8 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
     const T* src = (const T*)of(x.which, a.q.src, a.k.src, a.v.src) + b * of(x.which, a.q.sb, a.k.sb, a.v.sb) +
                    t * of(x.which, a.q.st, a.k.st, a.v.st) + h * of(x.which, a.q.sh, a.k.sh, a.v.sh);
     const int at = value ? flat : first, to = value ? flat + V : second;
-    x.u.load(src + at);
-    if (to < a.width) x.w.load(src + to);
+    x.u.template load<!IN_PLACE>(src + at);
+    if (to < a.width) x.w.template load<!IN_PLACE>(src + to);
   };
   // kHeads heads at a time, the first ones on their way before anything else is known.
   Pair x[kHeads];
@@ -217,8 +222,14 @@ int launch_rotary(RotaryArgs& a, int inter, cudaStream_t s) {
   }
   const unsigned ctas = (unsigned)((threads + kThreads - 1) / kThreads);
   a.early = starts_early((long long)kThreads * per * 4 * V * sizeof(T), ctas);
-  if (inter) GB_CUDA_OK(gbh::launch_if(a.early, rotary_kernel<T, V, true, APPEND>, dim3(ctas), dim3(kThreads), 0, s, a));
-  else GB_CUDA_OK(gbh::launch_if(a.early, rotary_kernel<T, V, false, APPEND>, dim3(ctas), dim3(kThreads), 0, s, a));
+  const auto go = [&](auto kernel) { return gbh::launch_if(a.early, kernel, dim3(ctas), dim3(kThreads), 0, s, a); };
+  if constexpr (!APPEND) {
+    if (a.q.src == a.q.dst) {
+      GB_CUDA_OK(inter ? go(rotary_kernel<T, V, true, false, true>) : go(rotary_kernel<T, V, false, false, true>));
+      return gbh::E_OK;
+    }
+  }
+  GB_CUDA_OK(inter ? go(rotary_kernel<T, V, true, APPEND, false>) : go(rotary_kernel<T, V, false, APPEND, false>));
   return gbh::E_OK;
 }
 
@@ -279,55 +290,66 @@ int checked(const char* what, int dtype, const RotaryArgs& a) {
 
 }  // namespace
 
-// y = x turned, both (batch, tokens, heads, width) with strides (batch, token, head, in elements); y may be x.  positions: int32 or int64 with strides (0 where
-// shared), or null for 0, 1, ...
-GB_EXPORT int gb_rotary(int dtype, const void* x, long long sb, long long st, long long sh, void* y, long long yb, long long yt, long long yh, int batch, int tokens, int heads, int width,
-                        int dim, int interleaved, const void* turns, double amplitude, int back, const void* positions, int positions64,
-                        long long pb, long long pt, void* stream) {
+// Sizes and strides (in elements) come as one array of 64-bit words: a call of many arguments costs its caller more than the launch.
+
+// y = x turned, both (batch, tokens, heads, width); y may be x.  sizes: [0..2] strides of x (batch, token, head), [3..5] of y, [6..9] batch, tokens,
+// heads, width, [10] columns that are turned, [11] pairs side by side, [12] turn back, [13] positions are int64, [14..15] their strides (batch, token; 0
+// where shared).  positions: null for 0, 1, ...
+GB_EXPORT int gb_rotary(int dtype, const void* x, void* y, const long long* sizes, const void* turns, const void* positions, double amplitude,
+                        void* stream) {
+  if (!sizes) {
+    gbh::set_error("gb_rotary: null pointer");
+    return gbh::E_BAD_ARG;
+  }
+  const long long* z = sizes;
   RotaryArgs a = {};
-  a.q = {x, y, sb, st, sh, yb, yh, yt, heads};
-  a.batch = batch; a.tokens = tokens; a.width = width; a.dim = dim; a.half = dim / 2;
+  a.q = {x, y, z[0], z[1], z[2], z[3], z[5], z[4], (int)z[8]};
+  a.batch = (int)z[6]; a.tokens = (int)z[7]; a.width = (int)z[9]; a.dim = (int)z[10]; a.half = a.dim / 2;
   a.turns = (const unsigned long long*)turns;
   a.amplitude = (float)amplitude;
-  a.back = back;
-  a.positions = positions; a.positions64 = positions64; a.pb = pb; a.pt = pt;
+  a.back = (int)z[12];
+  a.positions = positions; a.positions64 = (int)z[13]; a.pb = z[14]; a.pt = z[15];
   const int rc = checked("gb_rotary", dtype, a);
   if (rc != gbh::E_OK) return rc;
-  if (batch == 0 || tokens == 0 || heads == 0) return gbh::E_OK;
+  if (a.batch == 0 || a.tokens == 0 || a.q.heads == 0) return gbh::E_OK;
   if (!x || !y) {
     gbh::set_error("gb_rotary: null pointer");
     return gbh::E_BAD_ARG;
   }
   a.vec = vector_of(dtype == 2 ? 4 : 2, a);
-  return dispatch<false>(dtype, a, interleaved, (cudaStream_t)stream);
+  return dispatch<false>(dtype, a, (int)z[11], (cudaStream_t)stream);
 }
 
 // k and v (batch, tokens, heads, width) into the pages of their sequences, k turned (dim 0: as it is); q, where there is one, turned
-// into q_out.  Strides in elements: of q, k, v (batch, token, head), of both caches (page, head, row: strides[0..5]).
-GB_EXPORT int gb_cache_append(int dtype, const void* q, long long q_sb, long long q_st, long long q_sh, void* q_out, const void* k, long long k_sb,
-                              long long k_st, long long k_sh, const void* v, long long v_sb, long long v_st, long long v_sh, void* k_cache,
-                              void* v_cache, const long long* strides, int batch, int tokens, int q_heads, int heads, int width, int dim, int interleaved,
-                              const void* turns, double amplitude, const void* table, long long table_stride, int columns, int pages, int page,
-                              const void* lengths, const void* counts, void* stream) {
+// into q_out (contiguous).  sizes: [0..8] strides of q, k, v (batch, token, head), [9..14] of both caches (page, head, row), [15..19] batch, tokens, heads of
+// queries and of keys, width, [20] columns that are turned, [21] pairs side by side, [22] the table's stride, [23] its columns, [24] pages, [25] positions
+// of a page.
+GB_EXPORT int gb_cache_append(int dtype, const void* q, void* q_out, const void* k, const void* v, void* k_cache, void* v_cache, const long long* sizes,
+                              const void* turns, double amplitude, const void* table, const void* lengths, const void* counts, void* stream) {
+  if (!sizes) {
+    gbh::set_error("gb_cache_append: null pointer");
+    return gbh::E_BAD_ARG;
+  }
+  const long long* z = sizes;
   RotaryArgs a = {};
-  const long long zero[6] = {0, 0, 0, 0, 0, 0}, *s = strides ? strides : zero;
-  a.q = {q, q_out, q_sb, q_st, q_sh, (long long)tokens * q_heads * width, width, (long long)q_heads * width, q ? q_heads : 0};
-  a.k = {k, k_cache, k_sb, k_st, k_sh, s[0], s[1], s[2], heads};
-  a.v = {v, v_cache, v_sb, v_st, v_sh, s[3], s[4], s[5], heads};
-  a.batch = batch; a.tokens = tokens; a.width = width; a.dim = dim; a.half = dim / 2;
+  a.batch = (int)z[15]; a.tokens = (int)z[16]; a.width = (int)z[19]; a.dim = (int)z[20]; a.half = a.dim / 2;
+  const int q_heads = q ? (int)z[17] : 0, heads = (int)z[18];
+  a.q = {q, q_out, z[0], z[1], z[2], (long long)a.tokens * q_heads * a.width, a.width, (long long)q_heads * a.width, q_heads};
+  a.k = {k, k_cache, z[3], z[4], z[5], z[9], z[10], z[11], heads};
+  a.v = {v, v_cache, z[6], z[7], z[8], z[12], z[13], z[14], heads};
   a.turns = (const unsigned long long*)turns;
   a.amplitude = (float)amplitude;
-  a.table = (const int*)table; a.table_stride = table_stride; a.columns = columns; a.pages = pages; a.page = page;
+  a.table = (const int*)table; a.table_stride = z[22]; a.columns = (int)z[23]; a.pages = (int)z[24]; a.page = (int)z[25];
   a.lengths = (const int*)lengths;
   a.counts = (const int*)counts;
   const int rc = checked("gb_cache_append", dtype, a);
   if (rc != gbh::E_OK) return rc;
-  if (batch == 0 || tokens == 0) return gbh::E_OK;
-  if (!k || !v || !k_cache || !v_cache || !strides || !table || !lengths || (q && !q_out) || page < 1 || columns < 1 || pages < 1 || heads < 1) {
+  if (a.batch == 0 || a.tokens == 0) return gbh::E_OK;
+  if (!k || !v || !k_cache || !v_cache || !table || !lengths || (q && !q_out) || a.page < 1 || a.columns < 1 || a.pages < 1 || heads < 1) {
     gbh::set_error("gb_cache_append: null pointer or empty cache");
     return gbh::E_BAD_ARG;
   }
   a.status = gbh::status_ptr();
   a.vec = vector_of(dtype == 2 ? 4 : 2, a);
-  return dispatch<true>(dtype, a, interleaved, (cudaStream_t)stream);
+  return dispatch<true>(dtype, a, (int)z[21], (cudaStream_t)stream);
 }

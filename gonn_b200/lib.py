@@ -36,8 +36,7 @@ _ARGUMENTS = {
     "gb_mx_add_rms_norm": "iipLpLpipppLLdp", "gb_mx_matmul": "ipppppLpiLLLiip", "gb_mx_matmul_rows": "iipLpppLpiLLLiip",
     "gb_mx_linear": "iipLppppiLLLiipLp",
     "gb_mx_train_forward": "iipLpLppiLLLiipLpLp", "gb_mx_train_backward": "ipLppipipiLLLpLp",
-    "gb_rotary": "ipLLLpLLLiiiiiipdipiLLp", "gb_cache_append": "ipLLLppLLLpLLLpppiiiiiiipdpLiiippp",
-    "gb_cache_attn": "ipLLLppppiiiiipLiiippidpLp", "gb_cache_attn_bytes": "iLLLLLiL", "gb_cache_attn_kernels": "iLLLLLiL",
+    "gb_rotary": "ipppppdp", "gb_cache_append": "ippppppppdpppp", "gb_cache_attn": "ipppppppp" "dpLp", "gb_cache_attn_bytes": "iLLLLLiL", "gb_cache_attn_kernels": "iLLLLLiL",
     "gb_mx_plan": "LLLip", "gb_mx_linear_bytes": "LLLi", "gb_mx_train_bytes": "LLLiii",
 }
 

@@ -5,14 +5,13 @@ nothing here has a gradient."""
 from __future__ import annotations
 
 import math
-from ctypes import c_longlong
 from functools import lru_cache
 from typing import Optional
 
 import torch
 
 from .. import lib as _l
-from .rotary import _TYPES, rotate_ref
+from .rotary import _TYPES, rotate_ref, words
 
 MAX_HEAD = 128                    # largest head that attention on CUDA takes
 
@@ -38,7 +37,7 @@ class Layout:
         self.keys, self.values, self.dtype, self.code = keys, values, keys.dtype, _TYPES.get(keys.dtype)
         self.device, self.index = keys.device, keys.get_device()
         self.pages, self.heads, self.page, self.width = keys.shape
-        self.strides = (c_longlong * 6)(*keys.stride()[:3], *values.stride()[:3])
+        self.strides = (*keys.stride()[:3], *values.stride()[:3])
         self.scale = 1.0 / math.sqrt(self.width)
 
 
@@ -110,15 +109,15 @@ def append(c: Layout, k, v, table, lengths, counts=None, rope=None, q=None):
     if q is not None:
         q = _rows(q)
         q_heads = q.shape[2]
-        out = torch.empty((batch, tokens, q_heads, width), dtype=c.dtype, device=c.device)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
         q_at, out_at = q.data_ptr(), out.data_ptr()
         qsb, qst, qsh, _ = q.stride()
     if counts is not None:
         counts = _line(counts)
-    _l.call_on(c.index, "gb_cache_append", c.code, q_at, qsb, qst, qsh, out_at, k.data_ptr(), ksb, kst, ksh, v.data_ptr(), vsb, vst, vsh,
-               c.keys.data_ptr(), c.values.data_ptr(), c.strides, batch, tokens, q_heads, heads, width, dim, interleaved,
-               None if turns is None else turns.data_ptr(), amplitude, table.data_ptr(), table.stride(0), table.shape[1], c.pages, c.page,
-               lengths.data_ptr(), None if counts is None else counts.data_ptr())
+    _l.call_on(c.index, "gb_cache_append", c.code, q_at, out_at, k.data_ptr(), v.data_ptr(), c.keys.data_ptr(), c.values.data_ptr(),
+               words(qsb, qst, qsh, ksb, kst, ksh, vsb, vst, vsh, *c.strides, batch, tokens, q_heads, heads, width, dim, interleaved, table.stride(0),
+                     table.shape[1], c.pages, c.page),
+               None if turns is None else turns.data_ptr(), amplitude, table.data_ptr(), lengths.data_ptr(), None if counts is None else counts.data_ptr())
     return out
 
 
@@ -148,12 +147,14 @@ def _append_ref(c, k, v, table, lengths, counts, w, interleaved, amplitude, q):
     return torch.where(live[..., None, None], rotate_ref(q.detach(), at, w, interleaved, amplitude), torch.zeros((), dtype=q.dtype))
 
 
-@lru_cache(maxsize=1024)
-def _needs(*sizes):
-    """(bytes of the workspace, kernels beyond the first one) of a call."""
-    n = _l.lib().gb_cache_attn_bytes(*sizes)
+@lru_cache(maxsize=4096)
+def _plan(code, *sizes):
+    """(sizes for the native call, bytes of its workspace, kernels beyond the first one)."""
+    batch, tokens, heads, kv, width, _, columns, _, page, prefix = sizes[9:]
+    of = code, batch, tokens, heads, kv, width, prefix, columns * page
+    n = _l.lib().gb_cache_attn_bytes(*of)
     _l.check(min(n, 0), "gb_cache_attn_bytes")
-    return n, _l.lib().gb_cache_attn_kernels(*sizes) - 1
+    return words(*sizes), n, _l.lib().gb_cache_attn_kernels(*of) - 1
 
 
 def attend(c: Layout, q, table, lengths, counts=None, scale: Optional[float] = None, shared_pages: int = 0):
@@ -176,7 +177,7 @@ def attend(c: Layout, q, table, lengths, counts=None, scale: Optional[float] = N
         return _attend_ref(c, q, table, lengths, counts, scale, shared_pages)
     if width > MAX_HEAD:
         raise ValueError(f"{what}: heads of up to {MAX_HEAD} columns on CUDA, got {width}")
-    out = torch.empty((batch, tokens, heads, width), dtype=c.dtype, device=c.device)
+    out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
     if batch == 0 or tokens == 0:
         return out
     sb, st, sh, sd = q.stride()
@@ -188,12 +189,11 @@ def attend(c: Layout, q, table, lengths, counts=None, scale: Optional[float] = N
         counts = _line(counts)
     if table.stride(1) != 1:
         table = table.contiguous()
-    prefix = shared_pages * c.page
-    need, more = _needs(c.code, batch, tokens, heads, kv, width, prefix, columns * c.page)
-    ws = torch.empty(need, dtype=torch.uint8, device=c.device) if need else None
-    _l.call_on(c.index, "gb_cache_attn", c.code, q.data_ptr(), sb, st, sh, c.keys.data_ptr(), c.values.data_ptr(), c.strides, out.data_ptr(),
-               batch, tokens, heads, kv, width, table.data_ptr(), table.stride(0), columns, c.pages, c.page, lengths.data_ptr(),
-               None if counts is None else counts.data_ptr(), prefix, scale, None if ws is None else ws.data_ptr(), need)
+    sizes, need, more = _plan(c.code, sb, st, sh, *c.strides, batch, tokens, heads, kv, width, table.stride(0), columns, c.pages, c.page,
+                              shared_pages * c.page)
+    ws = q.new_empty(need, dtype=torch.uint8) if need else None
+    _l.call_on(c.index, "gb_cache_attn", c.code, q.data_ptr(), c.keys.data_ptr(), c.values.data_ptr(), out.data_ptr(), sizes, table.data_ptr(),
+               lengths.data_ptr(), None if counts is None else counts.data_ptr(), scale, None if ws is None else ws.data_ptr(), need)
     _l.kernel_count += more
     return out
 

@@ -5,6 +5,8 @@ operations, angles in fp64."""
 from __future__ import annotations
 
 import math
+from ctypes import c_longlong
+from functools import lru_cache
 from typing import Optional, Sequence
 
 import torch
@@ -52,20 +54,26 @@ def rotate_ref(x: torch.Tensor, positions: torch.Tensor, w: Sequence[float], int
     return torch.cat((part, rest), -1).to(x.dtype)
 
 
+@lru_cache(maxsize=4096)
+def words(*sizes: int):
+    """Sizes and strides as the native library takes them.  (A call of eight arguments with such an array takes the host 3 us less than one of 24.)"""
+    return (c_longlong * len(sizes))(*sizes)
+
+
 def _launch(x, positions, turns, interleaved, amplitude, back, out=None):
-    batch, tokens, heads, width = x.shape
+    shape = x.shape
+    batch, tokens, heads, width = shape
     if x.stride(3) != 1 and width > 1:
         x = x.contiguous()
-    y = torch.empty((batch, tokens, heads, width), dtype=x.dtype, device=x.device) if out is None else out
-    if positions is None:
-        at, wide, pb, pt = None, 0, 0, 0
-    else:
-        at, wide = positions.data_ptr(), positions.dtype == torch.int64
-        pb, pt = (0, positions.stride(0)) if positions.dim() == 1 else positions.stride()
+    y = out if out is not None else torch.empty_like(x) if x.is_contiguous() else x.new_empty(shape)
+    at, wide, pb, pt = None, 0, 0, 0
+    if positions is not None:
+        at, wide = positions.data_ptr(), positions.dtype is torch.int64
+        pb, pt = positions.stride() if positions.dim() == 2 else (0, positions.stride(0))
     sb, st, sh, _ = x.stride()
     yb, yt, yh, _ = y.stride()
-    _l.call_on(x.get_device(), "gb_rotary", _TYPES[x.dtype], x.data_ptr(), sb, st, sh, y.data_ptr(), yb, yt, yh, batch, tokens, heads, width,
-               2 * turns.shape[0], interleaved, turns.data_ptr(), amplitude, back, at, wide, pb, pt)
+    _l.call_on(x.get_device(), "gb_rotary", _TYPES[x.dtype], x.data_ptr(), y.data_ptr(),
+               words(sb, st, sh, yb, yt, yh, batch, tokens, heads, width, 2 * turns.shape[0], interleaved, back, wide, pb, pt), turns.data_ptr(), at, amplitude)
     return y
 
 

@@ -10,6 +10,10 @@
     python -m gonn_b200.utils.profile_cases conv 256 64 128 15 15     # N C_in C_out H W, 3x3: forward + backward
     python -m gonn_b200.utils.profile_cases general_attn 4 512 8 64 [bf16|fp32|fp64] [plain]
                                                                        # B S H D: masked + dropout attention, fwd and bwd
+    python -m gonn_b200.utils.profile_cases rotary 16 1024 24 64       # B S H D: rotary positions
+    python -m gonn_b200.utils.profile_cases append 4 2048 16 16 128    # B S H KV D: keys and values into a paged cache, queries turned
+    python -m gonn_b200.utils.profile_cases attend 32 1 8192 32 8 128 [page] [shared positions]
+                                                                       # B S positions H KV D: attention of new tokens from the cache
     python -m gonn_b200.utils.profile_cases suite                      # one launch or two of every other kernel family
     python -m gonn_b200.utils.profile_cases suite2                     # ... and of the families `suite` leaves out
     python -m gonn_b200.utils.profile_cases suite3                     # LSTM layer, convolutions, few-tile and exact products,
@@ -41,6 +45,37 @@ def _time(fn, iters=5):
     return e0.elapsed_time(e1) / iters
 
 
+def _cache_case(kind, n):
+    """Rotary positions and the paged cache, bf16."""
+    from .. import nn
+    bf, name = dict(device="cuda", dtype=torch.bfloat16), " ".join(map(str, n))
+    if kind == "rotary":
+        B, S, H, D = n
+        x, rope = torch.randn(B, S, H, D, **bf), nn.RotaryEmbedding(D, device="cuda")
+        ms, work = _time(lambda: rope(x)), 4 * x.numel()
+    else:
+        L, (B, S) = (0 if kind == "append" else n.pop(2)), n[:2]
+        H, KV, D = n[2:5]
+        page, shared = (n[5:] + [64, 0])[:2] if len(n) != 6 else (n[5], 0)
+        columns = -(-(L + S) // page)
+        cache = nn.KVCache(B * columns, page, KV, D, **bf)
+        cache.Keys.normal_()
+        cache.Values.normal_()
+        table = torch.randperm(B * columns, device="cuda").view(B, columns).int()
+        table[:, :shared // page] = table[0, :shared // page].clone()
+        at = torch.full((B,), L, device="cuda", dtype=torch.int32)
+        q, k, v = (torch.randn(B, S, h, D, **bf) for h in (H, KV, KV))
+        if kind == "append":
+            rope = nn.RotaryEmbedding(D, device="cuda")
+            ms, work = _time(lambda: cache.Append(k, v, table, at, rotary=rope, q=q)), 4 * (q.numel() + 2 * k.numel())
+        else:
+            ms = _time(lambda: cache.Attend(q, table, at, shared_pages=shared // page))
+            flop = 4 * B * H * D * S * (L + (S + 1) / 2)
+            work = 2 * (2 * KV * D * (shared + B * (L + S - shared)) + 2 * q.numel())
+            print(f"{flop / ms / 1e9:.1f} TFLOP/s")
+    print(f"{kind} {name}: {ms * 1e3:.1f} us, {work / ms / 1e6:.0f} GB/s")
+
+
 def main(argv):
     from .. import lib
     from ..ops.attention import flash_bwd, flash_fwd
@@ -48,6 +83,8 @@ def main(argv):
     from ..ops.norm import layer_norm
     kind = argv[0]
     dev = "cuda"
+    if kind in ("rotary", "append", "attend"):
+        return _cache_case(kind, [int(a) for a in argv[1:]])
     if kind == "gemm":
         M, N, K = (int(a) for a in argv[1:4])
         layout = argv[4] if len(argv) > 4 else "nt"
