@@ -848,8 +848,8 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 #pragma unroll
             for (int d = 1; d < LPK; d <<= 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], d);
             const int sees = s_sees[sg * ROWS + r];
-            const float x = key < min(sees ? sees : 0x7fffffff, seg.end) ? s[r] * a.scale_log2 : -INFINITY;
-            float top = x;
+            const float x = key < min(sees ? sees : 0x7fffffff, seg.end) ? s[r] : -INFINITY;
+            float top = x * a.scale_log2;
 #pragma unroll
             for (int d = LPK; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             if (top > m[r]) {
@@ -859,7 +859,8 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 #pragma unroll
               for (int c = 0; c < CPL; c++) o[r][c] *= f;
             }
-            s[r] = exp2f(x - (m[r] == -INFINITY ? 0.f : m[r]));
+            // (scaled and subtracted in one rounding)
+            s[r] = exp2f(fmaf(x, a.scale_log2, m[r] == -INFINITY ? 0.f : -m[r]));
             l[r] += slice == 0 ? s[r] : 0.f;                         // this lane's keys; summed over lanes at the end
           }
           if (slice == 0) {
