@@ -514,7 +514,8 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         if (RW < PER && sub >= RW) break;
         const long long from = s_from[r0 + sub];
         const int bytes = from >= 0 && inside ? 16 : 0;
-        cp_async16(dq + chunk_at<ROWS>(r0 + sub, chunk), (const T*)a.q + (bytes ? from + chunk * (16 / (int)sizeof(T)) : 0), bytes);
+        // (fp32: rows as they are, which all lanes read alike, at offsets that the compiler knows)
+        cp_async16(dq + (C::kMma ? chunk_at<ROWS>(r0 + sub, chunk) : (uint32_t)((r0 + sub) * C::CHUNKS + chunk) * 16), (const T*)a.q + (bytes ? from + chunk * (16 / (int)sizeof(T)) : 0), bytes);
       }
       __syncwarp();
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&seg_full[sg])) : "memory");
@@ -831,36 +832,55 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           float s[ROWS];
 #pragma unroll
           for (int r = 0; r < ROWS; r++) s[r] = 0.f;
-#pragma unroll 2
-          for (int c = slice; c < HD / 4; c += LPK) {
-            const float4 kk = *reinterpret_cast<const float4*>(kt + chunk_at<TILE>(warp * KW + mykey, c));
+          const uint8_t* mine = q + slice * 16;
+#pragma unroll 4
+          for (int c = 0; c < HD / 4 / LPK; c++) {
+            const float4 kk = *reinterpret_cast<const float4*>(kt + chunk_at<TILE>(warp * KW + mykey, c * LPK + slice));
 #pragma unroll
             for (int r = 0; r < ROWS; r++) {
-              const float4 qq = *reinterpret_cast<const float4*>(q + chunk_at<ROWS>(r, c));
+              const float4 qq = *reinterpret_cast<const float4*>(mine + (r * (HD / 4) + c * LPK) * 16);
               s[r] = fmaf(qq.x, kk.x, s[r]);
               s[r] = fmaf(qq.y, kk.y, s[r]);
               s[r] = fmaf(qq.z, kk.z, s[r]);
               s[r] = fmaf(qq.w, kk.w, s[r]);
             }
           }
+          // (step by step over all rows, whose exchanges between lanes do not wait for one another: row by row they took 2 us of a tile's 6)
+#pragma unroll
+          for (int d = 1; d < LPK; d <<= 1)
+#pragma unroll
+            for (int r = 0; r < ROWS; r++) s[r] += __shfl_xor_sync(0xffffffffu, s[r], d);
+          float top[ROWS];
 #pragma unroll
           for (int r = 0; r < ROWS; r++) {
-#pragma unroll
-            for (int d = 1; d < LPK; d <<= 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], d);
             const int sees = s_sees[sg * ROWS + r];
-            const float x = key < min(sees ? sees : 0x7fffffff, seg.end) ? s[r] : -INFINITY;
-            float top = x * a.scale_log2;
+            s[r] = key < min(sees ? sees : 0x7fffffff, seg.end) ? s[r] : -INFINITY;
+            top[r] = s[r];
+          }
 #pragma unroll
-            for (int d = LPK; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            if (top > m[r]) {
-              const float f = m[r] == -INFINITY ? 0.f : exp2f(m[r] - top);
-              m[r] = top;
+          for (int d = LPK; d < 32; d <<= 1)
+#pragma unroll
+            for (int r = 0; r < ROWS; r++) top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], d));
+          bool moved = false;
+#pragma unroll
+          for (int r = 0; r < ROWS; r++) {
+            top[r] = fmaxf(m[r], top[r] * a.scale_log2);
+            moved |= top[r] > m[r];
+          }
+          if (moved) {                                               // (the same for all lanes)
+#pragma unroll
+            for (int r = 0; r < ROWS; r++) {
+              const float f = m[r] == -INFINITY ? 0.f : exp2f(m[r] - top[r]);
+              m[r] = top[r];
               l[r] *= f;
 #pragma unroll
               for (int c = 0; c < CPL; c++) o[r][c] *= f;
             }
+          }
+#pragma unroll
+          for (int r = 0; r < ROWS; r++) {
             // (scaled and subtracted in one rounding)
-            s[r] = exp2f(fmaf(x, a.scale_log2, m[r] == -INFINITY ? 0.f : -m[r]));
+            s[r] = exp2f(fmaf(s[r], a.scale_log2, m[r] == -INFINITY ? 0.f : -m[r]));
             l[r] += slice == 0 ? s[r] : 0.f;                         // this lane's keys; summed over lanes at the end
           }
           if (slice == 0) {
@@ -868,6 +888,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
             for (int r = 0; r < ROWS; r += 4) *reinterpret_cast<float4*>(s_p + mykey * ROWS + r) = make_float4(s[r], s[r + 1], s[r + 2], s[r + 3]);
           }
           __syncwarp();
+#pragma unroll 4
           for (int j = 0; j < there; j++) {                          // (rows of V behind the last key are not read)
             float v[CPL];
             const uint8_t* vr = vt + chunk_at<TILE>(warp * KW + j, lane * CPL / 4);

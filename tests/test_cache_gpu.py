@@ -191,7 +191,11 @@ ATTEND = [
     (1, 1, 1, 1, 64, 16, [0], None), (1, 1, 16, 16, 128, 64, [2047], None), (3, 1, 8, 2, 128, 16, [5, 0, 700], None), (2, 5, 6, 2, 64, 24, [100, 3], None),
     (5, 3, 4, 4, 72, 1, [0, 1, 63, 64, 65], [3, 0, 2, 1, -1]), (1, 40, 12, 3, 128, 33, [500], None), (2, 300, 2, 1, 64, 64, [0, 77], [300, 13]),
     (7, 1, 40, 1, 128, 128, [0, 10, 200, 300, 4000, 31, 32], None), (150, 1, 2, 1, 16, 8, list(range(150)), None), (1, 2, 2, 2, 8, 5, [20000], None),
-    (2, 17, 8, 1, 104, 200, [1, 1500], [17, 16]), (400, 2, 1, 1, 24, 16, [0] * 399 + [900], [0] * 399 + [2])]
+    (2, 17, 8, 1, 104, 200, [1, 1500], [17, 16]),
+    # 6, 10, 24 and 48 rows to a key head: in clusters, and dealt out
+    (3, 2, 12, 4, 128, 16, [10, 300, 77], None), (3, 2, 12, 4, 128, 16, [10, 300, 15000], None), (2, 2, 6, 2, 64, 64, [9000, 8190], [2, 1]),
+    (2, 2, 10, 2, 128, 7, [9001, 3], None), (3, 5, 4, 2, 64, 64, [9000, 77, 9999], [5, 0, 3]), (2, 6, 8, 2, 128, 64, [9000, 4444], None),
+    (1, 12, 4, 1, 72, 24, [12345], None), (400, 2, 1, 1, 24, 16, [0] * 399 + [900], [0] * 399 + [2])]
 
 
 @pytest.mark.parametrize("dtype", [BF, F16, F32])
@@ -339,9 +343,12 @@ def test_other_streams_and_graphs():
     rope2 = nn.RotaryEmbedding(32, interleaved=True, device="cuda")
 
     def step(cache, rope, k, v, table, at, q):
-        return cache.Attend(cache.Append(k, v, table, at, rotary=rope, q=q), table, at)
+        return cache.Attend(cache.Append(k, v, table, at, rotary=rope, q=q), table, at, shared_pages=25 if table.shape[0] == 70 else 0)
 
-    args = (cache, rope, k, v, table, at, q), (other, rope2, k2, v2, table2, at2, q2)
+    # a batch over its shared prefix, which two kernels take side by side, and a third joins
+    wide, table3, at3, c3, new = batch(70, 2, 4, 1, 64, 16, [400 + i for i in range(70)], BF, prefix=25)
+    q3, k3, v3 = (t[:, :1] for t in new)
+    args = (cache, rope, k, v, table, at, q), (other, rope2, k2, v2, table2, at2, q2), (wide, rope2, k3, v3, table3, at3, q3)
     side = [torch.cuda.Stream() for _ in args]
     graphs, outs = [], []
     for s, a in zip(side, args):
@@ -355,7 +362,7 @@ def test_other_streams_and_graphs():
         graphs.append(g)
     for shift in (0, 1, 0):
         at += shift
-        at2 += 0
+        at3 += shift
         torch.cuda.synchronize()
         for _ in range(20):
             for s, g in zip(side, graphs):
@@ -460,6 +467,23 @@ def test_model_steps_in_a_graph():
         steps = float((torch.cat(outs, 1).cpu().double() - want).abs().max())
     # two ways through the same fp32 products: neither is off by much more than the other
     assert steps <= 4 * whole + 2.0 ** -20 * float(want.abs().max()), (steps, whole)
+
+
+def test_blocks_with_rotary_are_not_evaluated_without_it():
+    """The native evaluation of a block knows no rotation and leaves such blocks alone."""
+    from gonn_b200.models import GPT
+    from gonn_b200.nn import block
+    for rotary in (None, True):
+        model = GPT(vocab=31, d_model=128, n_layers=1, n_heads=2, d_ff=256, max_seq=32, rotary=rotary, dtype=BF, device="cuda")
+        x = torch.randn(1, 20, 128, device="cuda").to(BF)
+        with torch.no_grad():
+            assert (block.evaluate(x, *model.layers[0]._parts()) is None) == (rotary is not None)
+            ids = torch.randint(0, 31, (1, 20), device="cuda")
+            taped = None
+            with torch.enable_grad():
+                taped = model(ids).detach()
+            # two ways through the same layers in bf16: sixteen roundings, at the size of the largest logit
+            assert float((model(ids).double() - taped.double()).abs().max()) <= 16 * half(BF) * float(taped.double().abs().max())
 
 
 def test_samples_share_the_prompt():
