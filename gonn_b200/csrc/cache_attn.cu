@@ -3,23 +3,26 @@
 // Token t < counts[b] of sequence b sits at position lengths[b] + t and sees the positions up to its own:
 // o = sum_j p_j v_j / sum_j p_j with p_j = exp(scale q . k_j - m).  One pass over the keys with the running maximum m and sum l of
 // each row, in fp32; H / Hkv query heads share a key head and are rows of one tile.  The weights p are at most 1 and are rounded to the
-// inputs' type for the second product (2^-9 of each, as in csrc/flash_attn.cu); their sum is taken before that.
+// inputs' type for the second product (2^-9 of each in bf16, as in csrc/flash_attn.cu; in the kernel for many rows they are at most 2^8, which changes
+// nothing of that); their sum is taken before.
 //
-// What bounds it: every key and value is read once for a few rows of queries, so memory does.  The work is a list of tiles of kTile keys:
+// What bounds it: every key and value is read once for a few rows of queries, so memory does (64 sequences of up to 32 768 positions, 32 / 8 heads
+// of 128 bf16: 722 us, 7.0 TB/s).  The work is a list of tiles of 32 KB of keys and values:
 // sequence by sequence, key head by key head.  Its length is known on the device alone (lengths[]), so every CTA adds the
 // lengths up itself and takes an equal share of the list, across sequences and heads: no plan, no host, no idle SM with ragged
 // lengths.  A (sequence, head) whose tiles fall to several CTAs leaves partial rows (m, l, o) behind, which a second kernel joins in
 // the list's order; no atomics.
 //
 // Where few (sequence, head) pairs have short tables, a cluster of up to eight CTAs takes each of them, and their sums meet in distributed shared
-// memory instead: no second kernel, which is half of such a call's time.
+// memory instead: no second kernel (one token behind 2 047 positions of 16 heads: 9.6 us, 14.7 with it).
 //
 // A shared prefix is one more entry at the head of the list whose rows are the queries of all sequences: its keys are read once for
 // every 16, 32 or 64 rows.  The sequences' own entries then start behind it, and all rows are joined by the second kernel.
 //
-// A CTA: four warps that multiply (mma.sync for 16-bit types, FMA for fp32) and one that copies through a ring of stages: by TMA, a box of
+// A CTA: four warps that multiply (mma.sync for 16-bit types, FMA for fp32) and four that copy through a ring of stages: by TMA, a box of
 // as many rows as divide both a page and a tile, where these are at least eight (a multiple of the swizzle's period); else with cp.async,
-// 16 bytes a lane, a page looked up for every key.  What stands behind a sequence's last key in its last page may be anything, NaN
+// 16 bytes a lane, a page looked up for every key (64 sequences of up to 8 192 positions: pages of 64 222 us, of 8 225, of 4 250; with one
+// copying warp 228, 368, 396).  What stands behind a sequence's last key in its last page may be anything, NaN
 // too: those scores are masked, and those rows of V become zeros in shared memory.
 #include "common.cuh"
 #include "pair.cuh"
@@ -965,7 +968,8 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 // bytes, and a CTA takes 128 rows over a run of keys: scores and sums in TMEM, Q in shared memory, K and V by TMA in sub-tiles of 64
 // keys, weights written over their scores as the second product's operand; two score buffers, so that the next scores are computed while
 // a softmax warp (a row a thread) works.  The sum is rescaled only when the maximum has moved by more than 2^8.  Where the row tiles are too few
-// for the SMs, the keys are cut into `splits` runs, which leave partial rows.
+// for the SMs, the keys are cut into `splits` runs, which leave partial rows.  Four prompts of 2048 tokens behind 2048 others, 16 heads of 128 bf16:
+// 190 us, 972 TFLOP/s of the pairs that are seen; a softmax warp's chain bounds it (tensor pipe 51 % busy, exponentials 52 %).
 constexpr int kWideRows = 128, kWideKeys = 64, kWideThreads = 256, kWideCopiers = 3;
 
 template <int HD>
@@ -1466,7 +1470,6 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const CacheArgs a) {
 // host side
 // ---------------------------------------------------------------------------------------------------------------------------
 constexpr int kCtas = 2 * 148;
-constexpr int kClusterTiles = 8;
 constexpr long long kFewRows = 148 * 8;          // rows that are joined by eight warps each: those CTAs all fit at a time
 
 struct Sizes {
@@ -1483,6 +1486,9 @@ bool plan(Sizes& z, int dtype, long long B, long long T, long long H, long long 
   z = Sizes{};
   if (all >= 0x7fffffffLL) return false;
   // Many rows of a sequence: its keys with the prefix among them, nothing is gained by sharing.  Many rows of the batch alone: its prefix.
+  // us, few rows' kernel | this one, bf16, eight key heads of 128, 32, 48, 64, 96 rows to a key head: 8 sequences of 8 192 positions 63 | 60, 68 | 61, 70 | 62,
+  // 117 | 64; of 1 024 to 8 192 41 | 52, 50 | 54, 53 | 57; 64 such ones 211 | 241, 249 | 256, 263 | 254.  Heads of 64 37 | 39, 43 | 43, 45 | 44, 72 | 46.  A shared
+  // prefix of 16 384 (and 200 of its own for each sequence) 31 | 39, 37 | 40, 38 | 43, 51 | 46; 256 rows 91 | 57.
   const bool wide = dtype != 2;
   z.wide_own = wide && own > 64;
   const bool shared = prefix > 0 && !z.wide_own;
@@ -1502,15 +1508,17 @@ bool plan(Sizes& z, int dtype, long long B, long long T, long long H, long long 
   if (z.entries * Hkv >= 0x7fffffffLL) return false;
   z.own_tiles = (int)ot;
   z.prefix_tiles = (int)pt;
-  // A cluster for each (sequence, row tile, key head): as many CTAs, up to eight, as leave all of them on the SMs at a time.  The list is dealt out
-  // instead, which balances lengths over all CTAs but takes the second kernel (worth about kClusterTiles tiles), where that is less than what the longest
-  // sequence, a full table, costs more here than one of half its length with all CTAs at work.
+  // A cluster for each (sequence, row tile, key head): as many CTAs, up to eight, as leave all of them on the SMs at a time.  It saves the second
+  // kernel, 6 us, but the longest sequence's CTAs (a full table: `each` tiles at 0.75 us) may be at work when the others have ended, while
+  // the list, of half that length on average, takes 2.5 ns for each 32 KB tile on all SMs.  us, list | clusters, 16 heads of 128 bf16, equal lengths: one
+  // sequence of 1 000 positions 19.5 | 14.7, 4 000 20.5 | 15.8, 8 000 21.1 | 22.3, 16 000 34.0 | 38.7; four of 2 000 21.0 | 16.2, 8 000 53.2 | 47.1;
+  // sixteen of 500 21.3 | 15.5, 2 000 53.9 | 47.3.
   if (!shared && !z.wide_own && z.rows <= 16 && z.entries * Hkv <= kCtas) {
     const long long tile = 16384 / ((D <= 64 ? 64 : 128) * (dtype == 2 ? 4 : 2)), tiles = (room + tile - 1) / tile;
     z.peers = kPeers;
     while (z.peers > 1 && z.entries * Hkv * z.peers > kCtas) z.peers >>= 1;
     const long long each = (tiles + z.peers - 1) / z.peers, ctas = z.entries * Hkv * z.peers;
-    if (each * (2 * kCtas - ctas) > 2LL * kCtas * kClusterTiles) z.peers = 0;
+    if (each * (300 - ctas) > 2400) z.peers = 0;
     if (z.peers) return true;                                        // without a workspace
   }
   const long long rows = z.wide_own ? (z.splits > 1 ? z.splits * B * T * H : 0)
