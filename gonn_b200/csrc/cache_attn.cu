@@ -298,7 +298,14 @@ __device__ __forceinline__ void clear_rows(uint8_t* tile, int from, int to, int 
   __syncwarp();
 }
 
-// A row of a tile: its query, its output row and how many keys it sees.
+// After a wait that has given up: a copy on its way has to land before its CTA's memory is another's.  Bounded, too.
+__device__ __forceinline__ void let_land(uint64_t* bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity) && globaltimer_ns() - t0 < 10000000ull) {
+  }
+}
+
+// A row of a tile: its query, and how many keys it sees.
 struct Row {
   int b, t, g;
   bool there;            // a row of the entry
@@ -538,402 +545,402 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       if (lane == 0) mbar_arrive(&seg_full[sg]);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
+    if (TMA && *abort_flag)
+      for (int i = 0; i < STAGES; i++) let_land(&full[i], i < st ? ph : ph ^ 1);
   };
 
   auto products = [&]() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
-  int st = 0, sg = 0;
-  uint32_t ph = 0, sph = 0, jph = 0;
-  const int rg = warp / KG, kg = warp % KG;
-  float2* s_stat = reinterpret_cast<float2*>(s_join + (KG == 4 ? 4 * C::RJ : KG == 2 ? ROWS : 0) * C::PAD);
-  // Four key groups' sums of the rows from..from + RJ - 1 meet in shared memory; a warp joins every fourth row.
-  auto join_rows = [&](const Segment& seg, int from) {
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&joined[0]);
-    if (!mbar_wait(&joined[0], jph, abort_flag, a.status, ST_ATTN_TIMEOUT, 26)) return false;
-    jph ^= 1;
-    constexpr int CPL = HD / 32;                                     // columns of a lane
-    const int col = lane * CPL;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    int st = 0, sg = 0;
+    uint32_t ph = 0, sph = 0, jph = 0;
+    const int rg = warp / KG, kg = warp % KG;
+    float2* s_stat = reinterpret_cast<float2*>(s_join + (KG == 4 ? 4 * C::RJ : KG == 2 ? ROWS : 0) * C::PAD);
+    // Four key groups' sums of the rows from..from + RJ - 1 meet in shared memory; a warp joins every fourth row.
+    auto join_rows = [&](const Segment& seg, int from) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&joined[0]);
+      if (!mbar_wait(&joined[0], jph, abort_flag, a.status, ST_ATTN_TIMEOUT, 26)) return false;
+      jph ^= 1;
+      constexpr int CPL = HD / 32;                                     // columns of a lane
+      const int col = lane * CPL;
 #pragma unroll
-    for (int i = 0; i < C::RJ / 4; i++) {
-      const int r = i * 4 + warp;
-      if (r >= seg.rows - from) break;
-      float w[4], top = -INFINITY, l = 0.f, sum[CPL];
+      for (int i = 0; i < C::RJ / 4; i++) {
+        const int r = i * 4 + warp;
+        if (r >= seg.rows - from) break;
+        float w[4], top = -INFINITY, l = 0.f, sum[CPL];
 #pragma unroll
-      for (int k = 0; k < 4; k++) top = fmaxf(top, s_stat[k * C::RJ + r].x);
+        for (int k = 0; k < 4; k++) top = fmaxf(top, s_stat[k * C::RJ + r].x);
 #pragma unroll
-      for (int c = 0; c < CPL; c++) sum[c] = 0.f;
+        for (int c = 0; c < CPL; c++) sum[c] = 0.f;
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const float2 y = s_stat[k * C::RJ + r];
-        w[k] = y.x == -INFINITY ? (y.y == 0.f ? 0.f : 1.f) : exp2f(y.x - top);     // (scores of NaN leave no maximum, but a sum)
-        l += y.y * w[k];
-        float v[CPL];
-        load_floats<CPL>(v, s_join + (k * C::RJ + r) * C::PAD + col);
+        for (int k = 0; k < 4; k++) {
+          const float2 y = s_stat[k * C::RJ + r];
+          w[k] = y.x == -INFINITY ? (y.y == 0.f ? 0.f : 1.f) : exp2f(y.x - top);     // (scores of NaN leave no maximum, but a sum)
+          l += y.y * w[k];
+          float v[CPL];
+          load_floats<CPL>(v, s_join + (k * C::RJ + r) * C::PAD + col);
 #pragma unroll
-        for (int c = 0; c < CPL; c++) sum[c] += v[c] * w[k];
-      }
-      if constexpr (CLUSTER) {
-        const int to = col / slice, at = col - to * slice;
-        const uint32_t p = peer_address(smem_u32(x_sum + (rank * ROWS + from + r) * slice + at), to);
-#pragma unroll
-        for (int c = 0; c < CPL; c += 2) st_peer(p + 4 * c, sum[c], sum[c + 1]);
-        if (at == 0) st_peer(peer_address(smem_u32(x_stat + rank * ROWS + from + r), to), top, l);
-      } else {
-        const long long row = s_dst[sg * ROWS + from + r];
-        const bool counts = s_sees[sg * ROWS + from + r] && l != 0.f;
-        if (col < a.D) {
-          if (!seg.direct) {
-            store_floats<CPL>(a.part + row * a.D + col, sum);
-          } else {
-            const float f = counts ? __frcp_rn(l) : 0.f;
-#pragma unroll
-            for (int c = 0; c < CPL; c++) sum[c] = counts ? sum[c] * f : 0.f;
-            if constexpr (C::kMma) {
-#pragma unroll
-              for (int c = 0; c < CPL; c += 2) *reinterpret_cast<uint32_t*>((T*)a.out + row * a.D + col + c) = Elem<T>::pack(sum[c], sum[c + 1]);
-            } else {
-              store_floats<CPL>((float*)a.out + row * a.D + col, sum);
-            }
-          }
+          for (int c = 0; c < CPL; c++) sum[c] += v[c] * w[k];
         }
-        if (!seg.direct && lane == 0) a.stat[row] = make_float2(top, l);
-      }
-    }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&joined[1]);
-    return true;
-  };
-  for (;;) {
-    if (!mbar_wait(&seg_full[sg], sph, abort_flag, a.status, ST_ATTN_TIMEOUT, 24)) return;
-    const Segment seg = s_seg[sg];
-    if (seg.tiles == 0) return;                  // no more; of a cluster, none for this CTA
-    const int* sees_of = s_sees + sg * ROWS;
-    const long long* dst_of = s_dst + sg * ROWS;
-
-    if constexpr (C::kMma) {
-      constexpr int NK = TILE / KG;                                  // keys of this warp
-      const int r0 = rg * 16 + (lane >> 2), r1 = r0 + 8;
-      // rows of nothing are masked nowhere: what they add up to is not used
-      int sees0 = sees_of[r0], sees1 = sees_of[r1];
-      const bool idle = !__any_sync(0xffffffffu, sees0 | sees1);
-      sees0 = sees0 ? sees0 : 0x7fffffff;
-      sees1 = sees1 ? sees1 : 0x7fffffff;
-      uint32_t qf[HD / 16][4];
-      {
-        const uint32_t qa = smem_u32(s_q + sg * C::Q_BYTES);
+        if constexpr (CLUSTER) {
+          const int to = col / slice, at = col - to * slice;
+          const uint32_t p = peer_address(smem_u32(x_sum + (rank * ROWS + from + r) * slice + at), to);
 #pragma unroll
-        for (int x = 0; x < HD / 16; x++) ldm4(qf[x], qa + chunk_at<ROWS>(rg * 16 + (lane & 15), x * 2 + (lane >> 4)));
-      }
-      float o[HD / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+          for (int c = 0; c < CPL; c += 2) st_peer(p + 4 * c, sum[c], sum[c + 1]);
+          if (at == 0) st_peer(peer_address(smem_u32(x_stat + rank * ROWS + from + r), to), top, l);
+        } else {
+          const long long row = s_dst[sg * ROWS + from + r];
+          const bool counts = s_sees[sg * ROWS + from + r] && l != 0.f;
+          if (col < a.D) {
+            if (!seg.direct) {
+              store_floats<CPL>(a.part + row * a.D + col, sum);
+            } else {
+              const float f = counts ? __frcp_rn(l) : 0.f;
 #pragma unroll
-      for (int j = 0; j < HD / 8; j++)
+              for (int c = 0; c < CPL; c++) sum[c] = counts ? sum[c] * f : 0.f;
+              if constexpr (C::kMma) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) o[j][i] = 0.f;
-
-      for (int i = 0; i < seg.tiles; i++) {
-        if (!mbar_wait(&full[st], ph, abort_flag, a.status, ST_ATTN_TIMEOUT, 21)) return;
-        const int key0 = seg.key0 + i * TILE + kg * NK;
-        if (!idle && key0 < seg.end) {
-          const uint32_t ka = smem_u32(s_k + st * SUB), va = smem_u32(s_v + st * SUB);
-          float s[NK / 8][4], odd[2][4];
-#pragma unroll
-          for (int j = 0; j < NK / 8; j++)
-#pragma unroll
-            for (int c = 0; c < 4; c++) s[j][c] = 0.f;
-          // A warp with few keys has few chains of dependent products: two of half the length for each.
-          constexpr bool kHalves = NK == 16;
-#pragma unroll
-          for (int c = 0; c < 8; c++) odd[c / 4][c % 4] = 0.f;
-#pragma unroll
-          for (int j = 0; j < NK / 16; j++) {                        // 16 keys: two n8 tiles
-            const int row = kg * NK + j * 16 + (lane & 7) + ((lane >> 4) << 3);
-#pragma unroll
-            for (int x = 0; x < HD / 16; x++) {
-              uint32_t b[4];
-              ldm4(b, ka + chunk_at<TILE>(row, x * 2 + ((lane >> 3) & 1)));
-              mma16<T>(kHalves && x % 2 ? odd[0] : s[2 * j], qf[x], b[0], b[1]);
-              mma16<T>(kHalves && x % 2 ? odd[1] : s[2 * j + 1], qf[x], b[2], b[3]);
+                for (int c = 0; c < CPL; c += 2) *reinterpret_cast<uint32_t*>((T*)a.out + row * a.D + col + c) = Elem<T>::pack(sum[c], sum[c + 1]);
+              } else {
+                store_floats<CPL>((float*)a.out + row * a.D + col, sum);
+              }
             }
           }
-          if (kHalves) {
+          if (!seg.direct && lane == 0) a.stat[row] = make_float2(top, l);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&joined[1]);
+      return true;
+    };
+    for (;;) {
+      if (!mbar_wait(&seg_full[sg], sph, abort_flag, a.status, ST_ATTN_TIMEOUT, 24)) return;
+      const Segment seg = s_seg[sg];
+      if (seg.tiles == 0) return;                  // no more; of a cluster, none for this CTA
+      const int* sees_of = s_sees + sg * ROWS;
+      const long long* dst_of = s_dst + sg * ROWS;
+
+      if constexpr (C::kMma) {
+        constexpr int NK = TILE / KG;                                  // keys of this warp
+        const int r0 = rg * 16 + (lane >> 2), r1 = r0 + 8;
+        // rows of nothing are masked nowhere: what they add up to is not used
+        int sees0 = sees_of[r0], sees1 = sees_of[r1];
+        const bool idle = !__any_sync(0xffffffffu, sees0 | sees1);
+        sees0 = sees0 ? sees0 : 0x7fffffff;
+        sees1 = sees1 ? sees1 : 0x7fffffff;
+        uint32_t qf[HD / 16][4];
+        {
+          const uint32_t qa = smem_u32(s_q + sg * C::Q_BYTES);
 #pragma unroll
-            for (int c = 0; c < 8; c++) s[c / 4][c % 4] += odd[c / 4][c % 4];
-          }
-          const int low = min(min(sees0, sees1), seg.end);           // (zeros stand in for keys behind the last one)
-          if (__any_sync(0xffffffffu, low - key0 < NK)) {
+          for (int x = 0; x < HD / 16; x++) ldm4(qf[x], qa + chunk_at<ROWS>(rg * 16 + (lane & 15), x * 2 + (lane >> 4)));
+        }
+        float o[HD / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+#pragma unroll
+        for (int j = 0; j < HD / 8; j++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) o[j][i] = 0.f;
+
+        for (int i = 0; i < seg.tiles; i++) {
+          if (!mbar_wait(&full[st], ph, abort_flag, a.status, ST_ATTN_TIMEOUT, 21)) return;
+          const int key0 = seg.key0 + i * TILE + kg * NK;
+          if (!idle && key0 < seg.end) {
+            const uint32_t ka = smem_u32(s_k + st * SUB), va = smem_u32(s_v + st * SUB);
+            float s[NK / 8][4], odd[2][4];
 #pragma unroll
             for (int j = 0; j < NK / 8; j++)
 #pragma unroll
-              for (int c = 0; c < 4; c++) {
-                const int key = key0 + j * 8 + (lane & 3) * 2 + (c & 1);
-                if (key >= min((c & 2) ? sees1 : sees0, seg.end)) s[j][c] = -INFINITY;
+              for (int c = 0; c < 4; c++) s[j][c] = 0.f;
+            // A warp with few keys has few chains of dependent products: two of half the length for each.
+            constexpr bool kHalves = NK == 16;
+#pragma unroll
+            for (int c = 0; c < 8; c++) odd[c / 4][c % 4] = 0.f;
+#pragma unroll
+            for (int j = 0; j < NK / 16; j++) {                        // 16 keys: two n8 tiles
+              const int row = kg * NK + j * 16 + (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+              for (int x = 0; x < HD / 16; x++) {
+                uint32_t b[4];
+                ldm4(b, ka + chunk_at<TILE>(row, x * 2 + ((lane >> 3) & 1)));
+                mma16<T>(kHalves && x % 2 ? odd[0] : s[2 * j], qf[x], b[0], b[1]);
+                mma16<T>(kHalves && x % 2 ? odd[1] : s[2 * j + 1], qf[x], b[2], b[3]);
               }
-          }
-          if (TMA && seg.end - key0 < NK) clear_rows<TILE, C::CHUNKS>(s_v + st * SUB, kg * NK + seg.end - key0, kg * NK + NK, lane);
-          float x0 = -INFINITY, x1 = -INFINITY;
-#pragma unroll
-          for (int j = 0; j < NK / 8; j++) {
-            x0 = fmaxf(x0, fmaxf(s[j][0], s[j][1]));
-            x1 = fmaxf(x1, fmaxf(s[j][2], s[j][3]));
-          }
-#pragma unroll
-          for (int d = 1; d < 4; d <<= 1) {
-            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
-            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
-          }
-          const float n0 = fmaxf(m0, x0 * a.scale_log2), n1 = fmaxf(m1, x1 * a.scale_log2);
-          if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
-            const float f0 = m0 == -INFINITY ? 0.f : exp2f(m0 - n0), f1 = m1 == -INFINITY ? 0.f : exp2f(m1 - n1);
-            m0 = n0;
-            m1 = n1;
-            l0 *= f0;
-            l1 *= f1;
-#pragma unroll
-            for (int j = 0; j < HD / 8; j++) {
-              o[j][0] *= f0;
-              o[j][1] *= f0;
-              o[j][2] *= f1;
-              o[j][3] *= f1;
             }
-          }
-          const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
+            if (kHalves) {
 #pragma unroll
-          for (int j = 0; j < NK / 8; j++) {
-            s[j][0] = exp2f(fmaf(s[j][0], a.scale_log2, -z0));
-            s[j][1] = exp2f(fmaf(s[j][1], a.scale_log2, -z0));
-            s[j][2] = exp2f(fmaf(s[j][2], a.scale_log2, -z1));
-            s[j][3] = exp2f(fmaf(s[j][3], a.scale_log2, -z1));
-            l0 += s[j][0] + s[j][1];
-            l1 += s[j][2] + s[j][3];
-          }
-#pragma unroll
-          for (int j = 0; j < NK / 16; j++) {
-            const uint32_t p[4] = {Elem<T>::pack(s[2 * j][0], s[2 * j][1]), Elem<T>::pack(s[2 * j][2], s[2 * j][3]),
-                                   Elem<T>::pack(s[2 * j + 1][0], s[2 * j + 1][1]), Elem<T>::pack(s[2 * j + 1][2], s[2 * j + 1][3])};
-            const int row = kg * NK + j * 16 + (lane & 15);
-#pragma unroll
-            for (int x = 0; x < HD / 16; x++) {                      // 16 columns
-              uint32_t b[4];
-              ldm4t(b, va + chunk_at<TILE>(row, x * 2 + (lane >> 4)));
-              mma16<T>(o[2 * x], p, b[0], b[1]);
-              mma16<T>(o[2 * x + 1], p, b[2], b[3]);
+              for (int c = 0; c < 8; c++) s[c / 4][c % 4] += odd[c / 4][c % 4];
             }
-          }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[st]);
-        if (++st == STAGES) { st = 0; ph ^= 1; }
-      }
+            const int low = min(min(sees0, sees1), seg.end);           // (zeros stand in for keys behind the last one)
+            if (__any_sync(0xffffffffu, low - key0 < NK)) {
 #pragma unroll
-      for (int d = 1; d < 4; d <<= 1) {
-        l0 += __shfl_xor_sync(0xffffffffu, l0, d);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, d);
-      }
-      if constexpr (KG > 1) {
-        auto hand_over = [&](int half, int to_row) {
-          const int r = half ? r1 : r0;
-          if (r < seg.rows) {
-            float* to = s_join + to_row * C::PAD + (lane & 3) * 2;
+              for (int j = 0; j < NK / 8; j++)
 #pragma unroll
-            for (int j = 0; j < HD / 8; j++) *reinterpret_cast<float2*>(to + j * 8) = make_float2(o[j][2 * half], o[j][2 * half + 1]);
-            if ((lane & 3) == 0) s_stat[to_row] = half ? make_float2(m1, l1) : make_float2(m0, l0);
-          }
-        };
-        if constexpr (RG == 1) {
-          static_assert(C::RJ == 8, "a half of a warp's rows");
+                for (int c = 0; c < 4; c++) {
+                  const int key = key0 + j * 8 + (lane & 3) * 2 + (c & 1);
+                  if (key >= min((c & 2) ? sees1 : sees0, seg.end)) s[j][c] = -INFINITY;
+                }
+            }
+            if (TMA && seg.end - key0 < NK) clear_rows<TILE, C::CHUNKS>(s_v + st * SUB, kg * NK + seg.end - key0, kg * NK + NK, lane);
+            float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
-          for (int half = 0; half < 2; half++) {
-            if (half && seg.rows <= 8) break;
-            if (!mbar_wait(&joined[1], jph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 25)) return;      // (the last rows have been read)
-            hand_over(half, kg * 8 + (lane >> 2));
-            if (!join_rows(seg, half * 8)) return;
-          }
-        } else {
-          // of two key groups one hands its sums to the other
-          if (!mbar_wait(&joined[1], jph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 25)) return;
-          if (kg == 1) {
-            hand_over(0, r0);
-            hand_over(1, r1);
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&joined[0]);
-          if (!mbar_wait(&joined[0], jph, abort_flag, a.status, ST_ATTN_TIMEOUT, 26)) return;
-          jph ^= 1;
-          if (kg == 0) {
+            for (int j = 0; j < NK / 8; j++) {
+              x0 = fmaxf(x0, fmaxf(s[j][0], s[j][1]));
+              x1 = fmaxf(x1, fmaxf(s[j][2], s[j][3]));
+            }
 #pragma unroll
-          for (int half = 0; half < 2; half++) {
-            const int r = half ? r1 : r0;
-            float& m = half ? m1 : m0;
-            float& l = half ? l1 : l0;
-            if (r < seg.rows) {
-              const float2 y = s_stat[r];
-              const float top = fmaxf(m, y.x);
-              const float f = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2f(m - top), w = y.x == -INFINITY ? (y.y == 0.f ? 0.f : 1.f) : exp2f(y.x - top);
-              m = top;
-              l = l * f + y.y * w;
-              const float* from = s_join + r * C::PAD + (lane & 3) * 2;
+            for (int d = 1; d < 4; d <<= 1) {
+              x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
+              x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+            }
+            const float n0 = fmaxf(m0, x0 * a.scale_log2), n1 = fmaxf(m1, x1 * a.scale_log2);
+            if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
+              const float f0 = m0 == -INFINITY ? 0.f : exp2f(m0 - n0), f1 = m1 == -INFINITY ? 0.f : exp2f(m1 - n1);
+              m0 = n0;
+              m1 = n1;
+              l0 *= f0;
+              l1 *= f1;
 #pragma unroll
               for (int j = 0; j < HD / 8; j++) {
-                const float2 v = *reinterpret_cast<const float2*>(from + j * 8);
-                o[j][2 * half] = o[j][2 * half] * f + v.x * w;
-                o[j][2 * half + 1] = o[j][2 * half + 1] * f + v.y * w;
+                o[j][0] *= f0;
+                o[j][1] *= f0;
+                o[j][2] *= f1;
+                o[j][3] *= f1;
+              }
+            }
+            const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
+#pragma unroll
+            for (int j = 0; j < NK / 8; j++) {
+              s[j][0] = exp2f(fmaf(s[j][0], a.scale_log2, -z0));
+              s[j][1] = exp2f(fmaf(s[j][1], a.scale_log2, -z0));
+              s[j][2] = exp2f(fmaf(s[j][2], a.scale_log2, -z1));
+              s[j][3] = exp2f(fmaf(s[j][3], a.scale_log2, -z1));
+              l0 += s[j][0] + s[j][1];
+              l1 += s[j][2] + s[j][3];
+            }
+#pragma unroll
+            for (int j = 0; j < NK / 16; j++) {
+              const uint32_t p[4] = {Elem<T>::pack(s[2 * j][0], s[2 * j][1]), Elem<T>::pack(s[2 * j][2], s[2 * j][3]),
+                                     Elem<T>::pack(s[2 * j + 1][0], s[2 * j + 1][1]), Elem<T>::pack(s[2 * j + 1][2], s[2 * j + 1][3])};
+              const int row = kg * NK + j * 16 + (lane & 15);
+#pragma unroll
+              for (int x = 0; x < HD / 16; x++) {                      // 16 columns
+                uint32_t b[4];
+                ldm4t(b, va + chunk_at<TILE>(row, x * 2 + (lane >> 4)));
+                mma16<T>(o[2 * x], p, b[0], b[1]);
+                mma16<T>(o[2 * x + 1], p, b[2], b[3]);
               }
             }
           }
-          }
           __syncwarp();
-          if (lane == 0) mbar_arrive(&joined[1]);
+          if (lane == 0) mbar_arrive(&empty[st]);
+          if (++st == STAGES) { st = 0; ph ^= 1; }
         }
-      }
-      if (RG > 1 && kg == 0) {
 #pragma unroll
-        for (int half = 0; half < 2; half++) {
-          const float m = half ? m1 : m0, l = half ? l1 : l0;
-          const int r = half ? r1 : r0;
-          if (r < seg.rows) {
-            const long long row = dst_of[r];
-            if (seg.direct) {
-              const float f = sees_of[r] && l != 0.f ? __frcp_rn(l) : 0.f;
-              T* to = (T*)a.out + row * a.D + (lane & 3) * 2;
+        for (int d = 1; d < 4; d <<= 1) {
+          l0 += __shfl_xor_sync(0xffffffffu, l0, d);
+          l1 += __shfl_xor_sync(0xffffffffu, l1, d);
+        }
+        if constexpr (KG > 1) {
+          auto hand_over = [&](int half, int to_row) {
+            const int r = half ? r1 : r0;
+            if (r < seg.rows) {
+              float* to = s_join + to_row * C::PAD + (lane & 3) * 2;
 #pragma unroll
-              for (int j = 0; j < HD / 8; j++)
-                if (j * 8 < a.D)
-                  *reinterpret_cast<uint32_t*>(to + j * 8) = f == 0.f ? 0u : Elem<T>::pack(o[j][2 * half] * f, o[j][2 * half + 1] * f);
-            } else {
-              float* to = a.part + row * a.D + (lane & 3) * 2;
-#pragma unroll
-              for (int j = 0; j < HD / 8; j++)
-                if (j * 8 < a.D) *reinterpret_cast<float2*>(to + j * 8) = make_float2(o[j][2 * half], o[j][2 * half + 1]);
-              if ((lane & 3) == 0) a.stat[row] = make_float2(m, l);
+              for (int j = 0; j < HD / 8; j++) *reinterpret_cast<float2*>(to + j * 8) = make_float2(o[j][2 * half], o[j][2 * half + 1]);
+              if ((lane & 3) == 0) s_stat[to_row] = half ? make_float2(m1, l1) : make_float2(m0, l0);
             }
+          };
+          if constexpr (RG == 1) {
+            static_assert(C::RJ == 8, "a half of a warp's rows");
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+              if (half && seg.rows <= 8) break;
+              if (!mbar_wait(&joined[1], jph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 25)) return;      // (the last rows have been read)
+              hand_over(half, kg * 8 + (lane >> 2));
+              if (!join_rows(seg, half * 8)) return;
+            }
+          } else {
+            // of two key groups one hands its sums to the other
+            if (!mbar_wait(&joined[1], jph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 25)) return;
+            if (kg == 1) {
+              hand_over(0, r0);
+              hand_over(1, r1);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&joined[0]);
+            if (!mbar_wait(&joined[0], jph, abort_flag, a.status, ST_ATTN_TIMEOUT, 26)) return;
+            jph ^= 1;
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+              const int r = half ? r1 : r0;
+              float& m = half ? m1 : m0;
+              float& l = half ? l1 : l0;
+              if (kg == 0 && r < seg.rows) {
+                const float2 y = s_stat[r];
+                const float top = fmaxf(m, y.x);
+                const float f = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : exp2f(m - top), w = y.x == -INFINITY ? (y.y == 0.f ? 0.f : 1.f) : exp2f(y.x - top);
+                m = top;
+                l = l * f + y.y * w;
+                const float* from = s_join + r * C::PAD + (lane & 3) * 2;
+#pragma unroll
+                for (int j = 0; j < HD / 8; j++) {
+                  const float2 v = *reinterpret_cast<const float2*>(from + j * 8);
+                  o[j][2 * half] = o[j][2 * half] * f + v.x * w;
+                  o[j][2 * half + 1] = o[j][2 * half + 1] * f + v.y * w;
+                }
+              }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&joined[1]);
           }
         }
-      }
-    } else {
-      // fp32: a warp's quarter of the keys of a tile for all rows.  Scores: LPK lanes share a key, every LPK-th chunk of its columns each; products with
-      // the values: a lane is HD / 32 columns.
-      constexpr int KW = TILE / 4, LPK = 32 / KW, CPL = HD / 32;
-      const uint8_t* q = s_q + sg * C::Q_BYTES;
-      float* s_p = reinterpret_cast<float*>((uint8_t*)s_join + C::JOIN) + warp * (KW * ROWS);      // [KW][ROWS] of this warp
-      const int mykey = lane / LPK, slice = lane % LPK;
-      float o[ROWS][CPL], m[ROWS], l[ROWS];
+        if (RG > 1 && kg == 0) {
 #pragma unroll
-      for (int r = 0; r < ROWS; r++) {
-        m[r] = -INFINITY;
-        l[r] = 0.f;
+          for (int half = 0; half < 2; half++) {
+            const float m = half ? m1 : m0, l = half ? l1 : l0;
+            const int r = half ? r1 : r0;
+            if (r < seg.rows) {
+              const long long row = dst_of[r];
+              if (seg.direct) {
+                const float f = sees_of[r] && l != 0.f ? __frcp_rn(l) : 0.f;
+                T* to = (T*)a.out + row * a.D + (lane & 3) * 2;
 #pragma unroll
-        for (int c = 0; c < CPL; c++) o[r][c] = 0.f;
-      }
-      for (int i = 0; i < seg.tiles; i++) {
-        if (!mbar_wait(&full[st], ph, abort_flag, a.status, ST_ATTN_TIMEOUT, 22)) return;
-        const int key0 = seg.key0 + i * TILE + warp * KW, there = min(KW, seg.end - key0);
-        if (there > 0) {
-          const uint8_t* kt = s_k + st * SUB;
-          const uint8_t* vt = s_v + st * SUB;
-          const int key = key0 + mykey;
-          float s[ROWS];
+                for (int j = 0; j < HD / 8; j++)
+                  if (j * 8 < a.D)
+                    *reinterpret_cast<uint32_t*>(to + j * 8) = f == 0.f ? 0u : Elem<T>::pack(o[j][2 * half] * f, o[j][2 * half + 1] * f);
+              } else {
+                float* to = a.part + row * a.D + (lane & 3) * 2;
 #pragma unroll
-          for (int r = 0; r < ROWS; r++) s[r] = 0.f;
-          const uint8_t* mine = q + slice * 16;
-#pragma unroll 4
-          for (int c = 0; c < HD / 4 / LPK; c++) {
-            const float4 kk = *reinterpret_cast<const float4*>(kt + chunk_at<TILE>(warp * KW + mykey, c * LPK + slice));
-#pragma unroll
-            for (int r = 0; r < ROWS; r++) {
-              const float4 qq = *reinterpret_cast<const float4*>(mine + (r * (HD / 4) + c * LPK) * 16);
-              s[r] = fmaf(qq.x, kk.x, s[r]);
-              s[r] = fmaf(qq.y, kk.y, s[r]);
-              s[r] = fmaf(qq.z, kk.z, s[r]);
-              s[r] = fmaf(qq.w, kk.w, s[r]);
-            }
-          }
-          // (step by step over all rows, whose exchanges between lanes do not wait for one another: row by row they took 2 us of a tile's 6)
-#pragma unroll
-          for (int d = 1; d < LPK; d <<= 1)
-#pragma unroll
-            for (int r = 0; r < ROWS; r++) s[r] += __shfl_xor_sync(0xffffffffu, s[r], d);
-          float top[ROWS];
-#pragma unroll
-          for (int r = 0; r < ROWS; r++) {
-            const int sees = s_sees[sg * ROWS + r];
-            s[r] = key < min(sees ? sees : 0x7fffffff, seg.end) ? s[r] : -INFINITY;
-            top[r] = s[r];
-          }
-#pragma unroll
-          for (int d = LPK; d < 32; d <<= 1)
-#pragma unroll
-            for (int r = 0; r < ROWS; r++) top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], d));
-          bool moved = false;
-#pragma unroll
-          for (int r = 0; r < ROWS; r++) {
-            top[r] = fmaxf(m[r], top[r] * a.scale_log2);
-            moved |= top[r] > m[r];
-          }
-          if (moved) {                                               // (the same for all lanes)
-#pragma unroll
-            for (int r = 0; r < ROWS; r++) {
-              const float f = m[r] == -INFINITY ? 0.f : exp2f(m[r] - top[r]);
-              m[r] = top[r];
-              l[r] *= f;
-#pragma unroll
-              for (int c = 0; c < CPL; c++) o[r][c] *= f;
-            }
-          }
-#pragma unroll
-          for (int r = 0; r < ROWS; r++) {
-            // (scaled and subtracted in one rounding)
-            s[r] = exp2f(fmaf(s[r], a.scale_log2, m[r] == -INFINITY ? 0.f : -m[r]));
-            l[r] += slice == 0 ? s[r] : 0.f;                         // this lane's keys; summed over lanes at the end
-          }
-          if (slice == 0) {
-#pragma unroll
-            for (int r = 0; r < ROWS; r += 4) *reinterpret_cast<float4*>(s_p + mykey * ROWS + r) = make_float4(s[r], s[r + 1], s[r + 2], s[r + 3]);
-          }
-          __syncwarp();
-#pragma unroll 4
-          for (int j = 0; j < there; j++) {                          // (rows of V behind the last key are not read)
-            float v[CPL];
-            const uint8_t* vr = vt + chunk_at<TILE>(warp * KW + j, lane * CPL / 4);
-            if constexpr (CPL == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(vr);
-            else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(vr + (lane & 1) * 8);
-#pragma unroll
-            for (int r = 0; r < ROWS; r += 4) {
-              const float4 p = *reinterpret_cast<const float4*>(s_p + j * ROWS + r);
-#pragma unroll
-              for (int c = 0; c < CPL; c++) {
-                o[r][c] = fmaf(p.x, v[c], o[r][c]);
-                o[r + 1][c] = fmaf(p.y, v[c], o[r + 1][c]);
-                o[r + 2][c] = fmaf(p.z, v[c], o[r + 2][c]);
-                o[r + 3][c] = fmaf(p.w, v[c], o[r + 3][c]);
+                for (int j = 0; j < HD / 8; j++)
+                  if (j * 8 < a.D) *reinterpret_cast<float2*>(to + j * 8) = make_float2(o[j][2 * half], o[j][2 * half + 1]);
+                if ((lane & 3) == 0) a.stat[row] = make_float2(m, l);
               }
             }
           }
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[st]);
-        if (++st == STAGES) { st = 0; ph ^= 1; }
-      }
+      } else {
+        // fp32: a warp's quarter of the keys of a tile for all rows.  Scores: LPK lanes share a key, every LPK-th chunk of its columns each; products with
+        // the values: a lane is HD / 32 columns.
+        constexpr int KW = TILE / 4, LPK = 32 / KW, CPL = HD / 32;
+        const uint8_t* q = s_q + sg * C::Q_BYTES;
+        float* s_p = reinterpret_cast<float*>((uint8_t*)s_join + C::JOIN) + warp * (KW * ROWS);      // [KW][ROWS] of this warp
+        const int mykey = lane / LPK, slice = lane % LPK;
+        float o[ROWS][CPL], m[ROWS], l[ROWS];
 #pragma unroll
-      for (int from = 0; from < ROWS; from += C::RJ) {
-        if (from >= seg.rows) break;
-        if (!mbar_wait(&joined[1], jph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 25)) return;      // (the last rows have been read)
+        for (int r = 0; r < ROWS; r++) {
+          m[r] = -INFINITY;
+          l[r] = 0.f;
 #pragma unroll
-        for (int r = 0; r < C::RJ; r++) {
-          const float sum = warp_sum(l[from + r]);
-          float* to = s_join + (warp * C::RJ + r) * C::PAD + lane * CPL;
-#pragma unroll
-          for (int c = 0; c < CPL; c++) to[c] = o[from + r][c];
-          if (lane == 0) s_stat[warp * C::RJ + r] = make_float2(m[from + r], sum);
+          for (int c = 0; c < CPL; c++) o[r][c] = 0.f;
         }
-        if (!join_rows(seg, from)) return;
+        for (int i = 0; i < seg.tiles; i++) {
+          if (!mbar_wait(&full[st], ph, abort_flag, a.status, ST_ATTN_TIMEOUT, 22)) return;
+          const int key0 = seg.key0 + i * TILE + warp * KW, there = min(KW, seg.end - key0);
+          if (there > 0) {
+            const uint8_t* kt = s_k + st * SUB;
+            const uint8_t* vt = s_v + st * SUB;
+            const int key = key0 + mykey;
+            float s[ROWS];
+#pragma unroll
+            for (int r = 0; r < ROWS; r++) s[r] = 0.f;
+            const uint8_t* mine = q + slice * 16;
+#pragma unroll 4
+            for (int c = 0; c < HD / 4 / LPK; c++) {
+              const float4 kk = *reinterpret_cast<const float4*>(kt + chunk_at<TILE>(warp * KW + mykey, c * LPK + slice));
+#pragma unroll
+              for (int r = 0; r < ROWS; r++) {
+                const float4 qq = *reinterpret_cast<const float4*>(mine + (r * (HD / 4) + c * LPK) * 16);
+                s[r] = fmaf(qq.x, kk.x, s[r]);
+                s[r] = fmaf(qq.y, kk.y, s[r]);
+                s[r] = fmaf(qq.z, kk.z, s[r]);
+                s[r] = fmaf(qq.w, kk.w, s[r]);
+              }
+            }
+            // (step by step over all rows, whose exchanges between lanes do not wait for one another: row by row they took 2 us of a tile's 6)
+#pragma unroll
+            for (int d = 1; d < LPK; d <<= 1)
+#pragma unroll
+              for (int r = 0; r < ROWS; r++) s[r] += __shfl_xor_sync(0xffffffffu, s[r], d);
+            float top[ROWS];
+#pragma unroll
+            for (int r = 0; r < ROWS; r++) {
+              const int sees = s_sees[sg * ROWS + r];
+              s[r] = key < min(sees ? sees : 0x7fffffff, seg.end) ? s[r] : -INFINITY;
+              top[r] = s[r];
+            }
+#pragma unroll
+            for (int d = LPK; d < 32; d <<= 1)
+#pragma unroll
+              for (int r = 0; r < ROWS; r++) top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], d));
+            bool moved = false;
+#pragma unroll
+            for (int r = 0; r < ROWS; r++) {
+              top[r] = fmaxf(m[r], top[r] * a.scale_log2);
+              moved |= top[r] > m[r];
+            }
+            if (moved) {                                               // (the same for all lanes)
+#pragma unroll
+              for (int r = 0; r < ROWS; r++) {
+                const float f = m[r] == -INFINITY ? 0.f : exp2f(m[r] - top[r]);
+                m[r] = top[r];
+                l[r] *= f;
+#pragma unroll
+                for (int c = 0; c < CPL; c++) o[r][c] *= f;
+              }
+            }
+#pragma unroll
+            for (int r = 0; r < ROWS; r++) {
+              // (scaled and subtracted in one rounding)
+              s[r] = exp2f(fmaf(s[r], a.scale_log2, m[r] == -INFINITY ? 0.f : -m[r]));
+              l[r] += slice == 0 ? s[r] : 0.f;                         // this lane's keys; summed over lanes at the end
+            }
+            if (slice == 0) {
+#pragma unroll
+              for (int r = 0; r < ROWS; r += 4) *reinterpret_cast<float4*>(s_p + mykey * ROWS + r) = make_float4(s[r], s[r + 1], s[r + 2], s[r + 3]);
+            }
+            __syncwarp();
+#pragma unroll 4
+            for (int j = 0; j < there; j++) {                          // (rows of V behind the last key are not read)
+              float v[CPL];
+              const uint8_t* vr = vt + chunk_at<TILE>(warp * KW + j, lane * CPL / 4);
+              if constexpr (CPL == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(vr);
+              else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(vr + (lane & 1) * 8);
+#pragma unroll
+              for (int r = 0; r < ROWS; r += 4) {
+                const float4 p = *reinterpret_cast<const float4*>(s_p + j * ROWS + r);
+#pragma unroll
+                for (int c = 0; c < CPL; c++) {
+                  o[r][c] = fmaf(p.x, v[c], o[r][c]);
+                  o[r + 1][c] = fmaf(p.y, v[c], o[r + 1][c]);
+                  o[r + 2][c] = fmaf(p.z, v[c], o[r + 2][c]);
+                  o[r + 3][c] = fmaf(p.w, v[c], o[r + 3][c]);
+                }
+              }
+            }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&empty[st]);
+          if (++st == STAGES) { st = 0; ph ^= 1; }
+        }
+#pragma unroll
+        for (int from = 0; from < ROWS; from += C::RJ) {
+          if (from >= seg.rows) break;
+          if (!mbar_wait(&joined[1], jph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 25)) return;      // (the last rows have been read)
+#pragma unroll
+          for (int r = 0; r < C::RJ; r++) {
+            const float sum = warp_sum(l[from + r]);
+            float* to = s_join + (warp * C::RJ + r) * C::PAD + lane * CPL;
+#pragma unroll
+            for (int c = 0; c < CPL; c++) to[c] = o[from + r][c];
+            if (lane == 0) s_stat[warp * C::RJ + r] = make_float2(m[from + r], sum);
+          }
+          if (!join_rows(seg, from)) return;
+        }
       }
+      if constexpr (CLUSTER) return;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&seg_empty[sg]);
+      if (++sg == SEGS) { sg = 0; sph ^= 1; }
     }
-    if constexpr (CLUSTER) return;
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&seg_empty[sg]);
-    if (++sg == SEGS) { sg = 0; sph ^= 1; }
-  }
   };
 
   if (warp >= kConsumers) copies();
@@ -1104,6 +1111,11 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         copy(s_v + st * SUB, &tm_v, &v_full[st], pg, row);
         if (++st == STAGES) { st = 0; ph ^= 1; }
       }
+      if (*abort_flag)
+        for (int i = 0; i < STAGES; i++) {
+          let_land(&k_full[i], i < st ? ph : ph ^ 1);
+          let_land(&v_full[i], i < st ? ph : ph ^ 1);
+        }
     } else {
       // Key by key with cp.async, which the tensor core sees after a fence of the thread that copied: a sub-tile is handed on when the next copy is
       // on its way.
