@@ -34,8 +34,9 @@ def frequencies(dim: int, base: float, scaling: str = "none", factor: float = 1.
 
 def turns_of(w: Sequence[float]) -> torch.Tensor:
     """Fractions of a turn in 64 bits of fixed point, as int64."""
-    t = [round(f / (2 * math.pi) * 2.0 ** 64) % 2 ** 64 for f in w]
-    return torch.tensor([v - 2 ** 64 if v >= 2 ** 63 else v for v in t], dtype=torch.int64)
+    t = torch.tensor(w, dtype=torch.float64) / (2 * math.pi)
+    t = t - torch.floor(t + 0.5)                      # whole turns go; exact, like the power of two
+    return torch.round(t * 2.0 ** 64).to(torch.int64)
 
 
 def rotate_ref(x: torch.Tensor, positions: torch.Tensor, w: Sequence[float], interleaved: bool, amplitude: float, back: bool = False):
