@@ -115,8 +115,13 @@ struct Entry {                // rows of queries over a range of keys, for every
   bool cut;                   // keys behind the end of its table were asked for
 };
 
+// L2: past the SM's own cache, for a kernel that may start before the one in front of it has ended and waits for it at its end alone.
+template <bool L2>
+__device__ __forceinline__ int read(const int* p) { return L2 ? __ldcg(p) : *p; }
+
+template <bool L2 = false>
 __device__ __forceinline__ int count_of(const CacheArgs& a, int b) {
-  const int c = a.counts ? a.counts[b] : a.T;
+  const int c = a.counts ? read<L2>(a.counts + b) : a.T;
   return c < 0 ? 0 : c < a.T ? c : a.T;
 }
 
@@ -313,6 +318,7 @@ struct Row {
   int sees;
 };
 
+template <bool L2 = false>
 __device__ __forceinline__ Row row_of(const CacheArgs& a, const Entry& x, int r) {
   Row w;
   int i = x.row0 + r;
@@ -326,8 +332,8 @@ __device__ __forceinline__ Row row_of(const CacheArgs& a, const Entry& x, int r)
   }
   w.t = i / a.G;
   w.g = i - w.t * a.G;
-  w.counts = w.there && w.t < count_of(a, w.b);
-  const long long sees = w.counts ? (long long)a.lengths[w.b] + w.t + 1 : 0;
+  w.counts = w.there && w.t < count_of<L2>(a, w.b);
+  const long long sees = w.counts ? (long long)read<L2>(a.lengths + w.b) + w.t + 1 : 0;
   w.sees = (int)(sees < 0x7fffffffLL ? sees : 0x7fffffffLL);
   return w;
 }
@@ -976,7 +982,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 // keys, weights written over their scores as the second product's operand; two score buffers, so that the next scores are computed while
 // a softmax warp (a row a thread) works.  The sum is rescaled only when the maximum has moved by more than 2^8.  Where the row tiles are too few
 // for the SMs, the keys are cut into `splits` runs, which leave partial rows.  Four prompts of 2048 tokens behind 2048 others, 16 heads of 128 bf16:
-// 190 us, 972 TFLOP/s of the pairs that are seen; a softmax warp's chain bounds it (tensor pipe 51 % busy, exponentials 52 %).
+// 187 us, 987 TFLOP/s of the pairs that are seen; a softmax warp's chain bounds it (tensor pipe 51 % busy, exponentials 52 %).
 constexpr int kWideRows = 128, kWideKeys = 64, kWideThreads = 256, kWideCopiers = 3;
 
 template <int HD>
@@ -988,7 +994,7 @@ struct Wide {
   static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs to an SM");
 };
 
-template <typename T, int HD, bool TMA>
+template <typename T, int HD, bool TMA, bool PREFIX>
 __global__ void __launch_bounds__(kWideThreads, 2)
 cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const CacheArgs a) {
   using C = Wide<HD>;
@@ -1036,13 +1042,13 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   // Beside the kernel for few rows, which was launched first and has waited for all that came before: this one waits for that one's end alone, and at
-  // its own, so that what follows it follows both.
-  if (!a.wide_prefix) pdl_wait();
+  // its own, so that what follows it follows both.  What it reads it reads from L2.
+  if (!PREFIX) pdl_wait();
   pdl_trigger();
 
   // Row tiles of a sequence run from its last one, which sees the most keys, to its first: over the heads of a group, so that the kernel ends on
   // the shortest ones.  (sequence, head, run of keys) by groups, in a group by row tiles.
-  const unsigned runs = (unsigned)a.splits * a.Hkv * (a.wide_prefix ? 1 : a.B), per_group = (unsigned)a.wide_group * a.wide_tiles;
+  const unsigned runs = (unsigned)a.splits * a.Hkv * (PREFIX ? 1 : a.B), per_group = (unsigned)a.wide_group * a.wide_tiles;
   const unsigned group = blockIdx.x / per_group, in_group = blockIdx.x - group * per_group, size = min((unsigned)a.wide_group, runs - group * a.wide_group);
   const int rank = in_group / size;
   unsigned idx = group * a.wide_group + in_group - rank * size;
@@ -1050,10 +1056,10 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   idx /= a.splits;
   const int h = idx % a.Hkv;
   Entry x;
-  x.b = a.wide_prefix ? -1 : (int)(idx / a.Hkv);
-  x.row0 = (a.wide_prefix ? rank : a.wide_tiles - 1 - rank) * kWideRows;
+  x.b = PREFIX ? -1 : (int)(idx / a.Hkv);
+  x.row0 = (PREFIX ? rank : a.wide_tiles - 1 - rank) * kWideRows;
   x.begin = 0;
-  if (a.wide_prefix) {
+  if (PREFIX) {
     x.end = a.prefix;
   } else {
     const int c = count_of(a, x.b), last = min(a.T * a.G, x.row0 + kWideRows) - 1;
@@ -1075,7 +1081,8 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       if (mine && key < x.end) {
         const unsigned p = (unsigned)key / (unsigned)a.page;
         in_page = (int)((unsigned)key - p * (unsigned)a.page);
-        page = a.table[(key < a.prefix ? 0 : x.b) * a.table_stride + p];
+        const int* entry = a.table + (key < a.prefix ? 0 : x.b) * a.table_stride + p;
+        page = read<PREFIX>(entry);
         page = page == -1 ? -2 : page;
       }
     };
@@ -1209,14 +1216,14 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   } else {
     const int quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
-    const Row w = row_of(a, x, r);
+    const Row w = row_of<PREFIX>(a, x, r);
     bool ok = true;
     if (n_kv > 0) {
       // this row of Q, zeros where there is none
       const uint4* q = reinterpret_cast<const uint4*>((const T*)a.q + w.b * a.q_sb + w.t * a.q_st + (long long)(h * a.G + w.g) * a.q_sh);
 #pragma unroll
       for (int c = 0; c < HD / 8; c++)
-        *reinterpret_cast<uint4*>(s_q + chunk_at<kWideRows>(r, c)) = w.counts && c * 8 < a.D ? __ldg(q + c) : make_uint4(0u, 0u, 0u, 0u);
+        *reinterpret_cast<uint4*>(s_q + chunk_at<kWideRows>(r, c)) = w.counts && c * 8 < a.D ? (PREFIX ? __ldcg(q + c) : __ldg(q + c)) : make_uint4(0u, 0u, 0u, 0u);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
@@ -1308,11 +1315,11 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     if (ok) {
       tc_fence_after();
       const float l = lo_of(l2) + hi_of(l2);
-      const bool direct = !a.wide_prefix && a.splits == 1;
+      const bool direct = !PREFIX && a.splits == 1;
       const float f = direct ? (w.counts && l != 0.f ? __frcp_rn(l) : 0.f) : 1.f;
       const long long all = (long long)a.B * a.T * a.H;
       const long long here = w.there ? ((long long)w.b * a.T + w.t) * a.H + h * a.G + w.g : -1;
-      const long long row = here < 0 || direct ? here : (a.wide_prefix ? 2LL * a.ctas * a.slot_rows + all : 0) + split * all + here;
+      const long long row = here < 0 || direct ? here : (PREFIX ? 2LL * a.ctas * a.slot_rows + all : 0) + split * all + here;
       if (row >= 0 && !direct) a.stat[row] = make_float2(m, l);
       // through this warp's part of Q's tile (all products have read it), so that a row leaves in whole lines: 32 rows of 64 fp32 or HD 16-bit values
       uint8_t* buf = s_q + quarter * (32 * 128) * C::CH;
@@ -1366,7 +1373,7 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     tc_fence_after();
     tmem_dealloc(tmem, C::COLS);
   }
-  if (a.wide_prefix) pdl_wait();
+  if (PREFIX) pdl_wait();
 }
 
 // Joins the partial rows of a query row: those of the prefix and those of its own sequence.  WPR warps a row, a lane four columns.  First the
@@ -1556,11 +1563,12 @@ int allow_shared(K kernel, int bytes, std::atomic<uint32_t>& done) {
 template <typename T, int HD, bool TMA>
 int launch_wide(const CUtensorMap& tk, const CUtensorMap& tv, const CacheArgs& a, cudaStream_t s) {
   using C = Wide<HD>;
-  static std::atomic<uint32_t> done{0};
-  const int rc = allow_shared(cache_wide_kernel<T, HD, TMA>, C::SMEM, done);
+  static std::atomic<uint32_t> done[2];
+  const auto kernel = a.wide_prefix ? cache_wide_kernel<T, HD, TMA, true> : cache_wide_kernel<T, HD, TMA, false>;
+  const int rc = allow_shared(kernel, C::SMEM, done[a.wide_prefix ? 1 : 0]);
   if (rc) return rc;
   const long long ctas = (long long)a.wide_tiles * a.splits * a.Hkv * (a.wide_prefix ? 1 : a.B);
-  GB_CUDA_OK(gbh::launch(cache_wide_kernel<T, HD, TMA>, dim3((unsigned)ctas), dim3(kWideThreads), C::SMEM, s, 1, tk, tv, a));
+  GB_CUDA_OK(gbh::launch(kernel, dim3((unsigned)ctas), dim3(kWideThreads), C::SMEM, s, 1, tk, tv, a));
   return gbh::E_OK;
 }
 

@@ -288,6 +288,13 @@ def test_beyond_32_bits():
     close(cache.Attend(q, table, at), attended(cache, q, table, at, None))
 
 
+def test_tables_too_long_to_number_their_tiles():
+    cache = nn.KVCache(1, 1024, 64, 8, dtype=BF, device="cuda")
+    q, at = torch.zeros(1, 1, 64, 8, device="cuda", dtype=BF), torch.zeros(1, device="cuda", dtype=torch.int32)
+    with pytest.raises(lib.NativeError):
+        cache.Attend(q, torch.zeros(1, 2 ** 20, device="cuda", dtype=torch.int32), at)
+
+
 def test_calls_of_a_new_thread():
     """A thread whose first CUDA call is this one."""
     import threading
@@ -360,11 +367,11 @@ def test_other_streams_and_graphs():
         with torch.cuda.graph(g, stream=s):
             outs.append(step(*a))
         graphs.append(g)
-    for shift in (0, 1, 0):
+    for shift, times in ((0, 20), (1, 1), (-1, 1), (1, 20)):            # (once, too: nothing of the replay before may be left)
         at += shift
         at3 += shift
         torch.cuda.synchronize()
-        for _ in range(20):
+        for _ in range(times):
             for s, g in zip(side, graphs):
                 with torch.cuda.stream(s):
                     g.replay()
