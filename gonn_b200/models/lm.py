@@ -146,8 +146,11 @@ class GPT(Module):
         take the new ones up (see ``KVCache`` for table, lengths, counts and shared_pages).  For evaluation: under torch.no_grad()."""
         x = self.tok(ids)
         if self.pos is not None:
-            at = lengths.long()[:, None] + torch.arange(ids.shape[1], device=ids.device)
-            x = _binary("add", x, self.pos(at.clamp(max=self.max_seq - 1)))      # (tokens that do not count may lie beyond)
+            token = torch.arange(ids.shape[1], device=ids.device)
+            at = lengths.long()[:, None] + token
+            if counts is not None:               # tokens that do not count may lie behind the last position
+                at = torch.where(token < counts[:, None], at, 0)
+            x = _binary("add", x, self.pos(at))
         for block, cache in zip(self.layers, caches):
             x = block.Step(x, cache, table, lengths, counts, shared_pages)
         return self.head(self.norm(x))

@@ -205,3 +205,25 @@ def test_generate(rotary):
     if rotary is None:
         with pytest.raises(ValueError):
             model.Generate(ids, 26)
+
+
+def test_steps_behind_the_last_learned_position():
+    """Refused as ``forward`` refuses them; tokens that do not count may lie there."""
+    from gonn_b200.models import GPT
+    torch.manual_seed(6)
+    model = GPT(vocab=31, d_model=16, n_layers=1, n_heads=2, d_ff=24, max_seq=8, dtype=torch.float64)
+    ids = torch.randint(0, 31, (2, 12))
+    table, at = torch.arange(6, dtype=torch.int32).view(2, 3), torch.zeros(2, dtype=torch.int32)
+    with torch.no_grad():
+        with pytest.raises(IndexError):
+            model(ids)
+        with pytest.raises(IndexError):
+            model.Step(ids, model.Caches(6, 4), table, at)
+        caches = model.Caches(6, 4)
+        whole = model.Step(ids[:, :8], caches, table, at)
+        assert torch.allclose(whole, model(ids[:, :8]))
+        with pytest.raises(IndexError):
+            model.Step(ids[:, 8:9], caches, table, at + 8)
+        padded = model.Step(ids, model.Caches(6, 4), table, at, counts=torch.tensor([8, 3], dtype=torch.int32))
+        # (attention over 3 positions and over 8 may add in another order: at most 24 terms a sum, 24 2^-53 of their magnitudes, a few sums in a row)
+        assert torch.equal(padded[0, :8], whole[0]) and torch.allclose(padded[1, :3], whole[1, :3], rtol=1e-12, atol=1e-12)

@@ -501,3 +501,21 @@ def test_samples_share_the_prompt():
     ids = torch.randint(0, 61, (1, 150), device="cuda")
     out = model.Generate(ids, 6, samples=80, page_size=16)
     assert out.shape == (80, 156) and torch.equal(out, out[:1].expand(80, -1)) and torch.equal(out[:, :150], ids.expand(80, -1))
+
+
+def test_steps_behind_the_last_learned_position():
+    """Reported as ``forward`` reports them; tokens that do not count may lie there."""
+    from gonn_b200.models import GPT
+    torch.manual_seed(6)
+    model = GPT(vocab=31, d_model=128, n_layers=1, n_heads=2, d_ff=64, max_seq=8, device="cuda")
+    ids = torch.randint(0, 31, (2, 12), device="cuda")
+    table, at = torch.arange(6, device="cuda", dtype=torch.int32).view(2, 3), torch.zeros(2, device="cuda", dtype=torch.int32)
+    with torch.no_grad():
+        model(ids)
+        assert lib.read_status()[0] == 5
+        model.Step(ids, model.Caches(6, 4), table, at)
+        assert lib.read_status()[0] == 5
+        model.Step(ids[:, :1], model.Caches(6, 4), table, at + 8)
+        assert lib.read_status()[0] == 5
+        model.Step(ids, model.Caches(6, 4), table, at, counts=torch.tensor([8, 3], device="cuda", dtype=torch.int32))
+        lib.assert_status_ok()
