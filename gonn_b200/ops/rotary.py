@@ -92,12 +92,14 @@ class _Rotary(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, positions, turns, interleaved, amplitude, back):
-        ctx.rest = positions, turns, interleaved, amplitude, not back
+        ctx.save_for_backward(positions, turns)                 # (the tape tells if they have been written over)
+        ctx.rest = interleaved, amplitude, not back
         return _launch(x, positions, turns, interleaved, amplitude, back)
 
     @staticmethod
     def backward(ctx, dy):
-        dx = _Rotary.apply(dy, *ctx.rest) if torch.is_grad_enabled() else _launch(dy, *ctx.rest)
+        turn = _Rotary.apply if torch.is_grad_enabled() else _launch
+        dx = turn(dy, *ctx.saved_tensors, *ctx.rest)
         return dx, None, None, None, None, None
 
 

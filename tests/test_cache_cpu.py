@@ -227,3 +227,21 @@ def test_steps_behind_the_last_learned_position():
         padded = model.Step(ids, model.Caches(6, 4), table, at, counts=torch.tensor([8, 3], dtype=torch.int32))
         # (attention over 3 positions and over 8 may add in another order: at most 24 terms a sum, 24 2^-53 of their magnitudes, a few sums in a row)
         assert torch.equal(padded[0, :8], whole[0]) and torch.allclose(padded[1, :3], whole[1, :3], rtol=1e-12, atol=1e-12)
+
+
+def test_positions_changed_behind_the_tape(monkeypatch):
+    """The gradient's turn needs the positions of the forward's: the tape tells that they have been written over."""
+    from gonn_b200.ops import rotary
+    rope = nn.RotaryEmbedding(4)
+
+    def launch(x, positions, turns, interleaved, amplitude, back, out=None):       # the kernel's part, on the CPU
+        return rotary.rotate_ref(x.detach(), positions, rope._w, interleaved, amplitude, back)
+    monkeypatch.setattr(rotary, "_launch", launch)
+    x, at = torch.randn(1, 3, 2, 4, requires_grad=True), torch.arange(3)
+    call = lambda: rotary._Rotary.apply(x, at, rope.turns, False, 1.0, False)
+    dx, = torch.autograd.grad(call().sum(), x)
+    assert torch.allclose(dx, rotary.rotate_ref(torch.ones_like(x), at, rope._w, False, 1.0, True))
+    y = call()
+    at += 3
+    with pytest.raises(RuntimeError):
+        y.sum().backward()

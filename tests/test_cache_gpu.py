@@ -519,3 +519,14 @@ def test_steps_behind_the_last_learned_position():
         assert lib.read_status()[0] == 5
         model.Step(ids, model.Caches(6, 4), table, at, counts=torch.tensor([8, 3], device="cuda", dtype=torch.int32))
         lib.assert_status_ok()
+
+
+def test_positions_changed_behind_the_tape():
+    rope = nn.RotaryEmbedding(64, device="cuda")
+    x, at = torch.randn(1, 3, 2, 64, device="cuda", requires_grad=True), torch.arange(3, device="cuda")
+    y = rope(x, at)
+    at += 3
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
+    rope(x).sum().backward()                                            # without positions: 0, 1, ...
+    close(x.grad, turned(torch.ones_like(x), torch.arange(3, device="cuda"), rope, back=True))
