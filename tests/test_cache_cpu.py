@@ -245,3 +245,20 @@ def test_positions_changed_behind_the_tape(monkeypatch):
     at += 3
     with pytest.raises(RuntimeError):
         y.sum().backward()
+
+
+def test_checkpoints_leave_frequencies_alone(tmp_path):
+    """Frequencies follow from a module's options: a model saved with others, or before it had any, loads, and keeps its own."""
+    from gonn_b200.utils import checkpoint
+
+    class Layer(nn.Module):
+        def __init__(self, rope):
+            super().__init__()
+            self.proj, self.rope = nn.Linear(4, 4), rope
+    path, plain = str(tmp_path / "x"), nn.RotaryEmbedding(8)
+    first, other = Layer(plain), Layer(nn.RotaryEmbedding(8, scaling="linear", factor=4.0))
+    want = other.rope.turns.clone()
+    for source in (first, Layer(None)):
+        checkpoint.save(path, source)
+        checkpoint.load(path, other)
+        assert torch.equal(other.rope.turns, want) and torch.equal(other.proj.weight, source.proj.weight)
