@@ -162,6 +162,8 @@ class MultiHeadAttention(Module):
         B, T, E = x.shape
         H, D = self.num_heads, self.head_dim
         p = self.qproj, self.kproj, self.vproj
+        if torch.is_grad_enabled() and (x.requires_grad or any(t.requires_grad for l in p for t in l.parameters())):
+            raise RuntimeError("MultiHeadAttention.ForwardCached: no gradient goes through a cache; call under torch.no_grad()")
         w, b = fused_view([l.weight for l in p]), None
         if w is not None and p[0].bias is not None:
             b = fused_view([l.bias for l in p])

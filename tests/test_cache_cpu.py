@@ -262,3 +262,37 @@ def test_checkpoints_leave_frequencies_alone(tmp_path):
         checkpoint.save(path, source)
         checkpoint.load(path, other)
         assert torch.equal(other.rope.turns, want) and torch.equal(other.proj.weight, source.proj.weight)
+
+
+def test_steps_of_a_layer_under_a_tape_are_refused():
+    """Nothing has a gradient through a cache: refused wherever the input or a projection into the cache would need one."""
+    mha = nn.MultiHeadAttention(16, 2, dtype=torch.float64)
+    cache, x = nn.KVCache(1, 4, 2, 8, dtype=torch.float64), torch.randn(1, 1, 16, dtype=torch.float64)
+    table, at = torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(RuntimeError):
+        mha.ForwardCached(x, cache, table, at)
+    with torch.no_grad():
+        want = mha.ForwardCached(x, cache, table, at)
+    for p in mha.parameters():
+        p.requires_grad_(False)
+    with pytest.raises(RuntimeError):
+        mha.ForwardCached(x.clone().requires_grad_(), cache, table, at)
+    assert torch.equal(mha.ForwardCached(x, cache, table, at), want)
+    mha.outproj.weight.requires_grad_(True)                            # behind the cache: a gradient like any other
+    mha.ForwardCached(x, cache, table, at).sum().backward()
+    assert mha.outproj.weight.grad is not None
+    # the value's projection alone: its keys and queries need none
+    mha.vproj.bias.requires_grad_(True)
+    with pytest.raises(RuntimeError):
+        mha.ForwardCached(x, cache, table, at)
+
+
+def test_fused_steps_under_a_tape_are_refused(monkeypatch):
+    """The product of all three projections at once, which only CUDA takes, refuses them alike: here it would not be reached."""
+    from gonn_b200.nn import attention
+    mha, called = nn.MultiHeadAttention(16, 2), []
+    monkeypatch.setattr(attention, "fused_view", lambda parts: called.append(1))
+    table, at = torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(RuntimeError):
+        mha.ForwardCached(torch.randn(1, 1, 16), nn.KVCache(1, 4, 2, 8), table, at)
+    assert not called

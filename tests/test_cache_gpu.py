@@ -530,3 +530,20 @@ def test_positions_changed_behind_the_tape():
         y.sum().backward()
     rope(x).sum().backward()                                            # without positions: 0, 1, ...
     close(x.grad, turned(torch.ones_like(x), torch.arange(3, device="cuda"), rope, back=True))
+
+
+def test_steps_of_a_layer_under_a_tape_are_refused():
+    mha = nn.MultiHeadAttention(128, 2, dtype=BF, device="cuda")
+    cache, x = nn.KVCache(1, 16, 2, 64, dtype=BF, device="cuda"), torch.randn(1, 1, 128, device="cuda").to(BF)
+    table, at = torch.zeros(1, 1, device="cuda", dtype=torch.int32), torch.zeros(1, device="cuda", dtype=torch.int32)
+    for need in (mha.qproj.weight, mha.kproj.weight, mha.vproj.bias):
+        for p in mha.parameters():
+            p.requires_grad_(p is need)
+        with pytest.raises(RuntimeError):
+            mha.ForwardCached(x, cache, table, at)
+        with torch.no_grad():
+            mha.ForwardCached(x, cache, table, at)
+    for p in mha.parameters():
+        p.requires_grad_(p is mha.outproj.weight)                       # behind the cache: a gradient like any other
+    mha.ForwardCached(x, cache, table, at).sum().backward()
+    assert mha.outproj.weight.grad is not None
