@@ -66,7 +66,7 @@ def _check_batch(what, c, batch, table, lengths, counts):
 def _like_cache(what, name, t, c):
     if t.dtype is not c.dtype or t.get_device() != c.index:
         raise TypeError(f"{what}: {name} is {t.dtype} on {t.device}, the cache {c.dtype} on {c.device}")
-    if t.requires_grad and torch.is_grad_enabled():
+    if torch.is_grad_enabled() and (t.requires_grad or c.keys.requires_grad or c.values.requires_grad):
         raise RuntimeError(f"{what}: no gradient goes through a cache; call under torch.no_grad()")
 
 

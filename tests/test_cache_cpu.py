@@ -296,3 +296,17 @@ def test_fused_steps_under_a_tape_are_refused(monkeypatch):
     with pytest.raises(RuntimeError):
         mha.ForwardCached(torch.randn(1, 1, 16), nn.KVCache(1, 4, 2, 8), table, at)
     assert not called
+
+
+def test_caches_in_tensors_that_need_a_gradient():
+    q, k = torch.randn(1, 1, 2, 8), torch.randn(1, 1, 2, 8)
+    table, at = torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    for which in range(2):
+        tensors = [torch.zeros(1, 2, 4, 8) for _ in range(2)]
+        cache = nn.KVCache.Over(*tensors)
+        tensors[which].requires_grad_()
+        for call in (lambda: cache.Append(k, k, table, at), lambda: cache.Attend(q, table, at)):
+            with pytest.raises(RuntimeError, match="under torch.no_grad"):
+                call()
+            with torch.no_grad():
+                call()

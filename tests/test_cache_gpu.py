@@ -547,3 +547,17 @@ def test_steps_of_a_layer_under_a_tape_are_refused():
         p.requires_grad_(p is mha.outproj.weight)                       # behind the cache: a gradient like any other
     mha.ForwardCached(x, cache, table, at).sum().backward()
     assert mha.outproj.weight.grad is not None
+
+
+def test_caches_in_tensors_that_need_a_gradient():
+    q, k = torch.randn(1, 1, 2, 8, device="cuda"), torch.randn(1, 1, 2, 8, device="cuda")
+    table, at = torch.zeros(1, 1, device="cuda", dtype=torch.int32), torch.zeros(1, device="cuda", dtype=torch.int32)
+    for which in range(2):
+        tensors = [torch.zeros(1, 2, 4, 8, device="cuda") for _ in range(2)]
+        cache = nn.KVCache.Over(*tensors)
+        tensors[which].requires_grad_()
+        for call in (lambda: cache.Append(k, k, table, at), lambda: cache.Attend(q, table, at)):
+            with pytest.raises(RuntimeError, match="under torch.no_grad"):
+                call()
+            with torch.no_grad():
+                call()
