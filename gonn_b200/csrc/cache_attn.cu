@@ -1489,6 +1489,7 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const CacheArgs a) {
 // host side
 // ---------------------------------------------------------------------------------------------------------------------------
 constexpr int kCtas = 2 * 148;
+constexpr long long kMost = 0x7fffffffLL - 256;  // positions of a table, and rows of queries: a tile that starts within them ends within 32 bits
 constexpr long long kFewRows = 148 * 8;          // rows that are joined by eight warps each: those CTAs all fit at a time
 
 struct Sizes {
@@ -1500,10 +1501,9 @@ struct Sizes {
 
 // Which kernel takes what, and the workspace.
 bool plan(Sizes& z, int dtype, long long B, long long T, long long H, long long Hkv, long long D, int prefix, long long room) {
-  if (B * T * H >= 0x7fffffffLL) return false;
+  if (B * T * H > kMost || room > kMost) return false;
   const long long own = T * (H / Hkv), all = B * own;
   z = Sizes{};
-  if (all >= 0x7fffffffLL) return false;
   // Many rows of a sequence: its keys with the prefix among them, nothing is gained by sharing.  Many rows of the batch alone: its prefix.
   // us, few rows' kernel | this one, bf16, eight key heads of 128, 32, 48, 64, 96 rows to a key head: 8 sequences of 8 192 positions 63 | 60, 68 | 61, 70 | 62,
   // 117 | 64; of 1 024 to 8 192 41 | 52, 50 | 54, 53 | 57; 64 such ones 211 | 241, 249 | 256, 263 | 254.  Heads of 64 37 | 39, 43 | 43, 45 | 44, 72 | 46.  A shared
@@ -1667,7 +1667,7 @@ GB_EXPORT long long gb_cache_attn_bytes(int dtype, long long B, long long T, lon
   Sizes z;
   if (dtype < 0 || dtype > 2 || B < 0 || T < 1 || H < 1 || Hkv < 1 || H % Hkv || D < 1 || D > 128 ||
       !plan(z, dtype, B, T, H, Hkv, D, prefix, room)) {
-    gbh::set_error("gb_cache_attn: too many rows, or bad sizes (%lld sequences, %lld tokens, %lld and %lld heads of %lld)", B, T, H, Hkv, D);
+    gbh::set_error("gb_cache_attn: too many rows or positions, or bad sizes (%lld sequences, %lld tokens, %lld and %lld heads of %lld)", B, T, H, Hkv, D);
     return gbh::E_TOO_LARGE;
   }
   return z.total;
@@ -1703,7 +1703,7 @@ GB_EXPORT int gb_cache_attn(int dtype, const void* q, const void* k, const void*
     gbh::set_error("gb_cache_attn: null pointer or empty cache");
     return gbh::E_BAD_ARG;
   }
-  if ((long long)columns * page >= 0x7fffffffLL || prefix < 0 || prefix > (long long)columns * page || prefix % page || !(scale > 0)) {
+  if ((long long)columns * page > kMost || prefix < 0 || prefix > (long long)columns * page || prefix % page || !(scale > 0)) {
     gbh::set_error("gb_cache_attn: a table of %d pages of %d positions, %d of them shared, scale %g", columns, page, prefix, scale);
     return gbh::E_BAD_ARG;
   }

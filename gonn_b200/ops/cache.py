@@ -14,6 +14,7 @@ from .. import lib as _l
 from .rotary import _TYPES, rotate_ref, words
 
 MAX_HEAD = 128                    # largest head that attention on CUDA takes
+MAX_ROOM = 2 ** 31 - 257          # positions of a table: a tile of keys that starts within them ends within 32 bits
 
 
 class Layout:
@@ -46,7 +47,7 @@ _I32 = torch.int32
 
 def _check_batch(what, c, batch, table, lengths, counts):
     if (table.dtype is _I32 and lengths.dtype is _I32 and table.dim() == 2 and table.shape[0] == batch and table.shape[1] > 0
-            and lengths.shape == (batch,) and table.get_device() == c.index == lengths.get_device() and table.shape[1] * c.page < 2 ** 31 - 1
+            and lengths.shape == (batch,) and table.get_device() == c.index == lengths.get_device() and table.shape[1] * c.page <= MAX_ROOM
             and (counts is None or counts.dtype is _I32 and counts.shape == (batch,) and counts.get_device() == c.index)):
         return
     for name, t, dims in (("table", table, 2), ("lengths", lengths, 1), ("counts", counts, 1)):
@@ -60,7 +61,7 @@ def _check_batch(what, c, batch, table, lengths, counts):
             raise ValueError(f"{what}: {name} is on {t.device}, the cache on {c.device}")
     if table.shape[1] < 1:
         raise ValueError(f"{what}: the table has no columns")
-    raise ValueError(f"{what}: a sequence holds fewer than 2^31 - 1 positions, the table {table.shape[1]} pages of {c.page}")
+    raise ValueError(f"{what}: a sequence holds up to {MAX_ROOM} positions, the table {table.shape[1]} pages of {c.page}")
 
 
 def _like_cache(what, name, t, c):

@@ -310,3 +310,21 @@ def test_caches_in_tensors_that_need_a_gradient():
                 call()
             with torch.no_grad():
                 call()
+
+
+def test_tables_of_nearly_2_to_the_31_positions():
+    """A tile's last key is counted in 32 bits: tables whose last tile would pass them are refused, by the native library too, and so are rows of
+    queries."""
+    from gonn_b200 import lib
+    q = torch.zeros(0, 1, 1, 8)
+    table, at = torch.zeros(0, 1, dtype=torch.int32), torch.zeros(0, dtype=torch.int32)
+    for page, fits in ((2 ** 31 - 257, True), (2 ** 31 - 256, False), (2 ** 31 - 2, False)):
+        cache = nn.KVCache.Over(*(torch.zeros(1, 1, 1, 8).expand(1, 1, page, 8) for _ in range(2)))
+        for call in (lambda: cache.Attend(q, table, at), lambda: cache.Append(q, q, table, at)):
+            if fits:
+                call()
+            else:
+                with pytest.raises(ValueError):
+                    call()
+        assert (lib.lib().gb_cache_attn_bytes(0, 1, 1, 1, 1, 8, 0, page) >= 0) == fits
+        assert (lib.lib().gb_cache_attn_bytes(0, 1, page, 1, 1, 8, 0, 1024) >= 0) == fits
