@@ -17,7 +17,8 @@
 // memory instead: no second kernel (one token behind 2 047 positions of 16 heads: 9.6 us, 14.7 with it).
 //
 // A shared prefix is one more entry at the head of the list whose rows are the queries of all sequences: its keys are read once for
-// every 16, 32 or 64 rows.  The sequences' own entries then start behind it, and all rows are joined by the second kernel.
+// every 16, 32 or 64 rows.  The sequences' own entries then start behind it, and all rows are joined by the second kernel.  The prefix ends before the
+// page in which the shortest sequence ends, so that no row meets a value that its own sequence does not have.
 //
 // A CTA: four warps that multiply (mma.sync for 16-bit types, FMA for fp32) and four that copy through a ring of stages: by TMA, a box of
 // as many rows as divide both a page and a tile, where these are at least eight (a multiple of the swizzle's period); else with cp.async,
@@ -64,7 +65,7 @@ struct CacheArgs {
   int wide_prefix, wide_own;               // which of them the kernel for many rows takes
   int wide_tiles, splits, wide_group;      // its row tiles, of a sequence or of the prefix; runs of keys; runs whose tiles go together
   int slot_rows;                           // rows of the other kernel's tiles
-  int2* owner;                             // [(prefix tiles + B own_tiles) Hkv] first and last CTA
+  int2* owner;                             // [(prefix tiles + B own_tiles) Hkv] first and last CTA; then (end of the prefix, 0)
   int* status;
 };
 
@@ -125,16 +126,30 @@ __device__ __forceinline__ int count_of(const CacheArgs& a, int b) {
   return c < 0 ? 0 : c < a.T ? c : a.T;
 }
 
+// The least end of those of the sequences first, first + step, .. that have positions and tokens that count, the prefix's at most.
+template <bool L2 = false>
+__device__ __forceinline__ int least_end(const CacheArgs& a, int first, int step) {
+  int least = a.prefix;
+#pragma unroll 4
+  for (int b = first; b < a.B; b += step) {
+    const int c = count_of<L2>(a, b);
+    const long long end = (long long)read<L2>(a.lengths + b) + c;
+    if (c > 0 && end > 0 && end < least) least = (int)end;
+  }
+  return least;
+}
+
+// prefix: where the shared positions end.
 template <int ROWS, int TILE>
-__device__ __forceinline__ Entry entry_of(const CacheArgs& a, int e) {
+__device__ __forceinline__ Entry entry_of(const CacheArgs& a, int prefix, int e) {
   Entry x;
-  x.begin = a.prefix;
+  x.begin = prefix;
   x.cut = false;
   if (e < a.prefix_tiles) {
     x.b = -1;
     x.row0 = e * ROWS;
     x.begin = 0;
-    x.end = a.prefix;
+    x.end = prefix;
   } else {
     e -= a.prefix_tiles;
     long long end;
@@ -172,18 +187,24 @@ template <int ROWS, int TILE>
 struct Cursor {
   Shares shares;
   Entry x;
-  int e, h, entries, tile;
+  int e, h, entries, tile, prefix;
   unsigned left, segment0;           // tiles to go; the list's number of the segment's first tile
 
   // Adds up the tiles of all entries, an entry or a run of them a lane, and finds this CTA's share.  (Totals stay below 2^31.)
   __device__ __forceinline__ void start(const CacheArgs& a, int lane) {
     entries = a.prefix_tiles + a.B * a.own_tiles;
+    prefix = 0;
+    if (a.shared) {
+      // Whole pages that all sequences have: behind a sequence's end a row of V may be anything, and NaN times a weight of 0 is NaN.
+      prefix = __reduce_min_sync(0xffffffffu, least_end(a, lane, 32)) / a.page * a.page;
+      if (blockIdx.x == 0 && threadIdx.x == 32 * kConsumers) a.owner[entries * a.Hkv] = make_int2(prefix, 0);
+    }
     const int per = (entries + 31) / 32, lo = min(entries, lane * per), hi = min(entries, lo + per);
     unsigned mine = 0;
     Entry first_entry;
 #pragma unroll 4
     for (int k = lo; k < hi; k++) {
-      const Entry y = entry_of<ROWS, TILE>(a, k);
+      const Entry y = entry_of<ROWS, TILE>(a, prefix, k);
       if (k == lo) first_entry = y;
       mine += y.tiles;
       if (y.cut && blockIdx.x == 0 && threadIdx.x < 32 * (kConsumers + 1)) set_status(a.status, ST_BAD_INDEX, y.b);
@@ -211,7 +232,7 @@ struct Cursor {
         const unsigned n = (unsigned)x.tiles * a.Hkv;
         if (first < at + n) break;
         at += n;
-        x = entry_of<ROWS, TILE>(a, ++e);
+        x = entry_of<ROWS, TILE>(a, prefix, ++e);
       }
       h = (first - at) / x.tiles;
       at += h * x.tiles;
@@ -231,7 +252,7 @@ struct Cursor {
     const int seg = blockIdx.x / peers;
     e = seg / a.Hkv;
     h = seg - e * a.Hkv;
-    x = entry_of<ROWS, TILE>(a, e);
+    x = entry_of<ROWS, TILE>(a, 0, e);
     if (x.cut && rank == 0 && threadIdx.x == 32 * kConsumers) set_status(a.status, ST_BAD_INDEX, x.b);
     tile = x.tiles * rank / peers;
     left = x.tiles * (rank + 1) / peers - tile;
@@ -243,7 +264,7 @@ struct Cursor {
     h = 0;
     do {
       if (++e >= entries) return;
-      x = entry_of<ROWS, TILE>(a, e);
+      x = entry_of<ROWS, TILE>(a, prefix, e);
     } while (x.tiles == 0);
   }
 };
@@ -442,7 +463,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       if ((TMA ? unit < units : lane < MINE) && key < at.x.end) {
         const unsigned p = (unsigned)key / (unsigned)a.page;
         in_page = (int)((unsigned)key - p * (unsigned)a.page);
-        const int got = a.table[(at.x.b < 0 ? 0 : at.x.b) * a.table_stride + p];
+        const int got = a.table[(key < a.prefix ? 0 : at.x.b) * a.table_stride + p];
         page = got == -1 ? -2 : got;
       }
     };
@@ -1015,6 +1036,7 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   long long* s_off = (long long*)(pv_done + 2);                      // where the keys and values of a sub-tile start (cp.async)
   uint32_t* tmem_slot = (uint32_t*)(s_off + 2 * kWideKeys);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+  int* s_end = (int*)(tmem_slot + 2);                                // [8] least ends that the warps found
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -1036,6 +1058,10 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   if (warp == kWideCopiers) {
     tmem_alloc(tmem_slot, C::COLS);
     tmem_relinquish();
+  }
+  if (PREFIX) {
+    const int least = __reduce_min_sync(0xffffffffu, least_end<true>(a, threadIdx.x, kWideThreads));
+    if (lane == 0) s_end[warp] = least;
   }
   tc_fence_before();
   __syncthreads();
@@ -1060,7 +1086,9 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   x.row0 = (PREFIX ? rank : a.wide_tiles - 1 - rank) * kWideRows;
   x.begin = 0;
   if (PREFIX) {
-    x.end = a.prefix;
+    x.end = a.prefix;                            // as the other kernel finds it
+    for (int i = 0; i < kWideThreads / 32; i++) x.end = min(x.end, s_end[i]);
+    x.end = x.end / a.page * a.page;
   } else {
     const int c = count_of(a, x.b), last = min(a.T * a.G, x.row0 + kWideRows) - 1;
     const long long end = x.row0 / a.G < c ? (long long)a.lengths[x.b] + min(c, last / a.G + 1) : 0;
@@ -1396,8 +1424,9 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const CacheArgs a) {
   struct Parts { long long first, rest, step; int n; };
   Parts pre = {0, 0, 0, 0}, own = {0, 0, 0, 0};
   const long long whole = 2LL * a.ctas * ROWS;
+  const int prefix = a.shared ? a.owner[(a.prefix_tiles + a.B * a.own_tiles) * a.Hkv].x : 0;
   auto find = [&](Parts& p, int e, const int2 c, int r, long long at) {
-    if (entry_of<ROWS, TILE>(a, e).tiles == 0) return true;          // (whose owner is anything)
+    if (entry_of<ROWS, TILE>(a, prefix, e).tiles == 0) return true;  // (whose owner is anything)
     const int cta = c.x >> 1;
     if (cta == c.y) {                             // one CTA had all of it
       p = {at, at, 0, 1};
@@ -1545,7 +1574,7 @@ bool plan(Sizes& z, int dtype, long long B, long long T, long long H, long long 
   auto up = [](long long n) { return (n + 255) / 256 * 256; };
   z.part = up(rows * D * 4);
   z.stat = up(rows * 8);
-  z.owner = up(z.entries * Hkv * 8);
+  z.owner = up((z.entries * Hkv + 1) * 8);
   z.total = z.part + z.stat + z.owner;
   return true;
 }

@@ -87,5 +87,5 @@ class KVCache:
         head h.  Zeros where a token does not count.  scale: 1 / sqrt(head size).
 
         ``shared_pages``: all sequences have the same first pages (a common prompt), which are taken from the table's first row and read
-        once for many sequences."""
+        once for many sequences: those that lie before the end of the shortest sequence, which may end inside them."""
         return _cache.attend(self._of, q, table, lengths, counts, scale, shared_pages)

@@ -561,3 +561,48 @@ def test_caches_in_tensors_that_need_a_gradient():
                 call()
             with torch.no_grad():
                 call()
+
+
+def ended(B, T, H, kv, D, page, prefix, ends, dtype, counts, seed=0):
+    """A batch whose sequences share their first `prefix` pages and end (their last tokens that count included) at `ends`, inside them too; NaN in every
+    row behind the last sequence's end."""
+    g = torch.Generator("cuda").manual_seed(seed)
+    columns = max(prefix, -(-max(ends) // page)) + 1
+    order = torch.randperm(prefix + B * (columns - prefix), generator=g, device="cuda").int()
+    table = torch.empty(B, columns, dtype=torch.int32, device="cuda")
+    table[:, :prefix] = order[:prefix]
+    table[:, prefix:] = order[prefix:].view(B, -1)
+    kc, vc = (torch.full((order.numel(), kv, page, D), math.nan, device="cuda", dtype=dtype) for _ in range(2))
+    for b, n in enumerate(ends):
+        p = torch.arange(n, device="cuda")
+        pages = table[b].long()[p // page]
+        for t in (kc, vc):
+            t[pages, :, p % page] = torch.randn(n, kv, D, generator=g, device="cuda").to(dtype)
+    c = torch.tensor([T] * B if counts is None else counts, dtype=torch.int32, device="cuda")
+    q = torch.randn(B, T, H, D, generator=g, device="cuda").to(dtype)
+    return nn.KVCache.Over(kc, vc), q, table, torch.tensor(ends, dtype=torch.int32, device="cuda") - c, None if counts is None else c
+
+
+ENDED = [(3, 1, 4, 2, 64, 16, 4, [10, 40, 50], None), (70, 1, 8, 1, 128, 32, 3, [33 + i % 40 for i in range(70)], None),
+         (5, 3, 4, 2, 72, 24, 2, [3, 30, 47, 20, 48], [3, 0, 1, 2, 3]), (20, 2, 3, 1, 40, 7, 11, [50 + i for i in range(20)], None),
+         (2, 1, 2, 1, 128, 64, 1, [5, 63], None), (80, 1, 1, 1, 64, 64, 2, [0] * 40 + [100] * 40, [0] * 40 + [1] * 40),
+         (33, 1, 8, 2, 64, 64, 40, [2500 + i for i in range(33)], None), (4, 17, 4, 1, 128, 16, 30, [470, 471, 300, 479], None)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("B,T,H,kv,D,page,prefix,ends,counts", ENDED)
+def test_sequences_that_end_inside_the_shared_pages(dtype, B, T, H, kv, D, page, prefix, ends, counts):
+    cache, q, table, at, c = ended(B, T, H, kv, D, page, prefix, ends, dtype, counts)
+    close(cache.Attend(q, table, at, counts=c, shared_pages=prefix), attended(cache, q, table, at, c))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("B", [3, 70])
+def test_infinite_values_that_a_shorter_sequence_does_not_have(dtype, B):
+    """A value of the shared pages behind the end of the first sequence is infinite: the others' alone."""
+    cache, q, table, at, c = ended(B, 1, 4, 1, 64, 16, 6, [40] + [90 + i for i in range(B - 1)], dtype, None)
+    cache.Values[int(table[0, 3]), :, 2] = math.inf
+    out = cache.Attend(q, table, at, shared_pages=6)
+    want, tol = attended(cache, q[:1], table, at[:1], None)
+    close(out[:1], (want, tol))
+    assert bool((out[1:] == math.inf).all())
