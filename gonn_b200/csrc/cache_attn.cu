@@ -1719,6 +1719,11 @@ GB_EXPORT int gb_cache_attn(int dtype, const void* q, const void* k, const void*
     gbh::set_error("gb_cache_attn: null pointer");
     return gbh::E_BAD_ARG;
   }
+  for (int i = 9; i <= 18; i++)                  // kept in 32 bits, but for the table's stride
+    if (i != 14 && (sizes[i] < 0 || sizes[i] > 0x7fffffffLL)) {
+      gbh::set_error("gb_cache_attn: size %d is %lld, beyond 31 bits", i, sizes[i]);
+      return gbh::E_TOO_LARGE;
+    }
   const long long q_sb = sizes[0], q_st = sizes[1], q_sh = sizes[2], *strides = sizes + 3, table_stride = sizes[14];
   const int B = (int)sizes[9], T = (int)sizes[10], H = (int)sizes[11], Hkv = (int)sizes[12], D = (int)sizes[13], columns = (int)sizes[15];
   const int pages = (int)sizes[16], page = (int)sizes[17], prefix = (int)sizes[18];

@@ -273,6 +273,16 @@ int vector_of(int size, const RotaryArgs& a) {
   return v;
 }
 
+// Sizes that are kept in 32 bits from here on.
+bool sizes_fit(const char* what, const long long* sizes, int first, int last) {
+  for (int i = first; i <= last; i++)
+    if (sizes[i] < 0 || sizes[i] > 0x7fffffffLL) {
+      gbh::set_error("%s: size %d is %lld, beyond 31 bits", what, i, sizes[i]);
+      return false;
+    }
+  return true;
+}
+
 int checked(const char* what, int dtype, const RotaryArgs& a) {
   if (dtype < 0 || dtype > 2) {
     gbh::set_error("%s: bad dtype %d", what, dtype);
@@ -304,6 +314,7 @@ GB_EXPORT int gb_rotary(int dtype, const void* x, void* y, const long long* size
     return gbh::E_BAD_ARG;
   }
   const long long* z = sizes;
+  if (!sizes_fit("gb_rotary", z, 6, 10)) return gbh::E_TOO_LARGE;
   RotaryArgs a = {};
   a.q = {x, y, z[0], z[1], z[2], z[3], z[5], z[4], (int)z[8]};
   a.batch = (int)z[6]; a.tokens = (int)z[7]; a.width = (int)z[9]; a.dim = (int)z[10]; a.half = a.dim / 2;
@@ -333,6 +344,7 @@ GB_EXPORT int gb_cache_append(int dtype, const void* q, void* q_out, const void*
     return gbh::E_BAD_ARG;
   }
   const long long* z = sizes;
+  if (!sizes_fit("gb_cache_append", z, 15, 20) || !sizes_fit("gb_cache_append", z, 23, 25)) return gbh::E_TOO_LARGE;
   RotaryArgs a = {};
   a.batch = (int)z[15]; a.tokens = (int)z[16]; a.width = (int)z[19]; a.dim = (int)z[20]; a.half = a.dim / 2;
   const int q_heads = q ? (int)z[17] : 0, heads = (int)z[18];

@@ -328,3 +328,22 @@ def test_tables_of_nearly_2_to_the_31_positions():
                     call()
         assert (lib.lib().gb_cache_attn_bytes(0, 1, 1, 1, 1, 8, 0, page) >= 0) == fits
         assert (lib.lib().gb_cache_attn_bytes(0, 1, page, 1, 1, 8, 0, 1024) >= 0) == fits
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """By the native entries, before any launch (2^32 tokens were none)."""
+    from gonn_b200 import lib
+    from gonn_b200.ops.rotary import words
+    at, big = 256, 2 ** 32                                              # an address, looked at by nobody
+    rotary = [64, 64, 64, 64, 64, 64, 1, 0, 1, 64, 0, 0, 0, 0, 0, 0]
+    append = [64] * 15 + [1, 0, 1, 1, 64, 0, 0, 1, 1, 1, 1]
+    attend = [64] * 9 + [1, 0, 1, 1, 64, 1, 1, 1, 1, 0]
+    calls = ((rotary, range(6, 11), lambda z: lib.call("gb_rotary", 0, at, at, z, None, None, 1.0, None)),
+             (append, [*range(15, 21), 23, 24, 25], lambda z: lib.call("gb_cache_append", 0, at, at, at, at, at, at, z, None, 1.0, at, at, None, None)),
+             (attend, [*range(9, 14), *range(15, 19)], lambda z: lib.call("gb_cache_attn", 0, at, at, at, at, z, at, at, None, 1.0, None, 0, None)))
+    for sizes, which, call in calls:
+        call(words(*sizes))                                             # no tokens: nothing to do
+        for i in which:
+            for bad in (big, big + 1, -big):
+                with pytest.raises(lib.NativeError):
+                    call(words(*(bad if j == i else s for j, s in enumerate(sizes))))
