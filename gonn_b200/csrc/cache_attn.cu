@@ -1136,19 +1136,23 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         __syncwarp();
       };
       if (n_kv > 0) look_up(first * kWideKeys + box * a.box, mine);
+      int half = 0;                              // 1: keys of a stage have been asked for, its values not
       for (int j = 0; j < n_kv; j++) {
         check();
         const int pg = page < 0 ? a.pages : page, row = in_page;     // behind the last page: zeros
         if (j + 1 < n_kv) look_up((first + j + 1) * kWideKeys + box * a.box, mine);
         if (!mbar_wait(&k_empty[st], ph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 30)) break;
         copy(s_k + st * SUB, &tm_k, &k_full[st], pg, row);
+        half = 1;
         if (!mbar_wait(&v_empty[st], ph ^ 1, abort_flag, a.status, ST_ATTN_TIMEOUT, 31)) break;
         copy(s_v + st * SUB, &tm_v, &v_full[st], pg, row);
+        half = 0;
         if (++st == STAGES) { st = 0; ph ^= 1; }
       }
       if (*abort_flag)
         for (int i = 0; i < STAGES; i++) {
-          let_land(&k_full[i], i < st ? ph : ph ^ 1);
+          // (keys of stage st whose values' place was waited for in vain have been asked for)
+          let_land(&k_full[i], i < st + half ? ph : ph ^ 1);
           let_land(&v_full[i], i < st ? ph : ph ^ 1);
         }
     } else {
