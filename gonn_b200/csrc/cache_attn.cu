@@ -65,7 +65,7 @@ struct CacheArgs {
   int wide_prefix, wide_own;               // which of them the kernel for many rows takes
   int wide_tiles, splits, wide_group;      // its row tiles, of a sequence or of the prefix; runs of keys; runs whose tiles go together
   int slot_rows;                           // rows of the other kernel's tiles
-  int2* owner;                             // [(prefix tiles + B own_tiles) Hkv] first and last CTA; then (end of the prefix, 0)
+  int2* owner;                             // [(prefix tiles + B own_tiles) Hkv] first slot and last CTA, first -1: no keys
   int* status;
 };
 
@@ -197,7 +197,6 @@ struct Cursor {
     if (a.shared) {
       // Whole pages that all sequences have: behind a sequence's end a row of V may be anything, and NaN times a weight of 0 is NaN.
       prefix = __reduce_min_sync(0xffffffffu, least_end(a, lane, 32)) / a.page * a.page;
-      if (blockIdx.x == 0 && threadIdx.x == 32 * kConsumers) a.owner[entries * a.Hkv] = make_int2(prefix, 0);
     }
     const int per = (entries + 31) / 32, lo = min(entries, lane * per), hi = min(entries, lo + per);
     unsigned mine = 0;
@@ -207,7 +206,11 @@ struct Cursor {
       const Entry y = entry_of<ROWS, TILE>(a, prefix, k);
       if (k == lo) first_entry = y;
       mine += y.tiles;
-      if (y.cut && blockIdx.x == 0 && threadIdx.x < 32 * (kConsumers + 1)) set_status(a.status, ST_BAD_INDEX, y.b);
+      if (blockIdx.x == 0 && threadIdx.x < 32 * (kConsumers + 1)) {
+        if (y.cut) set_status(a.status, ST_BAD_INDEX, y.b);
+        if (y.tiles == 0)
+          for (int i = 0; i < a.Hkv; i++) a.owner[k * a.Hkv + i] = make_int2(-1, -1);
+      }
     }
     mine *= a.Hkv;
     unsigned sum = mine;
@@ -1412,7 +1415,7 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 // statistics, a part a lane, so that they are one wait and not one for each part; then the sums with their weights, eight parts on their
 // way at a time.  With eight warps to a row, every eighth part is a warp's, and they meet in shared memory: where rows are few and parts many,
 // which a warp alone would wait for by eights.  Rows that the first kernel has written are left alone; rows that see nothing become zeros.
-template <typename T, int ROWS, int TILE, int WPR>
+template <typename T, int ROWS, int WPR>
 __global__ void __launch_bounds__(256) cache_join_kernel(const CacheArgs a) {
   __shared__ float s_o[WPR > 1 ? 8 : 1][128];
   __shared__ float2 s_st[8];
@@ -1428,9 +1431,8 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const CacheArgs a) {
   struct Parts { long long first, rest, step; int n; };
   Parts pre = {0, 0, 0, 0}, own = {0, 0, 0, 0};
   const long long whole = 2LL * a.ctas * ROWS;
-  const int prefix = a.shared ? a.owner[(a.prefix_tiles + a.B * a.own_tiles) * a.Hkv].x : 0;
-  auto find = [&](Parts& p, int e, const int2 c, int r, long long at) {
-    if (entry_of<ROWS, TILE>(a, prefix, e).tiles == 0) return true;  // (whose owner is anything)
+  auto find = [&](Parts& p, const int2 c, int r, long long at) {
+    if (c.x < 0) return true;                     // no keys
     const int cta = c.x >> 1;
     if (cta == c.y) {                             // one CTA had all of it
       p = {at, at, 0, 1};
@@ -1446,9 +1448,9 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const CacheArgs a) {
   const int2 c_pre = a.prefix_tiles ? a.owner[e_pre * a.Hkv + h] : make_int2(0, 0), c_own = a.wide_own ? make_int2(0, 0) : a.owner[e_own * a.Hkv + h];
   if (t < count_of(a, b)) {
     if (a.wide_prefix) pre = {whole + rows + i, whole + rows + i, rows, a.splits};
-    else if (a.prefix_tiles) find(pre, e_pre, c_pre, all % ROWS, whole + rows + i);
+    else if (a.prefix_tiles) find(pre, c_pre, all % ROWS, whole + rows + i);
     if (a.wide_own) own = {i, i, rows, a.splits};
-    else if (!find(own, e_own, c_own, r % ROWS, whole + i)) return;
+    else if (!find(own, c_own, r % ROWS, whole + i)) return;
   }
   const int n = pre.n + own.n;
   float top = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
@@ -1578,7 +1580,7 @@ bool plan(Sizes& z, int dtype, long long B, long long T, long long H, long long 
   auto up = [](long long n) { return (n + 255) / 256 * 256; };
   z.part = up(rows * D * 4);
   z.stat = up(rows * 8);
-  z.owner = up((z.entries * Hkv + 1) * 8);
+  z.owner = up(z.entries * Hkv * 8);
   z.total = z.part + z.stat + z.owner;
   return true;
 }
@@ -1605,13 +1607,13 @@ int launch_wide(const CUtensorMap& tk, const CUtensorMap& tv, const CacheArgs& a
   return gbh::E_OK;
 }
 
-template <typename T, int ROWS, int TILE>
+template <typename T, int ROWS>
 int launch_join(const CacheArgs& a, cudaStream_t s) {
   const long long rows = (long long)a.B * a.T * a.H;
   // about as many parts as the CTAs are times the segments: above eight, which a warp fetches at a time
   const bool many_parts = a.wide_own || a.wide_prefix ? a.splits > 8 : kCtas > 8LL * a.Hkv * (a.prefix_tiles + (long long)a.B * a.own_tiles);
-  if (rows <= kFewRows && many_parts) GB_CUDA_OK(gbh::launch(cache_join_kernel<T, ROWS, TILE, 8>, dim3((unsigned)rows), dim3(256), 0, s, 1, a));
-  else GB_CUDA_OK(gbh::launch(cache_join_kernel<T, ROWS, TILE, 1>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, 1, a));
+  if (rows <= kFewRows && many_parts) GB_CUDA_OK(gbh::launch(cache_join_kernel<T, ROWS, 8>, dim3((unsigned)rows), dim3(256), 0, s, 1, a));
+  else GB_CUDA_OK(gbh::launch(cache_join_kernel<T, ROWS, 1>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, 1, a));
   return gbh::E_OK;
 }
 
@@ -1634,7 +1636,7 @@ int launch_kernel(const CUtensorMap& tk, const CUtensorMap& tv, CacheArgs& a, cu
         if (rc) return rc;
       }
     }
-    return launch_join<T, C::ROWS, C::TILE>(a, s);
+    return launch_join<T, C::ROWS>(a, s);
   }
 }
 
@@ -1686,7 +1688,7 @@ int launch_any(const CUtensorMap& k, const CUtensorMap& v, CacheArgs& a, int row
       const int rc = a.box ? (a.D <= 64 ? launch_wide<T, 64, true>(k, v, a, s) : launch_wide<T, 128, true>(k, v, a, s))
                            : (a.D <= 64 ? launch_wide<T, 64, false>(k, v, a, s) : launch_wide<T, 128, false>(k, v, a, s));
       if (rc) return rc;
-      return a.splits > 1 ? launch_join<T, 64, 64>(a, s) : gbh::E_OK;
+      return a.splits > 1 ? launch_join<T, 64>(a, s) : gbh::E_OK;
     }
   }
   return a.box ? launch_type<T, true>(k, v, a, rows, s) : launch_type<T, false>(k, v, a, rows, s);
