@@ -1743,7 +1743,7 @@ GB_EXPORT int gb_cache_attn(int dtype, const void* q, const void* k, const void*
     gbh::set_error("gb_cache_attn: null pointer or empty cache");
     return gbh::E_BAD_ARG;
   }
-  if ((long long)columns * page > kMost || prefix < 0 || prefix > (long long)columns * page || prefix % page || !(scale > 0)) {
+  if ((long long)columns * page > kMost || prefix < 0 || prefix > (long long)columns * page || prefix % page || !(scale >= 1e-37 && scale <= 1e38)) {          // (a scale that fp32 holds: 0 times a masked score is NaN)
     gbh::set_error("gb_cache_attn: a table of %d pages of %d positions, %d of them shared, scale %g", columns, page, prefix, scale);
     return gbh::E_BAD_ARG;
   }

@@ -178,6 +178,8 @@ def attend(c: Layout, q, table, lengths, counts=None, scale: Optional[float] = N
         return _attend_ref(c, q, table, lengths, counts, scale, shared_pages)
     if width > MAX_HEAD:
         raise ValueError(f"{what}: heads of up to {MAX_HEAD} columns on CUDA, got {width}")
+    if not 1e-37 <= scale <= 1e38:
+        raise ValueError(f"{what}: a scale between 1e-37 and 1e38 on CUDA, which fp32 holds, got {scale}")
     out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
     if batch == 0 or tokens == 0:
         return out

@@ -606,3 +606,13 @@ def test_infinite_values_that_a_shorter_sequence_does_not_have(dtype, B):
     want, tol = attended(cache, q[:1], table, at[:1], None)
     close(out[:1], (want, tol))
     assert bool((out[1:] == math.inf).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_scales_that_fp32_does_not_hold(dtype):
+    cache, table, at, c, (q, k, v) = batch(2, 2, 2, 1, 64, 16, [300, 40], dtype)
+    cache.Append(k, v, table, at)
+    for scale in (1e-50, 9e-38, 1.1e38, 1e300):
+        with pytest.raises(ValueError):
+            cache.Attend(q, table, at, scale=scale)
+    close(cache.Attend(q, table, at, scale=1e-37), attended(cache, q, table, at, c, 1e-37))       # the mean of what a token sees
