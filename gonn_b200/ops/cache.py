@@ -11,7 +11,7 @@ from typing import Optional
 import torch
 
 from .. import lib as _l
-from .rotary import _TYPES, rotate_ref, words
+from .rotary import _TYPES, has_tangent, rotate_ref, words
 
 MAX_HEAD = 128                    # largest head that attention on CUDA takes
 MAX_ROOM = 2 ** 31 - 257          # positions of a table: a tile of keys that starts within them ends within 32 bits
@@ -67,7 +67,7 @@ def _check_batch(what, c, batch, table, lengths, counts):
 def _like_cache(what, name, t, c):
     if t.dtype is not c.dtype or t.get_device() != c.index:
         raise TypeError(f"{what}: {name} is {t.dtype} on {t.device}, the cache {c.dtype} on {c.device}")
-    if torch.is_grad_enabled() and (t.requires_grad or c.keys.requires_grad or c.values.requires_grad):
+    if torch.is_grad_enabled() and (t.requires_grad or c.keys.requires_grad or c.values.requires_grad) or has_tangent(t):
         raise RuntimeError(f"{what}: no gradient goes through a cache; call under torch.no_grad()")
 
 

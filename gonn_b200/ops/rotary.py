@@ -13,6 +13,8 @@ import torch
 
 from .. import lib as _l
 
+_fwd_ad = torch.autograd.forward_ad
+
 _TYPES = {torch.bfloat16: _l.DT_BF16, torch.float16: _l.DT_F16, torch.float32: _l.DT_F32}
 
 
@@ -103,6 +105,16 @@ class _Rotary(torch.autograd.Function):
         dx = _Rotary.apply(dy, *ctx.rest) if torch.is_grad_enabled() else _launch(dy, *ctx.rest)
         return dx, None, None, None, None, None
 
+    @staticmethod
+    def jvp(ctx, dx, *_):
+        *rest, back = ctx.rest
+        return None if dx is None else _Rotary.apply(dx, *rest, not back)
+
+
+def has_tangent(t: torch.Tensor) -> bool:
+    """Whether a forward-mode derivative is asked for along t."""
+    return _fwd_ad._current_level >= 0 and _fwd_ad.unpack_dual(t).tangent is not None
+
 
 def _writes(positions) -> int:
     """How often a tensor has been written to in place (nothing counts that for tensors of inference mode)."""
@@ -135,6 +147,6 @@ def rotary(x: torch.Tensor, positions: Optional[torch.Tensor], w: Sequence[float
         raise TypeError(f"rotary: no CUDA kernel for dtype {x.dtype}")
     if turns.get_device() != device:
         raise ValueError(f"rotary: the frequencies are on {turns.device}, x on {x.device}; move the module there")
-    if torch.is_grad_enabled() and x.requires_grad:
+    if torch.is_grad_enabled() and x.requires_grad or has_tangent(x):
         return _Rotary.apply(x, positions, turns, interleaved, amplitude, False)
     return _launch(x, positions, turns, interleaved, amplitude, False)

@@ -347,3 +347,29 @@ def test_sizes_beyond_32_bits_are_refused():
             for bad in (big, big + 1, -big):
                 with pytest.raises(lib.NativeError):
                     call(words(*(bad if j == i else s for j, s in enumerate(sizes))))
+
+
+def test_tangents(monkeypatch):
+    """Forward-mode derivatives: the turn of the tangent; none goes through a cache."""
+    from gonn_b200.ops import rotary
+    fw = torch.autograd.forward_ad
+    rope = nn.RotaryEmbedding(4, interleaved=True, amplitude=1.5)
+    x, dx = torch.randn(2, 1, 3, 2, 6).unbind(0)
+    at = torch.tensor([3, 1, 7])
+    with fw.dual_level():
+        want = fw.unpack_dual(rope(fw.make_dual(x, dx), at))
+
+        def launch(x, positions, turns, interleaved, amplitude, back, out=None):   # the kernel's part, on the CPU
+            return rotary.rotate_ref(x.detach(), positions, rope._w, interleaved, amplitude, back)
+        monkeypatch.setattr(rotary, "_launch", launch)
+        got = fw.unpack_dual(rotary._Rotary.apply(fw.make_dual(x, dx), at, rope.turns, True, 1.5, False))
+        assert torch.equal(got.primal, want.primal) and torch.allclose(got.tangent, want.tangent)
+        back = fw.unpack_dual(rotary._Rotary.apply(fw.make_dual(x, dx), at, rope.turns, True, 1.5, True))
+        assert torch.allclose(back.tangent, rotary.rotate_ref(dx, at, rope._w, True, 1.5, True))
+        cache, q = nn.KVCache(1, 4, 2, 6), x[:, :1]
+        table, lengths = torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+        dual = fw.make_dual(q, dx[:, :1])
+        for call in (lambda: cache.Append(dual, q, table, lengths), lambda: cache.Append(q, dual, table, lengths), lambda: cache.Attend(dual, table, lengths)):
+            with pytest.raises(RuntimeError, match="no gradient"):
+                call()
+        cache.Append(q, q, table, lengths)

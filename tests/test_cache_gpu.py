@@ -616,3 +616,15 @@ def test_scales_that_fp32_does_not_hold(dtype):
         with pytest.raises(ValueError):
             cache.Attend(q, table, at, scale=scale)
     close(cache.Attend(q, table, at, scale=1e-37), attended(cache, q, table, at, c, 1e-37))       # the mean of what a token sees
+
+
+def test_tangents():
+    fw = torch.autograd.forward_ad
+    rope = nn.RotaryEmbedding(24, interleaved=True, amplitude=1.5, device="cuda")
+    x, dx = torch.randn(2, 2, 9, 3, 40, device="cuda").unbind(0)
+    at = torch.randint(0, 5000, (2, 9), device="cuda")
+    for grad in (False, True):
+        with fw.dual_level():
+            y, dy = fw.unpack_dual(rope(fw.make_dual(x.clone().requires_grad_(grad), dx), at))
+        close(y.detach(), turned(x, at, rope))
+        close(dy.detach(), turned(dx, at, rope))
