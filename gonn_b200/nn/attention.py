@@ -28,6 +28,8 @@ from .module import Module
 
 
 class MultiHeadAttention(Module):
+    rotary = None                     # (of layers pickled before they knew of it, too)
+
     def __init__(self, embed_dim: int, num_heads: int, kdim: Optional[int] = None,
                  vdim: Optional[int] = None, *, rotary=None, dtype=torch.float32, device=None):
         super().__init__()

@@ -373,3 +373,22 @@ def test_tangents(monkeypatch):
             with pytest.raises(RuntimeError, match="no gradient"):
                 call()
         cache.Append(q, q, table, lengths)
+
+
+def test_layers_pickled_without_rotary():
+    """A layer pickled whole before it knew of rotary positions has none."""
+    import pickle
+    mha = nn.MultiHeadAttention(8, 2, dtype=torch.float64)
+    x = torch.randn(1, 3, 8, dtype=torch.float64)
+    old = pickle.loads(pickle.dumps(mha))
+    del old.__dict__["rotary"]
+    old = pickle.loads(pickle.dumps(old))
+    assert old.rotary is None
+    assert torch.equal(old(x, causal=True), mha(x, causal=True)) and torch.equal(old.ForwardMasked(x), mha.ForwardMasked(x))
+    cache, table, at = nn.KVCache(1, 4, 2, 4, dtype=torch.float64), torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    with torch.no_grad():
+        old.ForwardCached(x, cache, table, at)
+    old.to(torch.float32)
+    # and one with them keeps them
+    with_rope = pickle.loads(pickle.dumps(nn.MultiHeadAttention(8, 2, rotary=nn.RotaryEmbedding(4))))
+    assert with_rope.rotary.dim == 4
