@@ -49,7 +49,6 @@ struct RotaryArgs {
   const int* counts;                  // null: all tokens count
   int* status;
   int groups;                         // threads that share a token's heads of an item
-  int early;
 };
 
 template <int BYTES> struct VecOf;
@@ -113,7 +112,7 @@ __device__ __forceinline__ void turn(Pack<T, V>& u, Pack<T, V>& w, const float2*
 // A head of any part is `items` items of two vectors: half / V turned ones, then the rest (of values: all of it) as it lies.
 template <typename T, int V, bool INTER, bool APPEND, bool IN_PLACE>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
-  if (a.early) pdl_trigger();
+  pdl_trigger();                      // (two heads a thread and more, or 1 184 CTAs at most: starts_early() holds for any size)
   const int items = (a.width + 2 * V - 1) / (2 * V), heads = APPEND ? a.q.heads + 2 * a.k.heads : a.q.heads;
   const unsigned i = blockIdx.x * kThreads + threadIdx.x, per_token = (unsigned)a.groups * items, token = i / per_token;
   const unsigned in_token = i - token * per_token, group = in_token / items;
@@ -223,8 +222,7 @@ int launch_rotary(RotaryArgs& a, int inter, cudaStream_t s) {
     return gbh::E_TOO_LARGE;
   }
   const unsigned ctas = (unsigned)((threads + kThreads - 1) / kThreads);
-  a.early = starts_early((long long)kThreads * per * 4 * V * sizeof(T), ctas);
-  const auto go = [&](auto kernel) { return gbh::launch_if(a.early, kernel, dim3(ctas), dim3(kThreads), 0, s, a); };
+  const auto go = [&](auto kernel) { return gbh::launch(kernel, dim3(ctas), dim3(kThreads), 0, s, 1, a); };
   if constexpr (!APPEND) {
     if (a.q.src == a.q.dst) {
       GB_CUDA_OK(inter ? go(rotary_kernel<T, V, true, false, true>) : go(rotary_kernel<T, V, false, false, true>));
