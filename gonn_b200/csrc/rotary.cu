@@ -5,8 +5,10 @@
 //
 // Angles.  p w in fp32 is off by p 2^-24: by 0.008 at position 131 072, twice a bf16's last bit.  So a frequency is held as the fraction
 // w / 2 pi of a turn in 64 bits of fixed point, and p times it, modulo 2^64, is the fraction of a turn that is left: an integer
-// product whose overflow is the reduction, off by p 2^-65 turns.  Its upper 32 bits become a float in half turns (off by 2^-25) for
-// sincospif.
+// product whose overflow is the reduction.  The fraction is a quotient in fp64, off by 2^-55 for w up to 1: p times it by p 2^-55 turns, as the
+// product p w itself in fp64 is, which is less than what comes next up to position 2^27.  For fp32 rows the upper two bits are the
+// quarter and the next 32 a float of up to an eighth of a turn either way, off by pi 2^-27 (2.4e-8; with the upper 32 bits as a float of half a turn
+// 9.4e-8), for sincospif; for 16-bit rows the upper 32 bits become that float of half a turn, off by 9.4e-8.
 //
 // What bounds it: memory, every element read and written once.  A thread takes an item, two vectors of 16 bytes (narrower ones where a size or an
 // address is odd) with the two halves of its pairs, of several heads of one token: their loads and the position's are on their way at once, and sines and
@@ -74,11 +76,21 @@ struct Pack {
 template <typename T>
 __device__ __forceinline__ float2 angle_of(unsigned long long turns, long long position, float amplitude, bool back) {
   const unsigned long long phase = turns * (unsigned long long)position;
-  const float x = (float)(int)(phase >> 32) * 4.656612873077393e-10f;          // 2^-31: half turns in [-1, 1)
   float s, c;
   if constexpr (sizeof(T) == 4) {
-    sincospif(x, &s, &c);
+    const unsigned quarter = (unsigned)((phase + (1ull << 61)) >> 62);
+    sincospif((float)(int)(phase >> 30) * 1.1641532182693481e-10f, &s, &c);    // 2^-33: half turns from the nearest quarter, in [-1/4, 1/4)
+    if (quarter & 1) {
+      const float t = s;
+      s = c;
+      c = -t;
+    }
+    if (quarter & 2) {
+      s = -s;
+      c = -c;
+    }
   } else {
+    const float x = (float)(int)(phase >> 32) * 4.656612873077393e-10f;        // 2^-31: half turns in [-1, 1)
     s = __sinf(x * 3.14159265358979f);
     c = __cosf(x * 3.14159265358979f);
   }

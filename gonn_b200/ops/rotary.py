@@ -1,7 +1,7 @@
 """Rotary positions: pairs of a head's columns turned by an angle that grows with the token's position.
 
-CUDA: ``csrc/rotary.cu``, where angles are exact to a float's last bit at any position.  CPU: the same formulas with tensor
-operations, angles in fp64."""
+CUDA: ``csrc/rotary.cu``, where angles come from 64 bits of fixed point: up to position 2^27 they are off by 2.4e-8 for fp32 rows, by 9.4e-8 for
+16-bit ones, whatever the position; behind it p w / 2 pi in fp64 is off by more.  CPU: the same formulas with tensor operations, angles in fp64."""
 from __future__ import annotations
 
 import math
@@ -35,7 +35,7 @@ def frequencies(dim: int, base: float, scaling: str = "none", factor: float = 1.
 
 
 def turns_of(w: Sequence[float]) -> torch.Tensor:
-    """Fractions of a turn in 64 bits of fixed point, as int64."""
+    """Fractions of a turn in 64 bits of fixed point, as int64; off by 2^-55 for frequencies up to 1, as their quotients in fp64 are."""
     t = torch.tensor(w, dtype=torch.float64) / (2 * math.pi)
     t = t - torch.floor(t + 0.5)                      # whole turns go; exact, like the power of two
     return torch.round(t * 2.0 ** 64).to(torch.int64)

@@ -392,3 +392,16 @@ def test_layers_pickled_without_rotary():
     # and one with them keeps them
     with_rope = pickle.loads(pickle.dumps(nn.MultiHeadAttention(8, 2, rotary=nn.RotaryEmbedding(4))))
     assert with_rope.rotary.dim == 4
+
+
+def test_fixed_point_angles_against_pi():
+    """p times the fraction of a turn against p w / 2 pi with pi to 60 digits: off by p 2^-55 turns at most, w / 2 pi being rounded to fp64 (w up to
+    1: below 0.16, off by 2^-56 and by what 2 pi in fp64 is off, 2^-54.5 of it)."""
+    from fractions import Fraction
+    pi = Fraction(3141592653589793238462643383279502884197169399375105820974944, 10 ** 60)
+    for base, dim in ((10000.0, 128), (500000.0, 64), (1e6, 48)):
+        w = nn.RotaryEmbedding(dim, base)._w
+        for f, t in zip(w, turns_of(w).tolist()):
+            for p in (1, 4095, 131071, 2 ** 31 - 1, -5):
+                d = abs(Fraction(t * p % 2 ** 64, 2 ** 64) - Fraction(f) * p / (2 * pi) % 1)
+                assert min(d, 1 - d) <= Fraction(abs(p), 2 ** 55)

@@ -628,3 +628,19 @@ def test_tangents():
             y, dy = fw.unpack_dual(rope(fw.make_dual(x.clone().requires_grad_(grad), dx), at))
         close(y.detach(), turned(x, at, rope))
         close(dy.detach(), turned(dx, at, rope))
+
+
+def test_angles_in_fp32():
+    """Cosine and sine themselves (pairs of 1 and 0): off by the angle's pi 2^-27 and what it is cut off, 2.4e-8 together, and a unit in the last
+    place of the function, at most 2^-23 of the value."""
+    rope = nn.RotaryEmbedding(64, device="cuda")
+    x = torch.zeros(1, 20000, 1, 64, device="cuda")
+    x[..., :32] = 1
+    for start in (0, 100003):
+        at = torch.arange(20000, device="cuda") + start
+        y = rope(x, at)[0, :, 0].double()
+        angle = at.double()[:, None] * torch.tensor(rope._w, dtype=torch.float64, device="cuda")
+        want = torch.cat((torch.cos(angle), torch.sin(angle)), -1)
+        # (and p w in fp64, 2^-52 of it on either side)
+        worst = ((y - want).abs() - 2.0 ** -23 * want.abs() - float(at[-1]) * 2.0 ** -51).max()
+        assert float(worst) <= 2.4e-8
