@@ -644,3 +644,36 @@ def test_angles_in_fp32():
         # (and p w in fp64, 2^-52 of it on either side)
         worst = ((y - want).abs() - 2.0 ** -23 * want.abs() - float(at[-1]) * 2.0 ** -51).max()
         assert float(worst) <= 2.4e-8
+
+
+# More row tiles of all heads and sequences than the SMs (148) or two rounds of them (296) hold: their results leave without the joining kernel, in one group of
+# runs or in several whose last one is smaller; the last one's table is so long that a group is one run.
+MANY = [(4, 300, 16, 8, 128, 64, [0, 77, 500, 64], [300, 13, 0, 299], 0), (5, 300, 14, 14, 64, 24, [3, 0, 100, 23, 24], None, 0),
+        (4, 290, 24, 12, 72, 7, [40, 0, 5, 6], [290, -3, 500, 129], 0), (3, 700, 23, 23, 128, 64, [0, 130, 63], None, 0),
+        (7, 257, 34, 34, 64, 64, [0, 1, 2, 300, 64, 65, 127], [257, 256, 0, 1, 128, 129, 257], 0), (5, 129, 48, 48, 128, 24, [9, 0, 48, 400, 24], [129, 1, 128, 0, 77], 0),
+        (2, 200, 80, 80, 64, 16, [30, 500], None, 2 ** 18)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("B,T,H,kv,D,page,lengths,counts,room", MANY)
+def test_attend_more_rows_than_a_round(dtype, B, T, H, kv, D, page, lengths, counts, room):
+    tiles = -(-T * (H // kv) // 128) * kv * B
+    assert tiles > 148
+    cache, table, at, c, (q, k, v) = batch(B, T, H, kv, D, page, lengths, dtype, counts=counts)
+    if room:
+        table = torch.cat((table, torch.full((B, room // page - table.shape[1]), -7, dtype=torch.int32, device="cuda")), 1)
+    cache.Append(k, v, table, at, counts=c)
+    before = lib.kernel_count
+    out = cache.Attend(q, table, at, counts=c)
+    assert lib.kernel_count == before + 1                               # no joining kernel
+    close(out, attended(cache, q, table, at, c))
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("B,T,H,kv,D,page,prefix,counts", [(310, 2, 32, 8, 64, 64, 4, None), (310, 4, 64, 8, 128, 24, 3, [i % 6 - 1 for i in range(310)])])
+def test_shared_more_rows_than_a_round(dtype, B, T, H, kv, D, page, prefix, counts):
+    """The prefix's row tiles alone are more than a round."""
+    assert -(-B * T * (H // kv) // 128) * kv > 148
+    cache, table, at, c, (q, k, v) = batch(B, T, H, kv, D, page, [prefix * page + i % 31 for i in range(B)], dtype, prefix=prefix, counts=counts)
+    cache.Append(k, v, table, at, counts=c)
+    close(cache.Attend(q, table, at, counts=c, shared_pages=prefix), attended(cache, q, table, at, c))
