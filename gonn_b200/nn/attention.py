@@ -28,8 +28,6 @@ from .module import Module
 
 
 class MultiHeadAttention(Module):
-    rotary = None                     # (of layers pickled before they knew of it, too)
-
     def __init__(self, embed_dim: int, num_heads: int, kdim: Optional[int] = None,
                  vdim: Optional[int] = None, *, rotary=None, dtype=torch.float32, device=None):
         super().__init__()
@@ -61,6 +59,11 @@ class MultiHeadAttention(Module):
         for i, p in enumerate(projs):
             p.weight.data = w[i * E:(i + 1) * E]
             p.bias.data = b[i * E:(i + 1) * E]
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if "rotary" not in self._modules:
+            self.__dict__.setdefault("rotary", None)          # (pickled before the layer knew of it)
 
     def fuse_groups(self):
         """Parameter groups that must stay adjacent in memory when a wrapper re-homes

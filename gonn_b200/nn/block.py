@@ -90,7 +90,7 @@ def _block_words(B, S, E, dt, dev, parts):
         return None
     code = _ACT.get(kind)
     ad = attn.__dict__
-    if ad.get("rotary") is not None:
+    if ad.get("rotary", _ABSENT) is not None:
         return None                # (its queries and keys are turned between the products)
     H = ad["num_heads"]
     D = E // H

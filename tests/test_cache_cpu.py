@@ -405,3 +405,16 @@ def test_fixed_point_angles_against_pi():
             for p in (1, 4095, 131071, 2 ** 31 - 1, -5):
                 d = abs(Fraction(t * p % 2 ** 64, 2 ** 64) - Fraction(f) * p / (2 * pi) % 1)
                 assert min(d, 1 - d) <= Fraction(abs(p), 2 ** 55)
+
+
+def test_rotary_given_to_a_layer_later():
+    """Assigned, it is a child of the layer, which uses it, pickles it and moves it."""
+    import pickle
+    rope = nn.RotaryEmbedding(4)
+    mha, given = nn.MultiHeadAttention(8, 2), nn.MultiHeadAttention(8, 2, rotary=rope)
+    given.load_state_dict(mha.state_dict())
+    x = torch.randn(1, 3, 8)
+    plain = mha(x, causal=True)
+    mha.rotary = rope
+    for layer in (mha, pickle.loads(pickle.dumps(mha)), mha.to("cpu")):
+        assert torch.equal(layer(x, causal=True), given(x, causal=True)) and not torch.equal(layer(x, causal=True), plain)

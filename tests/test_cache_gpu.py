@@ -677,3 +677,15 @@ def test_shared_more_rows_than_a_round(dtype, B, T, H, kv, D, page, prefix, coun
     cache, table, at, c, (q, k, v) = batch(B, T, H, kv, D, page, [prefix * page + i % 31 for i in range(B)], dtype, prefix=prefix, counts=counts)
     cache.Append(k, v, table, at, counts=c)
     close(cache.Attend(q, table, at, counts=c, shared_pages=prefix), attended(cache, q, table, at, c))
+
+
+def test_rotary_given_to_a_layer_later():
+    """The native evaluation of a block leaves a layer alone whose rotary positions were assigned."""
+    from gonn_b200.models import GPT
+    from gonn_b200.nn import block
+    model = GPT(vocab=31, d_model=128, n_layers=1, n_heads=2, d_ff=256, max_seq=32, dtype=BF, device="cuda")
+    x = torch.randn(1, 20, 128, device="cuda").to(BF)
+    with torch.no_grad():
+        assert block.evaluate(x, *model.layers[0]._parts()) is not None
+        model.layers[0].attn.rotary = nn.RotaryEmbedding(64, device="cuda")
+        assert block.evaluate(x, *model.layers[0]._parts()) is None
