@@ -37,15 +37,20 @@ class RotaryEmbedding(Module):
         self.dim, self.base, self.interleaved, self.amplitude = dim, float(base), bool(interleaved), float(amplitude)
         self.scaling, self.factor, self.original, self.low, self.high = scaling, float(factor), original, float(low), float(high)
         self._w = frequencies(dim, self.base, scaling, self.factor, original, self.low, self.high)
-        self.register_buffer("turns", turns_of(self._w).to(device), persistent=False)
+        self.turns = turns_of(self._w).to(device)              # (no buffer: it follows from the options, whatever a checkpoint holds)
+
+    def _apply(self, fn, *a, **kw):
+        r = super()._apply(fn, *a, **kw)
+        self.turns = fn(self.turns)
+        return r
 
     def forward(self, x, positions: Optional[torch.Tensor] = None):
         """x (batch, tokens, heads, width) with any strides, bf16, fp16 or fp32 on CUDA; positions int32 or int64, (tokens,) or
         (batch, tokens), None for 0, 1, ...  Differentiable in x."""
-        return rotary(x, positions, self._w, self._buffers["turns"], self.interleaved, self.amplitude)
+        return rotary(x, positions, self._w, self.turns, self.interleaved, self.amplitude)
 
     def _plan(self):
-        return self._w, self._buffers["turns"], self.interleaved, self.amplitude
+        return self._w, self.turns, self.interleaved, self.amplitude
 
 
 class KVCache:

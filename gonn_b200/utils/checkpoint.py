@@ -72,17 +72,11 @@ def _write_entry(f, name: str, kind: int, t: torch.Tensor):
     f.write(_encode(t, code))
 
 
-def _buffers(module: torch.nn.Module):
-    """Named buffers that are state; those registered as not persistent follow from a module's options."""
-    derived = {f"{prefix}.{n}" if prefix else n for prefix, m in module.named_modules() for n in m._non_persistent_buffers_set}
-    return [(n, b) for n, b in module.named_buffers() if n not in derived]
-
-
 def save(path: str, module: torch.nn.Module, optimizer=None) -> None:
     entries = []
     for n, p in module.named_parameters():
         entries.append((n, _K_PARAM, p.data))
-    for n, b in _buffers(module):
+    for n, b in module.named_buffers():
         entries.append((n, _K_BUF, b))
     if optimizer is not None:
         names = {id(p): n for n, p in module.named_parameters()}
@@ -128,7 +122,7 @@ def load(path: str, module: torch.nn.Module, optimizer=None, strict: bool = True
     such as an fp64 checkpoint into a bf16 model are allowed)."""
     ent = read(path)
     named = dict(module.named_parameters())
-    named.update(dict(_buffers(module)))
+    named.update(dict(module.named_buffers()))
     missing = [n for n in named if n not in ent]
     if strict and missing:
         raise KeyError(f"checkpoint is missing {missing}")
