@@ -14,7 +14,8 @@
 // the list's order; no atomics.
 //
 // Where few (sequence, head) pairs have short tables, a cluster of up to eight CTAs takes each of them, and their sums meet in distributed shared
-// memory instead: no second kernel (one token behind 2 047 positions of 16 heads: 9.6 us, 14.7 with it).
+// memory instead: no second kernel (one token behind 2 047 positions of 16 heads, in a graph: 8.5 us, 10.5 with it).  There a long sequence keeps its
+// cluster alone, see plan().
 //
 // A shared prefix is one more entry at the head of the list whose rows are the queries of all sequences: its keys are read once for
 // every 16, 32 or 64 rows.  The sequences' own entries then start behind it, and all rows are joined by the second kernel.  The prefix ends before the
@@ -1539,7 +1540,9 @@ bool plan(Sizes& z, int dtype, long long B, long long T, long long H, long long 
   if (B * T * H > kMost || room > kMost) return false;
   const long long own = T * (H / Hkv), all = B * own;
   z = Sizes{};
-  // Many rows of a sequence: its keys with the prefix among them, nothing is gained by sharing.  Many rows of the batch alone: its prefix.
+  // Many rows of a sequence: its keys with the prefix among them, which is then read and multiplied for each sequence.  Many rows of the batch alone: its
+  // prefix.  (64 sequences behind 16 384 shared positions, 16 heads to each of four keys of 128 bf16, in a graph: of four tokens, who share, 164 us; of five,
+  // 80 rows to a key head, who do not, 236, and 333 if every sequence has pages of its own.)
   // us, few rows' kernel | this one, bf16, eight key heads of 128, 32, 48, 64, 96 rows to a key head: 8 sequences of 8 192 positions 63 | 60, 68 | 61, 70 | 62,
   // 117 | 64; of 1 024 to 8 192 41 | 52, 50 | 54, 53 | 57; 64 such ones 211 | 241, 249 | 256, 263 | 254.  Heads of 64 37 | 39, 43 | 43, 45 | 44, 72 | 46.  A shared
   // prefix of 16 384 (and 200 of its own for each sequence) 31 | 39, 37 | 40, 38 | 43, 51 | 46; 256 rows 91 | 57.
@@ -1563,10 +1566,13 @@ bool plan(Sizes& z, int dtype, long long B, long long T, long long H, long long 
   z.own_tiles = (int)ot;
   z.prefix_tiles = (int)pt;
   // A cluster for each (sequence, row tile, key head): as many CTAs, up to eight, as leave all of them on the SMs at a time.  It saves the second
-  // kernel, 6 us, but the longest sequence's CTAs (a full table: `each` tiles at 0.75 us) may be at work when the others have ended, while
-  // the list, of half that length on average, takes 2.5 ns for each 32 KB tile on all SMs.  us, list | clusters, 16 heads of 128 bf16, equal lengths: one
-  // sequence of 1 000 positions 19.5 | 14.7, 4 000 20.5 | 15.8, 8 000 21.1 | 22.3, 16 000 34.0 | 38.7; four of 2 000 21.0 | 16.2, 8 000 53.2 | 47.1;
-  // sixteen of 500 21.3 | 15.5, 2 000 53.9 | 47.3.
+  // kernel, but the longest sequence's CTAs (a full table: `each` tiles at 0.75 us) may be at work when the others have ended, while
+  // the list, of half that length on average, takes 2.5 ns for each 32 KB tile on all SMs.  us in a graph, list | clusters, 16 heads of 128 bf16, equal
+  // lengths: one sequence of 1 000 positions 9.2 | 7.0, 2 047 10.5 | 8.5, 4 000 13.2 | 11.8; four of 2 000 15.8 | 12.3, 8 000 47.5 | 42.6; sixteen of 500
+  // 16.1 | 12.0, 2 000 48.8 | 43.1.
+  // The rule was fitted to equal lengths of up to 256 CTAs.  Near 296 it lets go of its limit on `each`, and ragged lengths lose there.  Eight key
+  // heads, table of 32 768 positions: 37 sequences (one CTA each) of 8 000 174 | 172, one of 32 000 beside 36 of 500 44 | 397; nine (four CTAs each) of 8 000 53 | 73,
+  // one of 32 000 beside eight of 500 36 | 101.
   if (!shared && !z.wide_own && z.rows <= 16 && z.entries * Hkv <= kCtas) {
     const long long tile = 16384 / ((D <= 64 ? 64 : 128) * (dtype == 2 ? 4 : 2)), tiles = (room + tile - 1) / tile;
     z.peers = kPeers;

@@ -89,8 +89,10 @@ class KVCache:
     def Attend(self, q, table, lengths, counts=None, scale: Optional[float] = None, shared_pages: int = 0):
         """softmax(scale q K^T) V of q (batch, tokens, heads, head size) over its sequence's positions up to its own, keys and values of
         this call's tokens included: they have been appended.  heads may be a multiple of the cache's: query heads h n .. h n + n - 1 share key
-        head h.  Zeros where a token does not count.  scale: 1 / sqrt(head size).
+        head h.  Zeros where a token does not count.  scale: 1 / sqrt(head size).  A value of a later token of the same call that is infinite or NaN
+        may reach the earlier ones (0 times it), as in a plain product.
 
         ``shared_pages``: all sequences have the same first pages (a common prompt), which are taken from the table's first row and read
-        once for many sequences: those that lie before the end of the shortest sequence, which may end inside them."""
+        once for many sequences: those that lie before the end of the shortest sequence, which may end inside them.  (bf16 and fp16 with more than 64
+        rows, tokens times heads to a key head: once for each sequence.)"""
         return _cache.attend(self._of, q, table, lengths, counts, scale, shared_pages)
