@@ -621,7 +621,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           if (at == 0) st_peer(peer_address(smem_u32(x_stat + rank * ROWS + from + r), to), top, l);
         } else {
           const long long row = s_dst[sg * ROWS + from + r];
-          const bool counts = s_sees[sg * ROWS + from + r] && l != 0.f;
+          const bool sees = s_sees[sg * ROWS + from + r], counts = sees && l != 0.f;
           if (col < a.D) {
             if (!seg.direct) {
               store_floats<CPL>(a.part + row * a.D + col, sum);
@@ -637,7 +637,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
               }
             }
           }
-          if (!seg.direct && lane == 0) a.stat[row] = make_float2(top, l);
+          if (!seg.direct && lane == 0) a.stat[row] = sees ? make_float2(top, l) : make_float2(-INFINITY, 0.f);      // (no key is seen: nothing to join)
         }
       }
       __syncwarp();
@@ -843,7 +843,7 @@ cache_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 #pragma unroll
                 for (int j = 0; j < HD / 8; j++)
                   if (j * 8 < a.D) *reinterpret_cast<float2*>(to + j * 8) = make_float2(o[j][2 * half], o[j][2 * half + 1]);
-                if ((lane & 3) == 0) a.stat[row] = make_float2(m, l);
+                if ((lane & 3) == 0) a.stat[row] = sees_of[r] ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
               }
             }
           }

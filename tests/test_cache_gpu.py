@@ -689,3 +689,16 @@ def test_rotary_given_to_a_layer_later():
         assert block.evaluate(x, *model.layers[0]._parts()) is not None
         model.layers[0].attn.rotary = nn.RotaryEmbedding(64, device="cuda")
         assert block.evaluate(x, *model.layers[0]._parts()) is None
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("B,T,H,kv,D,page,prefix,ends,counts", [
+    (3, 6, 3, 1, 72, 1, 1, [0, 2, 9], None), (8, 3, 8, 2, 8, 7, 1, [2, 1, 4, 5, 0, 2, 1, 0], [0, 3, 1, 2, 2, 3, 2, 1]), (2, 3, 6, 3, 48, 16, 2, [1, 42], None),
+    (5, 6, 16, 2, 64, 8, 3, [24, 3, 40, 24, 25], None), (14, 30, 4, 2, 48, 24, 1, [27, 26, 23] * 4 + [48, 5], None), (40, 4, 8, 1, 128, 64, 2, [3, 130] * 20, None)])
+def test_tokens_in_front_of_the_first_position(dtype, B, T, H, kv, D, page, prefix, ends, counts):
+    """Lengths below zero: tokens in front of position 0 see nothing, behind shared pages too."""
+    cache, q, table, at, c = ended(B, T, H, kv, D, page, prefix, ends, dtype, counts)
+    want = attended(cache, q, table, at, c)
+    assert bool((at < 0).any())
+    close(cache.Attend(q, table, at, counts=c, shared_pages=prefix), want)
+    close(cache.Attend(q, table, at, counts=c), want)
