@@ -18,8 +18,8 @@
 // cluster alone, see plan().
 //
 // A shared prefix is one more entry at the head of the list whose rows are the queries of all sequences: its keys are read once for
-// every 16, 32 or 64 rows.  The sequences' own entries then start behind it, and all rows are joined by the second kernel.  The prefix ends before the
-// page in which the shortest sequence ends, so that no row meets a value that its own sequence does not have.
+// every 16, 32 or 64 rows.  The sequences' own entries then start behind it, and all rows are joined by the second kernel.  A sequence that ends within
+// the prefix takes no part in it, so that no row meets a value that its own sequence does not have: all its keys are its own entry's.
 //
 // A CTA: four warps that multiply (mma.sync for 16-bit types, FMA for fp32) and four that copy through a ring of stages: by TMA, a box of
 // as many rows as divide both a page and a tile, where these are at least eight (a multiple of the swizzle's period); else with cp.async,
@@ -127,45 +127,32 @@ __device__ __forceinline__ int count_of(const CacheArgs& a, int b) {
   return c < 0 ? 0 : c < a.T ? c : a.T;
 }
 
-// The least end of those of the sequences first, first + step, .. that have positions and tokens that count, the prefix's at most.
-template <bool L2 = false>
-__device__ __forceinline__ int least_end(const CacheArgs& a, int first, int step) {
-  int least = a.prefix;
-#pragma unroll 4
-  for (int b = first; b < a.B; b += step) {
-    const int c = count_of<L2>(a, b);
-    const long long end = (long long)read<L2>(a.lengths + b) + c;
-    if (c > 0 && end > 0 && end < least) least = (int)end;
-  }
-  return least;
-}
-
-// prefix: where the shared positions end.
 template <int ROWS, int TILE>
-__device__ __forceinline__ Entry entry_of(const CacheArgs& a, int prefix, int e) {
+__device__ __forceinline__ Entry entry_of(const CacheArgs& a, int e) {
   Entry x;
-  x.begin = prefix;
   x.cut = false;
   if (e < a.prefix_tiles) {
     x.b = -1;
     x.row0 = e * ROWS;
     x.begin = 0;
-    x.end = prefix;
+    x.end = a.prefix;
   } else {
     e -= a.prefix_tiles;
-    long long end;
+    long long end, whole;                                              // of these rows, of the sequence
     if (a.own_tiles == 1) {
       x.b = e;
       x.row0 = 0;
       const int c = count_of(a, e);
-      end = c > 0 ? (long long)a.lengths[e] + c : 0;
+      end = whole = c > 0 ? (long long)a.lengths[e] + c : 0;
     } else {
       x.b = e / a.own_tiles;
       x.row0 = (e - x.b * a.own_tiles) * ROWS;
       const int c = count_of(a, x.b), last = min(a.T * a.G, x.row0 + ROWS) - 1;
       const int seen = min(c, last / a.G + 1);                       // tokens of these rows that count, and those before them
       end = x.row0 / a.G < c ? (long long)a.lengths[x.b] + seen : 0;
+      whole = (long long)a.lengths[x.b] + c;
     }
+    x.begin = whole < a.prefix ? 0 : a.prefix;                       // (one that ends within the prefix takes no part in it)
     x.cut = end > a.room;
     x.end = (int)(x.cut ? (long long)a.room : end > 0 ? end : 0);
   }
@@ -188,23 +175,18 @@ template <int ROWS, int TILE>
 struct Cursor {
   Shares shares;
   Entry x;
-  int e, h, entries, tile, prefix;
+  int e, h, entries, tile;
   unsigned left, segment0;           // tiles to go; the list's number of the segment's first tile
 
   // Adds up the tiles of all entries, an entry or a run of them a lane, and finds this CTA's share.  (Totals stay below 2^31.)
   __device__ __forceinline__ void start(const CacheArgs& a, int lane) {
     entries = a.prefix_tiles + a.B * a.own_tiles;
-    prefix = 0;
-    if (a.shared) {
-      // Whole pages that all sequences have: behind a sequence's end a row of V may be anything, and NaN times a weight of 0 is NaN.
-      prefix = __reduce_min_sync(0xffffffffu, least_end(a, lane, 32)) / a.page * a.page;
-    }
     const int per = (entries + 31) / 32, lo = min(entries, lane * per), hi = min(entries, lo + per);
     unsigned mine = 0;
     Entry first_entry;
 #pragma unroll 4
     for (int k = lo; k < hi; k++) {
-      const Entry y = entry_of<ROWS, TILE>(a, prefix, k);
+      const Entry y = entry_of<ROWS, TILE>(a, k);
       if (k == lo) first_entry = y;
       mine += y.tiles;
       if (blockIdx.x == 0 && threadIdx.x < 32 * (kConsumers + 1)) {
@@ -236,7 +218,7 @@ struct Cursor {
         const unsigned n = (unsigned)x.tiles * a.Hkv;
         if (first < at + n) break;
         at += n;
-        x = entry_of<ROWS, TILE>(a, prefix, ++e);
+        x = entry_of<ROWS, TILE>(a, ++e);
       }
       h = (first - at) / x.tiles;
       at += h * x.tiles;
@@ -256,7 +238,7 @@ struct Cursor {
     const int seg = blockIdx.x / peers;
     e = seg / a.Hkv;
     h = seg - e * a.Hkv;
-    x = entry_of<ROWS, TILE>(a, 0, e);
+    x = entry_of<ROWS, TILE>(a, e);
     if (x.cut && rank == 0 && threadIdx.x == 32 * kConsumers) set_status(a.status, ST_BAD_INDEX, x.b);
     tile = x.tiles * rank / peers;
     left = x.tiles * (rank + 1) / peers - tile;
@@ -268,7 +250,7 @@ struct Cursor {
     h = 0;
     do {
       if (++e >= entries) return;
-      x = entry_of<ROWS, TILE>(a, prefix, e);
+      x = entry_of<ROWS, TILE>(a, e);
     } while (x.tiles == 0);
   }
 };
@@ -357,8 +339,11 @@ __device__ __forceinline__ Row row_of(const CacheArgs& a, const Entry& x, int r)
   }
   w.t = i / a.G;
   w.g = i - w.t * a.G;
-  w.counts = w.there && w.t < count_of<L2>(a, w.b);
-  const long long sees = w.counts ? (long long)read<L2>(a.lengths + w.b) + w.t + 1 : 0;
+  const int c = count_of<L2>(a, w.b);
+  const long long length = read<L2>(a.lengths + w.b);
+  // Of the prefix, rows of sequences that have all of it: behind another one's end a row of V may be anything, and NaN times a weight of 0 is NaN.
+  w.counts = w.there && w.t < c && (x.b >= 0 || length + c >= a.prefix);
+  const long long sees = w.counts ? length + w.t + 1 : 0;
   w.sees = (int)(sees < 0x7fffffffLL ? sees : 0x7fffffffLL);
   return w;
 }
@@ -1040,7 +1025,6 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   long long* s_off = (long long*)(pv_done + 2);                      // where the keys and values of a sub-tile start (cp.async)
   uint32_t* tmem_slot = (uint32_t*)(s_off + 2 * kWideKeys);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
-  int* s_end = (int*)(tmem_slot + 2);                                // [8] least ends that the warps found
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -1062,10 +1046,6 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   if (warp == kWideCopiers) {
     tmem_alloc(tmem_slot, C::COLS);
     tmem_relinquish();
-  }
-  if (PREFIX) {
-    const int least = __reduce_min_sync(0xffffffffu, least_end<true>(a, threadIdx.x, kWideThreads));
-    if (lane == 0) s_end[warp] = least;
   }
   tc_fence_before();
   __syncthreads();
@@ -1090,9 +1070,7 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   x.row0 = (PREFIX ? rank : a.wide_tiles - 1 - rank) * kWideRows;
   x.begin = 0;
   if (PREFIX) {
-    x.end = a.prefix;                            // as the other kernel finds it
-    for (int i = 0; i < kWideThreads / 32; i++) x.end = min(x.end, s_end[i]);
-    x.end = x.end / a.page * a.page;
+    x.end = a.prefix;
   } else {
     const int c = count_of(a, x.b), last = min(a.T * a.G, x.row0 + kWideRows) - 1;
     const long long end = x.row0 / a.G < c ? (long long)a.lengths[x.b] + min(c, last / a.G + 1) : 0;
@@ -1356,7 +1334,7 @@ cache_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       const long long all = (long long)a.B * a.T * a.H;
       const long long here = w.there ? ((long long)w.b * a.T + w.t) * a.H + h * a.G + w.g : -1;
       const long long row = here < 0 || direct ? here : (PREFIX ? 2LL * a.ctas * a.slot_rows + all : 0) + split * all + here;
-      if (row >= 0 && !direct) a.stat[row] = make_float2(m, l);
+      if (row >= 0 && !direct) a.stat[row] = w.counts ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
       // through this warp's part of Q's tile (all products have read it), so that a row leaves in whole lines: 32 rows of 64 fp32 or HD 16-bit values
       uint8_t* buf = s_q + quarter * (32 * 128) * C::CH;
       constexpr int PIECE = HD == 128 ? 64 : 32;                     // fp32 columns at a time

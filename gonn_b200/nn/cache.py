@@ -93,6 +93,6 @@ class KVCache:
         may reach the earlier ones (0 times it), as in a plain product.
 
         ``shared_pages``: all sequences have the same first pages (a common prompt), which are taken from the table's first row and read
-        once for many sequences: those that lie before the end of the shortest sequence, which may end inside them.  (bf16 and fp16 with more than 64
+        once for many sequences: all those that have them whole; one that ends inside them is read by itself.  (bf16 and fp16 with more than 64
         rows, tokens times heads to a key head: once for each sequence.)"""
         return _cache.attend(self._of, q, table, lengths, counts, scale, shared_pages)
